@@ -443,6 +443,156 @@ int pjrtx_b200_dot_static_scratch(int device_ordinal, int dtype, const void *lhs
  * device: every call clears the word. */
 int pjrtx_b200_dot_static_scratch_status(int device_ordinal, void *stream);
 
+/* ---- operators on device memory ---------------------------------------------- */
+/* No counterparts in the reference. Operators that a host calls directly, with device pointers and a stream of its own:
+ * a paged key-value cache (append, attend, evict) and the scoring of a decoder's logits (log probabilities, entropy,
+ * likeliest tokens, and the gradient). They read and write the caller's memory, allocate nothing per call, and enqueue on
+ * `stream` (a cudaStream_t; NULL = the default stream); pjrtx_b200_device_stream gives the stream that buffers and
+ * executables of a device use, pjrtx_b200_buffer_device_pointer a buffer's memory. The caller's current device is left as
+ * it was. Set struct_size of every argument struct to its sizeof. Element types are f32, f16 and bf16; statistics and
+ * weights are f32, ids and lengths s32. Strides count elements; the innermost axis is dense.
+ * 1 when enqueued, 0 with last_error set. What only the device sees (a page id outside the pool, a length outside the page
+ * table, a token id outside the vocabulary) is never followed out of bounds: the kernel skips it and sets the device's error
+ * word, and the next pjrtx_b200_device_synchronize or copy to the host returns 0 and names it (codes 40, 41, 42). */
+void *pjrtx_b200_device_stream(int device_ordinal);
+/* NULL for a deleted or donated buffer, and for one without elements. */
+void *pjrtx_b200_buffer_device_pointer(PjrtxB200Buffer *buffer);
+
+/* A paged cache: keys and values of all sequences in two pools of `num_pages` pages of `page_size` rows. Row t of sequence b
+ * is row t % page_size of page page_table[b * table_stride + t / page_size]; entries beyond a sequence's rows are not read.
+ * The handle holds geometry and workspaces, not the pools, so one serves all layers of a shape. Calls on one handle share
+ * its workspaces: keep them on one stream or order them with events. */
+typedef struct PjrtxB200PagedCache PjrtxB200PagedCache;
+
+typedef struct PjrtxB200PagedCacheConfig {
+  uint64_t struct_size;
+  int32_t dtype;     /* of queries, keys, values and results */
+  int32_t track;     /* 1: attend can add up attention weights, evict can go by them (workspace for the scores) */
+  int64_t batch;     /* sequences of a call, at most */
+  int64_t heads;     /* query heads, a multiple of kv_heads: head h reads KV head h / (heads / kv_heads) */
+  int64_t kv_heads;
+  int64_t head_dim;  /* up to 256, a multiple of 16 bytes */
+  int64_t page_size; /* rows of a page, any number */
+  int64_t max_pages; /* pages of a sequence, at most; capacity = page_size * max_pages rows */
+} PjrtxB200PagedCacheConfig;
+
+/* What every call is told of the pools and of the batch. Pointers to pages and their strides keep 16-byte alignment. */
+typedef struct PjrtxB200PagedView {
+  uint64_t struct_size;
+  void *k_pages;             /* [num_pages, page_size, kv_heads, head_dim] through the strides, the same for both pools */
+  void *v_pages;
+  int64_t num_pages;
+  int64_t page_stride;
+  int64_t row_stride;
+  int64_t head_stride;
+  const int32_t *page_table; /* [batch, max_pages] */
+  int64_t table_stride;
+  const int32_t *lengths;    /* [batch]: rows of each sequence, those that the call appends among them; 0 = idle */
+  int64_t batch;
+  const int32_t *tokens;     /* [batch]: tokens each sequence has seen, the new ones among them; NULL without tracking */
+  float *weights;            /* [batch, kv_heads, capacity]: attention weight each row has had; NULL without tracking */
+  int32_t *positions;        /* [batch, kv_heads, capacity]: token of each row; NULL without tracking */
+} PjrtxB200PagedView;
+
+PjrtxB200PagedCache *pjrtx_b200_paged_cache_create(int device_ordinal, const PjrtxB200PagedCacheConfig *config);
+/* Waits for the device, then frees the workspaces. */
+void pjrtx_b200_paged_cache_destroy(PjrtxB200PagedCache *cache);
+
+/* Row lengths[b] - counts[b] + t of sequence b becomes new row t, t < counts[b]. Tracking: weight 0, position
+ * tokens[b] - counts[b] + t. */
+typedef struct PjrtxB200PagedAppendArgs {
+  uint64_t struct_size;
+  const void *k_new; /* [batch, rows, kv_heads, head_dim] through the strides */
+  const void *v_new;
+  int64_t rows;
+  int64_t batch_stride;
+  int64_t row_stride;
+  int64_t head_stride;
+  const int32_t *counts; /* [batch], NULL: `rows` for every sequence */
+} PjrtxB200PagedAppendArgs;
+int pjrtx_b200_paged_cache_append(PjrtxB200PagedCache *cache, const PjrtxB200PagedView *view,
+                                  const PjrtxB200PagedAppendArgs *args, void *stream);
+
+/* Attention of one query position per sequence over its rows: out = softmax(scale * q . k) v, lse = ln sum e^(scale * q . k).
+ * A sequence without rows gives zeros and -inf. With k_new / v_new, row lengths[b] - 1 is taken from there and stored.
+ * Tracking: weights[b, g, t] grows by the weights that the query heads of KV head g give row t (a new row's starts with
+ * them, its position is tokens[b] - 1). */
+typedef struct PjrtxB200PagedAttendArgs {
+  uint64_t struct_size;
+  const void *q; /* [batch, heads, head_dim] through the strides */
+  int64_t q_batch_stride;
+  int64_t q_head_stride;
+  void *out;     /* the same axes */
+  int64_t out_batch_stride;
+  int64_t out_head_stride;
+  float *lse;    /* [batch, heads], may be NULL */
+  const void *k_new; /* [batch, kv_heads, head_dim] through the strides, NULL: the row is in the pool already */
+  const void *v_new;
+  int64_t new_batch_stride;
+  int64_t new_head_stride;
+  float scale;
+} PjrtxB200PagedAttendArgs;
+int pjrtx_b200_paged_cache_attend(PjrtxB200PagedCache *cache, const PjrtxB200PagedView *view,
+                                  const PjrtxB200PagedAttendArgs *args, void *stream);
+
+/* Cuts every sequence of more than `keep` rows to `keep`, each KV head by itself: rows of the first `sinks` and the last
+ * `recent` tokens stay, then those with the most weight, of equal ones the lower row. The i-th kept row at or beyond `keep`
+ * moves into the place of the i-th dropped row before it; the others stay where they are. Rows without a token get weight
+ * 0 and position -1. The results may be the view's own arrays. Pages must not be shared between sequences. */
+typedef struct PjrtxB200PagedEvictArgs {
+  uint64_t struct_size;
+  int64_t keep;   /* at least sinks + recent, and 1 */
+  int64_t recent;
+  int64_t sinks;
+  int32_t *lengths_out;
+  float *weights_out;
+  int32_t *positions_out;
+} PjrtxB200PagedEvictArgs;
+int pjrtx_b200_paged_cache_evict(PjrtxB200PagedCache *cache, const PjrtxB200PagedView *view,
+                                 const PjrtxB200PagedEvictArgs *args, void *stream);
+
+/* Scores rows of logits. With p = softmax(scale * logits) of a row: log_probs = ln p[token], entropy = -sum p ln p,
+ * lse = ln sum e^(scale * logits), and the `top` likeliest ids with their log probabilities, likeliest first, of equal
+ * logits the lower id. Logits of -inf rule tokens out; a row of nothing else gives log probabilities and lse of -inf and
+ * entropy 0. NaN and +inf make a row's statistics NaN (NaN counts as likeliest). A negative token id: no token, log probability 0. */
+typedef struct PjrtxB200TokenLogProbsArgs {
+  uint64_t struct_size;
+  int32_t dtype;
+  int32_t top;           /* 0..64, at most vocab */
+  const void *logits;    /* [rows, vocab], rows row_stride elements apart, aligned to the element type */
+  int64_t rows;
+  int64_t vocab;         /* up to 2^22 */
+  int64_t row_stride;
+  const int32_t *tokens; /* [rows] */
+  float scale;           /* positive: 1 / temperature */
+  float *log_probs;      /* [rows] */
+  float *entropy;        /* [rows], may be NULL, as may the next three (one of the last two where top > 0) */
+  float *lse;            /* [rows] */
+  int32_t *top_ids;      /* [rows, top] */
+  float *top_log_probs;  /* [rows, top] */
+} PjrtxB200TokenLogProbsArgs;
+int pjrtx_b200_token_log_probs(int device_ordinal, const PjrtxB200TokenLogProbsArgs *args, void *stream);
+
+/* Gradient of sum_r (grad_log_probs[r] * log_probs[r] + grad_entropy[r] * entropy[r]) by the logits, in their element type.
+ * lse and entropy are the forward call's. A ruled-out logit has gradient 0 unless it is the token. */
+typedef struct PjrtxB200TokenLogProbsBackwardArgs {
+  uint64_t struct_size;
+  int32_t dtype;
+  float scale;
+  const void *logits;
+  void *grad_logits;     /* [rows, vocab]; may be the logits, with the same row stride */
+  int64_t rows;
+  int64_t vocab;
+  int64_t row_stride;
+  int64_t grad_row_stride;
+  const int32_t *tokens;
+  const float *lse;
+  const float *entropy;        /* with grad_entropy */
+  const float *grad_log_probs; /* [rows]; one of the two may be NULL */
+  const float *grad_entropy;   /* [rows] */
+} PjrtxB200TokenLogProbsBackwardArgs;
+int pjrtx_b200_token_log_probs_backward(int device_ordinal, const PjrtxB200TokenLogProbsBackwardArgs *args, void *stream);
+
 /* ---- generated-kernel check (no device needed) ---------------------------- */
 /* Compiles CUDA source for sm_100a with the run-time compiler; 1 when it compiles. The log goes to `out`. */
 int pjrtx_b200_compile_check(const char *source, char *out, uint64_t capacity);

@@ -17,6 +17,7 @@ from typing import List, Optional, Sequence
 
 import numpy as np
 
+from . import operators
 from . import plan as plan_mod
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -188,6 +189,7 @@ SYMBOLS = {
     "pjrtx_b200_executable_cache_install_placeholder": (ctypes.c_int, [_P, ctypes.c_char_p, ctypes.c_uint64, ctypes.c_uint64,
                                                                         ctypes.POINTER(ExecutableCacheTrim)]),
     "pjrtx_b200_executable_cache_set_compile_latency": (None, [_P, ctypes.c_char_p, ctypes.c_uint64]),
+    **operators.SYMBOLS,
 }
 
 _lib = None
@@ -247,6 +249,14 @@ class DeviceBuffer:
     @property
     def is_donated(self) -> bool:
         return bool(self._lib.pjrtx_b200_buffer_is_donated(self.handle))
+
+    @property
+    def device_pointer(self) -> int:
+        """Address of the buffer's memory on its device, for operators and for kernels of the caller's own."""
+        pointer = self._lib.pjrtx_b200_buffer_device_pointer(self.handle)
+        if not pointer and self.nbytes:
+            raise BackendError("BufferDeletedOrDonated", self._lib.pjrtx_b200_last_error().decode())
+        return pointer
 
     def to_numpy(self) -> np.ndarray:
         out = np.empty(self.dims, dtype=plan_mod.np_dtype(self.dtype))
@@ -689,6 +699,32 @@ class Backend:
         bounded device-side waits (its output is then not valid). Allocates nothing; ask before the next call."""
         if not self.lib.pjrtx_b200_dot_static_scratch_status(device, ctypes.c_void_p(stream)):
             raise BackendError("CommandSubmissionFailed", self._err())
+
+    # -- operators on device memory --
+    def device_stream(self, device: int = 0) -> int:
+        """The `cudaStream_t` on which the device's buffers and executables work."""
+        stream = self.lib.pjrtx_b200_device_stream(device)
+        if not stream:
+            raise BackendError("InvalidDeviceCount", self._err())
+        return stream
+
+    def paged_cache(self, dtype: int, batch: int, heads: int, kv_heads: int, head_dim: int, page_size: int, max_pages: int,
+                    track: bool = False, device: int = 0) -> operators.PagedCache:
+        """Handle of a paged key-value cache with `append`, `attend` and `evict`; batch and max_pages are upper bounds."""
+        return operators.PagedCache(self, dtype, batch, heads, kv_heads, head_dim, page_size, max_pages, track, device)
+
+    def token_log_probs(self, logits, tokens, log_probs, entropy=None, lse=None, top_ids=None, top_log_probs=None,
+                        scale: float = 1.0, stream: Optional[int] = None, device: int = 0) -> None:
+        """Scores logits [rows, vocabulary] with p = softmax(scale * logits): log_probs [rows] = ln p[tokens], entropy [rows],
+        lse [rows], and the likeliest ids and their log probabilities, as many as top_ids / top_log_probs [rows, k] have
+        columns (ties: the lower id first). A negative token id gives 0."""
+        operators.token_log_probs(self, logits, tokens, log_probs, entropy, lse, top_ids, top_log_probs, scale, stream, device)
+
+    def token_log_probs_backward(self, logits, tokens, lse, grad_logits, grad_log_probs=None, entropy=None, grad_entropy=None,
+                                 scale: float = 1.0, stream: Optional[int] = None, device: int = 0) -> None:
+        """grad_logits [rows, vocabulary] = gradient of sum(grad_log_probs * log_probs) + sum(grad_entropy * entropy) by the
+        logits; lse and entropy are the forward call's, grad_logits may be the logits."""
+        operators.token_log_probs_backward(self, logits, tokens, lse, grad_logits, grad_log_probs, entropy, grad_entropy, scale, stream, device)
 
     def compile_check(self, source: str) -> str:
         """Compiles generated CUDA source for sm_100a (no GPU needed); returns "" or the compiler log."""

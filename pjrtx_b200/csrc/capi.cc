@@ -11,6 +11,7 @@
 #include "device.h"
 #include "executable_cache.h"
 #include "executor.h"
+#include "operators.h"
 #include "plan.h"
 #include "program.h"
 #include "sharding.h"
@@ -38,6 +39,9 @@ struct PjrtxB200ExecutableCache {
           delete w;
         }),
         capacity_bytes(capacity) {}
+};
+struct PjrtxB200PagedCache {
+  PagedCache* cache;
 };
 struct PjrtxB200ExecutionEvent {
   int device;
@@ -68,6 +72,40 @@ uint64_t write_text(const std::string& s, char* out, uint64_t capacity) {
 PjrtxB200Buffer* wrap(Buffer* b) {
   if (!b) return nullptr;
   return new PjrtxB200Buffer{b};
+}
+
+// An argument struct of this header's size or a later one's.
+template <typename Args>
+bool have(const Args* args) {
+  if (args && args->struct_size >= sizeof(Args)) return true;
+  set_last_error(args ? "argument struct of %llu bytes (set struct_size)" : "null argument struct", args ? (unsigned long long)args->struct_size : 0ull);
+  return false;
+}
+
+// A 64-bit size that a kernel holds in 32 bits; what does not fit becomes -1, which the checks behind refuse.
+int narrow(int64_t v) { return v < 0 || v > INT32_MAX ? -1 : (int)v; }
+
+PagedView view_of(const PjrtxB200PagedView& v) {
+  PagedView r;
+  r.k = v.k_pages;
+  r.v = v.v_pages;
+  r.num_pages = v.num_pages;
+  r.page_stride = v.page_stride;
+  r.row_stride = v.row_stride;
+  r.head_stride = v.head_stride;
+  r.table = v.page_table;
+  r.table_stride = v.table_stride;
+  r.lengths = v.lengths;
+  r.batch = narrow(v.batch);
+  r.tokens = v.tokens;
+  r.weights = v.weights;
+  r.positions = v.positions;
+  return r;
+}
+
+bool have_cache(const PjrtxB200PagedCache* cache) {
+  if (!cache) set_last_error("null paged cache");
+  return cache != nullptr;
 }
 
 }  // namespace
@@ -722,6 +760,74 @@ int pjrtx_b200_dot_static_scratch(int device_ordinal, int dtype, const void* lhs
 
 int pjrtx_b200_dot_static_scratch_status(int device_ordinal, void* stream) {
   GUARD_INT(return stream_dot_static_scratch_status(device_ordinal, (cudaStream_t)stream);)
+}
+
+void* pjrtx_b200_device_stream(int device_ordinal) {
+  GUARD_PTR(Device* d = get_device(device_ordinal); return d ? (void*)d->stream : nullptr;)
+}
+
+void* pjrtx_b200_buffer_device_pointer(PjrtxB200Buffer* buffer) {
+  GUARD_PTR(if (!buffer || !buffer->b || buffer->b->donated || !buffer->b->bytes) {
+    set_last_error("buffer is deleted, donated or empty");
+    return nullptr;
+  } return buffer->b->ptr;)
+}
+
+PjrtxB200PagedCache* pjrtx_b200_paged_cache_create(int device_ordinal, const PjrtxB200PagedCacheConfig* config) {
+  GUARD_PTR(if (!have(config)) return nullptr; PagedCacheConfig c; c.dtype = config->dtype; c.track = config->track != 0;
+            c.batch = config->batch; c.heads = config->heads; c.kv_heads = config->kv_heads; c.head_dim = config->head_dim;
+            c.page_size = config->page_size; c.max_pages = config->max_pages;
+            PagedCache* made = paged_cache_create(device_ordinal, c); return made ? new PjrtxB200PagedCache{made} : nullptr;)
+}
+
+void pjrtx_b200_paged_cache_destroy(PjrtxB200PagedCache* cache) {
+  try {
+    if (!cache) return;
+    paged_cache_destroy(cache->cache);
+    delete cache;
+  } catch (...) {
+  }
+}
+
+int pjrtx_b200_paged_cache_append(PjrtxB200PagedCache* cache, const PjrtxB200PagedView* view, const PjrtxB200PagedAppendArgs* args,
+                                  void* stream) {
+  GUARD_INT(if (!have_cache(cache) || !have(view) || !have(args)) return 0; PagedAppend a; a.k_new = args->k_new; a.v_new = args->v_new;
+            a.rows = args->rows; a.batch_stride = args->batch_stride; a.row_stride = args->row_stride;
+            a.head_stride = args->head_stride; a.counts = args->counts;
+            return paged_cache_append(*cache->cache, view_of(*view), a, (cudaStream_t)stream);)
+}
+
+int pjrtx_b200_paged_cache_attend(PjrtxB200PagedCache* cache, const PjrtxB200PagedView* view, const PjrtxB200PagedAttendArgs* args,
+                                  void* stream) {
+  GUARD_INT(if (!have_cache(cache) || !have(view) || !have(args)) return 0; PagedAttend a; a.q = args->q;
+            a.q_batch_stride = args->q_batch_stride; a.q_head_stride = args->q_head_stride; a.out = args->out;
+            a.out_batch_stride = args->out_batch_stride; a.out_head_stride = args->out_head_stride; a.lse = args->lse;
+            a.k_new = args->k_new; a.v_new = args->v_new; a.new_batch_stride = args->new_batch_stride;
+            a.new_head_stride = args->new_head_stride; a.scale = args->scale;
+            return paged_cache_attend(*cache->cache, view_of(*view), a, (cudaStream_t)stream);)
+}
+
+int pjrtx_b200_paged_cache_evict(PjrtxB200PagedCache* cache, const PjrtxB200PagedView* view, const PjrtxB200PagedEvictArgs* args,
+                                 void* stream) {
+  GUARD_INT(if (!have_cache(cache) || !have(view) || !have(args)) return 0; PagedEvict e; e.keep = narrow(args->keep);
+            e.recent = narrow(args->recent); e.sinks = narrow(args->sinks); e.lengths_out = args->lengths_out;
+            e.weights_out = args->weights_out; e.positions_out = args->positions_out;
+            return paged_cache_evict(*cache->cache, view_of(*view), e, (cudaStream_t)stream);)
+}
+
+int pjrtx_b200_token_log_probs(int device_ordinal, const PjrtxB200TokenLogProbsArgs* args, void* stream) {
+  GUARD_INT(if (!have(args)) return 0; TokenScore s; s.dtype = args->dtype;
+            s.top = args->top; s.logits = args->logits; s.rows = args->rows; s.vocab = args->vocab; s.row_stride = args->row_stride;
+            s.tokens = args->tokens; s.scale = args->scale; s.log_probs = args->log_probs; s.entropy = args->entropy; s.lse = args->lse;
+            s.top_ids = args->top_ids; s.top_log_probs = args->top_log_probs; return token_log_probs(device_ordinal, s, (cudaStream_t)stream);)
+}
+
+int pjrtx_b200_token_log_probs_backward(int device_ordinal, const PjrtxB200TokenLogProbsBackwardArgs* args, void* stream) {
+  GUARD_INT(if (!have(args)) return 0; TokenScoreGrad s; s.dtype = args->dtype;
+            s.scale = args->scale; s.logits = args->logits; s.grad_logits = args->grad_logits; s.rows = args->rows;
+            s.vocab = args->vocab; s.row_stride = args->row_stride; s.grad_row_stride = args->grad_row_stride;
+            s.tokens = args->tokens; s.lse = args->lse; s.entropy = args->entropy; s.grad_log_probs = args->grad_log_probs;
+            s.grad_entropy = args->grad_entropy; return token_log_probs_backward(device_ordinal, s, (cudaStream_t)stream);)
 }
 
 int pjrtx_b200_compile_check(const char* source, char* out, uint64_t capacity) {

@@ -1,6 +1,7 @@
 #include "device.h"
 
 #include "kernels/kernels.h"
+#include "kernels/operators.h"
 
 #include <dlfcn.h>
 #include <nccl.h>
@@ -74,6 +75,14 @@ bool check_device_flag(Device* dev) {
   int code = *(volatile int*)dev->error_flag_host;
   if (code == 0) return true;
   *(volatile int*)dev->error_flag_host = 0;
+  if (code >= kErrorPageId && code <= kErrorToken) {
+    set_last_error("a kernel on device %d met %s (code %d); the results of that call are invalid", dev->ordinal,
+                   code == kErrorPageId ? "a page table entry outside the pool of pages"
+                   : code == kErrorLength ? "a length outside the page table or a count beyond its length"
+                                          : "a token id outside the vocabulary",
+                   code);
+    return false;
+  }
   set_last_error("a kernel on device %d gave up a bounded wait (code %d); results of this stream are invalid", dev->ordinal, code);
   return false;
 }

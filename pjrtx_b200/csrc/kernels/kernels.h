@@ -26,6 +26,19 @@ inline bool raise_smem_limit(const void* kernel, int bytes) {
   return true;
 }
 
+// Makes `device` current for the lifetime of the object and restores the caller's device afterwards.
+struct CurrentDevice {
+  int previous = -1;
+  bool ok = false;
+  explicit CurrentDevice(int device) {
+    if (cudaGetDevice(&previous) != cudaSuccess) previous = -1;
+    ok = cudaSetDevice(device) == cudaSuccess;
+  }
+  ~CurrentDevice() {
+    if (previous >= 0) cudaSetDevice(previous);
+  }
+};
+
 // Attributes of every launch of the library: programmatic stream serialization when `pdl`, and - when
 // PJRTX_B200_CARVEOUT is set (0..100) - that shared-memory carveout, the same for every kernel, so that consecutive
 // kernels never ask the SMs for different splits between L1 and shared memory. Returns the number filled in (<= 2).

@@ -63,19 +63,6 @@ unsigned char* setup_device(int device) {
   return ptr;
 }
 
-// Makes `device` current for the lifetime of the object and restores the caller's device afterwards.
-struct CurrentDevice {
-  int previous = -1;
-  bool ok = false;
-  explicit CurrentDevice(int device) {
-    if (cudaGetDevice(&previous) != cudaSuccess) previous = -1;
-    ok = cudaSetDevice(device) == cudaSuccess;
-  }
-  ~CurrentDevice() {
-    if (previous >= 0) cudaSetDevice(previous);
-  }
-};
-
 template <typename T>
 int launch(const DotShape& s, const DotScratch& plan, const void* lhs, const void* rhs, void* out, unsigned char* scratch,
            cudaStream_t stream) {
