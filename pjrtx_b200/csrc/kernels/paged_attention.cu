@@ -22,101 +22,744 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-template <typename T> __device__ __forceinline__ float to_float(T v);
-template <> __device__ __forceinline__ float to_float(float v) { return v; }
-template <> __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <typename T> __device__ __forceinline__ T from_float(float v);
 template <> __device__ __forceinline__ float from_float(float v) { return v; }
 template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
 
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ float max_nan(float a, float b) {
   float y;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
 
+// ---- division of the work ------------------------------------------------------------------------------------------
+// A unit is a tile of 64 rows of one (sequence, KV head, group of query heads). Units are numbered in that order, only those
+// that the lengths call for, and every block takes the same number of consecutive ones: lengths are device data, so each block
+// adds them up itself. What belongs to one (sequence, head group) is a segment; where several blocks share one, each leaves
+// (max, sum, values) in its slot of the workspace and the block that arrives last joins them in block order.
+
+constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kWarpRows = 16, kTileRows = kWarps * kWarpRows;
+
 struct AttendSpace {
-  float* lse2;    // [batch, heads]: lse / ln 2
-  float* scores;  // [batch, kv_heads, capacity, rep] in units of ln 2 (tracking only)
+  float* lse2;         // [batch, heads]: lse / ln 2
+  unsigned* counters;  // [batch * kv_heads * head groups]: blocks that have arrived, zero between calls
+  float* partials;     // [blocks][2][heads of a group][dims + 2]
+  float* scores;       // [batch, kv_heads, capacity, rep] in units of ln 2 (tracking only)
 };
 
-inline AttendSpace attend_space(const PagedView& c, int heads, void* workspace) {
-  AttendSpace s;
-  char* p = static_cast<char*>(workspace);
-  s.lse2 = reinterpret_cast<float*>(p);
-  s.scores = reinterpret_cast<float*>(p + ((uint64_t)c.batch_max * heads * 4 + 255) / 256 * 256);
+struct AttendArgs {
+  PagedView c;
+  PagedAttend a;
+  AttendSpace space;
+  int rep, groups;  // query heads of a KV head, groups of them
+  int pieces;       // 16-byte pieces of a row
+};
+
+struct Cursor {
+  int b, group, tile, tiles, length;  // group = KV head * groups + head group
+};
+
+__device__ __forceinline__ int tiles_of(int length) { return (length + kTileRows - 1) / kTileRows; }
+
+__device__ __forceinline__ void advance(const AttendArgs& p, Cursor& u) {
+  if (++u.tile < u.tiles) return;
+  u.tile = 0;
+  if (++u.group < p.c.kv_heads * p.groups) return;
+  u.group = 0;
+  do {
+    u.b++;
+    u.length = paged_length(p.c, u.b);
+    u.tiles = tiles_of(u.length);
+  } while (u.tiles == 0);
+}
+
+// What this block works on: units [begin, end) of all, starting at `at`; `quota` units a block.
+struct Share {
+  long long begin, end, quota;
+  Cursor at;
+};
+
+// Called by all threads. `scratch`: shared memory of kWarps + 1 long longs and 4 ints.
+__device__ __forceinline__ Share share_of_block(const AttendArgs& p, long long* scratch) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int per_thread = (p.c.batch + kThreads - 1) / kThreads;
+  const int first = min(p.c.batch, (int)threadIdx.x * per_thread), last = min(p.c.batch, first + per_thread);
+  const long long width = (long long)p.c.kv_heads * p.groups;
+  long long mine = 0;
+  for (int b = first; b < last; b++) mine += tiles_of(paged_length(p.c, b)) * width;
+  long long sum = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const long long o = __shfl_up_sync(~0u, sum, d);
+    if (lane >= d) sum += o;
+  }
+  if (lane == 31) scratch[warp] = sum;
+  __syncthreads();
+  long long before = sum - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; w++) {
+    if (w < warp) before += scratch[w];
+    total += scratch[w];
+  }
+  Share s;
+  s.quota = max(1ll, (total + gridDim.x - 1) / gridDim.x);
+  s.begin = min(total, blockIdx.x * s.quota);
+  s.end = min(total, s.begin + s.quota);
+  int* found = reinterpret_cast<int*>(scratch + kWarps);
+  if (s.begin < s.end && before <= s.begin && s.begin < before + mine) {
+    long long rest = s.begin - before;
+    int b = first, length = 0, tiles = 0;
+    for (;; b++) {
+      length = paged_length(p.c, b);
+      tiles = tiles_of(length);
+      if (rest < tiles * width) break;
+      rest -= tiles * width;
+    }
+    found[0] = b;
+    found[1] = (int)(rest / tiles);
+    found[2] = (int)(rest % tiles);
+    found[3] = length;
+  }
+  __syncthreads();
+  s.at.b = found[0];
+  s.at.group = found[1];
+  s.at.tile = found[2];
+  s.at.length = found[3];
+  s.at.tiles = tiles_of(s.at.length);
   return s;
 }
 
-constexpr int kSimpleWarps = 8;
+// ---- rows into shared memory ---------------------------------------------------------------------------------------
+// A warp works by itself: it fetches 16 rows of each tile with cp.async into stages of its own, so the warps of a block meet
+// only at the end of a segment. Rows outside the sequence (or without a page) are filled with zeros and masked.
 
-// One block per (query head, sequence), one key per warp and step.
-template <typename T>
-__global__ void __launch_bounds__(kSimpleWarps * 32) paged_attend_kernel(PagedView c, PagedAttend a, AttendSpace space) {
-  constexpr int R = 8;  // 256 / 32
-  __shared__ float acc[kSimpleWarps][32 * R];
-  __shared__ float stat[kSimpleWarps][2];
-  PJRTX_PDL_PROLOGUE();
-  const int h = blockIdx.x, b = blockIdx.y, rep = a.heads / c.kv_heads, g = h / rep;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, D = c.head_dim;
-  const int n = paged_length(c, b);
-  if (h == 0 && threadIdx.x == 0) paged_check_length(c, b);
-  const T* q = static_cast<const T*>(a.q) + b * a.q_batch_stride + h * a.q_head_stride;
-  float qr[R], o[R], m = -INFINITY, l = 0.f;
-  for (int i = 0; i < R; i++) {
-    const int d = lane + 32 * i;
-    qr[i] = d < D ? to_float(q[d]) * a.scale * kLog2e : 0.f;
-    o[i] = 0.f;
+template <typename T, int D>
+struct RowStage {
+  static constexpr int kPitch = D * (int)sizeof(T) + 16;  // bytes; rows of eight keys fall on different banks
+  static constexpr int kBytes = 2 * kWarpRows * kPitch;
+};
+
+__device__ __forceinline__ void copy16(unsigned to, const void* from, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Where row `lane % 16` of this warp's part of a tile lies.
+struct RowPlace {
+  int page, row;  // page -1: no such row
+};
+
+__device__ __forceinline__ RowPlace locate(const AttendArgs& p, const Cursor& u) {
+  const int t = u.tile * kTileRows + (threadIdx.x / 32) * kWarpRows + (threadIdx.x & 15);
+  RowPlace r = {-1, 0};
+  if (t < u.length) {
+    const int column = t / p.c.page_size;
+    r.row = t - column * p.c.page_size;
+    r.page = p.c.table[u.b * p.c.table_stride + column];
+    if (r.page < 0 || r.page >= p.c.num_pages) {
+      report(p.c.error_flag, kErrorPageId);
+      r.page = -1;
+    }
   }
-  for (int t = warp; t < n; t += kSimpleWarps) {
-    const long long row = paged_row(c, b, t);
-    if (row < 0) continue;
-    const T* k = static_cast<const T*>(c.k) + row + g * c.head_stride;
-    const T* v = static_cast<const T*>(c.v) + row + g * c.head_stride;
-    if (a.k_new && t == n - 1) {
-      const T* k_new = static_cast<const T*>(a.k_new) + b * a.new_batch_stride + g * a.new_head_stride;
-      const T* v_new = static_cast<const T*>(a.v_new) + b * a.new_batch_stride + g * a.new_head_stride;
-      if (h % rep == 0)
-        for (int d = lane; d < D; d += 32) {
-          const_cast<T*>(k)[d] = k_new[d];
-          const_cast<T*>(v)[d] = v_new[d];
-        }
+  return r;
+}
+
+// Requests the rows of `u`; the stage's mask word says which ones count.
+template <typename T, int D>
+__device__ __forceinline__ void request(const AttendArgs& p, const Cursor& u, const RowPlace& r, char* stage, unsigned* mask) {
+  using S = RowStage<T, D>;
+  constexpr int kPieces = D * (int)sizeof(T) / 16;
+  constexpr int kAcross = kPieces < 8 ? kPieces : 8;  // lanes beside each other on one row
+  const int lane = threadIdx.x % 32, g = u.group / p.groups;
+  const int t0 = u.tile * kTileRows + (threadIdx.x / 32) * kWarpRows;
+  const char *k = nullptr, *v = nullptr;
+  if (r.page >= 0) {
+    const long long at = (r.page * p.c.page_stride + r.row * p.c.row_stride + g * p.c.head_stride) * (long long)sizeof(T);
+    k = static_cast<const char*>(p.c.k) + at;
+    v = static_cast<const char*>(p.c.v) + at;
+  }
+  const int fresh = u.length - 1 - t0;  // which of the 16 rows comes with the call
+  if (p.a.k_new && fresh >= 0 && fresh < kWarpRows) {
+    const long long at = (u.b * p.a.new_batch_stride + g * p.a.new_head_stride) * (long long)sizeof(T);
+    const char* k_new = static_cast<const char*>(p.a.k_new) + at;
+    const char* v_new = static_cast<const char*>(p.a.v_new) + at;
+    char* k_to = reinterpret_cast<char*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(k), fresh));
+    char* v_to = reinterpret_cast<char*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(v), fresh));
+    if (k_to && u.group % p.groups == 0)
+      for (int i = lane; i < p.pieces; i += 32) {
+        reinterpret_cast<uint4*>(k_to)[i] = reinterpret_cast<const uint4*>(k_new)[i];
+        reinterpret_cast<uint4*>(v_to)[i] = reinterpret_cast<const uint4*>(v_new)[i];
+      }
+    if ((lane & 15) == fresh && k) {
       k = k_new;
       v = v_new;
     }
-    float s = 0.f;
-    for (int i = 0; i < R; i++)
-      if (lane + 32 * i < D) s = fmaf(qr[i], to_float(k[lane + 32 * i]), s);
-    for (int d = 16; d; d /= 2) s += __shfl_xor_sync(~0u, s, d);
-    if (c.weights && lane == 0) space.scores[(((long long)b * c.kv_heads + g) * c.page_size * c.max_pages + t) * rep + h % rep] = s;
-    const float to = max_nan(m, s), f = m == -INFINITY ? 0.f : exp2f(m - to), p = to == -INFINITY ? 0.f : exp2f(s - to);
-    l = l * f + p;
-    for (int i = 0; i < R; i++)
-      if (lane + 32 * i < D) o[i] = fmaf(p, to_float(v[lane + 32 * i]), o[i] * f);
-    m = to;
   }
-  if (lane == 0) {
-    stat[warp][0] = m;
-    stat[warp][1] = l;
+  const unsigned there = __ballot_sync(~0u, k != nullptr) & 0xffffu;
+  if (lane == 0) *mask = there;
+  const unsigned to = (unsigned)__cvta_generic_to_shared(stage);
+#pragma unroll
+  for (int j = 0; j < kWarpRows * kAcross / 32; j++) {
+    const int row = lane / kAcross + j * (32 / kAcross);
+    const char* kr = reinterpret_cast<const char*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(k), row));
+    const char* vr = reinterpret_cast<const char*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(v), row));
+#pragma unroll
+    for (int i = 0; i < kPieces / kAcross; i++) {
+      const int piece = lane % kAcross + i * kAcross;
+      const bool valid = kr != nullptr && piece < p.pieces;
+      copy16(to + row * S::kPitch + piece * 16, valid ? kr + piece * 16 : static_cast<const char*>(p.c.k), valid);
+      copy16(to + (kWarpRows + row) * S::kPitch + piece * 16, valid ? vr + piece * 16 : static_cast<const char*>(p.c.v), valid);
+    }
   }
-  for (int i = 0; i < R; i++) acc[warp][lane + 32 * i] = o[i];
-  __syncthreads();
-  float top = -INFINITY, total = 0.f;
-  for (int w = 0; w < kSimpleWarps; w++) top = max_nan(top, stat[w][0]);
-  for (int w = 0; w < kSimpleWarps; w++) total += stat[w][0] == -INFINITY ? 0.f : stat[w][1] * exp2f(stat[w][0] - top);
-  const float inverse = total > 0.f ? 1.f / total : (total != total ? total : 0.f);
-  T* out = static_cast<T*>(a.out) + b * a.out_batch_stride + h * a.out_head_stride;
-  for (int d = threadIdx.x; d < D; d += blockDim.x) {
-    float x = 0.f;
-    for (int w = 0; w < kSimpleWarps; w++) x += stat[w][0] == -INFINITY ? 0.f : acc[w][d] * exp2f(stat[w][0] - top);
-    out[d] = from_float<T>(x * inverse);
+}
+
+// ---- the arithmetic of one warp ------------------------------------------------------------------------------------
+
+template <typename T> struct Mma16;
+template <> struct Mma16<__nv_bfloat16> {
+  static __device__ __forceinline__ unsigned pack(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const unsigned*>(&h);
   }
-  if (threadIdx.x == 0) {
-    const float lse2 = total == 0.f ? -INFINITY : top + log2f(total);
-    space.lse2[(long long)b * a.heads + h] = lse2;
-    if (a.lse) a.lse[(long long)b * a.heads + h] = lse2 * kLn2;
+  static __device__ __forceinline__ float2 unpack(unsigned w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+  static __device__ __forceinline__ void mma(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+template <> struct Mma16<__half> {
+  static __device__ __forceinline__ unsigned pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const unsigned*>(&h);
+  }
+  static __device__ __forceinline__ float2 unpack(unsigned w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+  static __device__ __forceinline__ void mma(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+
+__device__ __forceinline__ void load_matrices(unsigned (&r)[4], unsigned at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void load_matrices_transposed(unsigned (&r)[4], unsigned at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ unsigned transpose(unsigned a) {
+  unsigned d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+// 16-bit types: rows and dimensions are the long sides of the products, heads the eight columns of m16n8k16, so that up to eight
+// query heads cost no more than one: scores^T [16 rows x heads] = K q^T, values^T [dims x heads] += V^T p^T. A probability goes in
+// as two 16-bit numbers, its rounding and what that leaves off: rounded to one, it would be as far off as the result's own rounding.
+// Lane i holds heads (i % 4) * 2 and + 1 of every eight.
+template <typename T, int D, int NB>
+struct MmaWarp {
+  static constexpr int kHeads = 8 * NB;
+  static constexpr int kSharedBytes = 0;
+  unsigned q[D / 16][NB][2];
+  float o[D / 16][NB][4];
+  float m[NB][2], l[NB][2];
+
+  __device__ __forceinline__ void start(const AttendArgs& p, const Cursor& u, char*) {
+    const int lane = threadIdx.x % 32, g = u.group / p.groups, h0 = (u.group % p.groups) * kHeads;
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+      const int h = h0 + n * 8 + lane / 4;
+      const T* from = static_cast<const T*>(p.a.q) + u.b * p.a.q_batch_stride + (long long)(g * p.rep + h) * p.a.q_head_stride;
+#pragma unroll
+      for (int i = 0; i < D / 16; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const int d = i * 16 + j * 8 + (lane % 4) * 2;
+          q[i][n][j] = h < p.rep && d < p.c.head_dim ? *reinterpret_cast<const unsigned*>(from + d) : 0u;
+        }
+#pragma unroll
+      for (int i = 0; i < D / 16; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[i][n][j] = 0.f;
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+    }
+  }
+
+  __device__ __forceinline__ void step(const AttendArgs& p, const Cursor& u, const char* stage, unsigned mask, float scale2) {
+    constexpr int kPitch = RowStage<T, D>::kPitch;
+    const int lane = threadIdx.x % 32;
+    const unsigned k_at = (unsigned)__cvta_generic_to_shared(stage), v_at = k_at + kWarpRows * kPitch;
+    float s[NB][4];
+#pragma unroll
+    for (int n = 0; n < NB; n++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) s[n][j] = 0.f;
+    const unsigned k_lane = k_at + ((lane / 8 % 2) * 8 + lane % 8) * kPitch + (lane / 16) * 16;
+#pragma unroll
+    for (int i = 0; i < D / 16; i++) {
+      unsigned a[4];
+      load_matrices(a, k_lane + i * 32);
+#pragma unroll
+      for (int n = 0; n < NB; n++) Mma16<T>::mma(s[n], a, q[i][n][0], q[i][n][1]);
+    }
+    const bool lo = mask >> (lane / 4) & 1, hi = mask >> (lane / 4 + 8) & 1;
+    bool grows = false;
+    float top[NB][2];
+#pragma unroll
+    for (int n = 0; n < NB; n++)
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        s[n][j] = lo ? s[n][j] * scale2 : -INFINITY;
+        s[n][2 + j] = hi ? s[n][2 + j] * scale2 : -INFINITY;
+        top[n][j] = max_nan(s[n][j], s[n][2 + j]);
+        grows |= !(top[n][j] <= m[n][j]);
+      }
+    if (p.c.weights) store_scores(p, u, s, lo, hi);
+    if (__any_sync(~0u, grows)) {
+#pragma unroll
+      for (int n = 0; n < NB; n++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          float t = top[n][j];
+#pragma unroll
+          for (int d = 4; d < 32; d *= 2) t = max_nan(t, __shfl_xor_sync(~0u, t, d));
+          t = max_nan(m[n][j], t);
+          const float f = m[n][j] == -INFINITY ? 0.f : exp2_fast(m[n][j] - t);
+          m[n][j] = t;
+          l[n][j] *= f;
+#pragma unroll
+          for (int i = 0; i < D / 16; i++) {
+            o[i][n][j] *= f;
+            o[i][n][2 + j] *= f;
+          }
+        }
+    }
+    unsigned big[NB][2], small[NB][2];
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const float from = m[n][j] == -INFINITY ? 0.f : m[n][j];
+        s[n][j] = exp2_fast(s[n][j] - from);
+        s[n][2 + j] = exp2_fast(s[n][2 + j] - from);
+        l[n][j] += s[n][j] + s[n][2 + j];
+      }
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        const unsigned b = Mma16<T>::pack(s[n][2 * r], s[n][2 * r + 1]);
+        const float2 back = Mma16<T>::unpack(b);
+        big[n][r] = transpose(b);
+        small[n][r] = transpose(Mma16<T>::pack(s[n][2 * r] - back.x, s[n][2 * r + 1] - back.y));
+      }
+    }
+    const unsigned v_lane = v_at + ((lane / 16) * 8 + lane % 8) * kPitch + (lane / 8 % 2) * 16;
+#pragma unroll
+    for (int i = 0; i < D / 16; i++) {
+      unsigned a[4];
+      load_matrices_transposed(a, v_lane + i * 32);
+#pragma unroll
+      for (int n = 0; n < NB; n++) {
+        Mma16<T>::mma(o[i][n], a, big[n][0], big[n][1]);
+        Mma16<T>::mma(o[i][n], a, small[n][0], small[n][1]);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void store_scores(const AttendArgs& p, const Cursor& u, const float (&s)[NB][4], bool lo, bool hi) const {
+    const int lane = threadIdx.x % 32, g = u.group / p.groups, h0 = (u.group % p.groups) * kHeads;
+    const int t = u.tile * kTileRows + (threadIdx.x / 32) * kWarpRows + lane / 4;
+    float* to = p.space.scores + (((long long)u.b * p.c.kv_heads + g) * p.c.page_size * p.c.max_pages + t) * p.rep + h0;
+#pragma unroll
+    for (int n = 0; n < NB; n++)
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const int h = n * 8 + (lane % 4) * 2 + j;
+        if (h0 + h >= p.rep) continue;
+        if (lo) to[h] = s[n][j];
+        if (hi) to[8 * p.rep + h] = s[n][2 + j];
+      }
+  }
+
+  // Leaves this warp's maxima and sums in stat[head][2].
+  __device__ __forceinline__ void statistics(float* stat) {
+    const int lane = threadIdx.x % 32;
+#pragma unroll
+    for (int n = 0; n < NB; n++)
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2) l[n][j] += __shfl_xor_sync(~0u, l[n][j], d);
+        if (lane < 4) {
+          stat[2 * (n * 8 + lane * 2 + j)] = m[n][j];
+          stat[2 * (n * 8 + lane * 2 + j) + 1] = l[n][j];
+        }
+      }
+  }
+  // values[head * pitch + dim] (+)= values * factor[head].
+  __device__ __forceinline__ void add_values(float* values, int pitch, const float* factor, bool first) const {
+    const int lane = threadIdx.x % 32;
+#pragma unroll
+    for (int n = 0; n < NB; n++)
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const int h = n * 8 + (lane % 4) * 2 + j;
+        const float f = factor[h];
+#pragma unroll
+        for (int i = 0; i < D / 16; i++)
+#pragma unroll
+          for (int r = 0; r < 2; r++) {
+            float* to = values + h * pitch + i * 16 + r * 8 + lane / 4;
+            const float x = o[i][n][2 * r + j] * f;
+            *to = first ? x : *to + x;
+          }
+      }
+  }
+};
+
+// f32: CUDA cores. Scores: lane i has row i % 16 and one half of the dimensions. Values: lane i has D / 32 neighbouring dimensions.
+template <int D, int H>
+struct FmaWarp {
+  static constexpr int kHeads = H, V = D / 32;
+  static constexpr int kSharedBytes = H * D * 4 + kWarps * kWarpRows * H * 4;  // queries; probabilities of every warp
+  float o[H][V];
+  float m[H], l[H];
+  const float* queries;
+  float* probabilities;
+
+  __device__ __forceinline__ void start(const AttendArgs& p, const Cursor& u, char* shared) {
+    const int g = u.group / p.groups, h0 = (u.group % p.groups) * H;
+    float* to = reinterpret_cast<float*>(shared);
+    queries = to;
+    probabilities = to + H * D + (threadIdx.x / 32) * kWarpRows * H;
+    __syncthreads();
+    for (int i = threadIdx.x; i < H * D; i += kThreads) {
+      const int h = h0 + i / D, d = i % D;
+      to[i] = h < p.rep && d < p.c.head_dim
+                  ? static_cast<const float*>(p.a.q)[u.b * p.a.q_batch_stride + (long long)(g * p.rep + h) * p.a.q_head_stride + d] : 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < H; h++) {
+#pragma unroll
+      for (int i = 0; i < V; i++) o[h][i] = 0.f;
+      m[h] = -INFINITY;
+      l[h] = 0.f;
+    }
+  }
+
+  __device__ __forceinline__ void step(const AttendArgs& p, const Cursor& u, const char* stage, unsigned mask, float scale2) {
+    constexpr int kPitch = RowStage<float, D>::kPitch;
+    const int lane = threadIdx.x % 32;
+    float s[H];
+#pragma unroll
+    for (int h = 0; h < H; h++) s[h] = 0.f;
+    const char* k = stage + (lane % 16) * kPitch;
+#pragma unroll 4
+    for (int i = 0; i < D / 8; i++) {  // the halves alternate in pieces of 16 bytes
+      const int d = (2 * i + lane / 16) * 4;
+      const float4 x = *reinterpret_cast<const float4*>(k + d * 4);
+#pragma unroll
+      for (int h = 0; h < H; h++) {
+        const float4 y = *reinterpret_cast<const float4*>(queries + h * D + d);
+        s[h] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s[h]))));
+      }
+    }
+    const bool there = mask >> (lane % 16) & 1;
+    bool grows = false;
+#pragma unroll
+    for (int h = 0; h < H; h++) {
+      s[h] += __shfl_xor_sync(~0u, s[h], 16);
+      s[h] = there ? s[h] * scale2 : -INFINITY;
+      grows |= !(s[h] <= m[h]);
+    }
+    if (p.c.weights && there && lane < 16) {
+      const int g = u.group / p.groups, h0 = (u.group % p.groups) * H;
+      const int t = u.tile * kTileRows + (threadIdx.x / 32) * kWarpRows + lane;
+      float* to = p.space.scores + (((long long)u.b * p.c.kv_heads + g) * p.c.page_size * p.c.max_pages + t) * p.rep + h0;
+#pragma unroll
+      for (int h = 0; h < H; h++)
+        if (h0 + h < p.rep) to[h] = s[h];
+    }
+    if (__any_sync(~0u, grows)) {
+#pragma unroll
+      for (int h = 0; h < H; h++) {
+        float t = s[h];
+#pragma unroll
+        for (int d = 1; d < 16; d *= 2) t = max_nan(t, __shfl_xor_sync(~0u, t, d));
+        t = max_nan(m[h], t);
+        const float f = m[h] == -INFINITY ? 0.f : exp2_fast(m[h] - t);
+        m[h] = t;
+        l[h] *= f;
+#pragma unroll
+        for (int i = 0; i < V; i++) o[h][i] *= f;
+      }
+    }
+    float* mine = probabilities + (lane % 16) * H;
+#pragma unroll
+    for (int h = 0; h < H; h++) {
+      s[h] = exp2_fast(s[h] - (m[h] == -INFINITY ? 0.f : m[h]));
+      if (lane < 16) {
+        mine[h] = s[h];
+        l[h] += s[h];
+      }
+    }
+    __syncwarp();
+    const char* v = stage + kWarpRows * kPitch + lane * V * 4;
+#pragma unroll 4
+    for (int t = 0; t < kWarpRows; t++) {
+      float x[V];
+#pragma unroll
+      for (int i = 0; i < V; i += 2) *reinterpret_cast<float2*>(x + i) = *reinterpret_cast<const float2*>(v + t * kPitch + i * 4);
+#pragma unroll
+      for (int h = 0; h < H; h++) {
+        const float w = probabilities[t * H + h];
+#pragma unroll
+        for (int i = 0; i < V; i++) o[h][i] = fmaf(w, x[i], o[h][i]);
+      }
+    }
+    __syncwarp();
+  }
+
+  __device__ __forceinline__ void statistics(float* stat) {
+    const int lane = threadIdx.x % 32;
+#pragma unroll
+    for (int h = 0; h < H; h++) {
+#pragma unroll
+      for (int d = 1; d < 32; d *= 2) l[h] += __shfl_xor_sync(~0u, l[h], d);
+      if (lane == 0) {
+        stat[2 * h] = m[h];
+        stat[2 * h + 1] = l[h];
+      }
+    }
+  }
+  __device__ __forceinline__ void add_values(float* values, int pitch, const float* factor, bool first) const {
+    const int lane = threadIdx.x % 32;
+#pragma unroll
+    for (int h = 0; h < H; h++)
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        float* to = values + h * pitch + lane * V + i;
+        const float x = o[h][i] * factor[h];
+        *to = first ? x : *to + x;
+      }
+  }
+};
+
+// ---- the kernel ----------------------------------------------------------------------------------------------------
+
+template <typename W, int D>
+struct JoinSpace {  // at the end of a segment
+  static constexpr int H = W::kHeads;
+  float values[H * (D + 4)];
+  float stat[kWarps][H][2];
+  float factor[kWarps][H];
+  float total[H], top[H];
+  float reduce[kThreads];
+  long long scratch[kWarps + 2];
+  unsigned mask[kWarps][8];
+  int last;
+};
+
+template <typename T> __device__ __forceinline__ void store4(T* to, float4 x);
+template <> __device__ __forceinline__ void store4(float* to, float4 x) { *reinterpret_cast<float4*>(to) = x; }
+template <> __device__ __forceinline__ void store4(__half* to, float4 x) {
+  *reinterpret_cast<uint2*>(to) = make_uint2(Mma16<__half>::pack(x.x, x.y), Mma16<__half>::pack(x.z, x.w));
+}
+template <> __device__ __forceinline__ void store4(__nv_bfloat16* to, float4 x) {
+  *reinterpret_cast<uint2*>(to) = make_uint2(Mma16<__nv_bfloat16>::pack(x.x, x.y), Mma16<__nv_bfloat16>::pack(x.z, x.w));
+}
+
+__device__ __forceinline__ void store_lse(const AttendArgs& p, int b, int h, float top, float total) {
+  const long long at = (long long)b * p.a.heads + h;
+  const float lse2 = total == 0.f ? -INFINITY : top + log2f(total);
+  p.space.lse2[at] = lse2;
+  if (p.a.lse) p.a.lse[at] = lse2 * kLn2;
+}
+
+template <typename T, typename W, int D, int STAGES, int PER_SM>
+__global__ void __launch_bounds__(kThreads, PER_SM) paged_attend_kernel(const __grid_constant__ AttendArgs p) {
+  using Stage = RowStage<T, D>;
+  using Join = JoinSpace<W, D>;
+  constexpr int H = W::kHeads, kPitch = D + 4;
+  extern __shared__ __align__(16) char smem[];
+  Join& join = *reinterpret_cast<Join*>(smem + kWarps * STAGES * Stage::kBytes + W::kSharedBytes);
+  char* shared = smem + kWarps * STAGES * Stage::kBytes;
+  PJRTX_PDL_PROLOGUE();
+  const int warp = threadIdx.x / 32;
+  char* stages = smem + warp * STAGES * Stage::kBytes;
+  for (int b = blockIdx.x; b < p.c.batch; b += gridDim.x) {  // idle sequences
+    if (threadIdx.x == 0) paged_check_length(p.c, b);
+    if (paged_length(p.c, b) > 0) continue;
+    T* out = static_cast<T*>(p.a.out) + b * p.a.out_batch_stride;
+    for (int i = threadIdx.x; i < p.a.heads * p.c.head_dim; i += kThreads)
+      out[i / p.c.head_dim * p.a.out_head_stride + i % p.c.head_dim] = from_float<T>(0.f);
+    for (int h = threadIdx.x; h < p.a.heads; h += kThreads) store_lse(p, b, h, 0.f, 0.f);
+  }
+  const Share share = share_of_block(p, join.scratch);
+  const int units = (int)(share.end - share.begin);
+  if (units <= 0) return;
+  const float scale2 = p.a.scale * kLog2e;
+
+  Cursor ahead = share.at, now = share.at;
+  {
+    RowPlace place[STAGES];
+    Cursor at[STAGES];
+#pragma unroll
+    for (int s = 0; s < STAGES; s++)
+      if (s < units) {
+        place[s] = locate(p, ahead);
+        at[s] = ahead;
+        if (s + 1 < units) advance(p, ahead);
+      }
+#pragma unroll
+    for (int s = 0; s < STAGES; s++) {
+      if (s < units) request<T, D>(p, at[s], place[s], stages + s * Stage::kBytes, &join.mask[warp][s]);
+      copies_commit();
+    }
+  }
+  RowPlace next = {-1, 0};
+  if (STAGES < units) next = locate(p, ahead);
+
+  W work;
+  work.start(p, now, shared);
+  long long segment = share.begin - now.tile;  // number of the segment's first unit
+  for (int i = 0, stage = 0; i < units; i++) {
+    copies_wait<STAGES - 1>();
+    __syncwarp();
+    work.step(p, now, stages + stage * Stage::kBytes, join.mask[warp][stage], scale2);
+    __syncwarp();
+    if (i + STAGES < units) {
+      request<T, D>(p, ahead, next, stages + stage * Stage::kBytes, &join.mask[warp][stage]);
+      if (i + STAGES + 1 < units) {
+        advance(p, ahead);
+        next = locate(p, ahead);
+      }
+    }
+    copies_commit();
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+    if (now.tile + 1 < now.tiles && i + 1 < units) {
+      now.tile++;
+      continue;
+    }
+
+    // The segment's part of this block is complete: join the warps.
+    work.statistics(&join.stat[warp][0][0]);
+    __syncthreads();
+    if (threadIdx.x < H) {
+      float top = -INFINITY, total = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; w++) top = max_nan(top, join.stat[w][threadIdx.x][0]);
+#pragma unroll
+      for (int w = 0; w < kWarps; w++) {
+        const float m = join.stat[w][threadIdx.x][0], f = m == -INFINITY ? 0.f : exp2_fast(m - top);
+        join.factor[w][threadIdx.x] = f;
+        total += f * join.stat[w][threadIdx.x][1];
+      }
+      join.top[threadIdx.x] = top;
+      join.total[threadIdx.x] = total;
+    }
+    __syncthreads();
+    for (int w = 0; w < kWarps; w++) {
+      if (w == warp) work.add_values(join.values, kPitch, join.factor[w], w == 0);
+      __syncthreads();
+    }
+    const int g = now.group / p.groups, h0 = (now.group % p.groups) * H;
+    const int heads = min(H, p.rep - h0);
+    const long long first = segment / share.quota, last = (segment + now.tiles - 1) / share.quota;
+    bool finish = true;
+    if (first != last) {
+      // Slot 1 holds a segment that begins with this block, slot 0 one that began before it.
+      constexpr int kSlot = H * (D + 2);
+      auto slot = [&](long long block) { return p.space.partials + (block * 2 + (segment >= block * share.quota ? 1 : 0)) * kSlot; };
+      float* mine = slot(blockIdx.x);
+      for (int j = threadIdx.x; j < heads * (D / 4); j += kThreads)
+        *reinterpret_cast<float4*>(mine + j * 4) = *reinterpret_cast<const float4*>(join.values + j / (D / 4) * kPitch + j % (D / 4) * 4);
+      if ((int)threadIdx.x < heads) {
+        mine[H * D + threadIdx.x] = join.top[threadIdx.x];
+        mine[H * D + H + threadIdx.x] = join.total[threadIdx.x];
+      }
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        const unsigned others = (unsigned)(last - first);
+        join.last = atomicInc(p.space.counters + (long long)now.b * p.c.kv_heads * p.groups + now.group, others) == others;
+      }
+      __syncthreads();
+      finish = join.last;
+      if (finish) {
+        __threadfence();
+        // Maxima and sums of all blocks, kThreads / H of them side by side.
+        constexpr int kBeside = kThreads / H;
+        const int h = threadIdx.x % H, part = threadIdx.x / H;
+        float top = -INFINITY;
+        if (h < heads)
+          for (long long block = first + part; block <= last; block += kBeside) top = max_nan(top, __ldcg(slot(block) + H * D + h));
+        join.reduce[threadIdx.x] = top;
+        __syncthreads();
+        for (int k = 0; k < kBeside; k++) top = max_nan(top, join.reduce[k * H + h]);
+        __syncthreads();
+        float total = 0.f;
+        if (h < heads)
+          for (long long block = first + part; block <= last; block += kBeside) {
+            const float m = __ldcg(slot(block) + H * D + h);
+            total += m == -INFINITY ? 0.f : exp2_fast(m - top) * __ldcg(slot(block) + H * D + H + h);
+          }
+        join.reduce[threadIdx.x] = total;
+        __syncthreads();
+        if (part == 0) {
+          total = 0.f;
+          for (int k = 0; k < kBeside; k++) total += join.reduce[k * H + h];
+          join.top[h] = top;
+          join.total[h] = total;
+        }
+        __syncthreads();
+        for (int j = threadIdx.x; j < heads * (D / 4); j += kThreads) {
+          const int hh = j / (D / 4), at = j * 4;
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (long long block = first; block <= last; block++) {
+            const float* from = slot(block);
+            const float m = __ldcg(from + H * D + hh), f = m == -INFINITY ? 0.f : exp2_fast(m - join.top[hh]);
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(from + at));
+            x.x = fmaf(f, y.x, x.x);
+            x.y = fmaf(f, y.y, x.y);
+            x.z = fmaf(f, y.z, x.z);
+            x.w = fmaf(f, y.w, x.w);
+          }
+          *reinterpret_cast<float4*>(join.values + hh * kPitch + j % (D / 4) * 4) = x;
+        }
+        __syncthreads();
+      }
+    }
+    if (finish) {
+      T* out = static_cast<T*>(p.a.out) + now.b * p.a.out_batch_stride + (long long)(g * p.rep + h0) * p.a.out_head_stride;
+      for (int j = threadIdx.x; j < heads * (D / 4); j += kThreads) {
+        const int hh = j / (D / 4), d = j % (D / 4) * 4;
+        if (d >= p.c.head_dim) continue;
+        const float total = join.total[hh], inverse = total == 0.f ? 0.f : 1.f / total;
+        float4 x = *reinterpret_cast<const float4*>(join.values + hh * kPitch + d);
+        x.x *= inverse; x.y *= inverse; x.z *= inverse; x.w *= inverse;
+        store4(out + hh * p.a.out_head_stride + d, x);
+      }
+      if ((int)threadIdx.x < heads) store_lse(p, now.b, g * p.rep + h0 + threadIdx.x, join.top[threadIdx.x], join.total[threadIdx.x]);
+    }
+    if (i + 1 < units) {
+      segment += now.tiles;
+      advance(p, now);
+      __syncthreads();  // `join` is used again
+      work.start(p, now, shared);
+    }
   }
 }
 
@@ -141,29 +784,94 @@ __global__ void __launch_bounds__(kTrackThreads) paged_track_kernel(PagedView c,
   }
 }
 
-template <typename T>
-bool attend(const PagedView& c, const PagedAttend& a, const AttendSpace& space, bool pdl, cudaStream_t stream) {
-  return launch_kernel(paged_attend_kernel<T>, dim3((unsigned)a.heads, (unsigned)c.batch), dim3(kSimpleWarps * 32), 0, stream, pdl, c, a,
-                       space) == cudaSuccess;
+// Which kernel a shape runs on.
+struct AttendPlan {
+  int dims = 0;    // dimensions a row is padded to
+  int heads = 0;   // query heads of a group
+  int stages = 0, per_sm = 0;
+  size_t smem = 0;
+};
+
+template <typename T, typename W, int D, int STAGES>
+constexpr size_t attend_smem() {
+  return (size_t)kWarps * STAGES * RowStage<T, D>::kBytes + W::kSharedBytes + sizeof(JoinSpace<W, D>);
+}
+
+template <typename F>
+auto with_kernel(int dtype, int head_dim, int rep, F&& f) {
+#define PJRTX_ATTEND(T, W, D, S, N) return f(paged_attend_kernel<T, W, D, S, N>, AttendPlan{D, W::kHeads, S, N, attend_smem<T, W, D, S>()})
+#define PJRTX_ATTEND_MMA(T, NB)                                                 \
+  if (head_dim <= 64) { using W = MmaWarp<T, 64, NB>; PJRTX_ATTEND(T, W, 64, 5, 2); }  \
+  if (head_dim <= 128) { using W = MmaWarp<T, 128, NB>; PJRTX_ATTEND(T, W, 128, 3, 2); } \
+  { using W = MmaWarp<T, 256, 1>; PJRTX_ATTEND(T, W, 256, 3, 1); }
+#define PJRTX_ATTEND_FMA(H)                                                     \
+  if (head_dim <= 64) { using W = FmaWarp<64, H>; PJRTX_ATTEND(float, W, 64, 3, 2); }  \
+  if (head_dim <= 128) { using W = FmaWarp<128, H>; PJRTX_ATTEND(float, W, 128, 3, 1); } \
+  { using W = FmaWarp<256, H>; PJRTX_ATTEND(float, W, 256, 1, 1); }
+  if (dtype == kF32) {
+    if (rep <= 4) { PJRTX_ATTEND_FMA(4) }
+    PJRTX_ATTEND_FMA(8)
+  }
+  if (dtype == kF16) {
+    if (rep <= 8) { PJRTX_ATTEND_MMA(__half, 1) }
+    PJRTX_ATTEND_MMA(__half, 2)
+  }
+  if (rep <= 8) { PJRTX_ATTEND_MMA(__nv_bfloat16, 1) }
+  PJRTX_ATTEND_MMA(__nv_bfloat16, 2)
+#undef PJRTX_ATTEND_FMA
+#undef PJRTX_ATTEND_MMA
+#undef PJRTX_ATTEND
+}
+
+uint64_t round256(uint64_t n) { return (n + 255) / 256 * 256; }
+
+struct AttendLayout {
+  uint64_t counters, partials, scores, bytes;
+};
+
+// Places go by the largest batch, so that the counters stay where they are.
+AttendLayout attend_layout(const PagedView& c, int heads, const AttendPlan& plan, bool track, int sm_count) {
+  const int rep = heads / c.kv_heads, groups = (rep + plan.heads - 1) / plan.heads;
+  AttendLayout l;
+  l.counters = round256((uint64_t)c.batch_max * heads * 4);
+  l.partials = l.counters + round256((uint64_t)c.batch_max * c.kv_heads * groups * 4);
+  l.scores = l.partials + round256((uint64_t)sm_count * plan.per_sm * 2 * plan.heads * (plan.dims + 2) * 4);
+  l.bytes = l.scores + (track ? (uint64_t)c.batch_max * heads * c.capacity() * 4 : 0);
+  return l;
 }
 
 }  // namespace
 
 uint64_t paged_attend_workspace_bytes(const PagedView& c, int heads, bool track, int sm_count) {
-  (void)sm_count;
-  return ((uint64_t)c.batch_max * heads * 4 + 255) / 256 * 256 + (track ? (uint64_t)c.batch_max * heads * c.capacity() * 4 : 0);
+  return with_kernel(c.dtype, c.head_dim, heads / c.kv_heads,
+                     [&](auto, const AttendPlan& plan) { return attend_layout(c, heads, plan, track, sm_count).bytes; });
 }
 
 int paged_attend_launch(const PagedView& c, const PagedAttend& a, int sm_count, bool pdl, cudaStream_t stream) {
-  const AttendSpace space = attend_space(c, a.heads, a.workspace);
-  const bool ok = c.dtype == kF32 ? attend<float>(c, a, space, pdl, stream) : c.dtype == kF16 ? attend<__half>(c, a, space, pdl, stream)
-                                                                                             : attend<__nv_bfloat16>(c, a, space, pdl, stream);
+  AttendArgs p;
+  p.c = c;
+  p.a = a;
+  p.rep = a.heads / c.kv_heads;
+  p.pieces = c.head_dim * (int)dtype_size(c.dtype) / 16;
+  const bool ok = with_kernel(c.dtype, c.head_dim, p.rep, [&](auto kernel, const AttendPlan& plan) {
+    const AttendLayout l = attend_layout(c, a.heads, plan, false, sm_count);
+    char* space = static_cast<char*>(a.workspace);
+    p.groups = (p.rep + plan.heads - 1) / plan.heads;
+    p.space.lse2 = reinterpret_cast<float*>(space);
+    p.space.counters = reinterpret_cast<unsigned*>(space + l.counters);
+    p.space.partials = reinterpret_cast<float*>(space + l.partials);
+    p.space.scores = reinterpret_cast<float*>(space + l.scores);
+    if (!raise_smem_limit((const void*)kernel, (int)plan.smem)) return false;
+    const long long units = (long long)c.batch * c.kv_heads * p.groups * ((c.capacity() + kTileRows - 1) / kTileRows);
+    const long long blocks = std::min<long long>(units, (long long)sm_count * plan.per_sm);
+    return launch_kernel(kernel, dim3((unsigned)blocks), dim3(kThreads), plan.smem, stream, pdl, p) == cudaSuccess;
+  });
   if (!ok) return 0;
   if (!c.weights) return 1;
   const long long pairs = (long long)c.batch * c.kv_heads;
   const long long blocks = std::max<long long>(1, std::min((c.capacity() + kTrackThreads - 1) / kTrackThreads, 8ll * sm_count / pairs + 1));
   return launch_kernel(paged_track_kernel, dim3((unsigned)blocks, (unsigned)c.kv_heads, (unsigned)c.batch), dim3(kTrackThreads), 0, stream, true,
-                       c, space, a.heads, a.k_new != nullptr) == cudaSuccess ? 2 : 0;
+                       c, p.space, a.heads, (int)(a.k_new != nullptr)) == cudaSuccess ? 2 : 0;
 }
 
 }  // namespace pjrtx
