@@ -29,13 +29,14 @@ inline bool raise_smem_limit(const void* kernel, int bytes) {
 // Makes `device` current for the lifetime of the object and restores the caller's device afterwards.
 struct CurrentDevice {
   int previous = -1;
-  bool ok = false;
+  bool changed = false, ok = false;
   explicit CurrentDevice(int device) {
     if (cudaGetDevice(&previous) != cudaSuccess) previous = -1;
-    ok = cudaSetDevice(device) == cudaSuccess;
+    changed = previous != device;
+    ok = !changed || cudaSetDevice(device) == cudaSuccess;
   }
   ~CurrentDevice() {
-    if (previous >= 0) cudaSetDevice(previous);
+    if (changed && previous >= 0) cudaSetDevice(previous);
   }
 };
 

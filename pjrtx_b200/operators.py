@@ -9,8 +9,10 @@ default stream); None is the stream on which the backend's buffers and executabl
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
-from typing import Optional, Sequence, Tuple
+import struct
+from typing import Optional, Tuple
 
 from . import plan as P
 
@@ -57,21 +59,35 @@ class TokenLogProbsBackwardArgs(ctypes.Structure):
 
 
 # Every symbol of the operator section of include/pjrtx_b200.h: name -> (restype, argtypes).
-_CACHE_CALL = [_P, ctypes.POINTER(PagedView)]
+# Argument structs go in as bytes or by reference.
 SYMBOLS = {
     "pjrtx_b200_device_stream": (_P, [ctypes.c_int]),
     "pjrtx_b200_buffer_device_pointer": (_P, [_P]),
     "pjrtx_b200_paged_cache_create": (_P, [ctypes.c_int, ctypes.POINTER(PagedCacheConfig)]),
     "pjrtx_b200_paged_cache_destroy": (None, [_P]),
-    "pjrtx_b200_paged_cache_append": (ctypes.c_int, _CACHE_CALL + [ctypes.POINTER(PagedAppendArgs), _P]),
-    "pjrtx_b200_paged_cache_attend": (ctypes.c_int, _CACHE_CALL + [ctypes.POINTER(PagedAttendArgs), _P]),
-    "pjrtx_b200_paged_cache_evict": (ctypes.c_int, _CACHE_CALL + [ctypes.POINTER(PagedEvictArgs), _P]),
-    "pjrtx_b200_token_log_probs": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(TokenLogProbsArgs), _P]),
-    "pjrtx_b200_token_log_probs_backward": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(TokenLogProbsBackwardArgs), _P]),
+    "pjrtx_b200_paged_cache_append": (ctypes.c_int, [_P, _P, _P, _P]),
+    "pjrtx_b200_paged_cache_attend": (ctypes.c_int, [_P, _P, _P, _P]),
+    "pjrtx_b200_paged_cache_evict": (ctypes.c_int, [_P, _P, _P, _P]),
+    "pjrtx_b200_token_log_probs": (ctypes.c_int, [ctypes.c_int, _P, _P]),
+    "pjrtx_b200_token_log_probs_backward": (ctypes.c_int, [ctypes.c_int, _P, _P]),
 }
 
+# Argument structs are packed in one step: filling a ctypes structure field by field takes twice as long as the call itself.
+_FORMAT = {_U64: "Q", _I64: "q", _I32: "i", _F32: "f", _P: "P"}
+
+
+def _packer(cls):
+    """pack(*fields behind struct_size) -> the struct as bytes."""
+    layout = struct.Struct("@" + "".join(_FORMAT[t] for _, t in cls._fields_) + "0Q")
+    assert layout.size == ctypes.sizeof(cls)
+    return functools.partial(layout.pack, layout.size)
+
+
+_pack_view, _pack_append, _pack_attend, _pack_evict, _pack_score, _pack_score_grad = map(
+    _packer, (PagedView, PagedAppendArgs, PagedAttendArgs, PagedEvictArgs, TokenLogProbsArgs, TokenLogProbsBackwardArgs))
+
 _TENSOR_TYPES = {"float32": P.F32, "float16": P.F16, "bfloat16": P.BF16_CODE, "int32": P.S32}
-_codes: dict = {}  # a tensor library's dtype object -> element-type code
+_codes: dict = {}  # a tensor library's dtype object -> element-type code, 0 for the others
 
 
 def _error(message: str):
@@ -80,51 +96,76 @@ def _error(message: str):
     return BackendError("InvalidArgument", message)
 
 
-def _code(dtype) -> Optional[int]:
+def _dims(x) -> Tuple[int, ...]:
+    try:
+        return x.shape
+    except AttributeError:
+        return x.dims
+
+
+def _code(x) -> int:
+    dtype = x.dtype
+    if isinstance(dtype, int):
+        return dtype
     code = _codes.get(dtype)
     if code is None:
-        code = _TENSOR_TYPES.get(str(dtype).split(".")[-1])
-        if code is not None:
-            _codes[dtype] = code
+        code = _codes[dtype] = _TENSOR_TYPES.get(str(dtype).split(".")[-1], 0)
     return code
 
 
-def _array(x, name: str, dtype: int, shape: Sequence[int]) -> Tuple[Optional[int], Tuple[int, ...]]:
-    """Device address and strides (elements) of an array that must have this type and shape (-1: any extent)."""
-    if hasattr(x, "data_ptr"):
-        code, dims, strides, pointer = _code(x.dtype), x.shape, x.stride(), x.data_ptr()
-    else:
-        code, dims, strides, pointer = x.dtype, x.dims, None, x.device_pointer
-    if code != dtype:
-        raise _error(f"{name} has element type {P.DTYPE_NAMES.get(code, 'other')}, {P.DTYPE_NAMES.get(dtype, dtype)} is needed")
-    if tuple(dims) != shape and (len(dims) != len(shape) or any(want not in (-1, have) for have, want in zip(dims, shape))):
-        raise _error(f"{name} has shape {tuple(dims)}, {tuple(shape)} is needed")
-    if strides is None:
+def _place(x):
+    """Device address and strides (elements)."""
+    try:
+        return x.data_ptr(), x.stride()
+    except AttributeError:
         strides, step = [], 1
-        for d in reversed(dims):
+        for d in reversed(x.dims):
             strides.insert(0, step)
             step *= d
-    return pointer, strides
+        return x.device_pointer or 0, tuple(strides)
 
 
-def _rows(x, name: str, dtype: int, shape: Sequence[int]):
-    """The same for an array whose innermost axis has to be dense."""
-    pointer, strides = _array(x, name, dtype, shape)
-    if strides[-1] != 1 and shape[-1] != 1:
-        raise _error(f"{name} has stride {strides[-1]} along its last axis, which has to be dense")
-    return pointer, strides
+def _check(x, name: str, dtype: int, shape: Tuple[int, ...]) -> None:
+    if _code(x) != dtype:
+        raise _error(f"{name} has element type {P.DTYPE_NAMES.get(_code(x), 'other')}, {P.DTYPE_NAMES.get(dtype, dtype)} is needed")
+    if _dims(x) != shape:
+        raise _error(f"{name} has shape {tuple(_dims(x))}, {shape} is needed")
 
 
-def _dense(x, name: str, dtype: int, shape: Sequence[int]):
-    """Address of an array that has to be dense; None stays None."""
+def _rows(x, name: str, dtype: int, shape: Tuple[int, ...]):
+    """Address and strides of an array whose innermost axis has to be dense."""
+    _check(x, name, dtype, shape)
+    place = _place(x)
+    if place[1][-1] != 1 and shape[-1] != 1:
+        raise _error(f"{name} has stride {place[1][-1]} along its last axis, which has to be dense")
+    return place
+
+
+def _twin(x, name: str, like, like_name: str, strides) -> int:
+    """Address of an array that has the type, shape and strides of `like`."""
+    if _code(x) != _code(like) or _dims(x) != _dims(like):
+        raise _error(f"{like_name} and {name} differ in type or shape")
+    pointer, own = _place(x)
+    if own != strides:
+        raise _error(f"{like_name} and {name} differ in their strides")
+    return pointer
+
+
+def _dense(x, name: str, dtype: int, shape: Tuple[int, ...]) -> int:
+    """Address of an array that has to be dense; None is 0."""
     if x is None:
-        return None
-    pointer, strides = _array(x, name, dtype, shape)
-    step = 1
-    for d, s in zip(reversed(shape), reversed(strides)):
-        if s != step and d != 1:
-            raise _error(f"{name} has to be dense, its strides are {tuple(strides)}")
-        step *= d
+        return 0
+    _check(x, name, dtype, shape)
+    try:
+        dense, pointer = x.is_contiguous(), x.data_ptr()
+    except AttributeError:
+        pointer, strides = _place(x)
+        step, dense = 1, True
+        for d, s in zip(reversed(shape), reversed(strides)):
+            dense = dense and (s == step or d == 1)
+            step *= d
+    if not dense:
+        raise _error(f"{name} has to be dense")
     return pointer
 
 
@@ -148,41 +189,42 @@ class PagedCache:
         if not self.handle:
             raise _error(self._err())
         self._stream = self._lib.pjrtx_b200_device_stream(device)
+        self._page_dims = (page_size, kv_heads, head_dim)
 
-    def _view(self, k_pages, v_pages, page_table, lengths, tokens=None, weights=None, positions=None) -> PagedView:
-        dims = (-1, self.page_size, self.kv_heads, self.head_dim)
+    def _view(self, k_pages, v_pages, page_table, lengths, tokens, weights, positions) -> Tuple[int, bytes]:
+        """The batch and the packed view."""
+        dims, batch_dims = tuple(_dims(k_pages)), _dims(lengths)
+        if len(dims) != 4 or dims[1:] != self._page_dims:
+            raise _error(f"k_pages has shape {dims}, (pages, {', '.join(map(str, self._page_dims))}) is needed")
+        if len(batch_dims) != 1:
+            raise _error(f"lengths has shape {tuple(batch_dims)}, (batch,) is needed")
         k, strides = _rows(k_pages, "k_pages", self.dtype, dims)
-        v, v_strides = _rows(v_pages, "v_pages", self.dtype, dims)
-        shape = k_pages.shape if hasattr(k_pages, "shape") else k_pages.dims
-        v_shape = v_pages.shape if hasattr(v_pages, "shape") else v_pages.dims
-        if shape[0] != v_shape[0] or tuple(strides) != tuple(v_strides):
-            raise _error("k_pages and v_pages differ in their number of pages or in their strides")
-        batch = (lengths.shape if hasattr(lengths, "shape") else lengths.dims)[0]
+        v = _twin(v_pages, "v_pages", k_pages, "k_pages", strides)
+        batch = batch_dims[0]
         table, table_strides = _rows(page_table, "page_table", P.S32, (batch, self.max_pages))
         tracked = (batch, self.kv_heads, self.capacity)
-        return PagedView(ctypes.sizeof(PagedView), k, v, shape[0], strides[0], strides[1], strides[2], table, table_strides[0],
-                         _dense(lengths, "lengths", P.S32, (batch,)), batch, _dense(tokens, "tokens", P.S32, (batch,)),
-                         _dense(weights, "weights", P.F32, tracked), _dense(positions, "positions", P.S32, tracked))
+        return batch, _pack_view(k, v, dims[0], strides[0], strides[1], strides[2], table, table_strides[0],
+                                 _dense(lengths, "lengths", P.S32, (batch,)), batch, _dense(tokens, "tokens", P.S32, (batch,)),
+                                 _dense(weights, "weights", P.F32, tracked), _dense(positions, "positions", P.S32, tracked))
 
     def _call(self, fn, view, args, stream) -> None:
         if not self.handle:
             raise _error("the paged cache was destroyed")
-        if not fn(self.handle, ctypes.byref(view), ctypes.byref(args), self._stream if stream is None else stream):
+        if not fn(self.handle, view, args, self._stream if stream is None else stream):
             raise _error(self._err())
 
     def append(self, k_pages, v_pages, page_table, lengths, k_new, v_new, counts=None, tokens=None, weights=None, positions=None,
                stream: Optional[int] = None) -> None:
         """Stores the first counts[b] of the rows k_new / v_new [batch, rows, kv_heads, head_dim] (None: all of them) as the
         last ones of the lengths[b] rows of each sequence; with tracking their weights become 0."""
-        view = self._view(k_pages, v_pages, page_table, lengths, tokens, weights, positions)
-        shape = (view.batch, -1, self.kv_heads, self.head_dim)
+        batch, view = self._view(k_pages, v_pages, page_table, lengths, tokens, weights, positions)
+        dims = _dims(k_new)
+        if len(dims) != 4:
+            raise _error(f"k_new has shape {tuple(dims)}, (batch, rows, KV heads, head dimension) is needed")
+        shape = (batch, dims[1], self.kv_heads, self.head_dim)
         k, strides = _rows(k_new, "k_new", self.dtype, shape)
-        v, v_strides = _rows(v_new, "v_new", self.dtype, shape)
-        rows, v_rows = ((x.shape if hasattr(x, "shape") else x.dims)[1] for x in (k_new, v_new))
-        if rows != v_rows or tuple(strides) != tuple(v_strides):
-            raise _error("k_new and v_new differ in their number of rows or in their strides")
-        args = PagedAppendArgs(ctypes.sizeof(PagedAppendArgs), k, v, rows, strides[0], strides[1], strides[2],
-                               _dense(counts, "counts", P.S32, (view.batch,)))
+        v = _twin(v_new, "v_new", k_new, "k_new", strides)
+        args = _pack_append(k, v, shape[1], strides[0], strides[1], strides[2], _dense(counts, "counts", P.S32, (batch,)))
         self._call(self._lib.pjrtx_b200_paged_cache_append, view, args, stream)
 
     def attend(self, q, k_pages, v_pages, page_table, lengths, out, lse=None, k_new=None, v_new=None, tokens=None, weights=None,
@@ -190,34 +232,32 @@ class PagedCache:
         """out [batch, heads, head_dim] = softmax(scale * q . k) v over each sequence's rows (`scale` None: 1 / sqrt(head_dim)),
         lse [batch, heads] its log-sum-exp. k_new / v_new [batch, kv_heads, head_dim] become row lengths[b] - 1 first. With
         tracking, weights[b, g, t] grows by what the query heads of KV head g give row t."""
-        view = self._view(k_pages, v_pages, page_table, lengths, tokens, weights, positions)
-        batch, shape = view.batch, (view.batch, self.heads, self.head_dim)
+        batch, view = self._view(k_pages, v_pages, page_table, lengths, tokens, weights, positions)
+        shape = (batch, self.heads, self.head_dim)
         q_at, q_strides = _rows(q, "q", self.dtype, shape)
         out_at, out_strides = _rows(out, "out", self.dtype, shape)
-        k = v = None
+        k = v = 0
         new_strides = (0, 0)
         if k_new is not None and v_new is not None:
-            k, new_strides = _rows(k_new, "k_new", self.dtype, (batch, self.kv_heads, self.head_dim))
-            v, v_strides = _rows(v_new, "v_new", self.dtype, (batch, self.kv_heads, self.head_dim))
-            if tuple(new_strides) != tuple(v_strides):
-                raise _error("k_new and v_new differ in their strides")
+            shape = (batch, self.kv_heads, self.head_dim)
+            k, new_strides = _rows(k_new, "k_new", self.dtype, shape)
+            v = _twin(v_new, "v_new", k_new, "k_new", new_strides)
         elif k_new is not None or v_new is not None:
             raise _error("a new key and a new value go together")
-        args = PagedAttendArgs(ctypes.sizeof(PagedAttendArgs), q_at, q_strides[0], q_strides[1], out_at, out_strides[0], out_strides[1],
-                               _dense(lse, "lse", P.F32, (batch, self.heads)), k, v, new_strides[0], new_strides[1],
-                               1.0 / math.sqrt(self.head_dim) if scale is None else scale)
+        args = _pack_attend(q_at, q_strides[0], q_strides[1], out_at, out_strides[0], out_strides[1],
+                            _dense(lse, "lse", P.F32, (batch, self.heads)), k, v, new_strides[0], new_strides[1],
+                            self.head_dim ** -0.5 if scale is None else scale)
         self._call(self._lib.pjrtx_b200_paged_cache_attend, view, args, stream)
 
     def evict(self, k_pages, v_pages, page_table, lengths, tokens, weights, positions, keep: int, recent: int = 0, sinks: int = 0,
               lengths_out=None, weights_out=None, positions_out=None, stream: Optional[int] = None) -> None:
         """Cuts every sequence to `keep` rows by weight; tokens before `sinks` and the last `recent` ones stay. Results go to the
         `*_out` arrays, None: in place. Pages must not be shared between sequences."""
-        view = self._view(k_pages, v_pages, page_table, lengths, tokens, weights, positions)
-        tracked = (view.batch, self.kv_heads, self.capacity)
-        args = PagedEvictArgs(ctypes.sizeof(PagedEvictArgs), keep, recent, sinks,
-                              _dense(lengths if lengths_out is None else lengths_out, "lengths_out", P.S32, (view.batch,)),
-                              _dense(weights if weights_out is None else weights_out, "weights_out", P.F32, tracked),
-                              _dense(positions if positions_out is None else positions_out, "positions_out", P.S32, tracked))
+        batch, view = self._view(k_pages, v_pages, page_table, lengths, tokens, weights, positions)
+        tracked = (batch, self.kv_heads, self.capacity)
+        args = _pack_evict(keep, recent, sinks, _dense(lengths if lengths_out is None else lengths_out, "lengths_out", P.S32, (batch,)),
+                           _dense(weights if weights_out is None else weights_out, "weights_out", P.F32, tracked),
+                           _dense(positions if positions_out is None else positions_out, "positions_out", P.S32, tracked))
         self._call(self._lib.pjrtx_b200_paged_cache_evict, view, args, stream)
 
     def destroy(self) -> None:
@@ -232,43 +272,38 @@ class PagedCache:
             pass
 
 
-def _logits(x, name: str):
-    dims = x.shape if hasattr(x, "data_ptr") else x.dims
+def _logits(x):
+    """Element type, rows, vocabulary, address and row stride."""
+    dims, code = _dims(x), _code(x)
     if len(dims) != 2:
-        raise _error(f"{name} has shape {tuple(dims)}, (rows, vocabulary) is needed")
-    code = _code(x.dtype) if hasattr(x, "data_ptr") else x.dtype
+        raise _error(f"logits has shape {tuple(dims)}, (rows, vocabulary) is needed")
     if code not in (P.F32, P.F16, P.BF16_CODE):
-        raise _error(f"{name} has element type {P.DTYPE_NAMES.get(code, 'other')}; f32, f16 and bf16 are supported")
-    pointer, strides = _rows(x, name, code, dims)
+        raise _error(f"logits has element type {P.DTYPE_NAMES.get(code, 'other')}; f32, f16 and bf16 are supported")
+    pointer, strides = _rows(x, "logits", code, dims)
     return code, dims[0], dims[1], pointer, strides[0]
 
 
 def token_log_probs(backend, logits, tokens, log_probs, entropy=None, lse=None, top_ids=None, top_log_probs=None, scale: float = 1.0,
                     stream: Optional[int] = None, device: int = 0) -> None:
-    dtype, rows, vocab, at, stride = _logits(logits, "logits")
-    top = 0
-    for x in (top_ids, top_log_probs):
-        if x is not None:
-            top = (x.shape if hasattr(x, "shape") else x.dims)[-1]
-    args = TokenLogProbsArgs(ctypes.sizeof(TokenLogProbsArgs), dtype, top, at, rows, vocab, stride, _dense(tokens, "tokens", P.S32, (rows,)), scale,
-                             _dense(log_probs, "log_probs", P.F32, (rows,)), _dense(entropy, "entropy", P.F32, (rows,)),
-                             _dense(lse, "lse", P.F32, (rows,)), _dense(top_ids, "top_ids", P.S32, (rows, top)),
-                             _dense(top_log_probs, "top_log_probs", P.F32, (rows, top)))
-    if not backend.lib.pjrtx_b200_token_log_probs(device, ctypes.byref(args), _stream_of(backend, device, stream)):
+    dtype, rows, vocab, at, stride = _logits(logits)
+    wide = top_ids if top_ids is not None else top_log_probs
+    top = 0 if wide is None else _dims(wide)[-1]
+    args = _pack_score(dtype, top, at, rows, vocab, stride, _dense(tokens, "tokens", P.S32, (rows,)), scale,
+                       _dense(log_probs, "log_probs", P.F32, (rows,)), _dense(entropy, "entropy", P.F32, (rows,)),
+                       _dense(lse, "lse", P.F32, (rows,)), _dense(top_ids, "top_ids", P.S32, (rows, top)),
+                       _dense(top_log_probs, "top_log_probs", P.F32, (rows, top)))
+    lib = backend.lib
+    if not lib.pjrtx_b200_token_log_probs(device, args, lib.pjrtx_b200_device_stream(device) if stream is None else stream):
         raise _error(backend._err())
 
 
 def token_log_probs_backward(backend, logits, tokens, lse, grad_logits, grad_log_probs=None, entropy=None, grad_entropy=None,
                              scale: float = 1.0, stream: Optional[int] = None, device: int = 0) -> None:
-    dtype, rows, vocab, at, stride = _logits(logits, "logits")
+    dtype, rows, vocab, at, stride = _logits(logits)
     grad_at, grad_strides = _rows(grad_logits, "grad_logits", dtype, (rows, vocab))
-    args = TokenLogProbsBackwardArgs(ctypes.sizeof(TokenLogProbsBackwardArgs), dtype, scale, at, grad_at, rows, vocab, stride, grad_strides[0],
-                                     _dense(tokens, "tokens", P.S32, (rows,)), _dense(lse, "lse", P.F32, (rows,)),
-                                     _dense(entropy, "entropy", P.F32, (rows,)), _dense(grad_log_probs, "grad_log_probs", P.F32, (rows,)),
-                                     _dense(grad_entropy, "grad_entropy", P.F32, (rows,)))
-    if not backend.lib.pjrtx_b200_token_log_probs_backward(device, ctypes.byref(args), _stream_of(backend, device, stream)):
+    args = _pack_score_grad(dtype, scale, at, grad_at, rows, vocab, stride, grad_strides[0], _dense(tokens, "tokens", P.S32, (rows,)),
+                            _dense(lse, "lse", P.F32, (rows,)), _dense(entropy, "entropy", P.F32, (rows,)),
+                            _dense(grad_log_probs, "grad_log_probs", P.F32, (rows,)), _dense(grad_entropy, "grad_entropy", P.F32, (rows,)))
+    lib = backend.lib
+    if not lib.pjrtx_b200_token_log_probs_backward(device, args, lib.pjrtx_b200_device_stream(device) if stream is None else stream):
         raise _error(backend._err())
-
-
-def _stream_of(backend, device: int, stream: Optional[int]):
-    return backend.lib.pjrtx_b200_device_stream(device) if stream is None else stream
