@@ -8,9 +8,10 @@
 // A row is read once: each thread keeps its own running (m, S, T) and rescales only when its maximum grows. The blocks of a
 // cluster share a row where there are too few rows to fill the GPU and join through distributed shared memory.
 //
-// Top k: a chunk is what a warp reads with one 16-byte load a thread, and its maximum goes to shared memory on the way. In the
-// order (value descending, id ascending) the k first elements lie in the k first chunks - an element of another chunk has k
-// elements before it, the maxima of those - so afterwards only these k chunks are read again.
+// Top k is a tournament of intervals. A chunk is 256 consecutive logits, a vector the 16 bytes of one load, and in the order
+// (value descending, id ascending) the k first elements lie in the k intervals that come first by (maximum descending,
+// position ascending): an element of any other interval has k elements before it, the maxima of those. So chunk maxima are left
+// in shared memory on the way, and afterwards the k first chunks are read again, then the k first of their vectors.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -30,6 +31,40 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// Two floats at a time.
+typedef unsigned long long Pair;
+__device__ __forceinline__ Pair pair_of(float a, float b) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 split(Pair p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ Pair pair_fma(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ Pair pair_add(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 template <typename T> struct Logit;
 template <> struct Logit<float> {
   static constexpr int V = 4;
@@ -38,6 +73,19 @@ template <> struct Logit<float> {
   }
   static __device__ __forceinline__ uint4 pack(const float* f) {
     return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+  // The largest element of `count` vectors.
+  template <int N>
+  static __device__ __forceinline__ float highest(const uint4* r) {
+    float m = max_nan(max_nan(__uint_as_float(r[0].x), __uint_as_float(r[0].y)), max_nan(__uint_as_float(r[0].z), __uint_as_float(r[0].w)));
+    if constexpr (N > 1) m = max_nan(m, highest<N - 1>(r + 1));
+    return m;
+  }
+  template <int N>
+  static __device__ __forceinline__ float lowest(const uint4* r) {
+    float m = fminf(fminf(__uint_as_float(r[0].x), __uint_as_float(r[0].y)), fminf(__uint_as_float(r[0].z), __uint_as_float(r[0].w)));
+    if constexpr (N > 1) m = fminf(m, lowest<N - 1>(r + 1));
+    return m;
   }
   static __device__ __forceinline__ float load(const float* p) { return *p; }
   static __device__ __forceinline__ void store(float* p, float v) { *p = v; }
@@ -58,6 +106,24 @@ template <> struct Logit<__nv_bfloat16> {
 #pragma unroll
     for (int i = 0; i < 4; i++) h[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
     return r;
+  }
+  template <int N>
+  static __device__ __forceinline__ __nv_bfloat162 extreme(const uint4* r, bool high) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(r);
+    __nv_bfloat162 m = h[0];
+#pragma unroll
+    for (int i = 1; i < 4 * N; i++) m = high ? __hmax2_nan(m, h[i]) : __hmin2(m, h[i]);
+    return m;
+  }
+  template <int N>
+  static __device__ __forceinline__ float highest(const uint4* r) {
+    const float2 m = __bfloat1622float2(extreme<N>(r, true));
+    return max_nan(m.x, m.y);
+  }
+  template <int N>
+  static __device__ __forceinline__ float lowest(const uint4* r) {
+    const float2 m = __bfloat1622float2(extreme<N>(r, false));
+    return fminf(m.x, m.y);
   }
   static __device__ __forceinline__ float load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
   static __device__ __forceinline__ void store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
@@ -80,20 +146,27 @@ template <> struct Logit<__half> {
     for (int i = 0; i < 4; i++) h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
     return r;
   }
+  template <int N>
+  static __device__ __forceinline__ __half2 extreme(const uint4* r, bool high) {
+    const __half2* h = reinterpret_cast<const __half2*>(r);
+    __half2 m = h[0];
+#pragma unroll
+    for (int i = 1; i < 4 * N; i++) m = high ? __hmax2_nan(m, h[i]) : __hmin2(m, h[i]);
+    return m;
+  }
+  template <int N>
+  static __device__ __forceinline__ float highest(const uint4* r) {
+    const float2 m = __half22float2(extreme<N>(r, true));
+    return max_nan(m.x, m.y);
+  }
+  template <int N>
+  static __device__ __forceinline__ float lowest(const uint4* r) {
+    const float2 m = __half22float2(extreme<N>(r, false));
+    return fminf(m.x, m.y);
+  }
   static __device__ __forceinline__ float load(const __half* p) { return __half2float(*p); }
   static __device__ __forceinline__ void store(__half* p, float v) { *p = __float2half_rn(v); }
 };
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float y;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-  return y;
-}
 
 // A float in the order of unsigned integers: -0 as +0, NaN above all; 0 stands for "no element".
 __device__ __forceinline__ unsigned order_key(float f) {
@@ -105,14 +178,22 @@ __device__ __forceinline__ float key_value(unsigned k) {
   return k == 0xffffffffu ? __uint_as_float(0x7fffffffu) : __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
 }
 
-// Running softmax statistics of raw logits; exponents count in units of ln 2 / scale. m = -inf: nothing but -inf so far.
+// Running softmax statistics: exponents count in units of ln 2 and relative to `reference(m)`, the product rounded once, so
+// that the exponent of a logit is one fused multiply-add. m = -inf: nothing but -inf so far.
 struct Stats {
   float m, s, t;
 };
-// What (s, t) of maximum `m` become under the maximum `to` >= m.
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+// The exponent of x under the maximum m. Where m * c overflows (a row of the type's lowest value), the difference comes first.
+__device__ __forceinline__ float exponent(float x, float m, float c) {
+  const float r = m * c;
+  return finite(r) ? fmaf(x, c, -r) : (x - m) * c;
+}
+// What (s, t) of maximum a.m become under the maximum `to` >= a.m.
 __device__ __forceinline__ void restate(Stats& a, float to, float c) {
   if (a.m == to) return;
-  const float d = a.m == -INFINITY ? -INFINITY : (a.m - to) * c;
+  const float r = to * c, q = a.m * c;
+  const float d = a.m == -INFINITY ? -INFINITY : finite(r) ? q - r : (a.m - to) * c;
   const float f = exp2_fast(d);
   a.t = f > 0.f ? f * (a.t + d * a.s) : (f != f ? f : 0.f);
   a.s *= f;
@@ -127,34 +208,124 @@ __device__ __forceinline__ Stats joined(Stats a, Stats b, float c) {
 
 // ---- forward -------------------------------------------------------------------------------------------------------
 
-constexpr int kScoreThreads = 512, kScoreWarps = kScoreThreads / 32;
-constexpr int kScoreUnroll = 4;      // 16-byte loads a thread has in flight
-constexpr int kScoreCandidates = 512;
+constexpr int kScoreThreads = 256, kScoreWarps = kScoreThreads / 32;
+constexpr int kScorePerSm = 4;
+constexpr int kScoreVectors = 4;  // 16-byte loads of a batch; the next batch's are in flight while one is added up
+constexpr int kChunk = 256;       // logits
 constexpr int kScoreClusterMax = 8;
+
+// An element or interval in the order of the tournament: value first, lower position first among equal ones. 0: none.
+typedef unsigned long long Entry;
+__device__ __forceinline__ Entry entry(unsigned key, unsigned position) { return (Entry)key << 32 | (0xffffffffu - position); }
+__device__ __forceinline__ unsigned position_of(Entry e) { return 0xffffffffu - (unsigned)e; }
+
+__device__ __forceinline__ Entry max_entry(Entry a, Entry b) { return a > b ? a : b; }
+
+// Places of a warp's entries among each other, N a lane, the largest first.
+template <int N, typename E>
+__device__ __forceinline__ void places(const E (&x)[N], int (&place)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    place[i] = 0;
+#pragma unroll
+    for (int j = 0; j < N; j++) place[i] += x[j] > x[i];
+  }
+#pragma unroll
+  for (int d = 1; d < 32; d++)
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      const E y = __shfl_xor_sync(~0u, x[j], d);
+#pragma unroll
+      for (int i = 0; i < N; i++) place[i] += y > x[i];
+    }
+}
+
+// The first k of the entries get(0..n-1), n <= 32 N, to out; 0 where there are fewer.
+template <int N, typename Get>
+__device__ __forceinline__ void select_few(Get&& get, int n, int k, Entry* out) {
+  const int lane = threadIdx.x % 32;
+  Entry x[N];
+  int place[N], have = 0;
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    x[i] = i * 32 + lane < n ? get(i * 32 + lane) : 0;
+    have += __popc(__ballot_sync(~0u, x[i] != 0));
+  }
+  places(x, place);
+#pragma unroll
+  for (int i = 0; i < N; i++)
+    if (x[i] && place[i] < k) out[place[i]] = x[i];
+  for (int i = have + lane; i < k; i += 32) out[i] = 0;
+}
+
+constexpr int kFew = 64;
+
+// The same for any n. One warp; `spare` has room for kFew entries.
+template <typename Get>
+__device__ __forceinline__ void select(Get&& get, int n, int k, Entry* out, Entry* spare) {
+  const int lane = threadIdx.x % 32;
+  if (n <= 32) return select_few<1>(get, n, k, out);
+  if (n <= kFew) return select_few<2>(get, n, k, out);
+  int count = kFew + 1;
+  if (k <= 32) {
+    // The k-th largest of 64 groups' maxima (a lane has two) is a lower bound; about 64 ln(64 / (64 - k)) entries reach it.
+    unsigned best[2] = {0, 0};
+    for (int i = lane; i < n; i += 64) {
+      best[0] = max(best[0], (unsigned)(get(i) >> 32));
+      if (i + 32 < n) best[1] = max(best[1], (unsigned)(get(i + 32) >> 32));
+    }
+    int place[2];
+    places(best, place);  // equal maxima share the first of their places
+    const unsigned low = min(place[0] < k ? best[0] : ~0u, place[1] < k ? best[1] : ~0u);
+    const unsigned bound = __reduce_min_sync(~0u, low);
+    count = 0;
+    for (int i0 = 0; i0 < n && count <= kFew; i0 += 32) {
+      const Entry x = i0 + lane < n ? get(i0 + lane) : 0;
+      const bool in = x != 0 && (unsigned)(x >> 32) >= bound;
+      const unsigned all = __ballot_sync(~0u, in);
+      const int at = count + __popc(all & ((1u << lane) - 1));
+      if (in && at < kFew) spare[at] = x;
+      count += __popc(all);
+    }
+    __syncwarp();
+  }
+  if (count <= 32) return select_few<1>([&](int i) { return spare[i]; }, count, k, out);
+  if (count <= kFew) return select_few<2>([&](int i) { return spare[i]; }, count, k, out);
+  Entry limit = ~0ull;  // many equal ones, or a long list: one by one
+  for (int j = 0; j < k; j++) {
+    Entry x = 0;
+    for (int i = lane; i < n; i += 32) {
+      const Entry y = get(i);
+      if (y < limit) x = max_entry(x, y);
+    }
+    const unsigned key = __reduce_max_sync(~0u, (unsigned)(x >> 32));
+    const unsigned low = __reduce_max_sync(~0u, (unsigned)(x >> 32) == key ? (unsigned)x : 0u);
+    limit = (Entry)key << 32 | low;
+    if (lane == 0) out[j] = limit;
+  }
+}
 
 struct ScoreShared {
   Stats stats[kScoreWarps];
-  Stats cluster_stats[kScoreClusterMax];                             // of the rank-0 block
-  unsigned long long cluster_top[kScoreClusterMax * kScoreTopMax];   // of the rank-0 block
-  unsigned long long candidate[kScoreCandidates];
-  int chunk[kScoreTopMax];
-  int count[34];
+  Stats cluster_stats[kScoreClusterMax];                    // of the rank-0 block
+  Entry cluster_top[kScoreClusterMax * kScoreTopMax];       // of the rank-0 block
+  Entry chosen[kScoreTopMax], spare[kFew];
   int n;
-  unsigned threshold;
 };
 
-// Sum of one small count per thread over the block; nothing used `slot` since it was cleared.
-__device__ __forceinline__ int block_count(int mine, int* slot) {
-  mine = __reduce_add_sync(~0u, mine);
-  if (threadIdx.x % 32 == 0 && mine) atomicAdd(slot, mine);
-  __syncthreads();
-  return *slot;
+__device__ __forceinline__ float warp_max(float x) {
+  float y;
+  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kScoreThreads) token_score_kernel(TokenScore a, int segment_chunks) {
+__global__ void __launch_bounds__(kScoreThreads, kScorePerSm) token_score_kernel(TokenScore a, int segment_chunks) {
   constexpr int V = Logit<T>::V;
-  extern __shared__ unsigned chunk_key[];  // TOP: the maxima of this block's chunks
+  constexpr int kVectorsOfChunk = kChunk / (32 * V);              // 16-byte loads a thread has of a chunk
+  constexpr int kChunks = kScoreVectors / kVectorsOfChunk;        // chunks of a batch
+  extern __shared__ Entry list[];                                 // TOP: vectors, then elements, of a round
+  float* chunk_max = reinterpret_cast<float*>(list + a.top * (kChunk / V));  // TOP: of this block's chunks
   __shared__ ScoreShared sh;
   PJRTX_PDL_PROLOGUE();
   cg::cluster_group cluster = cg::this_cluster();
@@ -163,70 +334,109 @@ __global__ void __launch_bounds__(kScoreThreads) token_score_kernel(TokenScore a
   const long long row = blockIdx.x / ranks;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const T* logits = static_cast<const T*>(a.logits) + row * a.row_stride;
-  // Vectors are 16-byte aligned: the row starts `shift` elements into the first one.
+  // Vectors are 16-byte aligned: the row is elements [shift, end) of `aligned`.
   const int shift = (int)((reinterpret_cast<uintptr_t>(logits) & 15) / sizeof(T));
   const T* aligned = logits - shift;
-  const int end = (int)a.vocab + shift;  // element positions [shift, end) of `aligned` are the row
-  const int vectors = (end + V - 1) / V;
-  const int chunks = (vectors + 31) / 32;
+  const int end = (int)a.vocab + shift;
+  const int chunks = (end + kChunk - 1) / kChunk;
   const int chunk0 = min(chunks, rank * segment_chunks), chunk1 = min(chunks, chunk0 + segment_chunks);
   const float c = a.scale * kLog2e;
 
-  auto load = [&](int v, float* f) {  // positions outside the row: -inf
-    const int p = v * V;
-    if (p >= shift && p + V <= end) {
-      Logit<T>::unpack(*reinterpret_cast<const uint4*>(aligned + p), f);
-    } else {
+  auto load = [&](int p) {  // the vector at element p; -inf outside the row
+    if (p >= shift && p + V <= end) return *reinterpret_cast<const uint4*>(aligned + p);
+    float f[V];
 #pragma unroll
-      for (int i = 0; i < V; i++) f[i] = p + i >= shift && p + i < end ? Logit<T>::load(aligned + p + i) : -INFINITY;
-    }
+    for (int i = 0; i < V; i++) f[i] = p + i >= shift && p + i < end ? Logit<T>::load(aligned + p + i) : -INFINITY;
+    return Logit<T>::pack(f);
   };
-
-  Stats mine = {-INFINITY, 0.f, 0.f};
-  for (int k0 = chunk0 + warp * kScoreUnroll; k0 < chunk1; k0 += kScoreWarps * kScoreUnroll) {
-    float f[kScoreUnroll][V];
-    const bool whole = k0 + kScoreUnroll <= chunk1 && k0 * 32 * V >= shift && (k0 + kScoreUnroll) * 32 * V <= end;
-    if (whole) {
-      uint4 r[kScoreUnroll];
+  auto load_batch = [&](int k0, uint4 (&r)[kScoreVectors]) {
+    const int p = k0 * kChunk + lane * V;
+    if (k0 * kChunk >= shift && (k0 + kChunks) * kChunk <= end && k0 + kChunks <= chunk1) {
 #pragma unroll
-      for (int u = 0; u < kScoreUnroll; u++) r[u] = *reinterpret_cast<const uint4*>(aligned + ((k0 + u) * 32 + lane) * V);
-#pragma unroll
-      for (int u = 0; u < kScoreUnroll; u++) Logit<T>::unpack(r[u], f[u]);
+      for (int u = 0; u < kScoreVectors; u++) r[u] = *reinterpret_cast<const uint4*>(aligned + p + u * 32 * V);
     } else {
+      const int stop = min(end, chunk1 * kChunk);
 #pragma unroll
-      for (int u = 0; u < kScoreUnroll; u++) {
-        if (k0 + u < chunk1) {
-          load((k0 + u) * 32 + lane, f[u]);
+      for (int u = 0; u < kScoreVectors; u++) {
+        if (p + u * 32 * V < stop) {
+          r[u] = load(p + u * 32 * V);
         } else {
+          float f[V];
 #pragma unroll
-          for (int i = 0; i < V; i++) f[u][i] = -INFINITY;
+          for (int i = 0; i < V; i++) f[i] = -INFINITY;
+          r[u] = Logit<T>::pack(f);
         }
       }
     }
+  };
+
+  float m = -INFINITY, reference = -INFINITY;
+  Pair s = pair_of(0.f, 0.f), t = pair_of(0.f, 0.f);
+  uint4 next[kScoreVectors];
+  const int step = kScoreWarps * kChunks;
+  int k0 = chunk0 + warp * kChunks;
+  if (k0 < chunk1) load_batch(k0, next);
+  for (; k0 < chunk1; k0 += step) {
+    uint4 r[kScoreVectors];
+#pragma unroll
+    for (int u = 0; u < kScoreVectors; u++) r[u] = next[u];
+    if (k0 + step < chunk1) load_batch(k0 + step, next);
     float top = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < kScoreUnroll; u++) {
-      float best = f[u][0];
-#pragma unroll
-      for (int i = 1; i < V; i++) best = max_nan(best, f[u][i]);
+    for (int j = 0; j < kChunks; j++) {
+      float high = Logit<T>::template highest<kVectorsOfChunk>(r + j * kVectorsOfChunk);
       if (TOP) {
-        const unsigned key = __reduce_max_sync(~0u, order_key(best));
-        if (lane == 0 && k0 + u < chunk1) chunk_key[k0 + u - chunk0] = key;
+        high = warp_max(high);
+        if (lane == 0 && k0 + j < chunk1) chunk_max[k0 + j - chunk0] = high;
       }
-      top = max_nan(top, best);
+      top = max_nan(top, high);
     }
-    if (!(top <= mine.m)) restate(mine, top, c);
-    if (mine.m == -INFINITY) continue;
+    if (!(top <= m)) {
+      const float2 s2 = split(s), t2 = split(t);
+      Stats x = {m, s2.x, t2.x}, y = {m, s2.y, t2.y};
+      restate(x, top, c);
+      restate(y, top, c);
+      s = pair_of(x.s, y.s);
+      t = pair_of(x.t, y.t);
+      m = top;
+      reference = m * c;
+    }
+    // Every exponent is finite unless a logit is -inf (or near the lowest number there is).
+    if (finite(reference) && fmaf(Logit<T>::template lowest<kScoreVectors>(r), c, -reference) > -INFINITY) {
+      const Pair c2 = pair_of(c, c), from = pair_of(-reference, -reference);
 #pragma unroll
-    for (int u = 0; u < kScoreUnroll; u++)
+      for (int u = 0; u < kScoreVectors; u++) {
+        float f[V];
+        Logit<T>::unpack(r[u], f);
 #pragma unroll
-      for (int i = 0; i < V; i++) {
-        const float y = max_nan((f[u][i] - mine.m) * c, -200.f);  // 2^-200 is 0, and so is that times -200
-        const float e = exp2_fast(y);
-        mine.s += e;
-        mine.t = fmaf(e, y, mine.t);
+        for (int i = 0; i < V; i += 2) {
+          const Pair y = pair_fma(pair_of(f[i], f[i + 1]), c2, from);
+          const float2 y2 = split(y);
+          const Pair e = pair_of(exp2_fast(y2.x), exp2_fast(y2.y));
+          s = pair_add(s, e);
+          t = pair_fma(e, y, t);
+        }
       }
+    } else if (m != -INFINITY) {
+      float2 s2 = split(s), t2 = split(t);
+#pragma unroll
+      for (int u = 0; u < kScoreVectors; u++) {
+        float f[V];
+        Logit<T>::unpack(r[u], f);
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+          const float y = max_nan(exponent(f[i], m, c), -200.f);  // 2^-200 is 0, and so is that times -200
+          const float e = exp2_fast(y);
+          s2.x += e;
+          t2.x = fmaf(e, y, t2.x);
+        }
+      }
+      s = pair_of(s2.x, s2.y);
+      t = pair_of(t2.x, t2.y);
+    }
   }
+  const float2 s2 = split(s), t2 = split(t);
+  Stats mine = {m, s2.x + s2.y, t2.x + t2.y};
 #pragma unroll
   for (int d = 16; d; d /= 2) {
     Stats o;
@@ -236,162 +446,92 @@ __global__ void __launch_bounds__(kScoreThreads) token_score_kernel(TokenScore a
     mine = joined(mine, o, c);
   }
   if (lane == 0) sh.stats[warp] = mine;
-  if (threadIdx.x < 34) sh.count[threadIdx.x] = 0;
   if (threadIdx.x == 0) sh.n = 0;
   cluster.barrier_wait(std::move(started));
   __syncthreads();
-  if (threadIdx.x == 0) {
-    Stats all = sh.stats[0];
-    for (int w = 1; w < kScoreWarps; w++) all = joined(all, sh.stats[w], c);
-    cluster.map_shared_rank(&sh, 0)->cluster_stats[rank] = all;
+  if (warp == kScoreWarps - 1) {
+    Stats all = lane < kScoreWarps ? sh.stats[lane] : Stats{-INFINITY, 0.f, 0.f};
+#pragma unroll
+    for (int d = kScoreWarps / 2; d; d /= 2) {
+      Stats o;
+      o.m = __shfl_xor_sync(~0u, all.m, d);
+      o.s = __shfl_xor_sync(~0u, all.s, d);
+      o.t = __shfl_xor_sync(~0u, all.t, d);
+      all = joined(all, o, c);
+    }
+    if (lane == 0) cluster.map_shared_rank(&sh, 0)->cluster_stats[rank] = all;
   }
 
   if (TOP) {
-    const int n = chunk1 - chunk0, k = a.top;
-    // The k first chunks: the k-th largest maximum bit by bit, then those above it and the first ones at it.
-    unsigned threshold = 0;
-    if (n > k) {
-      for (int bit = 31; bit >= 0; bit--) {
-        const unsigned t = threshold | (1u << bit);
-        int m = 0;
-        for (int i = threadIdx.x; i < n; i += kScoreThreads) m += chunk_key[i] >= t;
-        if (block_count(m, &sh.count[bit]) >= k) threshold = t;
-      }
-      for (int i = threadIdx.x; i < n; i += kScoreThreads)
-        if (chunk_key[i] > threshold) sh.chunk[atomicAdd(&sh.n, 1)] = i;
-      __syncthreads();
-      // The first warp walks the rest in order; it stops at k.
-      if (warp == 0) {
-        int have = sh.n;
-        for (int i0 = 0; i0 < n && have < k; i0 += 32) {
-          const unsigned same = __ballot_sync(~0u, i0 + lane < n && chunk_key[i0 + lane] == threshold);
-          const int at = have + __popc(same & ((1u << lane) - 1));
-          if ((same >> lane & 1) && at < k) sh.chunk[at] = i0 + lane;
-          have += __popc(same);
+    const int k = a.top, n = chunk1 - chunk0;
+    if (warp == 0) select([&](int i) { return entry(order_key(chunk_max[i]), (unsigned)i); }, n, k, sh.chosen, sh.spare);
+    __syncthreads();
+    {  // vectors of the chosen chunks that reach the last of their maxima
+      const unsigned bound = n < k ? 0u : (unsigned)(sh.chosen[k - 1] >> 32);
+      for (int j = warp; j < k; j += kScoreWarps) {
+        if (sh.chosen[j] == 0) break;
+        const int chunk = chunk0 + (int)position_of(sh.chosen[j]);
+#pragma unroll
+        for (int u = 0; u < kVectorsOfChunk; u++) {
+          const int p = chunk * kChunk + (u * 32 + lane) * V;
+          if (p >= end || p + V <= shift) continue;
+          const uint4 r = load(p);
+          const unsigned key = order_key(Logit<T>::template highest<1>(&r));
+          if (key >= bound) list[atomicAdd(&sh.n, 1)] = entry(key, (unsigned)p);
         }
       }
-    } else if ((int)threadIdx.x < n) {
-      sh.chunk[threadIdx.x] = threadIdx.x;
     }
     __syncthreads();
-    if (threadIdx.x < 34) sh.count[threadIdx.x] = 0;
+    const int vectors = sh.n;
+    __syncthreads();
     if (threadIdx.x == 0) sh.n = 0;
+    if (warp == 0) select([&](int i) { return list[i]; }, vectors, k, sh.chosen, sh.spare);
     __syncthreads();
-    // Their elements at or above the threshold: k of them at least (or all there are), usually few more.
-    const int read = min(n, k);
-    constexpr int R = kScoreTopMax / kScoreWarps;
-    unsigned key[R][V];
-    int found = 0;
-#pragma unroll
-    for (int r = 0; r < R; r++) {
-      const int j = warp + r * kScoreWarps;
+    if ((int)threadIdx.x < k && sh.chosen[threadIdx.x] != 0) {  // their elements
+      const unsigned bound = vectors < k ? 0u : (unsigned)(sh.chosen[k - 1] >> 32);
+      const int p = (int)position_of(sh.chosen[threadIdx.x]);
       float f[V];
-      const int v = j < read ? (chunk0 + sh.chunk[j]) * 32 + lane : 0;
-      if (j < read) load(v, f);
+      Logit<T>::unpack(load(p), f);
 #pragma unroll
       for (int i = 0; i < V; i++) {
-        const int p = v * V + i;
-        key[r][i] = j < read && p >= shift && p < end ? order_key(f[i]) : 0u;
-        found += key[r][i] != 0u && key[r][i] >= threshold;
-      }
-    }
-    int all = block_count(found, &sh.count[32]);
-    unsigned id_limit = 0xffffffffu;  // of the elements at the threshold only those up to this position
-    if (all > kScoreCandidates) {
-      // Too many at or above it (long ties, or values that crowd into few chunks): the k-th largest element itself, and
-      // of those equal to it the first positions.
-      auto count = [&](auto&& is, int* slot) {
-        int m = 0;
-#pragma unroll
-        for (int r = 0; r < R; r++)
-#pragma unroll
-          for (int i = 0; i < V; i++) {
-            const int j = warp + r * kScoreWarps;
-            if (key[r][i] && j < read) m += is(key[r][i], (unsigned)(((chunk0 + sh.chunk[j]) * 32 + lane) * V + i));
-          }
-        return block_count(m, slot);
-      };
-      unsigned kth = 0;
-      for (int bit = 31; bit >= 0; bit--) {
-        const unsigned t = kth | (1u << bit);
-        if (count([&](unsigned x, unsigned) { return x >= t; }, &sh.count[bit]) >= k) kth = t;
-      }
-      threshold = kth;
-      __syncthreads();
-      if (threadIdx.x < 34) sh.count[threadIdx.x] = 0;
-      __syncthreads();
-      const int above = count([&](unsigned x, unsigned) { return x > kth; }, &sh.count[33]);
-      // The (k - above)-th smallest position among the equal ones: the largest limit with fewer than that many below it.
-      unsigned limit = 0;
-      for (int bit = 31; bit >= 0; bit--) {
-        const unsigned t = limit | (1u << bit);
-        if (count([&](unsigned x, unsigned p) { return x == kth && p < t; }, &sh.count[bit]) < k - above) limit = t;
-      }
-      id_limit = limit;
-    }
-#pragma unroll
-    for (int r = 0; r < R; r++) {
-      const int j = warp + r * kScoreWarps;
-#pragma unroll
-      for (int i = 0; i < V; i++) {
-        if (j >= read || key[r][i] == 0u || key[r][i] < threshold) continue;
-        const unsigned p = (unsigned)(((chunk0 + sh.chunk[j]) * 32 + lane) * V + i);
-        if (key[r][i] == threshold && p > id_limit) continue;
-        const int at = atomicAdd(&sh.n, 1);
-        sh.candidate[at] = (unsigned long long)key[r][i] << 32 | (0xffffffffu - (p - (unsigned)shift));
+        const unsigned key = order_key(f[i]);
+        if (p + i >= shift && p + i < end && key >= bound) list[atomicAdd(&sh.n, 1)] = entry(key, (unsigned)(p + i - shift));
       }
     }
     __syncthreads();
-    const int have = sh.n;
-    unsigned long long* to = cluster.map_shared_rank(&sh, 0)->cluster_top + rank * kScoreTopMax;
-    if ((int)threadIdx.x < have) {
-      const unsigned long long x = sh.candidate[threadIdx.x];
-      int before = 0;
-      for (int i = 0; i < have; i++) before += sh.candidate[i] > x;
-      if (before < k) to[before] = x;
-    }
-    if ((int)threadIdx.x >= have && (int)threadIdx.x < k) to[threadIdx.x] = 0;
+    if (warp == 0) select([&](int i) { return list[i]; }, sh.n, k, cluster.map_shared_rank(&sh, 0)->cluster_top + rank * k, sh.spare);
   }
   cluster.sync();
-  if (rank != 0) return;
-  if (warp == 0 || TOP) {
-    Stats all = sh.cluster_stats[0];
-    for (int r = 1; r < ranks; r++) all = joined(all, sh.cluster_stats[r], c);
-    // Nothing but -inf: S = 0, lse = -inf, log probabilities -inf, entropy 0.
-    const float log_s = logf(all.s);
-    const bool none = all.m == -INFINITY;
-    const float top = all.m * a.scale;
-    if (threadIdx.x == 0) {
-      const int token = a.tokens[row];
-      float given = 0.f;
-      if (token >= 0) {
-        if (token < a.vocab) {
-          given = none ? -INFINITY : (Logit<T>::load(logits + token) - all.m) * a.scale - log_s;
-        } else {
-          given = __uint_as_float(0x7fffffffu);
-          report(a.error_flag, kErrorToken);
-        }
+  if (rank != 0 || warp != 0) return;
+  Stats all = sh.cluster_stats[0];
+  for (int r = 1; r < ranks; r++) all = joined(all, sh.cluster_stats[r], c);
+  // ln of the sum of e^(x - m): S counts from the rounded product m c. Nothing but -inf: S = 0, log probabilities and lse -inf.
+  const float from = all.m * c, log_s = finite(from) ? logf(all.s) - fmaf(all.m, c, -from) * kLn2 : logf(all.s);
+  const bool none = all.m == -INFINITY;
+  if (lane == 0) {
+    const int token = a.tokens[row];
+    float given = 0.f;
+    if (token >= 0) {
+      if (token < a.vocab) {
+        given = none ? -INFINITY : (Logit<T>::load(logits + token) - all.m) * a.scale - log_s;
+      } else {
+        given = __uint_as_float(0x7fffffffu);
+        report(a.error_flag, kErrorToken);
       }
-      a.log_probs[row] = given;
-      if (a.entropy) a.entropy[row] = none ? 0.f : log_s - all.t * kLn2 / all.s;
-      if (a.lse) a.lse[row] = none ? -INFINITY : top + log_s;
     }
-    if (TOP) {
-      const int k = a.top, n = ranks * k;
-      if ((int)threadIdx.x < n) {
-        const unsigned long long x = sh.cluster_top[threadIdx.x / k * kScoreTopMax + threadIdx.x % k];
-        int before = 0;
-        if (ranks == 1) {
-          before = threadIdx.x;
-        } else {
-          for (int i = 0; i < n; i++) before += sh.cluster_top[i / k * kScoreTopMax + i % k] > x;
-        }
-        if (before < k && x) {
-          const float value = key_value((unsigned)(x >> 32));
-          if (a.top_ids) a.top_ids[row * k + before] = (int)(0xffffffffu - (unsigned)x);
-          if (a.top_log_probs) a.top_log_probs[row * k + before] = none ? -INFINITY : (value - all.m) * a.scale - log_s;
-        }
-      }
+    a.log_probs[row] = given;
+    if (a.entropy) a.entropy[row] = none ? 0.f : logf(all.s) - all.t * kLn2 / all.s;
+    if (a.lse) a.lse[row] = none ? -INFINITY : all.m * a.scale + log_s;
+  }
+  if (TOP) {
+    const int k = a.top;
+    if (ranks > 1) select([&](int i) { return sh.cluster_top[i]; }, ranks * k, k, sh.chosen, sh.spare);
+    __syncwarp();
+    const Entry* best = ranks > 1 ? sh.chosen : sh.cluster_top;
+    for (int j = lane; j < k; j += 32) {
+      const float value = key_value((unsigned)(best[j] >> 32));
+      if (a.top_ids) a.top_ids[row * k + j] = (int)position_of(best[j]);
+      if (a.top_log_probs) a.top_log_probs[row * k + j] = none ? -INFINITY : (value - all.m) * a.scale - log_s;
     }
   }
 }
@@ -461,13 +601,14 @@ __global__ void __launch_bounds__(kGradThreads) token_score_grad_kernel(TokenSco
 
 template <typename T>
 int score_launch(const TokenScore& s, int sm_count, bool pdl, cudaStream_t stream) {
-  const int chunks = (int)((s.vocab + Logit<T>::V - 1 + Logit<T>::V - 1) / Logit<T>::V + 31) / 32;
-  // A cluster for each row: as many blocks as fill the GPU twice, none with less than a load of every thread.
+  const int chunks = (int)((s.vocab + Logit<T>::V - 1 + kChunk - 1) / kChunk);
+  // A cluster for each row: as many blocks as fill the GPU, none with less than a batch for every warp.
+  const int batch_chunks = kScoreWarps * kScoreVectors * 32 * Logit<T>::V / kChunk;
   int ranks = 1;
-  while (ranks < kScoreClusterMax && s.rows * ranks < 2 * sm_count && chunks > ranks * kScoreWarps) ranks *= 2;
+  while (ranks < kScoreClusterMax && s.rows * ranks < (long long)kScorePerSm * sm_count && chunks > ranks * batch_chunks) ranks *= 2;
   const int segment = (chunks + ranks - 1) / ranks;
   const bool top = s.top > 0;
-  const size_t smem = top ? (size_t)segment * sizeof(unsigned) : 0;
+  const size_t smem = top ? (size_t)s.top * (kChunk / Logit<T>::V) * sizeof(Entry) + (size_t)segment * sizeof(float) : 0;
   auto kernel = top ? token_score_kernel<T, true> : token_score_kernel<T, false>;
   if (smem > 32 * 1024 && !raise_smem_limit((const void*)kernel, 200 * 1024)) return 0;
   cudaLaunchConfig_t cfg = {};

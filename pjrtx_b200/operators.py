@@ -134,6 +134,13 @@ def _check(x, name: str, dtype: int, shape: Tuple[int, ...]) -> None:
 
 def _rows(x, name: str, dtype: int, shape: Tuple[int, ...]):
     """Address and strides of an array whose innermost axis has to be dense."""
+    try:  # a tensor that is as it has to be
+        if x.shape == shape and _codes[x.dtype] == dtype:
+            strides = x.stride()
+            if strides[-1] == 1:
+                return x.data_ptr(), strides
+    except (AttributeError, KeyError):
+        pass
     _check(x, name, dtype, shape)
     place = _place(x)
     if place[1][-1] != 1 and shape[-1] != 1:
@@ -143,6 +150,11 @@ def _rows(x, name: str, dtype: int, shape: Tuple[int, ...]):
 
 def _twin(x, name: str, like, like_name: str, strides) -> int:
     """Address of an array that has the type, shape and strides of `like`."""
+    try:
+        if x.shape == like.shape and x.dtype == like.dtype and x.stride() == strides:
+            return x.data_ptr()
+    except AttributeError:
+        pass
     if _code(x) != _code(like) or _dims(x) != _dims(like):
         raise _error(f"{like_name} and {name} differ in type or shape")
     pointer, own = _place(x)
@@ -155,17 +167,18 @@ def _dense(x, name: str, dtype: int, shape: Tuple[int, ...]) -> int:
     """Address of an array that has to be dense; None is 0."""
     if x is None:
         return 0
-    _check(x, name, dtype, shape)
     try:
-        dense, pointer = x.is_contiguous(), x.data_ptr()
-    except AttributeError:
-        pointer, strides = _place(x)
-        step, dense = 1, True
-        for d, s in zip(reversed(shape), reversed(strides)):
-            dense = dense and (s == step or d == 1)
-            step *= d
-    if not dense:
-        raise _error(f"{name} has to be dense")
+        if x.shape == shape and _codes[x.dtype] == dtype and x.is_contiguous():
+            return x.data_ptr()
+    except (AttributeError, KeyError):
+        pass
+    _check(x, name, dtype, shape)
+    pointer, strides = _place(x)
+    step = 1
+    for d, s in zip(reversed(shape), reversed(strides)):
+        if s != step and d != 1 and 0 not in shape:
+            raise _error(f"{name} has to be dense, its strides are {strides}")
+        step *= d
     return pointer
 
 
