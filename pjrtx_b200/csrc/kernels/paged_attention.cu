@@ -60,6 +60,7 @@ struct AttendArgs {
   AttendSpace space;
   int rep, groups;  // query heads of a KV head, groups of them
   int pieces;       // 16-byte pieces of a row
+  unsigned reciprocal;  // floor(2^32 / page_size), at most 2^32 - 1
 };
 
 struct Cursor {
@@ -146,7 +147,10 @@ struct RowStage {
   static constexpr int kBytes = 2 * kWarpRows * kPitch;
 };
 
-__device__ __forceinline__ void copy16(unsigned to, const void* from, bool valid) {
+__device__ __forceinline__ void copy16(unsigned to, unsigned long long from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy16_or_zero(unsigned to, unsigned long long from, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(valid ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -164,8 +168,12 @@ __device__ __forceinline__ RowPlace locate(const AttendArgs& p, const Cursor& u)
   const int t = u.tile * kTileRows + (threadIdx.x / 32) * kWarpRows + (threadIdx.x & 15);
   RowPlace r = {-1, 0};
   if (t < u.length) {
-    const int column = t / p.c.page_size;
+    int column = (int)__umulhi((unsigned)t, p.reciprocal);  // the quotient or one less
     r.row = t - column * p.c.page_size;
+    if (r.row >= p.c.page_size) {
+      column++;
+      r.row -= p.c.page_size;
+    }
     r.page = p.c.table[u.b * p.c.table_stride + column];
     if (r.page < 0 || r.page >= p.c.num_pages) {
       report(p.c.error_flag, kErrorPageId);
@@ -175,51 +183,62 @@ __device__ __forceinline__ RowPlace locate(const AttendArgs& p, const Cursor& u)
   return r;
 }
 
+__device__ __forceinline__ unsigned long long address_of(const void* p) { return reinterpret_cast<unsigned long long>(p); }
+
 // Requests the rows of `u`; the stage's mask word says which ones count.
 template <typename T, int D>
 __device__ __forceinline__ void request(const AttendArgs& p, const Cursor& u, const RowPlace& r, char* stage, unsigned* mask) {
   using S = RowStage<T, D>;
-  constexpr int kPieces = D * (int)sizeof(T) / 16;
-  constexpr int kAcross = kPieces < 8 ? kPieces : 8;  // lanes beside each other on one row
+  constexpr int kPieces = D * (int)sizeof(T) / 16, kAcross = 8;  // eight lanes beside each other on one row
   const int lane = threadIdx.x % 32, g = u.group / p.groups;
   const int t0 = u.tile * kTileRows + (threadIdx.x / 32) * kWarpRows;
-  const char *k = nullptr, *v = nullptr;
-  if (r.page >= 0) {
-    const long long at = (r.page * p.c.page_stride + r.row * p.c.row_stride + g * p.c.head_stride) * (long long)sizeof(T);
-    k = static_cast<const char*>(p.c.k) + at;
-    v = static_cast<const char*>(p.c.v) + at;
-  }
+  unsigned long long k = 0;  // address of the key; the value's is `apart` further
+  const unsigned long long apart_pools = address_of(p.c.v) - address_of(p.c.k);
+  unsigned long long apart = apart_pools;
+  if (r.page >= 0)
+    k = address_of(p.c.k) + (r.page * p.c.page_stride + r.row * p.c.row_stride + g * p.c.head_stride) * (long long)sizeof(T);
   const int fresh = u.length - 1 - t0;  // which of the 16 rows comes with the call
-  if (p.a.k_new && fresh >= 0 && fresh < kWarpRows) {
+  const bool has_fresh = p.a.k_new && fresh >= 0 && fresh < kWarpRows;
+  if (has_fresh) {
     const long long at = (u.b * p.a.new_batch_stride + g * p.a.new_head_stride) * (long long)sizeof(T);
     const char* k_new = static_cast<const char*>(p.a.k_new) + at;
     const char* v_new = static_cast<const char*>(p.a.v_new) + at;
-    char* k_to = reinterpret_cast<char*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(k), fresh));
-    char* v_to = reinterpret_cast<char*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(v), fresh));
-    if (k_to && u.group % p.groups == 0)
+    const unsigned long long to = __shfl_sync(~0u, k, fresh);
+    if (to && u.group % p.groups == 0)
       for (int i = lane; i < p.pieces; i += 32) {
-        reinterpret_cast<uint4*>(k_to)[i] = reinterpret_cast<const uint4*>(k_new)[i];
-        reinterpret_cast<uint4*>(v_to)[i] = reinterpret_cast<const uint4*>(v_new)[i];
+        reinterpret_cast<uint4*>(to)[i] = reinterpret_cast<const uint4*>(k_new)[i];
+        reinterpret_cast<uint4*>(to + apart_pools)[i] = reinterpret_cast<const uint4*>(v_new)[i];
       }
     if ((lane & 15) == fresh && k) {
-      k = k_new;
-      v = v_new;
+      k = address_of(k_new);
+      apart = address_of(v_new) - k;
     }
   }
-  const unsigned there = __ballot_sync(~0u, k != nullptr) & 0xffffu;
+  const unsigned there = __ballot_sync(~0u, k != 0) & 0xffffu;
   if (lane == 0) *mask = there;
-  const unsigned to = (unsigned)__cvta_generic_to_shared(stage);
+  const unsigned to = (unsigned)__cvta_generic_to_shared(stage) + lane / kAcross * S::kPitch + lane % kAcross * 16;
+  const bool whole = there == 0xffffu && p.pieces == kPieces;
 #pragma unroll
   for (int j = 0; j < kWarpRows * kAcross / 32; j++) {
     const int row = lane / kAcross + j * (32 / kAcross);
-    const char* kr = reinterpret_cast<const char*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(k), row));
-    const char* vr = reinterpret_cast<const char*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(v), row));
+    unsigned long long kr = __shfl_sync(~0u, k, row), vr = apart;
+    if (has_fresh) vr = __shfl_sync(~0u, apart, row);
+    const bool valid = kr != 0;
+    kr += lane % kAcross * 16;
+    vr += kr;
+    if (whole) {
 #pragma unroll
-    for (int i = 0; i < kPieces / kAcross; i++) {
-      const int piece = lane % kAcross + i * kAcross;
-      const bool valid = kr != nullptr && piece < p.pieces;
-      copy16(to + row * S::kPitch + piece * 16, valid ? kr + piece * 16 : static_cast<const char*>(p.c.k), valid);
-      copy16(to + (kWarpRows + row) * S::kPitch + piece * 16, valid ? vr + piece * 16 : static_cast<const char*>(p.c.v), valid);
+      for (int i = 0; i < kPieces / kAcross; i++) {
+        copy16(to + j * (32 / kAcross) * S::kPitch + i * kAcross * 16, kr + i * kAcross * 16);
+        copy16(to + (kWarpRows + j * (32 / kAcross)) * S::kPitch + i * kAcross * 16, vr + i * kAcross * 16);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPieces / kAcross; i++) {
+        const bool in = valid && lane % kAcross + i * kAcross < p.pieces;
+        copy16_or_zero(to + j * (32 / kAcross) * S::kPitch + i * kAcross * 16, in ? kr + i * kAcross * 16 : address_of(p.c.k), in);
+        copy16_or_zero(to + (kWarpRows + j * (32 / kAcross)) * S::kPitch + i * kAcross * 16, in ? vr + i * kAcross * 16 : address_of(p.c.v), in);
+      }
     }
   }
 }
@@ -407,24 +426,17 @@ struct MmaWarp {
         }
       }
   }
-  // values[head * pitch + dim] (+)= values * factor[head].
-  __device__ __forceinline__ void add_values(float* values, int pitch, const float* factor, bool first) const {
+  // This warp's sums to values[head * pitch + dim].
+  __device__ __forceinline__ void values(float* to, int pitch) const {
     const int lane = threadIdx.x % 32;
 #pragma unroll
     for (int n = 0; n < NB; n++)
 #pragma unroll
-      for (int j = 0; j < 2; j++) {
-        const int h = n * 8 + (lane % 4) * 2 + j;
-        const float f = factor[h];
+      for (int j = 0; j < 2; j++)
 #pragma unroll
         for (int i = 0; i < D / 16; i++)
 #pragma unroll
-          for (int r = 0; r < 2; r++) {
-            float* to = values + h * pitch + i * 16 + r * 8 + lane / 4;
-            const float x = o[i][n][2 * r + j] * f;
-            *to = first ? x : *to + x;
-          }
-      }
+          for (int r = 0; r < 2; r++) to[(n * 8 + (lane % 4) * 2 + j) * pitch + i * 16 + r * 8 + lane / 4] = o[i][n][2 * r + j];
   }
 };
 
@@ -544,29 +556,23 @@ struct FmaWarp {
       }
     }
   }
-  __device__ __forceinline__ void add_values(float* values, int pitch, const float* factor, bool first) const {
+  __device__ __forceinline__ void values(float* to, int pitch) const {
     const int lane = threadIdx.x % 32;
 #pragma unroll
     for (int h = 0; h < H; h++)
 #pragma unroll
-      for (int i = 0; i < V; i++) {
-        float* to = values + h * pitch + lane * V + i;
-        const float x = o[h][i] * factor[h];
-        *to = first ? x : *to + x;
-      }
+      for (int i = 0; i < V; i++) to[h * pitch + lane * V + i] = o[h][i];
   }
 };
 
 // ---- the kernel ----------------------------------------------------------------------------------------------------
 
-template <typename W, int D>
+template <typename W>
 struct JoinSpace {  // at the end of a segment
   static constexpr int H = W::kHeads;
-  float values[H * (D + 4)];
-  float stat[kWarps][H][2];
-  float factor[kWarps][H];
-  float total[H], top[H];
-  float reduce[kThreads];
+  float2 stat[kWarps][H];  // (max, sum)
+  float2 total[H];         // of all blocks
+  float2 reduce[kThreads];
   long long scratch[kWarps + 2];
   unsigned mask[kWarps][8];
   int last;
@@ -588,14 +594,101 @@ __device__ __forceinline__ void store_lse(const AttendArgs& p, int b, int h, flo
   if (p.a.lse) p.a.lse[at] = lse2 * kLn2;
 }
 
+// Four dimensions of the result from sums under the maximum `top`.
+template <typename T>
+__device__ __forceinline__ void finish(const AttendArgs& p, int b, int h, int d, T* out, float4 x, float top, float total) {
+  if (d == 0) store_lse(p, b, h, top, total);
+  if (d >= p.c.head_dim) return;
+  const float inverse = total == 0.f ? 0.f : 1.f / total;
+  x.x *= inverse; x.y *= inverse; x.z *= inverse; x.w *= inverse;
+  store4(out + d, x);
+}
+
+// Joins the `count` parts of a segment. One block's parts are kSlot * 2 floats apart, but for the first, which is a slot later.
+// The block reads them all (4 KB a part with eight heads of 128), so eight loads a thread are in flight at once; where there are
+// fewer pieces of results than threads, several threads share a piece and take every so many-th part.
+template <typename T, typename W, int D>
+__device__ __forceinline__ void merge(const AttendArgs& p, int b, int h0, int heads, const float* parts, int count, T* out,
+                                      JoinSpace<W>& join, char* space) {
+  constexpr int H = W::kHeads, kSlot = H * (D + 2), kBeside = kThreads / H, kAtOnce = 8;
+  auto part = [&](int i) { return parts + (i == 0 ? kSlot : (long long)i * 2 * kSlot); };
+  {
+    const int h = threadIdx.x % H, beside = threadIdx.x / H;
+    float top = -INFINITY, total = 0.f;
+    if (h < heads)
+      for (int i = beside; i < count; i += kBeside) {
+        const float2 stat = __ldcg(reinterpret_cast<const float2*>(part(i) + H * D + 2 * h));
+        const float m = max_nan(top, stat.x);
+        total = (top == -INFINITY ? 0.f : total * exp2_fast(top - m)) + (stat.x == -INFINITY ? 0.f : stat.y * exp2_fast(stat.x - m));
+        top = m;
+      }
+    join.reduce[threadIdx.x] = make_float2(top, total);
+    __syncthreads();
+    if (beside == 0) {
+      for (int k = 1; k < kBeside; k++) {
+        const float2 o = join.reduce[k * H + h];
+        const float m = max_nan(top, o.x);
+        total = (top == -INFINITY ? 0.f : total * exp2_fast(top - m)) + (o.x == -INFINITY ? 0.f : o.y * exp2_fast(o.x - m));
+        top = m;
+      }
+      join.total[h] = make_float2(top, total);
+    }
+    __syncthreads();
+  }
+  const int items = heads * (D / 4);
+  int sharers = 1;
+  while (sharers * 2 * items <= kThreads) sharers *= 2;
+  for (int j0 = 0; j0 < items; j0 += kThreads) {
+    const int j = sharers > 1 ? (int)threadIdx.x % items : j0 + (int)threadIdx.x, share = sharers > 1 ? (int)threadIdx.x / items : 0;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int h = min(j, items - 1) / (D / 4), d = j % (D / 4) * 4;
+    const float2 all = join.total[h];
+    if (j < items && share < sharers)
+      for (int i0 = share; i0 < count; i0 += sharers * kAtOnce) {
+        float4 y[kAtOnce];
+        float m[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; k++) {
+          const int i = i0 + k * sharers;
+          m[k] = -INFINITY;
+          if (i < count) {
+            m[k] = __ldcg(part(i) + H * D + 2 * h);
+            y[k] = __ldcg(reinterpret_cast<const float4*>(part(i) + j * 4));
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; k++)
+          if (m[k] != -INFINITY) {
+            const float f = exp2_fast(m[k] - all.x);
+            x.x = fmaf(f, y[k].x, x.x);
+            x.y = fmaf(f, y[k].y, x.y);
+            x.z = fmaf(f, y[k].z, x.z);
+            x.w = fmaf(f, y[k].w, x.w);
+          }
+      }
+    if (sharers > 1) {
+      float4* sums = reinterpret_cast<float4*>(space);
+      sums[threadIdx.x] = x;
+      __syncthreads();
+      if (share > 0 || (int)threadIdx.x >= items) continue;
+      for (int k = 1; k < sharers; k++) {
+        const float4 y = sums[k * items + j];
+        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+      }
+    }
+    if (j < items) finish(p, b, h0 + h, d, out + h * p.a.out_head_stride, x, all.x, all.y);
+  }
+}
+
 template <typename T, typename W, int D, int STAGES, int PER_SM>
 __global__ void __launch_bounds__(kThreads, PER_SM) paged_attend_kernel(const __grid_constant__ AttendArgs p) {
   using Stage = RowStage<T, D>;
-  using Join = JoinSpace<W, D>;
+  using Join = JoinSpace<W>;
   constexpr int H = W::kHeads, kPitch = D + 4;
+  static_assert(H * kPitch * 4 <= Stage::kBytes, "a warp's sums take the place of a stage");
   extern __shared__ __align__(16) char smem[];
-  Join& join = *reinterpret_cast<Join*>(smem + kWarps * STAGES * Stage::kBytes + W::kSharedBytes);
   char* shared = smem + kWarps * STAGES * Stage::kBytes;
+  Join& join = *reinterpret_cast<Join*>(shared + W::kSharedBytes);
   PJRTX_PDL_PROLOGUE();
   const int warp = threadIdx.x / 32;
   char* stages = smem + warp * STAGES * Stage::kBytes;
@@ -635,11 +728,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) paged_attend_kernel(const __
   W work;
   work.start(p, now, shared);
   long long segment = share.begin - now.tile;  // number of the segment's first unit
-  for (int i = 0, stage = 0; i < units; i++) {
-    copies_wait<STAGES - 1>();
-    __syncwarp();
-    work.step(p, now, stages + stage * Stage::kBytes, join.mask[warp][stage], scale2);
-    __syncwarp();
+  auto refill = [&](int i, int stage) {
     if (i + STAGES < units) {
       request<T, D>(p, ahead, next, stages + stage * Stage::kBytes, &join.mask[warp][stage]);
       if (i + STAGES + 1 < units) {
@@ -648,116 +737,72 @@ __global__ void __launch_bounds__(kThreads, PER_SM) paged_attend_kernel(const __
       }
     }
     copies_commit();
-    stage = stage + 1 == STAGES ? 0 : stage + 1;
+  };
+  for (int i = 0, stage = 0; i < units; i++, stage = stage + 1 == STAGES ? 0 : stage + 1) {
+    copies_wait<STAGES - 1>();
+    __syncwarp();
+    work.step(p, now, stages + stage * Stage::kBytes, join.mask[warp][stage], scale2);
+    __syncwarp();
     if (now.tile + 1 < now.tiles && i + 1 < units) {
+      refill(i, stage);
       now.tile++;
       continue;
     }
 
-    // The segment's part of this block is complete: join the warps.
-    work.statistics(&join.stat[warp][0][0]);
+    // This block's part of the segment is complete. The warps' sums take the place of the stages just read.
+    work.statistics(&join.stat[warp][0].x);
+    work.values(reinterpret_cast<float*>(stages + stage * Stage::kBytes), kPitch);
     __syncthreads();
-    if (threadIdx.x < H) {
-      float top = -INFINITY, total = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; w++) top = max_nan(top, join.stat[w][threadIdx.x][0]);
-#pragma unroll
-      for (int w = 0; w < kWarps; w++) {
-        const float m = join.stat[w][threadIdx.x][0], f = m == -INFINITY ? 0.f : exp2_fast(m - top);
-        join.factor[w][threadIdx.x] = f;
-        total += f * join.stat[w][threadIdx.x][1];
-      }
-      join.top[threadIdx.x] = top;
-      join.total[threadIdx.x] = total;
-    }
-    __syncthreads();
-    for (int w = 0; w < kWarps; w++) {
-      if (w == warp) work.add_values(join.values, kPitch, join.factor[w], w == 0);
-      __syncthreads();
-    }
     const int g = now.group / p.groups, h0 = (now.group % p.groups) * H;
     const int heads = min(H, p.rep - h0);
     const long long first = segment / share.quota, last = (segment + now.tiles - 1) / share.quota;
-    bool finish = true;
-    if (first != last) {
-      // Slot 1 holds a segment that begins with this block, slot 0 one that began before it.
-      constexpr int kSlot = H * (D + 2);
-      auto slot = [&](long long block) { return p.space.partials + (block * 2 + (segment >= block * share.quota ? 1 : 0)) * kSlot; };
-      float* mine = slot(blockIdx.x);
-      for (int j = threadIdx.x; j < heads * (D / 4); j += kThreads)
-        *reinterpret_cast<float4*>(mine + j * 4) = *reinterpret_cast<const float4*>(join.values + j / (D / 4) * kPitch + j % (D / 4) * 4);
-      if ((int)threadIdx.x < heads) {
-        mine[H * D + threadIdx.x] = join.top[threadIdx.x];
-        mine[H * D + H + threadIdx.x] = join.total[threadIdx.x];
+    const int others = (int)(last - first);
+    // Slot 1 of a block holds the segment that begins in it, slot 0 the one that began before it.
+    constexpr int kSlot = H * (D + 2);
+    float* mine = p.space.partials + ((long long)blockIdx.x * 2 + (blockIdx.x == first ? 1 : 0)) * kSlot;
+    T* out = static_cast<T*>(p.a.out) + now.b * p.a.out_batch_stride + (long long)(g * p.rep + h0) * p.a.out_head_stride;
+    const float* sums = reinterpret_cast<const float*>(smem + stage * Stage::kBytes);
+    for (int j = threadIdx.x; j < heads * (D / 4); j += kThreads) {
+      const int h = j / (D / 4), d = j % (D / 4) * 4;
+      float top = -INFINITY, total = 0.f;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; w++) top = max_nan(top, join.stat[w][h].x);
+#pragma unroll
+      for (int w = 0; w < kWarps; w++) {
+        const float2 stat = join.stat[w][h];
+        const float f = stat.x == -INFINITY ? 0.f : exp2_fast(stat.x - top);
+        const float4 y = *reinterpret_cast<const float4*>(sums + w * (STAGES * Stage::kBytes / 4) + h * kPitch + d);
+        total = fmaf(f, stat.y, total);
+        x.x = fmaf(f, y.x, x.x);
+        x.y = fmaf(f, y.y, x.y);
+        x.z = fmaf(f, y.z, x.z);
+        x.w = fmaf(f, y.w, x.w);
       }
-      __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        const unsigned others = (unsigned)(last - first);
-        join.last = atomicInc(p.space.counters + (long long)now.b * p.c.kv_heads * p.groups + now.group, others) == others;
-      }
-      __syncthreads();
-      finish = join.last;
-      if (finish) {
-        __threadfence();
-        // Maxima and sums of all blocks, kThreads / H of them side by side.
-        constexpr int kBeside = kThreads / H;
-        const int h = threadIdx.x % H, part = threadIdx.x / H;
-        float top = -INFINITY;
-        if (h < heads)
-          for (long long block = first + part; block <= last; block += kBeside) top = max_nan(top, __ldcg(slot(block) + H * D + h));
-        join.reduce[threadIdx.x] = top;
-        __syncthreads();
-        for (int k = 0; k < kBeside; k++) top = max_nan(top, join.reduce[k * H + h]);
-        __syncthreads();
-        float total = 0.f;
-        if (h < heads)
-          for (long long block = first + part; block <= last; block += kBeside) {
-            const float m = __ldcg(slot(block) + H * D + h);
-            total += m == -INFINITY ? 0.f : exp2_fast(m - top) * __ldcg(slot(block) + H * D + H + h);
-          }
-        join.reduce[threadIdx.x] = total;
-        __syncthreads();
-        if (part == 0) {
-          total = 0.f;
-          for (int k = 0; k < kBeside; k++) total += join.reduce[k * H + h];
-          join.top[h] = top;
-          join.total[h] = total;
-        }
-        __syncthreads();
-        for (int j = threadIdx.x; j < heads * (D / 4); j += kThreads) {
-          const int hh = j / (D / 4), at = j * 4;
-          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (long long block = first; block <= last; block++) {
-            const float* from = slot(block);
-            const float m = __ldcg(from + H * D + hh), f = m == -INFINITY ? 0.f : exp2_fast(m - join.top[hh]);
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(from + at));
-            x.x = fmaf(f, y.x, x.x);
-            x.y = fmaf(f, y.y, x.y);
-            x.z = fmaf(f, y.z, x.z);
-            x.w = fmaf(f, y.w, x.w);
-          }
-          *reinterpret_cast<float4*>(join.values + hh * kPitch + j % (D / 4) * 4) = x;
-        }
-        __syncthreads();
+      if (others == 0) {
+        finish(p, now.b, g * p.rep + h0 + h, d, out + h * p.a.out_head_stride, x, top, total);
+      } else {
+        *reinterpret_cast<float4*>(mine + j * 4) = x;
+        if (d == 0) *reinterpret_cast<float2*>(mine + H * D + 2 * h) = make_float2(top, total);
       }
     }
-    if (finish) {
-      T* out = static_cast<T*>(p.a.out) + now.b * p.a.out_batch_stride + (long long)(g * p.rep + h0) * p.a.out_head_stride;
-      for (int j = threadIdx.x; j < heads * (D / 4); j += kThreads) {
-        const int hh = j / (D / 4), d = j % (D / 4) * 4;
-        if (d >= p.c.head_dim) continue;
-        const float total = join.total[hh], inverse = total == 0.f ? 0.f : 1.f / total;
-        float4 x = *reinterpret_cast<const float4*>(join.values + hh * kPitch + d);
-        x.x *= inverse; x.y *= inverse; x.z *= inverse; x.w *= inverse;
-        store4(out + hh * p.a.out_head_stride + d, x);
+    if (others) {
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0)
+        join.last = atomicInc(p.space.counters + (long long)now.b * p.c.kv_heads * p.groups + now.group, (unsigned)others) == (unsigned)others;
+      __syncthreads();
+      if (join.last) {
+        __threadfence();
+        merge<T, W, D>(p, now.b, g * p.rep + h0, heads, p.space.partials + first * 2 * kSlot, others + 1, out, join,
+                       smem + stage * Stage::kBytes);  // the first warp's sums have been read
       }
-      if ((int)threadIdx.x < heads) store_lse(p, now.b, g * p.rep + h0 + threadIdx.x, join.top[threadIdx.x], join.total[threadIdx.x]);
     }
     if (i + 1 < units) {
       segment += now.tiles;
       advance(p, now);
-      __syncthreads();  // `join` is used again
+      __syncthreads();  // the stages are filled again, and so is `join`
+      refill(i, stage);
       work.start(p, now, shared);
     }
   }
@@ -794,15 +839,15 @@ struct AttendPlan {
 
 template <typename T, typename W, int D, int STAGES>
 constexpr size_t attend_smem() {
-  return (size_t)kWarps * STAGES * RowStage<T, D>::kBytes + W::kSharedBytes + sizeof(JoinSpace<W, D>);
+  return (size_t)kWarps * STAGES * RowStage<T, D>::kBytes + W::kSharedBytes + sizeof(JoinSpace<W>);
 }
 
 template <typename F>
 auto with_kernel(int dtype, int head_dim, int rep, F&& f) {
 #define PJRTX_ATTEND(T, W, D, S, N) return f(paged_attend_kernel<T, W, D, S, N>, AttendPlan{D, W::kHeads, S, N, attend_smem<T, W, D, S>()})
 #define PJRTX_ATTEND_MMA(T, NB)                                                 \
-  if (head_dim <= 64) { using W = MmaWarp<T, 64, NB>; PJRTX_ATTEND(T, W, 64, 5, 2); }  \
-  if (head_dim <= 128) { using W = MmaWarp<T, 128, NB>; PJRTX_ATTEND(T, W, 128, 3, 2); } \
+  if (head_dim <= 64) { using W = MmaWarp<T, 64, NB>; PJRTX_ATTEND(T, W, 64, NB == 1 ? 3 : 4, NB == 1 ? 4 : 3); }  \
+  if (head_dim <= 128) { using W = MmaWarp<T, 128, NB>; PJRTX_ATTEND(T, W, 128, NB == 1 ? 2 : 3, NB == 1 ? 3 : 2); } \
   { using W = MmaWarp<T, 256, 1>; PJRTX_ATTEND(T, W, 256, 3, 1); }
 #define PJRTX_ATTEND_FMA(H)                                                     \
   if (head_dim <= 64) { using W = FmaWarp<64, H>; PJRTX_ATTEND(float, W, 64, 3, 2); }  \
@@ -853,6 +898,7 @@ int paged_attend_launch(const PagedView& c, const PagedAttend& a, int sm_count, 
   p.a = a;
   p.rep = a.heads / c.kv_heads;
   p.pieces = c.head_dim * (int)dtype_size(c.dtype) / 16;
+  p.reciprocal = (unsigned)std::min<uint64_t>((1ull << 32) / c.page_size, 0xffffffffu);
   const bool ok = with_kernel(c.dtype, c.head_dim, p.rep, [&](auto kernel, const AttendPlan& plan) {
     const AttendLayout l = attend_layout(c, a.heads, plan, false, sm_count);
     char* space = static_cast<char*>(a.workspace);
