@@ -571,8 +571,6 @@ template <typename W>
 struct JoinSpace {  // at the end of a segment
   static constexpr int H = W::kHeads;
   float2 stat[kWarps][H];  // (max, sum)
-  float2 total[H];         // of all blocks
-  float2 reduce[kThreads];
   long long scratch[kWarps + 2];
   unsigned mask[kWarps][8];
   int last;
@@ -605,61 +603,46 @@ __device__ __forceinline__ void finish(const AttendArgs& p, int b, int h, int d,
 }
 
 // Joins the `count` parts of a segment. One block's parts are kSlot * 2 floats apart, but for the first, which is a slot later.
-// The block reads them all (4 KB a part with eight heads of 128), so eight loads a thread are in flight at once; where there are
-// fewer pieces of results than threads, several threads share a piece and take every so many-th part.
+// The block reads them all (4 KB a part with eight heads of 128) from L2, so every thread has as many loads in flight as it has
+// registers for; where there are fewer results than threads, several threads share one and take every so many-th part.
 template <typename T, typename W, int D>
-__device__ __forceinline__ void merge(const AttendArgs& p, int b, int h0, int heads, const float* parts, int count, T* out,
-                                      JoinSpace<W>& join, char* space) {
-  constexpr int H = W::kHeads, kSlot = H * (D + 2), kBeside = kThreads / H, kAtOnce = 8;
+__device__ __forceinline__ void merge(const AttendArgs& p, int b, int h0, int heads, const float* parts, int count, T* out, char* space) {
+  constexpr int H = W::kHeads, kSlot = H * (D + 2), kAtOnce = 6;
   auto part = [&](int i) { return parts + (i == 0 ? kSlot : (long long)i * 2 * kSlot); };
-  {
-    const int h = threadIdx.x % H, beside = threadIdx.x / H;
-    float top = -INFINITY, total = 0.f;
-    if (h < heads)
-      for (int i = beside; i < count; i += kBeside) {
-        const float2 stat = __ldcg(reinterpret_cast<const float2*>(part(i) + H * D + 2 * h));
-        const float m = max_nan(top, stat.x);
-        total = (top == -INFINITY ? 0.f : total * exp2_fast(top - m)) + (stat.x == -INFINITY ? 0.f : stat.y * exp2_fast(stat.x - m));
-        top = m;
-      }
-    join.reduce[threadIdx.x] = make_float2(top, total);
-    __syncthreads();
-    if (beside == 0) {
-      for (int k = 1; k < kBeside; k++) {
-        const float2 o = join.reduce[k * H + h];
-        const float m = max_nan(top, o.x);
-        total = (top == -INFINITY ? 0.f : total * exp2_fast(top - m)) + (o.x == -INFINITY ? 0.f : o.y * exp2_fast(o.x - m));
-        top = m;
-      }
-      join.total[h] = make_float2(top, total);
-    }
-    __syncthreads();
-  }
   const int items = heads * (D / 4);
   int sharers = 1;
   while (sharers * 2 * items <= kThreads) sharers *= 2;
   for (int j0 = 0; j0 < items; j0 += kThreads) {
-    const int j = sharers > 1 ? (int)threadIdx.x % items : j0 + (int)threadIdx.x, share = sharers > 1 ? (int)threadIdx.x / items : 0;
+    const int j = sharers > 1 ? (int)threadIdx.x % items : j0 + (int)threadIdx.x, first = sharers > 1 ? (int)threadIdx.x / items : 0;
+    const bool works = j < items && first < sharers;
+    const int h = works ? j / (D / 4) : 0, d = j % (D / 4) * 4;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int h = min(j, items - 1) / (D / 4), d = j % (D / 4) * 4;
-    const float2 all = join.total[h];
-    if (j < items && share < sharers)
-      for (int i0 = share; i0 < count; i0 += sharers * kAtOnce) {
+    float top = -INFINITY, total = 0.f;
+    if (works)
+      for (int i0 = first; i0 < count; i0 += sharers * kAtOnce) {
         float4 y[kAtOnce];
-        float m[kAtOnce];
+        float2 stat[kAtOnce];
 #pragma unroll
         for (int k = 0; k < kAtOnce; k++) {
           const int i = i0 + k * sharers;
-          m[k] = -INFINITY;
+          stat[k] = make_float2(-INFINITY, 0.f);
           if (i < count) {
-            m[k] = __ldcg(part(i) + H * D + 2 * h);
+            stat[k] = __ldcg(reinterpret_cast<const float2*>(part(i) + H * D + 2 * h));
             y[k] = __ldcg(reinterpret_cast<const float4*>(part(i) + j * 4));
           }
         }
+        float to = top;
+#pragma unroll
+        for (int k = 0; k < kAtOnce; k++) to = max_nan(to, stat[k].x);
+        const float keep = top == -INFINITY ? 0.f : exp2_fast(top - to);
+        x.x *= keep; x.y *= keep; x.z *= keep; x.w *= keep;
+        total *= keep;
+        top = to;
 #pragma unroll
         for (int k = 0; k < kAtOnce; k++)
-          if (m[k] != -INFINITY) {
-            const float f = exp2_fast(m[k] - all.x);
+          if (stat[k].x != -INFINITY) {
+            const float f = exp2_fast(stat[k].x - top);
+            total = fmaf(f, stat[k].y, total);
             x.x = fmaf(f, y[k].x, x.x);
             x.y = fmaf(f, y[k].y, x.y);
             x.z = fmaf(f, y[k].z, x.z);
@@ -668,15 +651,21 @@ __device__ __forceinline__ void merge(const AttendArgs& p, int b, int h0, int he
       }
     if (sharers > 1) {
       float4* sums = reinterpret_cast<float4*>(space);
+      float2* stats = reinterpret_cast<float2*>(sums + kThreads);
       sums[threadIdx.x] = x;
+      stats[threadIdx.x] = make_float2(top, total);
       __syncthreads();
-      if (share > 0 || (int)threadIdx.x >= items) continue;
+      if (first > 0 || !works) continue;
       for (int k = 1; k < sharers; k++) {
         const float4 y = sums[k * items + j];
-        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+        const float2 o = stats[k * items + j];
+        const float to = max_nan(top, o.x), f = top == -INFINITY ? 0.f : exp2_fast(top - to), e = o.x == -INFINITY ? 0.f : exp2_fast(o.x - to);
+        total = total * f + o.y * e;
+        x.x = x.x * f + y.x * e; x.y = x.y * f + y.y * e; x.z = x.z * f + y.z * e; x.w = x.w * f + y.w * e;
+        top = to;
       }
     }
-    if (j < items) finish(p, b, h0 + h, d, out + h * p.a.out_head_stride, x, all.x, all.y);
+    if (works) finish(p, b, h0 + h, d, out + h * p.a.out_head_stride, x, top, total);
   }
 }
 
@@ -794,7 +783,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) paged_attend_kernel(const __
       __syncthreads();
       if (join.last) {
         __threadfence();
-        merge<T, W, D>(p, now.b, g * p.rep + h0, heads, p.space.partials + first * 2 * kSlot, others + 1, out, join,
+        merge<T, W, D>(p, now.b, g * p.rep + h0, heads, p.space.partials + first * 2 * kSlot, others + 1, out,
                        smem + stage * Stage::kBytes);  // the first warp's sums have been read
       }
     }
