@@ -65,6 +65,8 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(PagedView 
 
 constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32;
 constexpr int kMoveThreads = 256;
+constexpr int kMoveHere = 64;
+constexpr int kMoveBatch = 512;
 
 // Weights in the order of unsigned integers: -0 as +0, NaN above all numbers, protected rows above NaN.
 __device__ __forceinline__ unsigned weight_key(float w, bool is_protected) {
@@ -74,64 +76,132 @@ __device__ __forceinline__ unsigned weight_key(float w, bool is_protected) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-// Copies the K and V rows of slot `from` to slot `to` of KV head g, one 16-byte piece of each per thread.
-__device__ __forceinline__ void move_row(const PagedView& c, int b, int g, int from, int to, int piece, int esize) {
-  const long long s = paged_row(c, b, from), d = paged_row(c, b, to);
-  if (s < 0 || d < 0) return;
-  const long long sa = (s + g * c.head_stride) * esize + piece * 16, da = (d + g * c.head_stride) * esize + piece * 16;
-  const uint4 k = *reinterpret_cast<const uint4*>(static_cast<const char*>(c.k) + sa);
-  const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const char*>(c.v) + sa);
-  *reinterpret_cast<uint4*>(static_cast<char*>(c.k) + da) = k;
-  *reinterpret_cast<uint4*>(static_cast<char*>(c.v) + da) = v;
-}
+// Where a row moves from and to, as byte offsets of its KV head's elements in either pool; to < 0: one of the two has no page.
+struct Move {
+  long long from, to;
+};
+
+// 32 rows: which of them stay, and how many dropped rows before `keep` and kept rows from `keep` on there are before them.
+struct Word {
+  unsigned kept;
+  int holes, sources;
+};
 
 // Workspace of evict: per sequence an arrival counter, per (sequence, KV head) the number of moves, then the moves.
 struct EvictSpace {
   unsigned* arrivals;  // [batch]
   int* moves;          // [batch * kv_heads]
-  int2* list;          // [batch * kv_heads][list_max] (from, to)
-  long long list_max;
+  Move* list;          // [batch * kv_heads][list_max]
+  Word* words;         // [batch * kv_heads][words_max], where shared memory does not hold them
+  long long list_max, words_max;
 };
 
-__host__ __device__ inline long long evict_list_max(const PagedView& c) { return (long long)c.page_size * c.max_pages / 2 + 1; }
+// Rows whose keys, and their words, a block has in shared memory.
+constexpr long long kRowsInShared = 40 * 1024;
+
+struct EvictLayout {
+  uint64_t moves, list, words, bytes;
+  long long list_max, words_max;
+};
 
 // Places go by the largest batch, so that the counters stay where they are.
-inline EvictSpace evict_space(const PagedView& c, void* workspace) {
-  EvictSpace s;
-  const uint64_t head = ((uint64_t)c.batch_max * 4 + 255) / 256 * 256, counts = ((uint64_t)c.batch_max * c.kv_heads * 4 + 255) / 256 * 256;
-  char* p = static_cast<char*>(workspace);
-  s.arrivals = reinterpret_cast<unsigned*>(p);
-  s.moves = reinterpret_cast<int*>(p + head);
-  s.list = reinterpret_cast<int2*>(p + head + counts);
-  s.list_max = evict_list_max(c);
-  return s;
+inline EvictLayout evict_layout(const PagedView& c) {
+  EvictLayout l;
+  const uint64_t pairs = (uint64_t)c.batch_max * c.kv_heads;
+  l.list_max = c.capacity() / 2 + 1;
+  l.words_max = c.capacity() > kRowsInShared ? c.capacity() / 32 + 1 : 0;
+  l.moves = ((uint64_t)c.batch_max * 4 + 255) / 256 * 256;
+  l.list = l.moves + (pairs * 4 + 255) / 256 * 256;
+  l.words = l.list + pairs * l.list_max * sizeof(Move);
+  l.bytes = l.words + pairs * l.words_max * sizeof(Word);
+  return l;
 }
 
-// Block-wide exclusive prefix over the warps of one value per warp; `total` gets the sum. All threads call it.
-__device__ __forceinline__ int warp_prefix(int value, int* buffer, int* total) {
+inline EvictSpace evict_space(const PagedView& c, void* workspace) {
+  const EvictLayout l = evict_layout(c);
+  char* p = static_cast<char*>(workspace);
+  return {reinterpret_cast<unsigned*>(p), reinterpret_cast<int*>(p + l.moves), reinterpret_cast<Move*>(p + l.list),
+          reinterpret_cast<Word*>(p + l.words), l.list_max, l.words_max};
+}
+
+// Copies the rows of moves 0..count-1, `lanes` (a power of two) threads a row, kMoveUnroll rows of each in flight.
+constexpr int kMoveUnroll = 4;
+__device__ __forceinline__ void move_rows(const PagedView& c, const Move* list, int count, int pieces, int lanes, int first, int step) {
+  const int piece = threadIdx.x & (lanes - 1);
+  if (piece >= pieces) return;
+  for (int i0 = first; i0 < count; i0 += step * kMoveUnroll) {
+    Move m[kMoveUnroll];
+    uint4 k[kMoveUnroll], v[kMoveUnroll];
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; u++) {
+      m[u].to = -1;
+      if (i0 + u * step < count) m[u] = list[i0 + u * step];
+    }
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; u++)
+      if (m[u].to >= 0) {
+        k[u] = *reinterpret_cast<const uint4*>(static_cast<const char*>(c.k) + m[u].from + piece * 16);
+        v[u] = *reinterpret_cast<const uint4*>(static_cast<const char*>(c.v) + m[u].from + piece * 16);
+      }
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; u++)
+      if (m[u].to >= 0) {
+        *reinterpret_cast<uint4*>(static_cast<char*>(c.k) + m[u].to + piece * 16) = k[u];
+        *reinterpret_cast<uint4*>(static_cast<char*>(c.v) + m[u].to + piece * 16) = v[u];
+      }
+  }
+}
+
+// Exclusive sums of two values over the threads of the block, and the totals. One barrier; `step` alternates between calls, so
+// that a buffer is written again only behind the next one.
+struct Sums {
+  int2 buffer[2][kSelectWarps];
+};
+struct Before {
+  int a, b, all_a, all_b;
+};
+__device__ __forceinline__ Before block_before(Sums& s, int& step, int a, int b) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  __syncthreads();
-  if (lane == 0) buffer[warp] = value;
-  __syncthreads();
-  int v = buffer[lane < kSelectWarps ? lane : 0], sum = v;
+  int x = a, y = b;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
-    const int o = __shfl_up_sync(~0u, sum, d);
-    if (lane >= d) sum += o;
+    const int u = __shfl_up_sync(~0u, x, d), v = __shfl_up_sync(~0u, y, d);
+    if (lane >= d) {
+      x += u;
+      y += v;
+    }
   }
-  *total = __shfl_sync(~0u, sum, 31);
-  return __shfl_sync(~0u, sum - v, warp);
+  int2* buffer = s.buffer[step++ & 1];
+  if (lane == 31) buffer[warp] = make_int2(x, y);
+  __syncthreads();
+  const int2 v = buffer[lane];
+  Before r;
+  r.all_a = __reduce_add_sync(~0u, v.x);
+  r.all_b = __reduce_add_sync(~0u, v.y);
+  r.a = x - a + __reduce_add_sync(~0u, lane < warp ? v.x : 0);
+  r.b = y - b + __reduce_add_sync(~0u, lane < warp ? v.y : 0);
+  return r;
 }
+static_assert(kSelectWarps == 32, "a lane for every warp");
 
-// One block per (sequence, KV head). The threshold - the keep-th largest key - is found two bits at a time by counting the keys
-// at or above three candidates; a warp owns a contiguous range of rows, so ranks within it are ballots and one prefix over
-// the warps orders the rest.
+constexpr int kDigitBits = 11;
+
+struct SelectShared {
+  union {
+    int histogram[1 << kDigitBits];
+    Move moves[kMoveBatch];  // when the threshold is known
+  };
+  Sums sums;
+  int digit, need;
+};
+
+// One block per (sequence, KV head). The threshold - the keep-th largest key - comes from three histograms of 11, 11 and 10 bits,
+// each over the keys that share the digits found so far. Then every 32 rows become a word of bits, the words' counts are added
+// up by a thread each, and the rows that move are listed by a warp a word.
 __global__ void __launch_bounds__(kSelectThreads) paged_evict_select_kernel(PagedView c, PagedEvict e, EvictSpace space, int pieces,
-                                                                            int esize, int keys_in_smem, int move_here) {
+                                                                            int lanes, int esize, int in_shared, int move_here) {
   extern __shared__ unsigned keys[];
-  __shared__ int buffer[kSelectWarps];
-  __shared__ int counts[16][4];
-  __shared__ int last;
+  __shared__ SelectShared sh;
   PJRTX_PDL_PROLOGUE();
   const int g = blockIdx.x, b = blockIdx.y;
   const int pair = b * c.kv_heads + g;
@@ -148,98 +218,125 @@ __global__ void __launch_bounds__(kSelectThreads) paged_evict_select_kernel(Page
   int moves = 0;
   if (n > keep) {
     const int newest = c.tokens[b] - e.recent;
-    auto key_of = [&](int t) {
-      const int p = positions[t];
-      return weight_key(weights[t], p < e.sinks || p >= newest);
-    };
-    if (threadIdx.x < 64) counts[threadIdx.x / 4][threadIdx.x % 4] = 0;
-    if (keys_in_smem)
-      for (int t = threadIdx.x; t < n; t += kSelectThreads) keys[t] = key_of(t);
-    auto key_at = [&](int t) { return keys_in_smem ? keys[t] : key_of(t); };
-    __syncthreads();
-    unsigned threshold = 0;
-    for (int step = 0; step < 16; step++) {
-      const int shift = 30 - 2 * step;
-      const unsigned c1 = threshold | (1u << shift), c2 = threshold | (2u << shift), c3 = threshold | (3u << shift);
-      int n1 = 0, n2 = 0, n3 = 0;
+    auto key_of = [&](float w, int p) { return weight_key(w, p < e.sinks || p >= newest); };
+    auto key_at = [&](int t) { return in_shared ? keys[t] : key_of(weights[t], positions[t]); };
+    if (in_shared) {
+      constexpr int U = 8;
+      for (int t0 = threadIdx.x; t0 < n; t0 += U * kSelectThreads) {
+        float w[U];
+        int p[U];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+          if (t0 + u * kSelectThreads < n) {
+            w[u] = weights[t0 + u * kSelectThreads];
+            p[u] = positions[t0 + u * kSelectThreads];
+          }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+          if (t0 + u * kSelectThreads < n) keys[t0 + u * kSelectThreads] = key_of(w[u], p[u]);
+      }
+    }
+    unsigned threshold = 0;  // its digits so far
+    int need = keep, step = 0;  // how many of the keys that share them stay
+    for (int shift = 32, bits = kDigitBits; shift > 0;) {
+      bits = min(kDigitBits, shift);
+      shift -= bits;
+      const int size = 1 << bits;
+      for (int i = threadIdx.x; i < size; i += kSelectThreads) sh.histogram[i] = 0;
+      __syncthreads();
+#pragma unroll 4
       for (int t = threadIdx.x; t < n; t += kSelectThreads) {
         const unsigned k = key_at(t);
-        n1 += k >= c1;
-        n2 += k >= c2;
-        n3 += k >= c3;
-      }
-      n1 = __reduce_add_sync(~0u, n1);
-      n2 = __reduce_add_sync(~0u, n2);
-      n3 = __reduce_add_sync(~0u, n3);
-      if (lane == 0) {
-        atomicAdd(&counts[step][1], n1);
-        atomicAdd(&counts[step][2], n2);
-        atomicAdd(&counts[step][3], n3);
+        if (shift + bits == 32 || k >> (shift + bits) == threshold) atomicAdd(&sh.histogram[k >> shift & (size - 1)], 1);
       }
       __syncthreads();
-      threshold = counts[step][3] >= keep ? c3 : counts[step][2] >= keep ? c2 : counts[step][1] >= keep ? c1 : threshold;
-    }
-    // Rows above the threshold stay, and of those at it the first ones.
-    const int range = ((n + kSelectWarps - 1) / kSelectWarps + 31) / 32 * 32;
-    const int begin = min(n, warp * range), end = min(n, begin + range);
-    int above = 0, equal = 0;
-    for (int t0 = begin; t0 < end; t0 += 32) {
-      const unsigned k = t0 + lane < end ? key_at(t0 + lane) : 0u;
-      const bool in = t0 + lane < end;
-      above += __popc(__ballot_sync(~0u, in && k > threshold));
-      equal += __popc(__ballot_sync(~0u, in && k == threshold));
-    }
-    int all_above, ignored;
-    warp_prefix(above, buffer, &all_above);
-    const int equal_before = warp_prefix(equal, buffer, &ignored);
-    const int equal_kept = keep - all_above;
-    auto walk = [&](auto&& row) {  // row(t, kept, ballot of dropped rows before `keep`, ballot of kept rows from `keep` on)
-      int rank = equal_before;
-      for (int t0 = begin; t0 < end; t0 += 32) {
-        const int t = t0 + lane;
-        const bool in = t < end;
-        const unsigned k = in ? key_at(t) : 0u;
-        const unsigned same = __ballot_sync(~0u, in && k == threshold);
-        const bool kept = in && (k > threshold || (k == threshold && rank + __popc(same & ((1u << lane) - 1)) < equal_kept));
-        rank += __popc(same);
-        const unsigned hole = __ballot_sync(~0u, in && !kept && t < keep), source = __ballot_sync(~0u, kept && t >= keep);
-        row(t, kept, hole, source);
+      const int high = size - 1 - 2 * (int)threadIdx.x;  // two digits a thread, the largest ones first
+      const int at_high = high > 0 ? sh.histogram[high] : 0, at_low = high > 0 ? sh.histogram[high - 1] : 0;
+      const int before = block_before(sh.sums, step, at_high + at_low, 0).a;
+      if (before < need && need <= before + at_high + at_low) {
+        const bool first = need <= before + at_high;
+        sh.digit = first ? high : high - 1;
+        sh.need = need - before - (first ? 0 : at_high);
       }
-    };
-    int holes = 0, sources = 0;
-    walk([&](int, bool, unsigned hole, unsigned source) {
-      holes += __popc(hole);
-      sources += __popc(source);
-    });
-    int hole_at = warp_prefix(holes, buffer, &moves);
-    int source_at = warp_prefix(sources, buffer, &ignored);
-    int2* list = space.list + pair * space.list_max;
-    walk([&](int t, bool kept, unsigned hole, unsigned source) {
-      const unsigned before = (1u << lane) - 1;
-      if (hole >> lane & 1) list[hole_at + __popc(hole & before)].y = t;
-      if (source >> lane & 1) list[source_at + __popc(source & before)].x = t;
-      if (kept && t < keep) {
-        const float w = weights[t];
-        const int p = positions[t];
-        weights_out[t] = w;
-        positions_out[t] = p;
+      __syncthreads();
+      threshold = threshold << bits | (unsigned)sh.digit;
+      need = sh.need;
+    }
+    // Rows above the threshold stay, and of those at it the first `need`.
+    const int words = (n + 31) / 32;
+    Word* word = in_shared ? reinterpret_cast<Word*>(keys + (capacity + 3) / 4 * 4) : space.words + pair * space.words_max;
+#pragma unroll 4
+    for (int i = warp; i < words; i += kSelectWarps) {
+      const int t = i * 32 + lane;
+      const unsigned k = t < n ? key_at(t) : 0u;
+      const unsigned above = __ballot_sync(~0u, t < n && k > threshold), equal = __ballot_sync(~0u, t < n && k == threshold);
+      if (lane == 0) {
+        word[i].kept = above;
+        word[i].holes = (int)equal;
       }
-      hole_at += __popc(hole);
-      source_at += __popc(source);
-    });
+    }
     __syncthreads();
-    for (int i = threadIdx.x; i < moves; i += kSelectThreads) {
-      const int2 m = list[i];
-      const float w = weights[m.x];
-      const int p = positions[m.x];
-      weights_out[m.y] = w;
-      positions_out[m.y] = p;
-    }
-    if (move_here)
-      for (long long i = threadIdx.x; i < (long long)moves * pieces; i += kSelectThreads) {
-        const int2 m = list[i / pieces];
-        move_row(c, b, g, m.x, m.y, (int)(i % pieces), esize);
+    int equals = 0, holes = 0, sources = 0;  // of the words so far
+    for (int i0 = 0; i0 < words; i0 += kSelectThreads) {
+      const int i = i0 + (int)threadIdx.x;
+      unsigned kept = 0, equal = 0;
+      if (i < words) {
+        kept = word[i].kept;
+        equal = (unsigned)word[i].holes;
       }
+      const Before same = block_before(sh.sums, step, __popc(equal), 0);
+      int room = need - equals - same.a;
+      for (; equal && room > 0; room--) {
+        kept |= equal & -equal;
+        equal &= equal - 1;
+      }
+      const int first = i * 32;
+      const unsigned in = first >= n ? 0u : n - first >= 32 ? ~0u : (1u << (n - first)) - 1;
+      const unsigned front = first >= keep ? 0u : keep - first >= 32 ? ~0u : (1u << (keep - first)) - 1;
+      const Before listed = block_before(sh.sums, step, __popc(~kept & in & front), __popc(kept & ~front));
+      if (i < words) word[i] = {kept, holes + listed.a, sources + listed.b};
+      equals += same.all_a;
+      holes += listed.all_a;
+      sources += listed.all_b;
+    }
+    moves = holes;
+    __syncthreads();
+    Move* list = space.list + pair * space.list_max;
+#pragma unroll 2
+    for (int i = warp; i < words; i += kSelectWarps) {  // rows first, their places in the pools behind the barrier
+      const Word x = word[i];
+      const int t = i * 32 + lane;
+      const bool kept = x.kept >> lane & 1, front = t < keep;
+      const unsigned hole = __ballot_sync(~0u, t < n && !kept && front), source = __ballot_sync(~0u, kept && !front);
+      const unsigned before = (1u << lane) - 1;
+      if (hole >> lane & 1) list[x.holes + __popc(hole & before)].to = t;
+      if (source >> lane & 1) list[x.sources + __popc(source & before)].from = t;
+      if (kept && front) {
+        if (weights_out != weights) weights_out[t] = weights[t];
+        if (positions_out != positions) positions_out[t] = positions[t];
+      }
+    }
+    __syncthreads();
+    for (int i0 = 0; i0 < moves; i0 += kMoveBatch) {
+      const int i = i0 + (int)threadIdx.x;
+      if ((int)threadIdx.x < kMoveBatch && i < moves) {
+        Move m = list[i];
+        const float w = weights[m.from];
+        const int p = positions[m.from];
+        const long long from = paged_row(c, b, (int)m.from), to = paged_row(c, b, (int)m.to);
+        weights_out[m.to] = w;
+        positions_out[m.to] = p;
+        m.from = (from + g * c.head_stride) * esize;
+        m.to = from < 0 || to < 0 ? -1 : (to + g * c.head_stride) * esize;
+        if (move_here) sh.moves[threadIdx.x] = m;
+        else list[i] = m;
+      }
+      if (move_here) {
+        __syncthreads();
+        move_rows(c, sh.moves, min(kMoveBatch, moves - i0), pieces, lanes, (int)threadIdx.x / lanes, kSelectThreads / lanes);
+        __syncthreads();
+      }
+    }
     __syncthreads();
   } else {
     for (int t = threadIdx.x; t < n; t += kSelectThreads) {
@@ -257,22 +354,16 @@ __global__ void __launch_bounds__(kSelectThreads) paged_evict_select_kernel(Page
   if (threadIdx.x == 0) {
     space.moves[pair] = moves;
     __threadfence();
-    last = atomicInc(&space.arrivals[b], (unsigned)c.kv_heads - 1) == (unsigned)c.kv_heads - 1;
-    if (last) e.lengths_out[b] = left;
+    if (atomicInc(&space.arrivals[b], (unsigned)c.kv_heads - 1) == (unsigned)c.kv_heads - 1) e.lengths_out[b] = left;
   }
 }
 
-// The rows of all moves, a group of `pieces` threads a row.
-__global__ void __launch_bounds__(kMoveThreads) paged_evict_move_kernel(PagedView c, EvictSpace space, int pieces, int esize) {
-  PJRTX_PDL_PROLOGUE();
-  const int g = blockIdx.y, b = blockIdx.z;
-  const int pair = b * c.kv_heads + g;
-  const long long total = (long long)space.moves[pair] * pieces;
-  const int2* list = space.list + pair * space.list_max;
-  for (long long i = (long long)blockIdx.x * kMoveThreads + threadIdx.x; i < total; i += (long long)gridDim.x * kMoveThreads) {
-    const int2 m = list[i / pieces];
-    move_row(c, b, g, m.x, m.y, (int)(i % pieces), esize);
-  }
+// The rows of all moves. It lets the next kernel of the stream start only as it ends: blocks that wait would take its place.
+__global__ void __launch_bounds__(kMoveThreads) paged_evict_move_kernel(PagedView c, EvictSpace space, int pieces, int lanes) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int pair = blockIdx.z * c.kv_heads + blockIdx.y;
+  const int rows = kMoveThreads / lanes;
+  move_rows(c, space.list + pair * space.list_max, space.moves[pair], pieces, lanes, blockIdx.x * rows + threadIdx.x / lanes, gridDim.x * rows);
 }
 
 }  // namespace
@@ -285,28 +376,26 @@ int paged_append_launch(const PagedView& c, const PagedAppend& a, bool pdl, cuda
                        stream, pdl, c, a, pieces, esize) == cudaSuccess;
 }
 
-uint64_t paged_evict_workspace_bytes(const PagedView& c) {
-  const uint64_t head = ((uint64_t)c.batch_max * 4 + 255) / 256 * 256, counts = ((uint64_t)c.batch_max * c.kv_heads * 4 + 255) / 256 * 256;
-  return head + counts + (uint64_t)c.batch_max * c.kv_heads * evict_list_max(c) * sizeof(int2);
-}
+uint64_t paged_evict_workspace_bytes(const PagedView& c) { return evict_layout(c).bytes; }
 
 int paged_evict_launch(const PagedView& c, const PagedEvict& e, int sm_count, bool pdl, cudaStream_t stream) {
   const int esize = (int)dtype_size(c.dtype), pieces = c.head_dim * esize / 16;
+  int lanes = 1;
+  while (lanes < pieces) lanes *= 2;
   const EvictSpace space = evict_space(c, e.workspace);
-  const long long capacity = c.capacity();
-  constexpr int kKeyBytesMax = 192 * 1024;
-  const int in_smem = capacity * 4 <= kKeyBytesMax;
-  if (!raise_smem_limit((const void*)paged_evict_select_kernel, kKeyBytesMax)) return 0;
+  const long long capacity = c.capacity(), pairs = (long long)c.batch * c.kv_heads;
+  const int in_shared = capacity <= kRowsInShared;
+  const size_t smem = in_shared ? (size_t)(capacity + 3) / 4 * 16 + (size_t)(capacity / 32 + 1) * sizeof(Word) : 0;
+  if (!raise_smem_limit((const void*)paged_evict_select_kernel, (int)(kRowsInShared * 4 + (kRowsInShared / 32 + 1) * sizeof(Word)))) return 0;
   const long long moves_max = std::min<long long>(e.keep, capacity - e.keep);
-  const int move_here = moves_max <= 64;
+  const int move_here = moves_max <= kMoveHere || pairs >= sm_count / 2;
   if (launch_kernel(paged_evict_select_kernel, dim3((unsigned)c.kv_heads, (unsigned)c.batch), dim3(kSelectThreads),
-                    in_smem ? (size_t)capacity * 4 : 0, stream, pdl, c, e, space, pieces, esize, in_smem, move_here) != cudaSuccess)
+                    smem, stream, pdl, c, e, space, pieces, lanes, esize, in_shared, move_here) != cudaSuccess)
     return 0;
   if (move_here || moves_max <= 0) return 1;
-  const long long pairs = (long long)c.batch * c.kv_heads;
-  const long long blocks = std::max<long long>(1, std::min((moves_max * pieces + kMoveThreads - 1) / kMoveThreads, 8ll * sm_count / pairs + 1));
+  const long long blocks = std::max<long long>(1, std::min((moves_max * lanes + kMoveThreads - 1) / kMoveThreads, 8ll * sm_count / pairs + 1));
   if (launch_kernel(paged_evict_move_kernel, dim3((unsigned)blocks, (unsigned)c.kv_heads, (unsigned)c.batch), dim3(kMoveThreads), 0, stream,
-                    true, c, space, pieces, esize) != cudaSuccess)
+                    true, c, space, pieces, lanes) != cudaSuccess)
     return 0;
   return 2;
 }
