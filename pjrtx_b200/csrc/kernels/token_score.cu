@@ -208,8 +208,10 @@ __device__ __forceinline__ Stats joined(Stats a, Stats b, float c) {
 
 // ---- forward -------------------------------------------------------------------------------------------------------
 
-constexpr int kScoreThreads = 256, kScoreWarps = kScoreThreads / 32;
-constexpr int kScorePerSm = 4;
+// Threads of a block. Small ones where there are rows enough to fill the GPU with them: eight share an SM, so that what one row's
+// alternatives wait for is hidden by seven others (4096 rows of 128256 bf16 logits, 5 alternatives: 185 us, 193 with four blocks of
+// 256); where a cluster has one row, larger ones (one row: 8.7 us, 10.3 with 128).
+constexpr int kScoreThreadsMany = 128, kScoreThreadsFew = 256, kScoreThreadsOfSm = 1024;
 constexpr int kScoreVectors = 4;  // 16-byte loads of a batch; the next batch's are in flight while one is added up
 constexpr int kChunk = 256;       // logits
 constexpr int kScoreClusterMax = 8;
@@ -306,7 +308,7 @@ __device__ __forceinline__ void select(Get&& get, int n, int k, Entry* out, Entr
 }
 
 struct ScoreShared {
-  Stats stats[kScoreWarps];
+  Stats stats[kScoreThreadsFew / 32];
   Stats cluster_stats[kScoreClusterMax];                    // of the rank-0 block
   Entry cluster_top[kScoreClusterMax * kScoreTopMax];       // of the rank-0 block
   Entry chosen[kScoreTopMax], spare[kFew];
@@ -319,12 +321,13 @@ __device__ __forceinline__ float warp_max(float x) {
   return y;
 }
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(kScoreThreads, kScorePerSm) token_score_kernel(TokenScore a, int segment_chunks) {
+template <typename T, bool TOP, int THREADS>
+__global__ void __launch_bounds__(THREADS, kScoreThreadsOfSm / THREADS) token_score_kernel(TokenScore a, int segment_chunks) {
+  constexpr int kScoreWarps = THREADS / 32;
   constexpr int V = Logit<T>::V;
   constexpr int kVectorsOfChunk = kChunk / (32 * V);              // 16-byte loads a thread has of a chunk
   constexpr int kChunks = kScoreVectors / kVectorsOfChunk;        // chunks of a batch
-  extern __shared__ Entry list[];                                 // TOP: vectors, then elements, of a round
+  extern __shared__ Entry list[];                                            // TOP: vectors, or elements, of the chosen chunks
   float* chunk_max = reinterpret_cast<float*>(list + a.top * (kChunk / V));  // TOP: of this block's chunks
   __shared__ ScoreShared sh;
   PJRTX_PDL_PROLOGUE();
@@ -466,10 +469,11 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm) token_score_kernel
     const int k = a.top, n = chunk1 - chunk0;
     if (warp == 0) select([&](int i) { return entry(order_key(chunk_max[i]), (unsigned)i); }, n, k, sh.chosen, sh.spare);
     __syncthreads();
-    {  // vectors of the chosen chunks that reach the last of their maxima
-      const unsigned bound = n < k ? 0u : (unsigned)(sh.chosen[k - 1] >> 32);
-      for (int j = warp; j < k; j += kScoreWarps) {
-        if (sh.chosen[j] == 0) break;
+    // What reaches the last of their maxima: elements at once where they are few, else vectors first and then theirs.
+    const unsigned bound = n < k ? 0u : (unsigned)(sh.chosen[k - 1] >> 32);
+    const int room = k * (kChunk / V);  // all their vectors
+    auto gather = [&](bool elements) {
+      for (int j = warp; j < k && sh.chosen[j] != 0; j += kScoreWarps) {
         const int chunk = chunk0 + (int)position_of(sh.chosen[j]);
 #pragma unroll
         for (int u = 0; u < kVectorsOfChunk; u++) {
@@ -477,28 +481,49 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm) token_score_kernel
           if (p >= end || p + V <= shift) continue;
           const uint4 r = load(p);
           const unsigned key = order_key(Logit<T>::template highest<1>(&r));
-          if (key >= bound) list[atomicAdd(&sh.n, 1)] = entry(key, (unsigned)p);
+          if (key < bound) continue;
+          if (!elements) {
+            list[atomicAdd(&sh.n, 1)] = entry(key, (unsigned)p);
+            continue;
+          }
+          float f[V];
+          Logit<T>::unpack(r, f);
+#pragma unroll
+          for (int i = 0; i < V; i++) {
+            const unsigned x = order_key(f[i]);
+            if (x < bound || p + i < shift || p + i >= end) continue;
+            const int at = atomicAdd(&sh.n, 1);
+            if (at < room) list[at] = entry(x, (unsigned)(p + i - shift));
+          }
         }
       }
-    }
+    };
+    gather(true);
     __syncthreads();
-    const int vectors = sh.n;
-    __syncthreads();
-    if (threadIdx.x == 0) sh.n = 0;
-    if (warp == 0) select([&](int i) { return list[i]; }, vectors, k, sh.chosen, sh.spare);
-    __syncthreads();
-    if ((int)threadIdx.x < k && sh.chosen[threadIdx.x] != 0) {  // their elements
-      const unsigned bound = vectors < k ? 0u : (unsigned)(sh.chosen[k - 1] >> 32);
-      const int p = (int)position_of(sh.chosen[threadIdx.x]);
-      float f[V];
-      Logit<T>::unpack(load(p), f);
+    if (sh.n > room) {  // long ties
+      __syncthreads();
+      if (threadIdx.x == 0) sh.n = 0;
+      __syncthreads();
+      gather(false);
+      __syncthreads();
+      const int vectors = sh.n;
+      __syncthreads();
+      if (threadIdx.x == 0) sh.n = 0;
+      if (warp == 0) select([&](int i) { return list[i]; }, vectors, k, sh.chosen, sh.spare);
+      __syncthreads();
+      if ((int)threadIdx.x < k && sh.chosen[threadIdx.x] != 0) {
+        const unsigned limit = vectors < k ? 0u : (unsigned)(sh.chosen[k - 1] >> 32);
+        const int p = (int)position_of(sh.chosen[threadIdx.x]);
+        float f[V];
+        Logit<T>::unpack(load(p), f);
 #pragma unroll
-      for (int i = 0; i < V; i++) {
-        const unsigned key = order_key(f[i]);
-        if (p + i >= shift && p + i < end && key >= bound) list[atomicAdd(&sh.n, 1)] = entry(key, (unsigned)(p + i - shift));
+        for (int i = 0; i < V; i++) {
+          const unsigned key = order_key(f[i]);
+          if (p + i >= shift && p + i < end && key >= limit) list[atomicAdd(&sh.n, 1)] = entry(key, (unsigned)(p + i - shift));
+        }
       }
+      __syncthreads();
     }
-    __syncthreads();
     if (warp == 0) select([&](int i) { return list[i]; }, sh.n, k, cluster.map_shared_rank(&sh, 0)->cluster_top + rank * k, sh.spare);
   }
   cluster.sync();
@@ -599,21 +624,21 @@ __global__ void __launch_bounds__(kGradThreads) token_score_grad_kernel(TokenSco
   }
 }
 
-template <typename T>
-int score_launch(const TokenScore& s, int sm_count, bool pdl, cudaStream_t stream) {
+template <typename T, int THREADS>
+int score_launch_of(const TokenScore& s, int sm_count, bool pdl, cudaStream_t stream) {
   const int chunks = (int)((s.vocab + Logit<T>::V - 1 + kChunk - 1) / kChunk);
   // A cluster for each row: as many blocks as fill the GPU, none with less than a batch for every warp.
-  const int batch_chunks = kScoreWarps * kScoreVectors * 32 * Logit<T>::V / kChunk;
+  const int batch_chunks = THREADS * kScoreVectors * Logit<T>::V / kChunk;
   int ranks = 1;
-  while (ranks < kScoreClusterMax && s.rows * ranks < (long long)kScorePerSm * sm_count && chunks > ranks * batch_chunks) ranks *= 2;
+  while (ranks < kScoreClusterMax && s.rows * ranks * THREADS < (long long)kScoreThreadsOfSm * sm_count && chunks > ranks * batch_chunks) ranks *= 2;
   const int segment = (chunks + ranks - 1) / ranks;
   const bool top = s.top > 0;
   const size_t smem = top ? (size_t)s.top * (kChunk / Logit<T>::V) * sizeof(Entry) + (size_t)segment * sizeof(float) : 0;
-  auto kernel = top ? token_score_kernel<T, true> : token_score_kernel<T, false>;
+  auto kernel = top ? token_score_kernel<T, true, THREADS> : token_score_kernel<T, false, THREADS>;
   if (smem > 32 * 1024 && !raise_smem_limit((const void*)kernel, 200 * 1024)) return 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(s.rows * ranks));
-  cfg.blockDim = dim3(kScoreThreads);
+  cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[3];
@@ -623,6 +648,12 @@ int score_launch(const TokenScore& s, int sm_count, bool pdl, cudaStream_t strea
   cfg.numAttrs++;
   cfg.attrs = attr;
   return cudaLaunchKernelEx(&cfg, kernel, s, segment) == cudaSuccess;
+}
+
+template <typename T>
+int score_launch(const TokenScore& s, int sm_count, bool pdl, cudaStream_t stream) {
+  return s.rows * kScoreThreadsMany >= (long long)kScoreThreadsOfSm * sm_count ? score_launch_of<T, kScoreThreadsMany>(s, sm_count, pdl, stream)
+                                                                               : score_launch_of<T, kScoreThreadsFew>(s, sm_count, pdl, stream);
 }
 
 template <typename T>
