@@ -39,12 +39,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 // ---- division of the work ------------------------------------------------------------------------------------------
-// A unit is a tile of 64 rows of one (sequence, KV head, group of query heads). Units are numbered in that order, only those
+// A unit is a tile of 96 rows of one (sequence, KV head, group of query heads). Units are numbered in that order, only those
 // that the lengths call for, and every block takes the same number of consecutive ones: lengths are device data, so each block
 // adds them up itself. What belongs to one (sequence, head group) is a segment; where several blocks share one, each leaves
 // (max, sum, values) in its slot of the workspace and the block that arrives last joins them in block order.
 
-constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kWarps = 6, kThreads = kWarps * 32;
 constexpr int kWarpRows = 16, kTileRows = kWarps * kWarpRows;
 
 struct AttendSpace {
@@ -185,9 +185,16 @@ __device__ __forceinline__ RowPlace locate(const AttendArgs& p, const Cursor& u)
 
 __device__ __forceinline__ unsigned long long address_of(const void* p) { return reinterpret_cast<unsigned long long>(p); }
 
-// Requests the rows of `u`; the stage's mask word says which ones count.
+// What a warp knows of a stage besides the rows.
+struct StageNote {
+  unsigned mask;             // rows that count
+  int fresh;                 // the row that came with the call and goes to the pool, -1: none
+  unsigned long long store;  // where its key goes
+};
+
+// Requests the rows of `u`.
 template <typename T, int D>
-__device__ __forceinline__ void request(const AttendArgs& p, const Cursor& u, const RowPlace& r, char* stage, unsigned* mask) {
+__device__ __forceinline__ void request(const AttendArgs& p, const Cursor& u, const RowPlace& r, char* stage, StageNote* note) {
   using S = RowStage<T, D>;
   constexpr int kPieces = D * (int)sizeof(T) / 16, kAcross = 8;  // eight lanes beside each other on one row
   const int lane = threadIdx.x % 32, g = u.group / p.groups;
@@ -203,19 +210,17 @@ __device__ __forceinline__ void request(const AttendArgs& p, const Cursor& u, co
     const long long at = (u.b * p.a.new_batch_stride + g * p.a.new_head_stride) * (long long)sizeof(T);
     const char* k_new = static_cast<const char*>(p.a.k_new) + at;
     const char* v_new = static_cast<const char*>(p.a.v_new) + at;
-    const unsigned long long to = __shfl_sync(~0u, k, fresh);
-    if (to && u.group % p.groups == 0)
-      for (int i = lane; i < p.pieces; i += 32) {
-        reinterpret_cast<uint4*>(to)[i] = reinterpret_cast<const uint4*>(k_new)[i];
-        reinterpret_cast<uint4*>(to + apart_pools)[i] = reinterpret_cast<const uint4*>(v_new)[i];
-      }
     if ((lane & 15) == fresh && k) {
+      if (lane < 16) note->store = k;
       k = address_of(k_new);
       apart = address_of(v_new) - k;
     }
   }
   const unsigned there = __ballot_sync(~0u, k != 0) & 0xffffu;
-  if (lane == 0) *mask = there;
+  if (lane == 0) {
+    note->mask = there;
+    note->fresh = has_fresh && (there >> fresh & 1) && u.group % p.groups == 0 ? fresh : -1;
+  }
   const unsigned to = (unsigned)__cvta_generic_to_shared(stage) + lane / kAcross * S::kPitch + lane % kAcross * 16;
   const bool whole = there == 0xffffu && p.pieces == kPieces;
 #pragma unroll
@@ -240,6 +245,18 @@ __device__ __forceinline__ void request(const AttendArgs& p, const Cursor& u, co
         copy16_or_zero(to + (kWarpRows + j * (32 / kAcross)) * S::kPitch + i * kAcross * 16, in ? vr + i * kAcross * 16 : address_of(p.c.v), in);
       }
     }
+  }
+}
+
+// Stores the row that came with the call from its stage into the pool.
+template <typename T, int D>
+__device__ __forceinline__ void store_fresh(const AttendArgs& p, const StageNote& note, const char* stage) {
+  if (note.fresh < 0) return;
+  const char* from = stage + note.fresh * RowStage<T, D>::kPitch;
+  char* to = reinterpret_cast<char*>(note.store);
+  for (int i = threadIdx.x % 32; i < p.pieces; i += 32) {
+    reinterpret_cast<uint4*>(to)[i] = reinterpret_cast<const uint4*>(from)[i];
+    reinterpret_cast<uint4*>(to + (address_of(p.c.v) - address_of(p.c.k)))[i] = reinterpret_cast<const uint4*>(from + kWarpRows * RowStage<T, D>::kPitch)[i];
   }
 }
 
@@ -294,7 +311,8 @@ struct MmaWarp {
   float o[D / 16][NB][4];
   float m[NB][2], l[NB][2];
 
-  __device__ __forceinline__ void start(const AttendArgs& p, const Cursor& u, char*) {
+  // Requests the queries of a segment; nothing else of the one before is touched.
+  __device__ __forceinline__ void load(const AttendArgs& p, const Cursor& u) {
     const int lane = threadIdx.x % 32, g = u.group / p.groups, h0 = (u.group % p.groups) * kHeads;
 #pragma unroll
     for (int n = 0; n < NB; n++) {
@@ -307,6 +325,11 @@ struct MmaWarp {
           const int d = i * 16 + j * 8 + (lane % 4) * 2;
           q[i][n][j] = h < p.rep && d < p.c.head_dim ? *reinterpret_cast<const unsigned*>(from + d) : 0u;
         }
+    }
+  }
+  __device__ __forceinline__ void start(const AttendArgs&, const Cursor&, char*) {
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
 #pragma unroll
       for (int i = 0; i < D / 16; i++)
 #pragma unroll
@@ -450,6 +473,7 @@ struct FmaWarp {
   const float* queries;
   float* probabilities;
 
+  __device__ __forceinline__ void load(const AttendArgs&, const Cursor&) {}
   __device__ __forceinline__ void start(const AttendArgs& p, const Cursor& u, char* shared) {
     const int g = u.group / p.groups, h0 = (u.group % p.groups) * H;
     float* to = reinterpret_cast<float*>(shared);
@@ -572,7 +596,7 @@ struct JoinSpace {  // at the end of a segment
   static constexpr int H = W::kHeads;
   float2 stat[kWarps][H];  // (max, sum)
   long long scratch[kWarps + 2];
-  unsigned mask[kWarps][8];
+  StageNote note[kWarps][8];
   int last;
 };
 
@@ -607,7 +631,7 @@ __device__ __forceinline__ void finish(const AttendArgs& p, int b, int h, int d,
 // registers for; where there are fewer results than threads, several threads share one and take every so many-th part.
 template <typename T, typename W, int D>
 __device__ __forceinline__ void merge(const AttendArgs& p, int b, int h0, int heads, const float* parts, int count, T* out, char* space) {
-  constexpr int H = W::kHeads, kSlot = H * (D + 2), kAtOnce = 6;
+  constexpr int H = W::kHeads, kSlot = H * (D + 2), kAtOnce = 10;
   auto part = [&](int i) { return parts + (i == 0 ? kSlot : (long long)i * 2 * kSlot); };
   const int items = heads * (D / 4);
   int sharers = 1;
@@ -707,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) paged_attend_kernel(const __
       }
 #pragma unroll
     for (int s = 0; s < STAGES; s++) {
-      if (s < units) request<T, D>(p, at[s], place[s], stages + s * Stage::kBytes, &join.mask[warp][s]);
+      if (s < units) request<T, D>(p, at[s], place[s], stages + s * Stage::kBytes, &join.note[warp][s]);
       copies_commit();
     }
   }
@@ -715,11 +739,12 @@ __global__ void __launch_bounds__(kThreads, PER_SM) paged_attend_kernel(const __
   if (STAGES < units) next = locate(p, ahead);
 
   W work;
+  work.load(p, now);
   work.start(p, now, shared);
   long long segment = share.begin - now.tile;  // number of the segment's first unit
   auto refill = [&](int i, int stage) {
     if (i + STAGES < units) {
-      request<T, D>(p, ahead, next, stages + stage * Stage::kBytes, &join.mask[warp][stage]);
+      request<T, D>(p, ahead, next, stages + stage * Stage::kBytes, &join.note[warp][stage]);
       if (i + STAGES + 1 < units) {
         advance(p, ahead);
         next = locate(p, ahead);
@@ -730,7 +755,8 @@ __global__ void __launch_bounds__(kThreads, PER_SM) paged_attend_kernel(const __
   for (int i = 0, stage = 0; i < units; i++, stage = stage + 1 == STAGES ? 0 : stage + 1) {
     copies_wait<STAGES - 1>();
     __syncwarp();
-    work.step(p, now, stages + stage * Stage::kBytes, join.mask[warp][stage], scale2);
+    store_fresh<T, D>(p, join.note[warp][stage], stages + stage * Stage::kBytes);
+    work.step(p, now, stages + stage * Stage::kBytes, join.note[warp][stage].mask, scale2);
     __syncwarp();
     if (now.tile + 1 < now.tiles && i + 1 < units) {
       refill(i, stage);
@@ -739,17 +765,22 @@ __global__ void __launch_bounds__(kThreads, PER_SM) paged_attend_kernel(const __
     }
 
     // This block's part of the segment is complete. The warps' sums take the place of the stages just read.
+    const Cursor done = now;
+    if (i + 1 < units) {
+      advance(p, now);
+      work.load(p, now);
+    }
     work.statistics(&join.stat[warp][0].x);
     work.values(reinterpret_cast<float*>(stages + stage * Stage::kBytes), kPitch);
     __syncthreads();
-    const int g = now.group / p.groups, h0 = (now.group % p.groups) * H;
+    const int g = done.group / p.groups, h0 = (done.group % p.groups) * H;
     const int heads = min(H, p.rep - h0);
-    const long long first = segment / share.quota, last = (segment + now.tiles - 1) / share.quota;
+    const long long first = segment / share.quota, last = (segment + done.tiles - 1) / share.quota;
     const int others = (int)(last - first);
     // Slot 1 of a block holds the segment that begins in it, slot 0 the one that began before it.
     constexpr int kSlot = H * (D + 2);
     float* mine = p.space.partials + ((long long)blockIdx.x * 2 + (blockIdx.x == first ? 1 : 0)) * kSlot;
-    T* out = static_cast<T*>(p.a.out) + now.b * p.a.out_batch_stride + (long long)(g * p.rep + h0) * p.a.out_head_stride;
+    T* out = static_cast<T*>(p.a.out) + done.b * p.a.out_batch_stride + (long long)(g * p.rep + h0) * p.a.out_head_stride;
     const float* sums = reinterpret_cast<const float*>(smem + stage * Stage::kBytes);
     for (int j = threadIdx.x; j < heads * (D / 4); j += kThreads) {
       const int h = j / (D / 4), d = j % (D / 4) * 4;
@@ -769,27 +800,27 @@ __global__ void __launch_bounds__(kThreads, PER_SM) paged_attend_kernel(const __
         x.w = fmaf(f, y.w, x.w);
       }
       if (others == 0) {
-        finish(p, now.b, g * p.rep + h0 + h, d, out + h * p.a.out_head_stride, x, top, total);
+        finish(p, done.b, g * p.rep + h0 + h, d, out + h * p.a.out_head_stride, x, top, total);
       } else {
         *reinterpret_cast<float4*>(mine + j * 4) = x;
         if (d == 0) *reinterpret_cast<float2*>(mine + H * D + 2 * h) = make_float2(top, total);
       }
     }
     if (others) {
-      __threadfence();
       __syncthreads();
-      if (threadIdx.x == 0)
-        join.last = atomicInc(p.space.counters + (long long)now.b * p.c.kv_heads * p.groups + now.group, (unsigned)others) == (unsigned)others;
+      if (threadIdx.x == 0) {  // its fences stand for the whole block: the barriers order the others' accesses before and behind them
+        __threadfence();
+        join.last = atomicInc(p.space.counters + (long long)done.b * p.c.kv_heads * p.groups + done.group, (unsigned)others) == (unsigned)others;
+        __threadfence();
+      }
       __syncthreads();
       if (join.last) {
-        __threadfence();
-        merge<T, W, D>(p, now.b, g * p.rep + h0, heads, p.space.partials + first * 2 * kSlot, others + 1, out,
+        merge<T, W, D>(p, done.b, g * p.rep + h0, heads, p.space.partials + first * 2 * kSlot, others + 1, out,
                        smem + stage * Stage::kBytes);  // the first warp's sums have been read
       }
     }
     if (i + 1 < units) {
-      segment += now.tiles;
-      advance(p, now);
+      segment += done.tiles;
       __syncthreads();  // the stages are filled again, and so is `join`
       refill(i, stage);
       work.start(p, now, shared);
@@ -799,22 +830,36 @@ __global__ void __launch_bounds__(kThreads, PER_SM) paged_attend_kernel(const __
 
 constexpr int kTrackThreads = 256;
 
+// A thread a row. What it needs is requested at once, also where the row turns out not to be there: the kernel is a few
+// microseconds behind the attention, and most of them are one trip to memory.
+template <int REP>  // query heads of a KV head; 0: any number
 __global__ void __launch_bounds__(kTrackThreads) paged_track_kernel(PagedView c, AttendSpace space, int heads, int appended) {
   PJRTX_PDL_PROLOGUE();
-  const int g = blockIdx.y, b = blockIdx.z, rep = heads / c.kv_heads;
-  const int n = paged_length(c, b);
-  const long long base = ((long long)b * c.kv_heads + g) * c.page_size * c.max_pages;
+  const int g = blockIdx.y, b = blockIdx.z, rep = heads / c.kv_heads, capacity = c.page_size * c.max_pages;
+  const long long base = ((long long)b * c.kv_heads + g) * capacity;
   const float* lse2 = space.lse2 + (long long)b * heads + g * rep;
-  for (int t = blockIdx.x * kTrackThreads + threadIdx.x; t < n; t += gridDim.x * kTrackThreads) {
+  for (int t = blockIdx.x * kTrackThreads + threadIdx.x; t < capacity; t += gridDim.x * kTrackThreads) {
+    const int n = paged_length(c, b);
     const float* s = space.scores + (base + t) * rep;
     float w = 0.f;
-    for (int r = 0; r < rep; r++) w += lse2[r] == -INFINITY ? 0.f : exp2f(s[r] - lse2[r]);
-    if (appended && t == n - 1) {
-      c.weights[base + t] = w;
-      c.positions[base + t] = c.tokens[b] - 1;
+    if constexpr (REP > 0) {
+      const float was = c.weights[base + t];
+      float x[REP], l[REP];
+#pragma unroll
+      for (int r = 0; r < REP; r++) {
+        x[r] = s[r];
+        l[r] = lse2[r];
+      }
+#pragma unroll
+      for (int r = 0; r < REP; r++) w += l[r] == -INFINITY ? 0.f : exp2_fast(x[r] - l[r]);
+      if (!(appended && t == n - 1)) w += was;
     } else {
-      c.weights[base + t] += w;
+      for (int r = 0; r < rep; r++) w += lse2[r] == -INFINITY ? 0.f : exp2_fast(s[r] - lse2[r]);
+      if (!(appended && t == n - 1)) w += c.weights[base + t];
     }
+    if (t >= n) break;
+    c.weights[base + t] = w;
+    if (appended && t == n - 1) c.positions[base + t] = c.tokens[b] - 1;
   }
 }
 
@@ -835,12 +880,12 @@ template <typename F>
 auto with_kernel(int dtype, int head_dim, int rep, F&& f) {
 #define PJRTX_ATTEND(T, W, D, S, N) return f(paged_attend_kernel<T, W, D, S, N>, AttendPlan{D, W::kHeads, S, N, attend_smem<T, W, D, S>()})
 #define PJRTX_ATTEND_MMA(T, NB)                                                 \
-  if (head_dim <= 64) { using W = MmaWarp<T, 64, NB>; PJRTX_ATTEND(T, W, 64, NB == 1 ? 3 : 4, NB == 1 ? 4 : 3); }  \
-  if (head_dim <= 128) { using W = MmaWarp<T, 128, NB>; PJRTX_ATTEND(T, W, 128, NB == 1 ? 2 : 3, NB == 1 ? 3 : 2); } \
-  { using W = MmaWarp<T, 256, 1>; PJRTX_ATTEND(T, W, 256, 3, 1); }
+  if (head_dim <= 64) { using W = MmaWarp<T, 64, NB>; PJRTX_ATTEND(T, W, 64, 4, 2); }  \
+  if (head_dim <= 128) { using W = MmaWarp<T, 128, NB>; PJRTX_ATTEND(T, W, 128, NB == 1 ? 2 : 4, NB == 1 ? 2 : 1); } \
+  { using W = MmaWarp<T, 256, 1>; PJRTX_ATTEND(T, W, 256, 2, 1); }
 #define PJRTX_ATTEND_FMA(H)                                                     \
-  if (head_dim <= 64) { using W = FmaWarp<64, H>; PJRTX_ATTEND(float, W, 64, 3, 2); }  \
-  if (head_dim <= 128) { using W = FmaWarp<128, H>; PJRTX_ATTEND(float, W, 128, 3, 1); } \
+  if (head_dim <= 64) { using W = FmaWarp<64, H>; PJRTX_ATTEND(float, W, 64, 2, 2); }  \
+  if (head_dim <= 128) { using W = FmaWarp<128, H>; PJRTX_ATTEND(float, W, 128, 2, 1); } \
   { using W = FmaWarp<256, H>; PJRTX_ATTEND(float, W, 256, 1, 1); }
   if (dtype == kF32) {
     if (rep <= 4) { PJRTX_ATTEND_FMA(4) }
@@ -905,8 +950,10 @@ int paged_attend_launch(const PagedView& c, const PagedAttend& a, int sm_count, 
   if (!c.weights) return 1;
   const long long pairs = (long long)c.batch * c.kv_heads;
   const long long blocks = std::max<long long>(1, std::min((c.capacity() + kTrackThreads - 1) / kTrackThreads, 8ll * sm_count / pairs + 1));
-  return launch_kernel(paged_track_kernel, dim3((unsigned)blocks, (unsigned)c.kv_heads, (unsigned)c.batch), dim3(kTrackThreads), 0, stream, true,
-                       c, p.space, a.heads, (int)(a.k_new != nullptr)) == cudaSuccess ? 2 : 0;
+  auto kernel = p.rep == 1 ? paged_track_kernel<1> : p.rep == 2 ? paged_track_kernel<2> : p.rep == 4 ? paged_track_kernel<4>
+                : p.rep == 8 ? paged_track_kernel<8> : paged_track_kernel<0>;
+  return launch_kernel(kernel, dim3((unsigned)blocks, (unsigned)c.kv_heads, (unsigned)c.batch), dim3(kTrackThreads), 0, stream, true, c, p.space,
+                       a.heads, (int)(a.k_new != nullptr)) == cudaSuccess ? 2 : 0;
 }
 
 }  // namespace pjrtx
