@@ -39,13 +39,15 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 // ---- division of the work ------------------------------------------------------------------------------------------
-// A unit is a tile of 96 rows of one (sequence, KV head, group of query heads). Units are numbered in that order, only those
-// that the lengths call for, and every block takes the same number of consecutive ones: lengths are device data, so each block
-// adds them up itself. What belongs to one (sequence, head group) is a segment; where several blocks share one, each leaves
-// (max, sum, values) in its slot of the workspace and the block that arrives last joins them in block order.
+// A unit is a tile of 96 rows of one (sequence, KV head, group of query heads), a segment what belongs to one of these. Segments
+// have numbers for their tiles and, behind them, for kSegmentCost more: what joining the warps and going on with another segment
+// takes. The numbers are cut into equal shares, one for each block that fits the GPU at once; lengths are device data, so each
+// block adds them up itself. Where several blocks share a segment, each leaves (max, sum, values) in its slot of the workspace and
+// the block that arrives last joins them in block order.
 
 constexpr int kWarps = 6, kThreads = kWarps * 32;
 constexpr int kWarpRows = 16, kTileRows = kWarps * kWarpRows;
+constexpr int kSegmentCost = 2;
 
 struct AttendSpace {
   float* lse2;         // [batch, heads]: lse / ln 2
@@ -81,20 +83,31 @@ __device__ __forceinline__ void advance(const AttendArgs& p, Cursor& u) {
   } while (u.tiles == 0);
 }
 
-// What this block works on: units [begin, end) of all, starting at `at`; `quota` units a block.
+// What this block works on: the tiles among numbers [begin, begin + size), the first of them at `first` of these.
 struct Share {
-  long long begin, end, quota;
+  long long begin, quota;
+  int size, first;  // first >= size: none
   Cursor at;
 };
 
-// Called by all threads. `scratch`: shared memory of kWarps + 1 long longs and 4 ints.
+// The next tile of a share; false at its end.
+__device__ __forceinline__ bool next_unit(const AttendArgs& p, Cursor& u, int& at, int size) {
+  const int to = at + (u.tile + 1 < u.tiles ? 1 : 1 + kSegmentCost);
+  if (to >= size) return false;
+  at = to;
+  advance(p, u);
+  return true;
+}
+
+// Called by all threads. `scratch`: shared memory of kWarps long longs and 8 ints.
 __device__ __forceinline__ Share share_of_block(const AttendArgs& p, long long* scratch) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int per_thread = (p.c.batch + kThreads - 1) / kThreads;
   const int first = min(p.c.batch, (int)threadIdx.x * per_thread), last = min(p.c.batch, first + per_thread);
   const long long width = (long long)p.c.kv_heads * p.groups;
+  auto numbers_of = [&](int tiles) { return tiles ? tiles + kSegmentCost : 0; };
   long long mine = 0;
-  for (int b = first; b < last; b++) mine += tiles_of(paged_length(p.c, b)) * width;
+  for (int b = first; b < last; b++) mine += numbers_of(tiles_of(paged_length(p.c, b))) * width;
   long long sum = mine;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
@@ -112,21 +125,30 @@ __device__ __forceinline__ Share share_of_block(const AttendArgs& p, long long* 
   Share s;
   s.quota = max(1ll, (total + gridDim.x - 1) / gridDim.x);
   s.begin = min(total, blockIdx.x * s.quota);
-  s.end = min(total, s.begin + s.quota);
+  s.size = (int)min(total - s.begin, s.quota);
   int* found = reinterpret_cast<int*>(scratch + kWarps);
-  if (s.begin < s.end && before <= s.begin && s.begin < before + mine) {
+  if (s.size > 0 && before <= s.begin && s.begin < before + mine) {
     long long rest = s.begin - before;
-    int b = first, length = 0, tiles = 0;
-    for (;; b++) {
-      length = paged_length(p.c, b);
-      tiles = tiles_of(length);
-      if (rest < tiles * width) break;
-      rest -= tiles * width;
+    Cursor u;
+    u.b = first;
+    for (;; u.b++) {
+      u.length = paged_length(p.c, u.b);
+      u.tiles = tiles_of(u.length);
+      if (rest < numbers_of(u.tiles) * width) break;
+      rest -= numbers_of(u.tiles) * width;
     }
-    found[0] = b;
-    found[1] = (int)(rest / tiles);
-    found[2] = (int)(rest % tiles);
-    found[3] = length;
+    u.group = (int)(rest / (u.tiles + kSegmentCost));
+    u.tile = (int)(rest % (u.tiles + kSegmentCost));
+    int at = 0;
+    if (u.tile >= u.tiles) {  // behind a segment's tiles: the share begins with the next one
+      at = u.tiles + kSegmentCost - u.tile;
+      if (at < s.size) advance(p, u);
+    }
+    found[0] = u.b;
+    found[1] = u.group;
+    found[2] = u.tile;
+    found[3] = u.length;
+    found[4] = at;
   }
   __syncthreads();
   s.at.b = found[0];
@@ -134,6 +156,7 @@ __device__ __forceinline__ Share share_of_block(const AttendArgs& p, long long* 
   s.at.tile = found[2];
   s.at.length = found[3];
   s.at.tiles = tiles_of(s.at.length);
+  s.first = s.size > 0 ? found[4] : 0;
   return s;
 }
 
@@ -595,7 +618,7 @@ template <typename W>
 struct JoinSpace {  // at the end of a segment
   static constexpr int H = W::kHeads;
   float2 stat[kWarps][H];  // (max, sum)
-  long long scratch[kWarps + 2];
+  long long scratch[kWarps + 4];
   StageNote note[kWarps][8];
   int last;
 };
@@ -714,62 +737,60 @@ __global__ void __launch_bounds__(kThreads, PER_SM) paged_attend_kernel(const __
     for (int h = threadIdx.x; h < p.a.heads; h += kThreads) store_lse(p, b, h, 0.f, 0.f);
   }
   const Share share = share_of_block(p, join.scratch);
-  const int units = (int)(share.end - share.begin);
-  if (units <= 0) return;
+  if (share.first >= share.size) return;
   const float scale2 = p.a.scale * kLog2e;
 
-  Cursor ahead = share.at, now = share.at;
+  Cursor ahead = share.at, now = share.at;  // the next tile to request, the one at work
+  int ahead_at = share.first, at = share.first;
+  bool more_ahead = true;
   {
     RowPlace place[STAGES];
-    Cursor at[STAGES];
+    Cursor tile[STAGES];
+    int requested = 0;
 #pragma unroll
     for (int s = 0; s < STAGES; s++)
-      if (s < units) {
+      if (more_ahead) {
         place[s] = locate(p, ahead);
-        at[s] = ahead;
-        if (s + 1 < units) advance(p, ahead);
+        tile[s] = ahead;
+        requested = s + 1;
+        more_ahead = next_unit(p, ahead, ahead_at, share.size);
       }
 #pragma unroll
     for (int s = 0; s < STAGES; s++) {
-      if (s < units) request<T, D>(p, at[s], place[s], stages + s * Stage::kBytes, &join.note[warp][s]);
+      if (s < requested) request<T, D>(p, tile[s], place[s], stages + s * Stage::kBytes, &join.note[warp][s]);
       copies_commit();
     }
   }
   RowPlace next = {-1, 0};
-  if (STAGES < units) next = locate(p, ahead);
+  if (more_ahead) next = locate(p, ahead);
 
   W work;
   work.load(p, now);
   work.start(p, now, shared);
-  long long segment = share.begin - now.tile;  // number of the segment's first unit
-  auto refill = [&](int i, int stage) {
-    if (i + STAGES < units) {
+  auto refill = [&](int stage) {
+    if (more_ahead) {
       request<T, D>(p, ahead, next, stages + stage * Stage::kBytes, &join.note[warp][stage]);
-      if (i + STAGES + 1 < units) {
-        advance(p, ahead);
-        next = locate(p, ahead);
-      }
+      more_ahead = next_unit(p, ahead, ahead_at, share.size);
+      if (more_ahead) next = locate(p, ahead);
     }
     copies_commit();
   };
-  for (int i = 0, stage = 0; i < units; i++, stage = stage + 1 == STAGES ? 0 : stage + 1) {
+  for (int stage = 0;; stage = stage + 1 == STAGES ? 0 : stage + 1) {
     copies_wait<STAGES - 1>();
     __syncwarp();
     store_fresh<T, D>(p, join.note[warp][stage], stages + stage * Stage::kBytes);
     work.step(p, now, stages + stage * Stage::kBytes, join.note[warp][stage].mask, scale2);
     __syncwarp();
-    if (now.tile + 1 < now.tiles && i + 1 < units) {
-      refill(i, stage);
-      now.tile++;
+    const Cursor done = now;
+    const long long segment = share.begin + at - done.tile;  // number of its first tile
+    const bool more = next_unit(p, now, at, share.size);
+    if (more && done.tile + 1 < done.tiles) {
+      refill(stage);
       continue;
     }
 
     // This block's part of the segment is complete. The warps' sums take the place of the stages just read.
-    const Cursor done = now;
-    if (i + 1 < units) {
-      advance(p, now);
-      work.load(p, now);
-    }
+    if (more) work.load(p, now);
     work.statistics(&join.stat[warp][0].x);
     work.values(reinterpret_cast<float*>(stages + stage * Stage::kBytes), kPitch);
     __syncthreads();
@@ -819,12 +840,10 @@ __global__ void __launch_bounds__(kThreads, PER_SM) paged_attend_kernel(const __
                        smem + stage * Stage::kBytes);  // the first warp's sums have been read
       }
     }
-    if (i + 1 < units) {
-      segment += done.tiles;
-      __syncthreads();  // the stages are filled again, and so is `join`
-      refill(i, stage);
-      work.start(p, now, shared);
-    }
+    if (!more) break;
+    __syncthreads();  // the stages are filled again, and so is `join`
+    refill(stage);
+    work.start(p, now, shared);
   }
 }
 
@@ -942,8 +961,8 @@ int paged_attend_launch(const PagedView& c, const PagedAttend& a, int sm_count, 
     p.space.partials = reinterpret_cast<float*>(space + l.partials);
     p.space.scores = reinterpret_cast<float*>(space + l.scores);
     if (!raise_smem_limit((const void*)kernel, (int)plan.smem)) return false;
-    const long long units = (long long)c.batch * c.kv_heads * p.groups * ((c.capacity() + kTileRows - 1) / kTileRows);
-    const long long blocks = std::min<long long>(units, (long long)sm_count * plan.per_sm);
+    const long long numbers = (long long)c.batch * c.kv_heads * p.groups * ((c.capacity() + kTileRows - 1) / kTileRows + kSegmentCost);
+    const long long blocks = std::min<long long>(numbers, (long long)sm_count * plan.per_sm);
     return launch_kernel(kernel, dim3((unsigned)blocks), dim3(kThreads), plan.smem, stream, pdl, p) == cudaSuccess;
   });
   if (!ok) return 0;
