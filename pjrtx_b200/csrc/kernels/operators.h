@@ -56,8 +56,11 @@ struct PagedAttend {
   float scale = 1.f;
   void* workspace = nullptr;
 };
-// Device memory that attend needs, and evict needs, for `c` with this many heads; both start out zeroed.
-uint64_t paged_attend_workspace_bytes(const PagedView& c, int heads, bool track, int sm_count);
+// Device memory that a call needs for `c`; the first `zeroed` bytes hold counters, which start out at zero and are left so.
+struct WorkspaceSize {
+  uint64_t bytes, zeroed;
+};
+WorkspaceSize paged_attend_workspace(const PagedView& c, int heads, bool track, int sm_count);
 int paged_attend_launch(const PagedView& c, const PagedAttend& a, int sm_count, bool pdl, cudaStream_t stream);
 
 struct PagedEvict {
@@ -67,7 +70,7 @@ struct PagedEvict {
   int* positions_out = nullptr;
   void* workspace = nullptr;
 };
-uint64_t paged_evict_workspace_bytes(const PagedView& c);
+WorkspaceSize paged_evict_workspace(const PagedView& c);
 int paged_evict_launch(const PagedView& c, const PagedEvict& e, int sm_count, bool pdl, cudaStream_t stream);
 
 struct TokenScore {

@@ -940,9 +940,11 @@ AttendLayout attend_layout(const PagedView& c, int heads, const AttendPlan& plan
 
 }  // namespace
 
-uint64_t paged_attend_workspace_bytes(const PagedView& c, int heads, bool track, int sm_count) {
-  return with_kernel(c.dtype, c.head_dim, heads / c.kv_heads,
-                     [&](auto, const AttendPlan& plan) { return attend_layout(c, heads, plan, track, sm_count).bytes; });
+WorkspaceSize paged_attend_workspace(const PagedView& c, int heads, bool track, int sm_count) {
+  return with_kernel(c.dtype, c.head_dim, heads / c.kv_heads, [&](auto, const AttendPlan& plan) {
+    const AttendLayout l = attend_layout(c, heads, plan, track, sm_count);
+    return WorkspaceSize{l.bytes, l.partials};
+  });
 }
 
 int paged_attend_launch(const PagedView& c, const PagedAttend& a, int sm_count, bool pdl, cudaStream_t stream) {

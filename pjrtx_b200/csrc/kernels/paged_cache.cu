@@ -377,7 +377,10 @@ int paged_append_launch(const PagedView& c, const PagedAppend& a, bool pdl, cuda
                        stream, pdl, c, a, pieces, esize) == cudaSuccess;
 }
 
-uint64_t paged_evict_workspace_bytes(const PagedView& c) { return evict_layout(c).bytes; }
+WorkspaceSize paged_evict_workspace(const PagedView& c) {
+  const EvictLayout l = evict_layout(c);
+  return {l.bytes, l.moves};
+}
 
 int paged_evict_launch(const PagedView& c, const PagedEvict& e, int sm_count, bool pdl, cudaStream_t stream) {
   const int esize = (int)dtype_size(c.dtype), pieces = c.head_dim * esize / 16;

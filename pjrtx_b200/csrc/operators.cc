@@ -76,19 +76,20 @@ PagedCache* paged_cache_create(int ordinal, const PagedCacheConfig& c) {
   v.page_size = (int)c.page_size;
   v.max_pages = (int)c.max_pages;
   v.dtype = c.dtype;
-  made.attend_bytes = paged_attend_workspace_bytes(v, (int)c.heads, c.track, dev->sm_count);
-  made.evict_bytes = c.track ? paged_evict_workspace_bytes(v) : 0;
+  const WorkspaceSize attend = paged_attend_workspace(v, (int)c.heads, c.track, dev->sm_count);
+  const WorkspaceSize evict = c.track ? paged_evict_workspace(v) : WorkspaceSize{0, 0};
+  const uint64_t evict_at = (attend.bytes + 255) / 256 * 256;
+  made.bytes = evict_at + evict.bytes;
   CurrentDevice scope(dev->ordinal);
-  made.attend_space = device_malloc(dev, made.attend_bytes);
-  if (made.evict_bytes) made.evict_space = device_malloc(dev, made.evict_bytes);
-  // The workspaces hold counters that every call leaves at zero; other streams may use them once this returns.
-  const bool ok = made.attend_space && (!made.evict_bytes || made.evict_space) &&
-                  check_cuda(cudaMemsetAsync(made.attend_space, 0, made.attend_bytes, dev->stream), "cudaMemsetAsync") &&
-                  (!made.evict_bytes || check_cuda(cudaMemsetAsync(made.evict_space, 0, made.evict_bytes, dev->stream), "cudaMemsetAsync")) &&
+  made.attend_space = device_malloc(dev, made.bytes);
+  if (!made.attend_space) return nullptr;
+  made.evict_space = c.track ? static_cast<char*>(made.attend_space) + evict_at : nullptr;
+  // Other streams may use the workspaces once this returns.
+  const bool ok = check_cuda(cudaMemsetAsync(made.attend_space, 0, attend.zeroed, dev->stream), "cudaMemsetAsync") &&
+                  (!c.track || check_cuda(cudaMemsetAsync(made.evict_space, 0, evict.zeroed, dev->stream), "cudaMemsetAsync")) &&
                   check_cuda(cudaStreamSynchronize(dev->stream), "cudaStreamSynchronize");
   if (!ok) {
-    device_free(dev, made.attend_space, made.attend_bytes);
-    device_free(dev, made.evict_space, made.evict_bytes);
+    device_free(dev, made.attend_space, made.bytes);
     return nullptr;
   }
   return new PagedCache(made);
@@ -98,8 +99,7 @@ void paged_cache_destroy(PagedCache* cache) {
   if (!cache) return;
   CurrentDevice scope(cache->device->ordinal);
   cudaDeviceSynchronize();  // calls on any stream may still use the workspaces
-  device_free(cache->device, cache->attend_space, cache->attend_bytes);
-  device_free(cache->device, cache->evict_space, cache->evict_bytes);
+  device_free(cache->device, cache->attend_space, cache->bytes);
   delete cache;
 }
 

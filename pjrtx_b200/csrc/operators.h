@@ -18,9 +18,9 @@ struct PagedCacheConfig {
 struct PagedCache {
   Device* device = nullptr;
   PagedCacheConfig config;
-  void* attend_space = nullptr;
-  void* evict_space = nullptr;
-  uint64_t attend_bytes = 0, evict_bytes = 0;
+  void* attend_space = nullptr;  // one allocation
+  void* evict_space = nullptr;   // in it, with tracking
+  uint64_t bytes = 0;
 };
 
 // Arguments are checked before the device is touched.

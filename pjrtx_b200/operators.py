@@ -148,18 +148,18 @@ def _rows(x, name: str, dtype: int, shape: Tuple[int, ...]):
     return place
 
 
-def _twin(x, name: str, like, like_name: str, strides) -> int:
-    """Address of an array that has the type, shape and strides of `like`."""
+def _twin(x, name: str, like: str, dtype: int, shape: Tuple[int, ...], strides) -> int:
+    """Address of an array that has the type, shape and strides of another one."""
     try:
-        if x.shape == like.shape and x.dtype == like.dtype and x.stride() == strides:
+        if x.shape == shape and _codes[x.dtype] == dtype and x.stride() == strides:
             return x.data_ptr()
-    except AttributeError:
+    except (AttributeError, KeyError):
         pass
-    if _code(x) != _code(like) or _dims(x) != _dims(like):
-        raise _error(f"{like_name} and {name} differ in type or shape")
+    if _code(x) != dtype or _dims(x) != shape:
+        raise _error(f"{like} and {name} differ in type or shape")
     pointer, own = _place(x)
     if own != strides:
-        raise _error(f"{like_name} and {name} differ in their strides")
+        raise _error(f"{like} and {name} differ in their strides")
     return pointer
 
 
@@ -206,13 +206,13 @@ class PagedCache:
 
     def _view(self, k_pages, v_pages, page_table, lengths, tokens, weights, positions) -> Tuple[int, bytes]:
         """The batch and the packed view."""
-        dims, batch_dims = tuple(_dims(k_pages)), _dims(lengths)
+        dims, batch_dims = _dims(k_pages), _dims(lengths)
         if len(dims) != 4 or dims[1:] != self._page_dims:
-            raise _error(f"k_pages has shape {dims}, (pages, {', '.join(map(str, self._page_dims))}) is needed")
+            raise _error(f"k_pages has shape {tuple(dims)}, (pages, {', '.join(map(str, self._page_dims))}) is needed")
         if len(batch_dims) != 1:
             raise _error(f"lengths has shape {tuple(batch_dims)}, (batch,) is needed")
         k, strides = _rows(k_pages, "k_pages", self.dtype, dims)
-        v = _twin(v_pages, "v_pages", k_pages, "k_pages", strides)
+        v = _twin(v_pages, "v_pages", "k_pages", self.dtype, dims, strides)
         batch = batch_dims[0]
         table, table_strides = _rows(page_table, "page_table", P.S32, (batch, self.max_pages))
         tracked = (batch, self.kv_heads, self.capacity)
@@ -236,7 +236,7 @@ class PagedCache:
             raise _error(f"k_new has shape {tuple(dims)}, (batch, rows, KV heads, head dimension) is needed")
         shape = (batch, dims[1], self.kv_heads, self.head_dim)
         k, strides = _rows(k_new, "k_new", self.dtype, shape)
-        v = _twin(v_new, "v_new", k_new, "k_new", strides)
+        v = _twin(v_new, "v_new", "k_new", self.dtype, shape, strides)
         args = _pack_append(k, v, shape[1], strides[0], strides[1], strides[2], _dense(counts, "counts", P.S32, (batch,)))
         self._call(self._lib.pjrtx_b200_paged_cache_append, view, args, stream)
 
@@ -254,7 +254,7 @@ class PagedCache:
         if k_new is not None and v_new is not None:
             shape = (batch, self.kv_heads, self.head_dim)
             k, new_strides = _rows(k_new, "k_new", self.dtype, shape)
-            v = _twin(v_new, "v_new", k_new, "k_new", new_strides)
+            v = _twin(v_new, "v_new", "k_new", self.dtype, shape, new_strides)
         elif k_new is not None or v_new is not None:
             raise _error("a new key and a new value go together")
         args = _pack_attend(q_at, q_strides[0], q_strides[1], out_at, out_strides[0], out_strides[1],
