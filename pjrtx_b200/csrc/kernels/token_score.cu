@@ -59,6 +59,11 @@ __device__ __forceinline__ Pair pair_fma(Pair a, Pair b, Pair c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+__device__ __forceinline__ Pair pair_mul(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ Pair pair_add(Pair a, Pair b) {
   Pair r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -563,7 +568,7 @@ __global__ void __launch_bounds__(THREADS, kScoreThreadsOfSm / THREADS) token_sc
 
 // ---- gradient ------------------------------------------------------------------------------------------------------
 
-constexpr int kGradThreads = 256;
+constexpr int kGradThreads = 128;
 constexpr int kGradUnroll = 4;
 
 template <typename T, bool ENTROPY>
@@ -579,30 +584,42 @@ __global__ void __launch_bounds__(kGradThreads) token_score_grad_kernel(TokenSco
   const float lse = a.lse[row];
   const float g = token >= 0 && a.grad_log_probs ? a.grad_log_probs[row] * a.scale : 0.f;
   const float h = ENTROPY ? a.grad_entropy[row] * a.scale : 0.f, entropy = ENTROPY ? a.entropy[row] : 0.f;
-  const bool none = lse == -INFINITY;
+  const bool none = lse == -INFINITY;  // nothing but -inf in the row: p = 0 everywhere
   // entropy - lse in two numbers, so that ln p + entropy, which is small where it matters, is rounded once.
   const float base = entropy - lse, part_of = base - entropy, rest = (entropy - (base - part_of)) + (-lse - part_of);
-  // d = [j = token] g - p (g + h (ln p + entropy)); p = 0 gives 0 also where ln p = -inf.
-  auto gradient = [&](float x, int j) {
-    const float log_p = fmaf(x, a.scale, -lse);
-    const float p = none ? 0.f : exp2_fast(log_p * kLog2e);
-    float d = g;
-    if (ENTROPY) d = p == 0.f ? g : fmaf(h, fmaf(x, a.scale, base) + rest, g);
-    d = -p * d;
-    return j == token ? d + g : d;
+  // -p (g + h (ln p + entropy)), two logits at a time; what the token's own logit gets besides is added by the thread that has it.
+  const Pair scale2 = pair_of(a.scale, a.scale), from2 = pair_of(none ? 0.f : -lse, none ? 0.f : -lse), log2e2 = pair_of(kLog2e, kLog2e);
+  const Pair base2 = pair_of(base, base), rest2 = pair_of(rest, rest), g2 = pair_of(-g, -g), h2 = pair_of(-h, -h);
+  auto gradient = [&](float& x0, float& x1) {
+    const Pair x = pair_of(x0, x1);
+    const float2 y = split(pair_mul(pair_fma(x, scale2, from2), log2e2));
+    const Pair p = pair_of(exp2_fast(y.x), exp2_fast(y.y));
+    Pair d = g2;
+    if (ENTROPY) {
+      const float2 t = split(pair_add(pair_fma(x, scale2, base2), rest2));
+      d = pair_fma(h2, pair_of(max_nan(t.x, -1e30f), max_nan(t.y, -1e30f)), g2);  // finite, for p = 0 to make it 0
+    }
+    const float2 r = split(pair_mul(p, d));
+    x0 = r.x;
+    x1 = r.y;
+  };
+  auto single = [&](float x, int j) {
+    float unused = 0.f;
+    gradient(x, unused);
+    return (none ? 0.f : x) + (j == token ? g : 0.f);
   };
   const int shift = (int)((reinterpret_cast<uintptr_t>(logits) & 15) / sizeof(T));
-  if (shift == (int)((reinterpret_cast<uintptr_t>(grad) & 15) / sizeof(T))) {
+  if (shift == (int)((reinterpret_cast<uintptr_t>(grad) & 15) / sizeof(T)) && !none) {
     const T* from = logits - shift;
     T* to = grad - shift;
-    const int end = (int)a.vocab + shift, vectors = (end + V - 1) / V;
+    const int end = (int)a.vocab + shift, vectors = (end + V - 1) / V, own = token + shift;
     const int step = blocks_per_row * kGradThreads;
     for (int v0 = part * kGradThreads + (int)threadIdx.x; v0 < vectors; v0 += step * kGradUnroll) {
       uint4 r[kGradUnroll];
 #pragma unroll
       for (int u = 0; u < kGradUnroll; u++) {
         const int p = (v0 + u * step) * V;
-        if (p >= shift && p + V <= end) r[u] = *reinterpret_cast<const uint4*>(from + p);
+        if (p >= shift && p + V <= end) r[u] = __ldcs(reinterpret_cast<const uint4*>(from + p));
       }
 #pragma unroll
       for (int u = 0; u < kGradUnroll; u++) {
@@ -611,16 +628,21 @@ __global__ void __launch_bounds__(kGradThreads) token_score_grad_kernel(TokenSco
           float f[V];
           Logit<T>::unpack(r[u], f);
 #pragma unroll
-          for (int i = 0; i < V; i++) f[i] = gradient(f[i], p + i - shift);
-          *reinterpret_cast<uint4*>(to + p) = Logit<T>::pack(f);
+          for (int i = 0; i < V; i += 2) gradient(f[i], f[i + 1]);
+          if (own >= p && own < p + V) {
+#pragma unroll
+            for (int i = 0; i < V; i++)
+              if (p + i == own) f[i] += g;
+          }
+          __stcs(reinterpret_cast<uint4*>(to + p), Logit<T>::pack(f));
         } else {
-          for (int i = max(p, shift); i < min(p + V, end); i++) Logit<T>::store(to + i, gradient(Logit<T>::load(from + i), i - shift));
+          for (int i = max(p, shift); i < min(p + V, end); i++) Logit<T>::store(to + i, single(Logit<T>::load(from + i), i - shift));
         }
       }
     }
   } else {
     for (long long j = part * kGradThreads + (int)threadIdx.x; j < a.vocab; j += blocks_per_row * kGradThreads)
-      Logit<T>::store(grad + j, gradient(Logit<T>::load(logits + j), (int)j));
+      Logit<T>::store(grad + j, single(Logit<T>::load(logits + j), (int)j));
   }
 }
 
