@@ -46,7 +46,6 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // the block that arrives last joins them in block order.
 
 constexpr int kWarps = 6, kThreads = kWarps * 32;
-constexpr int kWarpRows = 16, kTileRows = kWarps * kWarpRows;
 constexpr int kSegmentCost = 2;
 
 struct AttendSpace {
@@ -62,6 +61,7 @@ struct AttendArgs {
   AttendSpace space;
   int rep, groups;  // query heads of a KV head, groups of them
   int pieces;       // 16-byte pieces of a row
+  int tile_rows;    // of a tile: those of a warp times the warps
   unsigned reciprocal;  // floor(2^32 / page_size), at most 2^32 - 1
 };
 
@@ -69,7 +69,7 @@ struct Cursor {
   int b, group, tile, tiles, length;  // group = KV head * groups + head group
 };
 
-__device__ __forceinline__ int tiles_of(int length) { return (length + kTileRows - 1) / kTileRows; }
+__device__ __forceinline__ int tiles_of(const AttendArgs& p, int length) { return (length + p.tile_rows - 1) / p.tile_rows; }
 
 __device__ __forceinline__ void advance(const AttendArgs& p, Cursor& u) {
   if (++u.tile < u.tiles) return;
@@ -79,7 +79,7 @@ __device__ __forceinline__ void advance(const AttendArgs& p, Cursor& u) {
   do {
     u.b++;
     u.length = paged_length(p.c, u.b);
-    u.tiles = tiles_of(u.length);
+    u.tiles = tiles_of(p, u.length);
   } while (u.tiles == 0);
 }
 
@@ -107,7 +107,7 @@ __device__ __forceinline__ Share share_of_block(const AttendArgs& p, long long* 
   const long long width = (long long)p.c.kv_heads * p.groups;
   auto numbers_of = [&](int tiles) { return tiles ? tiles + kSegmentCost : 0; };
   long long mine = 0;
-  for (int b = first; b < last; b++) mine += numbers_of(tiles_of(paged_length(p.c, b))) * width;
+  for (int b = first; b < last; b++) mine += numbers_of(tiles_of(p, paged_length(p.c, b))) * width;
   long long sum = mine;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
@@ -133,7 +133,7 @@ __device__ __forceinline__ Share share_of_block(const AttendArgs& p, long long* 
     u.b = first;
     for (;; u.b++) {
       u.length = paged_length(p.c, u.b);
-      u.tiles = tiles_of(u.length);
+      u.tiles = tiles_of(p, u.length);
       if (rest < numbers_of(u.tiles) * width) break;
       rest -= numbers_of(u.tiles) * width;
     }
@@ -155,7 +155,7 @@ __device__ __forceinline__ Share share_of_block(const AttendArgs& p, long long* 
   s.at.group = found[1];
   s.at.tile = found[2];
   s.at.length = found[3];
-  s.at.tiles = tiles_of(s.at.length);
+  s.at.tiles = tiles_of(p, s.at.length);
   s.first = s.size > 0 ? found[4] : 0;
   return s;
 }
@@ -164,10 +164,10 @@ __device__ __forceinline__ Share share_of_block(const AttendArgs& p, long long* 
 // A warp works by itself: it fetches 16 rows of each tile with cp.async into stages of its own, so the warps of a block meet
 // only at the end of a segment. Rows outside the sequence (or without a page) are filled with zeros and masked.
 
-template <typename T, int D>
+template <typename T, int D, int ROWS>
 struct RowStage {
   static constexpr int kPitch = D * (int)sizeof(T) + 16;  // bytes; rows of eight keys fall on different banks
-  static constexpr int kBytes = 2 * kWarpRows * kPitch;
+  static constexpr int kBytes = 2 * ROWS * kPitch;
 };
 
 __device__ __forceinline__ void copy16(unsigned to, unsigned long long from) {
@@ -182,13 +182,14 @@ __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Where row `lane % 16` of this warp's part of a tile lies.
+// Where row `lane % ROWS` of this warp's part of a tile lies.
 struct RowPlace {
   int page, row;  // page -1: no such row
 };
 
+template <int ROWS>
 __device__ __forceinline__ RowPlace locate(const AttendArgs& p, const Cursor& u) {
-  const int t = u.tile * kTileRows + (threadIdx.x / 32) * kWarpRows + (threadIdx.x & 15);
+  const int t = u.tile * p.tile_rows + (threadIdx.x / 32) * ROWS + (threadIdx.x & (ROWS - 1));
   RowPlace r = {-1, 0};
   if (t < u.length) {
     int column = (int)__umulhi((unsigned)t, p.reciprocal);  // the quotient or one less
@@ -216,38 +217,39 @@ struct StageNote {
 };
 
 // Requests the rows of `u`.
-template <typename T, int D>
+template <typename T, int D, int ROWS>
 __device__ __forceinline__ void request(const AttendArgs& p, const Cursor& u, const RowPlace& r, char* stage, StageNote* note) {
-  using S = RowStage<T, D>;
+  using S = RowStage<T, D, ROWS>;
   constexpr int kPieces = D * (int)sizeof(T) / 16, kAcross = 8;  // eight lanes beside each other on one row
   const int lane = threadIdx.x % 32, g = u.group / p.groups;
-  const int t0 = u.tile * kTileRows + (threadIdx.x / 32) * kWarpRows;
+  const int t0 = u.tile * p.tile_rows + (threadIdx.x / 32) * ROWS;
   unsigned long long k = 0;  // address of the key; the value's is `apart` further
   const unsigned long long apart_pools = address_of(p.c.v) - address_of(p.c.k);
   unsigned long long apart = apart_pools;
   if (r.page >= 0)
     k = address_of(p.c.k) + (r.page * p.c.page_stride + r.row * p.c.row_stride + g * p.c.head_stride) * (long long)sizeof(T);
-  const int fresh = u.length - 1 - t0;  // which of the 16 rows comes with the call
-  const bool has_fresh = p.a.k_new && fresh >= 0 && fresh < kWarpRows;
+  const int fresh = u.length - 1 - t0;  // which of the warp's rows comes with the call
+  const bool has_fresh = p.a.k_new && fresh >= 0 && fresh < ROWS;
   if (has_fresh) {
     const long long at = (u.b * p.a.new_batch_stride + g * p.a.new_head_stride) * (long long)sizeof(T);
     const char* k_new = static_cast<const char*>(p.a.k_new) + at;
     const char* v_new = static_cast<const char*>(p.a.v_new) + at;
-    if ((lane & 15) == fresh && k) {
-      if (lane < 16) note->store = k;
+    if ((lane & (ROWS - 1)) == fresh && k) {
+      if (lane < ROWS) note->store = k;
       k = address_of(k_new);
       apart = address_of(v_new) - k;
     }
   }
-  const unsigned there = __ballot_sync(~0u, k != 0) & 0xffffu;
+  constexpr unsigned kAll = ROWS == 32 ? ~0u : (1u << ROWS) - 1;
+  const unsigned there = __ballot_sync(~0u, k != 0) & kAll;
   if (lane == 0) {
     note->mask = there;
     note->fresh = has_fresh && (there >> fresh & 1) && u.group % p.groups == 0 ? fresh : -1;
   }
   const unsigned to = (unsigned)__cvta_generic_to_shared(stage) + lane / kAcross * S::kPitch + lane % kAcross * 16;
-  const bool whole = there == 0xffffu && p.pieces == kPieces;
+  const bool whole = there == kAll && p.pieces == kPieces;
 #pragma unroll
-  for (int j = 0; j < kWarpRows * kAcross / 32; j++) {
+  for (int j = 0; j < ROWS * kAcross / 32; j++) {
     const int row = lane / kAcross + j * (32 / kAcross);
     unsigned long long kr = __shfl_sync(~0u, k, row), vr = apart;
     if (has_fresh) vr = __shfl_sync(~0u, apart, row);
@@ -258,28 +260,28 @@ __device__ __forceinline__ void request(const AttendArgs& p, const Cursor& u, co
 #pragma unroll
       for (int i = 0; i < kPieces / kAcross; i++) {
         copy16(to + j * (32 / kAcross) * S::kPitch + i * kAcross * 16, kr + i * kAcross * 16);
-        copy16(to + (kWarpRows + j * (32 / kAcross)) * S::kPitch + i * kAcross * 16, vr + i * kAcross * 16);
+        copy16(to + (ROWS + j * (32 / kAcross)) * S::kPitch + i * kAcross * 16, vr + i * kAcross * 16);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < kPieces / kAcross; i++) {
         const bool in = valid && lane % kAcross + i * kAcross < p.pieces;
         copy16_or_zero(to + j * (32 / kAcross) * S::kPitch + i * kAcross * 16, in ? kr + i * kAcross * 16 : address_of(p.c.k), in);
-        copy16_or_zero(to + (kWarpRows + j * (32 / kAcross)) * S::kPitch + i * kAcross * 16, in ? vr + i * kAcross * 16 : address_of(p.c.v), in);
+        copy16_or_zero(to + (ROWS + j * (32 / kAcross)) * S::kPitch + i * kAcross * 16, in ? vr + i * kAcross * 16 : address_of(p.c.v), in);
       }
     }
   }
 }
 
 // Stores the row that came with the call from its stage into the pool.
-template <typename T, int D>
+template <typename T, int D, int ROWS>
 __device__ __forceinline__ void store_fresh(const AttendArgs& p, const StageNote& note, const char* stage) {
   if (note.fresh < 0) return;
-  const char* from = stage + note.fresh * RowStage<T, D>::kPitch;
+  const char* from = stage + note.fresh * RowStage<T, D, ROWS>::kPitch;
   char* to = reinterpret_cast<char*>(note.store);
   for (int i = threadIdx.x % 32; i < p.pieces; i += 32) {
     reinterpret_cast<uint4*>(to)[i] = reinterpret_cast<const uint4*>(from)[i];
-    reinterpret_cast<uint4*>(to + (address_of(p.c.v) - address_of(p.c.k)))[i] = reinterpret_cast<const uint4*>(from + kWarpRows * RowStage<T, D>::kPitch)[i];
+    reinterpret_cast<uint4*>(to + (address_of(p.c.v) - address_of(p.c.k)))[i] = reinterpret_cast<const uint4*>(from + ROWS * RowStage<T, D, ROWS>::kPitch)[i];
   }
 }
 
@@ -326,9 +328,9 @@ __device__ __forceinline__ unsigned transpose(unsigned a) {
 // query heads cost no more than one: scores^T [16 rows x heads] = K q^T, values^T [dims x heads] += V^T p^T. A probability goes in
 // as two 16-bit numbers, its rounding and what that leaves off: rounded to one, it would be as far off as the result's own rounding.
 // Lane i holds heads (i % 4) * 2 and + 1 of every eight.
-template <typename T, int D, int NB>
+template <typename T, int D, int NB, int ROWS>
 struct MmaWarp {
-  static constexpr int kHeads = 8 * NB;
+  static constexpr int kHeads = 8 * NB, kRows = ROWS, R = ROWS / 16;
   static constexpr int kSharedBytes = 0;
   unsigned q[D / 16][NB][2];
   float o[D / 16][NB][4];
@@ -363,35 +365,45 @@ struct MmaWarp {
   }
 
   __device__ __forceinline__ void step(const AttendArgs& p, const Cursor& u, const char* stage, unsigned mask, float scale2) {
-    constexpr int kPitch = RowStage<T, D>::kPitch;
+    constexpr int kPitch = RowStage<T, D, ROWS>::kPitch;
     const int lane = threadIdx.x % 32;
-    const unsigned k_at = (unsigned)__cvta_generic_to_shared(stage), v_at = k_at + kWarpRows * kPitch;
-    float s[NB][4];
+    const unsigned k_at = (unsigned)__cvta_generic_to_shared(stage), v_at = k_at + ROWS * kPitch;
+    float s[R][NB][4];
 #pragma unroll
-    for (int n = 0; n < NB; n++)
+    for (int r = 0; r < R; r++)
 #pragma unroll
-      for (int j = 0; j < 4; j++) s[n][j] = 0.f;
+      for (int n = 0; n < NB; n++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) s[r][n][j] = 0.f;
     const unsigned k_lane = k_at + ((lane / 8 % 2) * 8 + lane % 8) * kPitch + (lane / 16) * 16;
 #pragma unroll
-    for (int i = 0; i < D / 16; i++) {
-      unsigned a[4];
-      load_matrices(a, k_lane + i * 32);
+    for (int i = 0; i < D / 16; i++)
 #pragma unroll
-      for (int n = 0; n < NB; n++) Mma16<T>::mma(s[n], a, q[i][n][0], q[i][n][1]);
-    }
-    const bool lo = mask >> (lane / 4) & 1, hi = mask >> (lane / 4 + 8) & 1;
+      for (int r = 0; r < R; r++) {
+        unsigned a[4];
+        load_matrices(a, k_lane + r * 16 * kPitch + i * 32);
+#pragma unroll
+        for (int n = 0; n < NB; n++) Mma16<T>::mma(s[r][n], a, q[i][n][0], q[i][n][1]);
+      }
     bool grows = false;
     float top[NB][2];
 #pragma unroll
     for (int n = 0; n < NB; n++)
 #pragma unroll
       for (int j = 0; j < 2; j++) {
-        s[n][j] = lo ? s[n][j] * scale2 : -INFINITY;
-        s[n][2 + j] = hi ? s[n][2 + j] * scale2 : -INFINITY;
-        top[n][j] = max_nan(s[n][j], s[n][2 + j]);
+        top[n][j] = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+          s[r][n][j] = mask >> (r * 16 + lane / 4) & 1 ? s[r][n][j] * scale2 : -INFINITY;
+          s[r][n][2 + j] = mask >> (r * 16 + lane / 4 + 8) & 1 ? s[r][n][2 + j] * scale2 : -INFINITY;
+          top[n][j] = max_nan(top[n][j], max_nan(s[r][n][j], s[r][n][2 + j]));
+        }
         grows |= !(top[n][j] <= m[n][j]);
       }
-    if (p.c.weights) store_scores(p, u, s, lo, hi);
+    if (p.c.weights) {
+#pragma unroll
+      for (int r = 0; r < R; r++) store_scores(p, u, s[r], r, mask);
+    }
     if (__any_sync(~0u, grows)) {
 #pragma unroll
       for (int n = 0; n < NB; n++)
@@ -411,40 +423,46 @@ struct MmaWarp {
           }
         }
     }
-    unsigned big[NB][2], small[NB][2];
+    unsigned big[R][NB][2], small[R][NB][2];
 #pragma unroll
-    for (int n = 0; n < NB; n++) {
-#pragma unroll
-      for (int j = 0; j < 2; j++) {
-        const float from = m[n][j] == -INFINITY ? 0.f : m[n][j];
-        s[n][j] = exp2_fast(s[n][j] - from);
-        s[n][2 + j] = exp2_fast(s[n][2 + j] - from);
-        l[n][j] += s[n][j] + s[n][2 + j];
-      }
-#pragma unroll
-      for (int r = 0; r < 2; r++) {
-        const unsigned b = Mma16<T>::pack(s[n][2 * r], s[n][2 * r + 1]);
-        const float2 back = Mma16<T>::unpack(b);
-        big[n][r] = transpose(b);
-        small[n][r] = transpose(Mma16<T>::pack(s[n][2 * r] - back.x, s[n][2 * r + 1] - back.y));
-      }
-    }
-    const unsigned v_lane = v_at + ((lane / 16) * 8 + lane % 8) * kPitch + (lane / 8 % 2) * 16;
-#pragma unroll
-    for (int i = 0; i < D / 16; i++) {
-      unsigned a[4];
-      load_matrices_transposed(a, v_lane + i * 32);
+    for (int r = 0; r < R; r++)
 #pragma unroll
       for (int n = 0; n < NB; n++) {
-        Mma16<T>::mma(o[i][n], a, big[n][0], big[n][1]);
-        Mma16<T>::mma(o[i][n], a, small[n][0], small[n][1]);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const float from = m[n][j] == -INFINITY ? 0.f : m[n][j];
+          s[r][n][j] = exp2_fast(s[r][n][j] - from);
+          s[r][n][2 + j] = exp2_fast(s[r][n][2 + j] - from);
+          l[n][j] += s[r][n][j] + s[r][n][2 + j];
+        }
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          const unsigned b = Mma16<T>::pack(s[r][n][2 * k], s[r][n][2 * k + 1]);
+          const float2 back = Mma16<T>::unpack(b);
+          big[r][n][k] = transpose(b);
+          small[r][n][k] = transpose(Mma16<T>::pack(s[r][n][2 * k] - back.x, s[r][n][2 * k + 1] - back.y));
+        }
       }
-    }
+    const unsigned v_lane = v_at + ((lane / 16) * 8 + lane % 8) * kPitch + (lane / 8 % 2) * 16;
+#pragma unroll
+    for (int i = 0; i < D / 16; i++)
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        unsigned a[4];
+        load_matrices_transposed(a, v_lane + r * 16 * kPitch + i * 32);
+#pragma unroll
+        for (int n = 0; n < NB; n++) {
+          Mma16<T>::mma(o[i][n], a, big[r][n][0], big[r][n][1]);
+          Mma16<T>::mma(o[i][n], a, small[r][n][0], small[r][n][1]);
+        }
+      }
   }
 
-  __device__ __forceinline__ void store_scores(const AttendArgs& p, const Cursor& u, const float (&s)[NB][4], bool lo, bool hi) const {
+  // Of 16 rows, the r-th of the warp's.
+  __device__ __forceinline__ void store_scores(const AttendArgs& p, const Cursor& u, const float (&s)[NB][4], int r, unsigned mask) const {
     const int lane = threadIdx.x % 32, g = u.group / p.groups, h0 = (u.group % p.groups) * kHeads;
-    const int t = u.tile * kTileRows + (threadIdx.x / 32) * kWarpRows + lane / 4;
+    const int t = u.tile * p.tile_rows + (threadIdx.x / 32) * ROWS + r * 16 + lane / 4;
+    const bool lo = mask >> (r * 16 + lane / 4) & 1, hi = mask >> (r * 16 + lane / 4 + 8) & 1;
     float* to = p.space.scores + (((long long)u.b * p.c.kv_heads + g) * p.c.page_size * p.c.max_pages + t) * p.rep + h0;
 #pragma unroll
     for (int n = 0; n < NB; n++)
@@ -489,8 +507,8 @@ struct MmaWarp {
 // f32: CUDA cores. Scores: lane i has row i % 16 and one half of the dimensions. Values: lane i has D / 32 neighbouring dimensions.
 template <int D, int H>
 struct FmaWarp {
-  static constexpr int kHeads = H, V = D / 32;
-  static constexpr int kSharedBytes = H * D * 4 + kWarps * kWarpRows * H * 4;  // queries; probabilities of every warp
+  static constexpr int kHeads = H, kRows = 16, V = D / 32;
+  static constexpr int kSharedBytes = H * D * 4 + kWarps * kRows * H * 4;  // queries; probabilities of every warp
   float o[H][V];
   float m[H], l[H];
   const float* queries;
@@ -501,7 +519,7 @@ struct FmaWarp {
     const int g = u.group / p.groups, h0 = (u.group % p.groups) * H;
     float* to = reinterpret_cast<float*>(shared);
     queries = to;
-    probabilities = to + H * D + (threadIdx.x / 32) * kWarpRows * H;
+    probabilities = to + H * D + (threadIdx.x / 32) * kRows * H;
     __syncthreads();
     for (int i = threadIdx.x; i < H * D; i += kThreads) {
       const int h = h0 + i / D, d = i % D;
@@ -519,7 +537,7 @@ struct FmaWarp {
   }
 
   __device__ __forceinline__ void step(const AttendArgs& p, const Cursor& u, const char* stage, unsigned mask, float scale2) {
-    constexpr int kPitch = RowStage<float, D>::kPitch;
+    constexpr int kPitch = RowStage<float, D, kRows>::kPitch;
     const int lane = threadIdx.x % 32;
     float s[H];
 #pragma unroll
@@ -545,7 +563,7 @@ struct FmaWarp {
     }
     if (p.c.weights && there && lane < 16) {
       const int g = u.group / p.groups, h0 = (u.group % p.groups) * H;
-      const int t = u.tile * kTileRows + (threadIdx.x / 32) * kWarpRows + lane;
+      const int t = u.tile * p.tile_rows + (threadIdx.x / 32) * kRows + lane;
       float* to = p.space.scores + (((long long)u.b * p.c.kv_heads + g) * p.c.page_size * p.c.max_pages + t) * p.rep + h0;
 #pragma unroll
       for (int h = 0; h < H; h++)
@@ -575,9 +593,9 @@ struct FmaWarp {
       }
     }
     __syncwarp();
-    const char* v = stage + kWarpRows * kPitch + lane * V * 4;
+    const char* v = stage + kRows * kPitch + lane * V * 4;
 #pragma unroll 4
-    for (int t = 0; t < kWarpRows; t++) {
+    for (int t = 0; t < kRows; t++) {
       float x[V];
 #pragma unroll
       for (int i = 0; i < V; i += 2) *reinterpret_cast<float2*>(x + i) = *reinterpret_cast<const float2*>(v + t * kPitch + i * 4);
@@ -718,7 +736,7 @@ __device__ __forceinline__ void merge(const AttendArgs& p, int b, int h0, int he
 
 template <typename T, typename W, int D, int STAGES, int PER_SM>
 __global__ void __launch_bounds__(kThreads, PER_SM) paged_attend_kernel(const __grid_constant__ AttendArgs p) {
-  using Stage = RowStage<T, D>;
+  using Stage = RowStage<T, D, W::kRows>;
   using Join = JoinSpace<W>;
   constexpr int H = W::kHeads, kPitch = D + 4;
   static_assert(H * kPitch * 4 <= Stage::kBytes, "a warp's sums take the place of a stage");
@@ -750,35 +768,35 @@ __global__ void __launch_bounds__(kThreads, PER_SM) paged_attend_kernel(const __
 #pragma unroll
     for (int s = 0; s < STAGES; s++)
       if (more_ahead) {
-        place[s] = locate(p, ahead);
+        place[s] = locate<W::kRows>(p, ahead);
         tile[s] = ahead;
         requested = s + 1;
         more_ahead = next_unit(p, ahead, ahead_at, share.size);
       }
 #pragma unroll
     for (int s = 0; s < STAGES; s++) {
-      if (s < requested) request<T, D>(p, tile[s], place[s], stages + s * Stage::kBytes, &join.note[warp][s]);
+      if (s < requested) request<T, D, W::kRows>(p, tile[s], place[s], stages + s * Stage::kBytes, &join.note[warp][s]);
       copies_commit();
     }
   }
   RowPlace next = {-1, 0};
-  if (more_ahead) next = locate(p, ahead);
+  if (more_ahead) next = locate<W::kRows>(p, ahead);
 
   W work;
   work.load(p, now);
   work.start(p, now, shared);
   auto refill = [&](int stage) {
     if (more_ahead) {
-      request<T, D>(p, ahead, next, stages + stage * Stage::kBytes, &join.note[warp][stage]);
+      request<T, D, W::kRows>(p, ahead, next, stages + stage * Stage::kBytes, &join.note[warp][stage]);
       more_ahead = next_unit(p, ahead, ahead_at, share.size);
-      if (more_ahead) next = locate(p, ahead);
+      if (more_ahead) next = locate<W::kRows>(p, ahead);
     }
     copies_commit();
   };
   for (int stage = 0;; stage = stage + 1 == STAGES ? 0 : stage + 1) {
     copies_wait<STAGES - 1>();
     __syncwarp();
-    store_fresh<T, D>(p, join.note[warp][stage], stages + stage * Stage::kBytes);
+    store_fresh<T, D, W::kRows>(p, join.note[warp][stage], stages + stage * Stage::kBytes);
     work.step(p, now, stages + stage * Stage::kBytes, join.note[warp][stage].mask, scale2);
     __syncwarp();
     const Cursor done = now;
@@ -886,25 +904,26 @@ __global__ void __launch_bounds__(kTrackThreads) paged_track_kernel(PagedView c,
 struct AttendPlan {
   int dims = 0;    // dimensions a row is padded to
   int heads = 0;   // query heads of a group
+  int rows = 0;    // of a warp's part of a tile
   int stages = 0, per_sm = 0;
   size_t smem = 0;
 };
 
 template <typename T, typename W, int D, int STAGES>
 constexpr size_t attend_smem() {
-  return (size_t)kWarps * STAGES * RowStage<T, D>::kBytes + W::kSharedBytes + sizeof(JoinSpace<W>);
+  return (size_t)kWarps * STAGES * RowStage<T, D, W::kRows>::kBytes + W::kSharedBytes + sizeof(JoinSpace<W>);
 }
 
 template <typename F>
 auto with_kernel(int dtype, int head_dim, int rep, F&& f) {
-#define PJRTX_ATTEND(T, W, D, S, N) return f(paged_attend_kernel<T, W, D, S, N>, AttendPlan{D, W::kHeads, S, N, attend_smem<T, W, D, S>()})
+#define PJRTX_ATTEND(T, W, D, S, N) return f(paged_attend_kernel<T, W, D, S, N>, AttendPlan{D, W::kHeads, W::kRows, S, N, attend_smem<T, W, D, S>()})
 #define PJRTX_ATTEND_MMA(T, NB)                                                 \
-  if (head_dim <= 64) { using W = MmaWarp<T, 64, NB>; PJRTX_ATTEND(T, W, 64, 4, 2); }  \
-  if (head_dim <= 128) { using W = MmaWarp<T, 128, NB>; PJRTX_ATTEND(T, W, 128, NB == 1 ? 2 : 4, NB == 1 ? 2 : 1); } \
-  { using W = MmaWarp<T, 256, 1>; PJRTX_ATTEND(T, W, 256, 2, 1); }
+  if (head_dim <= 64) { using W = MmaWarp<T, 64, NB, 32>; PJRTX_ATTEND(T, W, 64, 2, 2); }  \
+  if (head_dim <= 128) { using W = MmaWarp<T, 128, NB, 16>; PJRTX_ATTEND(T, W, 128, NB == 1 ? 2 : 4, NB == 1 ? 2 : 1); } \
+  { using W = MmaWarp<T, 256, 1, 16>; PJRTX_ATTEND(T, W, 256, 2, 1); }
 #define PJRTX_ATTEND_FMA(H)                                                     \
   if (head_dim <= 64) { using W = FmaWarp<64, H>; PJRTX_ATTEND(float, W, 64, 2, 2); }  \
-  if (head_dim <= 128) { using W = FmaWarp<128, H>; PJRTX_ATTEND(float, W, 128, 2, 1); } \
+  if (head_dim <= 128) { using W = FmaWarp<128, H>; PJRTX_ATTEND(float, W, 128, 1, 2); } \
   { using W = FmaWarp<256, H>; PJRTX_ATTEND(float, W, 256, 1, 1); }
   if (dtype == kF32) {
     if (rep <= 4) { PJRTX_ATTEND_FMA(4) }
@@ -958,12 +977,13 @@ int paged_attend_launch(const PagedView& c, const PagedAttend& a, int sm_count, 
     const AttendLayout l = attend_layout(c, a.heads, plan, false, sm_count);
     char* space = static_cast<char*>(a.workspace);
     p.groups = (p.rep + plan.heads - 1) / plan.heads;
+    p.tile_rows = kWarps * plan.rows;
     p.space.lse2 = reinterpret_cast<float*>(space);
     p.space.counters = reinterpret_cast<unsigned*>(space + l.counters);
     p.space.partials = reinterpret_cast<float*>(space + l.partials);
     p.space.scores = reinterpret_cast<float*>(space + l.scores);
     if (!raise_smem_limit((const void*)kernel, (int)plan.smem)) return false;
-    const long long numbers = (long long)c.batch * c.kv_heads * p.groups * ((c.capacity() + kTileRows - 1) / kTileRows + kSegmentCost);
+    const long long numbers = (long long)c.batch * c.kv_heads * p.groups * ((c.capacity() + p.tile_rows - 1) / p.tile_rows + kSegmentCost);
     const long long blocks = std::min<long long>(numbers, (long long)sm_count * plan.per_sm);
     return launch_kernel(kernel, dim3((unsigned)blocks), dim3(kThreads), plan.smem, stream, pdl, p) == cudaSuccess;
   });
