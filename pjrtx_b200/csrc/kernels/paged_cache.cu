@@ -22,6 +22,8 @@ namespace {
 
 // ---- append --------------------------------------------------------------------------------------------------------
 
+// One piece of a key and of its value in flight a thread: with two of each 8192 rows of 57 sequences took 55.3 us, with four 63.3,
+// with one 52.8 (floor 48.7).
 constexpr int kAppendThreads = 256;
 
 __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(PagedView c, PagedAppend a, int pieces, int esize) {
@@ -39,7 +41,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(PagedView 
   const long long total = (long long)count * per_row;
   const long long step = (long long)gridDim.x * kAppendThreads;
   for (long long i = (long long)blockIdx.x * kAppendThreads + threadIdx.x; i < total; i += step) {
-    const int t = (int)(i / per_row), r = (int)(i - (long long)t * per_row);
+    const int t = total >> 31 ? (int)(i / per_row) : (int)((unsigned)i / (unsigned)per_row), r = (int)(i - (long long)t * per_row);
     const int g = r / pieces, piece = r - g * pieces;
     const long long row = paged_row(c, b, first + t);
     if (row < 0) continue;
@@ -372,7 +374,7 @@ __global__ void __launch_bounds__(kMoveThreads) paged_evict_move_kernel(PagedVie
 int paged_append_launch(const PagedView& c, const PagedAppend& a, bool pdl, cudaStream_t stream) {
   const int esize = (int)dtype_size(c.dtype), pieces = c.head_dim * esize / 16;
   const long long work = a.rows * c.kv_heads * pieces;
-  const long long blocks = std::min<long long>((work + kAppendThreads - 1) / kAppendThreads, 1024);
+  const long long blocks = std::min<long long>((work + kAppendThreads - 1) / kAppendThreads, 2048);
   return launch_kernel(paged_append_kernel, dim3((unsigned)std::max<long long>(blocks, 1), (unsigned)c.batch), dim3(kAppendThreads), 0,
                        stream, pdl, c, a, pieces, esize) == cudaSuccess;
 }

@@ -86,8 +86,10 @@ def _packer(cls):
 _pack_view, _pack_append, _pack_attend, _pack_evict, _pack_score, _pack_score_grad = map(
     _packer, (PagedView, PagedAppendArgs, PagedAttendArgs, PagedEvictArgs, TokenLogProbsArgs, TokenLogProbsBackwardArgs))
 
+_FLOATS = frozenset((P.F32, P.F16, P.BF16_CODE))
 _TENSOR_TYPES = {"float32": P.F32, "float16": P.F16, "bfloat16": P.BF16_CODE, "int32": P.S32}
 _codes: dict = {}  # a tensor library's dtype object -> element-type code, 0 for the others
+_types: dict = {}  # element-type code -> the dtype object seen last
 
 
 def _error(message: str):
@@ -110,6 +112,8 @@ def _code(x) -> int:
     code = _codes.get(dtype)
     if code is None:
         code = _codes[dtype] = _TENSOR_TYPES.get(str(dtype).split(".")[-1], 0)
+        if code:
+            _types[code] = dtype
     return code
 
 
@@ -206,6 +210,22 @@ class PagedCache:
 
     def _view(self, k_pages, v_pages, page_table, lengths, tokens, weights, positions) -> Tuple[int, bytes]:
         """The batch and the packed view."""
+        try:  # tensors that are as they have to be, checked in one go; anything else takes the checks one by one
+            kind, s32 = _types[self.dtype], _types[P.S32]
+            dims, strides, (batch,) = k_pages.shape, k_pages.stride(), lengths.shape
+            if (dims[1:] == self._page_dims and k_pages.dtype is kind and strides[3] == 1 and v_pages.shape == dims and v_pages.dtype is kind
+                    and v_pages.stride() == strides and page_table.shape == (batch, self.max_pages) and page_table.dtype is s32
+                    and page_table.is_contiguous() and lengths.dtype is s32 and lengths.is_contiguous()):
+                if weights is None and tokens is None and positions is None:
+                    return batch, _pack_view(k_pages.data_ptr(), v_pages.data_ptr(), dims[0], strides[0], strides[1], strides[2],
+                                             page_table.data_ptr(), self.max_pages, lengths.data_ptr(), batch, 0, 0, 0)
+                tracked = (batch, self.kv_heads, self.capacity)
+                return batch, _pack_view(k_pages.data_ptr(), v_pages.data_ptr(), dims[0], strides[0], strides[1], strides[2],
+                                         page_table.data_ptr(), self.max_pages, lengths.data_ptr(), batch,
+                                         _dense(tokens, "tokens", P.S32, (batch,)), _dense(weights, "weights", P.F32, tracked),
+                                         _dense(positions, "positions", P.S32, tracked))
+        except (AttributeError, KeyError, ValueError, TypeError, IndexError):
+            pass
         dims, batch_dims = _dims(k_pages), _dims(lengths)
         if len(dims) != 4 or dims[1:] != self._page_dims:
             raise _error(f"k_pages has shape {tuple(dims)}, (pages, {', '.join(map(str, self._page_dims))}) is needed")
@@ -231,10 +251,9 @@ class PagedCache:
         """Stores the first counts[b] of the rows k_new / v_new [batch, rows, kv_heads, head_dim] (None: all of them) as the
         last ones of the lengths[b] rows of each sequence; with tracking their weights become 0."""
         batch, view = self._view(k_pages, v_pages, page_table, lengths, tokens, weights, positions)
-        dims = _dims(k_new)
-        if len(dims) != 4:
-            raise _error(f"k_new has shape {tuple(dims)}, (batch, rows, KV heads, head dimension) is needed")
-        shape = (batch, dims[1], self.kv_heads, self.head_dim)
+        shape = _dims(k_new)
+        if len(shape) != 4 or shape[0] != batch or shape[2] != self.kv_heads or shape[3] != self.head_dim:
+            raise _error(f"k_new has shape {tuple(shape)}, ({batch}, rows, {self.kv_heads}, {self.head_dim}) is needed")
         k, strides = _rows(k_new, "k_new", self.dtype, shape)
         v = _twin(v_new, "v_new", "k_new", self.dtype, shape, strides)
         args = _pack_append(k, v, shape[1], strides[0], strides[1], strides[2], _dense(counts, "counts", P.S32, (batch,)))
@@ -246,21 +265,36 @@ class PagedCache:
         lse [batch, heads] its log-sum-exp. k_new / v_new [batch, kv_heads, head_dim] become row lengths[b] - 1 first. With
         tracking, weights[b, g, t] grows by what the query heads of KV head g give row t."""
         batch, view = self._view(k_pages, v_pages, page_table, lengths, tokens, weights, positions)
-        shape = (batch, self.heads, self.head_dim)
+        scale = self.head_dim ** -0.5 if scale is None else scale
+        fn, stream = self._lib.pjrtx_b200_paged_cache_attend, self._stream if stream is None else stream
+        shape, new_shape = (batch, self.heads, self.head_dim), (batch, self.kv_heads, self.head_dim)
+        try:  # tensors that are as they have to be, as in _view
+            kind, qs, os = _types[self.dtype], q.stride(), out.stride()
+            if (q.shape == shape and q.dtype is kind and qs[2] == 1 and out.shape == shape and out.dtype is kind and os[2] == 1
+                    and (lse is None or lse.shape == shape[:2] and lse.dtype is _types[P.F32] and lse.is_contiguous())):
+                if k_new is None and v_new is None:
+                    return self._call(fn, view, _pack_attend(q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1],
+                                                             0 if lse is None else lse.data_ptr(), 0, 0, 0, 0, scale), stream)
+                ns = k_new.stride()
+                if (k_new.shape == new_shape and k_new.dtype is kind and ns[2] == 1 and v_new.shape == new_shape and v_new.dtype is kind
+                        and v_new.stride() == ns):
+                    return self._call(fn, view, _pack_attend(q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1],
+                                                             0 if lse is None else lse.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), ns[0],
+                                                             ns[1], scale), stream)
+        except (AttributeError, KeyError, IndexError):
+            pass
         q_at, q_strides = _rows(q, "q", self.dtype, shape)
         out_at, out_strides = _rows(out, "out", self.dtype, shape)
         k = v = 0
         new_strides = (0, 0)
         if k_new is not None and v_new is not None:
-            shape = (batch, self.kv_heads, self.head_dim)
-            k, new_strides = _rows(k_new, "k_new", self.dtype, shape)
-            v = _twin(v_new, "v_new", "k_new", self.dtype, shape, new_strides)
+            k, new_strides = _rows(k_new, "k_new", self.dtype, new_shape)
+            v = _twin(v_new, "v_new", "k_new", self.dtype, new_shape, new_strides)
         elif k_new is not None or v_new is not None:
             raise _error("a new key and a new value go together")
         args = _pack_attend(q_at, q_strides[0], q_strides[1], out_at, out_strides[0], out_strides[1],
-                            _dense(lse, "lse", P.F32, (batch, self.heads)), k, v, new_strides[0], new_strides[1],
-                            self.head_dim ** -0.5 if scale is None else scale)
-        self._call(self._lib.pjrtx_b200_paged_cache_attend, view, args, stream)
+                            _dense(lse, "lse", P.F32, (batch, self.heads)), k, v, new_strides[0], new_strides[1], scale)
+        return self._call(fn, view, args, stream)
 
     def evict(self, k_pages, v_pages, page_table, lengths, tokens, weights, positions, keep: int, recent: int = 0, sinks: int = 0,
               lengths_out=None, weights_out=None, positions_out=None, stream: Optional[int] = None) -> None:
@@ -287,10 +321,16 @@ class PagedCache:
 
 def _logits(x):
     """Element type, rows, vocabulary, address and row stride."""
+    try:
+        (rows, vocab), code, strides = x.shape, _codes[x.dtype], x.stride()
+        if code in _FLOATS and strides[1] == 1:
+            return code, rows, vocab, x.data_ptr(), strides[0]
+    except (AttributeError, KeyError, ValueError):
+        pass
     dims, code = _dims(x), _code(x)
     if len(dims) != 2:
         raise _error(f"logits has shape {tuple(dims)}, (rows, vocabulary) is needed")
-    if code not in (P.F32, P.F16, P.BF16_CODE):
+    if code not in _FLOATS:
         raise _error(f"logits has element type {P.DTYPE_NAMES.get(code, 'other')}; f32, f16 and bf16 are supported")
     pointer, strides = _rows(x, "logits", code, dims)
     return code, dims[0], dims[1], pointer, strides[0]
