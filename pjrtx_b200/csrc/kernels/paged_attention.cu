@@ -5,6 +5,13 @@
 // A sequence without rows gives zeros and an lse of -inf. Rows beyond the length are not read: what a page holds there, or the
 // table names for them, does not matter. With a new row in the call, row length - 1 is taken from there and stored.
 //
+// Bound by memory: at one query position the products take 1 FLOP a byte and query head of a KV head, where the GPU has 250 (bf16).
+// So one launch reads every row once with as many bytes in flight as fit, and the softmax keeps a running maximum and sum. Measured
+// (bf16, heads of 128, 32 query and 8 KV heads; one call after the other, device time):
+//   32 sequences up to 2048 rows, 180 MB: 38.7 us (4.6 TB/s). Rows arrive for 23 us of it, at 7.8 TB/s; before them 4 us of launch,
+//   shares and first addresses, behind them 2 to 5 us of joins, and blocks on busier ways to memory take longer for equal shares.
+//   2 sequences up to 65 536 rows, 64 query heads, 447 MB: 87 us (5.2 TB/s). 1 sequence of 517 rows: 7.4 us, all of it these latencies.
+//
 // Tracking adds to weights[b, g, t] the weights e^(s_t - lse) of the query heads that read KV head g. They need the whole row's
 // lse, so the scores (4 bytes a head and key, against 4 * head_dim of key and value) go through the workspace to a second kernel.
 #include <cuda_bf16.h>
@@ -39,11 +46,16 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 // ---- division of the work ------------------------------------------------------------------------------------------
-// A unit is a tile of 96 rows of one (sequence, KV head, group of query heads), a segment what belongs to one of these. Segments
-// have numbers for their tiles and, behind them, for kSegmentCost more: what joining the warps and going on with another segment
+// A unit is a tile of rows (96; 192 for 16-bit heads up to 64) of one (sequence, KV head, group of query heads), a segment what
+// belongs to one of these. Segments have numbers for their tiles and, behind them, for kSegmentCost more: what joining the warps and going on with another segment
 // takes. The numbers are cut into equal shares, one for each block that fits the GPU at once; lengths are device data, so each
 // block adds them up itself. Where several blocks share a segment, each leaves (max, sum, values) in its slot of the workspace and
 // the block that arrives last joins them in block order.
+//
+// Six warps, two blocks an SM: with twelve warps and one block, whose joins stop all of an SM's loads, batch 32 takes 43.5 us, not
+// 38.7 (65 536 rows 82.6, not 87); with four warps and three blocks 65 536 rows take 88.8. kSegmentCost 2: a join and the next start
+// take 3 to 5 us, a tile 1.9; with 0, batch 32 takes 39.2 us and 30 000 rows of one sequence 33.9 (31.6). It costs the shortest
+// rows, where a block could have had more segments: 64 sequences of 100 rows 12.2 us, 10.3 with 0.
 
 constexpr int kWarps = 6, kThreads = kWarps * 32;
 constexpr int kSegmentCost = 2;
@@ -161,8 +173,9 @@ __device__ __forceinline__ Share share_of_block(const AttendArgs& p, long long* 
 }
 
 // ---- rows into shared memory ---------------------------------------------------------------------------------------
-// A warp works by itself: it fetches 16 rows of each tile with cp.async into stages of its own, so the warps of a block meet
-// only at the end of a segment. Rows outside the sequence (or without a page) are filled with zeros and masked.
+// A warp works by itself: it fetches its 16 or 32 rows of each tile with cp.async into stages of its own, so the warps of a block
+// meet only at the end of a segment. Row by row, since a row of a page is the longest run that is contiguous in every layout. Rows
+// outside the sequence (or without a page) are filled with zeros and masked.
 
 template <typename T, int D, int ROWS>
 struct RowStage {
@@ -327,7 +340,8 @@ __device__ __forceinline__ unsigned transpose(unsigned a) {
 // 16-bit types: rows and dimensions are the long sides of the products, heads the eight columns of m16n8k16, so that up to eight
 // query heads cost no more than one: scores^T [16 rows x heads] = K q^T, values^T [dims x heads] += V^T p^T. A probability goes in
 // as two 16-bit numbers, its rounding and what that leaves off: rounded to one, it would be as far off as the result's own rounding.
-// Lane i holds heads (i % 4) * 2 and + 1 of every eight.
+// Tensor memory wants 64 rows at least on its M side and the scores through it to the softmax and back; with 1/60 of
+// its rate used (four heads) there is nothing to win by that. Lane i holds heads (i % 4) * 2 and + 1 of every eight.
 template <typename T, int D, int NB, int ROWS>
 struct MmaWarp {
   static constexpr int kHeads = 8 * NB, kRows = ROWS, R = ROWS / 16;
@@ -402,7 +416,7 @@ struct MmaWarp {
       }
     if (p.c.weights) {
 #pragma unroll
-      for (int r = 0; r < R; r++) store_scores(p, u, s[r], r, mask);
+      for (int r = 0; r < R; r++) store_scores(p, u, s[r], r);
     }
     if (__any_sync(~0u, grows)) {
 #pragma unroll
@@ -459,10 +473,10 @@ struct MmaWarp {
   }
 
   // Of 16 rows, the r-th of the warp's.
-  __device__ __forceinline__ void store_scores(const AttendArgs& p, const Cursor& u, const float (&s)[NB][4], int r, unsigned mask) const {
+  __device__ __forceinline__ void store_scores(const AttendArgs& p, const Cursor& u, const float (&s)[NB][4], int r) const {
     const int lane = threadIdx.x % 32, g = u.group / p.groups, h0 = (u.group % p.groups) * kHeads;
     const int t = u.tile * p.tile_rows + (threadIdx.x / 32) * ROWS + r * 16 + lane / 4;
-    const bool lo = mask >> (r * 16 + lane / 4) & 1, hi = mask >> (r * 16 + lane / 4 + 8) & 1;
+    const bool lo = t < u.length, hi = t + 8 < u.length;  // a row without a page has -inf
     float* to = p.space.scores + (((long long)u.b * p.c.kv_heads + g) * p.c.page_size * p.c.max_pages + t) * p.rep + h0;
 #pragma unroll
     for (int n = 0; n < NB; n++)
@@ -561,9 +575,9 @@ struct FmaWarp {
       s[h] = there ? s[h] * scale2 : -INFINITY;
       grows |= !(s[h] <= m[h]);
     }
-    if (p.c.weights && there && lane < 16) {
+    const int t = u.tile * p.tile_rows + (threadIdx.x / 32) * kRows + lane;
+    if (p.c.weights && lane < 16 && t < u.length) {
       const int g = u.group / p.groups, h0 = (u.group % p.groups) * H;
-      const int t = u.tile * p.tile_rows + (threadIdx.x / 32) * kRows + lane;
       float* to = p.space.scores + (((long long)u.b * p.c.kv_heads + g) * p.c.page_size * p.c.max_pages + t) * p.rep + h0;
 #pragma unroll
       for (int h = 0; h < H; h++)
@@ -867,8 +881,9 @@ __global__ void __launch_bounds__(kThreads, PER_SM) paged_attend_kernel(const __
 
 constexpr int kTrackThreads = 256;
 
-// A thread a row. What it needs is requested at once, also where the row turns out not to be there: the kernel is a few
-// microseconds behind the attention, and most of them are one trip to memory.
+// weights[t] += sum over heads of e^(s_t - lse). A thread a row. What it needs is requested at once, also where the row turns out
+// not to be there: the kernel is a few microseconds behind the attention, and most of them are one trip to memory. 16 sequences up
+// to 4096 rows: 6 us of the 45 of both kernels (13 MB of scores and weights, mostly from L2).
 template <int REP>  // query heads of a KV head; 0: any number
 __global__ void __launch_bounds__(kTrackThreads) paged_track_kernel(PagedView c, AttendSpace space, int heads, int appended) {
   PJRTX_PDL_PROLOGUE();
@@ -914,12 +929,20 @@ constexpr size_t attend_smem() {
   return (size_t)kWarps * STAGES * RowStage<T, D, W::kRows>::kBytes + W::kSharedBytes + sizeof(JoinSpace<W>);
 }
 
+// Dimensions are padded to 64, 128 or 256, and each width gets the stages and blocks an SM that its shared memory and registers allow:
+//   16 bits, 64: 32 rows a warp and step, since 16 (4 KB) wait longer for each other than they take: 46.6 us, not 42.1, where 128 MB
+//   are read. For 128 the same costs a block's second stage: 39.5 us, not 38.7.
+//   16 bits, over 8 query heads a KV head: 16 columns at once, which read the rows once but leave registers for one block (three
+//   stages; four: 24.9, not 24.0; two blocks spill: 33.9). 16 heads, 32 sequences up to 8000 rows: 53.6 us, as two groups of eight
+//   56.5; 12 heads, 8 sequences: 16.2, not 17.1; with little to read the two groups are the faster (2 sequences: 17.9, not 21.8).
+//   f32, 128: one stage and two blocks, not two stages and one: 63.4 us, not 66.8, at batch 32 (one short sequence 13.7, not 13.1).
+//   f32, up to 4 query heads a KV head: arithmetic for four; with that for eight 35.1 us, not 28.1.
 template <typename F>
 auto with_kernel(int dtype, int head_dim, int rep, F&& f) {
 #define PJRTX_ATTEND(T, W, D, S, N) return f(paged_attend_kernel<T, W, D, S, N>, AttendPlan{D, W::kHeads, W::kRows, S, N, attend_smem<T, W, D, S>()})
 #define PJRTX_ATTEND_MMA(T, NB)                                                 \
   if (head_dim <= 64) { using W = MmaWarp<T, 64, NB, 32>; PJRTX_ATTEND(T, W, 64, 2, 2); }  \
-  if (head_dim <= 128) { using W = MmaWarp<T, 128, NB, 16>; PJRTX_ATTEND(T, W, 128, NB == 1 ? 2 : 4, NB == 1 ? 2 : 1); } \
+  if (head_dim <= 128) { using W = MmaWarp<T, 128, NB, 16>; PJRTX_ATTEND(T, W, 128, NB == 1 ? 2 : 3, NB == 1 ? 2 : 1); } \
   { using W = MmaWarp<T, 256, 1, 16>; PJRTX_ATTEND(T, W, 256, 2, 1); }
 #define PJRTX_ATTEND_FMA(H)                                                     \
   if (head_dim <= 64) { using W = FmaWarp<64, H>; PJRTX_ATTEND(float, W, 64, 2, 2); }  \
