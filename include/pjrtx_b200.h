@@ -514,8 +514,8 @@ int pjrtx_b200_paged_cache_append(PjrtxB200PagedCache *cache, const PjrtxB200Pag
                                   const PjrtxB200PagedAppendArgs *args, void *stream);
 
 /* Attention of one query position per sequence over its rows: out = softmax(scale * q . k) v, lse = ln sum e^(scale * q . k).
- * A sequence without rows gives zeros and -inf, and so do scores that are all -inf. NaN in a row that counts makes the results it
- * enters NaN, and so may an infinite value; what lies beyond the length enters nothing. With k_new / v_new, row lengths[b] - 1 is taken from there and stored.
+ * A sequence without rows gives zeros and -inf, and so do scores that are all -inf. Infinities and NaN in rows that count go on
+ * as in the formula, with probabilities below 2^-126 of the largest as zero; what lies beyond the length enters nothing. With k_new / v_new, row lengths[b] - 1 is taken from there and stored.
  * Tracking: weights[b, g, t] grows by the weights that the query heads of KV head g give row t (a new row's starts with
  * them, its position is tokens[b] - 1). */
 typedef struct PjrtxB200PagedAttendArgs {

@@ -306,7 +306,13 @@ template <> struct Mma16<__nv_bfloat16> {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const unsigned*>(&h);
   }
-  static __device__ __forceinline__ float2 unpack(unsigned w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+  static constexpr float kLift = 0.f;
+  // (a, b) >= 0 as the sum of two pairs, the first rounded towards zero.
+  static __device__ __forceinline__ uint2 split(float a, float b) {
+    const float ra = a - __uint_as_float(__float_as_uint(a) & 0xffff0000u), rb = b - __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+    constexpr float kLeast = 1.1754944e-38f;  // 2^-126
+    return make_uint2(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632), pack(fmaxf(ra, kLeast), fmaxf(rb, kLeast)));
+  }
   static __device__ __forceinline__ void mma(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -317,7 +323,16 @@ template <> struct Mma16<__half> {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const unsigned*>(&h);
   }
-  static __device__ __forceinline__ float2 unpack(unsigned w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+  static constexpr float kLift = 15.f;
+  static __device__ __forceinline__ uint2 split(float a, float b) {
+    constexpr float kLeast = 5.9604645e-8f;  // 2^-24
+    if (a > 0.f) a = fmaxf(a, kLeast);
+    if (b > 0.f) b = fmaxf(b, kLeast);
+    unsigned w;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
+    const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return make_uint2(w, pack(fmaxf(a - back.x, kLeast), fmaxf(b - back.y, kLeast)));
+  }
   static __device__ __forceinline__ void mma(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -339,7 +354,9 @@ __device__ __forceinline__ unsigned transpose(unsigned a) {
 
 // 16-bit types: rows and dimensions are the long sides of the products, heads the eight columns of m16n8k16, so that up to eight
 // query heads cost no more than one: scores^T [16 rows x heads] = K q^T, values^T [dims x heads] += V^T p^T. A probability goes in
-// as two 16-bit numbers, its rounding and what that leaves off: rounded to one, it would be as far off as the result's own rounding.
+// as two 16-bit numbers, itself cut off and the rest: as one, it would be as far off as the result's own rounding. Neither is zero or
+// negative where the probability is above zero, so that an infinite value stays infinite, and f16 has 2^15 times the probabilities:
+// what is below 2^-39 of the largest counts as that, where plain f16 would lose 65 536 rows of 2^-25 each, 0.2 % of a result.
 // Tensor memory wants 64 rows at least on its M side and the scores through it to the softmax and back; with 1/60 of
 // its rate used (four heads) there is nothing to win by that. Lane i holds heads (i % 4) * 2 and + 1 of every eight.
 template <typename T, int D, int NB, int ROWS>
@@ -444,17 +461,16 @@ struct MmaWarp {
       for (int n = 0; n < NB; n++) {
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-          const float from = m[n][j] == -INFINITY ? 0.f : m[n][j];
+          const float from = m[n][j] == -INFINITY ? 0.f : m[n][j] - Mma16<T>::kLift;
           s[r][n][j] = exp2_fast(s[r][n][j] - from);
           s[r][n][2 + j] = exp2_fast(s[r][n][2 + j] - from);
           l[n][j] += s[r][n][j] + s[r][n][2 + j];
         }
 #pragma unroll
         for (int k = 0; k < 2; k++) {
-          const unsigned b = Mma16<T>::pack(s[r][n][2 * k], s[r][n][2 * k + 1]);
-          const float2 back = Mma16<T>::unpack(b);
-          big[r][n][k] = transpose(b);
-          small[r][n][k] = transpose(Mma16<T>::pack(s[r][n][2 * k] - back.x, s[r][n][2 * k + 1] - back.y));
+          const uint2 parts = Mma16<T>::split(s[r][n][2 * k], s[r][n][2 * k + 1]);
+          big[r][n][k] = transpose(parts.x);
+          small[r][n][k] = transpose(parts.y);
         }
       }
     const unsigned v_lane = v_at + ((lane / 16) * 8 + lane % 8) * kPitch + (lane / 8 % 2) * 16;
@@ -489,7 +505,7 @@ struct MmaWarp {
       }
   }
 
-  // Leaves this warp's maxima and sums in stat[head][2].
+  // Leaves this warp's references (the maxima, but for the lift) and sums in stat[head][2].
   __device__ __forceinline__ void statistics(float* stat) {
     const int lane = threadIdx.x % 32;
 #pragma unroll
@@ -499,7 +515,7 @@ struct MmaWarp {
 #pragma unroll
         for (int d = 4; d < 32; d *= 2) l[n][j] += __shfl_xor_sync(~0u, l[n][j], d);
         if (lane < 4) {
-          stat[2 * (n * 8 + lane * 2 + j)] = m[n][j];
+          stat[2 * (n * 8 + lane * 2 + j)] = m[n][j] - Mma16<T>::kLift;
           stat[2 * (n * 8 + lane * 2 + j) + 1] = l[n][j];
         }
       }

@@ -342,6 +342,58 @@ def test_attend_extreme_scores(gpu_backend):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("heads,kv_heads,head_dim", [(8, 2, 128), (12, 1, 128), (4, 2, 64), (3, 1, 256)])
+def test_attend_infinite_values_at_any_probability(gpu_backend, dtype, heads, kv_heads, head_dim):
+    """An infinite value makes its dimension infinite however small its (f32) probability is, and nothing else."""
+    c = _Case(dtype, heads, kv_heads, head_dim, 16, [300, 1, 40], seed=head_dim)
+    torch = c.torch
+    q = torch.zeros((3, heads, head_dim), dtype=_torch_type(dtype), device="cuda")
+    q[:, :, 0] = 1
+    pg, row = c.places(0, 300)
+    c.k[pg, row, :, 1:] = 0
+    c.k[pg, row, :, 0] = -c.torch.rand((300, kv_heads), generator=c.gen, device="cuda").to(q.dtype) * 60
+    c.k[pg[17], row[17], :, 0] = 0.5  # the largest
+    c.k[pg[40], row[40], :, 0] = -math.inf  # probability 0 with finite values: nothing
+    for j, (t, score) in enumerate([(17, 0.5), (3, -5.0), (100, -17.0), (200, -30.0), (299, -60.0), (150, -80.0)]):
+        c.k[pg[t], row[t], :, 0] = score
+        c.v[pg[t], row[t], :, 2 * j] = math.inf
+        c.v[pg[t], row[t], :, 2 * j + 1] = -math.inf
+    c.v[pg[20], row[20], :, 0] = -math.inf  # both: NaN
+    c.v[pg[8], row[8], :, 1] = math.nan
+    pg, row = c.places(1, 1)
+    c.v[pg[0], row[0], :, 3] = -math.inf
+    out = torch.empty_like(q)
+    c.handle(gpu_backend).attend(q, c.k, c.v, c.table, c.lengths, out, scale=1.0, stream=_stream())
+    want, _, _, bound, _, _ = c.attention(q, 1.0)
+    odd = ~want.isfinite()
+    assert int(odd[0, 0].sum()) == 12 and int(odd[1, 0].sum()) == 1 and not odd[2].any()
+    got = out.double()
+    assert ((got == want) | (got.isnan() & want.isnan()))[odd].all(), (got[odd], want[odd])
+    _within(out[~odd], want[~odd], bound[~odd], "beside the infinities")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("head_dim,score", [(64, -17.3), (128, -21.0), (256, -14.0)])
+def test_attend_many_small_probabilities(gpu_backend, dtype, head_dim, score):
+    """Thousands of rows that each weigh less than a 16-bit number can say, against one with all the rest and values of zero."""
+    c = _Case(dtype, 4, 1, head_dim, 16, [6000], seed=7)
+    q = c.torch.zeros((1, 4, head_dim), dtype=_torch_type(dtype), device="cuda")
+    q[:, :, 0] = 1
+    pg, row = c.places(0, 6000)
+    c.k[pg, row, 0, 0] = score
+    c.k[pg[1234], row[1234], 0, 0] = 0
+    c.v[pg, row] = c.v[pg, row].abs() * 2000
+    c.v[pg[1234], row[1234]] = 0
+    out = c.torch.empty_like(q)
+    c.handle(gpu_backend).attend(q, c.k, c.v, c.table, c.lengths, out, scale=1.0, stream=_stream())
+    want, _, _, bound, _, _ = c.attention(q, 1.0)
+    assert (want > 4 * bound).all()
+    _within(out, want, bound, "out")
+
+
+@pytest.mark.gpu
 def test_attend_offsets_beyond_32_bits(gpu_backend):
     import torch
 
