@@ -12,6 +12,10 @@
 // (value descending, id ascending) the k first elements lie in the k intervals that come first by (maximum descending,
 // position ascending): an element of any other interval has k elements before it, the maxima of those. So chunk maxima are left
 // in shared memory on the way, and afterwards the k first chunks are read again, then the k first of their vectors.
+//
+// Bound by memory, and where the logits are 16 bits wide nearly as much by the exponents' instructions: 4.5 a logit (two at a time).
+// 4096 rows of 128256 bf16 logits (1.05 GB) take 166 us without alternatives, 185 with five, 161 at the rate of a copy; one row,
+// 0.26 MB, 8 us of latencies. The gradient reads and writes each logit once: 2048 rows of 128256 f32 315 us (2.1 GB, 6.7 TB/s).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -215,8 +219,11 @@ __device__ __forceinline__ Stats joined(Stats a, Stats b, float c) {
 
 // Threads of a block. Small ones where there are rows enough to fill the GPU with them: eight share an SM, so that what one row's
 // alternatives wait for is hidden by seven others (4096 rows of 128256 bf16 logits, 5 alternatives: 185 us, 193 with four blocks of
-// 256); where a cluster has one row, larger ones (one row: 8.7 us, 10.3 with 128).
-constexpr int kScoreThreadsMany = 128, kScoreThreadsFew = 256, kScoreThreadsOfSm = 1024;
+// 256); where a cluster has one row, larger ones (one row: 8.7 us, 10.3 with 128). One warp, up to 32 of them an SM, for a row of
+// a few batches, where the others of a block would have none: 4000 rows of 1024 7.0 us, 13.3 with 128 threads (5 alternatives 14.3,
+// 26.0), of 4000 12.4 (18.8), of 5000 14.5 (22.2); but 20 alternatives of 5000 f32 logits 73 us, not 59, and with few rows, which
+// would have had a block of 256 each, 5 alternatives of 1500 logits 8.1 us, not 6.3.
+constexpr int kScoreThreadsMany = 128, kScoreThreadsFew = 256, kScoreThreadsShort = 32, kScoreThreadsOfSm = 1024;
 constexpr int kScoreVectors = 4;  // 16-byte loads of a batch; the next batch's are in flight while one is added up
 constexpr int kChunk = 256;       // logits
 constexpr int kScoreClusterMax = 8;
@@ -312,13 +319,22 @@ __device__ __forceinline__ void select(Get&& get, int n, int k, Entry* out, Entr
   }
 }
 
+template <int THREADS>
 struct ScoreShared {
-  Stats stats[kScoreThreadsFew / 32];
-  Stats cluster_stats[kScoreClusterMax];                    // of the rank-0 block
-  Entry cluster_top[kScoreClusterMax * kScoreTopMax];       // of the rank-0 block
+  static constexpr int kRanks = THREADS == kScoreThreadsShort ? 1 : kScoreClusterMax;
+  Stats stats[THREADS / 32];
+  Stats cluster_stats[kRanks];               // of the rank-0 block
+  Entry cluster_top[kRanks * kScoreTopMax];  // of the rank-0 block
   Entry chosen[kScoreTopMax], spare[kFew];
   int n;
 };
+
+// Entries that the chosen chunks' vectors or the chosen vectors' elements take.
+template <int V>
+constexpr __host__ __device__ int score_room(int top, int chunks) {
+  const int vectors = (top < chunks ? top : chunks) * (kChunk / V);
+  return vectors > top * V ? vectors : top * V;
+}
 
 __device__ __forceinline__ float warp_max(float x) {
   float y;
@@ -332,9 +348,9 @@ __global__ void __launch_bounds__(THREADS, kScoreThreadsOfSm / THREADS) token_sc
   constexpr int V = Logit<T>::V;
   constexpr int kVectorsOfChunk = kChunk / (32 * V);              // 16-byte loads a thread has of a chunk
   constexpr int kChunks = kScoreVectors / kVectorsOfChunk;        // chunks of a batch
-  extern __shared__ Entry list[];                                            // TOP: vectors, or elements, of the chosen chunks
-  float* chunk_max = reinterpret_cast<float*>(list + a.top * (kChunk / V));  // TOP: of this block's chunks
-  __shared__ ScoreShared sh;
+  extern __shared__ float chunk_max[];  // TOP: of this block's chunks
+  Entry* list = reinterpret_cast<Entry*>(chunk_max + (segment_chunks + 1) / 2 * 2);  // TOP: of vectors, or elements, of the chosen ones
+  __shared__ ScoreShared<THREADS> sh;
   PJRTX_PDL_PROLOGUE();
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -476,7 +492,7 @@ __global__ void __launch_bounds__(THREADS, kScoreThreadsOfSm / THREADS) token_sc
     __syncthreads();
     // What reaches the last of their maxima: elements at once where they are few, else vectors first and then theirs.
     const unsigned bound = n < k ? 0u : (unsigned)(sh.chosen[k - 1] >> 32);
-    const int room = k * (kChunk / V);  // all their vectors
+    const int room = score_room<V>(k, segment_chunks);
     auto gather = [&](bool elements) {
       for (int j = warp; j < k && sh.chosen[j] != 0; j += kScoreWarps) {
         const int chunk = chunk0 + (int)position_of(sh.chosen[j]);
@@ -503,9 +519,12 @@ __global__ void __launch_bounds__(THREADS, kScoreThreadsOfSm / THREADS) token_sc
         }
       }
     };
-    gather(true);
-    __syncthreads();
-    if (sh.n > room) {  // long ties
+    const bool by_vectors = n < k && min(end, chunk1 * kChunk) - chunk0 * kChunk > room;  // fewer chunks than places: no bound
+    if (!by_vectors) {
+      gather(true);
+      __syncthreads();
+    }
+    if (by_vectors || sh.n > room) {  // or long ties
       __syncthreads();
       if (threadIdx.x == 0) sh.n = 0;
       __syncthreads();
@@ -516,9 +535,9 @@ __global__ void __launch_bounds__(THREADS, kScoreThreadsOfSm / THREADS) token_sc
       if (threadIdx.x == 0) sh.n = 0;
       if (warp == 0) select([&](int i) { return list[i]; }, vectors, k, sh.chosen, sh.spare);
       __syncthreads();
-      if ((int)threadIdx.x < k && sh.chosen[threadIdx.x] != 0) {
-        const unsigned limit = vectors < k ? 0u : (unsigned)(sh.chosen[k - 1] >> 32);
-        const int p = (int)position_of(sh.chosen[threadIdx.x]);
+      const unsigned limit = vectors < k ? 0u : (unsigned)(sh.chosen[k - 1] >> 32);
+      for (int j = threadIdx.x; j < k && sh.chosen[j] != 0; j += THREADS) {
+        const int p = (int)position_of(sh.chosen[j]);
         float f[V];
         Logit<T>::unpack(load(p), f);
 #pragma unroll
@@ -568,6 +587,8 @@ __global__ void __launch_bounds__(THREADS, kScoreThreadsOfSm / THREADS) token_sc
 
 // ---- gradient ------------------------------------------------------------------------------------------------------
 
+// Four vectors a thread in flight, eight blocks an SM, both sides past the caches (nothing is read twice): 3111 rows of 128256 bf16
+// logits with an entropy term 253 us, floor 244; with the caches and one logit at a time 317.
 constexpr int kGradThreads = 128;
 constexpr int kGradUnroll = 4;
 
@@ -649,13 +670,17 @@ __global__ void __launch_bounds__(kGradThreads) token_score_grad_kernel(TokenSco
 template <typename T, int THREADS>
 int score_launch_of(const TokenScore& s, int sm_count, bool pdl, cudaStream_t stream) {
   const int chunks = (int)((s.vocab + Logit<T>::V - 1 + kChunk - 1) / kChunk);
-  // A cluster for each row: as many blocks as fill the GPU, none with less than a batch for every warp.
+  // A cluster for each row: as many blocks as fit the GPU at once, none with less than a batch for every warp. A few more than fit
+  // wait for the others to end: 150 rows of 32000 7.5 us by three blocks, 9.0 by four (600 of 592; with 20 alternatives 12.5 and
+  // 17.4). Only long rows gain by it: 300 of 128256 23.2 us by two, 28.9 by one.
   const int batch_chunks = THREADS * kScoreVectors * Logit<T>::V / kChunk;
-  int ranks = 1;
-  while (ranks < kScoreClusterMax && s.rows * ranks * THREADS < (long long)kScoreThreadsOfSm * sm_count && chunks > ranks * batch_chunks) ranks *= 2;
-  const int segment = (chunks + ranks - 1) / ranks;
+  const long long slots = (long long)kScoreThreadsOfSm / THREADS * sm_count;
+  long long ranks = std::max<long long>(1, slots / s.rows);
+  if ((ranks + 1) * s.rows <= slots + slots / 16 && chunks / (ranks + 1) >= 200) ranks++;
+  ranks = std::min({ranks, (long long)ScoreShared<THREADS>::kRanks, (chunks + batch_chunks - 1ll) / batch_chunks});
+  const int segment = (int)((chunks + ranks - 1) / ranks);
   const bool top = s.top > 0;
-  const size_t smem = top ? (size_t)s.top * (kChunk / Logit<T>::V) * sizeof(Entry) + (size_t)segment * sizeof(float) : 0;
+  const size_t smem = top ? score_room<Logit<T>::V>(s.top, segment) * sizeof(Entry) + (size_t)(segment + 1) / 2 * sizeof(Entry) : 0;
   auto kernel = top ? token_score_kernel<T, true, THREADS> : token_score_kernel<T, false, THREADS>;
   if (smem > 32 * 1024 && !raise_smem_limit((const void*)kernel, 200 * 1024)) return 0;
   cudaLaunchConfig_t cfg = {};
@@ -665,15 +690,20 @@ int score_launch_of(const TokenScore& s, int sm_count, bool pdl, cudaStream_t st
   cfg.stream = stream;
   cudaLaunchAttribute attr[3];
   cfg.numAttrs = fill_launch_attributes(attr, pdl);
-  attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-  attr[cfg.numAttrs].val.clusterDim = {(unsigned)ranks, 1, 1};
-  cfg.numAttrs++;
+  if (ranks > 1) {  // a cluster of one starts slower: 4000 rows of 1024 17.5 us, without 13.3
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim = {(unsigned)ranks, 1, 1};
+    cfg.numAttrs++;
+  }
   cfg.attrs = attr;
   return cudaLaunchKernelEx(&cfg, kernel, s, segment) == cudaSuccess;
 }
 
 template <typename T>
 int score_launch(const TokenScore& s, int sm_count, bool pdl, cudaStream_t stream) {
+  const long long chunks = (s.vocab + Logit<T>::V - 1 + kChunk - 1) / kChunk;
+  if (chunks <= (s.rows * kScoreThreadsFew < (long long)kScoreThreadsOfSm * sm_count ? 5 : s.top > 8 ? 16 : 24))
+    return score_launch_of<T, kScoreThreadsShort>(s, sm_count, pdl, stream);
   return s.rows * kScoreThreadsMany >= (long long)kScoreThreadsOfSm * sm_count ? score_launch_of<T, kScoreThreadsMany>(s, sm_count, pdl, stream)
                                                                                : score_launch_of<T, kScoreThreadsFew>(s, sm_count, pdl, stream);
 }

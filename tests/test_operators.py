@@ -683,6 +683,30 @@ def test_token_log_probs_of_masked_and_tied_rows(gpu_backend, dtype, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows,vocab,top,stride", [
+    (700, 1024, 5, 1024), (5, 1024, 64, 1027), (650, 131, 33, 133), (601, 4000, 20, 4001), (600, 6137, 8, 6137), (1300, 3, 3, 3),
+    (84, 30011, 5, 30011), (98, 40000, 3, 40001), (118, 33001, 20, 33001), (197, 9000, 1, 9000), (296, 130000, 2, 130000)])
+def test_token_log_probs_by_warps_and_by_any_number_of_blocks(gpu_backend, dtype, rows, vocab, top, stride):
+    """Rows of a few batches and clusters of each size, with masked logits, ties and empty rows among them."""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(vocab)
+    x = torch.empty((rows, stride), device="cuda")
+    x[:, :vocab] = torch.randn((rows, vocab), generator=gen, device="cuda") * 3
+    x[1::3, :vocab].masked_fill_(torch.rand((len(range(1, rows, 3)), vocab), generator=gen, device="cuda") < 0.9, -math.inf)
+    x[1::3, vocab - 1] = 0.5
+    x[2::3] = x[2::3].round()
+    x[3] = -math.inf
+    logits = x.to(_torch_type(dtype))[:, :vocab]
+    tokens = torch.randint(-1, vocab, (rows,), generator=gen, device="cuda", dtype=torch.int32)
+    out = _score(gpu_backend, logits, tokens, top)
+    keep = [i for i in range(rows) if i != 3]
+    _check_score({n: v[keep] for n, v in out.items()}, logits[keep], tokens[keep], top, 1.0)
+    assert out["lse"][3] == -math.inf and out["top_ids"][3].tolist() == list(range(top))
+
+
+@pytest.mark.gpu
 def test_token_log_probs_of_nan_and_infinity(gpu_backend):
     import torch
 
