@@ -20,6 +20,7 @@
 #include <algorithm>
 
 #include "../common.h"
+#include "arith.cuh"
 #include "kernels.h"
 #include "paged.cuh"
 
@@ -34,19 +35,8 @@ template <> __device__ __forceinline__ float from_float(float v) { return v; }
 template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
 
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float y;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-  return y;
-}
-
 // ---- division of the work ------------------------------------------------------------------------------------------
-// A unit is a tile of rows (96; 192 for 16-bit heads up to 64) of one (sequence, KV head, group of query heads), a segment what
+// A unit is a tile of rows (six warps have 8, 16 or 32 each) of one (sequence, KV head, group of query heads), a segment what
 // belongs to one of these. Segments have numbers for their tiles and, behind them, for kSegmentCost more: what joining the warps and going on with another segment
 // takes. The numbers are cut into equal shares, one for each block that fits the GPU at once; lengths are device data, so each
 // block adds them up itself. Where several blocks share a segment, each leaves (max, sum, values) in its slot of the workspace and
@@ -173,7 +163,7 @@ __device__ __forceinline__ Share share_of_block(const AttendArgs& p, long long* 
 }
 
 // ---- rows into shared memory ---------------------------------------------------------------------------------------
-// A warp works by itself: it fetches its 16 or 32 rows of each tile with cp.async into stages of its own, so the warps of a block
+// A warp works by itself: it fetches its 8, 16 or 32 rows of each tile with cp.async into stages of its own, so the warps of a block
 // meet only at the end of a segment. Row by row, since a row of a page is the longest run that is contiguous in every layout. Rows
 // outside the sequence (or without a page) are filled with zeros and masked.
 
@@ -534,15 +524,41 @@ struct MmaWarp {
   }
 };
 
-// f32: CUDA cores. Scores: lane i has row i % 16 and one half of the dimensions. Values: lane i has D / 32 neighbouring dimensions.
-template <int D, int H>
+// f32: CUDA cores, two products an instruction. Scores: eight lanes beside each other have a row, pieces of 16 bytes in turn, so that
+// a piece of a query serves four rows; the sums are exchanged so that a lane ends with the scores of one head. Values: lane i has
+// D / 32 neighbouring dimensions of all heads. With eight heads a KV head this is bound by what a warp waits for between its own
+// instructions (17 sequences up to 3877 rows of 8 KV heads of 128, 360 MB: 89 us, issue slots 39 % used), with fewer by memory.
+template <int D, int H, int ROWS>
 struct FmaWarp {
-  static constexpr int kHeads = H, kRows = 16, V = D / 32;
+  static constexpr int kHeads = H, kRows = ROWS, V = D / 32;
+  static constexpr int R = ROWS / 4, kOwn = R * H / 8;  // rows of eight lanes; scores a lane ends with
+  static_assert(kOwn > 0);
   static constexpr int kSharedBytes = H * D * 4 + kWarps * kRows * H * 4;  // queries; probabilities of every warp
-  float o[H][V];
-  float m[H], l[H];
+  Pair o[H][V / 2];
+  float m, l;  // of this lane's head
   const float* queries;
   float* probabilities;
+
+  static __device__ __forceinline__ int head_of(int lane) { return lane % 8 * H / 8; }
+  static __device__ __forceinline__ int row_of(int lane, int i) { return lane / 8 + 4 * (lane % 8 * kOwn % R + i); }
+  // Of 2 N sums of the lane and as many of the one `D2` further, each keeps one half and gets the other's share of it.
+  template <int N, int D2>
+  static __device__ __forceinline__ void exchange(float (&s)[R * H]) {
+    const bool upper = threadIdx.x & D2;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const float keep = upper ? s[N + i] : s[i], give = upper ? s[i] : s[N + i];
+      s[i] = keep + __shfl_xor_sync(~0u, give, D2);
+    }
+  }
+  // Over the lanes that have the same head.
+  template <typename F>
+  static __device__ __forceinline__ float over_head(float x, F&& join) {
+    if (H <= 4) x = join(x, __shfl_xor_sync(~0u, x, 1));
+    if (H <= 2) x = join(x, __shfl_xor_sync(~0u, x, 2));
+    x = join(x, __shfl_xor_sync(~0u, x, 8));
+    return join(x, __shfl_xor_sync(~0u, x, 16));
+  }
 
   __device__ __forceinline__ void load(const AttendArgs&, const Cursor&) {}
   __device__ __forceinline__ void start(const AttendArgs& p, const Cursor& u, char* shared) {
@@ -558,97 +574,113 @@ struct FmaWarp {
     }
     __syncthreads();
 #pragma unroll
-    for (int h = 0; h < H; h++) {
+    for (int h = 0; h < H; h++)
 #pragma unroll
-      for (int i = 0; i < V; i++) o[h][i] = 0.f;
-      m[h] = -INFINITY;
-      l[h] = 0.f;
-    }
+      for (int i = 0; i < V / 2; i++) o[h][i] = pair_of(0.f, 0.f);
+    m = -INFINITY;
+    l = 0.f;
   }
 
   __device__ __forceinline__ void step(const AttendArgs& p, const Cursor& u, const char* stage, unsigned mask, float scale2) {
     constexpr int kPitch = RowStage<float, D, kRows>::kPitch;
     const int lane = threadIdx.x % 32;
-    float s[H];
+    float s[R * H];  // [head][row]
+    constexpr int kAtOnce = H == 8 ? 2 : R;  // rows, as registers go
 #pragma unroll
-    for (int h = 0; h < H; h++) s[h] = 0.f;
-    const char* k = stage + (lane % 16) * kPitch;
-#pragma unroll 4
-    for (int i = 0; i < D / 8; i++) {  // the halves alternate in pieces of 16 bytes
-      const int d = (2 * i + lane / 16) * 4;
-      const float4 x = *reinterpret_cast<const float4*>(k + d * 4);
+    for (int j0 = 0; j0 < R; j0 += kAtOnce) {
+      Pair sums[kAtOnce * H];
 #pragma unroll
-      for (int h = 0; h < H; h++) {
-        const float4 y = *reinterpret_cast<const float4*>(queries + h * D + d);
-        s[h] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s[h]))));
+      for (int i = 0; i < kAtOnce * H; i++) sums[i] = pair_of(0.f, 0.f);
+      const char* k = stage + (lane / 8 + 4 * j0) * kPitch + lane % 8 * 16;
+      const float* q = queries + lane % 8 * 4;
+#pragma unroll 2
+      for (int i = 0; i < D / 32; i++) {
+        ulonglong2 x[kAtOnce];
+#pragma unroll
+        for (int j = 0; j < kAtOnce; j++) x[j] = *reinterpret_cast<const ulonglong2*>(k + 4 * j * kPitch + i * 128);
+#pragma unroll
+        for (int h = 0; h < H; h++) {
+          const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(q + h * D + i * 32);
+#pragma unroll
+          for (int j = 0; j < kAtOnce; j++) sums[h * kAtOnce + j] = pair_fma(x[j].x, y.x, pair_fma(x[j].y, y.y, sums[h * kAtOnce + j]));
+        }
       }
-    }
-    const bool there = mask >> (lane % 16) & 1;
-    bool grows = false;
-#pragma unroll
-    for (int h = 0; h < H; h++) {
-      s[h] += __shfl_xor_sync(~0u, s[h], 16);
-      s[h] = there ? s[h] * scale2 : -INFINITY;
-      grows |= !(s[h] <= m[h]);
-    }
-    const int t = u.tile * p.tile_rows + (threadIdx.x / 32) * kRows + lane;
-    if (p.c.weights && lane < 16 && t < u.length) {
-      const int g = u.group / p.groups, h0 = (u.group % p.groups) * H;
-      float* to = p.space.scores + (((long long)u.b * p.c.kv_heads + g) * p.c.page_size * p.c.max_pages + t) * p.rep + h0;
 #pragma unroll
       for (int h = 0; h < H; h++)
-        if (h0 + h < p.rep) to[h] = s[h];
+#pragma unroll
+        for (int j = 0; j < kAtOnce; j++) {
+          const float2 two = pair_split(sums[h * kAtOnce + j]);
+          s[h * R + j0 + j] = two.x + two.y;
+        }
     }
-    if (__any_sync(~0u, grows)) {
+    exchange<R * H / 2, 4>(s);
+    exchange<R * H / 4, 2>(s);
+    exchange<R * H / 8, 1>(s);
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kOwn; i++) {
+      s[i] = mask >> row_of(lane, i) & 1 ? s[i] * scale2 : -INFINITY;
+      top = max_nan(top, s[i]);
+    }
+    if (p.c.weights) {
+      const int g = u.group / p.groups, h = (u.group % p.groups) * H + head_of(lane);
+      const int t0 = u.tile * p.tile_rows + (threadIdx.x / 32) * kRows;
+      float* to = p.space.scores + (((long long)u.b * p.c.kv_heads + g) * p.c.page_size * p.c.max_pages + t0) * p.rep + h;
+#pragma unroll
+      for (int i = 0; i < kOwn; i++)
+        if (h < p.rep && t0 + row_of(lane, i) < u.length) to[row_of(lane, i) * p.rep] = s[i];
+    }
+    if (__any_sync(~0u, !(top <= m))) {
+      top = max_nan(m, over_head(top, [](float a, float b) { return max_nan(a, b); }));
+      const float f = m == -INFINITY ? 0.f : exp2_fast(m - top);
+      m = top;
+      l *= f;
 #pragma unroll
       for (int h = 0; h < H; h++) {
-        float t = s[h];
+        const float of_head = __shfl_sync(~0u, f, h * 8 / H);
 #pragma unroll
-        for (int d = 1; d < 16; d *= 2) t = max_nan(t, __shfl_xor_sync(~0u, t, d));
-        t = max_nan(m[h], t);
-        const float f = m[h] == -INFINITY ? 0.f : exp2_fast(m[h] - t);
-        m[h] = t;
-        l[h] *= f;
-#pragma unroll
-        for (int i = 0; i < V; i++) o[h][i] *= f;
+        for (int i = 0; i < V / 2; i++) o[h][i] = pair_mul(o[h][i], pair_of(of_head, of_head));
       }
     }
-    float* mine = probabilities + (lane % 16) * H;
 #pragma unroll
-    for (int h = 0; h < H; h++) {
-      s[h] = exp2_fast(s[h] - (m[h] == -INFINITY ? 0.f : m[h]));
-      if (lane < 16) {
-        mine[h] = s[h];
-        l[h] += s[h];
-      }
+    for (int i = 0; i < kOwn; i++) {
+      const float w = exp2_fast(s[i] - (m == -INFINITY ? 0.f : m));
+      probabilities[row_of(lane, i) * H + head_of(lane)] = w;
+      l += w;
     }
     __syncwarp();
     const char* v = stage + kRows * kPitch + lane * V * 4;
 #pragma unroll 4
     for (int t = 0; t < kRows; t++) {
-      float x[V];
+      Pair x[V / 2];
+      if constexpr (V == 2) {
+        x[0] = *reinterpret_cast<const Pair*>(v + t * kPitch);
+      } else {
 #pragma unroll
-      for (int i = 0; i < V; i += 2) *reinterpret_cast<float2*>(x + i) = *reinterpret_cast<const float2*>(v + t * kPitch + i * 4);
-#pragma unroll
-      for (int h = 0; h < H; h++) {
-        const float w = probabilities[t * H + h];
-#pragma unroll
-        for (int i = 0; i < V; i++) o[h][i] = fmaf(w, x[i], o[h][i]);
+        for (int i = 0; i < V / 2; i += 2) {
+          const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(v + t * kPitch + i * 8);
+          x[i] = two.x;
+          x[i + 1] = two.y;
+        }
       }
+      float w[H];
+      if constexpr (H == 2) *reinterpret_cast<float2*>(w) = *reinterpret_cast<const float2*>(probabilities + t * H);
+#pragma unroll
+      for (int h = 0; h + 4 <= H; h += 4) *reinterpret_cast<float4*>(w + h) = *reinterpret_cast<const float4*>(probabilities + t * H + h);
+#pragma unroll
+      for (int h = 0; h < H; h++)
+#pragma unroll
+        for (int i = 0; i < V / 2; i++) o[h][i] = pair_fma(pair_of(w[h], w[h]), x[i], o[h][i]);
     }
     __syncwarp();
   }
 
   __device__ __forceinline__ void statistics(float* stat) {
     const int lane = threadIdx.x % 32;
-#pragma unroll
-    for (int h = 0; h < H; h++) {
-#pragma unroll
-      for (int d = 1; d < 32; d *= 2) l[h] += __shfl_xor_sync(~0u, l[h], d);
-      if (lane == 0) {
-        stat[2 * h] = m[h];
-        stat[2 * h + 1] = l[h];
-      }
+    l = over_head(l, [](float a, float b) { return a + b; });
+    if (lane < 8 && lane * H % 8 == 0) {
+      stat[2 * head_of(lane)] = m;
+      stat[2 * head_of(lane) + 1] = l;
     }
   }
   __device__ __forceinline__ void values(float* to, int pitch) const {
@@ -656,7 +688,7 @@ struct FmaWarp {
 #pragma unroll
     for (int h = 0; h < H; h++)
 #pragma unroll
-      for (int i = 0; i < V; i++) to[h * pitch + lane * V + i] = o[h][i];
+      for (int i = 0; i < V / 2; i++) *reinterpret_cast<float2*>(to + h * pitch + lane * V + 2 * i) = pair_split(o[h][i]);
   }
 };
 
@@ -951,8 +983,11 @@ constexpr size_t attend_smem() {
 //   16 bits, over 8 query heads a KV head: 16 columns at once, which read the rows once but leave registers for one block (three
 //   stages; four: 24.9, not 24.0; two blocks spill: 33.9). 16 heads, 32 sequences up to 8000 rows: 53.6 us, as two groups of eight
 //   56.5; 12 heads, 8 sequences: 16.2, not 17.1; with little to read the two groups are the faster (2 sequences: 17.9, not 21.8).
-//   f32, 128: one stage and two blocks, not two stages and one: 63.4 us, not 66.8, at batch 32 (one short sequence 13.7, not 13.1).
-//   f32, up to 4 query heads a KV head: arithmetic for four; with that for eight 35.1 us, not 28.1.
+//   f32, 128 and more: two stages of 8 rows, not one of 16 (rows in flight while others are at work): 8 sequences up to 2048 rows 26.4
+//   us, not 27.1, 4 of 155 with eight heads a KV head 11.6, not 13.9. 64: two stages of 16, not four of 8: 69.0 us, not 80.5, at 53
+//   sequences up to 2487. Two blocks an SM, not one with twice the stages: 26.4 us, not 32.8.
+//   f32, up to 4 query heads a KV head: arithmetic for four: 26.4 us, 31.9 with that for eight. Up to 2 and heads of 65 to 128: for two,
+//   one stage of 16 rows: 50 sequences up to 399 rows 30.8 us, 33.8 with that for four (heads of 64: 38.8 and 39.0, so not there).
 template <typename F>
 auto with_kernel(int dtype, int head_dim, int rep, F&& f) {
 #define PJRTX_ATTEND(T, W, D, S, N) return f(paged_attend_kernel<T, W, D, S, N>, AttendPlan{D, W::kHeads, W::kRows, S, N, attend_smem<T, W, D, S>()})
@@ -961,10 +996,11 @@ auto with_kernel(int dtype, int head_dim, int rep, F&& f) {
   if (head_dim <= 128) { using W = MmaWarp<T, 128, NB, 16>; PJRTX_ATTEND(T, W, 128, NB == 1 ? 2 : 3, NB == 1 ? 2 : 1); } \
   { using W = MmaWarp<T, 256, 1, 16>; PJRTX_ATTEND(T, W, 256, 2, 1); }
 #define PJRTX_ATTEND_FMA(H)                                                     \
-  if (head_dim <= 64) { using W = FmaWarp<64, H>; PJRTX_ATTEND(float, W, 64, 2, 2); }  \
-  if (head_dim <= 128) { using W = FmaWarp<128, H>; PJRTX_ATTEND(float, W, 128, 1, 2); } \
-  { using W = FmaWarp<256, H>; PJRTX_ATTEND(float, W, 256, 1, 1); }
+  if (head_dim <= 64) { using W = FmaWarp<64, H, 16>; PJRTX_ATTEND(float, W, 64, 2, 2); }  \
+  if (head_dim <= 128) { using W = FmaWarp<128, H, 8>; PJRTX_ATTEND(float, W, 128, 2, 2); } \
+  { using W = FmaWarp<256, H, 8>; PJRTX_ATTEND(float, W, 256, 2, 1); }
   if (dtype == kF32) {
+    if (rep <= 2 && head_dim > 64 && head_dim <= 128) { using W = FmaWarp<128, 2, 16>; PJRTX_ATTEND(float, W, 128, 1, 2); }
     if (rep <= 4) { PJRTX_ATTEND_FMA(4) }
     PJRTX_ATTEND_FMA(8)
   }

@@ -24,6 +24,7 @@
 #include <utility>
 
 #include "../common.h"
+#include "arith.cuh"
 #include "kernels.h"
 #include "paged.cuh"
 
@@ -34,45 +35,6 @@ namespace pjrtx {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float y;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-  return y;
-}
-
-// Two floats at a time.
-typedef unsigned long long Pair;
-__device__ __forceinline__ Pair pair_of(float a, float b) {
-  Pair r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 split(Pair p) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
-  return r;
-}
-__device__ __forceinline__ Pair pair_fma(Pair a, Pair b, Pair c) {
-  Pair r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ Pair pair_mul(Pair a, Pair b) {
-  Pair r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ Pair pair_add(Pair a, Pair b) {
-  Pair r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 
 template <typename T> struct Logit;
 template <> struct Logit<float> {
@@ -416,7 +378,7 @@ __global__ void __launch_bounds__(THREADS, kScoreThreadsOfSm / THREADS) token_sc
       top = max_nan(top, high);
     }
     if (!(top <= m)) {
-      const float2 s2 = split(s), t2 = split(t);
+      const float2 s2 = pair_split(s), t2 = pair_split(t);
       Stats x = {m, s2.x, t2.x}, y = {m, s2.y, t2.y};
       restate(x, top, c);
       restate(y, top, c);
@@ -435,14 +397,14 @@ __global__ void __launch_bounds__(THREADS, kScoreThreadsOfSm / THREADS) token_sc
 #pragma unroll
         for (int i = 0; i < V; i += 2) {
           const Pair y = pair_fma(pair_of(f[i], f[i + 1]), c2, from);
-          const float2 y2 = split(y);
+          const float2 y2 = pair_split(y);
           const Pair e = pair_of(exp2_fast(y2.x), exp2_fast(y2.y));
           s = pair_add(s, e);
           t = pair_fma(e, y, t);
         }
       }
     } else if (m != -INFINITY) {
-      float2 s2 = split(s), t2 = split(t);
+      float2 s2 = pair_split(s), t2 = pair_split(t);
 #pragma unroll
       for (int u = 0; u < kScoreVectors; u++) {
         float f[V];
@@ -459,7 +421,7 @@ __global__ void __launch_bounds__(THREADS, kScoreThreadsOfSm / THREADS) token_sc
       t = pair_of(t2.x, t2.y);
     }
   }
-  const float2 s2 = split(s), t2 = split(t);
+  const float2 s2 = pair_split(s), t2 = pair_split(t);
   Stats mine = {m, s2.x + s2.y, t2.x + t2.y};
 #pragma unroll
   for (int d = 16; d; d /= 2) {
@@ -613,14 +575,14 @@ __global__ void __launch_bounds__(kGradThreads) token_score_grad_kernel(TokenSco
   const Pair base2 = pair_of(base, base), rest2 = pair_of(rest, rest), g2 = pair_of(-g, -g), h2 = pair_of(-h, -h);
   auto gradient = [&](float& x0, float& x1) {
     const Pair x = pair_of(x0, x1);
-    const float2 y = split(pair_mul(pair_fma(x, scale2, from2), log2e2));
+    const float2 y = pair_split(pair_mul(pair_fma(x, scale2, from2), log2e2));
     const Pair p = pair_of(exp2_fast(y.x), exp2_fast(y.y));
     Pair d = g2;
     if (ENTROPY) {
-      const float2 t = split(pair_add(pair_fma(x, scale2, base2), rest2));
+      const float2 t = pair_split(pair_add(pair_fma(x, scale2, base2), rest2));
       d = pair_fma(h2, pair_of(max_nan(t.x, -1e30f), max_nan(t.y, -1e30f)), g2);  // finite, for p = 0 to make it 0
     }
-    const float2 r = split(pair_mul(p, d));
+    const float2 r = pair_split(pair_mul(p, d));
     x0 = r.x;
     x1 = r.y;
   };

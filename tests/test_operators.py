@@ -374,6 +374,25 @@ def test_attend_infinite_values_at_any_probability(gpu_backend, dtype, heads, kv
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv_heads,head_dim", [(4, 2, 128), (2, 2, 68), (2, 1, 4), (9, 3, 100), (16, 2, 72), (11, 1, 256), (6, 2, 132)])
+@pytest.mark.parametrize("track", [False, True])
+def test_attend_f32_heads_and_widths(gpu_backend, heads, kv_heads, head_dim, track):
+    """Every grouping of heads and width on the CUDA cores, with lengths around the rows of a warp and of a tile."""
+    lengths = [0, 1, 7, 8, 9, 47, 48, 49, 95, 96, 97, 1500, 16, 17]
+    c = _Case("f32", heads, kv_heads, head_dim, 7, lengths, seed=heads * head_dim)
+    tracked = c.tracking() if track else {}
+    before = c.weights.clone() if track else None
+    q = c.randn(len(lengths), heads, head_dim)
+    out, lse = c.torch.empty_like(q), c.torch.empty((len(lengths), heads), device="cuda")
+    c.handle(gpu_backend, track=track).attend(q, c.k, c.v, c.table, c.lengths, out, lse=lse, stream=_stream(), **tracked)
+    want, want_lse, p, bound, lse_bound, p_bound = c.attention(q)
+    _within(out, want, bound, "out")
+    _within(lse, want_lse, lse_bound, "lse")
+    if track:
+        _within(c.weights, before.double() + p, p_bound + 2.0 ** -23 * (before.double() + p), "weights")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("head_dim,score", [(64, -17.3), (128, -21.0), (256, -14.0)])
 def test_attend_many_small_probabilities(gpu_backend, dtype, head_dim, score):
