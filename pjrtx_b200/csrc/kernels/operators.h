@@ -41,7 +41,7 @@ struct PagedAppend {
   long long rows = 0;
   const int* counts = nullptr;  // new rows of each sequence (null: `rows` of every one)
 };
-int paged_append_launch(const PagedView& c, const PagedAppend& a, bool pdl, cudaStream_t stream);
+int paged_append_launch(const PagedView& c, const PagedAppend& a, int sm_count, bool pdl, cudaStream_t stream);
 
 struct PagedAttend {
   const void* q = nullptr;  // [batch, heads, head_dim] through the strides; query head h reads KV head h / (heads / kv_heads)

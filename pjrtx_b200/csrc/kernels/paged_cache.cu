@@ -1,12 +1,15 @@
 // Writing into a paged key-value cache and cutting it back.
 //
 // append: row t of the new ones of sequence b becomes row lengths[b] - counts[b] + t of its pages. Pure copying: every row is
-// read once and written once, 16 bytes a thread, the threads of a warp on neighbouring pieces of one row.
+// read once and written once, 16 bytes a thread, the threads of a warp on neighbouring pieces of one row. Bound by memory: 319 MB
+// in 52.7 us (floor 48.7); 51 MB in 11.
 //
 // evict: of the n > keep rows of a (sequence, KV head) those stay that come first by (protected, weight descending, row
 // ascending), a row being protected when its token is among the first `sinks` or the last `recent`. Attention does not depend
 // on the order of its rows, so nothing is compacted: the i-th kept row at or beyond `keep` moves into the i-th dropped place
-// before it, and only those rows are read and written. The token of each row is kept beside it in `positions`.
+// before it, and only those rows are read and written. The token of each row is kept beside it in `positions`. Bound by what a
+// block waits for: 11 us until the moves are known, however few rows there are (8 pairs of 2049 rows, one over: 9.3 us in all), then
+// by rows of 256 bytes in no order: 128 pairs up to 4096 rows cut to 2048 (73 MB) 27 us, 14 of them moving.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -22,8 +25,8 @@ namespace {
 
 // ---- append --------------------------------------------------------------------------------------------------------
 
-// One piece of a key and of its value in flight a thread: with two of each 8192 rows of 57 sequences took 55.3 us, with four 63.3,
-// with one 52.8 (floor 48.7).
+// One piece of a key and of its value in flight a thread, and at most 64 blocks an SM for all sequences, which go on to further
+// pieces: 8177 rows each of 57 sequences (319 MB) 52.7 us, with 16 an SM 55.7, with a block for every 256 pieces 58.8 (floor 48.7).
 constexpr int kAppendThreads = 256;
 
 __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(PagedView c, PagedAppend a, int pieces, int esize) {
@@ -205,6 +208,8 @@ __global__ void __launch_bounds__(kSelectThreads) paged_evict_select_kernel(Page
                                                                             int lanes, int esize, int in_shared, int move_here) {
   extern __shared__ unsigned keys[];
   __shared__ SelectShared sh;
+  for (int i = threadIdx.x; i < 1 << kDigitBits; i += kSelectThreads) sh.histogram[i] = 0;
+  __syncthreads();
   PJRTX_PDL_PROLOGUE();
   const int g = blockIdx.x, b = blockIdx.y;
   const int pair = b * c.kv_heads + g;
@@ -236,7 +241,11 @@ __global__ void __launch_bounds__(kSelectThreads) paged_evict_select_kernel(Page
           }
 #pragma unroll
         for (int u = 0; u < U; u++)
-          if (t0 + u * kSelectThreads < n) keys[t0 + u * kSelectThreads] = key_of(w[u], p[u]);
+          if (t0 + u * kSelectThreads < n) {
+            const unsigned k = key_of(w[u], p[u]);
+            keys[t0 + u * kSelectThreads] = k;
+            atomicAdd(&sh.histogram[k >> (32 - kDigitBits)], 1);
+          }
       }
     }
     unsigned threshold = 0;  // its digits so far
@@ -245,16 +254,22 @@ __global__ void __launch_bounds__(kSelectThreads) paged_evict_select_kernel(Page
       bits = min(kDigitBits, shift);
       shift -= bits;
       const int size = 1 << bits;
-      for (int i = threadIdx.x; i < size; i += kSelectThreads) sh.histogram[i] = 0;
-      __syncthreads();
+      const bool first_digit = shift + bits == 32;
+      if (!first_digit || !in_shared) {
 #pragma unroll 4
-      for (int t = threadIdx.x; t < n; t += kSelectThreads) {
-        const unsigned k = key_at(t);
-        if (shift + bits == 32 || k >> (shift + bits) == threshold) atomicAdd(&sh.histogram[k >> shift & (size - 1)], 1);
+        for (int t = threadIdx.x; t < n; t += kSelectThreads) {
+          const unsigned k = key_at(t);
+          if (first_digit || k >> (shift + bits) == threshold) atomicAdd(&sh.histogram[k >> shift & (size - 1)], 1);
+        }
       }
       __syncthreads();
       const int high = size - 1 - 2 * (int)threadIdx.x;  // two digits a thread, the largest ones first
-      const int at_high = high > 0 ? sh.histogram[high] : 0, at_low = high > 0 ? sh.histogram[high - 1] : 0;
+      int at_high = 0, at_low = 0;
+      if (high > 0) {
+        at_high = sh.histogram[high];
+        at_low = sh.histogram[high - 1];
+        sh.histogram[high] = sh.histogram[high - 1] = 0;  // for the next digit
+      }
       const int before = block_before(sh.sums, step, at_high + at_low, 0).a;
       if (before < need && need <= before + at_high + at_low) {
         const bool first = need <= before + at_high;
@@ -371,11 +386,11 @@ __global__ void __launch_bounds__(kMoveThreads) paged_evict_move_kernel(PagedVie
 
 }  // namespace
 
-int paged_append_launch(const PagedView& c, const PagedAppend& a, bool pdl, cudaStream_t stream) {
+int paged_append_launch(const PagedView& c, const PagedAppend& a, int sm_count, bool pdl, cudaStream_t stream) {
   const int esize = (int)dtype_size(c.dtype), pieces = c.head_dim * esize / 16;
   const long long work = a.rows * c.kv_heads * pieces;
-  const long long blocks = std::min<long long>((work + kAppendThreads - 1) / kAppendThreads, 2048);
-  return launch_kernel(paged_append_kernel, dim3((unsigned)std::max<long long>(blocks, 1), (unsigned)c.batch), dim3(kAppendThreads), 0,
+  const long long blocks = std::min((work + kAppendThreads - 1) / kAppendThreads, (64ll * sm_count + c.batch - 1) / c.batch);
+  return launch_kernel(paged_append_kernel, dim3((unsigned)blocks, (unsigned)c.batch), dim3(kAppendThreads), 0,
                        stream, pdl, c, a, pieces, esize) == cudaSuccess;
 }
 

@@ -113,7 +113,7 @@ int paged_cache_append(const PagedCache& cache, PagedView view, const PagedAppen
       !stride_ok(a.row_stride, a.rows, c.dtype) || !stride_ok(a.head_stride, c.kv_heads, c.dtype))
     return refuse("append: new rows need 16-byte aligned pointers and strides (%lld, %lld, %lld elements)", a.batch_stride, a.row_stride, a.head_stride);
   CurrentDevice scope(cache.device->ordinal);
-  return launched(paged_append_launch(view, a, true, stream), "append");
+  return launched(paged_append_launch(view, a, cache.device->sm_count, true, stream), "append");
 }
 
 int paged_cache_attend(const PagedCache& cache, PagedView view, PagedAttend a, cudaStream_t stream) {
