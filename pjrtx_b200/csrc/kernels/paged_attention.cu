@@ -297,11 +297,12 @@ template <> struct Mma16<__nv_bfloat16> {
     return *reinterpret_cast<const unsigned*>(&h);
   }
   static constexpr float kLift = 0.f;
-  // (a, b) >= 0 as the sum of two pairs, the first rounded towards zero.
+  // (a, b) >= 0 as the sum of two pairs, the first rounded towards zero; the second is 0 only where a or b is.
   static __device__ __forceinline__ uint2 split(float a, float b) {
     const float ra = a - __uint_as_float(__float_as_uint(a) & 0xffff0000u), rb = b - __uint_as_float(__float_as_uint(b) & 0xffff0000u);
     constexpr float kLeast = 1.1754944e-38f;  // 2^-126
-    return make_uint2(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632), pack(fmaxf(ra, kLeast), fmaxf(rb, kLeast)));
+    return make_uint2(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632),
+                      pack(fmaxf(ra, fminf(a, kLeast)), fmaxf(rb, fminf(b, kLeast))));
   }
   static __device__ __forceinline__ void mma(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -321,7 +322,7 @@ template <> struct Mma16<__half> {
     unsigned w;
     asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
     const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&w));
-    return make_uint2(w, pack(fmaxf(a - back.x, kLeast), fmaxf(b - back.y, kLeast)));
+    return make_uint2(w, pack(fmaxf(a - back.x, fminf(a, kLeast)), fmaxf(b - back.y, fminf(b, kLeast))));
   }
   static __device__ __forceinline__ void mma(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -345,7 +346,7 @@ __device__ __forceinline__ unsigned transpose(unsigned a) {
 // 16-bit types: rows and dimensions are the long sides of the products, heads the eight columns of m16n8k16, so that up to eight
 // query heads cost no more than one: scores^T [16 rows x heads] = K q^T, values^T [dims x heads] += V^T p^T. A probability goes in
 // as two 16-bit numbers, itself cut off and the rest: as one, it would be as far off as the result's own rounding. Neither is zero or
-// negative where the probability is above zero, so that an infinite value stays infinite, and f16 has 2^15 times the probabilities:
+// negative where the probability is above zero, so that an infinite value stays infinite (both are zero where it is zero), and f16 has 2^15 times the probabilities:
 // what is below 2^-39 of the largest counts as that, where plain f16 would lose 65 536 rows of 2^-25 each, 0.2 % of a result.
 // Tensor memory wants 64 rows at least on its M side and the scores through it to the softmax and back; with 1/60 of
 // its rate used (four heads) there is nothing to win by that. Lane i holds heads (i % 4) * 2 and + 1 of every eight.

@@ -413,6 +413,32 @@ def test_attend_many_small_probabilities(gpu_backend, dtype, head_dim, score):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("heads,kv_heads,head_dim", [(4, 1, 64), (8, 2, 128), (12, 1, 128), (3, 1, 256)])
+@pytest.mark.parametrize("score", [-math.inf, -400.0])
+def test_attend_rows_of_probability_zero_add_nothing(gpu_backend, dtype, heads, kv_heads, head_dim, score):
+    """Rows whose probability is zero, or too small for f32, with values as large as sums of them allow: what they add rounds to 0."""
+    c = _Case(dtype, heads, kv_heads, head_dim, 16, [5000, 40], seed=11)
+    torch = c.torch
+    q = torch.zeros((2, heads, head_dim), dtype=_torch_type(dtype), device="cuda")
+    q[:, :, 0] = 1
+    for b, n in enumerate([5000, 40]):
+        pg, row = c.places(b, n)
+        c.k[pg, row] = 0
+        c.k[pg, row, :, 0] = score
+        c.v[pg, row] = min(torch.finfo(q.dtype).max, 2.0 ** 112)
+        top = slice(n // 3, n // 3 + 2)  # two rows with all of the probability
+        c.k[pg[top], row[top], :, 0] = 0
+        c.v[pg[top], row[top]] = 0
+        c.v[pg[top], row[top], :, ::2] = 0.5
+    out = torch.full_like(q, math.nan)
+    c.handle(gpu_backend).attend(q, c.k, c.v, c.table, c.lengths, out, scale=1.0, stream=_stream())
+    want = torch.zeros_like(out)
+    want[..., ::2] = 0.5
+    assert torch.equal(out, want), (out - want).abs().max()
+
+
+@pytest.mark.gpu
 def test_attend_offsets_beyond_32_bits(gpu_backend):
     import torch
 
