@@ -515,7 +515,8 @@ int pjrtx_b200_paged_cache_append(PjrtxB200PagedCache *cache, const PjrtxB200Pag
 
 /* Attention of one query position per sequence over its rows: out = softmax(scale * q . k) v, lse = ln sum e^(scale * q . k).
  * A sequence without rows gives zeros and -inf, and so do scores that are all -inf. Infinities and NaN in rows that count go on
- * as in the formula, with probabilities below 2^-126 of the largest as zero; what lies beyond the length enters nothing. With k_new / v_new, row lengths[b] - 1 is taken from there and stored.
+ * as in the formula, with probabilities below 2^-126 of the largest (f16: 2^-141) as zero; what lies beyond the length enters
+ * nothing. With k_new / v_new, row lengths[b] - 1 is taken from there and stored.
  * Tracking: weights[b, g, t] grows by the weights that the query heads of KV head g give row t (a new row's starts with
  * them, its position is tokens[b] - 1). */
 typedef struct PjrtxB200PagedAttendArgs {

@@ -296,7 +296,7 @@ template <> struct Mma16<__nv_bfloat16> {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const unsigned*>(&h);
   }
-  static constexpr float kLift = 0.f;
+  static constexpr float kLift = 0.f, kWhole = -INFINITY;  // kWhole: exponent of the least positive probability that `split` takes
   // (a, b) >= 0 as the sum of two pairs, the first rounded towards zero; the second is 0 only where a or b is.
   static __device__ __forceinline__ uint2 split(float a, float b) {
     const float ra = a - __uint_as_float(__float_as_uint(a) & 0xffff0000u), rb = b - __uint_as_float(__float_as_uint(b) & 0xffff0000u);
@@ -315,20 +315,27 @@ template <> struct Mma16<__half> {
     return *reinterpret_cast<const unsigned*>(&h);
   }
   static constexpr float kLift = 15.f;
+  static constexpr float kWhole = -8.f;  // 2^-23 of the largest
+  // For 0 and from 2^kWhole on: the first number leaves at least 2^-11 of the probability to the second, which is then off by 2^-25.
   static __device__ __forceinline__ uint2 split(float a, float b) {
-    constexpr float kLeast = 5.9604645e-8f;  // 2^-24
-    if (a > 0.f) a = fmaxf(a, kLeast);
-    if (b > 0.f) b = fmaxf(b, kLeast);
+    constexpr float kPart = 0.99951171875f;  // 1 - 2^-11
     unsigned w;
-    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b * kPart), "f"(a * kPart));
     const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&w));
-    return make_uint2(w, pack(fmaxf(a - back.x, fminf(a, kLeast)), fmaxf(b - back.y, fminf(b, kLeast))));
+    return make_uint2(w, pack(a - back.x, b - back.y));
   }
   static __device__ __forceinline__ void mma(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
 };
+
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const float (&a)[4], float b0, float b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])), "r"(__float_as_uint(a[3])),
+                 "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
+}
 
 __device__ __forceinline__ void load_matrices(unsigned (&r)[4], unsigned at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
@@ -346,8 +353,10 @@ __device__ __forceinline__ unsigned transpose(unsigned a) {
 // 16-bit types: rows and dimensions are the long sides of the products, heads the eight columns of m16n8k16, so that up to eight
 // query heads cost no more than one: scores^T [16 rows x heads] = K q^T, values^T [dims x heads] += V^T p^T. A probability goes in
 // as two 16-bit numbers, itself cut off and the rest: as one, it would be as far off as the result's own rounding. Neither is zero or
-// negative where the probability is above zero, so that an infinite value stays infinite (both are zero where it is zero), and f16 has 2^15 times the probabilities:
-// what is below 2^-39 of the largest counts as that, where plain f16 would lose 65 536 rows of 2^-25 each, 0.2 % of a result.
+// negative where the probability is above zero, so that an infinite value stays infinite; both are zero where it is zero. f16 takes
+// 2^15 times the probabilities, and tiles with one below 2^-23 of the largest go in as tf32: f16 ends at 2^-39, and to lose what is
+// below, or to raise it to that, changes a result whose likelier rows have small values. Tiles without one cost 1 % at most for the
+// question; with one in nearly every tile 32 sequences up to 2048 rows take 40.5 us, not 38.4, two up to 65 536 87.2, not 85.1.
 // Tensor memory wants 64 rows at least on its M side and the scores through it to the softmax and back; with 1/60 of
 // its rate used (four heads) there is nothing to win by that. Lane i holds heads (i % 4) * 2 and + 1 of every eight.
 template <typename T, int D, int NB, int ROWS>
@@ -445,26 +454,42 @@ struct MmaWarp {
           }
         }
     }
+    bool wide = false;  // asked of the exponents, so that the answer is there when the exponentials are
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+      for (int n = 0; n < NB; n++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          s[r][n][j] -= m[n][j % 2] == -INFINITY ? 0.f : m[n][j % 2] - Mma16<T>::kLift;
+          wide |= s[r][n][j] < Mma16<T>::kWhole && s[r][n][j] > -INFINITY;
+        }
+    if constexpr (Mma16<T>::kLift > 0.f) wide = __any_sync(~0u, wide);
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+      for (int n = 0; n < NB; n++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          s[r][n][j] = exp2_fast(s[r][n][j]);
+          s[r][n][2 + j] = exp2_fast(s[r][n][2 + j]);
+          l[n][j] += s[r][n][j] + s[r][n][2 + j];
+        }
+    const unsigned v_lane = v_at + ((lane / 16) * 8 + lane % 8) * kPitch + (lane / 8 % 2) * 16;
+    if constexpr (Mma16<T>::kLift > 0.f) {
+      if (wide) return add_wide(s, v_lane);
+    }
     unsigned big[R][NB][2], small[R][NB][2];
 #pragma unroll
     for (int r = 0; r < R; r++)
 #pragma unroll
-      for (int n = 0; n < NB; n++) {
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-          const float from = m[n][j] == -INFINITY ? 0.f : m[n][j] - Mma16<T>::kLift;
-          s[r][n][j] = exp2_fast(s[r][n][j] - from);
-          s[r][n][2 + j] = exp2_fast(s[r][n][2 + j] - from);
-          l[n][j] += s[r][n][j] + s[r][n][2 + j];
-        }
+      for (int n = 0; n < NB; n++)
 #pragma unroll
         for (int k = 0; k < 2; k++) {
           const uint2 parts = Mma16<T>::split(s[r][n][2 * k], s[r][n][2 * k + 1]);
           big[r][n][k] = transpose(parts.x);
           small[r][n][k] = transpose(parts.y);
         }
-      }
-    const unsigned v_lane = v_at + ((lane / 16) * 8 + lane % 8) * kPitch + (lane / 8 % 2) * 16;
 #pragma unroll
     for (int i = 0; i < D / 16; i++)
 #pragma unroll
@@ -477,6 +502,43 @@ struct MmaWarp {
           Mma16<T>::mma(o[i][n], a, small[r][n][0], small[r][n][1]);
         }
       }
+  }
+
+  // The values of a tile under probabilities that f16 does not hold: as tf32, which has the range of f32 and in which f16 values are
+  // exact, a probability as two numbers of 11 bits. Eight rows a product: even ones in slots 0 to 3, odd ones in 4 to 7, as they lie
+  // in the halves of the registers that the transposed load fills.
+  __device__ __forceinline__ void add_wide(const float (&s)[R][NB][4], unsigned v_lane) {
+    constexpr int kPitch = RowStage<T, D, ROWS>::kPitch;
+    const int lane = threadIdx.x % 32, from = lane % 4 * 8 + lane / 8;  // the lane that has this head's row 2 (lane % 4); row + 1: 4 further
+    const bool odd = lane / 4 & 1;                                      // head
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      float big[NB][4], small[NB][4];  // rows 2 (lane % 4) and + 1, then the same of the upper eight
+#pragma unroll
+      for (int n = 0; n < NB; n++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const float x = __shfl_sync(~0u, s[r][n][k / 2 * 2], from + k % 2 * 4), y = __shfl_sync(~0u, s[r][n][k / 2 * 2 + 1], from + k % 2 * 4);
+          const float w = odd ? y : x;
+          big[n][k] = __uint_as_float(__float_as_uint(w) & 0xffffe000u);
+          small[n][k] = fmaxf(w - big[n][k], fminf(w, 1.1754944e-38f));  // as in Mma16<__nv_bfloat16>::split
+        }
+#pragma unroll
+      for (int i = 0; i < D / 16; i++) {
+        unsigned a[4];
+        load_matrices_transposed(a, v_lane + r * 16 * kPitch + i * 32);
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {
+          const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&a[k])), hi = __half22float2(*reinterpret_cast<const __half2*>(&a[k + 1]));
+          const float v[4] = {lo.x, hi.x, lo.y, hi.y};
+#pragma unroll
+          for (int n = 0; n < NB; n++) {
+            mma_tf32(o[i][n], v, big[n][k], big[n][k + 1]);
+            mma_tf32(o[i][n], v, small[n][k], small[n][k + 1]);
+          }
+        }
+      }
+    }
   }
 
   // Of 16 rows, the r-th of the warp's.

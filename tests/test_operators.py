@@ -439,6 +439,29 @@ def test_attend_rows_of_probability_zero_add_nothing(gpu_backend, dtype, heads, 
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("heads,kv_heads,head_dim", [(4, 1, 64), (16, 1, 64), (8, 2, 128), (12, 1, 128), (3, 1, 256)])
+@pytest.mark.parametrize("score", [-14.0, -15.3, -22.0, -26.0, -30.0, -40.0, -60.0, None])
+def test_attend_probabilities_of_any_size(gpu_backend, dtype, heads, kv_heads, head_dim, score):
+    """Tens of thousands of rows of one sign against one row with all the rest and values of zero; None: scores from 0 to -60."""
+    n = 40000
+    c = _Case(dtype, heads, kv_heads, head_dim, 64, [n], seed=13)
+    torch = c.torch
+    q = torch.zeros((1, heads, head_dim), dtype=_torch_type(dtype), device="cuda")
+    q[:, :, 0] = 1
+    pg, row = c.places(0, n)
+    c.k[pg, row, :, 0] = score if score else (-60 * torch.rand((n, kv_heads), generator=c.gen, device="cuda")).to(q.dtype)
+    c.v[pg, row] = (c.v[pg, row].abs() * 15000).clamp(max=60000)
+    c.k[pg[12345], row[12345], :, 0] = 0
+    c.v[pg[12345], row[12345]] = 0
+    out, lse = torch.empty_like(q), torch.empty((1, heads), device="cuda")
+    c.handle(gpu_backend).attend(q, c.k, c.v, c.table, c.lengths, out, lse=lse, scale=1.0, stream=_stream())
+    want, want_lse, _, bound, lse_bound, _ = c.attention(q, 1.0)
+    _within(out, want, bound, "out")
+    _within(lse, want_lse, lse_bound, "lse")
+
+
+@pytest.mark.gpu
 def test_attend_offsets_beyond_32_bits(gpu_backend):
     import torch
 
