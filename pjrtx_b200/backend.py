@@ -230,6 +230,7 @@ class DeviceBuffer:
     def __init__(self, lib, handle):
         self._lib = lib
         self.handle = handle
+        self._device: Optional[int] = None
 
     @property
     def dtype(self) -> int:
@@ -249,6 +250,13 @@ class DeviceBuffer:
     @property
     def is_donated(self) -> bool:
         return bool(self._lib.pjrtx_b200_buffer_is_donated(self.handle))
+
+    @property
+    def device(self) -> int:
+        """Ordinal of the device that the buffer is on."""
+        if self._device is None:
+            self._device = self._lib.pjrtx_b200_buffer_device(self.handle)
+        return self._device
 
     @property
     def device_pointer(self) -> int:

@@ -2,9 +2,10 @@
 
 Bindings of the `pjrtx_b200_paged_cache_*` and `pjrtx_b200_token_log_probs*` entry points of include/pjrtx_b200.h, reached
 through `Backend.paged_cache`, `Backend.token_log_probs` and `Backend.token_log_probs_backward`. Arrays are `DeviceBuffer`s
-or any device tensors with `data_ptr()`, `shape`, `stride()` and `dtype` (torch's). Types and shapes are checked here, the
-rest behind the C ABI; nothing is copied, cast or kept. Calls enqueue on `stream`, a `cudaStream_t` as an integer (0: the
-default stream); None is the stream on which the backend's buffers and executables work.
+or any device tensors with `data_ptr()`, `shape`, `stride()` and `dtype` (torch's). Types, shapes and the device that an array
+says it is on (`get_device()` or `device`) are checked here, the rest behind the C ABI; nothing is copied, cast or kept. Calls
+enqueue on `stream`, a `cudaStream_t` as an integer (0: the default stream); None is the stream on which the backend's buffers and
+executables work.
 """
 from __future__ import annotations
 
@@ -129,54 +130,69 @@ def _place(x):
         return x.device_pointer or 0, tuple(strides)
 
 
-def _check(x, name: str, dtype: int, shape: Tuple[int, ...]) -> None:
+def _device(x) -> Optional[int]:
+    """Ordinal of the device an array is on, -1 for the host, None where it does not say."""
+    try:
+        return x.get_device()
+    except AttributeError:
+        at = getattr(x, "device", None)
+    if at is None or isinstance(at, int):
+        return at
+    return (at.index or 0) if at.type == "cuda" else -1
+
+
+def _check(x, name: str, dtype: int, shape: Tuple[int, ...], device: int) -> None:
     if _code(x) != dtype:
         raise _error(f"{name} has element type {P.DTYPE_NAMES.get(_code(x), 'other')}, {P.DTYPE_NAMES.get(dtype, dtype)} is needed")
     if _dims(x) != shape:
         raise _error(f"{name} has shape {tuple(_dims(x))}, {shape} is needed")
+    at = _device(x)
+    if at is not None and at != device:
+        raise _error(f"{name} is on {'the host' if at < 0 else f'device {at}'}, device {device} is needed")
 
 
-def _rows(x, name: str, dtype: int, shape: Tuple[int, ...]):
+def _rows(x, name: str, dtype: int, shape: Tuple[int, ...], device: int):
     """Address and strides of an array whose innermost axis has to be dense."""
     try:  # a tensor that is as it has to be
-        if x.shape == shape and _codes[x.dtype] == dtype:
+        if x.shape == shape and _codes[x.dtype] == dtype and x.get_device() == device:
             strides = x.stride()
             if strides[-1] == 1:
                 return x.data_ptr(), strides
     except (AttributeError, KeyError):
         pass
-    _check(x, name, dtype, shape)
+    _check(x, name, dtype, shape, device)
     place = _place(x)
     if place[1][-1] != 1 and shape[-1] != 1:
         raise _error(f"{name} has stride {place[1][-1]} along its last axis, which has to be dense")
     return place
 
 
-def _twin(x, name: str, like: str, dtype: int, shape: Tuple[int, ...], strides) -> int:
+def _twin(x, name: str, like: str, dtype: int, shape: Tuple[int, ...], strides, device: int) -> int:
     """Address of an array that has the type, shape and strides of another one."""
     try:
-        if x.shape == shape and _codes[x.dtype] == dtype and x.stride() == strides:
+        if x.shape == shape and _codes[x.dtype] == dtype and x.stride() == strides and x.get_device() == device:
             return x.data_ptr()
     except (AttributeError, KeyError):
         pass
     if _code(x) != dtype or _dims(x) != shape:
         raise _error(f"{like} and {name} differ in type or shape")
+    _check(x, name, dtype, shape, device)
     pointer, own = _place(x)
     if own != strides:
         raise _error(f"{like} and {name} differ in their strides")
     return pointer
 
 
-def _dense(x, name: str, dtype: int, shape: Tuple[int, ...]) -> int:
+def _dense(x, name: str, dtype: int, shape: Tuple[int, ...], device: int) -> int:
     """Address of an array that has to be dense; None is 0."""
     if x is None:
         return 0
     try:
-        if x.shape == shape and _codes[x.dtype] == dtype and x.is_contiguous():
+        if x.shape == shape and _codes[x.dtype] == dtype and x.is_contiguous() and x.get_device() == device:
             return x.data_ptr()
     except (AttributeError, KeyError):
         pass
-    _check(x, name, dtype, shape)
+    _check(x, name, dtype, shape, device)
     pointer, strides = _place(x)
     step = 1
     for d, s in zip(reversed(shape), reversed(strides)):
@@ -211,19 +227,20 @@ class PagedCache:
     def _view(self, k_pages, v_pages, page_table, lengths, tokens, weights, positions) -> Tuple[int, bytes]:
         """The batch and the packed view."""
         try:  # tensors that are as they have to be, checked in one go; anything else takes the checks one by one
-            kind, s32 = _types[self.dtype], _types[P.S32]
+            kind, s32, here = _types[self.dtype], _types[P.S32], self.device
             dims, strides, (batch,) = k_pages.shape, k_pages.stride(), lengths.shape
             if (dims[1:] == self._page_dims and k_pages.dtype is kind and strides[3] == 1 and v_pages.shape == dims and v_pages.dtype is kind
                     and v_pages.stride() == strides and page_table.shape == (batch, self.max_pages) and page_table.dtype is s32
-                    and page_table.is_contiguous() and lengths.dtype is s32 and lengths.is_contiguous()):
+                    and page_table.is_contiguous() and lengths.dtype is s32 and lengths.is_contiguous() and k_pages.get_device() == here
+                    and v_pages.get_device() == here and page_table.get_device() == here and lengths.get_device() == here):
                 if weights is None and tokens is None and positions is None:
                     return batch, _pack_view(k_pages.data_ptr(), v_pages.data_ptr(), dims[0], strides[0], strides[1], strides[2],
                                              page_table.data_ptr(), self.max_pages, lengths.data_ptr(), batch, 0, 0, 0)
                 tracked = (batch, self.kv_heads, self.capacity)
                 return batch, _pack_view(k_pages.data_ptr(), v_pages.data_ptr(), dims[0], strides[0], strides[1], strides[2],
                                          page_table.data_ptr(), self.max_pages, lengths.data_ptr(), batch,
-                                         _dense(tokens, "tokens", P.S32, (batch,)), _dense(weights, "weights", P.F32, tracked),
-                                         _dense(positions, "positions", P.S32, tracked))
+                                         _dense(tokens, "tokens", P.S32, (batch,), here), _dense(weights, "weights", P.F32, tracked, here),
+                                         _dense(positions, "positions", P.S32, tracked, here))
         except (AttributeError, KeyError, ValueError, TypeError, IndexError):
             pass
         dims, batch_dims = _dims(k_pages), _dims(lengths)
@@ -231,14 +248,15 @@ class PagedCache:
             raise _error(f"k_pages has shape {tuple(dims)}, (pages, {', '.join(map(str, self._page_dims))}) is needed")
         if len(batch_dims) != 1:
             raise _error(f"lengths has shape {tuple(batch_dims)}, (batch,) is needed")
-        k, strides = _rows(k_pages, "k_pages", self.dtype, dims)
-        v = _twin(v_pages, "v_pages", "k_pages", self.dtype, dims, strides)
+        k, strides = _rows(k_pages, "k_pages", self.dtype, dims, self.device)
+        v = _twin(v_pages, "v_pages", "k_pages", self.dtype, dims, strides, self.device)
         batch = batch_dims[0]
-        table, table_strides = _rows(page_table, "page_table", P.S32, (batch, self.max_pages))
+        table, table_strides = _rows(page_table, "page_table", P.S32, (batch, self.max_pages), self.device)
         tracked = (batch, self.kv_heads, self.capacity)
         return batch, _pack_view(k, v, dims[0], strides[0], strides[1], strides[2], table, table_strides[0],
-                                 _dense(lengths, "lengths", P.S32, (batch,)), batch, _dense(tokens, "tokens", P.S32, (batch,)),
-                                 _dense(weights, "weights", P.F32, tracked), _dense(positions, "positions", P.S32, tracked))
+                                 _dense(lengths, "lengths", P.S32, (batch,), self.device), batch,
+                                 _dense(tokens, "tokens", P.S32, (batch,), self.device),
+                                 _dense(weights, "weights", P.F32, tracked, self.device), _dense(positions, "positions", P.S32, tracked, self.device))
 
     def _call(self, fn, view, args, stream) -> None:
         if not self.handle:
@@ -254,9 +272,9 @@ class PagedCache:
         shape = _dims(k_new)
         if len(shape) != 4 or shape[0] != batch or shape[2] != self.kv_heads or shape[3] != self.head_dim:
             raise _error(f"k_new has shape {tuple(shape)}, ({batch}, rows, {self.kv_heads}, {self.head_dim}) is needed")
-        k, strides = _rows(k_new, "k_new", self.dtype, shape)
-        v = _twin(v_new, "v_new", "k_new", self.dtype, shape, strides)
-        args = _pack_append(k, v, shape[1], strides[0], strides[1], strides[2], _dense(counts, "counts", P.S32, (batch,)))
+        k, strides = _rows(k_new, "k_new", self.dtype, shape, self.device)
+        v = _twin(v_new, "v_new", "k_new", self.dtype, shape, strides, self.device)
+        args = _pack_append(k, v, shape[1], strides[0], strides[1], strides[2], _dense(counts, "counts", P.S32, (batch,), self.device))
         self._call(self._lib.pjrtx_b200_paged_cache_append, view, args, stream)
 
     def attend(self, q, k_pages, v_pages, page_table, lengths, out, lse=None, k_new=None, v_new=None, tokens=None, weights=None,
@@ -269,31 +287,32 @@ class PagedCache:
         fn, stream = self._lib.pjrtx_b200_paged_cache_attend, self._stream if stream is None else stream
         shape, new_shape = (batch, self.heads, self.head_dim), (batch, self.kv_heads, self.head_dim)
         try:  # tensors that are as they have to be, as in _view
-            kind, qs, os = _types[self.dtype], q.stride(), out.stride()
+            kind, qs, os, here = _types[self.dtype], q.stride(), out.stride(), self.device
             if (q.shape == shape and q.dtype is kind and qs[2] == 1 and out.shape == shape and out.dtype is kind and os[2] == 1
-                    and (lse is None or lse.shape == shape[:2] and lse.dtype is _types[P.F32] and lse.is_contiguous())):
+                    and q.get_device() == here and out.get_device() == here
+                    and (lse is None or lse.shape == shape[:2] and lse.dtype is _types[P.F32] and lse.is_contiguous() and lse.get_device() == here)):
                 if k_new is None and v_new is None:
                     return self._call(fn, view, _pack_attend(q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1],
                                                              0 if lse is None else lse.data_ptr(), 0, 0, 0, 0, scale), stream)
                 ns = k_new.stride()
                 if (k_new.shape == new_shape and k_new.dtype is kind and ns[2] == 1 and v_new.shape == new_shape and v_new.dtype is kind
-                        and v_new.stride() == ns):
+                        and v_new.stride() == ns and k_new.get_device() == here and v_new.get_device() == here):
                     return self._call(fn, view, _pack_attend(q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1],
                                                              0 if lse is None else lse.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), ns[0],
                                                              ns[1], scale), stream)
         except (AttributeError, KeyError, IndexError):
             pass
-        q_at, q_strides = _rows(q, "q", self.dtype, shape)
-        out_at, out_strides = _rows(out, "out", self.dtype, shape)
+        q_at, q_strides = _rows(q, "q", self.dtype, shape, self.device)
+        out_at, out_strides = _rows(out, "out", self.dtype, shape, self.device)
         k = v = 0
         new_strides = (0, 0)
         if k_new is not None and v_new is not None:
-            k, new_strides = _rows(k_new, "k_new", self.dtype, new_shape)
-            v = _twin(v_new, "v_new", "k_new", self.dtype, new_shape, new_strides)
+            k, new_strides = _rows(k_new, "k_new", self.dtype, new_shape, self.device)
+            v = _twin(v_new, "v_new", "k_new", self.dtype, new_shape, new_strides, self.device)
         elif k_new is not None or v_new is not None:
             raise _error("a new key and a new value go together")
         args = _pack_attend(q_at, q_strides[0], q_strides[1], out_at, out_strides[0], out_strides[1],
-                            _dense(lse, "lse", P.F32, (batch, self.heads)), k, v, new_strides[0], new_strides[1], scale)
+                            _dense(lse, "lse", P.F32, (batch, self.heads), self.device), k, v, new_strides[0], new_strides[1], scale)
         return self._call(fn, view, args, stream)
 
     def evict(self, k_pages, v_pages, page_table, lengths, tokens, weights, positions, keep: int, recent: int = 0, sinks: int = 0,
@@ -302,9 +321,9 @@ class PagedCache:
         `*_out` arrays, None: in place. Pages must not be shared between sequences."""
         batch, view = self._view(k_pages, v_pages, page_table, lengths, tokens, weights, positions)
         tracked = (batch, self.kv_heads, self.capacity)
-        args = _pack_evict(keep, recent, sinks, _dense(lengths if lengths_out is None else lengths_out, "lengths_out", P.S32, (batch,)),
-                           _dense(weights if weights_out is None else weights_out, "weights_out", P.F32, tracked),
-                           _dense(positions if positions_out is None else positions_out, "positions_out", P.S32, tracked))
+        args = _pack_evict(keep, recent, sinks, _dense(lengths if lengths_out is None else lengths_out, "lengths_out", P.S32, (batch,), self.device),
+                           _dense(weights if weights_out is None else weights_out, "weights_out", P.F32, tracked, self.device),
+                           _dense(positions if positions_out is None else positions_out, "positions_out", P.S32, tracked, self.device))
         self._call(self._lib.pjrtx_b200_paged_cache_evict, view, args, stream)
 
     def destroy(self) -> None:
@@ -319,11 +338,11 @@ class PagedCache:
             pass
 
 
-def _logits(x):
+def _logits(x, device: int):
     """Element type, rows, vocabulary, address and row stride."""
     try:
         (rows, vocab), code, strides = x.shape, _codes[x.dtype], x.stride()
-        if code in _FLOATS and strides[1] == 1:
+        if code in _FLOATS and strides[1] == 1 and x.get_device() == device:
             return code, rows, vocab, x.data_ptr(), strides[0]
     except (AttributeError, KeyError, ValueError):
         pass
@@ -332,19 +351,19 @@ def _logits(x):
         raise _error(f"logits has shape {tuple(dims)}, (rows, vocabulary) is needed")
     if code not in _FLOATS:
         raise _error(f"logits has element type {P.DTYPE_NAMES.get(code, 'other')}; f32, f16 and bf16 are supported")
-    pointer, strides = _rows(x, "logits", code, dims)
+    pointer, strides = _rows(x, "logits", code, dims, device)
     return code, dims[0], dims[1], pointer, strides[0]
 
 
 def token_log_probs(backend, logits, tokens, log_probs, entropy=None, lse=None, top_ids=None, top_log_probs=None, scale: float = 1.0,
                     stream: Optional[int] = None, device: int = 0) -> None:
-    dtype, rows, vocab, at, stride = _logits(logits)
+    dtype, rows, vocab, at, stride = _logits(logits, device)
     wide = top_ids if top_ids is not None else top_log_probs
     top = 0 if wide is None else _dims(wide)[-1]
-    args = _pack_score(dtype, top, at, rows, vocab, stride, _dense(tokens, "tokens", P.S32, (rows,)), scale,
-                       _dense(log_probs, "log_probs", P.F32, (rows,)), _dense(entropy, "entropy", P.F32, (rows,)),
-                       _dense(lse, "lse", P.F32, (rows,)), _dense(top_ids, "top_ids", P.S32, (rows, top)),
-                       _dense(top_log_probs, "top_log_probs", P.F32, (rows, top)))
+    args = _pack_score(dtype, top, at, rows, vocab, stride, _dense(tokens, "tokens", P.S32, (rows,), device), scale,
+                       _dense(log_probs, "log_probs", P.F32, (rows,), device), _dense(entropy, "entropy", P.F32, (rows,), device),
+                       _dense(lse, "lse", P.F32, (rows,), device), _dense(top_ids, "top_ids", P.S32, (rows, top), device),
+                       _dense(top_log_probs, "top_log_probs", P.F32, (rows, top), device))
     lib = backend.lib
     if not lib.pjrtx_b200_token_log_probs(device, args, lib.pjrtx_b200_device_stream(device) if stream is None else stream):
         raise _error(backend._err())
@@ -352,11 +371,12 @@ def token_log_probs(backend, logits, tokens, log_probs, entropy=None, lse=None, 
 
 def token_log_probs_backward(backend, logits, tokens, lse, grad_logits, grad_log_probs=None, entropy=None, grad_entropy=None,
                              scale: float = 1.0, stream: Optional[int] = None, device: int = 0) -> None:
-    dtype, rows, vocab, at, stride = _logits(logits)
-    grad_at, grad_strides = _rows(grad_logits, "grad_logits", dtype, (rows, vocab))
-    args = _pack_score_grad(dtype, scale, at, grad_at, rows, vocab, stride, grad_strides[0], _dense(tokens, "tokens", P.S32, (rows,)),
-                            _dense(lse, "lse", P.F32, (rows,)), _dense(entropy, "entropy", P.F32, (rows,)),
-                            _dense(grad_log_probs, "grad_log_probs", P.F32, (rows,)), _dense(grad_entropy, "grad_entropy", P.F32, (rows,)))
+    dtype, rows, vocab, at, stride = _logits(logits, device)
+    grad_at, grad_strides = _rows(grad_logits, "grad_logits", dtype, (rows, vocab), device)
+    args = _pack_score_grad(dtype, scale, at, grad_at, rows, vocab, stride, grad_strides[0], _dense(tokens, "tokens", P.S32, (rows,), device),
+                            _dense(lse, "lse", P.F32, (rows,), device), _dense(entropy, "entropy", P.F32, (rows,), device),
+                            _dense(grad_log_probs, "grad_log_probs", P.F32, (rows,), device),
+                            _dense(grad_entropy, "grad_entropy", P.F32, (rows,), device))
     lib = backend.lib
     if not lib.pjrtx_b200_token_log_probs_backward(device, args, lib.pjrtx_b200_device_stream(device) if stream is None else stream):
         raise _error(backend._err())

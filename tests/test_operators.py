@@ -127,6 +127,77 @@ def test_token_log_probs_backward_refuses(backend, change, message):
         backend.token_log_probs_backward(**a, stream=0)
 
 
+class _Placed(_Array):
+    """A device tensor that says where it is, as torch does (`get_device`) or by its `device`."""
+
+    def __init__(self, where, like, says):
+        super().__init__(like.dtype.name[5:], *like.shape)
+        if says == "get_device":
+            self.get_device = lambda: where
+        else:
+            self.device = type("Device", (), dict(type="cuda" if where >= 0 else "cpu", index=where if where >= 0 else None))()
+
+    def is_contiguous(self):
+        return True
+
+
+class _Unreachable:
+    """In the place of the library: no call with a refused argument may get there."""
+
+    def __getattr__(self, name):
+        def reached(*_):
+            raise AssertionError(f"{name} was reached")
+
+        return reached
+
+
+def _host_cache():
+    """A paged cache without a device: what the facade checks, and a library that must not be reached."""
+    cache = ops.PagedCache.__new__(ops.PagedCache)
+    cache.dtype, cache.batch, cache.heads, cache.kv_heads, cache.head_dim = P.BF16_CODE, 2, 8, 4, 64
+    cache.page_size, cache.max_pages, cache.track, cache.capacity, cache.device = 16, 4, True, 64, 1
+    cache._page_dims, cache._stream, cache._lib, cache.handle = (16, 4, 64), 0, _Unreachable(), 0
+    return cache
+
+
+@pytest.mark.parametrize("says", ["get_device", "device"])
+@pytest.mark.parametrize("where,message", [(-1, "on the host, device 1"), (0, "on device 0, device 1")])
+def test_arrays_of_the_host_and_of_other_devices_are_refused(backend, where, message, says):
+    def check(call, good):
+        place = lambda at, a: _Placed(at, a, says)
+        for name in good:
+            if isinstance(good[name], _Array):
+                with pytest.raises(be_mod.BackendError, match=f"{name} is {message}"):
+                    call(**{n: place(where if n == name else 1, a) if isinstance(a, _Array) else a for n, a in good.items()}, stream=0)
+
+    cache = _host_cache()
+    view = dict(k_pages=_Array("bfloat16", 9, 16, 4, 64), v_pages=_Array("bfloat16", 9, 16, 4, 64), page_table=_Array("int32", 2, 4),
+                lengths=_Array("int32", 2), tokens=_Array("int32", 2), weights=_Array("float32", 2, 4, 64), positions=_Array("int32", 2, 4, 64))
+    check(cache.append, dict(view, k_new=_Array("bfloat16", 2, 3, 4, 64), v_new=_Array("bfloat16", 2, 3, 4, 64), counts=_Array("int32", 2)))
+    check(cache.attend, dict(view, q=_Array("bfloat16", 2, 8, 64), out=_Array("bfloat16", 2, 8, 64), lse=_Array("float32", 2, 8),
+                             k_new=_Array("bfloat16", 2, 4, 64), v_new=_Array("bfloat16", 2, 4, 64)))
+    check(cache.evict, dict(view, keep=8, lengths_out=_Array("int32", 2), weights_out=_Array("float32", 2, 4, 64),
+                            positions_out=_Array("int32", 2, 4, 64)))
+    row = _Array("float32", 4)
+    scored = dict(logits=_Array("float16", 4, 100), tokens=_Array("int32", 4), entropy=row, lse=row, device=1)
+    check(backend.token_log_probs, dict(scored, log_probs=row, top_ids=_Array("int32", 4, 3), top_log_probs=_Array("float32", 4, 3)))
+    check(backend.token_log_probs_backward, dict(scored, grad_logits=_Array("float16", 4, 100), grad_log_probs=row, grad_entropy=row))
+
+
+def test_tensors_in_host_memory_are_refused(backend):
+    import torch
+
+    cache = _host_cache()
+    view = dict(k_pages=torch.zeros(9, 16, 4, 64).bfloat16(), v_pages=torch.zeros(9, 16, 4, 64).bfloat16(),
+                page_table=torch.zeros(2, 4, dtype=torch.int32), lengths=torch.zeros(2, dtype=torch.int32))
+    q = torch.zeros(2, 8, 64).bfloat16()
+    for _ in range(2):  # types are known after the first call
+        with pytest.raises(be_mod.BackendError, match="k_pages is on the host"):
+            cache.attend(q, **view, out=torch.zeros_like(q), stream=0)
+        with pytest.raises(be_mod.BackendError, match="logits is on the host"):
+            backend.token_log_probs(torch.zeros(4, 100), torch.zeros(4, dtype=torch.int32), torch.zeros(4), stream=0)
+
+
 @pytest.mark.gpu
 def test_paged_cache_calls_refuse_bad_arguments(gpu_backend):
     """Everything here is refused on the host: the addresses are never used."""
