@@ -452,8 +452,10 @@ int pjrtx_b200_dot_static_scratch_status(int device_ordinal, void *stream);
  * it was. Set struct_size of every argument struct to its sizeof. Element types are f32, f16 and bf16; statistics and
  * weights are f32, ids and lengths s32. Strides count elements; the innermost axis is dense.
  * 1 when enqueued, 0 with last_error set. What only the device sees (a page id outside the pool, a length outside the page
- * table, a token id outside the vocabulary) is never followed out of bounds: the kernel skips it and sets the device's error
- * word, and the next pjrtx_b200_device_synchronize or copy to the host returns 0 and names it (codes 40, 41, 42). */
+ * table, a token id outside the vocabulary) is never followed out of bounds: the kernel skips it and sets a word of its code
+ * (40, 41, 42). pjrtx_b200_operators_status waits for the stream of a call and tells. The words are the device's, not the
+ * call's: pjrtx_b200_device_synchronize and copies to the host, which wait for the stream of pjrtx_b200_device_stream alone,
+ * return 0 for what is set by then, whichever stream it came from, and what has been named once is not named again. */
 void *pjrtx_b200_device_stream(int device_ordinal);
 /* NULL for a deleted or donated buffer, and for one without elements. */
 void *pjrtx_b200_buffer_device_pointer(PjrtxB200Buffer *buffer);
@@ -594,6 +596,11 @@ typedef struct PjrtxB200TokenLogProbsBackwardArgs {
   const float *grad_entropy;   /* [rows] */
 } PjrtxB200TokenLogProbsBackwardArgs;
 int pjrtx_b200_token_log_probs_backward(int device_ordinal, const PjrtxB200TokenLogProbsBackwardArgs *args, void *stream);
+
+/* Waits for `stream`; 1, or 0 with last_error naming what the operators' kernels on the device met since it was last asked
+ * (all of codes 40, 41 and 42 that are set). A bounded wait of an executable's kernel that gave up is not among it and stays
+ * for pjrtx_b200_device_synchronize. Not during a stream capture. */
+int pjrtx_b200_operators_status(int device_ordinal, void *stream);
 
 /* ---- generated-kernel check (no device needed) ---------------------------- */
 /* Compiles CUDA source for sm_100a with the run-time compiler; 1 when it compiles. The log goes to `out`. */

@@ -734,6 +734,12 @@ class Backend:
         logits; lse and entropy are the forward call's, grad_logits may be the logits."""
         operators.token_log_probs_backward(self, logits, tokens, lse, grad_logits, grad_log_probs, entropy, grad_entropy, scale, stream, device)
 
+    def operators_status(self, stream: Optional[int] = None, device: int = 0) -> None:
+        """Waits for `stream` (None: the backend's) and raises if an operator on the device met a page id, length or token id that is
+        out of range since it was last reported."""
+        if not self.lib.pjrtx_b200_operators_status(device, self.device_stream(device) if stream is None else stream):
+            raise BackendError("CommandSubmissionFailed", self._err())
+
     def compile_check(self, source: str) -> str:
         """Compiles generated CUDA source for sm_100a (no GPU needed); returns "" or the compiler log."""
         buf = ctypes.create_string_buffer(1 << 16)

@@ -830,6 +830,10 @@ int pjrtx_b200_token_log_probs_backward(int device_ordinal, const PjrtxB200Token
             s.grad_entropy = args->grad_entropy; return token_log_probs_backward(device_ordinal, s, (cudaStream_t)stream);)
 }
 
+int pjrtx_b200_operators_status(int device_ordinal, void* stream) {
+  GUARD_INT(return operators_status(device_ordinal, (cudaStream_t)stream);)
+}
+
 int pjrtx_b200_compile_check(const char* source, char* out, uint64_t capacity) {
   GUARD_INT(if (!source) return 0; std::vector<char> cubin; std::string log; bool ok = jit_compile_cubin(source, &cubin, &log);
             write_text(log, out, capacity); if (!ok) set_last_error("%s", log.c_str()); return ok ? 1 : 0;)

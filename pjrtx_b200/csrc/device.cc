@@ -62,9 +62,11 @@ Device* get_device(int ordinal) {
   dev->staging_size = 1 << 20;
   if (!check_cuda(cudaMallocHost((void**)&dev->staging, dev->staging_size), "cudaMallocHost")) return nullptr;
   cudaEventCreateWithFlags(&dev->staging_wrap_event, cudaEventDisableTiming);
-  if (!check_cuda(cudaHostAlloc((void**)&dev->error_flag_host, sizeof(int), cudaHostAllocMapped), "cudaHostAlloc")) return nullptr;
-  *dev->error_flag_host = 0;
+  if (!check_cuda(cudaHostAlloc((void**)&dev->error_flag_host, (1 + kErrorWords) * sizeof(int), cudaHostAllocMapped), "cudaHostAlloc")) return nullptr;
+  memset(dev->error_flag_host, 0, (1 + kErrorWords) * sizeof(int));
   if (!check_cuda(cudaHostGetDevicePointer((void**)&dev->error_flag_dev, dev->error_flag_host, 0), "cudaHostGetDevicePointer")) return nullptr;
+  dev->operator_words_host = dev->error_flag_host + 1;
+  dev->operator_words_dev = dev->error_flag_dev + 1;
   Device* raw = dev.get();
   g_devices[ordinal] = std::move(dev);
   return raw;
@@ -73,17 +75,25 @@ Device* get_device(int ordinal) {
 bool check_device_flag(Device* dev) {
   if (!dev->error_flag_host) return true;
   int code = *(volatile int*)dev->error_flag_host;
-  if (code == 0) return true;
+  if (code == 0) return check_operator_words(dev);
   *(volatile int*)dev->error_flag_host = 0;
-  if (code >= kErrorPageId && code <= kErrorToken) {
-    set_last_error("a kernel on device %d met %s (code %d); the results of that call are invalid", dev->ordinal,
-                   code == kErrorPageId ? "a page table entry outside the pool of pages"
-                   : code == kErrorLength ? "a length outside the page table or a count beyond its length"
-                                          : "a token id outside the vocabulary",
-                   code);
-    return false;
-  }
   set_last_error("a kernel on device %d gave up a bounded wait (code %d); results of this stream are invalid", dev->ordinal, code);
+  return false;
+}
+
+bool check_operator_words(Device* dev) {
+  static const char* const kMet[kErrorWords] = {"a page table entry outside the pool of pages",
+                                                "a length outside the page table or a count beyond its length",
+                                                "a token id outside the vocabulary"};
+  std::string met;
+  for (int i = 0; i < kErrorWords; i++) {
+    volatile int* word = dev->operator_words_host + i;
+    if (*word == 0) continue;
+    *word = 0;
+    met += std::string(met.empty() ? "" : ", ") + kMet[i] + " (code " + std::to_string(kErrorPageId + i) + ")";
+  }
+  if (met.empty()) return true;
+  set_last_error("operators on device %d met %s; the results of those calls are invalid", dev->ordinal, met.c_str());
   return false;
 }
 

@@ -31,6 +31,9 @@ struct Device {
   // Written by kernels whose bounded waits give up (host-mapped so the host reads it without a copy).
   int* error_flag_host = nullptr;
   int* error_flag_dev = nullptr;
+  // Written by the operators' kernels, a word for each of their codes (kernels/operators.h), in the same allocation.
+  int* operator_words_host = nullptr;
+  int* operator_words_dev = nullptr;
   // Tensor-parallel communicator (void* = ncclComm_t), set by comm_init.
   void* comm = nullptr;
   int comm_rank = 0, comm_world = 1;
@@ -48,8 +51,10 @@ struct Device {
 int device_count();                 // 0 when no CUDA device is usable
 Device* get_device(int ordinal);    // nullptr + last_error on failure
 bool check_cuda(cudaError_t e, const char* what);
-// After a stream synchronize: false (with last_error set) when a kernel reported a timed-out device-side wait.
+// After a stream synchronize: false (with last_error set) when a kernel reported a timed-out device-side wait, or, of no such
+// report, an operator an argument that only the device sees. What is named is cleared.
 bool check_device_flag(Device* dev);
+bool check_operator_words(Device* dev);  // the second of these alone
 
 struct Buffer {
   int device = 0;

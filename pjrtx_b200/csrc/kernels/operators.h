@@ -9,10 +9,11 @@
 
 namespace pjrtx {
 
-// Codes that kernels leave in the device's error word for arguments which only the device can see.
+// Codes for arguments which only the device can see. Kernels set error_words[code - kErrorPageId], host-mapped memory of the device.
 constexpr int kErrorPageId = 40;   // a page table entry of a sequence's own rows names no page of the pool
 constexpr int kErrorLength = 41;   // a length is negative or beyond the page table, or a count does not fit its length
 constexpr int kErrorToken = 42;    // a token id is not below the vocabulary size
+constexpr int kErrorWords = 3;
 
 // Row t of sequence b: page table[b * table_stride + t / page_size], row t % page_size of it; element d of KV head g of that row
 // is at page * page_stride + row * row_stride + g * head_stride + d in both pools. Strides count elements.
@@ -30,7 +31,7 @@ struct PagedView {
   int batch = 0, batch_max = 0;  // of this call, and of any call on the same workspaces
   int kv_heads = 0, head_dim = 0, page_size = 0, max_pages = 0;
   int dtype = 0;
-  int* error_flag = nullptr;
+  int* error_words = nullptr;
   long long capacity() const { return (long long)page_size * max_pages; }
 };
 
@@ -85,7 +86,7 @@ struct TokenScore {
   int* top_ids = nullptr;
   float* top_log_probs = nullptr;
   int top = 0;
-  int* error_flag = nullptr;
+  int* error_words = nullptr;
 };
 constexpr int kScoreTopMax = 64;
 int token_score_launch(const TokenScore& s, int sm_count, bool pdl, cudaStream_t stream);
@@ -101,7 +102,7 @@ struct TokenScoreGrad {
   const float* grad_log_probs = nullptr;  // null: zeros
   const float* grad_entropy = nullptr;    // null: zeros, `entropy` is then not read
   float scale = 1.f;
-  int* error_flag = nullptr;
+  int* error_words = nullptr;
 };
 int token_score_grad_launch(const TokenScoreGrad& s, int sm_count, bool pdl, cudaStream_t stream);
 

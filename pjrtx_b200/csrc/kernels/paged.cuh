@@ -5,9 +5,9 @@
 
 namespace pjrtx {
 
-// Reports an argument that only the device sees; the host reads the word after a synchronize.
-__device__ __forceinline__ void report(int* error_flag, int code) {
-  if (error_flag) atomicExch(error_flag, code);
+// Reports an argument that only the device sees. A word for each code, so that none replaces another; every writer writes the same.
+__device__ __forceinline__ void report(int* error_words, int code) {
+  *const_cast<volatile int*>(error_words + (code - kErrorPageId)) = 1;
 }
 
 // Visible rows of a sequence, held to what its page table can name.
@@ -20,7 +20,7 @@ __device__ __forceinline__ int paged_length(const PagedView& c, int b) {
 // Whether the length itself is in range (asked by one thread of one block per sequence).
 __device__ __forceinline__ void paged_check_length(const PagedView& c, int b) {
   const int n = c.lengths[b];
-  if (n < 0 || n > c.page_size * c.max_pages) report(c.error_flag, kErrorLength);
+  if (n < 0 || n > c.page_size * c.max_pages) report(c.error_words, kErrorLength);
 }
 
 // Element offset of row `slot` of sequence b in either pool (KV head 0), or -1 where the table names no page.
@@ -28,7 +28,7 @@ __device__ __forceinline__ long long paged_row(const PagedView& c, int b, int sl
   const int column = slot / c.page_size;
   const int page = c.table[b * c.table_stride + column];
   if (page < 0 || page >= c.num_pages) {
-    report(c.error_flag, kErrorPageId);
+    report(c.error_words, kErrorPageId);
     return -1;
   }
   return page * c.page_stride + (long long)(slot - column * c.page_size) * c.row_stride;

@@ -203,7 +203,7 @@ __device__ __forceinline__ RowPlace locate(const AttendArgs& p, const Cursor& u)
     }
     r.page = p.c.table[u.b * p.c.table_stride + column];
     if (r.page < 0 || r.page >= p.c.num_pages) {
-      report(p.c.error_flag, kErrorPageId);
+      report(p.c.error_words, kErrorPageId);
       r.page = -1;
     }
   }

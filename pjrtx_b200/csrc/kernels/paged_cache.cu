@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(PagedView 
   int count = a.counts ? a.counts[b] : (int)a.rows;
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     paged_check_length(c, b);
-    if (count < 0 || count > a.rows || count > length) report(c.error_flag, kErrorLength);
+    if (count < 0 || count > a.rows || count > length) report(c.error_words, kErrorLength);
   }
   count = max(0, min(count, min((int)a.rows, length)));
   const int first = length - count;

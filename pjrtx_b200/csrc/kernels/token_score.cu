@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(THREADS, kScoreThreadsOfSm / THREADS) token_sc
         given = none ? -INFINITY : (Logit<T>::load(logits + token) - all.m) * a.scale - log_s;
       } else {
         given = __uint_as_float(0x7fffffffu);
-        report(a.error_flag, kErrorToken);
+        report(a.error_words, kErrorToken);
       }
     }
     a.log_probs[row] = given;
@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(kGradThreads) token_score_grad_kernel(TokenSco
   const T* logits = static_cast<const T*>(a.logits) + row * a.row_stride;
   T* grad = static_cast<T*>(a.grad_logits) + row * a.grad_row_stride;
   const int token = a.tokens[row];
-  if (part == 0 && threadIdx.x == 0 && token >= a.vocab) report(a.error_flag, kErrorToken);
+  if (part == 0 && threadIdx.x == 0 && token >= a.vocab) report(a.error_words, kErrorToken);
   const float lse = a.lse[row];
   const float g = token >= 0 && a.grad_log_probs ? a.grad_log_probs[row] * a.scale : 0.f;
   const float h = ENTROPY ? a.grad_entropy[row] * a.scale : 0.f, entropy = ENTROPY ? a.entropy[row] : 0.f;

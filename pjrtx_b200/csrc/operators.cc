@@ -37,7 +37,7 @@ bool complete(const PagedCache& cache, PagedView* v) {
   v->page_size = (int)c.page_size;
   v->max_pages = (int)c.max_pages;
   v->dtype = c.dtype;
-  v->error_flag = cache.device->error_flag_dev;
+  v->error_words = cache.device->operator_words_dev;
   if (v->batch < 0 || v->batch > c.batch) return refuse("paged cache: a batch of %lld, the cache was made for up to %lld", v->batch, c.batch);
   if (!v->k || !v->v || !v->table || !v->lengths) return refuse("paged cache: null pages, page table or lengths");
   if (v->num_pages < 1 || v->num_pages > INT32_MAX) return refuse("paged cache: %lld pages", v->num_pages);
@@ -182,7 +182,7 @@ int token_log_probs(int ordinal, TokenScore s, cudaStream_t stream) {
   if (!s.log_probs) return refuse("token log probabilities: null result");
   Device* dev = get_device(ordinal);
   if (!dev) return 0;
-  s.error_flag = dev->error_flag_dev;
+  s.error_words = dev->operator_words_dev;
   CurrentDevice scope(dev->ordinal);
   return launched(token_score_launch(s, dev->sm_count, true, stream), what);
 }
@@ -200,9 +200,16 @@ int token_log_probs_backward(int ordinal, TokenScoreGrad s, cudaStream_t stream)
     return refuse("gradient of token log probabilities: in place, but the rows are %lld and %lld apart", s.row_stride, s.grad_row_stride);
   Device* dev = get_device(ordinal);
   if (!dev) return 0;
-  s.error_flag = dev->error_flag_dev;
+  s.error_words = dev->operator_words_dev;
   CurrentDevice scope(dev->ordinal);
   return launched(token_score_grad_launch(s, dev->sm_count, true, stream), what);
+}
+
+int operators_status(int ordinal, cudaStream_t stream) {
+  Device* dev = get_device(ordinal);
+  if (!dev) return 0;
+  CurrentDevice scope(dev->ordinal);
+  return check_cuda(cudaStreamSynchronize(stream), "cudaStreamSynchronize") && check_operator_words(dev);
 }
 
 }  // namespace pjrtx

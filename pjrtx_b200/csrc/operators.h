@@ -33,5 +33,7 @@ int paged_cache_attend(const PagedCache& cache, PagedView view, PagedAttend args
 int paged_cache_evict(const PagedCache& cache, PagedView view, PagedEvict args, cudaStream_t stream);
 int token_log_probs(int ordinal, TokenScore args, cudaStream_t stream);
 int token_log_probs_backward(int ordinal, TokenScoreGrad args, cudaStream_t stream);
+// Waits for the stream; 0 with last_error set where an operator on the device has met what only the device sees.
+int operators_status(int ordinal, cudaStream_t stream);
 
 }  // namespace pjrtx

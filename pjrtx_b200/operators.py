@@ -71,6 +71,7 @@ SYMBOLS = {
     "pjrtx_b200_paged_cache_evict": (ctypes.c_int, [_P, _P, _P, _P]),
     "pjrtx_b200_token_log_probs": (ctypes.c_int, [ctypes.c_int, _P, _P]),
     "pjrtx_b200_token_log_probs_backward": (ctypes.c_int, [ctypes.c_int, _P, _P]),
+    "pjrtx_b200_operators_status": (ctypes.c_int, [ctypes.c_int, _P]),
 }
 
 # Argument structs are packed in one step: filling a ctypes structure field by field takes twice as long as the call itself.

@@ -583,6 +583,56 @@ def test_out_of_range_pages_and_lengths_are_reported_and_not_followed(gpu_backen
 
 
 @pytest.mark.gpu
+def test_status_waits_for_the_callers_stream(gpu_backend):
+    """A bad argument of a call that a stream has not come to yet is known when its status is."""
+    c = _Case("bf16", 4, 2, 64, 16, [40, 40], seed=10)
+    torch, cache = c.torch, c.handle(gpu_backend)
+    q, table = c.randn(2, 4, 64), c.table.clone()
+    table[1, 1] = 10 ** 6
+    out, x = torch.empty_like(q), torch.zeros((3, 100), device="cuda")
+    tokens, score = torch.tensor([5, 100, 7], dtype=torch.int32, device="cuda"), torch.empty(3, device="cuda")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)  # 0.1 s
+    cache.attend(q, c.k, c.v, table, c.lengths, out, stream=side.cuda_stream)
+    gpu_backend.synchronize()  # of the backend's stream, where nothing happened
+    with pytest.raises(be_mod.BackendError, match="outside the pool of pages .code 40.;"):
+        gpu_backend.operators_status(stream=side.cuda_stream)
+    gpu_backend.operators_status(stream=side.cuda_stream)  # reported once
+    # several of them, from several calls
+    cache.attend(q, c.k, c.v, table, c.lengths, out, stream=side.cuda_stream)
+    gpu_backend.token_log_probs(x, tokens, score, stream=side.cuda_stream)
+    with pytest.raises(be_mod.BackendError, match="code 40.*code 42"):
+        gpu_backend.operators_status(stream=side.cuda_stream)
+    gpu_backend.operators_status()
+    gpu_backend.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wait_first", [True, False])
+def test_an_operators_report_does_not_replace_that_of_a_wait(gpu_backend, wait_first):
+    import torch
+
+    x, score = torch.zeros((3, 100), device="cuda"), torch.empty(3, device="cuda")
+    tokens = torch.tensor([5, 100, 7], dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    for wait in (wait_first, not wait_first):
+        if wait:
+            gpu_backend.bounded_wait_probe(0, timeout_ms=20)
+        else:
+            gpu_backend.token_log_probs(x, tokens, score)
+    torch.cuda.synchronize()
+    reports = []
+    for _ in range(2):
+        with pytest.raises(be_mod.BackendError) as e:
+            gpu_backend.synchronize()
+        reports.append(str(e.value))
+    assert "bounded wait" in reports[0] and "outside the vocabulary" in reports[1]
+    gpu_backend.synchronize()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,kv_heads,head_dim,page", [("bf16", 8, 128, 16), ("f32", 2, 64, 5), ("f16", 1, 8, 3), ("f32", 3, 4, 64)])
 @pytest.mark.parametrize("track", [False, True])
 def test_append(gpu_backend, dtype, kv_heads, head_dim, page, track):
