@@ -763,7 +763,7 @@ int pjrtx_b200_dot_static_scratch_status(int device_ordinal, void* stream) {
 }
 
 void* pjrtx_b200_device_stream(int device_ordinal) {
-  GUARD_PTR(Device* d = get_device(device_ordinal); return d ? (void*)d->stream : nullptr;)
+  GUARD_PTR(Device* d = get_device_aside(device_ordinal); return d ? (void*)d->stream : nullptr;)
 }
 
 void* pjrtx_b200_buffer_device_pointer(PjrtxB200Buffer* buffer) {

@@ -72,6 +72,14 @@ Device* get_device(int ordinal) {
   return raw;
 }
 
+Device* get_device_aside(int ordinal) {
+  int before = -1, now = -1;
+  if (cudaGetDevice(&before) != cudaSuccess) before = -1;
+  Device* dev = get_device(ordinal);
+  if (before >= 0 && cudaGetDevice(&now) == cudaSuccess && now != before) cudaSetDevice(before);
+  return dev;
+}
+
 bool check_device_flag(Device* dev) {
   if (!dev->error_flag_host) return true;
   int code = *(volatile int*)dev->error_flag_host;

@@ -49,7 +49,8 @@ struct Device {
 };
 
 int device_count();                 // 0 when no CUDA device is usable
-Device* get_device(int ordinal);    // nullptr + last_error on failure
+Device* get_device(int ordinal);    // nullptr + last_error on failure; the first use of a device makes it current
+Device* get_device_aside(int ordinal);  // the same, with the caller's device current behind it
 bool check_cuda(cudaError_t e, const char* what);
 // After a stream synchronize: false (with last_error set) when a kernel reported a timed-out device-side wait, or, of no such
 // report, an operator an argument that only the device sees. What is named is cleared.

@@ -22,6 +22,8 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // Whether a stride keeps 16-byte pieces aligned; where the axis has one element it is not used.
 bool stride_ok(int64_t stride, int64_t extent, int dtype) { return extent <= 1 || (stride > 0 && stride * (int64_t)dtype_size(dtype) % 16 == 0); }
 
+bool entered(const CurrentDevice& scope, const Device* dev) { return scope.ok || refuse("cudaSetDevice(%lld) failed", dev->ordinal); }
+
 bool launched(int kernels, const char* what) {
   if (kernels > 0) return true;
   set_last_error("%s: launch failed: %s", what, cudaGetErrorString(cudaGetLastError()));
@@ -64,7 +66,7 @@ PagedCache* paged_cache_create(int ordinal, const PagedCacheConfig& c) {
     return bad(refuse("paged cache: head dimension %lld (up to %lld, a multiple of 16 bytes)", c.head_dim, kMaxHeadDim));
   if (c.page_size < 1 || c.max_pages < 1 || c.page_size > kMaxCapacity || c.max_pages > kMaxCapacity || c.page_size * c.max_pages > kMaxCapacity)
     return bad(refuse("paged cache: %lld pages of %lld rows a sequence (up to %lld rows)", c.max_pages, c.page_size, kMaxCapacity));
-  Device* dev = get_device(ordinal);
+  Device* dev = get_device_aside(ordinal);
   if (!dev) return nullptr;
   PagedCache made;
   made.device = dev;
@@ -81,6 +83,7 @@ PagedCache* paged_cache_create(int ordinal, const PagedCacheConfig& c) {
   const uint64_t evict_at = (attend.bytes + 255) / 256 * 256;
   made.bytes = evict_at + evict.bytes;
   CurrentDevice scope(dev->ordinal);
+  if (!entered(scope, dev)) return nullptr;
   made.attend_space = device_malloc(dev, made.bytes);
   if (!made.attend_space) return nullptr;
   made.evict_space = c.track ? static_cast<char*>(made.attend_space) + evict_at : nullptr;
@@ -113,6 +116,7 @@ int paged_cache_append(const PagedCache& cache, PagedView view, const PagedAppen
       !stride_ok(a.row_stride, a.rows, c.dtype) || !stride_ok(a.head_stride, c.kv_heads, c.dtype))
     return refuse("append: new rows need 16-byte aligned pointers and strides (%lld, %lld, %lld elements)", a.batch_stride, a.row_stride, a.head_stride);
   CurrentDevice scope(cache.device->ordinal);
+  if (!entered(scope, cache.device)) return 0;
   return launched(paged_append_launch(view, a, cache.device->sm_count, true, stream), "append");
 }
 
@@ -133,6 +137,7 @@ int paged_cache_attend(const PagedCache& cache, PagedView view, PagedAttend a, c
                   !stride_ok(a.new_head_stride, c.kv_heads, c.dtype)))
     return refuse("attend: the new row needs 16-byte aligned pointers and strides (%lld, %lld elements)", a.new_batch_stride, a.new_head_stride);
   CurrentDevice scope(cache.device->ordinal);
+  if (!entered(scope, cache.device)) return 0;
   return launched(paged_attend_launch(view, a, cache.device->sm_count, true, stream), "attend");
 }
 
@@ -145,6 +150,7 @@ int paged_cache_evict(const PagedCache& cache, PagedView view, PagedEvict e, cud
   if (!e.lengths_out || !e.weights_out || !e.positions_out) return refuse("evict: null lengths, weights or positions to write");
   if (view.batch == 0) return 1;
   CurrentDevice scope(cache.device->ordinal);
+  if (!entered(scope, cache.device)) return 0;
   return launched(paged_evict_launch(view, e, cache.device->sm_count, true, stream), "evict");
 }
 
@@ -180,10 +186,11 @@ int token_log_probs(int ordinal, TokenScore s, cudaStream_t stream) {
   if (s.top && !s.top_ids && !s.top_log_probs) return refuse("token log probabilities: alternatives are asked for and have no place");
   if (s.rows == 0) return 1;
   if (!s.log_probs) return refuse("token log probabilities: null result");
-  Device* dev = get_device(ordinal);
+  Device* dev = get_device_aside(ordinal);
   if (!dev) return 0;
   s.error_words = dev->operator_words_dev;
   CurrentDevice scope(dev->ordinal);
+  if (!entered(scope, dev)) return 0;
   return launched(token_score_launch(s, dev->sm_count, true, stream), what);
 }
 
@@ -198,17 +205,19 @@ int token_log_probs_backward(int ordinal, TokenScoreGrad s, cudaStream_t stream)
     return refuse("gradient of token log probabilities: null, misaligned or overlapping result rows");
   if (s.grad_logits == s.logits && s.rows > 1 && s.grad_row_stride != s.row_stride)
     return refuse("gradient of token log probabilities: in place, but the rows are %lld and %lld apart", s.row_stride, s.grad_row_stride);
-  Device* dev = get_device(ordinal);
+  Device* dev = get_device_aside(ordinal);
   if (!dev) return 0;
   s.error_words = dev->operator_words_dev;
   CurrentDevice scope(dev->ordinal);
+  if (!entered(scope, dev)) return 0;
   return launched(token_score_grad_launch(s, dev->sm_count, true, stream), what);
 }
 
 int operators_status(int ordinal, cudaStream_t stream) {
-  Device* dev = get_device(ordinal);
+  Device* dev = get_device_aside(ordinal);
   if (!dev) return 0;
   CurrentDevice scope(dev->ordinal);
+  if (!entered(scope, dev)) return 0;
   return check_cuda(cudaStreamSynchronize(stream), "cudaStreamSynchronize") && check_operator_words(dev);
 }
 
