@@ -497,7 +497,7 @@ typedef struct PjrtxB200PagedView {
 } PjrtxB200PagedView;
 
 PjrtxB200PagedCache *pjrtx_b200_paged_cache_create(int device_ordinal, const PjrtxB200PagedCacheConfig *config);
-/* Waits for the device, then frees the workspaces. */
+/* Waits for the device, then frees the workspaces. Not while a stream of the process is captured: the wait ends the capture. */
 void pjrtx_b200_paged_cache_destroy(PjrtxB200PagedCache *cache);
 
 /* Row lengths[b] - counts[b] + t of sequence b becomes new row t, t < counts[b]. Tracking: weight 0, position

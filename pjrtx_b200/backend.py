@@ -480,6 +480,7 @@ class Backend:
         return out.value
 
     def synchronize(self, device: int = 0) -> None:
+        operators.free_unreferenced()
         if not self.lib.pjrtx_b200_device_synchronize(device):
             raise BackendError("CommandSubmissionFailed", self._err())
 

@@ -203,6 +203,17 @@ def _dense(x, name: str, dtype: int, shape: Tuple[int, ...], device: int) -> int
     return pointer
 
 
+# (library, handle) of caches that the collector found. Freeing one waits for the device, which would end a stream capture that is
+# under way wherever the collector happens to run, so it is done where the caller waits for the device anyway.
+_unreferenced: list = []
+
+
+def free_unreferenced() -> None:
+    while _unreferenced:
+        lib, handle = _unreferenced.pop()
+        lib.pjrtx_b200_paged_cache_destroy(handle)
+
+
 class PagedCache:
     """Geometry and workspaces of a paged key-value cache: one handle serves all layers of a shape, on one stream at a time.
 
@@ -210,6 +221,9 @@ class PagedCache:
     the same for keys and values. Row t of sequence b is row t % page_size of page page_table[b, t // page_size]; `lengths[b]`
     counts the rows of a sequence, those that a call appends among them. With `track`, weights and positions are
     [batch, kv_heads, max_pages * page_size], and `tokens[b]` counts the tokens a sequence has seen.
+
+    `destroy` waits for the device and frees the workspaces; those of a cache that is only dropped are freed by the next `destroy`,
+    `Backend.paged_cache` or `Backend.synchronize`.
     """
 
     def __init__(self, backend, dtype: int, batch: int, heads: int, kv_heads: int, head_dim: int, page_size: int, max_pages: int,
@@ -218,6 +232,7 @@ class PagedCache:
         self.dtype, self.batch, self.heads, self.kv_heads, self.head_dim = dtype, batch, heads, kv_heads, head_dim
         self.page_size, self.max_pages, self.track, self.capacity = page_size, max_pages, bool(track), page_size * max_pages
         self.handle = None
+        free_unreferenced()
         config = PagedCacheConfig(ctypes.sizeof(PagedCacheConfig), dtype, int(bool(track)), batch, heads, kv_heads, head_dim, page_size, max_pages)
         self.handle = self._lib.pjrtx_b200_paged_cache_create(device, ctypes.byref(config))
         if not self.handle:
@@ -328,15 +343,14 @@ class PagedCache:
         self._call(self._lib.pjrtx_b200_paged_cache_evict, view, args, stream)
 
     def destroy(self) -> None:
+        free_unreferenced()
         if self.handle:
             self._lib.pjrtx_b200_paged_cache_destroy(self.handle)
             self.handle = None
 
     def __del__(self):
-        try:
-            self.destroy()
-        except Exception:
-            pass
+        if getattr(self, "handle", None):
+            _unreferenced.append((self._lib, self.handle))
 
 
 def _logits(x, device: int):

@@ -6,6 +6,7 @@ Tolerances follow from the arithmetic: a score is a sum of head_dim products in 
 exponential and what a split of it into two 16-bit numbers leaves; the result is rounded once to its type.
 """
 import ctypes
+import gc
 import math
 
 import numpy as np
@@ -139,6 +140,29 @@ class _Placed(_Array):
 
     def is_contiguous(self):
         return True
+
+
+def test_a_dropped_cache_is_freed_where_the_caller_waits(backend):
+    freed = []
+
+    class Library:
+        @staticmethod
+        def pjrtx_b200_paged_cache_destroy(handle):
+            freed.append(handle)
+
+    caches = [ops.PagedCache.__new__(ops.PagedCache) for _ in range(3)]
+    for i, c in enumerate(caches):
+        c._lib, c.handle = Library, 100 + i
+    del c
+    last = caches.pop()
+    caches.clear()
+    assert freed == []  # wherever the collector runs, a capture may be under way
+    last.destroy()
+    last.destroy()
+    assert sorted(freed) == [100, 101, 102] and last.handle is None
+    del last
+    ops.free_unreferenced()
+    assert len(freed) == 3
 
 
 class _Unreachable:
@@ -1084,6 +1108,30 @@ def test_operators_on_other_streams_and_in_graphs(gpu_backend):
     graph.replay()
     torch.cuda.synchronize()
     assert c.lengths.tolist() == [200, 41] and all(torch.equal(again[n], scored[n]) for n in scored)
+
+
+@pytest.mark.gpu
+def test_a_cache_dropped_during_a_capture_does_not_end_it(gpu_backend):
+    import torch
+
+    in_use = lambda: gpu_backend.memory_stats()["bytes_in_use"]
+    gc.collect()  # buffers that other tests have left
+    gpu_backend.synchronize()
+    before = in_use()
+    cache = gpu_backend.paged_cache(P.BF16_CODE, 4, 8, 2, 64, 16, 100, track=True)
+    held = in_use() - before
+    assert held > 0
+    x = torch.zeros(8, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x += 1
+        del cache
+        x += 1
+    graph.replay()
+    assert x.tolist() == [2.0] * 8
+    assert in_use() == before + held
+    gpu_backend.synchronize()
+    assert in_use() == before
 
 
 @pytest.mark.gpu
