@@ -490,7 +490,7 @@ typedef struct PjrtxB200PagedView {
   const int32_t *page_table; /* [batch, max_pages] */
   int64_t table_stride;
   const int32_t *lengths;    /* [batch]: rows of each sequence, those that the call appends among them; 0 = idle */
-  int64_t batch;
+  int64_t batch;             /* 0: the call does nothing, and arrays along the batch may be NULL */
   const int32_t *tokens;     /* [batch]: tokens each sequence has seen, the new ones among them; NULL without tracking */
   float *weights;            /* [batch, kv_heads, capacity]: attention weight each row has had; NULL without tracking */
   int32_t *positions;        /* [batch, kv_heads, capacity]: token of each row; NULL without tracking */

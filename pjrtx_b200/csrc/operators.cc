@@ -41,7 +41,8 @@ bool complete(const PagedCache& cache, PagedView* v) {
   v->dtype = c.dtype;
   v->error_words = cache.device->operator_words_dev;
   if (v->batch < 0 || v->batch > c.batch) return refuse("paged cache: a batch of %lld, the cache was made for up to %lld", v->batch, c.batch);
-  if (!v->k || !v->v || !v->table || !v->lengths) return refuse("paged cache: null pages, page table or lengths");
+  // Arrays of no sequences may have no address.
+  if (!v->k || !v->v || (v->batch > 0 && (!v->table || !v->lengths))) return refuse("paged cache: null pages, page table or lengths");
   if (v->num_pages < 1 || v->num_pages > INT32_MAX) return refuse("paged cache: %lld pages", v->num_pages);
   if (!aligned16(v->k) || !aligned16(v->v) || !stride_ok(v->page_stride, v->num_pages, c.dtype) ||
       !stride_ok(v->row_stride, c.page_size, c.dtype) || !stride_ok(v->head_stride, c.kv_heads, c.dtype))
@@ -144,11 +145,11 @@ int paged_cache_attend(const PagedCache& cache, PagedView view, PagedAttend a, c
 int paged_cache_evict(const PagedCache& cache, PagedView view, PagedEvict e, cudaStream_t stream) {
   if (!complete(cache, &view)) return 0;
   e.workspace = cache.evict_space;
-  if (!view.weights || !view.tokens) return refuse("evict: weights, positions and the sequences' token counts are needed");
   if (e.keep < 1 || e.recent < 0 || e.sinks < 0 || (int64_t)e.recent + e.sinks > e.keep)
     return refuse("evict: %lld rows to keep, %lld recent and %lld first tokens (at least 1, and room for the protected ones)", e.keep, e.recent, e.sinks);
-  if (!e.lengths_out || !e.weights_out || !e.positions_out) return refuse("evict: null lengths, weights or positions to write");
   if (view.batch == 0) return 1;
+  if (!view.weights || !view.tokens) return refuse("evict: weights, positions and the sequences' token counts are needed");
+  if (!e.lengths_out || !e.weights_out || !e.positions_out) return refuse("evict: null lengths, weights or positions to write");
   CurrentDevice scope(cache.device->ordinal);
   if (!entered(scope, cache.device)) return 0;
   return launched(paged_evict_launch(view, e, cache.device->sm_count, true, stream), "evict");

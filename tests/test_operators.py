@@ -783,6 +783,29 @@ def test_evict_of_a_cache_too_long_for_shared_memory(gpu_backend):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("track", [False, True])
+def test_a_batch_of_no_sequences(gpu_backend, track):
+    """Empty tensors have no address; such a call does nothing and is not an error, but its other arguments are looked at."""
+    import torch
+
+    cache = gpu_backend.paged_cache(P.BF16_CODE, 2, 4, 2, 64, 16, 3, track=track)
+    pools = [torch.zeros((9, 16, 2, 64), device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+    empty = lambda *d, t=torch.int32: torch.empty(d, dtype=t, device="cuda")
+    view = dict(k_pages=pools[0], v_pages=pools[1], page_table=empty(0, 3), lengths=empty(0), stream=_stream())
+    if track:
+        view.update(tokens=empty(0), weights=empty(0, 2, 48, t=torch.float32), positions=empty(0, 2, 48))
+    rows = lambda *d: empty(0, *d, t=torch.bfloat16)
+    cache.append(k_new=rows(5, 2, 64), v_new=rows(5, 2, 64), counts=empty(0), **view)
+    cache.attend(rows(4, 64), out=rows(4, 64), lse=empty(0, 4, t=torch.float32), k_new=rows(2, 64), v_new=rows(2, 64), **view)
+    if track:
+        cache.evict(keep=10, **view)
+        with pytest.raises(be_mod.BackendError, match="rows to keep"):
+            cache.evict(keep=0, **view)
+    gpu_backend.operators_status(stream=_stream())
+    assert not pools[0].any() and not pools[1].any()
+
+
+@pytest.mark.gpu
 def test_one_handle_serves_batches_of_different_sizes(gpu_backend):
     """Workspaces hold counters that every call leaves at zero, whatever the batch was before."""
     torch = None
