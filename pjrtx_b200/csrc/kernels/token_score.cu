@@ -580,7 +580,8 @@ __global__ void __launch_bounds__(kGradThreads) token_score_grad_kernel(TokenSco
     Pair d = g2;
     if (ENTROPY) {
       const float2 t = pair_split(pair_add(pair_fma(x, scale2, base2), rest2));
-      d = pair_fma(h2, pair_of(max_nan(t.x, -1e30f), max_nan(t.y, -1e30f)), g2);  // finite, for p = 0 to make it 0
+      // Finite, for p = 0 to make it 0; where p > 0, ln p is above -88 and the entropy is not negative.
+      d = pair_fma(h2, pair_of(max_nan(t.x, -128.f), max_nan(t.y, -128.f)), g2);
     }
     const float2 r = pair_split(pair_mul(p, d));
     x0 = r.x;

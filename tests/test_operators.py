@@ -1051,6 +1051,34 @@ def test_token_log_probs_backward(gpu_backend, dtype, rows, vocab, stride, grad_
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("large", [1e9, -1e20, 1e34])
+def test_gradient_of_ruled_out_logits_under_large_gradients(gpu_backend, dtype, large):
+    """What is ruled out, by -inf or by the type's lowest value, has gradient 0 whatever the entropy's gradient is."""
+    import torch
+
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    logits = (torch.randn((6, 1000), generator=gen, device="cuda") * 3).to(_torch_type(dtype))
+    out_of = torch.rand(logits.shape, generator=gen, device="cuda") < 0.5
+    logits[:3] = torch.where(out_of[:3], -math.inf, logits[:3])
+    logits[3:] = torch.where(out_of[3:], torch.finfo(logits.dtype).min, logits[3:])
+    tokens = torch.where(out_of, -1.0, 1.0).argmax(1).int()
+    fw = _score(gpu_backend, logits, tokens, 0)
+    g, h = torch.randn(6, generator=gen, device="cuda"), torch.full((6,), large, device="cuda")
+    grad = torch.empty_like(logits)
+    gpu_backend.token_log_probs_backward(logits, tokens, fw["lse"], grad, grad_log_probs=g, entropy=fw["entropy"], grad_entropy=h, stream=_stream())
+    log_p = logits.double() - fw["lse"].double()[:, None]
+    p = torch.exp(log_p)
+    term = torch.where(p > 0, (log_p + fw["entropy"].double()[:, None]) * h.double()[:, None], 0.0)
+    hot = torch.zeros_like(p).scatter(1, tokens.long()[:, None], g.double()[:, None])
+    size = p * (g.double().abs()[:, None] + term.abs()) * (2 + log_p.abs().clamp(max=200)) + hot.abs()
+    # beside the bound of the test above: ln p + entropy, of numbers below 16, may cancel down to their rounding
+    bound = 2 * HALF_ULP[dtype] * size + 2.0 ** -21 * size + p * abs(large) * 16 * 2.0 ** -23
+    assert (grad[out_of] == 0).all()
+    _within(grad, hot - p * (g.double()[:, None] + term), bound, "grad")
+
+
+@pytest.mark.gpu
 def test_gradient_of_a_row_without_possible_tokens_is_finite(gpu_backend):
     import torch
 
