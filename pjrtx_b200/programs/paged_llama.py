@@ -149,6 +149,12 @@ class PagedDecoder:
         """Takes the first counts[b] rows of contiguous caches [batch, rows, kv_heads, head_dim] in, keys and values of every
         layer in turn, as a prefill program returns them."""
         counts = np.asarray(counts, np.int32)
+        shapes = {tuple(getattr(c, "dims", None) or c.shape) for c in caches}  # buffers, or a tensor library's arrays
+        rows = max((s[1] for s in shapes if len(s) == 4), default=0)
+        if len(caches) != 2 * self.cfg.layers or shapes != {(self.batch, rows, self.cfg.kv_heads, self.cfg.head_dim)}:
+            raise ValueError(f"{2 * self.cfg.layers} caches [{self.batch}, rows, {self.cfg.kv_heads}, {self.cfg.head_dim}] are needed")
+        if counts.shape != (self.batch,) or np.any(counts < 0) or np.any(counts > rows):
+            raise ValueError(f"a count from 0 to {rows} for each of {self.batch} sequences is needed")
         self._grow(counts)
         table, lengths, tokens, new = (self._upload(a) for a in (self.table, self.lengths, self.tokens, counts))
         for i, ((k, v), tracked) in enumerate(zip(self.pools, self.tracked)):
@@ -156,13 +162,15 @@ class PagedDecoder:
 
     def step(self, tokens: Sequence[int]) -> Step:
         """Decodes one token of every sequence."""
-        be = self.backend
+        be, tokens = self.backend, np.asarray(tokens, np.int32)
+        if tokens.shape != (self.batch,):
+            raise ValueError(f"a token for each of {self.batch} sequences is needed")
         if self.keep is not None and np.any(self.lengths >= self.capacity):
             self._evict()
         position = self._upload(self.tokens)  # of the token that comes in now
         self._grow(np.ones(self.batch, np.int32))
         table, lengths, seen = self._upload(self.table), self._upload(self.lengths), self._upload(self.tokens)
-        x = be.execute_executable(self.embed, [self._upload(np.asarray(tokens)), self.weights["embed"]])[0]
+        x = be.execute_executable(self.embed, [self._upload(tokens), self.weights["embed"]])[0]
         for i, ((k, v), tracked) in enumerate(zip(self.pools, self.tracked)):
             q, k_new, v_new = be.execute_executable(self.before, [x, position] + self._layer(i, BEFORE))
             context = be.allocate_buffer(self.cfg.dtype, [self.batch, self.cfg.heads, self.cfg.head_dim], self.device)

@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 
+from pjrtx_b200 import backend as be_mod
 from pjrtx_b200.programs import llama, paged_llama
 from tests.util import assert_close
 
@@ -44,6 +45,26 @@ def test_paged_decoding_follows_contiguous_decoding(gpu_backend, batch, page_siz
         assert np.abs(got.log_prob - log_p[np.arange(batch), got.next_token]).max() < 1e-4
         assert np.abs(got.entropy + (np.exp(log_p) * log_p).sum(1)).max() < 1e-3
         token = outs[0].to_numpy()
+    be.synchronize()
+
+
+def test_a_refused_call_leaves_the_decoder_as_it_was(gpu_backend):
+    be, cfg, batch, seq = gpu_backend, llama.TINY, 2, 9
+    _, weights = _weights(be, cfg)
+    caches = [be.allocate_buffer(cfg.dtype, [batch, seq, cfg.kv_heads, cfg.head_dim]) for _ in range(2 * cfg.layers)]
+    decoder = paged_llama.PagedDecoder(be, cfg, weights, batch, 8, 4)
+    decoder.append(caches, [seq, 4])
+    state = lambda: (decoder.lengths.tolist(), decoder.tokens.tolist(), decoder.table.tolist(), list(decoder.free))
+    before = state()
+    short = [be.allocate_buffer(cfg.dtype, [batch, seq, cfg.kv_heads, cfg.head_dim - 8])] * (2 * cfg.layers)
+    for refused in (lambda: decoder.append(caches, [3]), lambda: decoder.append(caches, [-1, 2]), lambda: decoder.append(caches, [1, seq + 1]),
+                    lambda: decoder.append(caches[:-1], [1, 1]), lambda: decoder.append(short, [1, 1]), lambda: decoder.append(caches, [9, 30]),
+                    lambda: decoder.step([1]), lambda: decoder.step([1, 2, 3])):
+        with pytest.raises((ValueError, be_mod.BackendError)):
+            refused()
+        assert state() == before
+    decoder.step([1, 2])
+    assert decoder.lengths.tolist() == [seq + 1, 5]
     be.synchronize()
 
 
