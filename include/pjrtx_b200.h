@@ -448,8 +448,10 @@ int pjrtx_b200_dot_static_scratch_status(int device_ordinal, void *stream);
  * a paged key-value cache (append, attend, evict) and the scoring of a decoder's logits (log probabilities, entropy,
  * likeliest tokens, and the gradient). They read and write the caller's memory, allocate nothing per call, and enqueue on
  * `stream` (a cudaStream_t; NULL = the default stream); pjrtx_b200_device_stream gives the stream that buffers and
- * executables of a device use, pjrtx_b200_buffer_device_pointer a buffer's memory. The caller's current device is left as
- * it was. Set struct_size of every argument struct to its sizeof. Element types are f32, f16 and bf16; statistics and
+ * executables of a device use, pjrtx_b200_buffer_device_pointer a buffer's memory. That stream is ordered with no other, the
+ * default stream included. Buffers are filled and freed on it: a call on another stream that is given a buffer's memory has to
+ * be ordered behind the upload, and the buffer's destruction behind the call. The caller's current device is left as it was.
+ * Set struct_size of every argument struct to its sizeof. Element types are f32, f16 and bf16; statistics and
  * weights are f32, ids and lengths s32. Strides count elements; the innermost axis is dense.
  * 1 when enqueued, 0 with last_error set. What only the device sees (a page id outside the pool, a length outside the page
  * table, a token id outside the vocabulary) is never followed out of bounds: the kernel skips it and sets a word of its code

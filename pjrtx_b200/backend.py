@@ -726,13 +726,14 @@ class Backend:
                         scale: float = 1.0, stream: Optional[int] = None, device: int = 0) -> None:
         """Scores logits [rows, vocabulary] with p = softmax(scale * logits): log_probs [rows] = ln p[tokens], entropy [rows],
         lse [rows], and the likeliest ids and their log probabilities, as many as top_ids / top_log_probs [rows, k] have
-        columns (ties: the lower id first). A negative token id gives 0."""
+        columns (ties: the lower id first). A negative token id gives 0. Without `stream` the call goes to the backend's own, which
+        is not ordered with any stream of a tensor library."""
         operators.token_log_probs(self, logits, tokens, log_probs, entropy, lse, top_ids, top_log_probs, scale, stream, device)
 
     def token_log_probs_backward(self, logits, tokens, lse, grad_logits, grad_log_probs=None, entropy=None, grad_entropy=None,
                                  scale: float = 1.0, stream: Optional[int] = None, device: int = 0) -> None:
         """grad_logits [rows, vocabulary] = gradient of sum(grad_log_probs * log_probs) + sum(grad_entropy * entropy) by the
-        logits; lse and entropy are the forward call's, grad_logits may be the logits."""
+        logits; lse and entropy are the forward call's, grad_logits may be the logits. `stream` as in `token_log_probs`."""
         operators.token_log_probs_backward(self, logits, tokens, lse, grad_logits, grad_log_probs, entropy, grad_entropy, scale, stream, device)
 
     def operators_status(self, stream: Optional[int] = None, device: int = 0) -> None:

@@ -8,9 +8,9 @@
 // Bound by memory: at one query position the products take 1 FLOP a byte and query head of a KV head, where the GPU has 250 (bf16).
 // So one launch reads every row once with as many bytes in flight as fit, and the softmax keeps a running maximum and sum. Measured
 // (bf16, heads of 128, 32 query and 8 KV heads; one call after the other, device time):
-//   32 sequences up to 2048 rows, 180 MB: 38.7 us (4.6 TB/s). Rows arrive for 23 us of it, at 7.8 TB/s; before them 4 us of launch,
-//   shares and first addresses, behind them 2 to 5 us of joins, and blocks on busier ways to memory take longer for equal shares.
-//   2 sequences up to 65 536 rows, 64 query heads, 447 MB: 87 us (5.2 TB/s). 1 sequence of 517 rows: 7.4 us, all of it these latencies.
+//   32 sequences up to 2048 rows, 180 MB: 38.3 us (4.7 TB/s). Rows arrive for 23 us of it, at 7.8 TB/s; before them 4 us of launch,
+//   shares and first addresses, behind them 2 to 5 us of joins; blocks take 15 to 30 us for equal shares, why is not known.
+//   2 sequences up to 65 536 rows, 64 query heads, 447 MB: 85.5 us (5.2 TB/s). 1 sequence of 517 rows: 7.7 us, all of it these latencies.
 //
 // Tracking adds to weights[b, g, t] the weights e^(s_t - lse) of the query heads that read KV head g. They need the whole row's
 // lse, so the scores (4 bytes a head and key, against 4 * head_dim of key and value) go through the workspace to a second kernel.
@@ -43,8 +43,8 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { retur
 // the block that arrives last joins them in block order.
 //
 // Six warps, two blocks an SM: with twelve warps and one block, whose joins stop all of an SM's loads, batch 32 takes 43.5 us, not
-// 38.7 (65 536 rows 82.6, not 87); with four warps and three blocks 65 536 rows take 88.8. kSegmentCost 2: a join and the next start
-// take 3 to 5 us, a tile 1.9; with 0, batch 32 takes 39.2 us and 30 000 rows of one sequence 33.9 (31.6). It costs the shortest
+// 38.7 (65 536 rows 82.6, not 87); with four warps and three blocks 65 536 rows take 88.8. kSegmentCost 2 was taken for heads of 128 in
+// 16 bits, where a tile is 96 rows (192 for heads of 64, 48 and more for f32): a join and the next start take 3 to 5 us, a tile 1.9; with 0, batch 32 takes 39.2 us and 30 000 rows of one sequence 33.9 (31.6). It costs the shortest
 // rows, where a block could have had more segments: 64 sequences of 100 rows 12.2 us, 10.3 with 0.
 
 constexpr int kWarps = 6, kThreads = kWarps * 32;

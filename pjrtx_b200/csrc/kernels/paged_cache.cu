@@ -2,14 +2,14 @@
 //
 // append: row t of the new ones of sequence b becomes row lengths[b] - counts[b] + t of its pages. Pure copying: every row is
 // read once and written once, 16 bytes a thread, the threads of a warp on neighbouring pieces of one row. Bound by memory: 319 MB
-// in 52.7 us (floor 48.7); 51 MB in 11.
+// in 52.7 us (floor 48.7); 4 prompts up to 2048 rows of 8 heads of 128 in bf16, 51 MB, in 11.2.
 //
 // evict: of the n > keep rows of a (sequence, KV head) those stay that come first by (protected, weight descending, row
 // ascending), a row being protected when its token is among the first `sinks` or the last `recent`. Attention does not depend
 // on the order of its rows, so nothing is compacted: the i-th kept row at or beyond `keep` moves into the i-th dropped place
 // before it, and only those rows are read and written. The token of each row is kept beside it in `positions`. Bound by what a
-// block waits for: 11 us until the moves are known, however few rows there are (8 pairs of 2049 rows, one over: 9.3 us in all), then
-// by rows of 256 bytes in no order: 128 pairs up to 4096 rows cut to 2048 (73 MB) 27 us, 14 of them moving.
+// block waits for until the moves are known (8 pairs of 2049 rows, one over: 9.2 us in all), then by rows of 256 bytes in no order:
+// 128 pairs up to 4096 rows cut to 2048 (73 MB) 27.7 us, 14 of them moving.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -26,7 +26,7 @@ namespace {
 // ---- append --------------------------------------------------------------------------------------------------------
 
 // One piece of a key and of its value in flight a thread, and at most 64 blocks an SM for all sequences, which go on to further
-// pieces: 8177 rows each of 57 sequences (319 MB) 52.7 us, with 16 an SM 55.7, with a block for every 256 pieces 58.8 (floor 48.7).
+// pieces: up to 8177 rows of 57 sequences, 2 heads of 64 in bf16 (319 MB), 52.7 us, with 16 an SM 55.7, with a block for every 256 pieces 58.8 (floor 48.7).
 constexpr int kAppendThreads = 256;
 
 __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(PagedView c, PagedAppend a, int pieces, int esize) {

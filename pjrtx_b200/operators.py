@@ -4,8 +4,12 @@ Bindings of the `pjrtx_b200_paged_cache_*` and `pjrtx_b200_token_log_probs*` ent
 through `Backend.paged_cache`, `Backend.token_log_probs` and `Backend.token_log_probs_backward`. Arrays are `DeviceBuffer`s
 or any device tensors with `data_ptr()`, `shape`, `stride()` and `dtype` (torch's). Types, shapes and the device that an array
 says it is on (`get_device()` or `device`) are checked here, the rest behind the C ABI; nothing is copied, cast or kept. Calls
-enqueue on `stream`, a `cudaStream_t` as an integer (0: the default stream); None is the stream on which the backend's buffers and
-executables work.
+enqueue on `stream`, a `cudaStream_t` as an integer (0: the default stream).
+
+`stream=None` is the stream on which the backend's buffers and executables work. It does not wait for the default stream or for a
+tensor library's, nor they for it: tensors need the stream that they are worked on given, or events. Buffers are filled and freed
+on the backend's stream: a call that gets one on another stream has to be ordered behind its upload, and the buffer kept until the
+backend's stream is ordered behind the call.
 """
 from __future__ import annotations
 
@@ -220,7 +224,8 @@ class PagedCache:
     Pools are [pages, page_size, kv_heads, head_dim] in any layout that keeps the last axis dense and rows 16-byte aligned,
     the same for keys and values. Row t of sequence b is row t % page_size of page page_table[b, t // page_size]; `lengths[b]`
     counts the rows of a sequence, those that a call appends among them. With `track`, weights and positions are
-    [batch, kv_heads, max_pages * page_size], and `tokens[b]` counts the tokens a sequence has seen.
+    [batch, kv_heads, max_pages * page_size], and `tokens[b]` counts the tokens a sequence has seen. Calls go to `stream`, None: the
+    backend's own, which is not ordered with any stream of a tensor library.
 
     `destroy` waits for the device and frees the workspaces; those of a cache that is only dropped are freed by the next `destroy`,
     `Backend.paged_cache` or `Backend.synchronize`.
