@@ -213,9 +213,12 @@ _unreferenced: list = []
 
 
 def free_unreferenced() -> None:
-    while _unreferenced:
-        lib, handle = _unreferenced.pop()
-        lib.pjrtx_b200_paged_cache_destroy(handle)
+    try:
+        while True:
+            lib, handle = _unreferenced.pop()
+            lib.pjrtx_b200_paged_cache_destroy(handle)
+    except IndexError:  # empty, if only because another thread was faster
+        pass
 
 
 class PagedCache:
@@ -354,8 +357,11 @@ class PagedCache:
             self.handle = None
 
     def __del__(self):
-        if getattr(self, "handle", None):
-            _unreferenced.append((self._lib, self.handle))
+        try:
+            if self.handle:
+                _unreferenced.append((self._lib, self.handle))
+        except Exception:  # a half-made cache, or the interpreter's end
+            pass
 
 
 def _logits(x, device: int):
