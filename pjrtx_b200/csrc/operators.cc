@@ -10,6 +10,7 @@ namespace {
 
 constexpr int64_t kMaxHeadDim = 256;
 constexpr int64_t kMaxCapacity = 1 << 30;  // rows of one sequence
+constexpr int64_t kMaxTracked = 1ll << 40;  // scores of a tracked cache's workspace: 4 TB; sizes beyond 2^60 would not fit 64 bits
 constexpr int64_t kMaxVocab = 1 << 22;     // the chunk maxima of a row stay in shared memory
 
 bool refuse(const char* fmt, long long a = 0, long long b = 0, long long c = 0) {
@@ -67,6 +68,9 @@ PagedCache* paged_cache_create(int ordinal, const PagedCacheConfig& c) {
     return bad(refuse("paged cache: head dimension %lld (up to %lld, a multiple of 16 bytes)", c.head_dim, kMaxHeadDim));
   if (c.page_size < 1 || c.max_pages < 1 || c.page_size > kMaxCapacity || c.max_pages > kMaxCapacity || c.page_size * c.max_pages > kMaxCapacity)
     return bad(refuse("paged cache: %lld pages of %lld rows a sequence (up to %lld rows)", c.max_pages, c.page_size, kMaxCapacity));
+  if (c.track && c.batch * c.heads * (c.page_size * c.max_pages) > kMaxTracked)
+    return bad(refuse("paged cache: %lld sequences, %lld query heads and %lld rows are too many for a workspace of scores", c.batch, c.heads,
+                      c.page_size * c.max_pages));
   Device* dev = get_device_aside(ordinal);
   if (!dev) return nullptr;
   PagedCache made;

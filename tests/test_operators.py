@@ -80,6 +80,13 @@ def test_paged_cache_refuses_bad_geometry(backend, change, message):
         backend.paged_cache(**shape)
 
 
+@pytest.mark.parametrize("batch,heads,page_size", [(65535, 65535, 1 << 30), (50000, 30000, 993763988), (1 << 10, 1 << 10, (1 << 20) + 1)])
+def test_paged_cache_refuses_workspaces_beyond_any_memory(backend, batch, heads, page_size):
+    """Sizes of a tracked cache whose workspace would not fit 64 bits must not become those of a small one."""
+    with pytest.raises(be_mod.BackendError, match="too many for a workspace"):
+        backend.paged_cache(P.BF16_CODE, batch, heads, heads, 8, page_size, 1, track=True)
+
+
 def test_operator_structs_without_size_and_null_handles_are_refused(backend):
     lib = backend.lib
     config = ops.PagedCacheConfig(0, P.F32, 0, 1, 1, 1, 64, 16, 1)
