@@ -544,7 +544,8 @@ int pjrtx_b200_paged_cache_attend(PjrtxB200PagedCache *cache, const PjrtxB200Pag
 /* Cuts every sequence of more than `keep` rows to `keep`, each KV head by itself: rows of the first `sinks` and the last
  * `recent` tokens stay, then those with the most weight, of equal ones the lower row. The i-th kept row at or beyond `keep`
  * moves into the place of the i-th dropped row before it; the others stay where they are. Rows without a token get weight
- * 0 and position -1. The results may be the view's own arrays. Pages must not be shared between sequences. */
+ * 0 and position -1. The results may be the view's own arrays, but layers that share an array of lengths need another one for
+ * the new lengths, or the first would cut it for all. Pages must not be shared between sequences. */
 typedef struct PjrtxB200PagedEvictArgs {
   uint64_t struct_size;
   int64_t keep;   /* at least sinks + recent, and 1 */

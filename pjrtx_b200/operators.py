@@ -342,7 +342,8 @@ class PagedCache:
     def evict(self, k_pages, v_pages, page_table, lengths, tokens, weights, positions, keep: int, recent: int = 0, sinks: int = 0,
               lengths_out=None, weights_out=None, positions_out=None, stream: Optional[int] = None) -> None:
         """Cuts every sequence to `keep` rows by weight; tokens before `sinks` and the last `recent` ones stay. Results go to the
-        `*_out` arrays, None: in place. Pages must not be shared between sequences."""
+        `*_out` arrays, None: in place. Layers that share `lengths` need another array as `lengths_out`. Pages must not be shared
+        between sequences."""
         batch, view = self._view(k_pages, v_pages, page_table, lengths, tokens, weights, positions)
         tracked = (batch, self.kv_heads, self.capacity)
         args = _pack_evict(keep, recent, sinks, _dense(lengths if lengths_out is None else lengths_out, "lengths_out", P.S32, (batch,), self.device),
