@@ -445,17 +445,17 @@ int pjrtx_b200_dot_static_scratch_status(int device_ordinal, void *stream);
 
 /* ---- operators on device memory ---------------------------------------------- */
 /* No counterparts in the reference. Operators that a host calls directly, with device pointers and a stream of its own:
- * a paged key-value cache (append, attend, evict) and the scoring of a decoder's logits (log probabilities, entropy,
- * likeliest tokens, and the gradient). They read and write the caller's memory, allocate nothing per call, and enqueue on
+ * a paged key-value cache (append, store, attend, attend to trees, evict, page tables and slots), attention of packed prompts, and
+ * the scoring of a decoder's logits (log probabilities, entropy, likeliest tokens, and the gradient). They read and write the caller's memory, allocate nothing per call, and enqueue on
  * `stream` (a cudaStream_t; NULL = the default stream); pjrtx_b200_device_stream gives the stream that buffers and
  * executables of a device use, pjrtx_b200_buffer_device_pointer a buffer's memory. That stream is ordered with no other, the
  * default stream included. Buffers are filled and freed on it: a call on another stream that is given a buffer's memory has to
  * be ordered behind the upload, and the buffer's destruction behind the call. The caller's current device is left as it was.
  * Set struct_size of every argument struct to its sizeof. Element types are f32, f16 and bf16; statistics and
  * weights are f32, ids and lengths s32. Strides count elements; the innermost axis is dense.
- * 1 when enqueued, 0 with last_error set. What only the device sees (a page id outside the pool, a length outside the page
- * table, a token id outside the vocabulary) is never followed out of bounds: the kernel skips it and sets a word of its code
- * (40, 41, 42). pjrtx_b200_operators_status waits for the stream of a call and tells. The words are the device's, not the
+ * 1 when enqueued, 0 with last_error set. What only the device sees (a page id or slot outside the pool, a length outside the page
+ * table, a token id outside the vocabulary, a node's parent that does not come before it) is never followed out of bounds: the
+ * kernel skips it and sets a word of its code (40, 41, 42, 43). pjrtx_b200_operators_status waits for the stream of a call and tells. The words are the device's, not the
  * call's: pjrtx_b200_device_synchronize and copies to the host, which wait for the stream of pjrtx_b200_device_stream alone,
  * return 0 for what is set by then, whichever stream it came from, and what has been named once is not named again. */
 void *pjrtx_b200_device_stream(int device_ordinal);
@@ -478,6 +478,8 @@ typedef struct PjrtxB200PagedCacheConfig {
   int64_t head_dim;  /* up to 256, a multiple of 16 bytes */
   int64_t page_size; /* rows of a page, any number */
   int64_t max_pages; /* pages of a sequence, at most; capacity = page_size * max_pages rows */
+  int64_t tree_nodes; /* drafted tokens of a sequence that attend_tree can take, 0..64 (workspace for parts of results); a
+                         struct_size that ends before this field means 0 */
 } PjrtxB200PagedCacheConfig;
 
 /* What every call is told of the pools and of the batch. Pointers to pages and their strides keep 16-byte alignment. */
@@ -541,6 +543,99 @@ typedef struct PjrtxB200PagedAttendArgs {
 int pjrtx_b200_paged_cache_attend(PjrtxB200PagedCache *cache, const PjrtxB200PagedView *view,
                                   const PjrtxB200PagedAttendArgs *args, void *stream);
 
+/* Attention of a tree of drafted tokens per sequence, and of a further piece of a prompt (a tree that is a chain). Node i of
+ * sequence b sees the lengths[b] cached rows, its ancestors and itself: out = softmax(scale * q . k) v over these, lse its
+ * log-sum-exp. parents[b, i] is a node before i, or -1 for a root, of which there may be several; any other parent counts as
+ * -1 and is reported (43). Nothing is stored, lengths count cached rows only, and weights are not tracked. Results of nodes from counts[b]
+ * on are left as they were. Keys and values that a node does not see enter nothing, whatever they hold; infinities and NaN in those
+ * that it sees go on as in the formula, with probabilities below 2^-126 of the largest as zero. In 16 bits, probabilities are
+ * rounded to the element type (f16: to multiples of 2^-35 of the largest below 2^-25) before they meet the values, and so is what their sum is taken of. */
+typedef struct PjrtxB200PagedTreeArgs {
+  uint64_t struct_size;
+  const void *q; /* [batch, nodes, heads, head_dim] through the strides */
+  int64_t q_batch_stride;
+  int64_t q_node_stride;
+  int64_t q_head_stride;
+  void *out;     /* the same axes; not overlapping an input */
+  int64_t out_batch_stride;
+  int64_t out_node_stride;
+  int64_t out_head_stride;
+  float *lse;    /* [batch, nodes, heads], may be NULL */
+  const void *k_new; /* [batch, nodes, kv_heads, head_dim] through the strides */
+  const void *v_new;
+  int64_t new_batch_stride;
+  int64_t new_node_stride;
+  int64_t new_head_stride;
+  const int32_t *parents; /* [batch, nodes] */
+  const int32_t *counts;  /* [batch], NULL: `nodes` of every sequence */
+  int64_t nodes;          /* up to the cache's tree_nodes */
+  float scale;
+} PjrtxB200PagedTreeArgs;
+int pjrtx_b200_paged_cache_attend_tree(PjrtxB200PagedCache *cache, const PjrtxB200PagedView *view,
+                                       const PjrtxB200PagedTreeArgs *args, void *stream);
+
+/* Rows of packed keys and values go to slots: a row's slot is its page times page_size plus the row in the page. Negative slots
+ * are skipped. Of rows with the same slot, which one is stored is open (in pieces of 16 bytes). Takes no account of tracked weights. */
+typedef struct PjrtxB200PagedStoreArgs {
+  uint64_t struct_size;
+  const void *k_new; /* [rows, kv_heads, head_dim] through the strides */
+  const void *v_new;
+  int64_t rows;
+  int64_t row_stride;
+  int64_t head_stride;
+  const int32_t *slots; /* [rows] */
+} PjrtxB200PagedStoreArgs;
+/* Of the view, the pools and their strides are used; page table and lengths may be NULL. */
+int pjrtx_b200_paged_cache_store(PjrtxB200PagedCache *cache, const PjrtxB200PagedView *view, const PjrtxB200PagedStoreArgs *args,
+                                 void *stream);
+
+/* Gives every sequence the pages of lengths[b] rows. held[b] counts the pages a sequence has; free_pages is a stack of
+ * *free_count page ids, its top at the end. First, pages beyond what the lengths need go onto the stack, by sequence and column, and
+ * their table entries become -1. Then sequences take what they lack from the top, in order; the first that wants more than is
+ * left, and all behind it that want any, keep what they have (held_out[b] * page_size < lengths[b] tells). Popped places of the
+ * stack become -1. A sequence whose length or page count the table cannot hold is reported (41) and left as it is. With `slots`: packed
+ * token t of sequence b, starts[b] <= t < starts[b + 1], is one of its last starts[b + 1] - starts[b] rows, and slots[t] that row's
+ * slot; -1 for tokens of no sequence and of one without enough pages. Page tables must not name a page twice. The results may
+ * be the arrays that are read, or arrays that do not overlap them. */
+typedef struct PjrtxB200PagedAssignArgs {
+  uint64_t struct_size;
+  int64_t batch;
+  const int32_t *lengths;    /* [batch]: rows that each sequence is to have */
+  const int32_t *held;       /* [batch] */
+  const int32_t *page_table; /* [batch, max_pages], rows table_stride apart */
+  int64_t table_stride;
+  const int32_t *free_pages; /* [num_pages] */
+  const int32_t *free_count; /* [1] */
+  int64_t num_pages;         /* of the pool: ids are below it, and num_pages * page_size is below 2^31 */
+  int32_t *held_out;
+  int32_t *page_table_out;   /* rows table_out_stride apart */
+  int64_t table_out_stride;
+  int32_t *free_pages_out;
+  int32_t *free_count_out;
+  const int32_t *starts;     /* [batch + 1], NULL without slots */
+  int32_t *slots;            /* [tokens], NULL: none */
+  int64_t tokens;
+} PjrtxB200PagedAssignArgs;
+int pjrtx_b200_paged_cache_assign(PjrtxB200PagedCache *cache, const PjrtxB200PagedAssignArgs *args, void *stream);
+
+/* Slots of accepted drafts: the nodes on the way from leaves[b] to its root become, in their order, rows lengths[b], lengths[b] + 1,
+ * ... of sequence b, and slots[b, i] is where node i goes; -1 for the other nodes, and for all of them where leaves[b] is
+ * negative. lengths_out counts the rows with them. Pages for the rows have to be in the table; a row without one gets -1 and is
+ * reported (40), a path that ends beyond the table, or a leaf from `nodes` on, is reported (41) and accepts nothing. */
+typedef struct PjrtxB200PagedPathArgs {
+  uint64_t struct_size;
+  int64_t batch;
+  int64_t nodes;             /* 1..64 */
+  const int32_t *page_table; /* [batch, max_pages], rows table_stride apart */
+  int64_t table_stride;
+  const int32_t *lengths;    /* [batch] */
+  const int32_t *parents;    /* [batch, nodes], as in attend_tree */
+  const int32_t *leaves;     /* [batch] */
+  int32_t *slots;            /* [batch, nodes] */
+  int32_t *lengths_out;      /* [batch], may be lengths */
+} PjrtxB200PagedPathArgs;
+int pjrtx_b200_paged_cache_path_slots(PjrtxB200PagedCache *cache, const PjrtxB200PagedPathArgs *args, void *stream);
+
 /* Cuts every sequence of more than `keep` rows to `keep`, each KV head by itself: rows of the first `sinks` and the last
  * `recent` tokens stay, then those with the most weight, of equal ones the lower row. The i-th kept row at or beyond `keep`
  * moves into the place of the i-th dropped row before it; the others stay where they are. Rows without a token get weight
@@ -557,6 +652,36 @@ typedef struct PjrtxB200PagedEvictArgs {
 } PjrtxB200PagedEvictArgs;
 int pjrtx_b200_paged_cache_evict(PjrtxB200PagedCache *cache, const PjrtxB200PagedView *view,
                                  const PjrtxB200PagedEvictArgs *args, void *stream);
+
+/* Causal attention of whole prompts, packed one behind the other: token i of sequence b, starts[b] <= i < starts[b + 1], sees
+ * the tokens of its sequence up to itself: out = softmax(scale * q . k) v, lse = ln sum e^(scale * q . k). Rows of no sequence are
+ * neither read for a result nor written. A sequence that does not lie in 0..tokens is skipped and reported (41); starts that descend
+ * are reported too, and the results of the call are then open. Later tokens and other sequences enter nothing, whatever they hold; for the rest of infinities, NaN and rounding see attend_tree. */
+typedef struct PjrtxB200PromptAttentionArgs {
+  uint64_t struct_size;
+  int32_t dtype;
+  float scale;
+  const void *q;         /* [tokens, heads, head_dim] through the strides, 16-byte aligned rows; head h reads KV head h / (heads / kv_heads) */
+  const void *k;         /* [tokens, kv_heads, head_dim] */
+  const void *v;
+  void *out;             /* [tokens, heads, head_dim]; not overlapping an input */
+  float *lse;            /* [tokens, heads], may be NULL */
+  int64_t tokens;
+  int64_t heads;         /* a multiple of kv_heads */
+  int64_t kv_heads;
+  int64_t head_dim;      /* up to 256, a multiple of 16 bytes */
+  int64_t q_stride;      /* between tokens */
+  int64_t q_head_stride;
+  int64_t k_stride;
+  int64_t k_head_stride;
+  int64_t v_stride;
+  int64_t v_head_stride;
+  int64_t out_stride;
+  int64_t out_head_stride;
+  const int32_t *starts; /* [sequences + 1] */
+  int64_t sequences;
+} PjrtxB200PromptAttentionArgs;
+int pjrtx_b200_prompt_attention(int device_ordinal, const PjrtxB200PromptAttentionArgs *args, void *stream);
 
 /* Scores rows of logits. With p = softmax(scale * logits) of a row: log_probs = ln p[token], entropy = -sum p ln p,
  * lse = ln sum e^(scale * logits), and the `top` likeliest ids with their log probabilities, likeliest first, of equal
@@ -601,7 +726,7 @@ typedef struct PjrtxB200TokenLogProbsBackwardArgs {
 int pjrtx_b200_token_log_probs_backward(int device_ordinal, const PjrtxB200TokenLogProbsBackwardArgs *args, void *stream);
 
 /* Waits for `stream`; 1, or 0 with last_error naming what the operators' kernels on the device met since it was last asked
- * (all of codes 40, 41 and 42 that are set). A bounded wait of an executable's kernel that gave up is not among it and stays
+ * (all of codes 40 to 43 that are set). A bounded wait of an executable's kernel that gave up is not among it and stays
  * for pjrtx_b200_device_synchronize. Not during a stream capture. */
 int pjrtx_b200_operators_status(int device_ordinal, void *stream);
 

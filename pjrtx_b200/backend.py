@@ -718,9 +718,17 @@ class Backend:
         return stream
 
     def paged_cache(self, dtype: int, batch: int, heads: int, kv_heads: int, head_dim: int, page_size: int, max_pages: int,
-                    track: bool = False, device: int = 0) -> operators.PagedCache:
-        """Handle of a paged key-value cache with `append`, `attend` and `evict`; batch and max_pages are upper bounds."""
-        return operators.PagedCache(self, dtype, batch, heads, kv_heads, head_dim, page_size, max_pages, track, device)
+                    track: bool = False, device: int = 0, tree: int = 0) -> operators.PagedCache:
+        """Handle of a paged key-value cache with `append`, `store`, `attend`, `attend_tree`, `evict`, `assign_pages` and `path_slots`;
+        batch, max_pages and tree (drafted tokens of a sequence) are upper bounds."""
+        return operators.PagedCache(self, dtype, batch, heads, kv_heads, head_dim, page_size, max_pages, track, device, tree)
+
+    def prompt_attention(self, q, k, v, starts, out, lse=None, scale: Optional[float] = None, stream: Optional[int] = None,
+                         device: int = 0) -> None:
+        """Causal attention of packed prompts: out [tokens, heads, head_dim] = softmax(scale * q . k) v over a token's sequence up to
+        itself, sequence b being rows starts[b] to starts[b + 1] of all arrays; k and v are [tokens, kv_heads, head_dim], `scale`
+        None is 1 / sqrt(head_dim), lse [tokens, heads] the log-sum-exp. Rows of no sequence stay. `stream` as in `token_log_probs`."""
+        operators.prompt_attention(self, q, k, v, starts, out, lse, scale, stream, device)
 
     def token_log_probs(self, logits, tokens, log_probs, entropy=None, lse=None, top_ids=None, top_log_probs=None,
                         scale: float = 1.0, stream: Optional[int] = None, device: int = 0) -> None:
@@ -737,7 +745,7 @@ class Backend:
         operators.token_log_probs_backward(self, logits, tokens, lse, grad_logits, grad_log_probs, entropy, grad_entropy, scale, stream, device)
 
     def operators_status(self, stream: Optional[int] = None, device: int = 0) -> None:
-        """Waits for `stream` (None: the backend's) and raises if an operator on the device met a page id, length or token id that is
+        """Waits for `stream` (None: the backend's) and raises if an operator on the device met a page id, length, token id or parent that is
         out of range since it was last reported."""
         if not self.lib.pjrtx_b200_operators_status(device, self.device_stream(device) if stream is None else stream):
             raise BackendError("CommandSubmissionFailed", self._err())

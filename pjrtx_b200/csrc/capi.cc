@@ -3,6 +3,7 @@
 // the same way, e.g. src/backend/mlx_metal/api.cc:3391-3497).
 #include "../../include/pjrtx_b200.h"
 
+#include <cstddef>
 #include <cstring>
 #include <new>
 
@@ -76,8 +77,8 @@ PjrtxB200Buffer* wrap(Buffer* b) {
 
 // An argument struct of this header's size or a later one's.
 template <typename Args>
-bool have(const Args* args) {
-  if (args && args->struct_size >= sizeof(Args)) return true;
+bool have(const Args* args, size_t least = sizeof(Args)) {
+  if (args && args->struct_size >= least) return true;
   set_last_error(args ? "argument struct of %llu bytes (set struct_size)" : "null argument struct", args ? (unsigned long long)args->struct_size : 0ull);
   return false;
 }
@@ -774,9 +775,11 @@ void* pjrtx_b200_buffer_device_pointer(PjrtxB200Buffer* buffer) {
 }
 
 PjrtxB200PagedCache* pjrtx_b200_paged_cache_create(int device_ordinal, const PjrtxB200PagedCacheConfig* config) {
-  GUARD_PTR(if (!have(config)) return nullptr; PagedCacheConfig c; c.dtype = config->dtype; c.track = config->track != 0;
+  GUARD_PTR(if (!have(config, offsetof(PjrtxB200PagedCacheConfig, tree_nodes))) return nullptr; PagedCacheConfig c;
+            c.dtype = config->dtype; c.track = config->track != 0;
             c.batch = config->batch; c.heads = config->heads; c.kv_heads = config->kv_heads; c.head_dim = config->head_dim;
             c.page_size = config->page_size; c.max_pages = config->max_pages;
+            if (config->struct_size >= sizeof *config) c.tree_nodes = config->tree_nodes;
             PagedCache* made = paged_cache_create(device_ordinal, c); return made ? new PjrtxB200PagedCache{made} : nullptr;)
 }
 
@@ -813,6 +816,46 @@ int pjrtx_b200_paged_cache_evict(PjrtxB200PagedCache* cache, const PjrtxB200Page
             e.recent = narrow(args->recent); e.sinks = narrow(args->sinks); e.lengths_out = args->lengths_out;
             e.weights_out = args->weights_out; e.positions_out = args->positions_out;
             return paged_cache_evict(*cache->cache, view_of(*view), e, (cudaStream_t)stream);)
+}
+
+int pjrtx_b200_paged_cache_attend_tree(PjrtxB200PagedCache* cache, const PjrtxB200PagedView* view, const PjrtxB200PagedTreeArgs* args,
+                                       void* stream) {
+  GUARD_INT(if (!have_cache(cache) || !have(view) || !have(args)) return 0; PagedTree a; a.q = args->q;
+            a.q_batch_stride = args->q_batch_stride; a.q_node_stride = args->q_node_stride; a.q_head_stride = args->q_head_stride;
+            a.out = args->out; a.out_batch_stride = args->out_batch_stride; a.out_node_stride = args->out_node_stride;
+            a.out_head_stride = args->out_head_stride; a.lse = args->lse; a.k_new = args->k_new; a.v_new = args->v_new;
+            a.new_batch_stride = args->new_batch_stride; a.new_node_stride = args->new_node_stride;
+            a.new_head_stride = args->new_head_stride; a.parents = args->parents; a.counts = args->counts; a.nodes = narrow(args->nodes);
+            a.scale = args->scale; return paged_cache_attend_tree(*cache->cache, view_of(*view), a, (cudaStream_t)stream);)
+}
+
+int pjrtx_b200_paged_cache_store(PjrtxB200PagedCache* cache, const PjrtxB200PagedView* view, const PjrtxB200PagedStoreArgs* args, void* stream) {
+  GUARD_INT(if (!have_cache(cache) || !have(view) || !have(args)) return 0; PagedStore a; a.k_new = args->k_new; a.v_new = args->v_new;
+            a.rows = args->rows; a.row_stride = args->row_stride; a.head_stride = args->head_stride; a.slots = args->slots;
+            return paged_cache_store(*cache->cache, view_of(*view), a, (cudaStream_t)stream);)
+}
+
+int pjrtx_b200_paged_cache_assign(PjrtxB200PagedCache* cache, const PjrtxB200PagedAssignArgs* args, void* stream) {
+  GUARD_INT(if (!have_cache(cache) || !have(args)) return 0; PagedAssign a; a.lengths = args->lengths; a.held = args->held;
+            a.table = args->page_table; a.table_stride = args->table_stride; a.free_pages = args->free_pages; a.free_count = args->free_count;
+            a.held_out = args->held_out; a.table_out = args->page_table_out; a.table_out_stride = args->table_out_stride;
+            a.free_pages_out = args->free_pages_out; a.free_count_out = args->free_count_out; a.starts = args->starts; a.slots = args->slots;
+            a.tokens = args->tokens; return paged_cache_assign(*cache->cache, a, args->batch, args->num_pages, (cudaStream_t)stream);)
+}
+
+int pjrtx_b200_paged_cache_path_slots(PjrtxB200PagedCache* cache, const PjrtxB200PagedPathArgs* args, void* stream) {
+  GUARD_INT(if (!have_cache(cache) || !have(args)) return 0; PagedPath a; a.table = args->page_table; a.table_stride = args->table_stride;
+            a.lengths = args->lengths; a.parents = args->parents; a.leaves = args->leaves; a.slots = args->slots;
+            a.lengths_out = args->lengths_out; return paged_cache_path_slots(*cache->cache, a, args->batch, args->nodes, (cudaStream_t)stream);)
+}
+
+int pjrtx_b200_prompt_attention(int device_ordinal, const PjrtxB200PromptAttentionArgs* args, void* stream) {
+  GUARD_INT(if (!have(args)) return 0; PromptAttention a; a.dtype = args->dtype; a.scale = args->scale; a.q = args->q; a.k = args->k;
+            a.v = args->v; a.out = args->out; a.lse = args->lse; a.tokens = args->tokens; a.q_stride = args->q_stride;
+            a.q_head_stride = args->q_head_stride; a.k_stride = args->k_stride; a.k_head_stride = args->k_head_stride;
+            a.v_stride = args->v_stride; a.v_head_stride = args->v_head_stride; a.out_stride = args->out_stride;
+            a.out_head_stride = args->out_head_stride; a.starts = args->starts;
+            return prompt_attention(device_ordinal, a, args->heads, args->kv_heads, args->head_dim, args->sequences, (cudaStream_t)stream);)
 }
 
 int pjrtx_b200_token_log_probs(int device_ordinal, const PjrtxB200TokenLogProbsArgs* args, void* stream) {

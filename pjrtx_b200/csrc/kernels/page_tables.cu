@@ -1,0 +1,242 @@
+// Page tables and slots of a paged key-value cache, built where the lengths are: on the device.
+//
+// assign: need = ceil(length / page_size). Surplus pages go onto the stack of free ones, ordered by (sequence, column); then the i-th page
+// wanted, in the same order, is the i-th from the top, for the sequences whose running sum of wants fits what is there. Both orders are
+// prefix sums over the batch, so the result does not depend on who is first.
+//
+// path: a drafted token is accepted when it lies on the way from the leaf to its root; its row is the number of those before it.
+//
+// All of it is a few hundred KB at most (a table of 512 x 256 pages and its copy: 1 MB), so what counts is the number of trips to memory
+// in a row: one launch of one cluster, whose blocks pass sums and pages to each other between cluster barriers.
+#include <cooperative_groups.h>
+
+#include "../common.h"
+#include "kernels.h"
+#include "paged.cuh"
+#include "tree.cuh"
+
+namespace pjrtx {
+
+namespace {
+
+constexpr int kBlocks = 8, kThreads = 512, kWarps = kThreads / 32;
+
+// What a sequence has and is to have, in pages. A length or count that the table cannot hold: `ok` is 0 and need is what it has.
+struct Want {
+  int held, need, ok;
+};
+
+__device__ __forceinline__ Want want_of(const PagedAssign& a, int b, bool stack_ok) {
+  const int held = a.held[b], length = a.lengths[b];
+  Want w;
+  const bool known = held >= 0 && held <= a.max_pages;
+  w.held = known ? held : 0;
+  const long long need = length < 0 ? -1 : ((long long)length + a.page_size - 1) / a.page_size;
+  w.ok = known && need >= 0 && need <= a.max_pages;
+  w.need = w.ok && stack_ok ? (int)need : w.held;
+  return w;
+}
+
+// Sum over the block's threads before this one, and of all; called by all threads.
+__device__ __forceinline__ long long block_prefix(long long x, long long* warp_sums, long long* total) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  long long sum = x;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const long long o = __shfl_up_sync(~0u, sum, d);
+    if (lane >= d) sum += o;
+  }
+  __syncthreads();  // the sums of the call before have been read
+  if (lane == 31) warp_sums[warp] = sum;
+  __syncthreads();
+  long long before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; w++) {
+    if (w < warp) before += warp_sums[w];
+    all += warp_sums[w];
+  }
+  *total = all;
+  return before + sum - x;
+}
+
+struct Sums {
+  long long give, take, granted;
+};
+
+// Sequences are divided among the blocks in chunks; a warp has a sequence at a time, its lanes the pages. `offsets`: shared memory of
+// two numbers a sequence of the chunk. Sums have 64 bits: lengths may ask for more pages than there are.
+__global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads) paged_assign_kernel(const __grid_constant__ PagedAssign a) {
+  PJRTX_PDL_PROLOGUE();
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  extern __shared__ longlong2 offsets[];
+  __shared__ Sums sums[kBlocks];  // of every block of the cluster
+  __shared__ long long warp_sums[kWarps];
+  const int rank = (int)cluster.block_rank(), lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int chunk = (a.batch + kBlocks - 1) / kBlocks, first = min(a.batch, rank * chunk), last = min(a.batch, first + chunk);
+  const int had = *a.free_count;
+  const bool stack_ok = had >= 0 && had <= a.num_pages;
+  const int free_count = stack_ok ? had : 0;
+  if (!stack_ok && rank == 0 && threadIdx.x == 0) report(a.error_words, kErrorLength);
+
+  // How many pages the sequences before have to give and want.
+  long long give = 0, take = 0;
+  for (int b0 = first; b0 < last; b0 += kThreads) {
+    const int b = b0 + threadIdx.x;
+    Want w = {0, 0, 1};
+    if (b < last) w = want_of(a, b, stack_ok);
+    if (!w.ok) report(a.error_words, kErrorLength);
+    long long given, taken;
+    const long long give_at = give + block_prefix(max(0, w.held - w.need), warp_sums, &given);
+    const long long take_at = take + block_prefix(max(0, w.need - w.held), warp_sums, &taken);
+    if (b < last) offsets[b - first] = make_longlong2(give_at, take_at);
+    give += given;
+    take += taken;
+  }
+  if (threadIdx.x < kBlocks) *cluster.map_shared_rank(&sums[rank], threadIdx.x) = Sums{give, take, 0};
+  cluster.sync();
+  long long give_before = 0, take_before = 0, returned = 0;
+#pragma unroll
+  for (int r = 0; r < kBlocks; r++) {
+    if (r < rank) {
+      give_before += sums[r].give;
+      take_before += sums[r].take;
+    }
+    returned += sums[r].give;
+  }
+  // More pages than the pool has come back only where a page was held twice; what does not fit the stack is dropped.
+  const int there = (int)min((long long)a.num_pages, free_count + returned);
+  if (free_count + returned > a.num_pages && rank == 0 && threadIdx.x == 0) report(a.error_words, kErrorLength);
+
+  // Surplus pages onto the stack, and how many pages this block's sequences get.
+  long long granted = 0;
+  for (int b = first + warp; b < last; b += kWarps) {
+    const Want w = want_of(a, b, stack_ok);
+    const longlong2 at = offsets[b - first];
+    for (int j = lane; j < w.held - w.need; j += 32) {
+      const long long place = free_count + give_before + at.x + j;
+      const int page = a.table[b * a.table_stride + w.need + j];
+      if (page < 0 || page >= a.num_pages) report(a.error_words, kErrorPageId);
+      if (place < a.num_pages) a.free_pages_out[place] = page;
+    }
+    const int wanted = w.need - w.held;
+    if (wanted > 0 && take_before + at.y + wanted <= there) granted += wanted;
+  }
+  __syncthreads();
+  if (lane == 0) warp_sums[warp] = granted;
+  __syncthreads();
+  granted = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; w++) granted += warp_sums[w];
+  if (threadIdx.x < kBlocks) cluster.map_shared_rank(&sums[rank], threadIdx.x)->granted = granted;
+  cluster.sync();  // the stack has what came back, too
+  int count = there;
+#pragma unroll
+  for (int r = 0; r < kBlocks; r++) count -= (int)sums[r].granted;
+  if (rank == 0 && threadIdx.x == 0) *a.free_count_out = stack_ok ? count : had;
+
+  // The new tables. A popped place of the stack is cleared by whoever popped it.
+  const bool copy_table = a.table != a.table_out, copy_stack = a.free_pages != a.free_pages_out;
+  for (int b = first + warp; b < last; b += kWarps) {
+    const Want w = want_of(a, b, stack_ok);
+    const longlong2 at = offsets[b - first];
+    const int wanted = w.need - w.held;
+    const bool served = wanted <= 0 || take_before + at.y + wanted <= there;
+    const int held = served ? w.need : w.held;
+    const int* from = a.table + b * a.table_stride;
+    int* to = a.table_out + b * a.table_out_stride;
+    const int c0 = copy_table ? 0 : min(w.held, held), c1 = copy_table ? a.max_pages : max(w.held, held);
+    for (int c = c0 + lane; c < c1; c += 32) {
+      int page;
+      if (c >= w.held && c < held) {
+        const int place = there - 1 - (int)(take_before + at.y + c - w.held);
+        page = place < free_count ? a.free_pages[place] : __ldcg(a.free_pages_out + place);
+        a.free_pages_out[place] = -1;
+        if (page < 0 || page >= a.num_pages) report(a.error_words, kErrorPageId);
+      } else {
+        page = c >= held && c < w.held ? -1 : from[c];
+      }
+      to[c] = page;
+    }
+    __syncwarp();  // in place: all lanes have read what the sequence had
+    if (lane == 0) a.held_out[b] = w.ok ? held : a.held[b];
+  }
+  if (copy_stack)
+    for (int i = rank * kThreads + threadIdx.x; i < a.num_pages; i += kBlocks * kThreads)
+      if (i < min(count, free_count) || i >= there) a.free_pages_out[i] = a.free_pages[i];
+  if (a.tokens == 0) return;
+
+  // Slots of the packed tokens: the sequence by bisection, the row from its end.
+  cluster.sync();
+  for (long long t = rank * kThreads + threadIdx.x; t < a.tokens; t += kBlocks * kThreads) {
+    int slot = -1;
+    if (a.batch > 0 && t >= a.starts[0] && t < a.starts[a.batch]) {
+      int lo = 0, hi = a.batch;  // starts[lo] <= t < starts[hi]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (a.starts[mid] <= t) lo = mid;
+        else hi = mid;
+      }
+      const int length = a.lengths[lo];
+      const long long row = length - (a.starts[lo + 1] - t);
+      const int held = __ldcg(a.held_out + lo);
+      if (row < 0 || length > (long long)a.page_size * a.max_pages) {
+        report(a.error_words, kErrorLength);
+      } else if ((long long)held * a.page_size >= length) {
+        const int column = (int)(row / a.page_size), page = __ldcg(a.table_out + lo * a.table_out_stride + column);
+        if (page >= 0 && page < a.num_pages) slot = page * a.page_size + (int)(row - (long long)column * a.page_size);
+        else report(a.error_words, kErrorPageId);
+      }
+    }
+    a.slots[t] = slot;
+  }
+}
+
+constexpr int kPathThreads = 128;
+
+// A warp a sequence, a lane two nodes.
+__global__ void __launch_bounds__(kPathThreads) paged_path_kernel(const PagedPath a) {
+  PJRTX_PDL_PROLOGUE();
+  const int b = (blockIdx.x * kPathThreads + threadIdx.x) / 32, lane = threadIdx.x % 32;
+  if (b >= a.batch) return;
+  const int length = a.lengths[b], leaf = a.leaves[b];
+  const Ancestors above = tree_ancestors(a.parents + (long long)b * a.nodes, a.nodes, a.error_words);
+  unsigned long long path = tree_of_node(above, max(0, min(leaf, kTreeNodesMax - 1)));
+  const int rows = __popcll(path);
+  if (leaf < 0) path = 0;
+  if (leaf >= a.nodes || length < 0 || (path && length + (long long)rows > (long long)a.page_size * a.max_pages)) {
+    if (lane == 0) report(a.error_words, kErrorLength);
+    path = 0;
+  }
+#pragma unroll
+  for (int u = 0; u < 2; u++) {
+    const int node = lane + u * 32;
+    if (node >= a.nodes) continue;
+    int slot = -1;
+    if (path >> node & 1) {
+      const int row = length + __popcll(path & ((1ull << node) - 1)), column = row / a.page_size;
+      const int page = a.table[b * a.table_stride + column];
+      const long long at = (long long)page * a.page_size + (row - column * a.page_size);
+      if (page >= 0 && at <= INT32_MAX) slot = (int)at;
+      else report(a.error_words, kErrorPageId);
+    }
+    a.slots[(long long)b * a.nodes + node] = slot;
+  }
+  if (lane == 0) a.lengths_out[b] = length + __popcll(path);
+}
+
+}  // namespace
+
+int paged_assign_launch(const PagedAssign& a, bool pdl, cudaStream_t stream) {
+  const size_t smem = (size_t)((a.batch + kBlocks - 1) / kBlocks) * sizeof(longlong2);
+  constexpr size_t kMost = (65535 + kBlocks - 1) / kBlocks * sizeof(longlong2);
+  if (!raise_smem_limit((const void*)paged_assign_kernel, (int)kMost)) return 0;
+  return launch_kernel(paged_assign_kernel, dim3(kBlocks), dim3(kThreads), smem, stream, pdl, a) == cudaSuccess;
+}
+
+int paged_path_launch(const PagedPath& a, bool pdl, cudaStream_t stream) {
+  constexpr int kPerBlock = kPathThreads / 32;
+  return launch_kernel(paged_path_kernel, dim3((unsigned)((a.batch + kPerBlock - 1) / kPerBlock)), dim3(kPathThreads), 0, stream, pdl, a) == cudaSuccess;
+}
+
+}  // namespace pjrtx

@@ -4,6 +4,8 @@
 // read once and written once, 16 bytes a thread, the threads of a warp on neighbouring pieces of one row. Bound by memory: 319 MB
 // in 52.7 us (floor 48.7); 4 prompts up to 2048 rows of 8 heads of 128 in bf16, 51 MB, in 11.2.
 //
+// store: packed rows go to the slots that are named for them. The same copying.
+//
 // evict: of the n > keep rows of a (sequence, KV head) those stay that come first by (protected, weight descending, row
 // ascending), a row being protected when its token is among the first `sinks` or the last `recent`. Attention does not depend
 // on the order of its rows, so nothing is compacted: the i-th kept row at or beyond `keep` moves into the i-th dropped place
@@ -63,6 +65,31 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(PagedView 
     const long long at = ((long long)b * c.kv_heads + g) * capacity + first + t;
     c.weights[at] = 0.f;
     c.positions[at] = token + t;
+  }
+}
+
+// ---- store ---------------------------------------------------------------------------------------------------------
+
+// The same for packed rows with a slot each: a thread a 16-byte piece of a key and of its value.
+__global__ void __launch_bounds__(kAppendThreads) paged_store_kernel(PagedView c, PagedStore a, int pieces, int esize) {
+  PJRTX_PDL_PROLOGUE();
+  const int per_row = c.kv_heads * pieces;
+  const long long total = a.rows * per_row, step = (long long)gridDim.x * kAppendThreads, rows = c.num_pages * c.page_size;
+  for (long long i = (long long)blockIdx.x * kAppendThreads + threadIdx.x; i < total; i += step) {
+    const int t = total >> 31 ? (int)(i / per_row) : (int)((unsigned)i / (unsigned)per_row), r = (int)(i - (long long)t * per_row);
+    const int g = r / pieces, piece = r - g * pieces, slot = a.slots[t];
+    if (slot < 0) continue;
+    if (slot >= rows) {
+      report(c.error_words, kErrorPageId);
+      continue;
+    }
+    const int page = slot / c.page_size;
+    const long long from = (t * a.row_stride + g * a.head_stride) * esize + piece * 16;
+    const long long to = (page * c.page_stride + (long long)(slot - page * c.page_size) * c.row_stride + g * c.head_stride) * esize + piece * 16;
+    const uint4 k = *reinterpret_cast<const uint4*>(static_cast<const char*>(a.k_new) + from);
+    const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const char*>(a.v_new) + from);
+    *reinterpret_cast<uint4*>(static_cast<char*>(c.k) + to) = k;
+    *reinterpret_cast<uint4*>(static_cast<char*>(c.v) + to) = v;
   }
 }
 
@@ -392,6 +419,13 @@ int paged_append_launch(const PagedView& c, const PagedAppend& a, int sm_count, 
   const long long blocks = std::min((work + kAppendThreads - 1) / kAppendThreads, (64ll * sm_count + c.batch - 1) / c.batch);
   return launch_kernel(paged_append_kernel, dim3((unsigned)blocks, (unsigned)c.batch), dim3(kAppendThreads), 0,
                        stream, pdl, c, a, pieces, esize) == cudaSuccess;
+}
+
+int paged_store_launch(const PagedView& c, const PagedStore& a, int sm_count, bool pdl, cudaStream_t stream) {
+  const int esize = (int)dtype_size(c.dtype), pieces = c.head_dim * esize / 16;
+  const long long work = a.rows * c.kv_heads * pieces;
+  const long long blocks = std::min<long long>((work + kAppendThreads - 1) / kAppendThreads, 64ll * sm_count);
+  return launch_kernel(paged_store_kernel, dim3((unsigned)blocks), dim3(kAppendThreads), 0, stream, pdl, c, a, pieces, esize) == cudaSuccess;
 }
 
 WorkspaceSize paged_evict_workspace(const PagedView& c) {

@@ -1,0 +1,135 @@
+// Causal attention of whole prompts, packed one behind the other, with grouped query heads. A tile of query rows is some positions of
+// one sequence times the query heads of a KV head: row x is head x % heads of position x / heads, so the rows of a tile share its keys.
+//
+// The starts of the sequences are on the device: the grid has a block for every tile that there can be, sequence b's from
+// starts[b] / positions + b on (a sequence of n tokens has at most that many before the next one's), and blocks without a tile leave. The
+// tiles of a sequence run from its end, where they have most to do, to its beginning.
+#include <algorithm>
+
+#include "../common.h"
+#include "kernels.h"
+#include "paged.cuh"
+#include "row_attention.cuh"
+
+namespace pjrtx {
+
+namespace {
+
+struct PromptArgs {
+  PromptAttention a;
+  int rep, heads, groups;  // query heads of a KV head; those of a tile; tiles that share a position
+  int positions;           // of a tile
+};
+
+struct PromptTile {
+  int start, tokens, tile;  // tile < 0: none
+};
+
+// Tile `x` of the launch, for all lanes of a warp. Sequences that are not in order are skipped.
+__device__ __forceinline__ PromptTile prompt_tile(const PromptArgs& p, int positions, long long x) {
+  const int lane = threadIdx.x % 32, *starts = p.a.starts;
+  int b = 0, n = p.a.sequences;
+  while (n > 1) {  // the last sequence whose first tile is not behind x
+    const int step = (n + 31) / 32, at = b + lane * step;
+    const bool before = lane * step < n && starts[at] / positions + (long long)at <= x;
+    const int seen = max(1, __popc(__ballot_sync(~0u, before)));
+    b += (seen - 1) * step;
+    n = min(step, n - (seen - 1) * step);
+  }
+  const int start = starts[b], end = starts[b + 1];
+  PromptTile t = {start, end - start, -1};
+  if (start < 0 || end < start || end > p.a.tokens) return t;
+  const long long at = x - (start / positions + (long long)b), tiles = (t.tokens + positions - 1) / positions;
+  if (at >= 0 && at < tiles) t.tile = (int)(tiles - 1 - at);
+  return t;
+}
+
+__device__ __forceinline__ void check_starts(const PromptAttention& a, long long thread, long long threads) {
+  for (long long b = thread; b < a.sequences; b += threads)
+    if (a.starts[b] < 0 || a.starts[b + 1] < a.starts[b] || a.starts[b + 1] > a.tokens) report(a.error_words, kErrorLength);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(rows::kThreads) prompt_rows_kernel(const __grid_constant__ PromptArgs p) {
+  PJRTX_PDL_PROLOGUE();
+  using namespace rows;
+  extern __shared__ __align__(16) char smem[];
+  Shared<D>& s = *reinterpret_cast<Shared<D>*>(smem);
+  const PromptAttention& a = p.a;
+  if (blockIdx.y == 0) check_starts(a, (long long)blockIdx.x * kThreads + threadIdx.x, (long long)gridDim.x * kThreads);
+  const PromptTile t = prompt_tile(p, p.positions, blockIdx.x);
+  if (t.tile < 0) return;
+  const int g = blockIdx.y / p.groups, h0 = blockIdx.y % p.groups * p.heads, heads = min(p.heads, p.rep - h0);
+  const int first = t.tile * p.positions, positions = min(p.positions, t.tokens - first);
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  auto place = [&](int r, int* position, int* head) {
+    *position = first + r / p.heads;
+    *head = r % p.heads;
+    return r / p.heads < positions && *head < heads;
+  };
+  load_rows<T, D>(s.q, a.head_dim, [&](int r) -> const T* {
+    int position, head;
+    if (!place(r, &position, &head)) return nullptr;
+    return static_cast<const T*>(a.q) + (long long)(t.start + position) * a.q_stride + (long long)(g * p.rep + h0 + head) * a.q_head_stride;
+  });
+  Sight sight[4];
+  Sums<D> sum;
+  sum.clear();
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    int position, head;
+    sight[i] = {place(ty * 4 + i, &position, &head) ? position + 1 : 0, 0ull};
+  }
+  const int keys = first + positions;
+  const T* k = static_cast<const T*>(a.k) + (long long)t.start * a.k_stride + (long long)g * a.k_head_stride;
+  const T* v = static_cast<const T*>(a.v) + (long long)t.start * a.v_stride + (long long)g * a.v_head_stride;
+  for (int key0 = 0; key0 < keys; key0 += kKeys)
+    block_of_keys<T, D>(s, sum, sight, key0, keys, keys, a.head_dim, a.scale * kLog2e, [&](int j) { return k + j * a.k_stride; },
+                        [&](int j) { return v + j * a.v_stride; });
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    int position, head;
+    if (!place(ty * 4 + i, &position, &head)) continue;
+    const long long row = t.start + position;
+    const int h = g * p.rep + h0 + head;
+    const float inverse = inverse_of(sum.l[i]);
+    T* out = static_cast<T*>(a.out) + row * a.out_stride + h * a.out_head_stride;
+#pragma unroll
+    for (int c = 0; c < D / 64; c++) {
+      const float2 x = pair_split(sum.o[i][c][0]), y = pair_split(sum.o[i][c][1]);
+      if (c * 64 + tx * 4 < a.head_dim) store4(out + c * 64 + tx * 4, make_float4(x.x * inverse, x.y * inverse, y.x * inverse, y.y * inverse));
+    }
+    if (a.lse && tx == 0) a.lse[row * a.heads + h] = lse_of(sum.m[i], sum.l[i]);
+  }
+}
+
+template <typename T, int D>
+int launch_rows(PromptArgs p, bool pdl, cudaStream_t stream) {
+  constexpr size_t smem = sizeof(rows::Shared<D>);
+  if (!raise_smem_limit((const void*)prompt_rows_kernel<T, D>, (int)smem)) return 0;
+  p.heads = std::min(p.rep, rows::kRows);
+  p.groups = (p.rep + p.heads - 1) / p.heads;
+  p.positions = rows::kRows / p.heads;
+  const dim3 grid((unsigned)(p.a.tokens / p.positions + p.a.sequences), (unsigned)(p.a.kv_heads * p.groups));
+  return launch_kernel(prompt_rows_kernel<T, D>, grid, dim3(rows::kThreads), smem, stream, pdl, p) == cudaSuccess;
+}
+
+template <typename T>
+int launch_rows_of(const PromptArgs& p, bool pdl, cudaStream_t stream) {
+  return p.a.head_dim <= 64    ? launch_rows<T, 64>(p, pdl, stream)
+         : p.a.head_dim <= 128 ? launch_rows<T, 128>(p, pdl, stream)
+                               : launch_rows<T, 256>(p, pdl, stream);
+}
+
+}  // namespace
+
+int prompt_attention_launch(const PromptAttention& a, int sm_count, bool pdl, cudaStream_t stream) {
+  PromptArgs p;
+  p.a = a;
+  p.rep = a.heads / a.kv_heads;
+  return a.dtype == kF32   ? launch_rows_of<float>(p, pdl, stream)
+         : a.dtype == kF16 ? launch_rows_of<__half>(p, pdl, stream)
+                           : launch_rows_of<__nv_bfloat16>(p, pdl, stream);
+}
+
+}  // namespace pjrtx

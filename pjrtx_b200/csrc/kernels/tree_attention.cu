@@ -1,0 +1,415 @@
+// Attention of a tree of drafted tokens per sequence over a paged cache: node i sees the cached rows, its ancestors and itself.
+//
+// Cached rows and nodes are one axis of keys, rows 0..length - 1 and behind them nodes 0..count - 1, cut into tiles; which source a key
+// comes from is known where it is fetched, and what a row sees are the keys below `length` and a word of bits from there on. A tile of
+// query rows is some nodes of a sequence times the query heads of a KV head: row x is head x % heads of node x / heads. So each cached row
+// is read once for all nodes and heads that share it, which is what the operator is for: one node at a time would read it once for each.
+#include <algorithm>
+
+#include "../common.h"
+#include "kernels.h"
+#include "paged.cuh"
+#include "row_attention.cuh"
+#include "tree.cuh"
+
+namespace pjrtx {
+
+namespace {
+
+// ---- division of the work ------------------------------------------------------------------------------------------
+// A segment is a (sequence, KV head, tile of query rows), a unit a tile of its keys. Segments have numbers for their units and, behind
+// them, for kSegmentCost more: what ending one and going on with the next takes. The numbers are cut into equal shares, one for each
+// block; lengths are device data, so each block adds them up itself. Where several blocks share a segment, each leaves (sums, max, total)
+// in its slot of the workspace, and a second kernel joins them in block order.
+
+constexpr int kSegmentCost = 2;
+constexpr int kJoinWarps = 8;
+
+// A segment that ends in another block than it begins in: written by the block it begins in, first >= last where there is none.
+struct Cut {
+  int b, group, first, last;
+};
+
+struct TreeArgs {
+  PagedView c;
+  PagedTree a;
+  int rep, heads, groups;  // query heads of a KV head; those of a tile; tiles that share a node
+  int nodes;               // of a tile
+  int tile_keys;
+  int slot_rows, dims;     // of a part's sums in the workspace: dims values a row, then (max, total) of every row
+  unsigned reciprocal;     // floor(2^32 / page_size), at most 2^32 - 1
+  Cut* cuts;               // [blocks]
+  float* parts;            // [blocks][2][slot_rows * (dims + 2)]
+};
+
+struct Sequence {
+  int length, count, tiles, segments;  // cached rows, nodes; units of a segment; segments
+};
+
+__device__ __forceinline__ Sequence sequence_of(const TreeArgs& p, int b) {
+  Sequence s;
+  const int count = p.a.counts ? p.a.counts[b] : p.a.nodes;
+  s.length = paged_length(p.c, b);
+  s.count = max(0, min(count, p.a.nodes));
+  s.tiles = s.count ? (s.length + s.count + p.tile_keys - 1) / p.tile_keys : 0;
+  s.segments = p.c.kv_heads * p.groups * ((s.count + p.nodes - 1) / p.nodes);
+  return s;
+}
+
+struct Cursor {
+  int b, group, tile;  // group: the segment's number in its sequence, ((tile of nodes) * KV heads + KV head) * groups + group of heads
+  Sequence s;
+};
+
+// What this block works on: the units among numbers [begin, begin + size), the first of them at `first` of these.
+struct Share {
+  long long begin, quota, size, first;  // first >= size: none
+  Cursor at;
+};
+
+__device__ __forceinline__ long long numbers_of(const Sequence& s) { return s.tiles ? (long long)s.segments * (s.tiles + kSegmentCost) : 0; }
+
+__device__ __forceinline__ void advance(const TreeArgs& p, Cursor& u) {
+  if (++u.tile < u.s.tiles) return;
+  u.tile = 0;
+  if (++u.group < u.s.segments) return;
+  u.group = 0;
+  do {
+    u.b++;
+    u.s = sequence_of(p, u.b);
+  } while (u.s.tiles == 0);
+}
+
+// The next unit of a share; false at its end.
+__device__ __forceinline__ bool next_unit(const TreeArgs& p, Cursor& u, long long& at, long long size) {
+  const long long to = at + (u.tile + 1 < u.s.tiles ? 1 : 1 + kSegmentCost);
+  if (to >= size) return false;
+  at = to;
+  advance(p, u);
+  return true;
+}
+
+template <int THREADS>
+struct ShareSpace {
+  long long sums[THREADS / 32], first;
+  Cursor at;
+};
+
+// Called by all threads.
+template <int THREADS>
+__device__ __forceinline__ Share share_of_block(const TreeArgs& p, ShareSpace<THREADS>& space) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int per_thread = (p.c.batch + THREADS - 1) / THREADS;
+  const int first = min(p.c.batch, (int)threadIdx.x * per_thread), last = min(p.c.batch, first + per_thread);
+  long long mine = 0;
+  for (int b = first; b < last; b++) mine += numbers_of(sequence_of(p, b));
+  long long sum = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const long long o = __shfl_up_sync(~0u, sum, d);
+    if (lane >= d) sum += o;
+  }
+  if (lane == 31) space.sums[warp] = sum;
+  __syncthreads();
+  long long before = sum - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; w++) {
+    if (w < warp) before += space.sums[w];
+    total += space.sums[w];
+  }
+  Share s;
+  s.quota = max(1ll, (total + gridDim.x - 1) / gridDim.x);
+  s.begin = min(total, blockIdx.x * s.quota);
+  s.size = min(total - s.begin, s.quota);
+  if (s.size > 0 && before <= s.begin && s.begin < before + mine) {
+    long long rest = s.begin - before;
+    Cursor u;
+    u.b = first;
+    for (;; u.b++) {
+      u.s = sequence_of(p, u.b);
+      if (rest < numbers_of(u.s)) break;
+      rest -= numbers_of(u.s);
+    }
+    u.group = (int)(rest / (u.s.tiles + kSegmentCost));
+    u.tile = (int)(rest % (u.s.tiles + kSegmentCost));
+    long long at = 0;
+    if (u.tile >= u.s.tiles) {  // behind a segment's units: the share begins with the next one
+      at = u.s.tiles + kSegmentCost - u.tile;
+      if (at < s.size) advance(p, u);
+    }
+    space.at = u;
+    space.first = at;
+  }
+  __syncthreads();
+  s.at = space.at;
+  s.first = s.size > 0 ? space.first : 0;
+  return s;
+}
+
+// What the query rows of a segment are.
+struct Segment {
+  int b, node0, nodes, g, h0, heads;  // nodes and heads of the tile
+  __device__ __forceinline__ bool place(const TreeArgs& p, int row, int* node, int* head) const {
+    *node = node0 + row / p.heads;
+    *head = row % p.heads;
+    return row / p.heads < nodes && *head < heads;
+  }
+};
+
+__device__ __forceinline__ Segment segment_of(const TreeArgs& p, int b, int group, int count) {
+  Segment s;
+  s.b = b;
+  const int across = p.c.kv_heads * p.groups, r = group % across;
+  s.node0 = group / across * p.nodes;
+  s.nodes = min(p.nodes, count - s.node0);
+  s.g = r / p.groups;
+  s.h0 = r % p.groups * p.heads;
+  s.heads = min(p.heads, p.rep - s.h0);
+  return s;
+}
+
+__device__ __forceinline__ long long query_at(const TreeArgs& p, const Segment& s, int node, int head) {
+  return s.b * p.a.q_batch_stride + node * p.a.q_node_stride + (long long)(s.g * p.rep + s.h0 + head) * p.a.q_head_stride;
+}
+__device__ __forceinline__ long long out_at(const TreeArgs& p, const Segment& s, int node, int head) {
+  return s.b * p.a.out_batch_stride + node * p.a.out_node_stride + (long long)(s.g * p.rep + s.h0 + head) * p.a.out_head_stride;
+}
+__device__ __forceinline__ long long lse_at(const TreeArgs& p, const Segment& s, int node, int head) {
+  return ((long long)s.b * p.a.nodes + node) * p.a.heads + s.g * p.rep + s.h0 + head;
+}
+
+// Element offset of cached row t of sequence b in either pool (KV head 0), -1 where the table names no page.
+__device__ __forceinline__ long long cached_row(const TreeArgs& p, int b, int t) {
+  int column = (int)__umulhi((unsigned)t, p.reciprocal);  // the quotient or one less
+  int row = t - column * p.c.page_size;
+  if (row >= p.c.page_size) {
+    column++;
+    row -= p.c.page_size;
+  }
+  const int page = p.c.table[b * p.c.table_stride + column];
+  if (page < 0 || page >= p.c.num_pages) {
+    report(p.c.error_words, kErrorPageId);
+    return -1;
+  }
+  return page * p.c.page_stride + row * p.c.row_stride;
+}
+
+__device__ __forceinline__ void check_sequences(const TreeArgs& p) {
+  for (int b = blockIdx.x * blockDim.x + threadIdx.x; b < p.c.batch; b += gridDim.x * blockDim.x) {
+    paged_check_length(p.c, b);
+    if (p.a.counts && (p.a.counts[b] < 0 || p.a.counts[b] > p.a.nodes)) report(p.c.error_words, kErrorLength);
+  }
+}
+
+// The slot of this block's part of a segment that other blocks share, and the cut that the join goes by; null where none does. Slot 1
+// of a block holds the segment that begins in it, slot 0 the one that began before.
+__device__ __forceinline__ float* part_of(const TreeArgs& p, const Share& share, const Cursor& u, long long segment) {
+  const long long first = segment / share.quota, last = (segment + u.s.tiles - 1) / share.quota;
+  if (first == last) return nullptr;
+  if (threadIdx.x == 0 && blockIdx.x == first) p.cuts[blockIdx.x] = {u.b, u.group, (int)first, (int)last};
+  return p.parts + ((long long)blockIdx.x * 2 + (blockIdx.x == first ? 1 : 0)) * p.slot_rows * (p.dims + 2);
+}
+
+// ---- on the CUDA cores ---------------------------------------------------------------------------------------------
+
+template <typename T, int D>
+__global__ void __launch_bounds__(rows::kThreads) tree_rows_kernel(const __grid_constant__ TreeArgs p) {
+  PJRTX_PDL_PROLOGUE();
+  using namespace rows;
+  extern __shared__ __align__(16) char smem[];
+  __shared__ ShareSpace<kThreads> space;
+  __shared__ unsigned long long ancestors[kTreeNodesMax];
+  __shared__ long long place_of[kKeys];  // of the keys of a block
+  Shared<D>& s = *reinterpret_cast<Shared<D>*>(smem);
+  if (threadIdx.x == 0) p.cuts[blockIdx.x] = {0, 0, 0, 0};
+  check_sequences(p);
+  const Share share = share_of_block(p, space);
+  if (share.first >= share.size) return;
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  Cursor now = share.at;
+  long long at = share.first;
+  for (bool more = true; more;) {
+    const Segment seg = segment_of(p, now.b, now.group, now.s.count);
+    const Cursor here = now;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      const Ancestors above = tree_ancestors(p.a.parents + (long long)seg.b * p.a.nodes, p.a.nodes, p.c.error_words);
+      ancestors[threadIdx.x] = above.low;
+      ancestors[threadIdx.x + 32] = above.high;
+    }
+    load_rows<T, D>(s.q, p.c.head_dim, [&](int r) -> const T* {
+      int node, head;
+      return seg.place(p, r, &node, &head) ? static_cast<const T*>(p.a.q) + query_at(p, seg, node, head) : nullptr;
+    });
+    __syncthreads();
+    Sight sight[4];
+    Sums<D> sum;
+    sum.clear();
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      int node, head;
+      sight[i] = {0, 0ull};
+      if (seg.place(p, ty * 4 + i, &node, &head)) sight[i] = {here.s.length, ancestors[node]};
+    }
+    const long long segment = share.begin + at - here.tile;  // number of its first unit
+    const int keys = here.s.length + here.s.count;
+    for (;;) {
+      const int key0 = now.tile * kKeys;
+      __syncthreads();
+      if (threadIdx.x < kKeys && key0 + threadIdx.x < here.s.length) {
+        const long long row = cached_row(p, seg.b, key0 + threadIdx.x);
+        place_of[threadIdx.x] = row < 0 ? -1 : row + seg.g * p.c.head_stride;
+      }
+      __syncthreads();
+      auto from = [&](const void* pool, const void* fresh, int t) -> const T* {
+        if (t < here.s.length) return place_of[t - key0] < 0 ? nullptr : static_cast<const T*>(pool) + place_of[t - key0];
+        return static_cast<const T*>(fresh) + seg.b * p.a.new_batch_stride + (t - here.s.length) * p.a.new_node_stride + seg.g * p.a.new_head_stride;
+      };
+      block_of_keys<T, D>(s, sum, sight, key0, keys, here.s.length, p.c.head_dim, p.a.scale * kLog2e,
+                          [&](int t) { return from(p.c.k, p.a.k_new, t); }, [&](int t) { return from(p.c.v, p.a.v_new, t); });
+      more = next_unit(p, now, at, share.size);
+      if (!more || now.group != here.group || now.b != here.b) break;
+    }
+    float* part = part_of(p, share, here, segment);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      int node, head;
+      const int row = ty * 4 + i;
+      if (!seg.place(p, row, &node, &head)) continue;
+      const float inverse = part ? 1.f : inverse_of(sum.l[i]);
+      T* out = static_cast<T*>(p.a.out) + out_at(p, seg, node, head);
+#pragma unroll
+      for (int c = 0; c < D / 64; c++) {
+        const float2 x = pair_split(sum.o[i][c][0]), y = pair_split(sum.o[i][c][1]);
+        const int d = c * 64 + tx * 4;
+        const float4 o = make_float4(x.x * inverse, x.y * inverse, y.x * inverse, y.y * inverse);
+        if (part) *reinterpret_cast<float4*>(part + row * D + d) = o;
+        else if (d < p.c.head_dim) store4(out + d, o);
+      }
+      if (tx) continue;
+      if (part) *reinterpret_cast<float2*>(part + p.slot_rows * D + 2 * row) = make_float2(sum.m[i], sum.l[i]);
+      else if (p.a.lse) p.a.lse[lse_at(p, seg, node, head)] = lse_of(sum.m[i], sum.l[i]);
+    }
+  }
+}
+
+// ---- parts of a segment ---------------------------------------------------------------------------------------------
+
+// A warp a row: the parts' (max, total) of every 32 by the lanes, then the values of each dimension over the parts, in block order.
+template <typename T>
+__global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const __grid_constant__ TreeArgs p) {
+  PJRTX_PDL_PROLOGUE();
+  using namespace rows;
+  const Cut cut = p.cuts[blockIdx.x];
+  if (cut.first >= cut.last) return;
+  const int lane = threadIdx.x % 32, row = blockIdx.y * kJoinWarps + threadIdx.x / 32;
+  const Segment seg = segment_of(p, cut.b, cut.group, sequence_of(p, cut.b).count);
+  int node, head;
+  if (!seg.place(p, row, &node, &head)) return;
+  const long long slot = (long long)p.slot_rows * (p.dims + 2);
+  auto part = [&](int i) { return p.parts + ((long long)(cut.first + i) * 2 + (i ? 0 : 1)) * slot; };
+  const int parts = cut.last - cut.first + 1;
+  float top = -INFINITY;
+  for (int i = lane; i < parts; i += 32) top = fmaxf(top, part(i)[p.slot_rows * p.dims + 2 * row]);
+#pragma unroll
+  for (int w = 16; w; w /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, w));
+  const float shift = top == -INFINITY ? 0.f : top;
+  float total = 0.f;
+  for (int d0 = 0; d0 < p.dims; d0 += 128) {
+    const int d = d0 + lane * 4;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    total = 0.f;
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+      float weight = 0.f, mass = 0.f;
+      if (i0 + lane < parts) {
+        const float2 stat = *reinterpret_cast<const float2*>(part(i0 + lane) + p.slot_rows * p.dims + 2 * row);
+        weight = stat.x == -INFINITY && stat.y == 0.f ? 0.f : stat.x == top ? 1.f : exp2_fast(stat.x - shift);
+        mass = stat.y;
+      }
+      const int n = min(32, parts - i0);
+#pragma unroll 8
+      for (int i = 0; i < n; i++) {
+        const float w = __shfl_sync(~0u, weight, i);
+        total = fmaf(w, __shfl_sync(~0u, mass, i), total);
+        if (d < p.dims && w != 0.f) {
+          const float4 y = *reinterpret_cast<const float4*>(part(i0 + i) + row * p.dims + d);
+          x.x = fmaf(w, y.x, x.x);
+          x.y = fmaf(w, y.y, x.y);
+          x.z = fmaf(w, y.z, x.z);
+          x.w = fmaf(w, y.w, x.w);
+        }
+      }
+    }
+    const float inverse = inverse_of(total);
+    if (d < p.c.head_dim)
+      store4(static_cast<T*>(p.a.out) + out_at(p, seg, node, head) + d, make_float4(x.x * inverse, x.y * inverse, x.z * inverse, x.w * inverse));
+  }
+  if (p.a.lse && lane == 0) p.a.lse[lse_at(p, seg, node, head)] = lse_of(top, total);
+}
+
+// ---- launches ------------------------------------------------------------------------------------------------------
+
+// Which kernel a shape runs on.
+struct TreePlan {
+  int dims = 0, rows = 0, keys = 0;  // of a row, of a tile of queries, of a tile of keys
+  size_t smem = 0;
+  const void* kernel = nullptr;
+};
+
+template <typename F>
+auto with_kernel(int dtype, int head_dim, F&& f) {
+#define PJRTX_TREE_ROWS(T, D) return f(tree_rows_kernel<T, D>, TreePlan{D, rows::kRows, rows::kKeys, sizeof(rows::Shared<D>)})
+#define PJRTX_TREE_ROWS_OF(T)                         \
+  if (head_dim <= 64) PJRTX_TREE_ROWS(T, 64);         \
+  if (head_dim <= 128) PJRTX_TREE_ROWS(T, 128);       \
+  PJRTX_TREE_ROWS(T, 256)
+  if (dtype == kF32) { PJRTX_TREE_ROWS_OF(float); }
+  if (dtype == kF16) { PJRTX_TREE_ROWS_OF(__half); }
+  PJRTX_TREE_ROWS_OF(__nv_bfloat16);
+#undef PJRTX_TREE_ROWS_OF
+#undef PJRTX_TREE_ROWS
+}
+
+uint64_t round256(uint64_t n) { return (n + 255) / 256 * 256; }
+
+}  // namespace
+
+uint64_t paged_tree_workspace(const PagedView& c, int heads, int nodes, int sm_count) {
+  return with_kernel(c.dtype, c.head_dim, [&](auto, const TreePlan& plan) {
+    return round256((uint64_t)sm_count * sizeof(Cut)) + (uint64_t)sm_count * 2 * plan.rows * (plan.dims + 2) * 4;
+  });
+}
+
+int paged_tree_launch(const PagedView& c, const PagedTree& a, int sm_count, bool pdl, cudaStream_t stream) {
+  TreeArgs p;
+  p.c = c;
+  p.a = a;
+  p.rep = a.heads / c.kv_heads;
+  p.reciprocal = (unsigned)std::min<uint64_t>((1ull << 32) / c.page_size, 0xffffffffu);
+  char* space = static_cast<char*>(a.workspace);
+  p.cuts = reinterpret_cast<Cut*>(space);
+  p.parts = reinterpret_cast<float*>(space + round256((uint64_t)sm_count * sizeof(Cut)));
+  long long blocks = 0;
+  const bool ok = with_kernel(c.dtype, c.head_dim, [&](auto kernel, const TreePlan& plan) {
+    p.heads = std::min(p.rep, plan.rows);
+    p.groups = (p.rep + p.heads - 1) / p.heads;
+    p.nodes = plan.rows / p.heads;
+    p.tile_keys = plan.keys;
+    p.slot_rows = plan.rows;
+    p.dims = plan.dims;
+    if (!raise_smem_limit((const void*)kernel, (int)plan.smem)) return false;
+    const long long numbers = (long long)c.batch * c.kv_heads * p.groups * ((a.nodes + p.nodes - 1) / p.nodes) *
+                              ((c.capacity() + a.nodes + p.tile_keys - 1) / p.tile_keys + kSegmentCost);
+    blocks = std::min<long long>(numbers, sm_count);
+    return launch_kernel(kernel, dim3((unsigned)blocks), dim3(rows::kThreads), plan.smem, stream, pdl, p) == cudaSuccess;
+  });
+  if (!ok) return 0;
+  auto join = c.dtype == kF32 ? tree_join_kernel<float> : c.dtype == kF16 ? tree_join_kernel<__half> : tree_join_kernel<__nv_bfloat16>;
+  const int rows = std::min(p.slot_rows, std::min(p.nodes, a.nodes) * p.heads);
+  return launch_kernel(join, dim3((unsigned)blocks, (unsigned)((rows + kJoinWarps - 1) / kJoinWarps)), dim3(kJoinWarps * 32), 0, stream, true, p) ==
+                 cudaSuccess
+             ? 2
+             : 0;
+}
+
+}  // namespace pjrtx

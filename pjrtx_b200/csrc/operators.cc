@@ -11,6 +11,7 @@ namespace {
 constexpr int64_t kMaxHeadDim = 256;
 constexpr int64_t kMaxCapacity = 1 << 30;  // rows of one sequence
 constexpr int64_t kMaxTracked = 1ll << 40;  // scores of a tracked cache's workspace: 4 TB; sizes beyond 2^60 would not fit 64 bits
+constexpr int64_t kMaxPacked = 1 << 24, kMaxSequences = 1 << 20;  // of packed prompts
 constexpr int64_t kMaxVocab = 1 << 22;     // the chunk maxima of a row stay in shared memory
 
 bool refuse(const char* fmt, long long a = 0, long long b = 0, long long c = 0) {
@@ -32,7 +33,7 @@ bool launched(int kernels, const char* what) {
 }
 
 // Completes a view with the cache's geometry and checks it.
-bool complete(const PagedCache& cache, PagedView* v) {
+bool complete(const PagedCache& cache, PagedView* v, bool sequences = true) {
   const PagedCacheConfig& c = cache.config;
   v->batch_max = (int)c.batch;
   v->kv_heads = (int)c.kv_heads;
@@ -43,13 +44,13 @@ bool complete(const PagedCache& cache, PagedView* v) {
   v->error_words = cache.device->operator_words_dev;
   if (v->batch < 0 || v->batch > c.batch) return refuse("paged cache: a batch of %lld, the cache was made for up to %lld", v->batch, c.batch);
   // Arrays of no sequences may have no address.
-  if (!v->k || !v->v || (v->batch > 0 && (!v->table || !v->lengths))) return refuse("paged cache: null pages, page table or lengths");
+  if (!v->k || !v->v || (sequences && v->batch > 0 && (!v->table || !v->lengths))) return refuse("paged cache: null pages, page table or lengths");
   if (v->num_pages < 1 || v->num_pages > INT32_MAX) return refuse("paged cache: %lld pages", v->num_pages);
   if (!aligned16(v->k) || !aligned16(v->v) || !stride_ok(v->page_stride, v->num_pages, c.dtype) ||
       !stride_ok(v->row_stride, c.page_size, c.dtype) || !stride_ok(v->head_stride, c.kv_heads, c.dtype))
     return refuse("paged cache: pages need 16-byte aligned rows (page, row and head strides %lld, %lld, %lld elements)", v->page_stride,
                   v->row_stride, v->head_stride);
-  if (v->batch > 1 && v->table_stride < c.max_pages)
+  if (sequences && v->batch > 1 && v->table_stride < c.max_pages)
     return refuse("paged cache: a page table of %lld columns, the cache has %lld pages a sequence", v->table_stride, c.max_pages);
   if ((v->weights != nullptr) != (v->positions != nullptr)) return refuse("paged cache: weights and positions go together");
   if (v->weights && !c.track) return refuse("paged cache: weights need a cache that was made to track them");
@@ -71,6 +72,8 @@ PagedCache* paged_cache_create(int ordinal, const PagedCacheConfig& c) {
   if (c.track && c.batch * c.heads * (c.page_size * c.max_pages) > kMaxTracked)
     return bad(refuse("paged cache: %lld sequences, %lld query heads and %lld rows are too many for a workspace of scores", c.batch, c.heads,
                       c.page_size * c.max_pages));
+  if (c.tree_nodes < 0 || c.tree_nodes > kTreeNodesMax)
+    return bad(refuse("paged cache: trees of %lld nodes (up to %lld)", c.tree_nodes, kTreeNodesMax));
   Device* dev = get_device_aside(ordinal);
   if (!dev) return nullptr;
   PagedCache made;
@@ -86,12 +89,15 @@ PagedCache* paged_cache_create(int ordinal, const PagedCacheConfig& c) {
   const WorkspaceSize attend = paged_attend_workspace(v, (int)c.heads, c.track, dev->sm_count);
   const WorkspaceSize evict = c.track ? paged_evict_workspace(v) : WorkspaceSize{0, 0};
   const uint64_t evict_at = (attend.bytes + 255) / 256 * 256;
-  made.bytes = evict_at + evict.bytes;
+  const uint64_t tree_at = (evict_at + evict.bytes + 255) / 256 * 256;
+  const uint64_t tree = c.tree_nodes ? paged_tree_workspace(v, (int)c.heads, (int)c.tree_nodes, dev->sm_count) : 0;
+  made.bytes = tree ? tree_at + tree : evict_at + evict.bytes;
   CurrentDevice scope(dev->ordinal);
   if (!entered(scope, dev)) return nullptr;
   made.attend_space = device_malloc(dev, made.bytes);
   if (!made.attend_space) return nullptr;
   made.evict_space = c.track ? static_cast<char*>(made.attend_space) + evict_at : nullptr;
+  made.tree_space = tree ? static_cast<char*>(made.attend_space) + tree_at : nullptr;
   // Other streams may use the workspaces once this returns.
   const bool ok = check_cuda(cudaMemsetAsync(made.attend_space, 0, attend.zeroed, dev->stream), "cudaMemsetAsync") &&
                   (!c.track || check_cuda(cudaMemsetAsync(made.evict_space, 0, evict.zeroed, dev->stream), "cudaMemsetAsync")) &&
@@ -157,6 +163,116 @@ int paged_cache_evict(const PagedCache& cache, PagedView view, PagedEvict e, cud
   CurrentDevice scope(cache.device->ordinal);
   if (!entered(scope, cache.device)) return 0;
   return launched(paged_evict_launch(view, e, cache.device->sm_count, true, stream), "evict");
+}
+
+int paged_cache_attend_tree(const PagedCache& cache, PagedView view, PagedTree a, cudaStream_t stream) {
+  if (!complete(cache, &view)) return 0;
+  const PagedCacheConfig& c = cache.config;
+  a.heads = (int)c.heads;
+  a.workspace = cache.tree_space;
+  if (a.nodes < 0 || a.nodes > c.tree_nodes) return refuse("attend to a tree: %lld nodes, the cache was made for up to %lld", a.nodes, c.tree_nodes);
+  if (view.batch == 0 || a.nodes == 0) return 1;
+  if (!std::isfinite(a.scale)) return refuse("attend to a tree: the scale is not finite");
+  if (!a.parents) return refuse("attend to a tree: null parents");
+  if (!a.q || !a.out || !aligned16(a.q) || !aligned16(a.out) || !stride_ok(a.q_batch_stride, view.batch, c.dtype) ||
+      !stride_ok(a.q_node_stride, a.nodes, c.dtype) || !stride_ok(a.q_head_stride, c.heads, c.dtype) ||
+      !stride_ok(a.out_batch_stride, view.batch, c.dtype) || !stride_ok(a.out_node_stride, a.nodes, c.dtype) ||
+      !stride_ok(a.out_head_stride, c.heads, c.dtype))
+    return refuse("attend to a tree: queries and results need 16-byte aligned pointers and strides");
+  if (!a.k_new || !a.v_new || !aligned16(a.k_new) || !aligned16(a.v_new) || !stride_ok(a.new_batch_stride, view.batch, c.dtype) ||
+      !stride_ok(a.new_node_stride, a.nodes, c.dtype) || !stride_ok(a.new_head_stride, c.kv_heads, c.dtype))
+    return refuse("attend to a tree: its keys and values need 16-byte aligned pointers and strides (%lld, %lld, %lld elements)", a.new_batch_stride,
+                  a.new_node_stride, a.new_head_stride);
+  CurrentDevice scope(cache.device->ordinal);
+  if (!entered(scope, cache.device)) return 0;
+  return launched(paged_tree_launch(view, a, cache.device->sm_count, true, stream), "attend to a tree");
+}
+
+int paged_cache_store(const PagedCache& cache, PagedView view, const PagedStore& a, cudaStream_t stream) {
+  view.batch = 0;
+  if (!complete(cache, &view, false)) return 0;
+  const PagedCacheConfig& c = cache.config;
+  if (a.rows < 0 || a.rows > INT32_MAX) return refuse("store: %lld rows", a.rows);
+  if (view.num_pages * c.page_size > INT32_MAX) return refuse("store: %lld pages of %lld rows, slots have 32 bits", view.num_pages, c.page_size);
+  if (a.rows == 0) return 1;
+  if (!a.slots) return refuse("store: null slots");
+  if (!a.k_new || !a.v_new || !aligned16(a.k_new) || !aligned16(a.v_new) || !stride_ok(a.row_stride, a.rows, c.dtype) ||
+      !stride_ok(a.head_stride, c.kv_heads, c.dtype))
+    return refuse("store: rows need 16-byte aligned pointers and strides (%lld, %lld elements)", a.row_stride, a.head_stride);
+  CurrentDevice scope(cache.device->ordinal);
+  if (!entered(scope, cache.device)) return 0;
+  return launched(paged_store_launch(view, a, cache.device->sm_count, true, stream), "store");
+}
+
+int paged_cache_assign(const PagedCache& cache, PagedAssign a, int64_t batch, int64_t num_pages, cudaStream_t stream) {
+  const PagedCacheConfig& c = cache.config;
+  if (batch < 0 || batch > c.batch) return refuse("assign pages: a batch of %lld, the cache was made for up to %lld", batch, c.batch);
+  if (num_pages < 1 || num_pages > INT32_MAX || num_pages * c.page_size > INT32_MAX)
+    return refuse("assign pages: %lld pages of %lld rows (up to 2^31 - 1 rows)", num_pages, c.page_size);
+  if (a.tokens < 0 || a.tokens > INT32_MAX) return refuse("assign pages: %lld tokens", a.tokens);
+  if (!a.free_pages || !a.free_count || !a.free_pages_out || !a.free_count_out) return refuse("assign pages: null stack of free pages");
+  if (batch > 0 && (!a.lengths || !a.held || !a.table || !a.held_out || !a.table_out)) return refuse("assign pages: null lengths, page counts or page table");
+  if (batch > 1 && (a.table_stride < c.max_pages || a.table_out_stride < c.max_pages))
+    return refuse("assign pages: a page table of %lld and %lld columns, the cache has %lld pages a sequence", a.table_stride, a.table_out_stride, c.max_pages);
+  if (a.table == a.table_out && a.table && batch > 1 && a.table_stride != a.table_out_stride)
+    return refuse("assign pages: in place, but the table's rows are %lld and %lld apart", a.table_stride, a.table_out_stride);
+  if (a.tokens > 0 && a.slots && !a.starts) return refuse("assign pages: slots need the starts of the sequences");
+  if (a.tokens > 0 && !a.slots) return refuse("assign pages: null slots");
+  a.batch = (int)batch;
+  a.num_pages = (int)num_pages;
+  a.page_size = (int)c.page_size;
+  a.max_pages = (int)c.max_pages;
+  a.error_words = cache.device->operator_words_dev;
+  CurrentDevice scope(cache.device->ordinal);
+  if (!entered(scope, cache.device)) return 0;
+  return launched(paged_assign_launch(a, true, stream), "assign pages");
+}
+
+int paged_cache_path_slots(const PagedCache& cache, PagedPath a, int64_t batch, int64_t nodes, cudaStream_t stream) {
+  const PagedCacheConfig& c = cache.config;
+  if (batch < 0 || batch > c.batch) return refuse("path slots: a batch of %lld, the cache was made for up to %lld", batch, c.batch);
+  if (nodes < 0 || nodes > kTreeNodesMax) return refuse("path slots: %lld nodes (up to %lld)", nodes, kTreeNodesMax);
+  if (batch == 0) return 1;
+  if (!a.table || !a.lengths || !a.leaves || !a.lengths_out || (nodes > 0 && (!a.parents || !a.slots)))
+    return refuse("path slots: null page table, lengths, parents, leaves or slots");
+  if (batch > 1 && a.table_stride < c.max_pages)
+    return refuse("path slots: a page table of %lld columns, the cache has %lld pages a sequence", a.table_stride, c.max_pages);
+  a.batch = (int)batch;
+  a.nodes = (int)nodes;
+  a.page_size = (int)c.page_size;
+  a.max_pages = (int)c.max_pages;
+  a.error_words = cache.device->operator_words_dev;
+  CurrentDevice scope(cache.device->ordinal);
+  if (!entered(scope, cache.device)) return 0;
+  return launched(paged_path_launch(a, true, stream), "path slots");
+}
+
+int prompt_attention(int ordinal, PromptAttention a, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t sequences, cudaStream_t stream) {
+  if (!dtype_is_float(a.dtype)) return refuse("prompt attention: element type %lld; f32, f16 and bf16 are supported", a.dtype);
+  if (kv_heads < 1 || kv_heads > 65535 || heads < kv_heads || heads > 65535 || heads % kv_heads)
+    return refuse("prompt attention: %lld query heads, %lld KV heads (up to 65535 each, query heads a multiple of KV heads)", heads, kv_heads);
+  if (head_dim < 1 || head_dim > kMaxHeadDim || head_dim * (int64_t)dtype_size(a.dtype) % 16)
+    return refuse("prompt attention: head dimension %lld (up to %lld, a multiple of 16 bytes)", head_dim, kMaxHeadDim);
+  if (a.tokens < 0 || a.tokens > kMaxPacked || sequences < 0 || sequences > kMaxSequences)
+    return refuse("prompt attention: %lld tokens of %lld sequences (up to 2^24 and 2^20)", a.tokens, sequences);
+  if (!std::isfinite(a.scale)) return refuse("prompt attention: the scale is not finite");
+  if (a.tokens == 0 || sequences == 0) return 1;
+  if (!a.starts) return refuse("prompt attention: null starts");
+  if (!a.q || !a.k || !a.v || !a.out || !aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) || !aligned16(a.out) ||
+      !stride_ok(a.q_stride, a.tokens, a.dtype) || !stride_ok(a.q_head_stride, heads, a.dtype) || !stride_ok(a.k_stride, a.tokens, a.dtype) ||
+      !stride_ok(a.k_head_stride, kv_heads, a.dtype) || !stride_ok(a.v_stride, a.tokens, a.dtype) || !stride_ok(a.v_head_stride, kv_heads, a.dtype) ||
+      !stride_ok(a.out_stride, a.tokens, a.dtype) || !stride_ok(a.out_head_stride, heads, a.dtype))
+    return refuse("prompt attention: queries, keys, values and results need 16-byte aligned pointers and strides");
+  a.heads = (int)heads;
+  a.kv_heads = (int)kv_heads;
+  a.head_dim = (int)head_dim;
+  a.sequences = (int)sequences;
+  Device* dev = get_device_aside(ordinal);
+  if (!dev) return 0;
+  a.error_words = dev->operator_words_dev;
+  CurrentDevice scope(dev->ordinal);
+  if (!entered(scope, dev)) return 0;
+  return launched(prompt_attention_launch(a, dev->sm_count, true, stream), "prompt attention");
 }
 
 namespace {

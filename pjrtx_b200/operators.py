@@ -1,7 +1,8 @@
-"""Operators on device memory: a paged key-value cache and the scoring of a decoder's logits.
+"""Operators on device memory: a paged key-value cache, attention of packed prompts and the scoring of a decoder's logits.
 
-Bindings of the `pjrtx_b200_paged_cache_*` and `pjrtx_b200_token_log_probs*` entry points of include/pjrtx_b200.h, reached
-through `Backend.paged_cache`, `Backend.token_log_probs` and `Backend.token_log_probs_backward`. Arrays are `DeviceBuffer`s
+Bindings of the `pjrtx_b200_paged_cache_*`, `pjrtx_b200_prompt_attention` and `pjrtx_b200_token_log_probs*` entry points of
+include/pjrtx_b200.h, reached through `Backend.paged_cache`, `Backend.prompt_attention`, `Backend.token_log_probs` and
+`Backend.token_log_probs_backward`. Arrays are `DeviceBuffer`s
 or any device tensors with `data_ptr()`, `shape`, `stride()` and `dtype` (torch's). Types, shapes and the device that an array
 says it is on (`get_device()` or `device`) are checked here, the rest behind the C ABI; nothing is copied, cast or kept. Calls
 enqueue on `stream`, a `cudaStream_t` as an integer (0: the default stream).
@@ -26,7 +27,7 @@ _P, _I32, _I64, _U64, _F32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ct
 
 class PagedCacheConfig(ctypes.Structure):
     _fields_ = [("struct_size", _U64), ("dtype", _I32), ("track", _I32), ("batch", _I64), ("heads", _I64), ("kv_heads", _I64),
-                ("head_dim", _I64), ("page_size", _I64), ("max_pages", _I64)]
+                ("head_dim", _I64), ("page_size", _I64), ("max_pages", _I64), ("tree_nodes", _I64)]
 
 
 class PagedView(ctypes.Structure):
@@ -51,6 +52,35 @@ class PagedEvictArgs(ctypes.Structure):
                 ("positions_out", _P)]
 
 
+class PagedTreeArgs(ctypes.Structure):
+    _fields_ = [("struct_size", _U64), ("q", _P), ("q_batch_stride", _I64), ("q_node_stride", _I64), ("q_head_stride", _I64), ("out", _P),
+                ("out_batch_stride", _I64), ("out_node_stride", _I64), ("out_head_stride", _I64), ("lse", _P), ("k_new", _P), ("v_new", _P),
+                ("new_batch_stride", _I64), ("new_node_stride", _I64), ("new_head_stride", _I64), ("parents", _P), ("counts", _P),
+                ("nodes", _I64), ("scale", _F32)]
+
+
+class PagedStoreArgs(ctypes.Structure):
+    _fields_ = [("struct_size", _U64), ("k_new", _P), ("v_new", _P), ("rows", _I64), ("row_stride", _I64), ("head_stride", _I64), ("slots", _P)]
+
+
+class PagedAssignArgs(ctypes.Structure):
+    _fields_ = [("struct_size", _U64), ("batch", _I64), ("lengths", _P), ("held", _P), ("page_table", _P), ("table_stride", _I64),
+                ("free_pages", _P), ("free_count", _P), ("num_pages", _I64), ("held_out", _P), ("page_table_out", _P),
+                ("table_out_stride", _I64), ("free_pages_out", _P), ("free_count_out", _P), ("starts", _P), ("slots", _P), ("tokens", _I64)]
+
+
+class PagedPathArgs(ctypes.Structure):
+    _fields_ = [("struct_size", _U64), ("batch", _I64), ("nodes", _I64), ("page_table", _P), ("table_stride", _I64), ("lengths", _P),
+                ("parents", _P), ("leaves", _P), ("slots", _P), ("lengths_out", _P)]
+
+
+class PromptAttentionArgs(ctypes.Structure):
+    _fields_ = [("struct_size", _U64), ("dtype", _I32), ("scale", _F32), ("q", _P), ("k", _P), ("v", _P), ("out", _P), ("lse", _P),
+                ("tokens", _I64), ("heads", _I64), ("kv_heads", _I64), ("head_dim", _I64), ("q_stride", _I64), ("q_head_stride", _I64),
+                ("k_stride", _I64), ("k_head_stride", _I64), ("v_stride", _I64), ("v_head_stride", _I64), ("out_stride", _I64),
+                ("out_head_stride", _I64), ("starts", _P), ("sequences", _I64)]
+
+
 class TokenLogProbsArgs(ctypes.Structure):
     _fields_ = [("struct_size", _U64), ("dtype", _I32), ("top", _I32), ("logits", _P), ("rows", _I64), ("vocab", _I64),
                 ("row_stride", _I64), ("tokens", _P), ("scale", _F32), ("log_probs", _P), ("entropy", _P), ("lse", _P),
@@ -73,6 +103,11 @@ SYMBOLS = {
     "pjrtx_b200_paged_cache_append": (ctypes.c_int, [_P, _P, _P, _P]),
     "pjrtx_b200_paged_cache_attend": (ctypes.c_int, [_P, _P, _P, _P]),
     "pjrtx_b200_paged_cache_evict": (ctypes.c_int, [_P, _P, _P, _P]),
+    "pjrtx_b200_paged_cache_attend_tree": (ctypes.c_int, [_P, _P, _P, _P]),
+    "pjrtx_b200_paged_cache_store": (ctypes.c_int, [_P, _P, _P, _P]),
+    "pjrtx_b200_paged_cache_assign": (ctypes.c_int, [_P, _P, _P]),
+    "pjrtx_b200_paged_cache_path_slots": (ctypes.c_int, [_P, _P, _P]),
+    "pjrtx_b200_prompt_attention": (ctypes.c_int, [ctypes.c_int, _P, _P]),
     "pjrtx_b200_token_log_probs": (ctypes.c_int, [ctypes.c_int, _P, _P]),
     "pjrtx_b200_token_log_probs_backward": (ctypes.c_int, [ctypes.c_int, _P, _P]),
     "pjrtx_b200_operators_status": (ctypes.c_int, [ctypes.c_int, _P]),
@@ -91,6 +126,8 @@ def _packer(cls):
 
 _pack_view, _pack_append, _pack_attend, _pack_evict, _pack_score, _pack_score_grad = map(
     _packer, (PagedView, PagedAppendArgs, PagedAttendArgs, PagedEvictArgs, TokenLogProbsArgs, TokenLogProbsBackwardArgs))
+_pack_tree, _pack_store, _pack_assign, _pack_path, _pack_prompt = map(
+    _packer, (PagedTreeArgs, PagedStoreArgs, PagedAssignArgs, PagedPathArgs, PromptAttentionArgs))
 
 _FLOATS = frozenset((P.F32, P.F16, P.BF16_CODE))
 _TENSOR_TYPES = {"float32": P.F32, "float16": P.F16, "bfloat16": P.BF16_CODE, "int32": P.S32}
@@ -230,18 +267,21 @@ class PagedCache:
     [batch, kv_heads, max_pages * page_size], and `tokens[b]` counts the tokens a sequence has seen. Calls go to `stream`, None: the
     backend's own, which is not ordered with any stream of a tensor library.
 
+    `tree` is how many drafted tokens of a sequence `attend_tree` can take, up to 64; it sizes a workspace.
+
     `destroy` waits for the device and frees the workspaces; those of a cache that is only dropped are freed by the next `destroy`,
     `Backend.paged_cache` or `Backend.synchronize`.
     """
 
     def __init__(self, backend, dtype: int, batch: int, heads: int, kv_heads: int, head_dim: int, page_size: int, max_pages: int,
-                 track: bool = False, device: int = 0):
+                 track: bool = False, device: int = 0, tree: int = 0):
         self._lib, self._err, self.device = backend.lib, backend._err, device
         self.dtype, self.batch, self.heads, self.kv_heads, self.head_dim = dtype, batch, heads, kv_heads, head_dim
         self.page_size, self.max_pages, self.track, self.capacity = page_size, max_pages, bool(track), page_size * max_pages
         self.handle = None
         free_unreferenced()
-        config = PagedCacheConfig(ctypes.sizeof(PagedCacheConfig), dtype, int(bool(track)), batch, heads, kv_heads, head_dim, page_size, max_pages)
+        config = PagedCacheConfig(ctypes.sizeof(PagedCacheConfig), dtype, int(bool(track)), batch, heads, kv_heads, head_dim, page_size,
+                                  max_pages, tree)
         self.handle = self._lib.pjrtx_b200_paged_cache_create(device, ctypes.byref(config))
         if not self.handle:
             raise _error(self._err())
@@ -286,6 +326,13 @@ class PagedCache:
         if not self.handle:
             raise _error("the paged cache was destroyed")
         if not fn(self.handle, view, args, self._stream if stream is None else stream):
+            raise _error(self._err())
+
+    def _hand(self, fn, args, stream) -> None:
+        """A call without a view."""
+        if not self.handle:
+            raise _error("the paged cache was destroyed")
+        if not fn(self.handle, args, self._stream if stream is None else stream):
             raise _error(self._err())
 
     def append(self, k_pages, v_pages, page_table, lengths, k_new, v_new, counts=None, tokens=None, weights=None, positions=None,
@@ -339,6 +386,83 @@ class PagedCache:
                             _dense(lse, "lse", P.F32, (batch, self.heads), self.device), k, v, new_strides[0], new_strides[1], scale)
         return self._call(fn, view, args, stream)
 
+    def attend_tree(self, q, k_pages, v_pages, page_table, lengths, out, k_new, v_new, parents, counts=None, lse=None,
+                    scale: Optional[float] = None, stream: Optional[int] = None) -> None:
+        """out [batch, nodes, heads, head_dim] = softmax(scale * q . k) v for a tree of drafted tokens per sequence: node i sees the
+        lengths[b] cached rows, its ancestors by parents [batch, nodes] (a node before i, -1: a root) and itself, whose keys and
+        values are k_new / v_new [batch, nodes, kv_heads, head_dim]. counts [batch]: nodes of each sequence (None: all), results
+        behind them stay. lse [batch, nodes, heads]: log-sum-exp. Stores nothing and tracks no weights; a chain is a further piece of
+        a prompt."""
+        batch, view = self._view(k_pages, v_pages, page_table, lengths, None, None, None)
+        dims = _dims(parents)
+        if len(dims) != 2 or dims[0] != batch:
+            raise _error(f"parents has shape {tuple(dims)}, ({batch}, nodes) is needed")
+        nodes = dims[1]
+        shape, new_shape = (batch, nodes, self.heads, self.head_dim), (batch, nodes, self.kv_heads, self.head_dim)
+        q_at, qs = _rows(q, "q", self.dtype, shape, self.device)
+        out_at, os = _rows(out, "out", self.dtype, shape, self.device)
+        k, ns = _rows(k_new, "k_new", self.dtype, new_shape, self.device)
+        v = _twin(v_new, "v_new", "k_new", self.dtype, new_shape, ns, self.device)
+        args = _pack_tree(q_at, qs[0], qs[1], qs[2], out_at, os[0], os[1], os[2], _dense(lse, "lse", P.F32, shape[:3], self.device), k, v, ns[0],
+                          ns[1], ns[2], _dense(parents, "parents", P.S32, dims, self.device), _dense(counts, "counts", P.S32, (batch,), self.device),
+                          nodes, self.head_dim ** -0.5 if scale is None else scale)
+        self._call(self._lib.pjrtx_b200_paged_cache_attend_tree, view, args, stream)
+
+    def store(self, k_pages, v_pages, k_new, v_new, slots, stream: Optional[int] = None) -> None:
+        """Stores rows k_new / v_new [rows, kv_heads, head_dim] at slots [rows] of the pools: a page times the page size plus a row in
+        it, negative: nowhere. A slot must not come twice."""
+        dims, shape = _dims(k_pages), _dims(k_new)
+        if len(dims) != 4 or dims[1:] != self._page_dims:
+            raise _error(f"k_pages has shape {tuple(dims)}, (pages, {', '.join(map(str, self._page_dims))}) is needed")
+        if len(shape) != 3 or shape[1:] != self._page_dims[1:]:
+            raise _error(f"k_new has shape {tuple(shape)}, (rows, {self.kv_heads}, {self.head_dim}) is needed")
+        k_at, strides = _rows(k_pages, "k_pages", self.dtype, dims, self.device)
+        v_at = _twin(v_pages, "v_pages", "k_pages", self.dtype, dims, strides, self.device)
+        k, ns = _rows(k_new, "k_new", self.dtype, shape, self.device)
+        v = _twin(v_new, "v_new", "k_new", self.dtype, shape, ns, self.device)
+        view = _pack_view(k_at, v_at, dims[0], strides[0], strides[1], strides[2], 0, 0, 0, 0, 0, 0, 0)
+        args = _pack_store(k, v, shape[0], ns[0], ns[1], _dense(slots, "slots", P.S32, shape[:1], self.device))
+        self._call(self._lib.pjrtx_b200_paged_cache_store, view, args, stream)
+
+    def assign_pages(self, lengths, held, page_table, free_pages, free_count, starts=None, slots=None, held_out=None, page_table_out=None,
+                     free_pages_out=None, free_count_out=None, stream: Optional[int] = None) -> None:
+        """Pages for lengths[b] rows of every sequence: those beyond them go back onto the stack of free_count[0] page ids in free_pages
+        [pages of the pool], what sequences lack comes from its top, in order; the first that wants more than is left, and those
+        behind it that want any, keep what they have. held [batch] counts pages. Results go to the `*_out` arrays, None: in place.
+        slots [tokens] gets the slots of packed new tokens, those of sequence b from starts[b] to starts[b + 1] being its last rows;
+        -1 where there is no page."""
+        shape = _dims(lengths)
+        if len(shape) != 1:
+            raise _error(f"lengths has shape {tuple(shape)}, (batch,) is needed")
+        pool, tokens = _dims(free_pages), () if slots is None else _dims(slots)
+        if len(pool) != 1 or len(tokens) > 1:
+            raise _error(f"{'free_pages' if len(pool) != 1 else 'slots'} has shape {tuple(pool if len(pool) != 1 else tokens)}, one axis is needed")
+        here, tables = self.device, shape + (self.max_pages,)
+        table, strides = _rows(page_table, "page_table", P.S32, tables, here)
+        table_out, out_strides = (table, strides) if page_table_out is None else _rows(page_table_out, "page_table_out", P.S32, tables, here)
+        args = _pack_assign(
+            shape[0], _dense(lengths, "lengths", P.S32, shape, here), _dense(held, "held", P.S32, shape, here), table, strides[0],
+            _dense(free_pages, "free_pages", P.S32, pool, here), _dense(free_count, "free_count", P.S32, (1,), here), pool[0],
+            _dense(held if held_out is None else held_out, "held_out", P.S32, shape, here), table_out, out_strides[0],
+            _dense(free_pages if free_pages_out is None else free_pages_out, "free_pages_out", P.S32, pool, here),
+            _dense(free_count if free_count_out is None else free_count_out, "free_count_out", P.S32, (1,), here),
+            _dense(starts, "starts", P.S32, (shape[0] + 1,), here), _dense(slots, "slots", P.S32, tokens, here), tokens[0] if tokens else 0)
+        self._hand(self._lib.pjrtx_b200_paged_cache_assign, args, stream)
+
+    def path_slots(self, page_table, lengths, parents, leaves, slots, lengths_out=None, stream: Optional[int] = None) -> None:
+        """slots [batch, nodes] of the nodes on the way from leaves[b] to its root, as rows lengths[b], lengths[b] + 1, ... of each
+        sequence; -1 for the others, and for all where the leaf is negative. lengths_out (None: in place) counts them."""
+        dims = _dims(parents)
+        if len(dims) != 2:
+            raise _error(f"parents has shape {tuple(dims)}, (batch, nodes) is needed")
+        here, batch = self.device, dims[:1]
+        table, strides = _rows(page_table, "page_table", P.S32, batch + (self.max_pages,), here)
+        args = _pack_path(batch[0], dims[1], table, strides[0], _dense(lengths, "lengths", P.S32, batch, here),
+                          _dense(parents, "parents", P.S32, dims, here), _dense(leaves, "leaves", P.S32, batch, here),
+                          _dense(slots, "slots", P.S32, dims, here),
+                          _dense(lengths if lengths_out is None else lengths_out, "lengths_out", P.S32, batch, here))
+        self._hand(self._lib.pjrtx_b200_paged_cache_path_slots, args, stream)
+
     def evict(self, k_pages, v_pages, page_table, lengths, tokens, weights, positions, keep: int, recent: int = 0, sinks: int = 0,
               lengths_out=None, weights_out=None, positions_out=None, stream: Optional[int] = None) -> None:
         """Cuts every sequence to `keep` rows by weight; tokens before `sinks` and the last `recent` ones stay. Results go to the
@@ -363,6 +487,30 @@ class PagedCache:
                 _unreferenced.append((self._lib, self.handle))
         except Exception:  # a half-made cache, or the interpreter's end
             pass
+
+
+def prompt_attention(backend, q, k, v, starts, out, lse=None, scale: Optional[float] = None, stream: Optional[int] = None,
+                     device: int = 0) -> None:
+    shape, new_shape, code = _dims(q), _dims(k), _code(q)
+    if code not in _FLOATS:
+        raise _error(f"q has element type {P.DTYPE_NAMES.get(code, 'other')}; f32, f16 and bf16 are supported")
+    if len(shape) != 3:
+        raise _error(f"q has shape {tuple(shape)}, (tokens, heads, head_dim) is needed")
+    if len(new_shape) != 3 or new_shape[0] != shape[0] or new_shape[2] != shape[2]:
+        raise _error(f"k has shape {tuple(new_shape)}, ({shape[0]}, KV heads, {shape[2]}) is needed")
+    ends = _dims(starts)
+    if len(ends) != 1 or ends[0] < 1:
+        raise _error(f"starts has shape {tuple(ends)}, (sequences + 1,) is needed")
+    q_at, qs = _rows(q, "q", code, shape, device)
+    k_at, ks = _rows(k, "k", code, new_shape, device)
+    v_at, vs = _rows(v, "v", code, new_shape, device)
+    out_at, os = _rows(out, "out", code, shape, device)
+    args = _pack_prompt(code, shape[2] ** -0.5 if scale is None else scale, q_at, k_at, v_at, out_at, _dense(lse, "lse", P.F32, shape[:2], device),
+                        shape[0], shape[1], new_shape[1], shape[2], qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1],
+                        _dense(starts, "starts", P.S32, ends, device), ends[0] - 1)
+    lib = backend.lib
+    if not lib.pjrtx_b200_prompt_attention(device, args, lib.pjrtx_b200_device_stream(device) if stream is None else stream):
+        raise _error(backend._err())
 
 
 def _logits(x, device: int):
