@@ -726,7 +726,7 @@ typedef struct PjrtxB200TokenLogProbsBackwardArgs {
 int pjrtx_b200_token_log_probs_backward(int device_ordinal, const PjrtxB200TokenLogProbsBackwardArgs *args, void *stream);
 
 /* Waits for `stream`; 1, or 0 with last_error naming what the operators' kernels on the device met since it was last asked
- * (all of codes 40 to 43 that are set). A bounded wait of an executable's kernel that gave up is not among it and stays
+ * (all of codes 40 to 44 that are set; 44 is a bounded wait of theirs that gave up). A bounded wait of an executable's kernel that gave up is not among it and stays
  * for pjrtx_b200_device_synchronize. Not during a stream capture. */
 int pjrtx_b200_operators_status(int device_ordinal, void *stream);
 

@@ -92,7 +92,8 @@ bool check_device_flag(Device* dev) {
 bool check_operator_words(Device* dev) {
   static const char* const kMet[kErrorWords] = {"a page table entry outside the pool of pages",
                                                 "a length outside the page table or a count beyond its length",
-                                                "a token id outside the vocabulary", "a parent that does not come before its node"};
+                                                "a token id outside the vocabulary", "a parent that does not come before its node",
+                                                "a bounded wait that gave up"};
   std::string met;
   for (int i = 0; i < kErrorWords; i++) {
     volatile int* word = dev->operator_words_host + i;

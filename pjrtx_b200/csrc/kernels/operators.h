@@ -10,12 +10,13 @@
 
 namespace pjrtx {
 
-// Codes for arguments which only the device can see. Kernels set error_words[code - kErrorPageId], host-mapped memory of the device.
+// Codes for arguments which only the device can see, and for what went wrong there. Kernels set error_words[code - kErrorPageId], host-mapped memory of the device.
 constexpr int kErrorPageId = 40;   // a page table entry of a sequence's own rows names no page of the pool
 constexpr int kErrorLength = 41;   // a length is negative or beyond the page table, or a count does not fit its length
 constexpr int kErrorToken = 42;    // a token id is not below the vocabulary size
 constexpr int kErrorParent = 43;   // a node's parent is neither -1 nor a node before it
-constexpr int kErrorWords = 4;
+constexpr int kErrorWait = 44;     // a bounded wait gave up
+constexpr int kErrorWords = 5;
 
 // Row t of sequence b: page table[b * table_stride + t / page_size], row t % page_size of it; element d of KV head g of that row
 // is at page * page_stride + row * row_stride + g * head_stride + d in both pools. Strides count elements.

@@ -4,7 +4,10 @@
 // The starts of the sequences are on the device: the grid has a block for every tile that there can be, sequence b's from
 // starts[b] / positions + b on (a sequence of n tokens has at most that many before the next one's), and blocks without a tile leave. The
 // tiles of a sequence run from its end, where they have most to do, to its beginning.
+//
+// 16-bit types go to the tensor cores (umma_prompt.cuh), f32 to the CUDA cores (row_attention.cuh).
 #include <algorithm>
+#include <type_traits>
 
 #include "../common.h"
 #include "kernels.h"
@@ -48,6 +51,14 @@ __device__ __forceinline__ void check_starts(const PromptAttention& a, long long
   for (long long b = thread; b < a.sequences; b += threads)
     if (a.starts[b] < 0 || a.starts[b + 1] < a.starts[b] || a.starts[b + 1] > a.tokens) report(a.error_words, kErrorLength);
 }
+
+}  // namespace
+}  // namespace pjrtx
+
+#include "umma_prompt.cuh"
+
+namespace pjrtx {
+namespace {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(rows::kThreads) prompt_rows_kernel(const __grid_constant__ PromptArgs p) {
@@ -121,12 +132,79 @@ int launch_rows_of(const PromptArgs& p, bool pdl, cudaStream_t stream) {
                                : launch_rows<T, 256>(p, pdl, stream);
 }
 
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// A map of `rank` axes, head_dim first, for boxes of 64 elements; `strides` (elements) are those of the axes behind the first. An axis of
+// one element may come with any stride, which the encoder does not take.
+bool encode_map(CUtensorMap* map, const void* base, bool f16, int rank, const long long* extents, const long long* strides, const int* box) {
+  static const EncodeTiledFn encode = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess) f = nullptr;
+    return (EncodeTiledFn)f;
+  }();
+  if (!encode) return false;
+  cuuint64_t dims[4], bytes[3];
+  cuuint32_t boxes[4], steps[4];
+  for (int d = 0; d < rank; d++) {
+    dims[d] = (cuuint64_t)extents[d];
+    boxes[d] = (cuuint32_t)box[d];
+    steps[d] = 1;
+    if (d) bytes[d - 1] = (cuuint64_t)(extents[d] == 1 ? extents[0] : strides[d - 1]) * 2;
+  }
+  return encode(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), dims, bytes,
+                boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool BF16, int HD, int TILES>
+int launch_umma(const umma::PromptKernelArgs& a, bool pdl, cudaStream_t stream) {
+  const PromptAttention& p = a.p.a;
+  const long long q_extents[4] = {p.head_dim, a.p.rep, p.kv_heads, p.tokens}, k_extents[3] = {p.head_dim, p.tokens, p.kv_heads};
+  const long long q_strides[3] = {p.q_head_stride, a.p.rep * p.q_head_stride, p.q_stride};
+  const long long k_strides[2] = {p.k_stride, p.k_head_stride}, v_strides[2] = {p.v_stride, p.v_head_stride};
+  const int q_box[4] = {64, a.p.heads, 1, a.p.positions}, k_box[3] = {64, umma::prompt_keys(HD), 1};
+  CUtensorMap qmap, kmap, vmap;
+  if (!encode_map(&qmap, p.q, !BF16, 4, q_extents, q_strides, q_box) || !encode_map(&kmap, p.k, !BF16, 3, k_extents, k_strides, k_box) ||
+      !encode_map(&vmap, p.v, !BF16, 3, k_extents, v_strides, k_box))
+    return -1;
+  constexpr size_t smem = umma::prompt_smem(HD, TILES);
+  auto kernel = umma::umma_prompt_kernel<BF16, HD, TILES>;
+  if (!raise_smem_limit((const void*)kernel, (int)smem)) return 0;
+  const dim3 grid((unsigned)(p.tokens / (TILES * a.p.positions) + p.sequences), (unsigned)(p.kv_heads * a.p.groups));
+  return launch_kernel(kernel, grid, dim3(umma::prompt_threads(TILES)), smem, stream, pdl, a, qmap, kmap, vmap) == cudaSuccess;
+}
+
+// 1, 0 where the launch failed, -1 where a layout has no tensor map.
+template <bool BF16>
+int launch_umma_of(PromptArgs p, int sm_count, bool pdl, cudaStream_t stream) {
+  umma::PromptKernelArgs a;
+  p.heads = std::min(p.rep, umma::kAttnRows);
+  p.groups = (p.rep + p.heads - 1) / p.heads;
+  p.positions = umma::kAttnRows / p.heads;
+  a.p = p;
+  const float scale = p.a.scale;
+  a.scale_log2 = scale == 0.f ? 1.f : (scale < 0.f ? -scale : scale) * rows::kLog2e;
+  a.sign = scale > 0.f ? 1.f : scale < 0.f ? -1.f : 0.f;
+  a.timeout_ns = wait_timeout_ns();
+  const long long pairs = p.a.tokens / (2 * p.positions) * p.a.kv_heads * p.groups;
+  const bool two = pairs >= sm_count && p.a.tokens / p.a.sequences > p.positions;
+  if (p.a.head_dim > 128) return launch_umma<BF16, 256, 1>(a, pdl, stream);
+  if (p.a.head_dim > 64) return two ? launch_umma<BF16, 128, 2>(a, pdl, stream) : launch_umma<BF16, 128, 1>(a, pdl, stream);
+  return two ? launch_umma<BF16, 64, 2>(a, pdl, stream) : launch_umma<BF16, 64, 1>(a, pdl, stream);
+}
+
 }  // namespace
 
 int prompt_attention_launch(const PromptAttention& a, int sm_count, bool pdl, cudaStream_t stream) {
   PromptArgs p;
   p.a = a;
   p.rep = a.heads / a.kv_heads;
+  if (a.dtype != kF32) {
+    const int launched = a.dtype == kF16 ? launch_umma_of<false>(p, sm_count, pdl, stream) : launch_umma_of<true>(p, sm_count, pdl, stream);
+    if (launched >= 0) return launched;
+  }
   return a.dtype == kF32   ? launch_rows_of<float>(p, pdl, stream)
          : a.dtype == kF16 ? launch_rows_of<__half>(p, pdl, stream)
                            : launch_rows_of<__nv_bfloat16>(p, pdl, stream);

@@ -1,0 +1,439 @@
+// Causal attention of packed prompts on the 5th-generation tensor cores: scores, probabilities and results of a tile of 128 query rows
+// stay in tensor memory while its keys pass by in blocks (the formulas and the tiles are those of prompt_attention.cu).
+//
+// Roles of a block of threads, which has TILES tiles of neighbouring positions:
+//   copy warp      the queries once, then keys and values into a ring of shared-memory slots (tiled tensor-map copies, 128-byte swizzle)
+//   MMA warp       S_t = Q_t . K^T and O_t += P_t . V with P_t in tensor memory, for the tiles in turn: while the softmax warps of one
+//                  tile work, the tensor core has the other's products
+//   softmax warps  four a tile, a query row a thread (its lane of tensor memory), so a row's maximum and sum need no exchange
+//
+// Probabilities go to the tensor core in the element type, and the sum is taken of them as they are then, so that equal values under all
+// keys give that value. In f16 they are multiplied by 2^11 first: f16 then holds them down to 2^-35 of the largest, and not only to 2^-24.
+// They are relative to a maximum that follows the row's when that has grown by 2^8 (f16: 2^4, so that they stay below 2^16): the factor
+// cancels in the division, and the results in tensor memory are rescaled that much more rarely.
+//
+// Hidden keys have probability 0, but the tensor core multiplies it by their values, and 0 times infinity or NaN is NaN. So values
+// behind the last position of the block of threads are cleared in shared memory, and a row with a result that is not finite looks at
+// the values between its position and there; only where one is infinite or NaN it is computed once more, by its warp and without them.
+#pragma once
+
+#include "umma_attention.cuh"
+
+namespace pjrtx {
+namespace umma {
+
+struct PromptKernelArgs {
+  PromptArgs p;       // `heads` and `positions` of one tile of 128 rows
+  float scale_log2;   // |scale| * log2(e) (1 where scale is zero)
+  float sign;         // 1, -1 or 0: what scores are multiplied by first, so that the largest score has the largest exponent
+  unsigned long long timeout_ns;
+};
+
+template <bool BF16> struct Probability { static constexpr float kLift = 0.f, kGrow = 8.f; };
+template <> struct Probability<false> { static constexpr float kLift = 11.f, kGrow = 4.f; };
+
+__host__ __device__ constexpr int prompt_keys(int hd) { return hd == 256 ? 64 : 128; }  // of a block
+constexpr int kPromptSlots = 5;
+__host__ __device__ constexpr int prompt_threads(int tiles) { return tiles == 2 ? 384 : 192; }
+__host__ __device__ constexpr int prompt_per_sm(int hd, int tiles) { return hd == 64 && tiles == 1 ? 2 : 1; }
+__host__ __device__ constexpr uint32_t prompt_tmem(int hd, int tiles) { return tiles == 2 || hd == 256 ? 512 : 256; }
+__host__ __device__ constexpr size_t prompt_smem(int hd, int tiles) {
+  const size_t bytes = (size_t)tiles * kAttnRows * hd * 2 + (size_t)kPromptSlots * prompt_keys(hd) * hd * 2 + 512 + 1024;
+  const size_t least = least_smem(prompt_per_sm(hd, tiles) == 2 ? 256 : 512);
+  return bytes < least ? least : bytes;
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_dst),
+               "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+template <int REGISTERS>
+__device__ __forceinline__ void take_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGISTERS));
+}
+template <int REGISTERS>
+__device__ __forceinline__ void leave_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGISTERS));
+}
+// Whether one of two packed 16-bit elements is infinite or NaN.
+template <bool BF16>
+__device__ __forceinline__ bool odd_pair(uint32_t w) {
+  constexpr uint32_t kExponent = BF16 ? 0x7f80u : 0x7c00u;
+  return (w & kExponent) == kExponent || (w >> 16 & kExponent) == kExponent;
+}
+
+// Row `pos` once more, over the keys that it sees; called by a whole warp, `m` and `total` being the row's.
+template <bool BF16, int HD>
+__device__ __noinline__ void redo_row(const PromptKernelArgs& a, const unsigned short* q, const unsigned short* k, const unsigned short* v,
+                                      unsigned short* out, int pos, float m, float total) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  const PromptAttention& p = a.p.a;
+  const int lane = threadIdx.x % 32;
+  float o[HD / 32];
+#pragma unroll
+  for (int e = 0; e < HD / 32; e++) o[e] = 0.f;
+  const float shift = m == -INFINITY ? 0.f : Probability<BF16>::kLift - m;
+  for (int key0 = 0; key0 <= pos; key0 += 32) {
+    float s = 0.f;
+    if (key0 + lane <= pos) {
+      const unsigned short* row = k + (key0 + lane) * p.k_stride;
+      for (int d = 0; d < p.head_dim; d += 8) {
+        float x[8], y[8];
+        rows::unpack16<T>(*reinterpret_cast<const uint4*>(row + d), x);
+        rows::unpack16<T>(*reinterpret_cast<const uint4*>(q + d), y);
+#pragma unroll
+        for (int e = 0; e < 8; e++) s = fmaf(x[e], y[e], s);
+      }
+      s = exp2_approx(fmaf(s * a.sign, a.scale_log2, shift));
+    }
+    for (int i = 0; i < 32 && key0 + i <= pos; i++) {
+      const float w = __shfl_sync(0xffffffffu, s, i);
+      const unsigned short* row = v + (key0 + i) * p.v_stride;
+#pragma unroll
+      for (int e = 0; e < HD / 32; e++)
+        if (e * 32 + lane < p.head_dim) o[e] = fmaf(w, (float)reinterpret_cast<const T*>(row)[e * 32 + lane], o[e]);
+    }
+  }
+  const float inverse = rows::inverse_of(total);
+#pragma unroll
+  for (int e = 0; e < HD / 32; e++)
+    if (e * 32 + lane < p.head_dim) reinterpret_cast<T*>(out)[e * 32 + lane] = rows::from_float<T>(o[e] * inverse);
+}
+
+template <bool BF16, int HD, int TILES>
+__global__ void __launch_bounds__(prompt_threads(TILES), prompt_per_sm(HD, TILES))
+umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                   const __grid_constant__ CUtensorMap vmap) {
+  constexpr int kKeys = prompt_keys(HD), kHalves = HD / 64, kSlots = kPromptSlots;
+  constexpr uint32_t kTileBytes = kAttnRows * HD * 2, kSlotBytes = kKeys * HD * 2;
+  constexpr uint32_t kQueryBlock = kAttnRows * 128, kKeyBlock = kKeys * 128;  // bytes of 64 elements of all rows
+  constexpr uint32_t kTmemCols = prompt_tmem(HD, TILES);
+  static_assert(TILES * (kKeys + HD) <= kTmemCols, "");
+  extern __shared__ unsigned char smem_dyn[];
+  const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
+  unsigned char* base_ptr = smem_dyn + (base - smem_u32(smem_dyn));
+  const uint32_t ring = base + TILES * kTileBytes;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(base_ptr + TILES * kTileBytes + kSlots * kSlotBytes);
+  uint64_t* slot_full = q_full + 1;             // [kSlots]
+  uint64_t* slot_empty = slot_full + kSlots;    // [kSlots]
+  uint64_t* v_clean = slot_empty + kSlots;      // values behind the last position have been cleared
+  uint64_t* s_full = v_clean + 1;               // [TILES] scores of the next block are in tensor memory
+  uint64_t* p_ready = s_full + TILES;           // [TILES] probabilities are in tensor memory, O may be accumulated
+  uint64_t* o_full = p_ready + TILES;           // [TILES] the last product has completed
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + TILES);
+  int* flags = reinterpret_cast<int*>(tmem_slot + 1);  // [0] abort
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kMmaWarp = 4 * TILES, kCopyWarp = 4 * TILES + 1;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const PromptAttention& p = a.p.a;
+  if (blockIdx.y == 0) check_starts(p, (long long)blockIdx.x * blockDim.x + threadIdx.x, (long long)gridDim.x * blockDim.x);
+  const PromptTile item = prompt_tile(a.p, TILES * a.p.positions, blockIdx.x);
+  if (item.tile < 0) return;
+  const WaitBudget budget{global_timer_ns() + a.timeout_ns, flags};
+  const int g = blockIdx.y / a.p.groups, h0 = blockIdx.y % a.p.groups * a.p.heads, heads = min(a.p.heads, a.p.rep - h0);
+  const int first = item.tile * TILES * a.p.positions;
+  const int keys = min(first + TILES * a.p.positions, item.tokens);  // behind the last position of the block
+  // Of a tile: its positions, and the blocks of keys up to the last of them (0: there is no such tile).
+  auto first_of = [&](int t) { return first + t * a.p.positions; };
+  auto blocks_of = [&](int t) { return first_of(t) >= keys ? 0 : (min(first_of(t) + a.p.positions, keys) + kKeys - 1) / kKeys; };
+  const int blocks = (keys + kKeys - 1) / kKeys;
+  const bool ragged = keys % kKeys != 0;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int s = 0; s < kSlots; s++) {
+      mbar_init(&slot_full[s], 1);
+      mbar_init(&slot_empty[s], 1);
+    }
+    mbar_init(v_clean, 1);
+    for (int t = 0; t < TILES; t++) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_ready[t], 4);
+      mbar_init(&o_full[t], 1);
+    }
+    flags[0] = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const uint32_t tmem_base = *tmem_slot;
+  auto s_col = [&](int t) { return tmem_base + (uint32_t)(t * kKeys); };
+  auto o_col = [&](int t) { return tmem_base + (uint32_t)(TILES * kKeys + t * HD); };
+
+  if (warp >= 4 * TILES) {
+    if constexpr (TILES == 2) leave_registers<72>();
+    const bool leader = elect_one();
+    if (warp == kCopyWarp) {
+      // K0 V0 K1 V1 ...
+      if (leader) {
+        mbar_expect_tx(q_full, (blocks_of(TILES - 1) ? TILES : 1) * kHalves * (uint32_t)(a.p.heads * a.p.positions) * 128u);
+        for (int t = 0; t < TILES; t++)
+          if (blocks_of(t))
+            for (int c = 0; c < kHalves; c++)
+              tma_load_4d(base + t * kTileBytes + c * kQueryBlock, &qmap, c * 64, h0, g, item.start + first_of(t), q_full);
+      }
+      __syncwarp();
+      int slot = 0;
+      unsigned phase = 0;
+      bool ok = true;
+      for (int i = 0; i < 2 * blocks; i++) {
+        if (i >= kSlots && !__all_sync(0xffffffffu, mbar_wait(&slot_empty[slot], phase ^ 1, budget))) {
+          // The copies in flight get a bounded time to land before the block of threads leaves.
+          for (int r = 1; r <= kSlots && leader; r++) {
+            const int j = i - r;
+            for (unsigned spin = 0; spin < (1u << 16) && !mbar_try_wait(&slot_full[j % kSlots], (unsigned)(j / kSlots) & 1u); spin++) {
+            }
+          }
+          ok = false;
+          break;
+        }
+        if (leader) {
+          const CUtensorMap* map = (i & 1) ? &vmap : &kmap;
+          const uint32_t dst = ring + (uint32_t)slot * kSlotBytes;
+          mbar_expect_tx(&slot_full[slot], kSlotBytes);
+          for (int c = 0; c < kHalves; c++) tma_load_3d(dst + c * kKeyBlock, map, c * 64, item.start + (i >> 1) * kKeys, g, &slot_full[slot]);
+        }
+        __syncwarp();
+        if (++slot == kSlots) {
+          slot = 0;
+          phase ^= 1;
+        }
+      }
+      if (ok && ragged) {
+        const int last = 2 * blocks - 1;
+        if (__all_sync(0xffffffffu, mbar_wait(&slot_full[last % kSlots], (unsigned)(last / kSlots) & 1u, budget))) {
+          unsigned char* rows0 = base_ptr + TILES * kTileBytes + (last % kSlots) * kSlotBytes;
+          const int from = keys % kKeys * 8;  // pieces of 16 bytes
+          for (int c = 0; c < kHalves; c++)
+            for (int i = from + lane; i < kKeys * 8; i += 32) *reinterpret_cast<uint4*>(rows0 + c * kKeyBlock + i * 16) = make_uint4(0, 0, 0, 0);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(v_clean);
+        }
+      }
+      __syncwarp();
+    } else if (warp == kMmaWarp) {
+      // N = keys with K as a K-major B operand; N = HD with V as an MN-major one (bit 16).
+      const uint32_t idesc_s = instr_desc(BF16, kKeys, 0);
+      const uint32_t idesc_o = instr_desc(BF16, HD, 0) | 1u << 16;
+      const uint64_t q_first = smem_desc(base, 16, 1024), k_first = smem_desc(ring, 16, 1024), v_first = smem_desc(ring, kKeyBlock, 1024);
+      int slot = 0;
+      unsigned phase = 0;
+      auto next_slot = [&]() {
+        const int s = slot;
+        if (++slot == kSlots) {
+          slot = 0;
+          phase ^= 1;
+        }
+        return s;
+      };
+      auto wait = [&](uint64_t* bar, unsigned parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, budget)) != 0; };
+      // Issued by the elected thread.
+      auto scores = [&](int t, int k_slot) {
+        const uint64_t q = desc_advance(q_first, t * kTileBytes), k = desc_advance(k_first, (uint32_t)k_slot * kSlotBytes);
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; kk++)
+          mma_f16(s_col(t), desc_advance(q, (uint32_t)(kk >> 2) * kQueryBlock + (uint32_t)(kk & 3) * 32u),
+                  desc_advance(k, (uint32_t)(kk >> 2) * kKeyBlock + (uint32_t)(kk & 3) * 32u), idesc_s, kk ? 1u : 0u);
+        mma_commit(&s_full[t]);
+      };
+      auto values = [&](int t, int v_slot, bool accumulate) {
+        const uint64_t v = desc_advance(v_first, (uint32_t)v_slot * kSlotBytes);
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 16; kk++)
+          mma_f16_tmem_a(o_col(t), s_col(t) + (uint32_t)kk * 8u, desc_advance(v, (uint32_t)kk * 2048u), idesc_o, (accumulate || kk) ? 1u : 0u);
+      };
+      bool ok = wait(q_full, 0) && wait(&slot_full[0], 0);
+      if (ok) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (leader) {
+          for (int t = 0; t < TILES; t++)
+            if (blocks_of(t)) scores(t, 0);
+          mma_commit(&slot_empty[0]);
+        }
+        __syncwarp();
+        next_slot();
+      }
+      int of_tile[TILES];
+#pragma unroll
+      for (int t = 0; t < TILES; t++) of_tile[t] = blocks_of(t);
+      for (int j = 0; j < blocks && ok; j++) {
+        const unsigned v_phase = phase;
+        const int v_slot = next_slot();
+        const unsigned k_phase = phase;
+        const bool more = j + 1 < blocks;
+        const int k_slot = more ? next_slot() : 0;
+        ok = wait(&slot_full[v_slot], v_phase) && (more || !ragged || wait(v_clean, 0)) && (!more || wait(&slot_full[k_slot], k_phase));
+#pragma unroll
+        for (int t = 0; t < TILES; t++) {
+          if (!ok || j >= of_tile[t]) continue;
+          ok = wait(&p_ready[t], (unsigned)j & 1u);
+          if (!ok) continue;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          if (leader) {
+            values(t, v_slot, j > 0);
+            if (j + 1 < of_tile[t]) scores(t, k_slot);
+            else mma_commit(&o_full[t]);
+          }
+          __syncwarp();
+        }
+        if (ok && leader) {
+          mma_commit(&slot_empty[v_slot]);
+          if (more) mma_commit(&slot_empty[k_slot]);
+        }
+        __syncwarp();
+      }
+      if (!ok && leader) report(p.error_words, kErrorWait);
+      __syncwarp();
+    }
+  } else {
+    if constexpr (TILES == 2) take_registers<216>();
+    const int t = warp >> 2;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_addr = s_col(t) + lanes, o_addr = o_col(t) + lanes;
+    const int row = (warp & 3) * 32 + lane;
+    // Rows that are not there have position -1: every key is hidden and nothing is stored.
+    const int head = row % a.p.heads, at = row / a.p.heads;
+    const int pos = at < a.p.positions && head < heads && first_of(t) + at < keys ? first_of(t) + at : -1;
+    const int first_pos = first_of(t) + (warp & 3) * 32 / a.p.heads;  // of the warp
+    const int mine = blocks_of(t);
+    float m_used = -INFINITY, sum = 0.f;
+    bool ok = true;
+    for (int j = 0; j < mine; j++) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], (unsigned)j & 1u, budget));
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      float s[kKeys];
+#pragma unroll
+      for (int c = 0; c < kKeys / 32; c++) tmem_load_32(s_addr + c * 32, s + c * 32);
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      if (a.sign != 1.f) {
+#pragma unroll
+        for (int e = 0; e < kKeys; e++) s[e] *= a.sign;
+      }
+      const int key0 = j * kKeys;
+      if (key0 + kKeys - 1 > first_pos) {
+#pragma unroll
+        for (int e = 0; e < kKeys; e++)
+          if (key0 + e > pos) s[e] = -INFINITY;
+      }
+      float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int e = 4; e + 8 <= kKeys; e += 8)
+#pragma unroll
+        for (int i = 0; i < 4; i++) mx[i] = max3(mx[i], s[e + 2 * i], s[e + 2 * i + 1]);
+#pragma unroll
+      for (int i = 0; i < 4; i++) mx[i] = fmaxf(mx[i], s[kKeys - 4 + i]);
+      const float m_block = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+      float corr = 1.f;
+      if (m_block > m_used + Probability<BF16>::kGrow) {
+        corr = exp2_approx(m_used - m_block);  // 0 the first time
+        m_used = m_block;
+        sum *= corr;
+      }
+      if (j > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
+#pragma unroll 1
+        for (int c = 0; c < HD; c += 32) {
+          float o[32];
+          tmem_load_32(o_addr + c, o);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+          for (int e = 0; e < 32; e++) o[e] *= corr;
+          tmem_store_32(o_addr + c, o);
+        }
+      }
+      const float shift = m_used == -INFINITY ? 0.f : Probability<BF16>::kLift - m_used;
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < kKeys / 64; c++) {
+        float packed[32];
+#pragma unroll
+        for (int e = 0; e < 32; e++) {
+          const float x = exp2_approx(fmaf(s[c * 64 + 2 * e], a.scale_log2, shift));
+          const float y = exp2_approx(fmaf(s[c * 64 + 2 * e + 1], a.scale_log2, shift));
+          const uint32_t pair = pack_pair<BF16>(x, y);
+          add_pair<BF16>(pair, part[(2 * e) & 3], part[(2 * e + 1) & 3]);
+          packed[e] = __uint_as_float(pair);
+        }
+        tmem_store_32(s_addr + c * 32, packed);
+      }
+      sum += (part[0] + part[1]) + (part[2] + part[3]);
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_ready[t]);
+    }
+    ok = ok && (mine == 0 || __all_sync(0xffffffffu, mbar_wait(&o_full[t], 0, budget)));
+    if (ok && mine > 0) {
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const float inverse = rows::inverse_of(sum);
+      const int h = g * a.p.rep + h0 + head;
+      unsigned short* out = static_cast<unsigned short*>(p.out) + (long long)(item.start + pos) * p.out_stride + h * p.out_head_stride;
+      bool odd = false;
+#pragma unroll
+      for (int c = 0; c < HD; c += 32) {
+        float o[32];
+        tmem_load_32(o_addr + c, o);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (pos >= 0) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              odd = odd || rows::odd(o[e + 2 * i]) || rows::odd(o[e + 2 * i + 1]);
+              w[i] = pack_pair<BF16>(o[e + 2 * i] * inverse, o[e + 2 * i + 1] * inverse);
+            }
+            if (c + e < p.head_dim) *reinterpret_cast<uint4*>(out + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      if (p.lse && pos >= 0)
+        p.lse[(long long)(item.start + pos) * p.heads + h] =
+            sum == 0.f ? -INFINITY : fmaf(m_used - Probability<BF16>::kLift, rows::kLn2, logf(sum));
+      // Rows that a hidden value may have spoilt.
+      const unsigned short* k = static_cast<const unsigned short*>(p.k) + (long long)item.start * p.k_stride + (long long)g * p.k_head_stride;
+      const unsigned short* v = static_cast<const unsigned short*>(p.v) + (long long)item.start * p.v_stride + (long long)g * p.v_head_stride;
+      for (unsigned left = __ballot_sync(0xffffffffu, odd && pos >= 0); left; left &= left - 1) {
+        const int r = __ffs(left) - 1, row_pos = __shfl_sync(0xffffffffu, pos, r), row_h = __shfl_sync(0xffffffffu, h, r);
+        const int hidden = min(mine * kKeys, keys);
+        bool spoilt = false;
+        const int pieces = p.head_dim / 8;
+        for (long long i = (long long)(row_pos + 1) * pieces + lane; i < (long long)hidden * pieces; i += 32) {
+          const uint4 x = *reinterpret_cast<const uint4*>(v + i / pieces * p.v_stride + i % pieces * 8);
+          spoilt = spoilt || odd_pair<BF16>(x.x) || odd_pair<BF16>(x.y) || odd_pair<BF16>(x.z) || odd_pair<BF16>(x.w);
+        }
+        if (!__any_sync(0xffffffffu, spoilt)) continue;
+        const long long token = item.start + row_pos;
+        redo_row<BF16, HD>(a, static_cast<const unsigned short*>(p.q) + token * p.q_stride + row_h * p.q_head_stride, k, v,
+                           static_cast<unsigned short*>(p.out) + token * p.out_stride + row_h * p.out_head_stride, row_pos,
+                           __shfl_sync(0xffffffffu, m_used, r), __shfl_sync(0xffffffffu, sum, r));
+      }
+    } else if (!ok && lane == 0) {
+      report(p.error_words, kErrorWait);
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  }
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    __syncwarp();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
+  }
+}
+
+}  // namespace umma
+}  // namespace pjrtx
