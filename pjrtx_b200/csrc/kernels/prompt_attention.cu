@@ -3,7 +3,7 @@
 //
 // The starts of the sequences are on the device: the grid has a block for every tile that there can be, sequence b's from
 // starts[b] / positions + b on (a sequence of n tokens has at most that many before the next one's), and blocks without a tile leave. The
-// tiles of a sequence run from its end, where they have most to do, to its beginning.
+// tiles of a sequence run from its end, where they have most to do, to its beginning, a tile for all KV heads before the next tile.
 //
 // 16-bit types go to the tensor cores (umma_prompt.cuh), f32 to the CUDA cores (row_attention.cuh).
 #include <algorithm>
@@ -47,8 +47,18 @@ __device__ __forceinline__ PromptTile prompt_tile(const PromptArgs& p, int posit
   return t;
 }
 
-__device__ __forceinline__ void check_starts(const PromptAttention& a, long long thread, long long threads) {
-  for (long long b = thread; b < a.sequences; b += threads)
+// The grid: heads by tiles, the tiles folded where one axis does not hold them.
+constexpr long long kGridAxis = 65535;
+__device__ __forceinline__ long long prompt_block() { return blockIdx.z * kGridAxis + blockIdx.y; }
+inline dim3 prompt_grid(const PromptArgs& p, int positions) {
+  const long long tiles = p.a.tokens / positions + p.a.sequences;
+  return dim3((unsigned)(p.a.kv_heads * p.groups), (unsigned)std::min(tiles, kGridAxis), (unsigned)((tiles + kGridAxis - 1) / kGridAxis));
+}
+
+__device__ __forceinline__ void check_starts(const PromptAttention& a) {
+  if (blockIdx.x) return;
+  const long long step = (long long)gridDim.y * gridDim.z * blockDim.x;
+  for (long long b = (blockIdx.z * (long long)gridDim.y + blockIdx.y) * blockDim.x + threadIdx.x; b < a.sequences; b += step)
     if (a.starts[b] < 0 || a.starts[b + 1] < a.starts[b] || a.starts[b + 1] > a.tokens) report(a.error_words, kErrorLength);
 }
 
@@ -60,17 +70,19 @@ __device__ __forceinline__ void check_starts(const PromptAttention& a, long long
 namespace pjrtx {
 namespace {
 
-template <typename T, int D>
+// In f32.
+template <int D>
 __global__ void __launch_bounds__(rows::kThreads) prompt_rows_kernel(const __grid_constant__ PromptArgs p) {
   PJRTX_PDL_PROLOGUE();
   using namespace rows;
+  using T = float;
   extern __shared__ __align__(16) char smem[];
   Shared<D>& s = *reinterpret_cast<Shared<D>*>(smem);
   const PromptAttention& a = p.a;
-  if (blockIdx.y == 0) check_starts(a, (long long)blockIdx.x * kThreads + threadIdx.x, (long long)gridDim.x * kThreads);
-  const PromptTile t = prompt_tile(p, p.positions, blockIdx.x);
+  check_starts(a);
+  const PromptTile t = prompt_tile(p, p.positions, prompt_block());
   if (t.tile < 0) return;
-  const int g = blockIdx.y / p.groups, h0 = blockIdx.y % p.groups * p.heads, heads = min(p.heads, p.rep - h0);
+  const int g = blockIdx.x / p.groups, h0 = blockIdx.x % p.groups * p.heads, heads = min(p.heads, p.rep - h0);
   const int first = t.tile * p.positions, positions = min(p.positions, t.tokens - first);
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   auto place = [&](int r, int* position, int* head) {
@@ -114,22 +126,14 @@ __global__ void __launch_bounds__(rows::kThreads) prompt_rows_kernel(const __gri
   }
 }
 
-template <typename T, int D>
+template <int D>
 int launch_rows(PromptArgs p, bool pdl, cudaStream_t stream) {
   constexpr size_t smem = sizeof(rows::Shared<D>);
-  if (!raise_smem_limit((const void*)prompt_rows_kernel<T, D>, (int)smem)) return 0;
+  if (!raise_smem_limit((const void*)prompt_rows_kernel<D>, (int)smem)) return 0;
   p.heads = std::min(p.rep, rows::kRows);
   p.groups = (p.rep + p.heads - 1) / p.heads;
   p.positions = rows::kRows / p.heads;
-  const dim3 grid((unsigned)(p.a.tokens / p.positions + p.a.sequences), (unsigned)(p.a.kv_heads * p.groups));
-  return launch_kernel(prompt_rows_kernel<T, D>, grid, dim3(rows::kThreads), smem, stream, pdl, p) == cudaSuccess;
-}
-
-template <typename T>
-int launch_rows_of(const PromptArgs& p, bool pdl, cudaStream_t stream) {
-  return p.a.head_dim <= 64    ? launch_rows<T, 64>(p, pdl, stream)
-         : p.a.head_dim <= 128 ? launch_rows<T, 128>(p, pdl, stream)
-                               : launch_rows<T, 256>(p, pdl, stream);
+  return launch_kernel(prompt_rows_kernel<D>, prompt_grid(p, p.positions), dim3(rows::kThreads), smem, stream, pdl, p) == cudaSuccess;
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -168,15 +172,13 @@ int launch_umma(const umma::PromptKernelArgs& a, bool pdl, cudaStream_t stream) 
   CUtensorMap qmap, kmap, vmap;
   if (!encode_map(&qmap, p.q, !BF16, 4, q_extents, q_strides, q_box) || !encode_map(&kmap, p.k, !BF16, 3, k_extents, k_strides, k_box) ||
       !encode_map(&vmap, p.v, !BF16, 3, k_extents, v_strides, k_box))
-    return -1;
+    return 0;
   constexpr size_t smem = umma::prompt_smem(HD, TILES);
   auto kernel = umma::umma_prompt_kernel<BF16, HD, TILES>;
   if (!raise_smem_limit((const void*)kernel, (int)smem)) return 0;
-  const dim3 grid((unsigned)(p.tokens / (TILES * a.p.positions) + p.sequences), (unsigned)(p.kv_heads * a.p.groups));
-  return launch_kernel(kernel, grid, dim3(umma::prompt_threads(TILES)), smem, stream, pdl, a, qmap, kmap, vmap) == cudaSuccess;
+  return launch_kernel(kernel, prompt_grid(a.p, TILES * a.p.positions), dim3(umma::prompt_threads(TILES)), smem, stream, pdl, a, qmap, kmap, vmap) == cudaSuccess;
 }
 
-// 1, 0 where the launch failed, -1 where a layout has no tensor map.
 template <bool BF16>
 int launch_umma_of(PromptArgs p, int sm_count, bool pdl, cudaStream_t stream) {
   umma::PromptKernelArgs a;
@@ -201,13 +203,9 @@ int prompt_attention_launch(const PromptAttention& a, int sm_count, bool pdl, cu
   PromptArgs p;
   p.a = a;
   p.rep = a.heads / a.kv_heads;
-  if (a.dtype != kF32) {
-    const int launched = a.dtype == kF16 ? launch_umma_of<false>(p, sm_count, pdl, stream) : launch_umma_of<true>(p, sm_count, pdl, stream);
-    if (launched >= 0) return launched;
-  }
-  return a.dtype == kF32   ? launch_rows_of<float>(p, pdl, stream)
-         : a.dtype == kF16 ? launch_rows_of<__half>(p, pdl, stream)
-                           : launch_rows_of<__nv_bfloat16>(p, pdl, stream);
+  if (a.dtype == kF16) return launch_umma_of<false>(p, sm_count, pdl, stream);
+  if (a.dtype == kBF16) return launch_umma_of<true>(p, sm_count, pdl, stream);
+  return a.head_dim <= 64 ? launch_rows<64>(p, pdl, stream) : a.head_dim <= 128 ? launch_rows<128>(p, pdl, stream) : launch_rows<256>(p, pdl, stream);
 }
 
 }  // namespace pjrtx

@@ -4,6 +4,8 @@
 // comes from is known where it is fetched, and what a row sees are the keys below `length` and a word of bits from there on. A tile of
 // query rows is some nodes of a sequence times the query heads of a KV head: row x is head x % heads of node x / heads. So each cached row
 // is read once for all nodes and heads that share it, which is what the operator is for: one node at a time would read it once for each.
+//
+// 16-bit types go to the tensor cores (umma_tree.cuh), f32 to the CUDA cores (row_attention.cuh).
 #include <algorithm>
 
 #include "../common.h"
@@ -210,6 +212,14 @@ __device__ __forceinline__ float* part_of(const TreeArgs& p, const Share& share,
   return p.parts + ((long long)blockIdx.x * 2 + (blockIdx.x == first ? 1 : 0)) * p.slot_rows * (p.dims + 2);
 }
 
+}  // namespace
+}  // namespace pjrtx
+
+#include "umma_tree.cuh"
+
+namespace pjrtx {
+namespace {
+
 // ---- on the CUDA cores ---------------------------------------------------------------------------------------------
 
 template <typename T, int D>
@@ -351,23 +361,48 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const __grid
 
 // Which kernel a shape runs on.
 struct TreePlan {
-  int dims = 0, rows = 0, keys = 0;  // of a row, of a tile of queries, of a tile of keys
-  size_t smem = 0;
-  const void* kernel = nullptr;
+  int dims, rows, keys;  // of a row, of a tile of queries, of a tile of keys
+  int threads;
+  size_t smem;
 };
 
+// f(kernel, plan) for calls with `rows` query rows a sequence and KV head at most: two tiles read the keys once for up to 256 of them.
 template <typename F>
-auto with_kernel(int dtype, int head_dim, F&& f) {
-#define PJRTX_TREE_ROWS(T, D) return f(tree_rows_kernel<T, D>, TreePlan{D, rows::kRows, rows::kKeys, sizeof(rows::Shared<D>)})
-#define PJRTX_TREE_ROWS_OF(T)                         \
-  if (head_dim <= 64) PJRTX_TREE_ROWS(T, 64);         \
-  if (head_dim <= 128) PJRTX_TREE_ROWS(T, 128);       \
-  PJRTX_TREE_ROWS(T, 256)
-  if (dtype == kF32) { PJRTX_TREE_ROWS_OF(float); }
-  if (dtype == kF16) { PJRTX_TREE_ROWS_OF(__half); }
-  PJRTX_TREE_ROWS_OF(__nv_bfloat16);
-#undef PJRTX_TREE_ROWS_OF
+auto with_kernel(int dtype, int head_dim, long long rows, F&& f) {
+#define PJRTX_TREE_ROWS(D) return f(tree_rows_kernel<float, D>, TreePlan{D, rows::kRows, rows::kKeys, rows::kThreads, sizeof(rows::Shared<D>)})
+#define PJRTX_TREE_UMMA(BF16, D, TILES) \
+  return f(umma::umma_tree_kernel<BF16, D, TILES>, \
+           TreePlan{D, TILES * umma::kAttnRows, umma::tree_keys(D), umma::tree_threads(TILES), umma::tree_smem(D, TILES)})
+#define PJRTX_TREE_UMMA_OF(BF16)                                                     \
+  if (head_dim > 128) PJRTX_TREE_UMMA(BF16, 256, 1);                                 \
+  if (head_dim > 64 && rows > umma::kAttnRows) PJRTX_TREE_UMMA(BF16, 128, 2);        \
+  if (head_dim > 64) PJRTX_TREE_UMMA(BF16, 128, 1);                                  \
+  if (rows > umma::kAttnRows) PJRTX_TREE_UMMA(BF16, 64, 2);                          \
+  PJRTX_TREE_UMMA(BF16, 64, 1)
+  if (dtype == kF32) {
+    if (head_dim <= 64) PJRTX_TREE_ROWS(64);
+    if (head_dim <= 128) PJRTX_TREE_ROWS(128);
+    PJRTX_TREE_ROWS(256);
+  }
+  if (dtype == kF16) { PJRTX_TREE_UMMA_OF(false); }
+  PJRTX_TREE_UMMA_OF(true);
+#undef PJRTX_TREE_UMMA_OF
+#undef PJRTX_TREE_UMMA
 #undef PJRTX_TREE_ROWS
+}
+
+// The tensor-core kernels take the scale apart.
+bool start(void (*kernel)(const TreeArgs), const TreeArgs& p, const TreePlan& plan, long long blocks, bool pdl, cudaStream_t stream) {
+  return launch_kernel(kernel, dim3((unsigned)blocks), dim3((unsigned)plan.threads), plan.smem, stream, pdl, p) == cudaSuccess;
+}
+bool start(void (*kernel)(const umma::TreeKernelArgs), const TreeArgs& p, const TreePlan& plan, long long blocks, bool pdl, cudaStream_t stream) {
+  const float scale = p.a.scale;
+  umma::TreeKernelArgs a;
+  a.p = p;
+  a.scale_log2 = scale == 0.f ? 1.f : (scale < 0.f ? -scale : scale) * rows::kLog2e;
+  a.sign = scale > 0.f ? 1.f : scale < 0.f ? -1.f : 0.f;
+  a.timeout_ns = wait_timeout_ns();
+  return launch_kernel(kernel, dim3((unsigned)blocks), dim3((unsigned)plan.threads), plan.smem, stream, pdl, a) == cudaSuccess;
 }
 
 uint64_t round256(uint64_t n) { return (n + 255) / 256 * 256; }
@@ -375,7 +410,7 @@ uint64_t round256(uint64_t n) { return (n + 255) / 256 * 256; }
 }  // namespace
 
 uint64_t paged_tree_workspace(const PagedView& c, int heads, int nodes, int sm_count) {
-  return with_kernel(c.dtype, c.head_dim, [&](auto, const TreePlan& plan) {
+  return with_kernel(c.dtype, c.head_dim, (long long)nodes * (heads / c.kv_heads), [&](auto, const TreePlan& plan) {
     return round256((uint64_t)sm_count * sizeof(Cut)) + (uint64_t)sm_count * 2 * plan.rows * (plan.dims + 2) * 4;
   });
 }
@@ -390,7 +425,7 @@ int paged_tree_launch(const PagedView& c, const PagedTree& a, int sm_count, bool
   p.cuts = reinterpret_cast<Cut*>(space);
   p.parts = reinterpret_cast<float*>(space + round256((uint64_t)sm_count * sizeof(Cut)));
   long long blocks = 0;
-  const bool ok = with_kernel(c.dtype, c.head_dim, [&](auto kernel, const TreePlan& plan) {
+  const bool ok = with_kernel(c.dtype, c.head_dim, (long long)a.nodes * p.rep, [&](auto kernel, const TreePlan& plan) {
     p.heads = std::min(p.rep, plan.rows);
     p.groups = (p.rep + p.heads - 1) / p.heads;
     p.nodes = plan.rows / p.heads;
@@ -401,7 +436,7 @@ int paged_tree_launch(const PagedView& c, const PagedTree& a, int sm_count, bool
     const long long numbers = (long long)c.batch * c.kv_heads * p.groups * ((a.nodes + p.nodes - 1) / p.nodes) *
                               ((c.capacity() + a.nodes + p.tile_keys - 1) / p.tile_keys + kSegmentCost);
     blocks = std::min<long long>(numbers, sm_count);
-    return launch_kernel(kernel, dim3((unsigned)blocks), dim3(rows::kThreads), plan.smem, stream, pdl, p) == cudaSuccess;
+    return start(kernel, p, plan, blocks, pdl, stream);
   });
   if (!ok) return 0;
   auto join = c.dtype == kF32 ? tree_join_kernel<float> : c.dtype == kF16 ? tree_join_kernel<__half> : tree_join_kernel<__nv_bfloat16>;

@@ -7,17 +7,12 @@
 //                  tile work, the tensor core has the other's products
 //   softmax warps  four a tile, a query row a thread (its lane of tensor memory), so a row's maximum and sum need no exchange
 //
-// Probabilities go to the tensor core in the element type, and the sum is taken of them as they are then, so that equal values under all
-// keys give that value. In f16 they are multiplied by 2^11 first: f16 then holds them down to 2^-35 of the largest, and not only to 2^-24.
-// They are relative to a maximum that follows the row's when that has grown by 2^8 (f16: 2^4, so that they stay below 2^16): the factor
-// cancels in the division, and the results in tensor memory are rescaled that much more rarely.
-//
 // Hidden keys have probability 0, but the tensor core multiplies it by their values, and 0 times infinity or NaN is NaN. So values
 // behind the last position of the block of threads are cleared in shared memory, and a row with a result that is not finite looks at
 // the values between its position and there; only where one is infinite or NaN it is computed once more, by its warp and without them.
 #pragma once
 
-#include "umma_attention.cuh"
+#include "umma_rows.cuh"
 
 namespace pjrtx {
 namespace umma {
@@ -28,9 +23,6 @@ struct PromptKernelArgs {
   float sign;         // 1, -1 or 0: what scores are multiplied by first, so that the largest score has the largest exponent
   unsigned long long timeout_ns;
 };
-
-template <bool BF16> struct Probability { static constexpr float kLift = 0.f, kGrow = 8.f; };
-template <> struct Probability<false> { static constexpr float kLift = 11.f, kGrow = 4.f; };
 
 __host__ __device__ constexpr int prompt_keys(int hd) { return hd == 256 ? 64 : 128; }  // of a block
 constexpr int kPromptSlots = 5;
@@ -48,26 +40,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap
                "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
                : "memory");
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float y;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-  return y;
-}
-template <int REGISTERS>
-__device__ __forceinline__ void take_registers() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGISTERS));
-}
-template <int REGISTERS>
-__device__ __forceinline__ void leave_registers() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGISTERS));
-}
-// Whether one of two packed 16-bit elements is infinite or NaN.
-template <bool BF16>
-__device__ __forceinline__ bool odd_pair(uint32_t w) {
-  constexpr uint32_t kExponent = BF16 ? 0x7f80u : 0x7c00u;
-  return (w & kExponent) == kExponent || (w >> 16 & kExponent) == kExponent;
-}
-
 // Row `pos` once more, over the keys that it sees; called by a whole warp, `m` and `total` being the row's.
 template <bool BF16, int HD>
 __device__ __noinline__ void redo_row(const PromptKernelArgs& a, const unsigned short* q, const unsigned short* k, const unsigned short* v,
@@ -133,11 +105,11 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
   constexpr int kMmaWarp = 4 * TILES, kCopyWarp = 4 * TILES + 1;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const PromptAttention& p = a.p.a;
-  if (blockIdx.y == 0) check_starts(p, (long long)blockIdx.x * blockDim.x + threadIdx.x, (long long)gridDim.x * blockDim.x);
-  const PromptTile item = prompt_tile(a.p, TILES * a.p.positions, blockIdx.x);
+  check_starts(p);
+  const PromptTile item = prompt_tile(a.p, TILES * a.p.positions, prompt_block());
   if (item.tile < 0) return;
   const WaitBudget budget{global_timer_ns() + a.timeout_ns, flags};
-  const int g = blockIdx.y / a.p.groups, h0 = blockIdx.y % a.p.groups * a.p.heads, heads = min(a.p.heads, a.p.rep - h0);
+  const int g = blockIdx.x / a.p.groups, h0 = blockIdx.x % a.p.groups * a.p.heads, heads = min(a.p.heads, a.p.rep - h0);
   const int first = item.tile * TILES * a.p.positions;
   const int keys = min(first + TILES * a.p.positions, item.tokens);  // behind the last position of the block
   // Of a tile: its positions, and the blocks of keys up to the last of them (0: there is no such tile).
@@ -174,7 +146,7 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
   auto o_col = [&](int t) { return tmem_base + (uint32_t)(TILES * kKeys + t * HD); };
 
   if (warp >= 4 * TILES) {
-    if constexpr (TILES == 2) leave_registers<72>();
+    if constexpr (TILES == 2) leave_registers<104>();
     const bool leader = elect_one();
     if (warp == kCopyWarp) {
       // K0 V0 K1 V1 ...
@@ -300,7 +272,7 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
       __syncwarp();
     }
   } else {
-    if constexpr (TILES == 2) take_registers<216>();
+    if constexpr (TILES == 2) take_registers<200>();
     const int t = warp >> 2;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_addr = s_col(t) + lanes, o_addr = o_col(t) + lanes;
