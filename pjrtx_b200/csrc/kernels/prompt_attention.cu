@@ -136,32 +136,6 @@ int launch_rows(PromptArgs p, bool pdl, cudaStream_t stream) {
   return launch_kernel(prompt_rows_kernel<D>, prompt_grid(p, p.positions), dim3(rows::kThreads), smem, stream, pdl, p) == cudaSuccess;
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// A map of `rank` axes, head_dim first, for boxes of 64 elements; `strides` (elements) are those of the axes behind the first. An axis of
-// one element may come with any stride, which the encoder does not take.
-bool encode_map(CUtensorMap* map, const void* base, bool f16, int rank, const long long* extents, const long long* strides, const int* box) {
-  static const EncodeTiledFn encode = [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess) f = nullptr;
-    return (EncodeTiledFn)f;
-  }();
-  if (!encode) return false;
-  cuuint64_t dims[4], bytes[3];
-  cuuint32_t boxes[4], steps[4];
-  for (int d = 0; d < rank; d++) {
-    dims[d] = (cuuint64_t)extents[d];
-    boxes[d] = (cuuint32_t)box[d];
-    steps[d] = 1;
-    if (d) bytes[d - 1] = (cuuint64_t)(extents[d] == 1 ? extents[0] : strides[d - 1]) * 2;
-  }
-  return encode(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), dims, bytes,
-                boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <bool BF16, int HD, int TILES>
 int launch_umma(const umma::PromptKernelArgs& a, bool pdl, cudaStream_t stream) {
   const PromptAttention& p = a.p.a;
@@ -170,8 +144,8 @@ int launch_umma(const umma::PromptKernelArgs& a, bool pdl, cudaStream_t stream) 
   const long long k_strides[2] = {p.k_stride, p.k_head_stride}, v_strides[2] = {p.v_stride, p.v_head_stride};
   const int q_box[4] = {64, a.p.heads, 1, a.p.positions}, k_box[3] = {64, umma::prompt_keys(HD), 1};
   CUtensorMap qmap, kmap, vmap;
-  if (!encode_map(&qmap, p.q, !BF16, 4, q_extents, q_strides, q_box) || !encode_map(&kmap, p.k, !BF16, 3, k_extents, k_strides, k_box) ||
-      !encode_map(&vmap, p.v, !BF16, 3, k_extents, v_strides, k_box))
+  if (!umma::encode_map(&qmap, p.q, !BF16, 4, q_extents, q_strides, q_box) || !umma::encode_map(&kmap, p.k, !BF16, 3, k_extents, k_strides, k_box) ||
+      !umma::encode_map(&vmap, p.v, !BF16, 3, k_extents, v_strides, k_box))
     return 0;
   constexpr size_t smem = umma::prompt_smem(HD, TILES);
   auto kernel = umma::umma_prompt_kernel<BF16, HD, TILES>;

@@ -38,7 +38,7 @@ struct TreeArgs {
   int rep, heads, groups;  // query heads of a KV head; those of a tile; tiles that share a node
   int nodes;               // of a tile
   int tile_keys;
-  int slot_rows, dims;     // of a part's sums in the workspace: dims values a row, then (max, total) of every row
+  int slot_rows, dims;     // of a part's sums in the workspace: [dims][rows], then the rows' maxima and totals
   unsigned reciprocal;     // floor(2^32 / page_size), at most 2^32 - 1
   Cut* cuts;               // [blocks]
   float* parts;            // [blocks][2][slot_rows * (dims + 2)]
@@ -48,10 +48,14 @@ struct Sequence {
   int length, count, tiles, segments;  // cached rows, nodes; units of a segment; segments
 };
 
-__device__ __forceinline__ Sequence sequence_of(const TreeArgs& p, int b) {
+__device__ __forceinline__ Sequence sequence_of(const TreeArgs& p, int b, bool check = false) {
   Sequence s;
   const int count = p.a.counts ? p.a.counts[b] : p.a.nodes;
   s.length = paged_length(p.c, b);
+  if (check) {
+    paged_check_length(p.c, b);
+    if (count < 0 || count > p.a.nodes) report(p.c.error_words, kErrorLength);
+  }
   s.count = max(0, min(count, p.a.nodes));
   s.tiles = s.count ? (s.length + s.count + p.tile_keys - 1) / p.tile_keys : 0;
   s.segments = p.c.kv_heads * p.groups * ((s.count + p.nodes - 1) / p.nodes);
@@ -104,7 +108,7 @@ __device__ __forceinline__ Share share_of_block(const TreeArgs& p, ShareSpace<TH
   const int per_thread = (p.c.batch + THREADS - 1) / THREADS;
   const int first = min(p.c.batch, (int)threadIdx.x * per_thread), last = min(p.c.batch, first + per_thread);
   long long mine = 0;
-  for (int b = first; b < last; b++) mine += numbers_of(sequence_of(p, b));
+  for (int b = first; b < last; b++) mine += numbers_of(sequence_of(p, b, blockIdx.x == 0));
   long long sum = mine;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
@@ -180,27 +184,20 @@ __device__ __forceinline__ long long lse_at(const TreeArgs& p, const Segment& s,
   return ((long long)s.b * p.a.nodes + node) * p.a.heads + s.g * p.rep + s.h0 + head;
 }
 
+// Column of the page table that row t is in.
+__device__ __forceinline__ int column_of(const TreeArgs& p, int t) {
+  const int column = (int)__umulhi((unsigned)t, p.reciprocal);  // the quotient or one less
+  return t - column * p.c.page_size >= p.c.page_size ? column + 1 : column;
+}
+
 // Element offset of cached row t of sequence b in either pool (KV head 0), -1 where the table names no page.
 __device__ __forceinline__ long long cached_row(const TreeArgs& p, int b, int t) {
-  int column = (int)__umulhi((unsigned)t, p.reciprocal);  // the quotient or one less
-  int row = t - column * p.c.page_size;
-  if (row >= p.c.page_size) {
-    column++;
-    row -= p.c.page_size;
-  }
-  const int page = p.c.table[b * p.c.table_stride + column];
+  const int column = column_of(p, t), page = p.c.table[b * p.c.table_stride + column];
   if (page < 0 || page >= p.c.num_pages) {
     report(p.c.error_words, kErrorPageId);
     return -1;
   }
-  return page * p.c.page_stride + row * p.c.row_stride;
-}
-
-__device__ __forceinline__ void check_sequences(const TreeArgs& p) {
-  for (int b = blockIdx.x * blockDim.x + threadIdx.x; b < p.c.batch; b += gridDim.x * blockDim.x) {
-    paged_check_length(p.c, b);
-    if (p.a.counts && (p.a.counts[b] < 0 || p.a.counts[b] > p.a.nodes)) report(p.c.error_words, kErrorLength);
-  }
+  return page * p.c.page_stride + (t - column * p.c.page_size) * p.c.row_stride;
 }
 
 // The slot of this block's part of a segment that other blocks share, and the cut that the join goes by; null where none does. Slot 1
@@ -210,6 +207,11 @@ __device__ __forceinline__ float* part_of(const TreeArgs& p, const Share& share,
   if (first == last) return nullptr;
   if (threadIdx.x == 0 && blockIdx.x == first) p.cuts[blockIdx.x] = {u.b, u.group, (int)first, (int)last};
   return p.parts + ((long long)blockIdx.x * 2 + (blockIdx.x == first ? 1 : 0)) * p.slot_rows * (p.dims + 2);
+}
+
+__device__ __forceinline__ void store_statistics(const TreeArgs& p, float* part, int row, float m, float total) {
+  part[(long long)p.slot_rows * p.dims + row] = m;
+  part[(long long)p.slot_rows * (p.dims + 1) + row] = total;
 }
 
 }  // namespace
@@ -232,7 +234,6 @@ __global__ void __launch_bounds__(rows::kThreads) tree_rows_kernel(const __grid_
   __shared__ long long place_of[kKeys];  // of the keys of a block
   Shared<D>& s = *reinterpret_cast<Shared<D>*>(smem);
   if (threadIdx.x == 0) p.cuts[blockIdx.x] = {0, 0, 0, 0};
-  check_sequences(p);
   const Share share = share_of_block(p, space);
   if (share.first >= share.size) return;
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
@@ -280,81 +281,106 @@ __global__ void __launch_bounds__(rows::kThreads) tree_rows_kernel(const __grid_
       more = next_unit(p, now, at, share.size);
       if (!more || now.group != here.group || now.b != here.b) break;
     }
-    float* part = part_of(p, share, here, segment);
+    if (float* part = part_of(p, share, here, segment)) {
+#pragma unroll
+      for (int c = 0; c < D / 64; c++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          float x[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const float2 o = pair_split(sum.o[i][c][e / 2]);
+            x[i] = e % 2 ? o.y : o.x;
+          }
+          *reinterpret_cast<float4*>(part + (c * 64 + tx * 4 + e) * p.slot_rows + ty * 4) = make_float4(x[0], x[1], x[2], x[3]);
+        }
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (tx == 0) store_statistics(p, part, ty * 4 + i, sum.m[i], sum.l[i]);
+      continue;
+    }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       int node, head;
-      const int row = ty * 4 + i;
-      if (!seg.place(p, row, &node, &head)) continue;
-      const float inverse = part ? 1.f : inverse_of(sum.l[i]);
+      if (!seg.place(p, ty * 4 + i, &node, &head)) continue;
+      const float inverse = inverse_of(sum.l[i]);
       T* out = static_cast<T*>(p.a.out) + out_at(p, seg, node, head);
 #pragma unroll
       for (int c = 0; c < D / 64; c++) {
         const float2 x = pair_split(sum.o[i][c][0]), y = pair_split(sum.o[i][c][1]);
         const int d = c * 64 + tx * 4;
-        const float4 o = make_float4(x.x * inverse, x.y * inverse, y.x * inverse, y.y * inverse);
-        if (part) *reinterpret_cast<float4*>(part + row * D + d) = o;
-        else if (d < p.c.head_dim) store4(out + d, o);
+        if (d < p.c.head_dim) store4(out + d, make_float4(x.x * inverse, x.y * inverse, y.x * inverse, y.y * inverse));
       }
-      if (tx) continue;
-      if (part) *reinterpret_cast<float2*>(part + p.slot_rows * D + 2 * row) = make_float2(sum.m[i], sum.l[i]);
-      else if (p.a.lse) p.a.lse[lse_at(p, seg, node, head)] = lse_of(sum.m[i], sum.l[i]);
+      if (tx == 0 && p.a.lse) p.a.lse[lse_at(p, seg, node, head)] = lse_of(sum.m[i], sum.l[i]);
     }
   }
 }
 
 // ---- parts of a segment ---------------------------------------------------------------------------------------------
 
-// A warp a row: the parts' (max, total) of every 32 by the lanes, then the values of each dimension over the parts, in block order.
+// A block has 32 rows and 16 dimensions of a cut segment, a lane a row. Its warps take the parts in turn, each with a maximum of its own
+// that it follows, and are joined in order, so that the result does not depend on which is first.
+constexpr int kJoinDims = 16;
+
 template <typename T>
 __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const __grid_constant__ TreeArgs p) {
   PJRTX_PDL_PROLOGUE();
   using namespace rows;
+  __shared__ float sums[kJoinWarps][kJoinDims][32], stats[kJoinWarps][2][32];
+  __shared__ float results[32][kJoinDims + 4];
   const Cut cut = p.cuts[blockIdx.x];
   if (cut.first >= cut.last) return;
-  const int lane = threadIdx.x % 32, row = blockIdx.y * kJoinWarps + threadIdx.x / 32;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, row0 = blockIdx.y * 32, row = row0 + lane, d0 = blockIdx.z * kJoinDims;
   const Segment seg = segment_of(p, cut.b, cut.group, sequence_of(p, cut.b).count);
   int node, head;
-  if (!seg.place(p, row, &node, &head)) return;
+  const bool there = seg.place(p, row, &node, &head);
+  if (!__any_sync(~0u, there)) return;  // the same rows in every warp
   const long long slot = (long long)p.slot_rows * (p.dims + 2);
-  auto part = [&](int i) { return p.parts + ((long long)(cut.first + i) * 2 + (i ? 0 : 1)) * slot; };
-  const int parts = cut.last - cut.first + 1;
-  float top = -INFINITY;
-  for (int i = lane; i < parts; i += 32) top = fmaxf(top, part(i)[p.slot_rows * p.dims + 2 * row]);
+  const int parts = cut.last - cut.first + 1, maxima = p.slot_rows * p.dims, totals = maxima + p.slot_rows;
+  float m = -INFINITY, total = 0.f, x[kJoinDims];
 #pragma unroll
-  for (int w = 16; w; w /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, w));
-  const float shift = top == -INFINITY ? 0.f : top;
-  float total = 0.f;
-  for (int d0 = 0; d0 < p.dims; d0 += 128) {
-    const int d = d0 + lane * 4;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    total = 0.f;
-    for (int i0 = 0; i0 < parts; i0 += 32) {
-      float weight = 0.f, mass = 0.f;
-      if (i0 + lane < parts) {
-        const float2 stat = *reinterpret_cast<const float2*>(part(i0 + lane) + p.slot_rows * p.dims + 2 * row);
-        weight = stat.x == -INFINITY && stat.y == 0.f ? 0.f : stat.x == top ? 1.f : exp2_fast(stat.x - shift);
-        mass = stat.y;
-      }
-      const int n = min(32, parts - i0);
-#pragma unroll 8
-      for (int i = 0; i < n; i++) {
-        const float w = __shfl_sync(~0u, weight, i);
-        total = fmaf(w, __shfl_sync(~0u, mass, i), total);
-        if (d < p.dims && w != 0.f) {
-          const float4 y = *reinterpret_cast<const float4*>(part(i0 + i) + row * p.dims + d);
-          x.x = fmaf(w, y.x, x.x);
-          x.y = fmaf(w, y.y, x.y);
-          x.z = fmaf(w, y.z, x.z);
-          x.w = fmaf(w, y.w, x.w);
-        }
-      }
+  for (int e = 0; e < kJoinDims; e++) x[e] = 0.f;
+  // Adds sums y relative to m_new.
+  auto add = [&](float m_new, float mass, const float (&y)[kJoinDims]) {
+    if (m_new == -INFINITY && mass == 0.f) return;
+    const float top = fmaxf(m, m_new), shift = top == -INFINITY ? 0.f : top;
+    const float was = m == top ? 1.f : exp2_fast(m - shift), is = m_new == top ? 1.f : exp2_fast(m_new - shift);
+    total = fmaf(total, was, mass * is);
+#pragma unroll
+    for (int e = 0; e < kJoinDims; e++) x[e] = fmaf(x[e], was, y[e] * is);
+    m = top;
+  };
+  if (there)
+    for (int i = warp; i < parts; i += kJoinWarps) {
+      const float* from = p.parts + ((long long)(cut.first + i) * 2 + (i ? 0 : 1)) * slot + row;
+      float y[kJoinDims];
+#pragma unroll
+      for (int e = 0; e < kJoinDims; e++) y[e] = from[(d0 + e) * p.slot_rows];
+      add(from[maxima], from[totals], y);
+    }
+  stats[warp][0][lane] = m;
+  stats[warp][1][lane] = total;
+#pragma unroll
+  for (int e = 0; e < kJoinDims; e++) sums[warp][e][lane] = x[e];
+  __syncthreads();
+  if (warp == 0) {
+    for (int w = 1; w < kJoinWarps; w++) {
+      float y[kJoinDims];
+#pragma unroll
+      for (int e = 0; e < kJoinDims; e++) y[e] = sums[w][e][lane];
+      add(stats[w][0][lane], stats[w][1][lane], y);
     }
     const float inverse = inverse_of(total);
-    if (d < p.c.head_dim)
-      store4(static_cast<T*>(p.a.out) + out_at(p, seg, node, head) + d, make_float4(x.x * inverse, x.y * inverse, x.z * inverse, x.w * inverse));
+#pragma unroll
+    for (int e = 0; e < kJoinDims; e++) results[lane][e] = x[e] * inverse;
+    if (p.a.lse && there && blockIdx.z == 0) p.a.lse[lse_at(p, seg, node, head)] = lse_of(m, total);
+    __syncwarp();
+    for (int i = lane; i < 32 * (kJoinDims / 4); i += 32) {
+      const int r = i / (kJoinDims / 4), d = i % (kJoinDims / 4) * 4;
+      if (d0 + d < p.c.head_dim && seg.place(p, row0 + r, &node, &head))
+        store4(static_cast<T*>(p.a.out) + out_at(p, seg, node, head) + d0 + d, *reinterpret_cast<const float4*>(&results[r][d]));
+    }
   }
-  if (p.a.lse && lane == 0) p.a.lse[lse_at(p, seg, node, head)] = lse_of(top, total);
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------------
@@ -395,14 +421,23 @@ auto with_kernel(int dtype, int head_dim, long long rows, F&& f) {
 bool start(void (*kernel)(const TreeArgs), const TreeArgs& p, const TreePlan& plan, long long blocks, bool pdl, cudaStream_t stream) {
   return launch_kernel(kernel, dim3((unsigned)blocks), dim3((unsigned)plan.threads), plan.smem, stream, pdl, p) == cudaSuccess;
 }
-bool start(void (*kernel)(const umma::TreeKernelArgs), const TreeArgs& p, const TreePlan& plan, long long blocks, bool pdl, cudaStream_t stream) {
+bool start(void (*kernel)(const umma::TreeKernelArgs, const CUtensorMap, const CUtensorMap), const TreeArgs& p, const TreePlan& plan, long long blocks, bool pdl, cudaStream_t stream) {
   const float scale = p.a.scale;
   umma::TreeKernelArgs a;
   a.p = p;
   a.scale_log2 = scale == 0.f ? 1.f : (scale < 0.f ? -scale : scale) * rows::kLog2e;
   a.sign = scale > 0.f ? 1.f : scale < 0.f ? -1.f : 0.f;
   a.timeout_ns = wait_timeout_ns();
-  return launch_kernel(kernel, dim3((unsigned)blocks), dim3((unsigned)plan.threads), plan.smem, stream, pdl, a) == cudaSuccess;
+  a.box = umma::tree_box(plan.dims, p.c.page_size);
+  CUtensorMap kmap{}, vmap{};
+  if (a.box) {
+    const PagedView& c = p.c;
+    const long long extents[4] = {c.head_dim, c.page_size, c.kv_heads, c.num_pages}, strides[3] = {c.row_stride, c.head_stride, c.page_stride};
+    const int box[4] = {64, a.box, 1, 1};
+    if (!umma::encode_map(&kmap, c.k, c.dtype == kF16, 4, extents, strides, box) || !umma::encode_map(&vmap, c.v, c.dtype == kF16, 4, extents, strides, box))
+      return false;
+  }
+  return launch_kernel(kernel, dim3((unsigned)blocks), dim3((unsigned)plan.threads), plan.smem, stream, pdl, a, kmap, vmap) == cudaSuccess;
 }
 
 uint64_t round256(uint64_t n) { return (n + 255) / 256 * 256; }
@@ -441,7 +476,7 @@ int paged_tree_launch(const PagedView& c, const PagedTree& a, int sm_count, bool
   if (!ok) return 0;
   auto join = c.dtype == kF32 ? tree_join_kernel<float> : c.dtype == kF16 ? tree_join_kernel<__half> : tree_join_kernel<__nv_bfloat16>;
   const int rows = std::min(p.slot_rows, std::min(p.nodes, a.nodes) * p.heads);
-  return launch_kernel(join, dim3((unsigned)blocks, (unsigned)((rows + kJoinWarps - 1) / kJoinWarps)), dim3(kJoinWarps * 32), 0, stream, true, p) ==
+  return launch_kernel(join, dim3((unsigned)blocks, (unsigned)((rows + 31) / 32), (unsigned)((c.head_dim + kJoinDims - 1) / kJoinDims)), dim3(kJoinWarps * 32), 0, stream, true, p) ==
                  cudaSuccess
              ? 2
              : 0;

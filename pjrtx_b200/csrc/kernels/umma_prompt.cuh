@@ -302,14 +302,8 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
         for (int e = 0; e < kKeys; e++)
           if (key0 + e > pos) s[e] = -INFINITY;
       }
-      float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-      for (int e = 4; e + 8 <= kKeys; e += 8)
-#pragma unroll
-        for (int i = 0; i < 4; i++) mx[i] = max3(mx[i], s[e + 2 * i], s[e + 2 * i + 1]);
-#pragma unroll
-      for (int i = 0; i < 4; i++) mx[i] = fmaxf(mx[i], s[kKeys - 4 + i]);
-      const float m_block = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      const float m_block = max_of<kKeys>(s, mx) * a.scale_log2;
       float corr = 1.f;
       if (m_block > m_used + Probability<BF16>::kGrow) {
         corr = exp2_approx(m_used - m_block);  // 0 the first time
@@ -330,19 +324,9 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
       const float shift = m_used == -INFINITY ? 0.f : Probability<BF16>::kLift - m_used;
       float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < kKeys / 64; c++) {
-        float packed[32];
-#pragma unroll
-        for (int e = 0; e < 32; e++) {
-          const float x = exp2_approx(fmaf(s[c * 64 + 2 * e], a.scale_log2, shift));
-          const float y = exp2_approx(fmaf(s[c * 64 + 2 * e + 1], a.scale_log2, shift));
-          const uint32_t pair = pack_pair<BF16>(x, y);
-          add_pair<BF16>(pair, part[(2 * e) & 3], part[(2 * e + 1) & 3]);
-          packed[e] = __uint_as_float(pair);
-        }
-        tmem_store_32(s_addr + c * 32, packed);
-      }
+      for (int c = 0; c < kKeys / 64; c++) store_probabilities<BF16>(s + c * 64, a.scale_log2, shift, part, s_addr + c * 32);
       sum += (part[0] + part[1]) + (part[2] + part[3]);
+      if (!(m_block < INFINITY)) sum = NAN;  // a score of NaN or infinity, which not every way to 2^x passes on
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();

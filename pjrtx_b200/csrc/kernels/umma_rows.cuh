@@ -3,6 +3,7 @@
 
 #include <type_traits>
 
+#include "arith.cuh"
 #include "paged.cuh"
 #include "row_attention.cuh"
 #include "umma_attention.cuh"
@@ -17,10 +18,59 @@ namespace umma {
 template <bool BF16> struct Probability { static constexpr float kLift = 0.f, kGrow = 8.f; };
 template <> struct Probability<false> { static constexpr float kLift = 11.f, kGrow = 4.f; };
 
+// NaN where one of them is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float y;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
+}
+
+// The largest of a row's N scores; four chains.
+template <int N>
+__device__ __forceinline__ float max_of(const float* s, float (&mx)[4]) {
+#pragma unroll
+  for (int e = 0; e < N; e += 8)
+#pragma unroll
+    for (int i = 0; i < 4; i++) mx[i] = max3(mx[i], s[e + 2 * i], s[e + 2 * i + 1]);
+  return max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3]));
+}
+
+// 2^x of two numbers on the FMA units, x <= 127: x = n + f with the whole number n nearest to x (what adding 1.5 * 2^23 leaves in the
+// lowest bits), 2^f for |f| <= 1/2 by a polynomial of degree four whose largest relative error is the least possible with 1 at f = 0
+// (2^-18.4; its coefficients solve that linear programme), n added to the exponent. From -127 down the result is 0. The exponential unit gives 16
+// results a cycle and SM, so that a block of 128 x 128 keeps it busy for 1024 cycles, as long as its products take; the FMA units have
+// time left.
+__device__ __forceinline__ float2 exp2_by_fma(float2 x) {
+  const Pair magic = pair_of(12582912.f, 12582912.f), back = pair_of(-12582912.f, -12582912.f), minus = pair_of(-1.f, -1.f), one = pair_of(1.f, 1.f);
+  const Pair v = pair_of(fmaxf(x.x, -127.f), fmaxf(x.y, -127.f));
+  const Pair t = pair_add(v, magic);
+  const Pair f = pair_fma(pair_add(t, back), minus, v);
+  Pair y = pair_fma(f, pair_of(0.009585382416844368f, 0.009585382416844368f), pair_of(0.05590662732720375f, 0.05590662732720375f));
+  y = pair_fma(f, y, pair_of(0.24024038016796112f, 0.24024038016796112f));
+  y = pair_fma(f, y, pair_of(0.6931241750717163f, 0.6931241750717163f));
+  y = pair_fma(f, y, one);
+  const float2 r = pair_split(y), n = pair_split(t);
+  return make_float2(__uint_as_float((__float_as_uint(n.x) << 23) + __float_as_uint(r.x)),
+                     __uint_as_float((__float_as_uint(n.y) << 23) + __float_as_uint(r.y)));
+}
+
+// Of every eight pairs of scores, how many go that way.
+constexpr int kByFma = 2;
+
+// Probabilities 2^(s * scale + shift) of 64 scores into 32 columns of tensor memory, as pairs of the element type; `part` adds them up.
+template <bool BF16>
+__device__ __forceinline__ void store_probabilities(const float* s, float scale, float shift, float (&part)[4], uint32_t to) {
+  const Pair scale2 = pair_of(scale, scale), shift2 = pair_of(shift, shift);
+  float packed[32];
+#pragma unroll
+  for (int e = 0; e < 32; e++) {
+    const float2 x = pair_split(pair_fma(pair_of(s[2 * e], s[2 * e + 1]), scale2, shift2));
+    const float2 y = e % 8 >= 8 - kByFma ? exp2_by_fma(x) : make_float2(exp2_approx(x.x), exp2_approx(x.y));
+    const uint32_t pair = pack_pair<BF16>(y.x, y.y);
+    add_pair<BF16>(pair, part[(2 * e) & 3], part[(2 * e + 1) & 3]);
+    packed[e] = __uint_as_float(pair);
+  }
+  tmem_store_32(to, packed);
 }
 template <int REGISTERS>
 __device__ __forceinline__ void take_registers() {
@@ -35,6 +85,32 @@ template <bool BF16>
 __device__ __forceinline__ bool odd_pair(uint32_t w) {
   constexpr uint32_t kExponent = BF16 ? 0x7f80u : 0x7c00u;
   return (w & kExponent) == kExponent || (w >> 16 & kExponent) == kExponent;
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// A map of `rank` axes, head_dim first, for boxes of 64 elements; `strides` (elements) are those of the axes behind the first. An axis of
+// one element may come with any stride, which the encoder does not take.
+inline bool encode_map(CUtensorMap* map, const void* base, bool f16, int rank, const long long* extents, const long long* strides, const int* box) {
+  static const EncodeTiledFn encode = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess) f = nullptr;
+    return (EncodeTiledFn)f;
+  }();
+  if (!encode) return false;
+  cuuint64_t dims[4], bytes[3];
+  cuuint32_t boxes[4], steps[4];
+  for (int d = 0; d < rank; d++) {
+    dims[d] = (cuuint64_t)extents[d];
+    boxes[d] = (cuuint32_t)box[d];
+    steps[d] = 1;
+    if (d) bytes[d - 1] = (cuuint64_t)(extents[d] == 1 ? extents[0] : strides[d - 1]) * 2;
+  }
+  return encode(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), dims, bytes,
+                boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace umma

@@ -2,9 +2,10 @@
 //
 // A block of threads goes through its share as one row of steps, a step being a block of keys of a segment, and nothing drains between
 // segments: rows of the next one are fetched while the last ones of this are at work.
-//   loader warps   two; queries of a segment, then keys and values of the steps into a ring of shared-memory slots, by cp.async: a row
-//                  of a page is the longest run that is contiguous whatever the layout. Rows are written in the 128-byte swizzle that the
-//                  tensor core reads, and handed over some slots later, when they have landed
+//   loader warps   two; queries of a segment, then keys and values of the steps into a ring of shared-memory slots, in the 128-byte
+//                  swizzle that the tensor core reads. Blocks of cached rows come by tensor-map copies of a page's rows, where pages are
+//                  8, 16, 32 or a multiple of 64 rows; the last rows, nodes, and pages of other sizes by cp.async, a row at a time,
+//                  each thread's copies counting themselves in on the slot's barrier when they have landed
 //   MMA warp       S = Q . K^T, O += P . V with P in tensor memory. With one tile of 128 query rows the scores have two buffers, so
 //                  that those of the next step are there when the softmax warps are done; with two tiles these take turns
 //   softmax warps  four a tile, a query row a thread; those whose rows are not there only count along
@@ -12,8 +13,8 @@
 // Bound by memory up to two tiles: 128 keys of 128 elements are 64 KB of keys and values, 2800 cycles of this SM's share of the memory, and
 // take 1024 cycles of tensor core and of exponentials for each tile.
 //
-// Hidden nodes have probability 0, and 0 times infinity or NaN is NaN on the tensor core. So a node with such a value goes into shared memory
-// as zeros, and rows that see it add their probability times its values when they take their results out. Rounding and the lazily
+// Hidden nodes have probability 0, and 0 times infinity or NaN is NaN on the tensor core. So a node with such a value is cleared in shared
+// memory (one more warp, the checker, looks at the nodes' values where they have landed), and rows that see it add their probability times its values when they take their results out. Rounding and the lazily
 // followed maximum: umma_rows.cuh.
 #pragma once
 
@@ -22,7 +23,7 @@
 namespace pjrtx {
 namespace umma {
 
-constexpr int kTreeLoaders = 2, kOddRing = 16;
+constexpr int kTreeLoaders = 2, kOddRing = 16, kCleanRing = 16;  // rings are longer than a checker can be ahead: its slots are
 __host__ __device__ constexpr int tree_keys(int hd) { return hd == 256 ? 64 : 128; }
 __host__ __device__ constexpr int tree_slot_bytes(int hd) { return tree_keys(hd) * hd * 2; }
 __host__ __device__ constexpr int tree_query_buffers(int hd, int tiles) { return tiles == 1 && hd <= 128 ? 2 : 1; }
@@ -38,23 +39,26 @@ __host__ __device__ constexpr size_t tree_smem(int hd, int tiles) {
   const size_t least = least_smem(512);
   return bytes < least ? least : bytes;
 }
-// Four softmax warps a tile, the loaders, the warp that issues, and one that has nothing to do: eight or twelve, which divide the registers evenly.
+// Four softmax warps a tile, the loaders, the warp that issues, and the checker: eight or twelve, which divide the registers evenly.
 __host__ __device__ constexpr int tree_threads(int tiles) { return 128 * tiles + 128; }
 
 struct TreeKernelArgs {
   TreeArgs p;
   float scale_log2, sign;  // scale: |scale| * log2(e), 1 where it is zero, and its sign, by which scores are multiplied first
   unsigned long long timeout_ns;
+  int box;  // rows of a page that a tensor-map copy takes, a multiple of eight; 0: rows are copied one by one
 };
+
+// Rows of a box: as many as a page has, at most a loader's part of a block; 0 where blocks are not made of such.
+inline int tree_box(int hd, int page_size) {
+  const int most = tree_keys(hd) / kTreeLoaders;
+  const int box = page_size < most ? page_size : most;
+  return box % 8 == 0 && most % box == 0 && page_size % box == 0 ? box : 0;
+}
 
 __device__ __forceinline__ void row_copy16(uint32_t to, unsigned long long from, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
-template <int N>
-__device__ __forceinline__ void row_copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // Of keys key0 + 32 w .. + 31, those that a row sees.
 __device__ __forceinline__ unsigned seen_word(int key0, int length, unsigned long long bits) {
   const int below = length - key0;  // cached rows among them and behind
@@ -79,7 +83,7 @@ __device__ __noinline__ float node_probability(const TreeKernelArgs& a, const un
 }
 
 template <bool BF16, int HD, int TILES>
-__global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const __grid_constant__ TreeKernelArgs a) {
+__global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const __grid_constant__ TreeKernelArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   constexpr int kThreads = tree_threads(TILES), kKeys = tree_keys(HD), kSlots = tree_slots(HD, TILES);
   constexpr int kBuffers = TILES == 1 ? 2 : 1;  // of scores, a tile
   constexpr int kQueries = tree_query_buffers(HD, TILES);
@@ -91,8 +95,9 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
     uint64_t q_full[kQueries], q_empty[kQueries], slot_full[kSlots], slot_empty[kSlots];
     uint64_t s_full[TILES][kBuffers];   // the step's scores are in tensor memory, and the products two uses back are done
     uint64_t p_ready[TILES][kBuffers];  // its probabilities are
+    uint64_t clean[kCleanRing];         // nodes with values that are infinite or NaN have been cleared in the slot
     uint64_t odd_ready[kOddRing];       // of a segment
-    unsigned long long odd[kOddRing][kTreeLoaders];  // nodes with values that are infinite or NaN
+    unsigned long long odd[kOddRing];   // which nodes these are
     uint32_t tmem;
     int abort;
     ShareSpace<kThreads> share;
@@ -109,22 +114,22 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const TreeArgs& p = a.p;
   if (threadIdx.x == 0) p.cuts[blockIdx.x] = {0, 0, 0, 0};
-  check_sequences(p);
   if (threadIdx.x == 0) {
     for (int i = 0; i < kQueries; i++) {
-      mbar_init(&bar.q_full[i], kTreeLoaders);
+      mbar_init(&bar.q_full[i], kTreeLoaders * 32);
       mbar_init(&bar.q_empty[i], 1);
     }
     for (int i = 0; i < kSlots; i++) {
-      mbar_init(&bar.slot_full[i], kTreeLoaders);
-      mbar_init(&bar.slot_empty[i], 1);
+      mbar_init(&bar.slot_full[i], kTreeLoaders * 32);
+      mbar_init(&bar.slot_empty[i], 2);  // the products, and the checker: it sees every use of a slot, or could take one for another
     }
     for (int t = 0; t < TILES; t++)
       for (int i = 0; i < kBuffers; i++) {
         mbar_init(&bar.s_full[t][i], 1);
         mbar_init(&bar.p_ready[t][i], 4);
       }
-    for (int i = 0; i < kOddRing; i++) mbar_init(&bar.odd_ready[i], kTreeLoaders);
+    for (int i = 0; i < kCleanRing; i++) mbar_init(&bar.clean[i], 1);
+    for (int i = 0; i < kOddRing; i++) mbar_init(&bar.odd_ready[i], 1);
     bar.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -144,55 +149,51 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
   WaitBudget budget{global_timer_ns() + a.timeout_ns, &bar.abort};  // renewed with every segment
   auto renew = [&]() { budget.deadline = global_timer_ns() + a.timeout_ns; };
   auto wait = [&](uint64_t* b, unsigned parity) { return __all_sync(0xffffffffu, mbar_wait(b, parity, budget)) != 0; };
+  auto has_nodes = [&](const Cursor& u) { return (u.tile + 1) * kKeys > u.s.length; };
 
   if (warp >= kFirstLoader && warp < kMmaWarp) {
     const int lw = warp - kFirstLoader;
-    constexpr int kLag = kSlots - 2;  // copies under way, in groups
+    const bool leader = elect_one();
     constexpr int kPieces = HD / 8, kAcross = 32 / kPieces, kRowsOfWarp = kKeys / kTreeLoaders, kRowsOfLane = kRowsOfWarp / 32;
-    uint32_t pending[kLag];  // barriers of the groups that have not been handed over, the oldest first
-#pragma unroll
-    for (int i = 0; i < kLag; i++) pending[i] = 0;
-    auto hand_over = [&](uint32_t b) {
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (b && lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(b) : "memory");
+    // Counts this thread in once its copies so far have landed.
+    auto arrive_when_landed = [&](uint64_t* b) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(b)) : "memory"); };
+    // Page ids of this warp's part of a block, fetched a step before they are looked at: of rows `lane`, `lane + 32`, .. or, for blocks of
+    // nothing but cached rows whose pages are made of boxes, of the boxes, the same in all lanes.
+    constexpr int kBoxes = kRowsOfWarp / 8;  // at most
+    struct Pages {
+      int of_row[kRowsOfLane], of_box[kBoxes];
     };
-    auto commit = [&](uint64_t* b) {
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      row_copies_wait<kLag>();
-      hand_over(pending[0]);
+    auto first_key = [&](const Cursor& u) { return u.tile * kKeys + lw * kRowsOfWarp; };
+    auto whole = [&](const Cursor& u) { return a.box > 0 && first_key(u) + kRowsOfWarp <= u.s.length; };
+    auto fetch = [&](const Cursor& u, Pages& k) {
+      const int* table = p.c.table + u.b * p.c.table_stride;
+      if (whole(u)) {
 #pragma unroll
-      for (int i = 0; i + 1 < kLag; i++) pending[i] = pending[i + 1];
-      pending[kLag - 1] = smem_u32(b);
-    };
-    auto drain = [&]() {
-      row_copies_wait<0>();
+        for (int i = 0; i < kBoxes; i++)
+          if (i * a.box < kRowsOfWarp) k.of_box[i] = table[column_of(p, first_key(u) + i * a.box)];
+      } else {
 #pragma unroll
-      for (int i = 0; i < kLag; i++) {
-        hand_over(pending[i]);
-        pending[i] = 0;
+        for (int i = 0; i < kRowsOfLane; i++) {
+          const int t = first_key(u) + i * 32 + lane;
+          k.of_row[i] = t < u.s.length ? table[column_of(p, t)] : 0;
+        }
       }
     };
-    // Address of the key of row `lane` of the warp's i-th 32 in the step's block: bit 0 marks a node, 0 stands for none.
-    auto locate_row = [&](const Cursor& u, int g, int i) -> unsigned long long {
-      const int t = u.tile * kKeys + lw * kRowsOfWarp + i * 32 + lane;
+    // Address of the key of row `lane` of the i-th 32: bit 0 marks a node, 0 stands for none.
+    auto locate = [&](const Cursor& u, int g, const Pages& k, int i) -> unsigned long long {
+      const int t = first_key(u) + i * 32 + lane;
       if (t < u.s.length) {
-        const long long row = cached_row(p, u.b, t);
-        return row < 0 ? 0ull : (unsigned long long)(static_cast<const unsigned short*>(p.c.k) + row + g * p.c.head_stride);
+        if (k.of_row[i] < 0 || k.of_row[i] >= p.c.num_pages) {
+          report(p.c.error_words, kErrorPageId);
+          return 0ull;
+        }
+        return (unsigned long long)(static_cast<const unsigned short*>(p.c.k) + k.of_row[i] * p.c.page_stride +
+                                    (t - column_of(p, t) * p.c.page_size) * p.c.row_stride + g * p.c.head_stride);
       }
       const int node = t - u.s.length;
       if (node >= u.s.count) return 0ull;
       return (unsigned long long)(static_cast<const unsigned short*>(p.a.k_new) + u.b * p.a.new_batch_stride + node * p.a.new_node_stride +
                                   g * p.a.new_head_stride) | 1ull;
-    };
-    struct Keys {
-      unsigned long long at[kRowsOfLane];
-    };
-    auto locate = [&](const Cursor& u, int g) {
-      Keys k;
-#pragma unroll
-      for (int i = 0; i < kRowsOfLane; i++) k.at[i] = locate_row(u, g, i);
-      return k;
     };
     const unsigned long long apart = (unsigned long long)p.c.v - (unsigned long long)p.c.k;
     const unsigned long long apart_new = (unsigned long long)p.a.v_new - (unsigned long long)p.a.k_new;
@@ -206,102 +207,131 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
       *at = ring + (uint32_t)slot * kSlotBytes;
       return true;
     };
-    auto next_slot = [&]() {
-      commit(&bar.slot_full[slot]);
+    auto advance_slot = [&]() {
       if (++slot == kSlots) {
         slot = 0;
         phase ^= 1;
       }
     };
-    auto place = [&](uint32_t at, int row) { return at + (uint32_t)(piece / 8) * kKeyBlock + (uint32_t)row * 128u + (uint32_t)(((piece & 7) ^ (row & 7)) << 4); };
-    auto load_keys = [&](const Keys& key) {
-      uint32_t at;
-      if (!take_slot(&at)) return false;
+    // Row `lw * kRowsOfWarp + i * 32 + j * kAcross + lane / kPieces` of a slot: what goes by the lane repeats every 8 / kAcross rows.
+    constexpr int kTurns = kAcross >= 8 ? 1 : 8 / kAcross;
+    uint32_t corner[kTurns];
 #pragma unroll
-      for (int i = 0; i < kRowsOfLane; i++)
-#pragma unroll 4
-        for (int j = 0; j < 32 / kAcross; j++) {
-          const int r = j * kAcross + lane / kPieces;
-          const unsigned long long from = __shfl_sync(~0u, key.at[i], r) & ~1ull;
-          row_copy16(place(at, lw * kRowsOfWarp + i * 32 + r), from && inside ? from + piece * 16 : (unsigned long long)p.c.k, from && inside);
-        }
-      next_slot();
-      return true;
-    };
-    unsigned long long odd = 0;
-    auto load_values = [&](const Keys& key, const Cursor& u) {
-      uint32_t at;
-      if (!take_slot(&at)) return false;
+    for (int j = 0; j < kTurns; j++) {
+      const int row = j * kAcross + lane / kPieces;
+      corner[j] = (uint32_t)(piece / 8) * kKeyBlock + (uint32_t)(lw * kRowsOfWarp + lane / kPieces) * 128u + (uint32_t)(((piece & 7) ^ (row & 7)) << 4);
+    }
+    auto place = [&](uint32_t at, int i, int j) { return at + corner[j % kTurns] + (uint32_t)(i * 32 + j * kAcross) * 128u; };
+    // A page outside the pool: a box of nothing, which the copy fills with zeros.
+    auto load_boxes = [&](const CUtensorMap* map, const Cursor& u, int g, const Pages& k, uint32_t at) {
+      if (leader) mbar_expect_tx(&bar.slot_full[slot], kRowsOfWarp * HD * 2);
+      __syncwarp();
+      const uint32_t to = at + (uint32_t)(lw * kRowsOfWarp) * 128u;
+      const int t = first_key(u), row = t - column_of(p, t) * p.c.page_size;  // 0 where a page has no more than a box
 #pragma unroll
-      for (int i = 0; i < kRowsOfLane; i++) {
-        const bool nodes = __any_sync(~0u, key.at[i] & 1);
-#pragma unroll 4
-        for (int j = 0; j < 32 / kAcross; j++) {
-          const int r = j * kAcross + lane / kPieces, row = lw * kRowsOfWarp + i * 32 + r;
-          unsigned long long from = __shfl_sync(~0u, key.at[i], r);
-          const bool node = from & 1, there = from && inside;
-          from = (from & ~1ull) + (node ? apart_new : apart) + piece * 16;
-          if (!nodes) {
-            row_copy16(place(at, row), there ? from : (unsigned long long)p.c.v, there);
-            continue;
-          }
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (there) x = *reinterpret_cast<const uint4*>(from);
-          const bool bad = node && (odd_pair<BF16>(x.x) || odd_pair<BF16>(x.y) || odd_pair<BF16>(x.z) || odd_pair<BF16>(x.w));
-          // Whether any lane of the row has found one.
-          const unsigned found = __ballot_sync(~0u, bad) >> (lane / kPieces * kPieces) & (unsigned)((1ull << kPieces) - 1);
-          if (found) {
-            x = make_uint4(0, 0, 0, 0);
-            odd |= 1ull << (u.tile * kKeys + row - u.s.length);
-          }
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place(at, row)), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+      for (int i = 0; i < kBoxes; i++) {
+        if (i * a.box >= kRowsOfWarp) break;
+        const int page = k.of_box[i];
+        const bool valid = page >= 0 && page < p.c.num_pages;
+        if (leader) {
+          if (!valid) report(p.c.error_words, kErrorPageId);
+#pragma unroll
+          for (int c = 0; c < HD / 64; c++)
+            tma_load_4d(to + (uint32_t)c * kKeyBlock + (uint32_t)(i * a.box) * 128u, map, c * 64, row, g, valid ? page : (int)p.c.num_pages,
+                        &bar.slot_full[slot]);
         }
       }
-      next_slot();
+      __syncwarp();
+      if (!leader) mbar_arrive(&bar.slot_full[slot]);
+      advance_slot();
+    };
+    auto load_keys = [&](const Cursor& u, int g, const Pages& k) {
+      uint32_t at;
+      if (!take_slot(&at)) return false;
+      if (whole(u)) {
+        load_boxes(&kmap, u, g, k, at);
+        return true;
+      }
+#pragma unroll
+      for (int i = 0; i < kRowsOfLane; i++) {
+        const unsigned long long key = locate(u, g, k, i);
+#pragma unroll
+        for (int j = 0; j < 32 / kAcross; j++) {
+          const unsigned long long from = __shfl_sync(~0u, key, j * kAcross + lane / kPieces) & ~1ull;
+          row_copy16(place(at, i, j), from && inside ? from + piece * 16 : (unsigned long long)p.c.k, from && inside);
+        }
+      }
+      arrive_when_landed(&bar.slot_full[slot]);
+      advance_slot();
+      return true;
+    };
+    auto load_values = [&](const Cursor& u, int g, const Pages& k) {
+      uint32_t at;
+      if (!take_slot(&at)) return false;
+      if (whole(u)) {
+        load_boxes(&vmap, u, g, k, at);
+        return true;
+      }
+#pragma unroll
+      for (int i = 0; i < kRowsOfLane; i++) {
+        const unsigned long long key = locate(u, g, k, i);
+        const unsigned long long value = key == 0 ? 0 : (key & ~1ull) + (key & 1 ? apart_new : apart);
+#pragma unroll
+        for (int j = 0; j < 32 / kAcross; j++) {
+          const unsigned long long from = __shfl_sync(~0u, value, j * kAcross + lane / kPieces);
+          row_copy16(place(at, i, j), from && inside ? from + piece * 16 : (unsigned long long)p.c.v, from && inside);
+        }
+      }
+      arrive_when_landed(&bar.slot_full[slot]);
+      advance_slot();
       return true;
     };
     auto load_queries = [&](const Segment& seg, long long number) {
       const int buffer = (int)(number % kQueries);
-      if (number >= kQueries) {
-        drain();  // the products that the buffer waits for may need what is under way
-        if (!wait(&bar.q_empty[buffer], (unsigned)(number / kQueries - 1) & 1u)) return false;
-      }
+      if (number >= kQueries && !wait(&bar.q_empty[buffer], (unsigned)(number / kQueries - 1) & 1u)) return false;
       const uint32_t at = base + buffer * kQueryBytes;
       constexpr int kEach = TILES * kAttnRows / kTreeLoaders;
-      for (int j = 0; j < kEach / kAcross; j++) {
-        const int r = lw * kEach + j * kAcross + lane / kPieces, tile = r / kAttnRows, row = r % kAttnRows;
+#pragma unroll 1
+      for (int i = 0; i < kEach; i += 32) {
+        const int r0 = lw * kEach + i, tile = r0 / kAttnRows;
         int node, head;
-        const bool there = seg.place(p, r, &node, &head) && inside;
-        const unsigned short* from = static_cast<const unsigned short*>(p.a.q);
-        if (there) from += query_at(p, seg, node, head) + piece * 8;
-        row_copy16(at + tile * kTileBytes + (uint32_t)(piece / 8) * kQueryBlock + (uint32_t)row * 128u + (uint32_t)(((piece & 7) ^ (row & 7)) << 4),
-                   (unsigned long long)from, there);
+        unsigned long long row = 0;
+        if (seg.place(p, r0 + lane, &node, &head))
+          row = (unsigned long long)(static_cast<const unsigned short*>(p.a.q) + query_at(p, seg, node, head));
+        const uint32_t to = at + tile * kTileBytes + (uint32_t)(piece / 8) * kQueryBlock + (uint32_t)(r0 % kAttnRows + lane / kPieces) * 128u;
+#pragma unroll
+        for (int j = 0; j < 32 / kAcross; j++) {
+          const unsigned long long from = __shfl_sync(~0u, row, j * kAcross + lane / kPieces);
+          row_copy16(to + (uint32_t)(j * kAcross) * 128u + (uint32_t)(((piece & 7) ^ ((j * kAcross + lane / kPieces) & 7)) << 4),
+                     from && inside ? from + piece * 16 : (unsigned long long)p.a.q, from && inside);
+        }
       }
-      commit(&bar.q_full[buffer]);
+      arrive_when_landed(&bar.q_full[buffer]);
       return true;
     };
     if (work) {
       // Keys run `kBuffers` steps ahead of the values, as the products do.
       Cursor key_at = share.at, value_at = share.at;
-      long long key_number = share.first, value_number = share.first, segments = 0, value_segment = 0;
+      long long key_number = share.first, value_number = share.first, segments = 0;
       bool keys_left = true, ok = true, fresh = true;
-      Keys place_of[kBuffers + 1];  // keys of the steps whose values are still to come
-      int g = segment_of(p, key_at.b, key_at.group, key_at.s.count).g;
-      Keys next = locate(key_at, g);
+      Pages pages[kBuffers + 1];  // of the steps whose values are still to come
+      int g = segment_of(p, key_at.b, key_at.group, key_at.s.count).g, value_g = g;
+      Pages next;
+      fetch(key_at, next);
       auto step_keys = [&](int into) {
         if (fresh) {
           renew();
           ok = load_queries(segment_of(p, key_at.b, key_at.group, key_at.s.count), segments++);
           if (!ok) return;
         }
-        place_of[into] = next;
-        ok = load_keys(next);
+        pages[into] = next;
+        ok = load_keys(key_at, g, next);
         const int b = key_at.b, group = key_at.group;
         keys_left = next_unit(p, key_at, key_number, share.size);
         fresh = key_at.b != b || key_at.group != group;
         if (keys_left) {
           if (fresh) g = segment_of(p, key_at.b, key_at.group, key_at.s.count).g;
-          next = locate(key_at, g);
+          fetch(key_at, next);
         }
       };
       int ahead = 0;
@@ -312,29 +342,24 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
           ahead++;
         }
       while (ok && ahead > 0) {
-        ok = load_values(place_of[0], value_at);
+        ok = load_values(value_at, value_g, pages[0]);
         if (!ok) break;
-        const Cursor here = value_at;
-        const bool more = next_unit(p, value_at, value_number, share.size);
-        if (!more || value_at.b != here.b || value_at.group != here.group) {
-          odd |= __shfl_xor_sync(~0u, odd, 16);  // lanes of different rows
-          if (kPieces <= 8) odd |= __shfl_xor_sync(~0u, odd, 8);
-          if (lane == 0) {
-            bar.odd[value_segment % kOddRing][lw] = odd;
-            mbar_arrive(&bar.odd_ready[value_segment % kOddRing]);
-          }
-          value_segment++;
-          odd = 0;
-        }
+        const int b = value_at.b, group = value_at.group;
+        if (next_unit(p, value_at, value_number, share.size) && (value_at.b != b || value_at.group != group))
+          value_g = segment_of(p, value_at.b, value_at.group, value_at.s.count).g;
 #pragma unroll
-        for (int i = 0; i + 1 < kBuffers; i++) place_of[i] = place_of[i + 1];
+        for (int i = 0; i + 1 < kBuffers; i++) pages[i] = pages[i + 1];
         ahead--;
         if (keys_left) {
           step_keys(kBuffers - 1);
           ahead++;
         }
       }
-      drain();
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      // Given up: the boxes under way get a bounded time to land before the block of threads leaves.
+      for (long long u = used - 1; !ok && u >= 0 && u >= used - kSlots; u--)
+        for (unsigned spin = 0; spin < (1u << 14) && !mbar_try_wait(&bar.slot_full[u % kSlots], (unsigned)(u / kSlots) & 1u); spin++) {
+        }
     }
   } else if (warp == kMmaWarp) {
     const bool leader = elect_one();
@@ -390,6 +415,7 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
         if (ok && left) {
           scores_wait();
           if (!ok) break;
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the copies are seen by the threads' own accesses first
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           if (leader)
             for (int t = 0; t < TILES; t++) {
@@ -400,12 +426,18 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
           scores_done();
         }
       bool first = true;
+      long long checked = 0;
       for (long long step = 0; ok; step++) {
         const int buffer = (int)(step % kBuffers), v_slot = slot;
         ok = wait(&bar.slot_full[slot], phase);
         next_slot();
         const bool more = left;
         if (more) scores_wait();
+        if (has_nodes(now)) {
+          ok = ok && wait(&bar.clean[checked % kCleanRing], (unsigned)(checked / kCleanRing) & 1u);
+          checked++;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 #pragma unroll
         for (int t = 0; t < TILES; t++) {
           ok = ok && wait(&bar.p_ready[t][buffer], (unsigned)(step / kBuffers) & 1u);
@@ -431,6 +463,74 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
       }
       if (!ok && leader) report(p.c.error_words, kErrorWait);
       __syncwarp();
+    }
+  } else if (warp == kMmaWarp + 1) {
+    // The checker: looks at the values of nodes where they have landed.
+    Cursor now = share.at;
+    long long number = share.first, used = 0, checked = 0, segments = 0;
+    unsigned long long odd = 0;
+    bool left = work, more_keys = true, fresh = true;
+    // Slots in the order in which they are used: `kBuffers` steps of keys, then a step's values and the keys `kBuffers` further on.
+    Cursor ahead = share.at;
+    long long ahead_number = share.first;
+    bool ok = true;
+    auto next_use = [&]() {
+      const int slot = (int)(used % kSlots);
+      ok = ok && wait(&bar.slot_full[slot], (unsigned)(used / kSlots) & 1u);
+      used++;
+      return slot;
+    };
+    auto pass = [&](int slot) {
+      if (ok && lane == 0) mbar_arrive(&bar.slot_empty[slot]);
+    };
+    auto pass_keys = [&]() {
+      pass(next_use());
+      more_keys = next_unit(p, ahead, ahead_number, share.size);
+    };
+    for (int i = 0; i < kBuffers && left && more_keys; i++) pass_keys();
+    while (left && ok) {
+      if (fresh) renew();
+      const int slot = next_use();
+      if (ok && has_nodes(now)) {
+        const int from = max(0, now.s.length - now.tile * kKeys), to = min(kKeys, now.s.length + now.s.count - now.tile * kKeys);
+        unsigned char* rows0 = base_ptr + kQueries * kQueryBytes + slot * kSlotBytes;
+        constexpr int kPieces = HD / 8, kAcross = 32 / kPieces;
+        const int piece = lane % kPieces;
+#pragma unroll 4
+        for (int r0 = from; r0 < to; r0 += kAcross) {
+          const int r = r0 + lane / kPieces;
+          uint4* const at = reinterpret_cast<uint4*>(rows0 + (piece / 8) * kKeyBlock + r * 128 + (((piece & 7) ^ (r & 7)) << 4));
+          bool bad = false;
+          if (r < to) {
+            const uint4 x = *at;
+            bad = odd_pair<BF16>(x.x) || odd_pair<BF16>(x.y) || odd_pair<BF16>(x.z) || odd_pair<BF16>(x.w);
+          }
+          // Whether any lane of the row has found one.
+          if (__ballot_sync(~0u, bad) >> (lane / kPieces * kPieces) & (unsigned)((1ull << kPieces) - 1)) {
+            *at = make_uint4(0, 0, 0, 0);
+            odd |= 1ull << (now.tile * kKeys + r - now.s.length);
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.clean[checked % kCleanRing]);
+        checked++;
+      }
+      pass(slot);
+      if (more_keys) pass_keys();
+      const int b = now.b, group = now.group;
+      left = next_unit(p, now, number, share.size);
+      fresh = !left || now.b != b || now.group != group;
+      if (fresh) {
+        odd |= __shfl_xor_sync(~0u, odd, 16);  // lanes of different rows
+        odd |= __shfl_xor_sync(~0u, odd, 8);
+        if (lane == 0) {
+          bar.odd[segments % kOddRing] = odd;
+          mbar_arrive(&bar.odd_ready[segments % kOddRing]);
+        }
+        segments++;
+        odd = 0;
+      }
     }
   } else if (warp < kFirstLoader) {
     const int t = warp >> 2;
@@ -485,16 +585,13 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
               }
             }
           };
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, m_block = -INFINITY;
 #pragma unroll 1
           for (int c = 0; c < kKeys / kChunk; c++) {
             load(c);
-#pragma unroll
-            for (int e = 0; e < kChunk; e += 8)
-#pragma unroll
-              for (int i = 0; i < 4; i++) mx[i] = max3(mx[i], s[e + 2 * i], s[e + 2 * i + 1]);
+            m_block = max_of<kChunk>(s, mx);
           }
-          const float m_block = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+          m_block *= a.scale_log2;
           float corr = 1.f;
           if (m_block > m_used + Probability<BF16>::kGrow) {
             corr = exp2_approx(m_used - m_block);  // 0 the first time
@@ -522,20 +619,11 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
           for (int c = 0; c < kKeys / kChunk; c++) {
             if (kChunk < kKeys) load(c);
 #pragma unroll
-            for (int h = 0; h < kChunk / 64; h++) {
-              float packed[32];
-#pragma unroll
-              for (int e = 0; e < 32; e++) {
-                const float x = exp2_approx(fmaf(s[h * 64 + 2 * e], a.scale_log2, shift));
-                const float y = exp2_approx(fmaf(s[h * 64 + 2 * e + 1], a.scale_log2, shift));
-                const uint32_t pair = pack_pair<BF16>(x, y);
-                add_pair<BF16>(pair, part[(2 * e) & 3], part[(2 * e + 1) & 3]);
-                packed[e] = __uint_as_float(pair);
-              }
-              tmem_store_32(s_addr + (c * kChunk / 64 + h) * 32, packed);
-            }
+            for (int h = 0; h < kChunk / 64; h++)
+              store_probabilities<BF16>(s + h * 64, a.scale_log2, shift, part, s_addr + (c * kChunk / 64 + h) * 32);
           }
           sum += (part[0] + part[1]) + (part[2] + part[3]);
+          if (!(m_block < INFINITY)) sum = NAN;  // a score of NaN or infinity, which not every way to 2^x passes on
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         }
@@ -552,9 +640,7 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
       float* part = part_of(p, share, here, segment);
       if (!active) continue;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      unsigned long long odd = 0;
-      for (int i = 0; i < kTreeLoaders; i++) odd |= bar.odd[segments % kOddRing][i];
-      odd &= bits;
+      const unsigned long long odd = bar.odd[segments % kOddRing] & bits;
       const float m = m_used - Probability<BF16>::kLift;  // what the sums are relative to
       const float shift = m_used == -INFINITY ? 0.f : -m;
       const float inverse = part ? 1.f : rows::inverse_of(sum);
@@ -577,8 +663,7 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
         }
         if (part) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<float4*>(part + row * HD + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          for (int e = 0; e < 32; e++) part[(c + e) * p.slot_rows + row] = o[e];
         } else {
 #pragma unroll
           for (int e = 0; e < 32; e += 8)
@@ -589,7 +674,7 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
         }
       }
       if (!there) continue;
-      if (part) *reinterpret_cast<float2*>(part + p.slot_rows * HD + 2 * row) = make_float2(m, sum);
+      if (part) store_statistics(p, part, row, m, sum);
       else if (p.a.lse) p.a.lse[lse_at(p, seg, node, head)] = sum == 0.f ? -INFINITY : fmaf(m, rows::kLn2, logf(sum));
     }
     if (!ok && lane == 0) report(p.c.error_words, kErrorWait);
