@@ -59,6 +59,11 @@ inline int tree_box(int hd, int page_size) {
 __device__ __forceinline__ void row_copy16(uint32_t to, unsigned long long from, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
+// A whole warp's wait. One for all places: see the loops of the loaders.
+__device__ __noinline__ bool warp_wait(uint64_t* bar, unsigned parity, unsigned long long deadline, volatile int* abort) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, WaitBudget{deadline, abort})) != 0;
+}
+
 // Of keys key0 + 32 w .. + 31, those that a row sees.
 __device__ __forceinline__ unsigned seen_word(int key0, int length, unsigned long long bits) {
   const int below = length - key0;  // cached rows among them and behind
@@ -148,7 +153,7 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
   auto o_col = [&](int t) { return tmem_base + (uint32_t)(TILES * kBuffers * kKeys + t * HD); };
   WaitBudget budget{global_timer_ns() + a.timeout_ns, &bar.abort};  // renewed with every segment
   auto renew = [&]() { budget.deadline = global_timer_ns() + a.timeout_ns; };
-  auto wait = [&](uint64_t* b, unsigned parity) { return __all_sync(0xffffffffu, mbar_wait(b, parity, budget)) != 0; };
+  auto wait = [&](uint64_t* b, unsigned parity) { return warp_wait(b, parity, budget.deadline, budget.abort); };
   auto has_nodes = [&](const Cursor& u) { return (u.tile + 1) * kKeys > u.s.length; };
 
   if (warp >= kFirstLoader && warp < kMmaWarp) {
@@ -157,37 +162,30 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
     constexpr int kPieces = HD / 8, kAcross = 32 / kPieces, kRowsOfWarp = kKeys / kTreeLoaders, kRowsOfLane = kRowsOfWarp / 32;
     // Counts this thread in once its copies so far have landed.
     auto arrive_when_landed = [&](uint64_t* b) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(b)) : "memory"); };
-    // Page ids of this warp's part of a block, fetched a step before they are looked at: of rows `lane`, `lane + 32`, .. or, for blocks of
-    // nothing but cached rows whose pages are made of boxes, of the boxes, the same in all lanes.
-    constexpr int kBoxes = kRowsOfWarp / 8;  // at most
+    // Page ids of this warp's part of a block, fetched a step before they are looked at: of rows `lane` and `lane + 32` or, for blocks of
+    // nothing but cached rows whose pages are made of boxes, of box `lane`.
     struct Pages {
-      int of_row[kRowsOfLane], of_box[kBoxes];
+      int low, high;
     };
     auto first_key = [&](const Cursor& u) { return u.tile * kKeys + lw * kRowsOfWarp; };
     auto whole = [&](const Cursor& u) { return a.box > 0 && first_key(u) + kRowsOfWarp <= u.s.length; };
-    auto fetch = [&](const Cursor& u, Pages& k) {
+    auto fetch = [&](const Cursor& u) {
       const int* table = p.c.table + u.b * p.c.table_stride;
-      if (whole(u)) {
-#pragma unroll
-        for (int i = 0; i < kBoxes; i++)
-          if (i * a.box < kRowsOfWarp) k.of_box[i] = table[column_of(p, first_key(u) + i * a.box)];
-      } else {
-#pragma unroll
-        for (int i = 0; i < kRowsOfLane; i++) {
-          const int t = first_key(u) + i * 32 + lane;
-          k.of_row[i] = t < u.s.length ? table[column_of(p, t)] : 0;
-        }
-      }
+      const int step = whole(u) ? a.box : 1, t = first_key(u) + lane * step, end = min(u.s.length, first_key(u) + kRowsOfWarp);
+      Pages k = {0, 0};
+      if (t < end) k.low = table[column_of(p, t)];
+      if (kRowsOfLane == 2 && step == 1 && t + 32 < end) k.high = table[column_of(p, t + 32)];
+      return k;
     };
     // Address of the key of row `lane` of the i-th 32: bit 0 marks a node, 0 stands for none.
     auto locate = [&](const Cursor& u, int g, const Pages& k, int i) -> unsigned long long {
-      const int t = first_key(u) + i * 32 + lane;
+      const int t = first_key(u) + i * 32 + lane, page = i ? k.high : k.low;
       if (t < u.s.length) {
-        if (k.of_row[i] < 0 || k.of_row[i] >= p.c.num_pages) {
+        if (page < 0 || page >= p.c.num_pages) {
           report(p.c.error_words, kErrorPageId);
           return 0ull;
         }
-        return (unsigned long long)(static_cast<const unsigned short*>(p.c.k) + k.of_row[i] * p.c.page_stride +
+        return (unsigned long long)(static_cast<const unsigned short*>(p.c.k) + page * p.c.page_stride +
                                     (t - column_of(p, t) * p.c.page_size) * p.c.row_stride + g * p.c.head_stride);
       }
       const int node = t - u.s.length;
@@ -213,25 +211,27 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
         phase ^= 1;
       }
     };
-    // Row `lw * kRowsOfWarp + i * 32 + j * kAcross + lane / kPieces` of a slot: what goes by the lane repeats every 8 / kAcross rows.
-    constexpr int kTurns = kAcross >= 8 ? 1 : 8 / kAcross;
-    uint32_t corner[kTurns];
-#pragma unroll
-    for (int j = 0; j < kTurns; j++) {
-      const int row = j * kAcross + lane / kPieces;
-      corner[j] = (uint32_t)(piece / 8) * kKeyBlock + (uint32_t)(lw * kRowsOfWarp + lane / kPieces) * 128u + (uint32_t)(((piece & 7) ^ (row & 7)) << 4);
-    }
-    auto place = [&](uint32_t at, int i, int j) { return at + corner[j % kTurns] + (uint32_t)(i * 32 + j * kAcross) * 128u; };
+    // Where this lane's piece of row `row` of a slot goes.
+    auto place = [&](uint32_t at, int row) { return at + (uint32_t)(piece / 8) * kKeyBlock + (uint32_t)row * 128u + (uint32_t)(((piece & 7) ^ (row & 7)) << 4); };
+    // 32 rows one by one, `from` being the address of row `lane`, 0: none. The loops are not unrolled: the code of all roles runs side by
+    // side, and what does not fit the instruction cache costs more than it saves (5.1 of a warp's 10 cycles an instruction before).
+    auto copy_rows = [&](unsigned long long row, uint32_t at, int row0, const void* any) {
+#pragma unroll 2
+      for (int j = 0; j < 32 / kAcross; j++) {
+        const int r = j * kAcross + lane / kPieces;
+        const unsigned long long from = __shfl_sync(~0u, row, r);
+        row_copy16(place(at, row0 + r), from && inside ? from + piece * 16 : (unsigned long long)any, from && inside);
+      }
+    };
     // A page outside the pool: a box of nothing, which the copy fills with zeros.
     auto load_boxes = [&](const CUtensorMap* map, const Cursor& u, int g, const Pages& k, uint32_t at) {
       if (leader) mbar_expect_tx(&bar.slot_full[slot], kRowsOfWarp * HD * 2);
       __syncwarp();
       const uint32_t to = at + (uint32_t)(lw * kRowsOfWarp) * 128u;
       const int t = first_key(u), row = t - column_of(p, t) * p.c.page_size;  // 0 where a page has no more than a box
-#pragma unroll
-      for (int i = 0; i < kBoxes; i++) {
-        if (i * a.box >= kRowsOfWarp) break;
-        const int page = k.of_box[i];
+#pragma unroll 1
+      for (int i = 0; i * a.box < kRowsOfWarp; i++) {
+        const int page = __shfl_sync(~0u, k.low, i);
         const bool valid = page >= 0 && page < p.c.num_pages;
         if (leader) {
           if (!valid) report(p.c.error_words, kErrorPageId);
@@ -245,42 +245,19 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
       if (!leader) mbar_arrive(&bar.slot_full[slot]);
       advance_slot();
     };
-    auto load_keys = [&](const Cursor& u, int g, const Pages& k) {
+    // Keys, or values.
+    auto load_block = [&](bool values, const Cursor& u, int g, const Pages& k) {
       uint32_t at;
       if (!take_slot(&at)) return false;
       if (whole(u)) {
-        load_boxes(&kmap, u, g, k, at);
+        load_boxes(values ? &vmap : &kmap, u, g, k, at);
         return true;
       }
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < kRowsOfLane; i++) {
-        const unsigned long long key = locate(u, g, k, i);
-#pragma unroll
-        for (int j = 0; j < 32 / kAcross; j++) {
-          const unsigned long long from = __shfl_sync(~0u, key, j * kAcross + lane / kPieces) & ~1ull;
-          row_copy16(place(at, i, j), from && inside ? from + piece * 16 : (unsigned long long)p.c.k, from && inside);
-        }
-      }
-      arrive_when_landed(&bar.slot_full[slot]);
-      advance_slot();
-      return true;
-    };
-    auto load_values = [&](const Cursor& u, int g, const Pages& k) {
-      uint32_t at;
-      if (!take_slot(&at)) return false;
-      if (whole(u)) {
-        load_boxes(&vmap, u, g, k, at);
-        return true;
-      }
-#pragma unroll
-      for (int i = 0; i < kRowsOfLane; i++) {
-        const unsigned long long key = locate(u, g, k, i);
-        const unsigned long long value = key == 0 ? 0 : (key & ~1ull) + (key & 1 ? apart_new : apart);
-#pragma unroll
-        for (int j = 0; j < 32 / kAcross; j++) {
-          const unsigned long long from = __shfl_sync(~0u, value, j * kAcross + lane / kPieces);
-          row_copy16(place(at, i, j), from && inside ? from + piece * 16 : (unsigned long long)p.c.v, from && inside);
-        }
+        unsigned long long row = locate(u, g, k, i);
+        if (row) row = (row & ~1ull) + (values ? row & 1 ? apart_new : apart : 0);
+        copy_rows(row, at, lw * kRowsOfWarp + i * 32, p.c.k);
       }
       arrive_when_landed(&bar.slot_full[slot]);
       advance_slot();
@@ -298,11 +275,11 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
         unsigned long long row = 0;
         if (seg.place(p, r0 + lane, &node, &head))
           row = (unsigned long long)(static_cast<const unsigned short*>(p.a.q) + query_at(p, seg, node, head));
-        const uint32_t to = at + tile * kTileBytes + (uint32_t)(piece / 8) * kQueryBlock + (uint32_t)(r0 % kAttnRows + lane / kPieces) * 128u;
-#pragma unroll
+#pragma unroll 2
         for (int j = 0; j < 32 / kAcross; j++) {
+          const int r = r0 % kAttnRows + j * kAcross + lane / kPieces;
           const unsigned long long from = __shfl_sync(~0u, row, j * kAcross + lane / kPieces);
-          row_copy16(to + (uint32_t)(j * kAcross) * 128u + (uint32_t)(((piece & 7) ^ ((j * kAcross + lane / kPieces) & 7)) << 4),
+          row_copy16(at + tile * kTileBytes + (uint32_t)(piece / 8) * kQueryBlock + (uint32_t)r * 128u + (uint32_t)(((piece & 7) ^ (r & 7)) << 4),
                      from && inside ? from + piece * 16 : (unsigned long long)p.a.q, from && inside);
         }
       }
@@ -316,8 +293,7 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
       bool keys_left = true, ok = true, fresh = true;
       Pages pages[kBuffers + 1];  // of the steps whose values are still to come
       int g = segment_of(p, key_at.b, key_at.group, key_at.s.count).g, value_g = g;
-      Pages next;
-      fetch(key_at, next);
+      Pages next = fetch(key_at);
       auto step_keys = [&](int into) {
         if (fresh) {
           renew();
@@ -325,13 +301,13 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
           if (!ok) return;
         }
         pages[into] = next;
-        ok = load_keys(key_at, g, next);
+        ok = load_block(false, key_at, g, next);
         const int b = key_at.b, group = key_at.group;
         keys_left = next_unit(p, key_at, key_number, share.size);
         fresh = key_at.b != b || key_at.group != group;
         if (keys_left) {
           if (fresh) g = segment_of(p, key_at.b, key_at.group, key_at.s.count).g;
-          fetch(key_at, next);
+          next = fetch(key_at);
         }
       };
       int ahead = 0;
@@ -342,7 +318,7 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
           ahead++;
         }
       while (ok && ahead > 0) {
-        ok = load_values(value_at, value_g, pages[0]);
+        ok = load_block(true, value_at, value_g, pages[0]);
         if (!ok) break;
         const int b = value_at.b, group = value_at.group;
         if (next_unit(p, value_at, value_number, share.size) && (value_at.b != b || value_at.group != group))
@@ -563,8 +539,9 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
         if (!ok) break;
         if (active) {
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          // Columns c * kChunk on, hidden ones at -inf. Two tiles leave registers for half a block: the scores are then read twice.
-          constexpr int kChunk = TILES == 2 ? 64 : kKeys;
+          // Columns c * kChunk on, hidden ones at -inf. The scores are read twice, half a block at a time: reading takes 100 cycles, and
+          // the code is half as long.
+          constexpr int kChunk = 64;
           float s[kChunk];
           const int key0 = now.tile * kKeys;
           auto load = [&](int c) {
