@@ -75,8 +75,8 @@ struct Share {
 
 __device__ __forceinline__ long long numbers_of(const Sequence& s) { return s.tiles ? (long long)s.segments * (s.tiles + kSegmentCost) : 0; }
 
-__device__ __forceinline__ void advance(const TreeArgs& p, Cursor& u) {
-  if (++u.tile < u.s.tiles) return;
+// On to the next segment. A call, since many places do it and none often.
+__device__ __noinline__ void next_segment(const TreeArgs& p, Cursor& u) {
   u.tile = 0;
   if (++u.group < u.s.segments) return;
   u.group = 0;
@@ -84,6 +84,10 @@ __device__ __forceinline__ void advance(const TreeArgs& p, Cursor& u) {
     u.b++;
     u.s = sequence_of(p, u.b);
   } while (u.s.tiles == 0);
+}
+
+__device__ __forceinline__ void advance(const TreeArgs& p, Cursor& u) {
+  if (++u.tile >= u.s.tiles) next_segment(p, u);
 }
 
 // The next unit of a share; false at its end.
@@ -162,7 +166,7 @@ struct Segment {
   }
 };
 
-__device__ __forceinline__ Segment segment_of(const TreeArgs& p, int b, int group, int count) {
+__device__ __noinline__ Segment segment_of(const TreeArgs& p, int b, int group, int count) {
   Segment s;
   s.b = b;
   const int across = p.c.kv_heads * p.groups, r = group % across;

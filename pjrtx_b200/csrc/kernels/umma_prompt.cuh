@@ -324,7 +324,7 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
       const float shift = m_used == -INFINITY ? 0.f : Probability<BF16>::kLift - m_used;
       float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < kKeys / 64; c++) store_probabilities<BF16>(s + c * 64, a.scale_log2, shift, part, s_addr + c * 32);
+      for (int c = 0; c < kKeys / 64; c++) store_probabilities<BF16, 64, 2>(s + c * 64, a.scale_log2, shift, part, s_addr + c * 32);
       sum += (part[0] + part[1]) + (part[2] + part[3]);
       if (!(m_block < INFINITY)) sum = NAN;  // a score of NaN or infinity, which not every way to 2^x passes on
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");

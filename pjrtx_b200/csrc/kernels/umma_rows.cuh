@@ -54,23 +54,31 @@ __device__ __forceinline__ float2 exp2_by_fma(float2 x) {
                      __uint_as_float((__float_as_uint(n.y) << 23) + __float_as_uint(r.y)));
 }
 
-// Of every eight pairs of scores, how many go that way.
-constexpr int kByFma = 2;
+__device__ __forceinline__ void tmem_store_16(uint32_t addr, const float* v) {
+  const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr), "r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+      "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 
-// Probabilities 2^(s * scale + shift) of 64 scores into 32 columns of tensor memory, as pairs of the element type; `part` adds them up.
-template <bool BF16>
+// Probabilities 2^(s * scale + shift) of N scores (32 or 64) into N / 2 columns of tensor memory, as pairs of the element type; `part` adds
+// them up. Of every eight pairs, FMA go by the FMA units.
+template <bool BF16, int N, int FMA>
 __device__ __forceinline__ void store_probabilities(const float* s, float scale, float shift, float (&part)[4], uint32_t to) {
   const Pair scale2 = pair_of(scale, scale), shift2 = pair_of(shift, shift);
-  float packed[32];
+  float packed[N / 2];
 #pragma unroll
-  for (int e = 0; e < 32; e++) {
+  for (int e = 0; e < N / 2; e++) {
     const float2 x = pair_split(pair_fma(pair_of(s[2 * e], s[2 * e + 1]), scale2, shift2));
-    const float2 y = e % 8 >= 8 - kByFma ? exp2_by_fma(x) : make_float2(exp2_approx(x.x), exp2_approx(x.y));
+    const float2 y = e % 8 >= 8 - FMA ? exp2_by_fma(x) : make_float2(exp2_approx(x.x), exp2_approx(x.y));
     const uint32_t pair = pack_pair<BF16>(y.x, y.y);
     add_pair<BF16>(pair, part[(2 * e) & 3], part[(2 * e + 1) & 3]);
     packed[e] = __uint_as_float(pair);
   }
-  tmem_store_32(to, packed);
+  if constexpr (N == 64) tmem_store_32(to, packed);
+  else tmem_store_16(to, packed);
 }
 template <int REGISTERS>
 __device__ __forceinline__ void take_registers() {

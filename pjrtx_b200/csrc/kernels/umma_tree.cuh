@@ -539,36 +539,26 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
         if (!ok) break;
         if (active) {
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          // Columns c * kChunk on, hidden ones at -inf. The scores are read twice, half a block at a time: reading takes 100 cycles, and
-          // the code is half as long.
-          constexpr int kChunk = 64;
-          float s[kChunk];
+          // The scores are read twice, 32 columns at a time: that takes some 200 cycles, and the code is a quarter as long. Where some are
+          // hidden or the scale is not positive, they go back as they are to be.
           const int key0 = now.tile * kKeys;
-          auto load = [&](int c) {
-#pragma unroll
-            for (int i = 0; i < kChunk / 32; i++) tmem_load_32(s_addr + c * kChunk + i * 32, s + i * 32);
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            if (a.sign != 1.f) {
-#pragma unroll
-              for (int e = 0; e < kChunk; e++) s[e] *= a.sign;
-            }
-            if (key0 + kKeys > here.s.length) {
-#pragma unroll
-              for (int w = 0; w < kChunk / 32; w++) {
-                const unsigned seen = there ? seen_word(key0 + c * kChunk + w * 32, here.s.length, bits) : 0u;
-#pragma unroll
-                for (int e = 0; e < 32; e++)
-                  if (!(seen >> e & 1)) s[w * 32 + e] = -INFINITY;
-              }
-            }
-          };
+          const bool special = a.sign != 1.f || key0 + kKeys > here.s.length;
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, m_block = -INFINITY;
 #pragma unroll 1
-          for (int c = 0; c < kKeys / kChunk; c++) {
-            load(c);
-            m_block = max_of<kChunk>(s, mx);
+          for (int c = 0; c < kKeys; c += 32) {
+            float s[32];
+            tmem_load_32(s_addr + c, s);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            if (special) {
+              const unsigned seen = there ? seen_word(key0 + c, here.s.length, bits) : 0u;
+#pragma unroll
+              for (int e = 0; e < 32; e++) s[e] = seen >> e & 1 ? s[e] * a.sign : -INFINITY;
+              tmem_store_32(s_addr + c, s);
+            }
+            m_block = max_of<32>(s, mx);
           }
           m_block *= a.scale_log2;
+          if (special) asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
           float corr = 1.f;
           if (m_block > m_used + Probability<BF16>::kGrow) {
             corr = exp2_approx(m_used - m_block);  // 0 the first time
@@ -593,11 +583,11 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
           const float shift = m_used == -INFINITY ? 0.f : Probability<BF16>::kLift - m_used;
           float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-          for (int c = 0; c < kKeys / kChunk; c++) {
-            if (kChunk < kKeys) load(c);
-#pragma unroll
-            for (int h = 0; h < kChunk / 64; h++)
-              store_probabilities<BF16>(s + h * 64, a.scale_log2, shift, part, s_addr + (c * kChunk / 64 + h) * 32);
+          for (int c = 0; c < kKeys; c += 32) {
+            float s[32];
+            tmem_load_32(s_addr + c, s);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            store_probabilities<BF16, 32, 0>(s, a.scale_log2, shift, part, s_addr + c / 2);
           }
           sum += (part[0] + part[1]) + (part[2] + part[3]);
           if (!(m_block < INFINITY)) sum = NAN;  // a score of NaN or infinity, which not every way to 2^x passes on
