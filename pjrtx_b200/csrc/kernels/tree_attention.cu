@@ -76,18 +76,19 @@ struct Share {
 __device__ __forceinline__ long long numbers_of(const Sequence& s) { return s.tiles ? (long long)s.segments * (s.tiles + kSegmentCost) : 0; }
 
 // On to the next segment. A call, since many places do it and none often.
-__device__ __noinline__ void next_segment(const TreeArgs& p, Cursor& u) {
+__device__ __noinline__ Cursor next_segment(const TreeArgs& p, Cursor u) {
   u.tile = 0;
-  if (++u.group < u.s.segments) return;
+  if (++u.group < u.s.segments) return u;
   u.group = 0;
   do {
     u.b++;
     u.s = sequence_of(p, u.b);
   } while (u.s.tiles == 0);
+  return u;
 }
 
 __device__ __forceinline__ void advance(const TreeArgs& p, Cursor& u) {
-  if (++u.tile >= u.s.tiles) next_segment(p, u);
+  if (++u.tile >= u.s.tiles) u = next_segment(p, u);
 }
 
 // The next unit of a share; false at its end.
