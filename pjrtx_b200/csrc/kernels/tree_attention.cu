@@ -40,6 +40,7 @@ struct TreeArgs {
   int tile_keys;
   int slot_rows, dims;     // of a part's sums in the workspace: [dims][rows], then the rows' maxima and totals
   unsigned reciprocal;     // floor(2^32 / page_size), at most 2^32 - 1
+  int blocks;
   Cut* cuts;               // [blocks]
   float* parts;            // [blocks][2][slot_rows * (dims + 2)]
 };
@@ -333,8 +334,27 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const __grid
   using namespace rows;
   __shared__ float sums[kJoinWarps][kJoinDims][32], stats[kJoinWarps][2][32];
   __shared__ float results[32][kJoinDims + 4];
-  const Cut cut = p.cuts[blockIdx.x];
-  if (cut.first >= cut.last) return;
+  // The blockIdx.x-th cut there is.
+  __shared__ int found;
+  if (threadIdx.x == 0) found = -1;
+  int before = 0;
+  for (int i0 = 0; i0 < p.blocks && before <= (int)blockIdx.x; i0 += kJoinWarps * 32) {
+    const int i = i0 + threadIdx.x;
+    const bool valid = i < p.blocks && p.cuts[i].first < p.cuts[i].last;
+    const unsigned mask = __ballot_sync(~0u, valid);
+    __shared__ int counts[kJoinWarps];
+    if (threadIdx.x % 32 == 0) counts[threadIdx.x / 32] = __popc(mask);
+    __syncthreads();
+    int at = before + __popc(mask & ((1u << threadIdx.x % 32) - 1));
+    for (int w = 0; w < kJoinWarps; w++) {
+      if (w < threadIdx.x / 32) at += counts[w];
+      before += counts[w];
+    }
+    if (valid && at == (int)blockIdx.x) found = i;
+    __syncthreads();
+  }
+  if (found < 0) return;
+  const Cut cut = p.cuts[found];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, row0 = blockIdx.y * 32, row = row0 + lane, d0 = blockIdx.z * kJoinDims;
   const Segment seg = segment_of(p, cut.b, cut.group, sequence_of(p, cut.b).count);
   int node, head;
@@ -423,17 +443,17 @@ auto with_kernel(int dtype, int head_dim, long long rows, F&& f) {
 }
 
 // The tensor-core kernels take the scale apart.
-bool start(void (*kernel)(const TreeArgs), const TreeArgs& p, const TreePlan& plan, long long blocks, bool pdl, cudaStream_t stream) {
-  return launch_kernel(kernel, dim3((unsigned)blocks), dim3((unsigned)plan.threads), plan.smem, stream, pdl, p) == cudaSuccess;
+bool start(void (*kernel)(const TreeArgs), const TreeArgs& p, const TreePlan& plan, bool pdl, cudaStream_t stream) {
+  return launch_kernel(kernel, dim3((unsigned)p.blocks), dim3((unsigned)plan.threads), plan.smem, stream, pdl, p) == cudaSuccess;
 }
-bool start(void (*kernel)(const umma::TreeKernelArgs, const CUtensorMap, const CUtensorMap), const TreeArgs& p, const TreePlan& plan, long long blocks, bool pdl, cudaStream_t stream) {
+bool start(void (*kernel)(const umma::TreeKernelArgs, const CUtensorMap, const CUtensorMap), const TreeArgs& p, const TreePlan& plan, bool pdl, cudaStream_t stream) {
   const float scale = p.a.scale;
   umma::TreeKernelArgs a;
   a.p = p;
   a.scale_log2 = scale == 0.f ? 1.f : (scale < 0.f ? -scale : scale) * rows::kLog2e;
   a.sign = scale > 0.f ? 1.f : scale < 0.f ? -1.f : 0.f;
   a.timeout_ns = wait_timeout_ns();
-  a.box = umma::tree_box(plan.dims, p.c.page_size);
+  a.box = umma::tree_box(plan.keys, p.c.page_size);
   CUtensorMap kmap{}, vmap{};
   if (a.box) {
     const PagedView& c = p.c;
@@ -442,7 +462,7 @@ bool start(void (*kernel)(const umma::TreeKernelArgs, const CUtensorMap, const C
     if (!umma::encode_map(&kmap, c.k, c.dtype == kF16, 4, extents, strides, box) || !umma::encode_map(&vmap, c.v, c.dtype == kF16, 4, extents, strides, box))
       return false;
   }
-  return launch_kernel(kernel, dim3((unsigned)blocks), dim3((unsigned)plan.threads), plan.smem, stream, pdl, a, kmap, vmap) == cudaSuccess;
+  return launch_kernel(kernel, dim3((unsigned)p.blocks), dim3((unsigned)plan.threads), plan.smem, stream, pdl, a, kmap, vmap) == cudaSuccess;
 }
 
 uint64_t round256(uint64_t n) { return (n + 255) / 256 * 256; }
@@ -464,7 +484,7 @@ int paged_tree_launch(const PagedView& c, const PagedTree& a, int sm_count, bool
   char* space = static_cast<char*>(a.workspace);
   p.cuts = reinterpret_cast<Cut*>(space);
   p.parts = reinterpret_cast<float*>(space + round256((uint64_t)sm_count * sizeof(Cut)));
-  long long blocks = 0;
+  long long segments = 0;
   const bool ok = with_kernel(c.dtype, c.head_dim, (long long)a.nodes * p.rep, [&](auto kernel, const TreePlan& plan) {
     p.heads = std::min(p.rep, plan.rows);
     p.groups = (p.rep + p.heads - 1) / p.heads;
@@ -473,15 +493,15 @@ int paged_tree_launch(const PagedView& c, const PagedTree& a, int sm_count, bool
     p.slot_rows = plan.rows;
     p.dims = plan.dims;
     if (!raise_smem_limit((const void*)kernel, (int)plan.smem)) return false;
-    const long long numbers = (long long)c.batch * c.kv_heads * p.groups * ((a.nodes + p.nodes - 1) / p.nodes) *
-                              ((c.capacity() + a.nodes + p.tile_keys - 1) / p.tile_keys + kSegmentCost);
-    blocks = std::min<long long>(numbers, sm_count);
-    return start(kernel, p, plan, blocks, pdl, stream);
+    segments = (long long)c.batch * c.kv_heads * p.groups * ((a.nodes + p.nodes - 1) / p.nodes);
+    const long long numbers = segments * ((c.capacity() + a.nodes + p.tile_keys - 1) / p.tile_keys + kSegmentCost);
+    p.blocks = (int)std::min<long long>(numbers, sm_count);
+    return start(kernel, p, plan, pdl, stream);
   });
   if (!ok) return 0;
   auto join = c.dtype == kF32 ? tree_join_kernel<float> : c.dtype == kF16 ? tree_join_kernel<__half> : tree_join_kernel<__nv_bfloat16>;
   const int rows = std::min(p.slot_rows, std::min(p.nodes, a.nodes) * p.heads);
-  return launch_kernel(join, dim3((unsigned)blocks, (unsigned)((rows + 31) / 32), (unsigned)((c.head_dim + kJoinDims - 1) / kJoinDims)), dim3(kJoinWarps * 32), 0, stream, true, p) ==
+  return launch_kernel(join, dim3((unsigned)std::min<long long>(segments, p.blocks), (unsigned)((rows + 31) / 32), (unsigned)((c.head_dim + kJoinDims - 1) / kJoinDims)), dim3(kJoinWarps * 32), 0, stream, true, p) ==
                  cudaSuccess
              ? 2
              : 0;

@@ -2,12 +2,13 @@
 //
 // A block of threads goes through its share as one row of steps, a step being a block of keys of a segment, and nothing drains between
 // segments: rows of the next one are fetched while the last ones of this are at work.
-//   loader warps   two; queries of a segment, then keys and values of the steps into a ring of shared-memory slots, in the 128-byte
+//   loader warps   four; queries of a segment, then keys and values of the steps into a ring of shared-memory slots, in the 128-byte
 //                  swizzle that the tensor core reads. Blocks of cached rows come by tensor-map copies of a page's rows, where pages are
-//                  8, 16, 32 or a multiple of 64 rows; the last rows, nodes, and pages of other sizes by cp.async, a row at a time,
+//                  8, 16 or a multiple of 32 rows; the last rows, nodes, and pages of other sizes by cp.async, a row at a time,
 //                  each thread's copies counting themselves in on the slot's barrier when they have landed
 //   MMA warp       S = Q . K^T, O += P . V with P in tensor memory. With one tile of 128 query rows the scores have two buffers, so
-//                  that those of the next step are there when the softmax warps are done; with two tiles these take turns
+//                  that those of the next step are there when the softmax warps are done; with two tiles these take turns (blocks of
+//                  64 keys, for which two buffers fit: 211 us, not 171, where 64 nodes of 64 heads see 65536 rows)
 //   softmax warps  four a tile, a query row a thread; those whose rows are not there only count along
 //
 // Bound by memory up to two tiles: 128 keys of 128 elements are 64 KB of keys and values, 2800 cycles of this SM's share of the memory, and
@@ -23,7 +24,9 @@
 namespace pjrtx {
 namespace umma {
 
-constexpr int kTreeLoaders = 2, kOddRing = 16, kCleanRing = 16;  // rings are longer than a checker can be ahead: its slots are
+constexpr int kTreeLoaders = 4;
+constexpr int kByFma = 0;
+constexpr int kOddRing = 16, kCleanRing = 16;  // longer than a checker can be ahead, which has the slots
 __host__ __device__ constexpr int tree_keys(int hd) { return hd == 256 ? 64 : 128; }
 __host__ __device__ constexpr int tree_slot_bytes(int hd) { return tree_keys(hd) * hd * 2; }
 __host__ __device__ constexpr int tree_query_buffers(int hd, int tiles) { return tiles == 1 && hd <= 128 ? 2 : 1; }
@@ -39,8 +42,8 @@ __host__ __device__ constexpr size_t tree_smem(int hd, int tiles) {
   const size_t least = least_smem(512);
   return bytes < least ? least : bytes;
 }
-// Four softmax warps a tile, the loaders, the warp that issues, and the checker: eight or twelve, which divide the registers evenly.
-__host__ __device__ constexpr int tree_threads(int tiles) { return 128 * tiles + 128; }
+// Four softmax warps a tile, the loaders, the warp that issues, the checker.
+__host__ __device__ constexpr int tree_threads(int tiles) { return 128 * tiles + 32 * (kTreeLoaders + 2); }
 
 struct TreeKernelArgs {
   TreeArgs p;
@@ -50,8 +53,8 @@ struct TreeKernelArgs {
 };
 
 // Rows of a box: as many as a page has, at most a loader's part of a block; 0 where blocks are not made of such.
-inline int tree_box(int hd, int page_size) {
-  const int most = tree_keys(hd) / kTreeLoaders;
+inline int tree_box(int keys, int page_size) {
+  const int most = keys / kTreeLoaders;
   const int box = page_size < most ? page_size : most;
   return box % 8 == 0 && most % box == 0 && page_size % box == 0 ? box : 0;
 }
@@ -159,27 +162,22 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
   if (warp >= kFirstLoader && warp < kMmaWarp) {
     const int lw = warp - kFirstLoader;
     const bool leader = elect_one();
-    constexpr int kPieces = HD / 8, kAcross = 32 / kPieces, kRowsOfWarp = kKeys / kTreeLoaders, kRowsOfLane = kRowsOfWarp / 32;
+    constexpr int kPieces = HD / 8, kAcross = 32 / kPieces, kRowsOfWarp = kKeys / kTreeLoaders;
+    static_assert(kRowsOfWarp <= 32, "");
     // Counts this thread in once its copies so far have landed.
     auto arrive_when_landed = [&](uint64_t* b) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(b)) : "memory"); };
-    // Page ids of this warp's part of a block, fetched a step before they are looked at: of rows `lane` and `lane + 32` or, for blocks of
-    // nothing but cached rows whose pages are made of boxes, of box `lane`.
-    struct Pages {
-      int low, high;
-    };
+    // Page id of row `lane` of this warp's part of a block, fetched a step before it is looked at, or, for blocks of nothing but cached
+    // rows whose pages are made of boxes, of box `lane`.
     auto first_key = [&](const Cursor& u) { return u.tile * kKeys + lw * kRowsOfWarp; };
     auto whole = [&](const Cursor& u) { return a.box > 0 && first_key(u) + kRowsOfWarp <= u.s.length; };
     auto fetch = [&](const Cursor& u) {
-      const int* table = p.c.table + u.b * p.c.table_stride;
-      const int step = whole(u) ? a.box : 1, t = first_key(u) + lane * step, end = min(u.s.length, first_key(u) + kRowsOfWarp);
-      Pages k = {0, 0};
-      if (t < end) k.low = table[column_of(p, t)];
-      if (kRowsOfLane == 2 && step == 1 && t + 32 < end) k.high = table[column_of(p, t + 32)];
-      return k;
+      const int t = first_key(u) + lane * (whole(u) ? a.box : 1);
+      return t < min(u.s.length, first_key(u) + kRowsOfWarp) ? p.c.table[u.b * p.c.table_stride + column_of(p, t)] : 0;
     };
-    // Address of the key of row `lane` of the i-th 32: bit 0 marks a node, 0 stands for none.
-    auto locate = [&](const Cursor& u, int g, const Pages& k, int i) -> unsigned long long {
-      const int t = first_key(u) + i * 32 + lane, page = i ? k.high : k.low;
+    // Address of the key of row `lane`: bit 0 marks a node, 0 stands for none.
+    auto locate = [&](const Cursor& u, int g, int page) -> unsigned long long {
+      const int t = first_key(u) + lane;
+      if (lane >= kRowsOfWarp) return 0ull;
       if (t < u.s.length) {
         if (page < 0 || page >= p.c.num_pages) {
           report(p.c.error_words, kErrorPageId);
@@ -213,25 +211,25 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
     };
     // Where this lane's piece of row `row` of a slot goes.
     auto place = [&](uint32_t at, int row) { return at + (uint32_t)(piece / 8) * kKeyBlock + (uint32_t)row * 128u + (uint32_t)(((piece & 7) ^ (row & 7)) << 4); };
-    // 32 rows one by one, `from` being the address of row `lane`, 0: none. The loops are not unrolled: the code of all roles runs side by
+    // The warp's rows one by one, `row` being the address of row `lane`, 0: none. The loops are not unrolled: the code of all roles runs side by
     // side, and what does not fit the instruction cache costs more than it saves (5.1 of a warp's 10 cycles an instruction before).
     auto copy_rows = [&](unsigned long long row, uint32_t at, int row0, const void* any) {
 #pragma unroll 2
-      for (int j = 0; j < 32 / kAcross; j++) {
+      for (int j = 0; j < kRowsOfWarp / kAcross; j++) {
         const int r = j * kAcross + lane / kPieces;
         const unsigned long long from = __shfl_sync(~0u, row, r);
         row_copy16(place(at, row0 + r), from && inside ? from + piece * 16 : (unsigned long long)any, from && inside);
       }
     };
     // A page outside the pool: a box of nothing, which the copy fills with zeros.
-    auto load_boxes = [&](const CUtensorMap* map, const Cursor& u, int g, const Pages& k, uint32_t at) {
+    auto load_boxes = [&](const CUtensorMap* map, const Cursor& u, int g, int pages, uint32_t at) {
       if (leader) mbar_expect_tx(&bar.slot_full[slot], kRowsOfWarp * HD * 2);
       __syncwarp();
       const uint32_t to = at + (uint32_t)(lw * kRowsOfWarp) * 128u;
       const int t = first_key(u), row = t - column_of(p, t) * p.c.page_size;  // 0 where a page has no more than a box
 #pragma unroll 1
       for (int i = 0; i * a.box < kRowsOfWarp; i++) {
-        const int page = __shfl_sync(~0u, k.low, i);
+        const int page = __shfl_sync(~0u, pages, i);
         const bool valid = page >= 0 && page < p.c.num_pages;
         if (leader) {
           if (!valid) report(p.c.error_words, kErrorPageId);
@@ -246,19 +244,16 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
       advance_slot();
     };
     // Keys, or values.
-    auto load_block = [&](bool values, const Cursor& u, int g, const Pages& k) {
+    auto load_block = [&](bool values, const Cursor& u, int g, int pages) {
       uint32_t at;
       if (!take_slot(&at)) return false;
       if (whole(u)) {
-        load_boxes(values ? &vmap : &kmap, u, g, k, at);
+        load_boxes(values ? &vmap : &kmap, u, g, pages, at);
         return true;
       }
-#pragma unroll 1
-      for (int i = 0; i < kRowsOfLane; i++) {
-        unsigned long long row = locate(u, g, k, i);
-        if (row) row = (row & ~1ull) + (values ? row & 1 ? apart_new : apart : 0);
-        copy_rows(row, at, lw * kRowsOfWarp + i * 32, p.c.k);
-      }
+      unsigned long long row = locate(u, g, pages);
+      if (row) row = (row & ~1ull) + (values ? row & 1 ? apart_new : apart : 0);
+      copy_rows(row, at, lw * kRowsOfWarp, p.c.k);
       arrive_when_landed(&bar.slot_full[slot]);
       advance_slot();
       return true;
@@ -291,9 +286,9 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
       Cursor key_at = share.at, value_at = share.at;
       long long key_number = share.first, value_number = share.first, segments = 0;
       bool keys_left = true, ok = true, fresh = true;
-      Pages pages[kBuffers + 1];  // of the steps whose values are still to come
+      int pages[kBuffers + 1];  // of the steps whose values are still to come
       int g = segment_of(p, key_at.b, key_at.group, key_at.s.count).g, value_g = g;
-      Pages next = fetch(key_at);
+      int next = fetch(key_at);
       auto step_keys = [&](int into) {
         if (fresh) {
           renew();
@@ -539,23 +534,27 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
         if (!ok) break;
         if (active) {
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          // The scores are read twice, 32 columns at a time: that takes some 200 cycles, and the code is a quarter as long. Where some are
-          // hidden or the scale is not positive, they go back as they are to be.
+          // The scores are read twice, in pieces, and the loops are not unrolled: that takes some 200 cycles, and the code is a fifth as
+          // long. Where some are hidden or the scale is not positive, they go back as they are to be.
           const int key0 = now.tile * kKeys;
           const bool special = a.sign != 1.f || key0 + kKeys > here.s.length;
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, m_block = -INFINITY;
 #pragma unroll 1
-          for (int c = 0; c < kKeys; c += 32) {
-            float s[32];
+          for (int c = 0; c < kKeys; c += 64) {
+            float s[64];
             tmem_load_32(s_addr + c, s);
+            tmem_load_32(s_addr + c + 32, s + 32);
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
             if (special) {
-              const unsigned seen = there ? seen_word(key0 + c, here.s.length, bits) : 0u;
 #pragma unroll
-              for (int e = 0; e < 32; e++) s[e] = seen >> e & 1 ? s[e] * a.sign : -INFINITY;
-              tmem_store_32(s_addr + c, s);
+              for (int h = 0; h < 64; h += 32) {
+                const unsigned seen = there ? seen_word(key0 + c + h, here.s.length, bits) : 0u;
+#pragma unroll
+                for (int e = 0; e < 32; e++) s[h + e] = seen >> e & 1 ? s[h + e] * a.sign : -INFINITY;
+                tmem_store_32(s_addr + c + h, s + h);
+              }
             }
-            m_block = max_of<32>(s, mx);
+            m_block = max_of<64>(s, mx);
           }
           m_block *= a.scale_log2;
           if (special) asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -582,13 +581,16 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
           }
           const float shift = m_used == -INFINITY ? 0.f : Probability<BF16>::kLift - m_used;
           float part[4] = {0.f, 0.f, 0.f, 0.f};
+          float s[2][32];  // the next piece is on its way while this one is at work
+          tmem_load_32(s_addr, s[0]);
 #pragma unroll 1
-          for (int c = 0; c < kKeys; c += 32) {
-            float s[32];
-            tmem_load_32(s_addr + c, s);
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            store_probabilities<BF16, 32, 0>(s, a.scale_log2, shift, part, s_addr + c / 2);
-          }
+          for (int c = 0; c < kKeys; c += 64)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+              if (c + h * 32 + 32 < kKeys) tmem_load_32(s_addr + c + h * 32 + 32, s[h ^ 1]);
+              store_probabilities<BF16, 32, kByFma>(s[h], a.scale_log2, shift, part, s_addr + (c + h * 32) / 2);
+            }
           sum += (part[0] + part[1]) + (part[2] + part[3]);
           if (!(m_block < INFINITY)) sum = NAN;  // a score of NaN or infinity, which not every way to 2^x passes on
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
