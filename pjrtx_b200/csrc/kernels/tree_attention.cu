@@ -25,7 +25,7 @@ namespace {
 // in its slot of the workspace, and a second kernel joins them in block order.
 
 constexpr int kSegmentCost = 2;
-constexpr int kJoinWarps = 8;
+constexpr int kJoinWarps = 16;
 
 // A segment that ends in another block than it begins in: written by the block it begins in, first >= last where there is none.
 struct Cut {
@@ -324,87 +324,103 @@ __global__ void __launch_bounds__(rows::kThreads) tree_rows_kernel(const __grid_
 
 // ---- parts of a segment ---------------------------------------------------------------------------------------------
 
-// A block has 32 rows and 16 dimensions of a cut segment, a lane a row. Its warps take the parts in turn, each with a maximum of its own
-// that it follows, and are joined in order, so that the result does not depend on which is first.
-constexpr int kJoinDims = 16;
+// A block has 32 rows of a cut segment, a lane a row, a warp eight dimensions and every `splits`-th part, in an order that does not depend on
+// which is first. Many segments are cut once or twice and take the parts one after the other; where few blocks have a place, more warps share a row's
+// parts, and blocks go by the cuts that there are (looking for one takes a microsecond). Loops are not unrolled: every launch fetches
+// its instructions anew, and 16 dimensions a warp with unrolled loops took 8 us for each part behind the first.
+constexpr int kJoinDims = 8;
 
-template <typename T>
-__global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const __grid_constant__ TreeArgs p) {
-  PJRTX_PDL_PROLOGUE();
-  using namespace rows;
-  __shared__ float sums[kJoinWarps][kJoinDims][32], stats[kJoinWarps][2][32];
-  __shared__ float results[32][kJoinDims + 4];
-  // The blockIdx.x-th cut there is.
-  __shared__ int found;
+// The n-th cut there is, -1: none. Called by all threads.
+__device__ __forceinline__ int cut_of(const TreeArgs& p, int n) {
+  __shared__ int found, counts[kJoinWarps];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   if (threadIdx.x == 0) found = -1;
   int before = 0;
-  for (int i0 = 0; i0 < p.blocks && before <= (int)blockIdx.x; i0 += kJoinWarps * 32) {
+  for (int i0 = 0; i0 < p.blocks && before <= n; i0 += kJoinWarps * 32) {
     const int i = i0 + threadIdx.x;
     const bool valid = i < p.blocks && p.cuts[i].first < p.cuts[i].last;
     const unsigned mask = __ballot_sync(~0u, valid);
-    __shared__ int counts[kJoinWarps];
-    if (threadIdx.x % 32 == 0) counts[threadIdx.x / 32] = __popc(mask);
+    if (lane == 0) counts[warp] = __popc(mask);
     __syncthreads();
-    int at = before + __popc(mask & ((1u << threadIdx.x % 32) - 1));
+    int at = before + __popc(mask & ((1u << lane) - 1));
+#pragma unroll 1
     for (int w = 0; w < kJoinWarps; w++) {
-      if (w < threadIdx.x / 32) at += counts[w];
+      if (w < warp) at += counts[w];
       before += counts[w];
     }
-    if (valid && at == (int)blockIdx.x) found = i;
+    if (valid && at == n) found = i;
     __syncthreads();
   }
-  if (found < 0) return;
-  const Cut cut = p.cuts[found];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, row0 = blockIdx.y * 32, row = row0 + lane, d0 = blockIdx.z * kJoinDims;
+  return found;
+}
+
+// Sums of a row relative to m, with more of them.
+__device__ __forceinline__ void join(float& m, float& total, float (&x)[kJoinDims], float m_new, float mass, const float (&y)[kJoinDims]) {
+  if (m_new == -INFINITY && mass == 0.f) return;
+  const float top = fmaxf(m, m_new), shift = top == -INFINITY ? 0.f : top;
+  const float was = m == top ? 1.f : exp2_fast(m - shift), is = m_new == top ? 1.f : exp2_fast(m_new - shift);
+  total = fmaf(total, was, mass * is);
+#pragma unroll
+  for (int e = 0; e < kJoinDims; e++) x[e] = fmaf(x[e], was, y[e] * is);
+  m = top;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const __grid_constant__ TreeArgs p, int splits, int look) {
+  PJRTX_PDL_PROLOGUE();
+  __shared__ float parts[kJoinWarps][kJoinDims + 2][32];
+  __shared__ __align__(16) float results[32][kJoinWarps * kJoinDims + 4];
+  const int at = look ? cut_of(p, blockIdx.x) : (int)blockIdx.x;
+  if (at < 0) return;
+  const Cut cut = p.cuts[at];
+  if (cut.first >= cut.last) return;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, row0 = blockIdx.y * 32, chunks = kJoinWarps / splits;
+  const int first = blockIdx.z * chunks * kJoinDims, mine = warp / splits * kJoinDims, d0 = first + mine;  // dimensions: the block's, the warp's
   const Segment seg = segment_of(p, cut.b, cut.group, sequence_of(p, cut.b).count);
   int node, head;
-  const bool there = seg.place(p, row, &node, &head);
+  const bool there = seg.place(p, row0 + lane, &node, &head);
   if (!__any_sync(~0u, there)) return;  // the same rows in every warp
-  const long long slot = (long long)p.slot_rows * (p.dims + 2);
-  const int parts = cut.last - cut.first + 1, maxima = p.slot_rows * p.dims, totals = maxima + p.slot_rows;
-  float m = -INFINITY, total = 0.f, x[kJoinDims];
+  float m = -INFINITY, total = 0.f, x[kJoinDims], y[kJoinDims];
 #pragma unroll
   for (int e = 0; e < kJoinDims; e++) x[e] = 0.f;
-  // Adds sums y relative to m_new.
-  auto add = [&](float m_new, float mass, const float (&y)[kJoinDims]) {
-    if (m_new == -INFINITY && mass == 0.f) return;
-    const float top = fmaxf(m, m_new), shift = top == -INFINITY ? 0.f : top;
-    const float was = m == top ? 1.f : exp2_fast(m - shift), is = m_new == top ? 1.f : exp2_fast(m_new - shift);
-    total = fmaf(total, was, mass * is);
-#pragma unroll
-    for (int e = 0; e < kJoinDims; e++) x[e] = fmaf(x[e], was, y[e] * is);
-    m = top;
-  };
-  if (there)
-    for (int i = warp; i < parts; i += kJoinWarps) {
-      const float* from = p.parts + ((long long)(cut.first + i) * 2 + (i ? 0 : 1)) * slot + row;
-      float y[kJoinDims];
+  if (there && d0 < p.dims) {
+#pragma unroll 1
+    for (int i = warp % splits; i <= cut.last - cut.first; i += splits) {
+      const float* from = p.parts + ((long long)(cut.first + i) * 2 + (i ? 0 : 1)) * p.slot_rows * (p.dims + 2) + row0 + lane;
+      const float m_new = from[p.slot_rows * p.dims], mass = from[p.slot_rows * (p.dims + 1)];
 #pragma unroll
       for (int e = 0; e < kJoinDims; e++) y[e] = from[(d0 + e) * p.slot_rows];
-      add(from[maxima], from[totals], y);
+      join(m, total, x, m_new, mass, y);
     }
-  stats[warp][0][lane] = m;
-  stats[warp][1][lane] = total;
+  }
+  if (splits > 1) {
+    parts[warp][kJoinDims][lane] = m;
+    parts[warp][kJoinDims + 1][lane] = total;
 #pragma unroll
-  for (int e = 0; e < kJoinDims; e++) sums[warp][e][lane] = x[e];
+    for (int e = 0; e < kJoinDims; e++) parts[warp][e][lane] = x[e];
+    __syncthreads();
+    if (warp % splits == 0) {
+#pragma unroll 1
+      for (int w = warp + 1; w < warp + splits; w++) {
+#pragma unroll
+        for (int e = 0; e < kJoinDims; e++) y[e] = parts[w][e][lane];
+        join(m, total, x, parts[w][kJoinDims][lane], parts[w][kJoinDims + 1][lane], y);
+      }
+    }
+  }
+  if (warp % splits == 0) {
+    const float inverse = rows::inverse_of(total);
+#pragma unroll
+    for (int e = 0; e < kJoinDims; e++) results[lane][mine + e] = x[e] * inverse;
+    if (p.a.lse && there && d0 == 0) p.a.lse[lse_at(p, seg, node, head)] = rows::lse_of(m, total);
+  }
   __syncthreads();
-  if (warp == 0) {
-    for (int w = 1; w < kJoinWarps; w++) {
-      float y[kJoinDims];
-#pragma unroll
-      for (int e = 0; e < kJoinDims; e++) y[e] = sums[w][e][lane];
-      add(stats[w][0][lane], stats[w][1][lane], y);
-    }
-    const float inverse = inverse_of(total);
-#pragma unroll
-    for (int e = 0; e < kJoinDims; e++) results[lane][e] = x[e] * inverse;
-    if (p.a.lse && there && blockIdx.z == 0) p.a.lse[lse_at(p, seg, node, head)] = lse_of(m, total);
-    __syncwarp();
-    for (int i = lane; i < 32 * (kJoinDims / 4); i += 32) {
-      const int r = i / (kJoinDims / 4), d = i % (kJoinDims / 4) * 4;
-      if (d0 + d < p.c.head_dim && seg.place(p, row0 + r, &node, &head))
-        store4(static_cast<T*>(p.a.out) + out_at(p, seg, node, head) + d0 + d, *reinterpret_cast<const float4*>(&results[r][d]));
-    }
+  const int pieces = chunks * kJoinDims / 4;
+#pragma unroll 1
+  for (int i = threadIdx.x; i < 32 * pieces; i += kJoinWarps * 32) {
+    const int r = i / pieces, d = i % pieces * 4;
+    if (first + d < p.c.head_dim && seg.place(p, row0 + r, &node, &head))
+      rows::store4(static_cast<T*>(p.a.out) + out_at(p, seg, node, head) + first + d, *reinterpret_cast<const float4*>(&results[r][d]));
   }
 }
 
@@ -499,12 +515,11 @@ int paged_tree_launch(const PagedView& c, const PagedTree& a, int sm_count, bool
     return start(kernel, p, plan, pdl, stream);
   });
   if (!ok) return 0;
+  const int groups = (std::min(p.slot_rows, std::min(p.nodes, a.nodes) * p.heads) + 31) / 32;
+  const int look = segments * 4 <= p.blocks, splits = look ? 8 : 1, across = kJoinWarps / splits * kJoinDims;
+  const dim3 grid((unsigned)(look ? segments : p.blocks), (unsigned)groups, (unsigned)((c.head_dim + across - 1) / across));
   auto join = c.dtype == kF32 ? tree_join_kernel<float> : c.dtype == kF16 ? tree_join_kernel<__half> : tree_join_kernel<__nv_bfloat16>;
-  const int rows = std::min(p.slot_rows, std::min(p.nodes, a.nodes) * p.heads);
-  return launch_kernel(join, dim3((unsigned)std::min<long long>(segments, p.blocks), (unsigned)((rows + 31) / 32), (unsigned)((c.head_dim + kJoinDims - 1) / kJoinDims)), dim3(kJoinWarps * 32), 0, stream, true, p) ==
-                 cudaSuccess
-             ? 2
-             : 0;
+  return launch_kernel(join, grid, dim3(kJoinWarps * 32), 0, stream, true, p, splits, look) == cudaSuccess ? 2 : 0;
 }
 
 }  // namespace pjrtx
