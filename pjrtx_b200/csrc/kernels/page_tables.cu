@@ -63,9 +63,33 @@ struct Sums {
   long long give, take, granted;
 };
 
+// Slot of a packed token, once tables and page counts are written: the sequence by bisection, the row from its end.
+__device__ __forceinline__ int slot_of(const PagedAssign& a, long long t) {
+  if (a.batch == 0 || t < a.starts[0] || t >= a.starts[a.batch]) return -1;
+  int lo = 0, hi = a.batch;  // starts[lo] <= t < starts[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (a.starts[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  const int length = a.lengths[lo], held = __ldcg(a.held_out + lo);
+  const long long row = length - (a.starts[lo + 1] - t);
+  if (row < 0 || length > (long long)a.page_size * a.max_pages) {
+    report(a.error_words, kErrorLength);
+    return -1;
+  }
+  if ((long long)held * a.page_size < length) return -1;
+  const int column = (int)row / a.page_size, page = __ldcg(a.table_out + lo * a.table_out_stride + column);
+  if (page < 0 || page >= a.num_pages) {
+    report(a.error_words, kErrorPageId);
+    return -1;
+  }
+  return page * a.page_size + ((int)row - column * a.page_size);
+}
+
 // Sequences are divided among the blocks in chunks; a warp has a sequence at a time, its lanes the pages. `offsets`: shared memory of
 // two numbers a sequence of the chunk. Sums have 64 bits: lengths may ask for more pages than there are.
-__global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads) paged_assign_kernel(const __grid_constant__ PagedAssign a) {
+__global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads) paged_assign_kernel(const __grid_constant__ PagedAssign a, int slots) {
   PJRTX_PDL_PROLOGUE();
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
@@ -164,32 +188,19 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads) page
   if (copy_stack)
     for (int i = rank * kThreads + threadIdx.x; i < a.num_pages; i += kBlocks * kThreads)
       if (i < min(count, free_count) || i >= there) a.free_pages_out[i] = a.free_pages[i];
-  if (a.tokens == 0) return;
-
-  // Slots of the packed tokens: the sequence by bisection, the row from its end.
+  if (!slots) return;
   cluster.sync();
-  for (long long t = rank * kThreads + threadIdx.x; t < a.tokens; t += kBlocks * kThreads) {
-    int slot = -1;
-    if (a.batch > 0 && t >= a.starts[0] && t < a.starts[a.batch]) {
-      int lo = 0, hi = a.batch;  // starts[lo] <= t < starts[hi]
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (a.starts[mid] <= t) lo = mid;
-        else hi = mid;
-      }
-      const int length = a.lengths[lo];
-      const long long row = length - (a.starts[lo + 1] - t);
-      const int held = __ldcg(a.held_out + lo);
-      if (row < 0 || length > (long long)a.page_size * a.max_pages) {
-        report(a.error_words, kErrorLength);
-      } else if ((long long)held * a.page_size >= length) {
-        const int column = (int)(row / a.page_size), page = __ldcg(a.table_out + lo * a.table_out_stride + column);
-        if (page >= 0 && page < a.num_pages) slot = page * a.page_size + (int)(row - (long long)column * a.page_size);
-        else report(a.error_words, kErrorPageId);
-      }
-    }
-    a.slots[t] = slot;
-  }
+  for (long long t = rank * kThreads + threadIdx.x; t < a.tokens; t += kBlocks * kThreads) a.slots[t] = slot_of(a, t);
+}
+
+// The same for more tokens than a cluster gets through while another kernel starts.
+constexpr int kSlotThreads = 256;
+constexpr long long kSlotsHere = 4 * kBlocks * kThreads;
+
+__global__ void __launch_bounds__(kSlotThreads) paged_slots_kernel(const __grid_constant__ PagedAssign a) {
+  PJRTX_PDL_PROLOGUE();
+  const long long t = (long long)blockIdx.x * kSlotThreads + threadIdx.x;
+  if (t < a.tokens) a.slots[t] = slot_of(a, t);
 }
 
 constexpr int kPathThreads = 128;
@@ -231,7 +242,12 @@ int paged_assign_launch(const PagedAssign& a, bool pdl, cudaStream_t stream) {
   const size_t smem = (size_t)((a.batch + kBlocks - 1) / kBlocks) * sizeof(longlong2);
   constexpr size_t kMost = (65535 + kBlocks - 1) / kBlocks * sizeof(longlong2);
   if (!raise_smem_limit((const void*)paged_assign_kernel, (int)kMost)) return 0;
-  return launch_kernel(paged_assign_kernel, dim3(kBlocks), dim3(kThreads), smem, stream, pdl, a) == cudaSuccess;
+  const bool here = a.tokens <= kSlotsHere;
+  if (launch_kernel(paged_assign_kernel, dim3(kBlocks), dim3(kThreads), smem, stream, pdl, a, (int)(here && a.tokens > 0)) != cudaSuccess) return 0;
+  if (here) return 1;
+  return launch_kernel(paged_slots_kernel, dim3((unsigned)((a.tokens + kSlotThreads - 1) / kSlotThreads)), dim3(kSlotThreads), 0, stream, true, a) == cudaSuccess
+             ? 2
+             : 0;
 }
 
 int paged_path_launch(const PagedPath& a, bool pdl, cudaStream_t stream) {
