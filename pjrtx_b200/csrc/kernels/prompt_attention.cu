@@ -71,52 +71,69 @@ namespace pjrtx {
 namespace {
 
 // In f32.
+constexpr int kRowsOfThread = 4;
+
 template <int D>
 __global__ void __launch_bounds__(rows::kThreads) prompt_rows_kernel(const __grid_constant__ PromptArgs p) {
   PJRTX_PDL_PROLOGUE();
   using namespace rows;
-  using T = float;
+  constexpr int R = kRowsOfThread;
+  using Space = Shared<D, R>;
   extern __shared__ __align__(16) char smem[];
-  Shared<D>& s = *reinterpret_cast<Shared<D>*>(smem);
+  Space& s = *reinterpret_cast<Space*>(smem);
   const PromptAttention& a = p.a;
   check_starts(a);
   const PromptTile t = prompt_tile(p, p.positions, prompt_block());
   if (t.tile < 0) return;
   const int g = blockIdx.x / p.groups, h0 = blockIdx.x % p.groups * p.heads, heads = min(p.heads, p.rep - h0);
   const int first = t.tile * p.positions, positions = min(p.positions, t.tokens - first);
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   auto place = [&](int r, int* position, int* head) {
     *position = first + r / p.heads;
     *head = r % p.heads;
     return r / p.heads < positions && *head < heads;
   };
-  load_rows<T, D>(s.q, a.head_dim, [&](int r) -> const T* {
+  const int keys = first + positions;
+  const float* any = static_cast<const float*>(a.q);
+  const float* k = static_cast<const float*>(a.k) + (long long)t.start * a.k_stride + (long long)g * a.k_head_stride;
+  const float* v = static_cast<const float*>(a.v) + (long long)t.start * a.v_stride + (long long)g * a.v_head_stride;
+  auto request = [&](int stage) {
+    constexpr int kOfWarp = Space::kKeys / 8;
+    const int key = stage * Space::kKeys + warp * kOfWarp + lane;
+    const bool there = lane < kOfWarp && key < keys;
+    request_rows<D, Space::kKeys>(s.k[stage & 1], there ? k + key * a.k_stride : nullptr, a.head_dim, any);
+    request_rows<D, Space::kKeys>(s.v[stage & 1], there ? v + key * a.v_stride : nullptr, a.head_dim, any);
+  };
+  {
+    constexpr int kOfWarp = Space::kRows / 8;
     int position, head;
-    if (!place(r, &position, &head)) return nullptr;
-    return static_cast<const T*>(a.q) + (long long)(t.start + position) * a.q_stride + (long long)(g * p.rep + h0 + head) * a.q_head_stride;
-  });
-  Sight sight[4];
-  Sums<D> sum;
+    const float* q = nullptr;
+    if (lane < kOfWarp && place(warp * kOfWarp + lane, &position, &head))
+      q = any + (long long)(t.start + position) * a.q_stride + (long long)(g * p.rep + h0 + head) * a.q_head_stride;
+    request_rows<D, Space::kRows>(s.q, q, a.head_dim, any);
+  }
+  request(0);
+  Sight sight[R];
+  Sums<D, R> sum;
   sum.clear();
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
+  for (int i = 0; i < R; i++) {
     int position, head;
-    sight[i] = {place(ty * 4 + i, &position, &head) ? position + 1 : 0, 0ull};
+    sight[i] = {place(ty * R + i, &position, &head) ? position + 1 : 0, 0ull};
   }
-  const int keys = first + positions;
-  const T* k = static_cast<const T*>(a.k) + (long long)t.start * a.k_stride + (long long)g * a.k_head_stride;
-  const T* v = static_cast<const T*>(a.v) + (long long)t.start * a.v_stride + (long long)g * a.v_head_stride;
-  for (int key0 = 0; key0 < keys; key0 += kKeys)
-    block_of_keys<T, D>(s, sum, sight, key0, keys, keys, a.head_dim, a.scale * kLog2e, [&](int j) { return k + j * a.k_stride; },
-                        [&](int j) { return v + j * a.v_stride; });
+  const int blocks = (keys + Space::kKeys - 1) / Space::kKeys;
+  for (int j = 0; j < blocks; j++)
+    block_of_keys<D, R>(s, sum, sight, j, j * Space::kKeys, keys, keys, a.scale * kLog2e, [&] {
+      if (j + 1 < blocks) request(j + 1);
+    });
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
+  for (int i = 0; i < R; i++) {
     int position, head;
-    if (!place(ty * 4 + i, &position, &head)) continue;
+    if (!place(ty * R + i, &position, &head)) continue;
     const long long row = t.start + position;
     const int h = g * p.rep + h0 + head;
     const float inverse = inverse_of(sum.l[i]);
-    T* out = static_cast<T*>(a.out) + row * a.out_stride + h * a.out_head_stride;
+    float* out = static_cast<float*>(a.out) + row * a.out_stride + h * a.out_head_stride;
 #pragma unroll
     for (int c = 0; c < D / 64; c++) {
       const float2 x = pair_split(sum.o[i][c][0]), y = pair_split(sum.o[i][c][1]);
@@ -128,12 +145,12 @@ __global__ void __launch_bounds__(rows::kThreads) prompt_rows_kernel(const __gri
 
 template <int D>
 int launch_rows(PromptArgs p, bool pdl, cudaStream_t stream) {
-  constexpr size_t smem = sizeof(rows::Shared<D>);
-  if (!raise_smem_limit((const void*)prompt_rows_kernel<D>, (int)smem)) return 0;
-  p.heads = std::min(p.rep, rows::kRows);
+  using Space = rows::Shared<D, kRowsOfThread>;
+  if (!raise_smem_limit((const void*)prompt_rows_kernel<D>, (int)sizeof(Space))) return 0;
+  p.heads = std::min(p.rep, Space::kRows);
   p.groups = (p.rep + p.heads - 1) / p.heads;
-  p.positions = rows::kRows / p.heads;
-  return launch_kernel(prompt_rows_kernel<D>, prompt_grid(p, p.positions), dim3(rows::kThreads), smem, stream, pdl, p) == cudaSuccess;
+  p.positions = Space::kRows / p.heads;
+  return launch_kernel(prompt_rows_kernel<D>, prompt_grid(p, p.positions), dim3(rows::kThreads), sizeof(Space), stream, pdl, p) == cudaSuccess;
 }
 
 template <bool BF16, int HD, int TILES>

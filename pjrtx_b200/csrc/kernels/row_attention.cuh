@@ -5,8 +5,9 @@
 // A row sees the keys below its limit, and of 64 keys from `base` on those in its word of bits: for a prompt the limit is the position
 // and there are no bits, for a tree of drafted tokens the limit is the cached length and the bits are the ancestors.
 //
-// 256 threads, 64 rows and 64 keys at a time: a thread has four rows by four keys of the scores, then four rows by a sixteenth of the
-// dimensions of the values, two products an instruction; the running maximum and sum of a row are in the sixteen threads that have it.
+// 256 threads, 16, 32 or 64 rows and 64 keys (32 of 256 dimensions) at a time: a thread has up to four rows by four keys of the
+// scores, then its rows by a sixteenth of the dimensions of the values, two products an instruction; the running maximum and sum of a row are in
+// the sixteen threads that have it. The next keys and values come by cp.async while these are at work.
 // What a row does not see enters nothing: scores are replaced, and where values of a block are infinite or NaN the products with
 // hidden keys are left out one by one.
 #pragma once
@@ -19,7 +20,8 @@
 namespace pjrtx {
 namespace rows {
 
-constexpr int kRows = 64, kKeys = 64, kThreads = 256;
+constexpr int kThreads = 256;
+__host__ __device__ constexpr int keys_of(int d) { return d == 256 ? 32 : 64; }  // of a block
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // What a query row sees.
@@ -57,23 +59,23 @@ template <> __device__ __forceinline__ void unpack16<__nv_bfloat16>(const uint4&
 }
 __device__ __forceinline__ bool odd(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }  // infinite or NaN
 
-template <int D>
+template <int D, int R>  // R rows a thread
 struct Shared {
-  static constexpr int kPitch = D + 4;  // rows of neighbouring threads fall on different banks
+  static constexpr int kRows = 16 * R, kKeys = keys_of(D), kPitch = D + 4;  // rows of neighbouring threads fall on different banks
   float q[kRows][kPitch];
-  float k[kKeys][kPitch];
-  float v[kKeys][D];
+  float k[2][kKeys][kPitch];
+  float v[2][kKeys][D];
   float p[kRows][kKeys + 4];
 };
 
-// Sums of a thread: rows ty * 4 + i, dimensions c * 64 + tx * 4 + 0..3 for c < D / 64 (ty = thread / 16, tx = thread % 16).
-template <int D>
+// Sums of a thread: rows ty * R + i, dimensions c * 64 + tx * 4 + 0..3 for c < D / 64 (ty = thread / 16, tx = thread % 16).
+template <int D, int R>
 struct Sums {
-  Pair o[4][D / 64][2];
-  float m[4], l[4];  // in units of ln 2; the same in the sixteen threads of a row
+  Pair o[R][D / 64][2];
+  float m[R], l[R];  // in units of ln 2; the same in the sixteen threads of a row
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < R; i++) {
 #pragma unroll
       for (int c = 0; c < D / 64; c++) o[i][c][0] = o[i][c][1] = 0;
       m[i] = -INFINITY;
@@ -82,61 +84,75 @@ struct Sums {
   }
 };
 
-// Rows of `count` x head_dim elements into shared memory; row(i) is a row's address or null, which gives zeros. True where a value is odd.
-template <typename T, int D, int PITCH, typename Row>
-__device__ __forceinline__ bool load_rows(float (*to)[PITCH], int head_dim, Row row) {
-  constexpr int kPer = 16 / (int)sizeof(T), kPieces = D / kPer;
-  bool found = false;
-  for (int i = threadIdx.x; i < 64 * kPieces; i += kThreads) {
-    const int r = i / kPieces, d = i % kPieces * kPer;
-    const T* from = row(r);
-    float x[kPer];
-    if (from && d < head_dim) {
-      unpack16<T>(*reinterpret_cast<const uint4*>(from + d), x);
-    } else {
+__device__ __forceinline__ void copy16_or_zero(float* to, const float* from, bool there, const float* any) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(there ? from : any), "r"(there ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// Rows of a block are copied by warps, ROWS / 8 neighbouring ones each, a lane 16 bytes: visit(i, row, d) for each piece that this lane has,
+// row `i` of the warp's.
+template <int D, int ROWS, typename Visit>
+__device__ __forceinline__ void pieces_of_lane(Visit visit) {
+  constexpr int kPieces = D / 4, kAcross = kPieces >= 32 ? 1 : 32 / kPieces, kOfWarp = ROWS / 8;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+#pragma unroll 4
+  for (int i0 = 0; i0 < kOfWarp; i0 += kAcross) {
+    const int i = i0 + lane / kPieces;
 #pragma unroll
-      for (int e = 0; e < kPer; e++) x[e] = 0.f;
-    }
-#pragma unroll
-    for (int e = 0; e < kPer; e += 4) {
-      *reinterpret_cast<float4*>(&to[r][d + e]) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-      found = found || odd(x[e]) || odd(x[e + 1]) || odd(x[e + 2]) || odd(x[e + 3]);
-    }
+    for (int d = lane % kPieces * 4; d < D; d += 128) visit(i, warp * kOfWarp + i, d);
   }
-  return found;
 }
 
-// Keys key0..key0 + 63 (those before `keys`) into the sums. The queries are in shared memory. key(t) and value(t): addresses or null.
-template <typename T, int D, typename Key, typename Value>
-__device__ __forceinline__ void block_of_keys(Shared<D>& s, Sums<D>& sum, const Sight (&sight)[4], int key0, int keys, int base, int head_dim,
-                                              float scale2, Key key, Value value) {
+// Requests the rows of a block, `row` being the address of row `lane` of the warp's part (null: zeros).
+template <int D, int ROWS, int PITCH>
+__device__ __forceinline__ void request_rows(float (*to)[PITCH], const float* row, int head_dim, const float* any) {
+  const unsigned long long at = reinterpret_cast<unsigned long long>(row);
+  pieces_of_lane<D, ROWS>([&](int i, int r, int d) {
+    const float* from = reinterpret_cast<const float*>(__shfl_sync(~0u, at, i));
+    copy16_or_zero(&to[r][d], from + d, from && d < head_dim, any);
+  });
+}
+
+// Block `stage & 1`: keys key0 .. (those before `keys`), which has been requested, into the sums; requests the next one by `next()`. The
+// queries are in shared memory once the first block is.
+template <int D, int R, typename Next>
+__device__ __forceinline__ void block_of_keys(Shared<D, R>& s, Sums<D, R>& sum, const Sight (&sight)[R], int stage, int key0, int keys, int base,
+                                              float scale2, Next next) {
+  constexpr int kKeys = keys_of(D), kColumns = kKeys / 16;
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  __syncthreads();  // the block before has been read
-  load_rows<T, D>(s.k, head_dim, [&](int r) { return key0 + r < keys ? key(key0 + r) : nullptr; });
-  const bool found = load_rows<T, D>(s.v, head_dim, [&](int r) { return key0 + r < keys ? value(key0 + r) : nullptr; });
-  const bool careful = __syncthreads_or(found);
-  Pair a[4][4];
+  float(*const sk)[D + 4] = s.k[stage & 1];
+  float(*const sv)[D] = s.v[stage & 1];
+  copies_wait();
+  bool found = false;
+  pieces_of_lane<D, kKeys>([&](int, int r, int d) {
+    const float4 x = *reinterpret_cast<const float4*>(&sv[r][d]);
+    found = found || odd(x.x) || odd(x.y) || odd(x.z) || odd(x.w);
+  });
+  const bool careful = __syncthreads_or(found);  // all rows have landed, and the other stage has been read
+  next();
+  Pair a[R][kColumns];
 #pragma unroll
-  for (int i = 0; i < 4; i++)
+  for (int i = 0; i < R; i++)
 #pragma unroll
-    for (int j = 0; j < 4; j++) a[i][j] = 0;
+    for (int j = 0; j < kColumns; j++) a[i][j] = 0;
 #pragma unroll 4
   for (int d = 0; d < D; d += 4) {
-    ulonglong2 q[4], k[4];
+    ulonglong2 q[R], k[kColumns];
 #pragma unroll
-    for (int i = 0; i < 4; i++) q[i] = *reinterpret_cast<const ulonglong2*>(&s.q[ty * 4 + i][d]);
+    for (int i = 0; i < R; i++) q[i] = *reinterpret_cast<const ulonglong2*>(&s.q[ty * R + i][d]);
 #pragma unroll
-    for (int j = 0; j < 4; j++) k[j] = *reinterpret_cast<const ulonglong2*>(&s.k[tx + 16 * j][d]);
+    for (int j = 0; j < kColumns; j++) k[j] = *reinterpret_cast<const ulonglong2*>(&sk[tx + 16 * j][d]);
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+    for (int i = 0; i < R; i++)
 #pragma unroll
-      for (int j = 0; j < 4; j++) a[i][j] = pair_fma(q[i].y, k[j].y, pair_fma(q[i].x, k[j].x, a[i][j]));
+      for (int j = 0; j < kColumns; j++) a[i][j] = pair_fma(q[i].y, k[j].y, pair_fma(q[i].x, k[j].x, a[i][j]));
   }
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    float x[4], top = -INFINITY;
+  for (int i = 0; i < R; i++) {
+    float x[kColumns], top = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
+    for (int j = 0; j < kColumns; j++) {
       const float2 f = pair_split(a[i][j]);
       const int t = key0 + tx + 16 * j;
       x[j] = t < keys && sees(sight[i], t, base) ? (f.x + f.y) * scale2 : -INFINITY;
@@ -148,9 +164,9 @@ __device__ __forceinline__ void block_of_keys(Shared<D>& s, Sums<D>& sum, const 
     const float shift = top == -INFINITY ? 0.f : top, corr = top == sum.m[i] ? 1.f : exp2_fast(sum.m[i] - shift);
     float total = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
+    for (int j = 0; j < kColumns; j++) {
       x[j] = exp2_fast(x[j] - shift);
-      s.p[ty * 4 + i][tx + 16 * j] = x[j];
+      s.p[ty * R + i][tx + 16 * j] = x[j];
       total += x[j];
     }
 #pragma unroll
@@ -169,13 +185,13 @@ __device__ __forceinline__ void block_of_keys(Shared<D>& s, Sums<D>& sum, const 
     for (int t = 0; t < kKeys; t++) {
       if (key0 + t >= keys) break;
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
+      for (int i = 0; i < R; i++) {
         if (!sees(sight[i], key0 + t, base)) continue;
-        const float p = s.p[ty * 4 + i][t];
+        const float p = s.p[ty * R + i][t];
         const Pair p2 = pair_of(p, p);
 #pragma unroll
         for (int c = 0; c < D / 64; c++) {
-          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&s.v[t][c * 64 + tx * 4]);
+          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sv[t][c * 64 + tx * 4]);
           sum.o[i][c][0] = pair_fma(p2, v.x, sum.o[i][c][0]);
           sum.o[i][c][1] = pair_fma(p2, v.y, sum.o[i][c][1]);
         }
@@ -185,16 +201,16 @@ __device__ __forceinline__ void block_of_keys(Shared<D>& s, Sums<D>& sum, const 
   }
 #pragma unroll 2
   for (int t = 0; t < kKeys; t += 4) {
-    float4 p[4];
+    float4 p[R];
 #pragma unroll
-    for (int i = 0; i < 4; i++) p[i] = *reinterpret_cast<const float4*>(&s.p[ty * 4 + i][t]);
+    for (int i = 0; i < R; i++) p[i] = *reinterpret_cast<const float4*>(&s.p[ty * R + i][t]);
 #pragma unroll
     for (int u = 0; u < 4; u++) {
       ulonglong2 v[D / 64];
 #pragma unroll
-      for (int c = 0; c < D / 64; c++) v[c] = *reinterpret_cast<const ulonglong2*>(&s.v[t + u][c * 64 + tx * 4]);
+      for (int c = 0; c < D / 64; c++) v[c] = *reinterpret_cast<const ulonglong2*>(&sv[t + u][c * 64 + tx * 4]);
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
+      for (int i = 0; i < R; i++) {
         const float x = u == 0 ? p[i].x : u == 1 ? p[i].y : u == 2 ? p[i].z : p[i].w;
         const Pair p2 = pair_of(x, x);
 #pragma unroll

@@ -230,87 +230,99 @@ namespace {
 
 // ---- on the CUDA cores ---------------------------------------------------------------------------------------------
 
-template <typename T, int D>
+template <int D, int R>
 __global__ void __launch_bounds__(rows::kThreads) tree_rows_kernel(const __grid_constant__ TreeArgs p) {
   PJRTX_PDL_PROLOGUE();
   using namespace rows;
+  using Space = Shared<D, R>;
   extern __shared__ __align__(16) char smem[];
   __shared__ ShareSpace<kThreads> space;
   __shared__ unsigned long long ancestors[kTreeNodesMax];
-  __shared__ long long place_of[kKeys];  // of the keys of a block
-  Shared<D>& s = *reinterpret_cast<Shared<D>*>(smem);
+  Space& s = *reinterpret_cast<Space*>(smem);
   if (threadIdx.x == 0) p.cuts[blockIdx.x] = {0, 0, 0, 0};
   const Share share = share_of_block(p, space);
   if (share.first >= share.size) return;
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const float* any = static_cast<const float*>(p.a.q);
   Cursor now = share.at;
   long long at = share.first;
+  int stage = 0;
   for (bool more = true; more;) {
     const Segment seg = segment_of(p, now.b, now.group, now.s.count);
     const Cursor here = now;
-    __syncthreads();
-    if (threadIdx.x < 32) {
+    const int keys = here.s.length + here.s.count;
+    auto request = [&](int tile, int to) {
+      constexpr int kOfWarp = Space::kKeys / 8;
+      const int t = tile * Space::kKeys + warp * kOfWarp + lane;
+      const float *k = nullptr, *v = nullptr;
+      if (lane < kOfWarp && t < here.s.length) {
+        const long long row = cached_row(p, seg.b, t);
+        if (row >= 0) {
+          k = static_cast<const float*>(p.c.k) + row + seg.g * p.c.head_stride;
+          v = static_cast<const float*>(p.c.v) + row + seg.g * p.c.head_stride;
+        }
+      } else if (lane < kOfWarp && t < keys) {
+        const long long row = seg.b * p.a.new_batch_stride + (t - here.s.length) * p.a.new_node_stride + seg.g * p.a.new_head_stride;
+        k = static_cast<const float*>(p.a.k_new) + row;
+        v = static_cast<const float*>(p.a.v_new) + row;
+      }
+      request_rows<D, Space::kKeys>(s.k[to & 1], k, p.c.head_dim, any);
+      request_rows<D, Space::kKeys>(s.v[to & 1], v, p.c.head_dim, any);
+    };
+    __syncthreads();  // the segment before has been read
+    if (warp == 0) {
       const Ancestors above = tree_ancestors(p.a.parents + (long long)seg.b * p.a.nodes, p.a.nodes, p.c.error_words);
-      ancestors[threadIdx.x] = above.low;
-      ancestors[threadIdx.x + 32] = above.high;
+      ancestors[lane] = above.low;
+      ancestors[lane + 32] = above.high;
     }
-    load_rows<T, D>(s.q, p.c.head_dim, [&](int r) -> const T* {
+    {
+      constexpr int kOfWarp = Space::kRows / 8;
       int node, head;
-      return seg.place(p, r, &node, &head) ? static_cast<const T*>(p.a.q) + query_at(p, seg, node, head) : nullptr;
-    });
+      const float* q = nullptr;
+      if (lane < kOfWarp && seg.place(p, warp * kOfWarp + lane, &node, &head)) q = any + query_at(p, seg, node, head);
+      request_rows<D, Space::kRows>(s.q, q, p.c.head_dim, any);
+    }
+    request(now.tile, stage);
     __syncthreads();
-    Sight sight[4];
-    Sums<D> sum;
+    Sight sight[R];
+    Sums<D, R> sum;
     sum.clear();
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < R; i++) {
       int node, head;
       sight[i] = {0, 0ull};
-      if (seg.place(p, ty * 4 + i, &node, &head)) sight[i] = {here.s.length, ancestors[node]};
+      if (seg.place(p, ty * R + i, &node, &head)) sight[i] = {here.s.length, ancestors[node]};
     }
     const long long segment = share.begin + at - here.tile;  // number of its first unit
-    const int keys = here.s.length + here.s.count;
-    for (;;) {
-      const int key0 = now.tile * kKeys;
-      __syncthreads();
-      if (threadIdx.x < kKeys && key0 + threadIdx.x < here.s.length) {
-        const long long row = cached_row(p, seg.b, key0 + threadIdx.x);
-        place_of[threadIdx.x] = row < 0 ? -1 : row + seg.g * p.c.head_stride;
-      }
-      __syncthreads();
-      auto from = [&](const void* pool, const void* fresh, int t) -> const T* {
-        if (t < here.s.length) return place_of[t - key0] < 0 ? nullptr : static_cast<const T*>(pool) + place_of[t - key0];
-        return static_cast<const T*>(fresh) + seg.b * p.a.new_batch_stride + (t - here.s.length) * p.a.new_node_stride + seg.g * p.a.new_head_stride;
-      };
-      block_of_keys<T, D>(s, sum, sight, key0, keys, here.s.length, p.c.head_dim, p.a.scale * kLog2e,
-                          [&](int t) { return from(p.c.k, p.a.k_new, t); }, [&](int t) { return from(p.c.v, p.a.v_new, t); });
+    for (bool same = true; same; stage++) {
+      const int tile = now.tile;
       more = next_unit(p, now, at, share.size);
-      if (!more || now.group != here.group || now.b != here.b) break;
+      same = more && now.group == here.group && now.b == here.b;
+      block_of_keys<D, R>(s, sum, sight, stage, tile * Space::kKeys, keys, here.s.length, p.a.scale * kLog2e, [&] {
+        if (same) request(now.tile, stage + 1);
+      });
     }
     if (float* part = part_of(p, share, here, segment)) {
 #pragma unroll
       for (int c = 0; c < D / 64; c++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          float x[4];
+        for (int e = 0; e < 4; e++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
+          for (int i = 0; i < R; i++) {
             const float2 o = pair_split(sum.o[i][c][e / 2]);
-            x[i] = e % 2 ? o.y : o.x;
+            part[(c * 64 + tx * 4 + e) * p.slot_rows + ty * R + i] = e % 2 ? o.y : o.x;
           }
-          *reinterpret_cast<float4*>(part + (c * 64 + tx * 4 + e) * p.slot_rows + ty * 4) = make_float4(x[0], x[1], x[2], x[3]);
-        }
 #pragma unroll
-      for (int i = 0; i < 4; i++)
-        if (tx == 0) store_statistics(p, part, ty * 4 + i, sum.m[i], sum.l[i]);
+      for (int i = 0; i < R; i++)
+        if (tx == 0) store_statistics(p, part, ty * R + i, sum.m[i], sum.l[i]);
       continue;
     }
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < R; i++) {
       int node, head;
-      if (!seg.place(p, ty * 4 + i, &node, &head)) continue;
+      if (!seg.place(p, ty * R + i, &node, &head)) continue;
       const float inverse = inverse_of(sum.l[i]);
-      T* out = static_cast<T*>(p.a.out) + out_at(p, seg, node, head);
+      float* out = static_cast<float*>(p.a.out) + out_at(p, seg, node, head);
 #pragma unroll
       for (int c = 0; c < D / 64; c++) {
         const float2 x = pair_split(sum.o[i][c][0]), y = pair_split(sum.o[i][c][1]);
@@ -429,32 +441,40 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const __grid
 // Which kernel a shape runs on.
 struct TreePlan {
   int dims, rows, keys;  // of a row, of a tile of queries, of a tile of keys
-  int threads;
+  int threads, per_sm;   // threads of a block, blocks an SM
   size_t smem;
 };
 
-// f(kernel, plan) for calls with `rows` query rows a sequence and KV head at most: two tiles read the keys once for up to 256 of them.
+// f(kernel, plan) for calls with `wanted` query rows a sequence and KV head at most: two tiles read the keys once for up to 256 of them, and in
+// f32 no more rows are computed than there are, up to 64.
 template <typename F>
-auto with_kernel(int dtype, int head_dim, long long rows, F&& f) {
-#define PJRTX_TREE_ROWS(D) return f(tree_rows_kernel<float, D>, TreePlan{D, rows::kRows, rows::kKeys, rows::kThreads, sizeof(rows::Shared<D>)})
+auto with_kernel(int dtype, int head_dim, long long wanted, F&& f) {
+#define PJRTX_TREE_ROWS(D, R) return f(tree_rows_kernel<D, R>, TreePlan{D, 16 * R, rows::keys_of(D), rows::kThreads, D == 64 ? 2 : 1, sizeof(rows::Shared<D, R>)})
+#define PJRTX_TREE_ROWS_OF(D)              \
+  {                                        \
+    if (wanted <= 16) PJRTX_TREE_ROWS(D, 1); \
+    if (wanted <= 32) PJRTX_TREE_ROWS(D, 2); \
+    PJRTX_TREE_ROWS(D, 4);                 \
+  }
 #define PJRTX_TREE_UMMA(BF16, D, TILES) \
   return f(umma::umma_tree_kernel<BF16, D, TILES>, \
-           TreePlan{D, TILES * umma::kAttnRows, umma::tree_keys(D), umma::tree_threads(TILES), umma::tree_smem(D, TILES)})
+           TreePlan{D, TILES * umma::kAttnRows, umma::tree_keys(D), umma::tree_threads(TILES), 1, umma::tree_smem(D, TILES)})
 #define PJRTX_TREE_UMMA_OF(BF16)                                                     \
   if (head_dim > 128) PJRTX_TREE_UMMA(BF16, 256, 1);                                 \
-  if (head_dim > 64 && rows > umma::kAttnRows) PJRTX_TREE_UMMA(BF16, 128, 2);        \
+  if (head_dim > 64 && wanted > umma::kAttnRows) PJRTX_TREE_UMMA(BF16, 128, 2);        \
   if (head_dim > 64) PJRTX_TREE_UMMA(BF16, 128, 1);                                  \
-  if (rows > umma::kAttnRows) PJRTX_TREE_UMMA(BF16, 64, 2);                          \
+  if (wanted > umma::kAttnRows) PJRTX_TREE_UMMA(BF16, 64, 2);                          \
   PJRTX_TREE_UMMA(BF16, 64, 1)
   if (dtype == kF32) {
-    if (head_dim <= 64) PJRTX_TREE_ROWS(64);
-    if (head_dim <= 128) PJRTX_TREE_ROWS(128);
-    PJRTX_TREE_ROWS(256);
+    if (head_dim <= 64) PJRTX_TREE_ROWS_OF(64)
+    if (head_dim <= 128) PJRTX_TREE_ROWS_OF(128)
+    PJRTX_TREE_ROWS_OF(256)
   }
   if (dtype == kF16) { PJRTX_TREE_UMMA_OF(false); }
   PJRTX_TREE_UMMA_OF(true);
 #undef PJRTX_TREE_UMMA_OF
 #undef PJRTX_TREE_UMMA
+#undef PJRTX_TREE_ROWS_OF
 #undef PJRTX_TREE_ROWS
 }
 
@@ -487,7 +507,8 @@ uint64_t round256(uint64_t n) { return (n + 255) / 256 * 256; }
 
 uint64_t paged_tree_workspace(const PagedView& c, int heads, int nodes, int sm_count) {
   return with_kernel(c.dtype, c.head_dim, (long long)nodes * (heads / c.kv_heads), [&](auto, const TreePlan& plan) {
-    return round256((uint64_t)sm_count * sizeof(Cut)) + (uint64_t)sm_count * 2 * plan.rows * (plan.dims + 2) * 4;
+    const uint64_t blocks = (uint64_t)sm_count * plan.per_sm;
+    return round256(blocks * sizeof(Cut)) + blocks * 2 * plan.rows * (plan.dims + 2) * 4;
   });
 }
 
@@ -499,7 +520,6 @@ int paged_tree_launch(const PagedView& c, const PagedTree& a, int sm_count, bool
   p.reciprocal = (unsigned)std::min<uint64_t>((1ull << 32) / c.page_size, 0xffffffffu);
   char* space = static_cast<char*>(a.workspace);
   p.cuts = reinterpret_cast<Cut*>(space);
-  p.parts = reinterpret_cast<float*>(space + round256((uint64_t)sm_count * sizeof(Cut)));
   long long segments = 0;
   const bool ok = with_kernel(c.dtype, c.head_dim, (long long)a.nodes * p.rep, [&](auto kernel, const TreePlan& plan) {
     p.heads = std::min(p.rep, plan.rows);
@@ -511,7 +531,8 @@ int paged_tree_launch(const PagedView& c, const PagedTree& a, int sm_count, bool
     if (!raise_smem_limit((const void*)kernel, (int)plan.smem)) return false;
     segments = (long long)c.batch * c.kv_heads * p.groups * ((a.nodes + p.nodes - 1) / p.nodes);
     const long long numbers = segments * ((c.capacity() + a.nodes + p.tile_keys - 1) / p.tile_keys + kSegmentCost);
-    p.blocks = (int)std::min<long long>(numbers, sm_count);
+    p.blocks = (int)std::min<long long>(numbers, (long long)sm_count * plan.per_sm);
+    p.parts = reinterpret_cast<float*>(space + round256((uint64_t)sm_count * plan.per_sm * sizeof(Cut)));
     return start(kernel, p, plan, pdl, stream);
   });
   if (!ok) return 0;
