@@ -151,7 +151,7 @@ struct PromptAttention {
   float scale = 1.f;
   int* error_words = nullptr;
 };
-int prompt_attention_launch(const PromptAttention& a, int sm_count, bool pdl, cudaStream_t stream);
+int prompt_attention_launch(const PromptAttention& a, bool pdl, cudaStream_t stream);
 
 struct TokenScore {
   int dtype = 0;

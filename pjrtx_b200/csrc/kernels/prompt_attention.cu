@@ -29,8 +29,8 @@ struct PromptTile {
 };
 
 // Tile `x` of the launch, for all lanes of a warp. Sequences that are not in order are skipped.
-__device__ __forceinline__ PromptTile prompt_tile(const PromptArgs& p, int positions, long long x) {
-  const int lane = threadIdx.x % 32, *starts = p.a.starts;
+__device__ __forceinline__ PromptTile prompt_tile(const PromptArgs& p, long long x) {
+  const int lane = threadIdx.x % 32, positions = p.positions, *starts = p.a.starts;
   int b = 0, n = p.a.sequences;
   while (n > 1) {  // the last sequence whose first tile is not behind x
     const int step = (n + 31) / 32, at = b + lane * step;
@@ -50,8 +50,8 @@ __device__ __forceinline__ PromptTile prompt_tile(const PromptArgs& p, int posit
 // The grid: heads by tiles, the tiles folded where one axis does not hold them.
 constexpr long long kGridAxis = 65535;
 __device__ __forceinline__ long long prompt_block() { return blockIdx.z * kGridAxis + blockIdx.y; }
-inline dim3 prompt_grid(const PromptArgs& p, int positions) {
-  const long long tiles = p.a.tokens / positions + p.a.sequences;
+inline dim3 prompt_grid(const PromptArgs& p) {
+  const long long tiles = p.a.tokens / p.positions + p.a.sequences;
   return dim3((unsigned)(p.a.kv_heads * p.groups), (unsigned)std::min(tiles, kGridAxis), (unsigned)((tiles + kGridAxis - 1) / kGridAxis));
 }
 
@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(rows::kThreads) prompt_rows_kernel(const __gri
   Space& s = *reinterpret_cast<Space*>(smem);
   const PromptAttention& a = p.a;
   check_starts(a);
-  const PromptTile t = prompt_tile(p, p.positions, prompt_block());
+  const PromptTile t = prompt_tile(p, prompt_block());
   if (t.tile < 0) return;
   const int g = blockIdx.x / p.groups, h0 = blockIdx.x % p.groups * p.heads, heads = min(p.heads, p.rep - h0);
   const int first = t.tile * p.positions, positions = min(p.positions, t.tokens - first);
@@ -150,28 +150,28 @@ int launch_rows(PromptArgs p, bool pdl, cudaStream_t stream) {
   p.heads = std::min(p.rep, Space::kRows);
   p.groups = (p.rep + p.heads - 1) / p.heads;
   p.positions = Space::kRows / p.heads;
-  return launch_kernel(prompt_rows_kernel<D>, prompt_grid(p, p.positions), dim3(rows::kThreads), sizeof(Space), stream, pdl, p) == cudaSuccess;
+  return launch_kernel(prompt_rows_kernel<D>, prompt_grid(p), dim3(rows::kThreads), sizeof(Space), stream, pdl, p) == cudaSuccess;
 }
 
-template <bool BF16, int HD, int TILES>
+template <bool BF16, int HD>
 int launch_umma(const umma::PromptKernelArgs& a, bool pdl, cudaStream_t stream) {
   const PromptAttention& p = a.p.a;
   const long long q_extents[4] = {p.head_dim, a.p.rep, p.kv_heads, p.tokens}, k_extents[3] = {p.head_dim, p.tokens, p.kv_heads};
   const long long q_strides[3] = {p.q_head_stride, a.p.rep * p.q_head_stride, p.q_stride};
   const long long k_strides[2] = {p.k_stride, p.k_head_stride}, v_strides[2] = {p.v_stride, p.v_head_stride};
-  const int q_box[4] = {64, a.p.heads, 1, a.p.positions}, k_box[3] = {64, umma::prompt_keys(HD), 1};
+  const int q_box[4] = {64, a.p.heads, 1, a.p.positions}, k_box[3] = {64, umma::kPromptKeys, 1};
   CUtensorMap qmap, kmap, vmap;
   if (!umma::encode_map(&qmap, p.q, !BF16, 4, q_extents, q_strides, q_box) || !umma::encode_map(&kmap, p.k, !BF16, 3, k_extents, k_strides, k_box) ||
       !umma::encode_map(&vmap, p.v, !BF16, 3, k_extents, v_strides, k_box))
     return 0;
-  constexpr size_t smem = umma::prompt_smem(HD, TILES);
-  auto kernel = umma::umma_prompt_kernel<BF16, HD, TILES>;
+  constexpr size_t smem = umma::prompt_smem(HD);
+  auto kernel = umma::umma_prompt_kernel<BF16, HD>;
   if (!raise_smem_limit((const void*)kernel, (int)smem)) return 0;
-  return launch_kernel(kernel, prompt_grid(a.p, TILES * a.p.positions), dim3(umma::prompt_threads(TILES)), smem, stream, pdl, a, qmap, kmap, vmap) == cudaSuccess;
+  return launch_kernel(kernel, prompt_grid(a.p), dim3(umma::kPromptThreads), smem, stream, pdl, a, qmap, kmap, vmap) == cudaSuccess;
 }
 
 template <bool BF16>
-int launch_umma_of(PromptArgs p, int sm_count, bool pdl, cudaStream_t stream) {
+int launch_umma_of(PromptArgs p, bool pdl, cudaStream_t stream) {
   umma::PromptKernelArgs a;
   p.heads = std::min(p.rep, umma::kAttnRows);
   p.groups = (p.rep + p.heads - 1) / p.heads;
@@ -181,21 +181,19 @@ int launch_umma_of(PromptArgs p, int sm_count, bool pdl, cudaStream_t stream) {
   a.scale_log2 = scale == 0.f ? 1.f : (scale < 0.f ? -scale : scale) * rows::kLog2e;
   a.sign = scale > 0.f ? 1.f : scale < 0.f ? -1.f : 0.f;
   a.timeout_ns = wait_timeout_ns();
-  const long long pairs = p.a.tokens / (2 * p.positions) * p.a.kv_heads * p.groups;
-  const bool two = pairs >= sm_count && p.a.tokens / p.a.sequences > p.positions;
-  if (p.a.head_dim > 128) return launch_umma<BF16, 256, 1>(a, pdl, stream);
-  if (p.a.head_dim > 64) return two ? launch_umma<BF16, 128, 2>(a, pdl, stream) : launch_umma<BF16, 128, 1>(a, pdl, stream);
-  return two ? launch_umma<BF16, 64, 2>(a, pdl, stream) : launch_umma<BF16, 64, 1>(a, pdl, stream);
+  return p.a.head_dim <= 64    ? launch_umma<BF16, 64>(a, pdl, stream)
+         : p.a.head_dim <= 128 ? launch_umma<BF16, 128>(a, pdl, stream)
+                               : launch_umma<BF16, 256>(a, pdl, stream);
 }
 
 }  // namespace
 
-int prompt_attention_launch(const PromptAttention& a, int sm_count, bool pdl, cudaStream_t stream) {
+int prompt_attention_launch(const PromptAttention& a, bool pdl, cudaStream_t stream) {
   PromptArgs p;
   p.a = a;
   p.rep = a.heads / a.kv_heads;
-  if (a.dtype == kF16) return launch_umma_of<false>(p, sm_count, pdl, stream);
-  if (a.dtype == kBF16) return launch_umma_of<true>(p, sm_count, pdl, stream);
+  if (a.dtype == kF16) return launch_umma_of<false>(p, pdl, stream);
+  if (a.dtype == kBF16) return launch_umma_of<true>(p, pdl, stream);
   return a.head_dim <= 64 ? launch_rows<64>(p, pdl, stream) : a.head_dim <= 128 ? launch_rows<128>(p, pdl, stream) : launch_rows<256>(p, pdl, stream);
 }
 

@@ -1,11 +1,15 @@
 // Causal attention of packed prompts on the 5th-generation tensor cores: scores, probabilities and results of a tile of 128 query rows
 // stay in tensor memory while its keys pass by in blocks (the formulas and the tiles are those of prompt_attention.cu).
 //
-// Roles of a block of threads, which has TILES tiles of neighbouring positions:
-//   copy warp      the queries once, then keys and values into a ring of shared-memory slots (tiled tensor-map copies, 128-byte swizzle)
-//   MMA warp       S_t = Q_t . K^T and O_t += P_t . V with P_t in tensor memory, for the tiles in turn: while the softmax warps of one
-//                  tile work, the tensor core has the other's products
-//   softmax warps  four a tile, a query row a thread (its lane of tensor memory), so a row's maximum and sum need no exchange
+// Roles of a block of threads, which has one tile; an SM has two, which overlap what either waits for (of 256 dimensions one):
+//   copy warp      the queries once, then keys and values, 64 at a time, into a ring of shared-memory slots (tiled tensor-map copies, 128-byte
+//                  swizzle)
+//   MMA warp       S = Q . K^T and O += P . V with P in tensor memory. The scores have two buffers, so that those of the next block are there
+//                  when the softmax warps are done with one
+//   softmax warps  four, a query row a thread (its lane of tensor memory), so a row's maximum and sum need no exchange
+//
+// Two tiles in a block of threads of twice the size, with blocks of 128 keys that they share and buffers for one block of scores each, were slower up to
+// 4096 tokens: 517 of 32 heads over 8 14.4 us (10.8), 64 x 20 28 (16), 4 x 2048 162 (149), 2 x 4096 258 (254); 2 x 8192 916 (947).
 //
 // Hidden keys have probability 0, but the tensor core multiplies it by their values, and 0 times infinity or NaN is NaN. So values
 // behind the last position of the block of threads are cleared in shared memory, and a row with a result that is not finite looks at
@@ -24,16 +28,16 @@ struct PromptKernelArgs {
   unsigned long long timeout_ns;
 };
 
-__host__ __device__ constexpr int prompt_keys(int hd) { return hd == 256 ? 64 : 128; }  // of a block
-constexpr int kPromptSlots = 5;
-__host__ __device__ constexpr int prompt_threads(int tiles) { return tiles == 2 ? 384 : 192; }
-__host__ __device__ constexpr int prompt_per_sm(int hd, int tiles) { return hd == 64 && tiles == 1 ? 2 : 1; }
-__host__ __device__ constexpr uint32_t prompt_tmem(int hd, int tiles) { return tiles == 2 || hd == 256 ? 512 : 256; }
-__host__ __device__ constexpr size_t prompt_smem(int hd, int tiles) {
-  const size_t bytes = (size_t)tiles * kAttnRows * hd * 2 + (size_t)kPromptSlots * prompt_keys(hd) * hd * 2 + 512 + 1024;
-  const size_t least = least_smem(prompt_per_sm(hd, tiles) == 2 ? 256 : 512);
+constexpr int kPromptKeys = 64, kPromptThreads = 192;
+__host__ __device__ constexpr int prompt_slots(int hd) { return hd == 256 ? 5 : hd == 128 ? 4 : 8; }
+__host__ __device__ constexpr int prompt_per_sm(int hd) { return hd <= 128 ? 2 : 1; }
+__host__ __device__ constexpr uint32_t prompt_tmem(int hd) { return prompt_per_sm(hd) == 2 ? 256 : 512; }
+__host__ __device__ constexpr size_t prompt_smem(int hd) {
+  const size_t bytes = (size_t)kAttnRows * hd * 2 + (size_t)prompt_slots(hd) * kPromptKeys * hd * 2 + 512 + 1024;
+  const size_t least = least_smem(prompt_tmem(hd));
   return bytes < least ? least : bytes;
 }
+static_assert(prompt_smem(128) <= kSharedSmem && prompt_smem(64) <= kSharedSmem, "two blocks of threads an SM");
 
 __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_dst),
@@ -78,43 +82,38 @@ __device__ __noinline__ void redo_row(const PromptKernelArgs& a, const unsigned 
     if (e * 32 + lane < p.head_dim) reinterpret_cast<T*>(out)[e * 32 + lane] = rows::from_float<T>(o[e] * inverse);
 }
 
-template <bool BF16, int HD, int TILES>
-__global__ void __launch_bounds__(prompt_threads(TILES), prompt_per_sm(HD, TILES))
+template <bool BF16, int HD>
+__global__ void __launch_bounds__(kPromptThreads, prompt_per_sm(HD))
 umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                    const __grid_constant__ CUtensorMap vmap) {
-  constexpr int kKeys = prompt_keys(HD), kHalves = HD / 64, kSlots = kPromptSlots;
+  constexpr int kKeys = kPromptKeys, kHalves = HD / 64, kSlots = prompt_slots(HD);
   constexpr uint32_t kTileBytes = kAttnRows * HD * 2, kSlotBytes = kKeys * HD * 2;
   constexpr uint32_t kQueryBlock = kAttnRows * 128, kKeyBlock = kKeys * 128;  // bytes of 64 elements of all rows
-  constexpr uint32_t kTmemCols = prompt_tmem(HD, TILES);
-  static_assert(TILES * (kKeys + HD) <= kTmemCols, "");
+  constexpr uint32_t kTmemCols = prompt_tmem(HD);
+  static_assert(2 * kKeys + HD <= kTmemCols, "");
   extern __shared__ unsigned char smem_dyn[];
   const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
   unsigned char* base_ptr = smem_dyn + (base - smem_u32(smem_dyn));
-  const uint32_t ring = base + TILES * kTileBytes;
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(base_ptr + TILES * kTileBytes + kSlots * kSlotBytes);
+  const uint32_t ring = base + kTileBytes;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(base_ptr + kTileBytes + kSlots * kSlotBytes);
   uint64_t* slot_full = q_full + 1;             // [kSlots]
   uint64_t* slot_empty = slot_full + kSlots;    // [kSlots]
   uint64_t* v_clean = slot_empty + kSlots;      // values behind the last position have been cleared
-  uint64_t* s_full = v_clean + 1;               // [TILES] scores of the next block are in tensor memory
-  uint64_t* p_ready = s_full + TILES;           // [TILES] probabilities are in tensor memory, O may be accumulated
-  uint64_t* o_full = p_ready + TILES;           // [TILES] the last product has completed
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + TILES);
+  uint64_t* s_full = v_clean + 1;  // [2] scores of a block are in tensor memory, and the product two blocks before it is done
+  uint64_t* p_ready = s_full + 2;  // [2] its probabilities are
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_ready + 2);
   int* flags = reinterpret_cast<int*>(tmem_slot + 1);  // [0] abort
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kMmaWarp = 4 * TILES, kCopyWarp = 4 * TILES + 1;
+  constexpr int kMmaWarp = 4, kCopyWarp = 5;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const PromptAttention& p = a.p.a;
   check_starts(p);
-  const PromptTile item = prompt_tile(a.p, TILES * a.p.positions, prompt_block());
+  const PromptTile item = prompt_tile(a.p, prompt_block());
   if (item.tile < 0) return;
   const WaitBudget budget{global_timer_ns() + a.timeout_ns, flags};
   const int g = blockIdx.x / a.p.groups, h0 = blockIdx.x % a.p.groups * a.p.heads, heads = min(a.p.heads, a.p.rep - h0);
-  const int first = item.tile * TILES * a.p.positions;
-  const int keys = min(first + TILES * a.p.positions, item.tokens);  // behind the last position of the block
-  // Of a tile: its positions, and the blocks of keys up to the last of them (0: there is no such tile).
-  auto first_of = [&](int t) { return first + t * a.p.positions; };
-  auto blocks_of = [&](int t) { return first_of(t) >= keys ? 0 : (min(first_of(t) + a.p.positions, keys) + kKeys - 1) / kKeys; };
+  const int first = item.tile * a.p.positions, keys = min(first + a.p.positions, item.tokens);  // the first position, and behind the last
   const int blocks = (keys + kKeys - 1) / kKeys;
   const bool ragged = keys % kKeys != 0;
 
@@ -125,10 +124,9 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
       mbar_init(&slot_empty[s], 1);
     }
     mbar_init(v_clean, 1);
-    for (int t = 0; t < TILES; t++) {
-      mbar_init(&s_full[t], 1);
-      mbar_init(&p_ready[t], 4);
-      mbar_init(&o_full[t], 1);
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_ready[i], 4);
     }
     flags[0] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -142,25 +140,22 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem_base = *tmem_slot;
-  auto s_col = [&](int t) { return tmem_base + (uint32_t)(t * kKeys); };
-  auto o_col = [&](int t) { return tmem_base + (uint32_t)(TILES * kKeys + t * HD); };
+  auto s_col = [&](int buffer) { return tmem_base + (uint32_t)(buffer * kKeys); };
+  const uint32_t o_col = tmem_base + 2 * kKeys;
 
-  if (warp >= 4 * TILES) {
-    if constexpr (TILES == 2) leave_registers<104>();
+  if (warp >= 4) {
     const bool leader = elect_one();
     if (warp == kCopyWarp) {
-      // K0 V0 K1 V1 ...
+      // In the order in which the products use them: K0 K1 V0 K2 V1 ..
       if (leader) {
-        mbar_expect_tx(q_full, (blocks_of(TILES - 1) ? TILES : 1) * kHalves * (uint32_t)(a.p.heads * a.p.positions) * 128u);
-        for (int t = 0; t < TILES; t++)
-          if (blocks_of(t))
-            for (int c = 0; c < kHalves; c++)
-              tma_load_4d(base + t * kTileBytes + c * kQueryBlock, &qmap, c * 64, h0, g, item.start + first_of(t), q_full);
+        mbar_expect_tx(q_full, kHalves * (uint32_t)(a.p.heads * a.p.positions) * 128u);
+        for (int c = 0; c < kHalves; c++) tma_load_4d(base + c * kQueryBlock, &qmap, c * 64, h0, g, item.start + first, q_full);
       }
       __syncwarp();
       int slot = 0;
       unsigned phase = 0;
       bool ok = true;
+      int keys_of = 0, values_of = 0;  // the next blocks
       for (int i = 0; i < 2 * blocks; i++) {
         if (i >= kSlots && !__all_sync(0xffffffffu, mbar_wait(&slot_empty[slot], phase ^ 1, budget))) {
           // The copies in flight get a bounded time to land before the block of threads leaves.
@@ -172,11 +167,13 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
           ok = false;
           break;
         }
+        const bool is_keys = keys_of < blocks && keys_of < values_of + 2;
+        const int block = is_keys ? keys_of++ : values_of++;
         if (leader) {
-          const CUtensorMap* map = (i & 1) ? &vmap : &kmap;
+          const CUtensorMap* map = is_keys ? &kmap : &vmap;
           const uint32_t dst = ring + (uint32_t)slot * kSlotBytes;
           mbar_expect_tx(&slot_full[slot], kSlotBytes);
-          for (int c = 0; c < kHalves; c++) tma_load_3d(dst + c * kKeyBlock, map, c * 64, item.start + (i >> 1) * kKeys, g, &slot_full[slot]);
+          for (int c = 0; c < kHalves; c++) tma_load_3d(dst + c * kKeyBlock, map, c * 64, item.start + block * kKeys, g, &slot_full[slot]);
         }
         __syncwarp();
         if (++slot == kSlots) {
@@ -187,7 +184,7 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
       if (ok && ragged) {
         const int last = 2 * blocks - 1;
         if (__all_sync(0xffffffffu, mbar_wait(&slot_full[last % kSlots], (unsigned)(last / kSlots) & 1u, budget))) {
-          unsigned char* rows0 = base_ptr + TILES * kTileBytes + (last % kSlots) * kSlotBytes;
+          unsigned char* rows0 = base_ptr + kTileBytes + (last % kSlots) * kSlotBytes;
           const int from = keys % kKeys * 8;  // pieces of 16 bytes
           for (int c = 0; c < kHalves; c++)
             for (int i = from + lane; i < kKeys * 8; i += 32) *reinterpret_cast<uint4*>(rows0 + c * kKeyBlock + i * 16) = make_uint4(0, 0, 0, 0);
@@ -214,55 +211,47 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
       };
       auto wait = [&](uint64_t* bar, unsigned parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, budget)) != 0; };
       // Issued by the elected thread.
-      auto scores = [&](int t, int k_slot) {
-        const uint64_t q = desc_advance(q_first, t * kTileBytes), k = desc_advance(k_first, (uint32_t)k_slot * kSlotBytes);
+      auto scores = [&](int buffer, int k_slot) {
+        const uint64_t k = desc_advance(k_first, (uint32_t)k_slot * kSlotBytes);
 #pragma unroll
         for (int kk = 0; kk < HD / 16; kk++)
-          mma_f16(s_col(t), desc_advance(q, (uint32_t)(kk >> 2) * kQueryBlock + (uint32_t)(kk & 3) * 32u),
+          mma_f16(s_col(buffer), desc_advance(q_first, (uint32_t)(kk >> 2) * kQueryBlock + (uint32_t)(kk & 3) * 32u),
                   desc_advance(k, (uint32_t)(kk >> 2) * kKeyBlock + (uint32_t)(kk & 3) * 32u), idesc_s, kk ? 1u : 0u);
-        mma_commit(&s_full[t]);
       };
-      auto values = [&](int t, int v_slot, bool accumulate) {
-        const uint64_t v = desc_advance(v_first, (uint32_t)v_slot * kSlotBytes);
+      bool ok = wait(q_full, 0);
 #pragma unroll
-        for (int kk = 0; kk < kKeys / 16; kk++)
-          mma_f16_tmem_a(o_col(t), s_col(t) + (uint32_t)kk * 8u, desc_advance(v, (uint32_t)kk * 2048u), idesc_o, (accumulate || kk) ? 1u : 0u);
-      };
-      bool ok = wait(q_full, 0) && wait(&slot_full[0], 0);
-      if (ok) {
+      for (int i = 0; i < 2; i++) {
+        if (!ok || i >= blocks) continue;
+        const unsigned k_phase = phase;
+        const int k_slot = next_slot();
+        ok = wait(&slot_full[k_slot], k_phase);
+        if (!ok) continue;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (leader) {
-          for (int t = 0; t < TILES; t++)
-            if (blocks_of(t)) scores(t, 0);
-          mma_commit(&slot_empty[0]);
+          scores(i, k_slot);
+          mma_commit(&s_full[i]);
+          mma_commit(&slot_empty[k_slot]);
         }
         __syncwarp();
-        next_slot();
       }
-      int of_tile[TILES];
-#pragma unroll
-      for (int t = 0; t < TILES; t++) of_tile[t] = blocks_of(t);
       for (int j = 0; j < blocks && ok; j++) {
+        const int buffer = j & 1;
         const unsigned v_phase = phase;
         const int v_slot = next_slot();
         const unsigned k_phase = phase;
-        const bool more = j + 1 < blocks;
+        const bool more = j + 2 < blocks;
         const int k_slot = more ? next_slot() : 0;
-        ok = wait(&slot_full[v_slot], v_phase) && (more || !ragged || wait(v_clean, 0)) && (!more || wait(&slot_full[k_slot], k_phase));
+        ok = wait(&slot_full[v_slot], v_phase) && (j + 1 < blocks || !ragged || wait(v_clean, 0)) && (!more || wait(&slot_full[k_slot], k_phase)) &&
+             wait(&p_ready[buffer], (unsigned)(j >> 1) & 1u);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (leader) {
+          const uint64_t v = desc_advance(v_first, (uint32_t)v_slot * kSlotBytes);
 #pragma unroll
-        for (int t = 0; t < TILES; t++) {
-          if (!ok || j >= of_tile[t]) continue;
-          ok = wait(&p_ready[t], (unsigned)j & 1u);
-          if (!ok) continue;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          if (leader) {
-            values(t, v_slot, j > 0);
-            if (j + 1 < of_tile[t]) scores(t, k_slot);
-            else mma_commit(&o_full[t]);
-          }
-          __syncwarp();
-        }
-        if (ok && leader) {
+          for (int kk = 0; kk < kKeys / 16; kk++)
+            mma_f16_tmem_a(o_col, s_col(buffer) + (uint32_t)kk * 8u, desc_advance(v, (uint32_t)kk * 2048u), idesc_o, (j > 0 || kk) ? 1u : 0u);
+          if (more) scores(buffer, k_slot);
+          mma_commit(&s_full[buffer]);
           mma_commit(&slot_empty[v_slot]);
           if (more) mma_commit(&slot_empty[k_slot]);
         }
@@ -272,20 +261,18 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
       __syncwarp();
     }
   } else {
-    if constexpr (TILES == 2) take_registers<200>();
-    const int t = warp >> 2;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = s_col(t) + lanes, o_addr = o_col(t) + lanes;
-    const int row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16, o_addr = o_col + lanes;
+    const int row = warp * 32 + lane;
     // Rows that are not there have position -1: every key is hidden and nothing is stored.
     const int head = row % a.p.heads, at = row / a.p.heads;
-    const int pos = at < a.p.positions && head < heads && first_of(t) + at < keys ? first_of(t) + at : -1;
-    const int first_pos = first_of(t) + (warp & 3) * 32 / a.p.heads;  // of the warp
-    const int mine = blocks_of(t);
+    const int pos = at < a.p.positions && head < heads && first + at < keys ? first + at : -1;
+    const int first_pos = first + warp * 32 / a.p.heads;  // of the warp
     float m_used = -INFINITY, sum = 0.f;
     bool ok = true;
-    for (int j = 0; j < mine; j++) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], (unsigned)j & 1u, budget));
+    for (int j = 0; j < blocks; j++) {
+      const int buffer = j & 1;
+      const uint32_t s_addr = s_col(buffer) + lanes;
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[buffer], (unsigned)(j >> 1) & 1u, budget));
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       float s[kKeys];
@@ -311,6 +298,10 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
         sum *= corr;
       }
       if (j > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
+        // The product of the block before may still be adding to the results.
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[buffer ^ 1], (unsigned)(((j - 1) >> 1) + 1) & 1u, budget));
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
         for (int c = 0; c < HD; c += 32) {
           float o[32];
@@ -330,10 +321,10 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_ready[t]);
+      if (lane == 0) mbar_arrive(&p_ready[buffer]);
     }
-    ok = ok && (mine == 0 || __all_sync(0xffffffffu, mbar_wait(&o_full[t], 0, budget)));
-    if (ok && mine > 0) {
+    ok = ok && __all_sync(0xffffffffu, mbar_wait(&s_full[(blocks - 1) & 1], (unsigned)(((blocks - 1) >> 1) + 1) & 1u, budget));
+    if (ok) {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const float inverse = rows::inverse_of(sum);
       const int h = g * a.p.rep + h0 + head;
@@ -365,10 +356,9 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
       const unsigned short* v = static_cast<const unsigned short*>(p.v) + (long long)item.start * p.v_stride + (long long)g * p.v_head_stride;
       for (unsigned left = __ballot_sync(0xffffffffu, odd && pos >= 0); left; left &= left - 1) {
         const int r = __ffs(left) - 1, row_pos = __shfl_sync(0xffffffffu, pos, r), row_h = __shfl_sync(0xffffffffu, h, r);
-        const int hidden = min(mine * kKeys, keys);
         bool spoilt = false;
         const int pieces = p.head_dim / 8;
-        for (long long i = (long long)(row_pos + 1) * pieces + lane; i < (long long)hidden * pieces; i += 32) {
+        for (long long i = (long long)(row_pos + 1) * pieces + lane; i < (long long)keys * pieces; i += 32) {
           const uint4 x = *reinterpret_cast<const uint4*>(v + i / pieces * p.v_stride + i % pieces * 8);
           spoilt = spoilt || odd_pair<BF16>(x.x) || odd_pair<BF16>(x.y) || odd_pair<BF16>(x.z) || odd_pair<BF16>(x.w);
         }
@@ -378,7 +368,7 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
                            static_cast<unsigned short*>(p.out) + token * p.out_stride + row_h * p.out_head_stride, row_pos,
                            __shfl_sync(0xffffffffu, m_used, r), __shfl_sync(0xffffffffu, sum, r));
       }
-    } else if (!ok && lane == 0) {
+    } else if (lane == 0) {
       report(p.error_words, kErrorWait);
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

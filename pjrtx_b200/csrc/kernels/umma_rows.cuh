@@ -80,14 +80,6 @@ __device__ __forceinline__ void store_probabilities(const float* s, float scale,
   if constexpr (N == 64) tmem_store_32(to, packed);
   else tmem_store_16(to, packed);
 }
-template <int REGISTERS>
-__device__ __forceinline__ void take_registers() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGISTERS));
-}
-template <int REGISTERS>
-__device__ __forceinline__ void leave_registers() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGISTERS));
-}
 // Whether one of two packed 16-bit elements is infinite or NaN.
 template <bool BF16>
 __device__ __forceinline__ bool odd_pair(uint32_t w) {

@@ -272,7 +272,7 @@ int prompt_attention(int ordinal, PromptAttention a, int64_t heads, int64_t kv_h
   a.error_words = dev->operator_words_dev;
   CurrentDevice scope(dev->ordinal);
   if (!entered(scope, dev)) return 0;
-  return launched(prompt_attention_launch(a, dev->sm_count, true, stream), "prompt attention");
+  return launched(prompt_attention_launch(a, true, stream), "prompt attention");
 }
 
 namespace {
