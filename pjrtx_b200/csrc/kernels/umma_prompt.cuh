@@ -90,7 +90,7 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
   constexpr uint32_t kTileBytes = kAttnRows * HD * 2, kSlotBytes = kKeys * HD * 2;
   constexpr uint32_t kQueryBlock = kAttnRows * 128, kKeyBlock = kKeys * 128;  // bytes of 64 elements of all rows
   constexpr uint32_t kTmemCols = prompt_tmem(HD);
-  static_assert(2 * kKeys + HD <= kTmemCols, "");
+  static_assert(kKeys == 64 && 2 * kKeys + HD <= kTmemCols, "");
   extern __shared__ unsigned char smem_dyn[];
   const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
   unsigned char* base_ptr = smem_dyn + (base - smem_u32(smem_dyn));
@@ -275,49 +275,48 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
       ok = __all_sync(0xffffffffu, mbar_wait(&s_full[buffer], (unsigned)(j >> 1) & 1u, budget));
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      float s[kKeys];
+      float s[kKeys / 32][32];
 #pragma unroll
-      for (int c = 0; c < kKeys / 32; c++) tmem_load_32(s_addr + c * 32, s + c * 32);
+      for (int c = 0; c < kKeys / 32; c++) tmem_load_32(s_addr + c * 32, s[c]);
       asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
       if (a.sign != 1.f) {
 #pragma unroll
-        for (int e = 0; e < kKeys; e++) s[e] *= a.sign;
+        for (int e = 0; e < kKeys; e++) s[e / 32][e % 32] *= a.sign;
       }
       const int key0 = j * kKeys;
       if (key0 + kKeys - 1 > first_pos) {
 #pragma unroll
         for (int e = 0; e < kKeys; e++)
-          if (key0 + e > pos) s[e] = -INFINITY;
+          if (key0 + e > pos) s[e / 32][e % 32] = -INFINITY;
       }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      const float m_block = max_of<kKeys>(s, mx) * a.scale_log2;
-      float corr = 1.f;
-      if (m_block > m_used + Probability<BF16>::kGrow) {
-        corr = exp2_approx(m_used - m_block);  // 0 the first time
-        m_used = m_block;
+      max_of<32>(s[0], mx);
+      const float m_block = max_of<32>(s[1], mx) * a.scale_log2;
+      if (__any_sync(0xffffffffu, m_block > m_used + Probability<BF16>::kGrow)) {
+        const float top = fmaxf(m_used, m_block), corr = top == m_used ? 1.f : exp2_approx(m_used - top);  // 0 the first time
+        m_used = top;
         sum *= corr;
-      }
-      if (j > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
-        // The product of the block before may still be adding to the results.
-        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[buffer ^ 1], (unsigned)(((j - 1) >> 1) + 1) & 1u, budget));
-        if (!ok) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (j > 0) {
+          // The product of the block before may still be adding to the results.
+          ok = __all_sync(0xffffffffu, mbar_wait(&s_full[buffer ^ 1], (unsigned)(((j - 1) >> 1) + 1) & 1u, budget));
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-        for (int c = 0; c < HD; c += 32) {
-          float o[32];
-          tmem_load_32(o_addr + c, o);
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          for (int c = 0; c < HD; c += 32) {
+            float o[32];
+            tmem_load_32(o_addr + c, o);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-          for (int e = 0; e < 32; e++) o[e] *= corr;
-          tmem_store_32(o_addr + c, o);
+            for (int e = 0; e < 32; e++) o[e] *= corr;
+            tmem_store_32(o_addr + c, o);
+          }
         }
       }
       const float shift = m_used == -INFINITY ? 0.f : Probability<BF16>::kLift - m_used;
       float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < kKeys / 64; c++) store_probabilities<BF16, 64, 2>(s + c * 64, a.scale_log2, shift, part, s_addr + c * 32);
+      for (int c = 0; c < kKeys / 32; c++) store_probabilities<BF16>(s[c], a.scale_log2, shift, part, s_addr + c * 16);
       sum += (part[0] + part[1]) + (part[2] + part[3]);
-      if (!(m_block < INFINITY)) sum = NAN;  // a score of NaN or infinity, which not every way to 2^x passes on
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();

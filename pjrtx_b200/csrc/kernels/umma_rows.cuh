@@ -14,44 +14,25 @@ namespace umma {
 // Probabilities go to the tensor core in the element type, and the sum is taken of them as they are then, so that equal values under all
 // keys give that value. In f16 they are multiplied by 2^11 first: f16 then holds them down to 2^-35 of the largest, and not only to 2^-24.
 // They are relative to a maximum that follows the row's when that has grown by 2^8 (f16: 2^4, so that they stay below 2^16): the factor
-// cancels in the division, and the results in tensor memory are rescaled that much more rarely.
+// cancels in the division, and the results in tensor memory are rescaled that much more rarely. Where one row of a warp has to, all of them
+// follow theirs, so that the next time is later.
 template <bool BF16> struct Probability { static constexpr float kLift = 0.f, kGrow = 8.f; };
 template <> struct Probability<false> { static constexpr float kLift = 11.f, kGrow = 4.f; };
 
-// NaN where one of them is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float y;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
 
-// The largest of a row's N scores; four chains.
+// The largest of N of a row's scores and of those before them, which `mx` has in four chains.
 template <int N>
 __device__ __forceinline__ float max_of(const float* s, float (&mx)[4]) {
 #pragma unroll
   for (int e = 0; e < N; e += 8)
 #pragma unroll
     for (int i = 0; i < 4; i++) mx[i] = max3(mx[i], s[e + 2 * i], s[e + 2 * i + 1]);
-  return max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3]));
-}
-
-// 2^x of two numbers on the FMA units, x <= 127: x = n + f with the whole number n nearest to x (what adding 1.5 * 2^23 leaves in the
-// lowest bits), 2^f for |f| <= 1/2 by a polynomial of degree four whose largest relative error is the least possible with 1 at f = 0
-// (2^-18.4; its coefficients solve that linear programme), n added to the exponent. From -127 down the result is 0. The exponential unit gives 16
-// results a cycle and SM, so that a block of 128 x 128 keeps it busy for 1024 cycles, as long as its products take; the FMA units have
-// time left.
-__device__ __forceinline__ float2 exp2_by_fma(float2 x) {
-  const Pair magic = pair_of(12582912.f, 12582912.f), back = pair_of(-12582912.f, -12582912.f), minus = pair_of(-1.f, -1.f), one = pair_of(1.f, 1.f);
-  const Pair v = pair_of(fmaxf(x.x, -127.f), fmaxf(x.y, -127.f));
-  const Pair t = pair_add(v, magic);
-  const Pair f = pair_fma(pair_add(t, back), minus, v);
-  Pair y = pair_fma(f, pair_of(0.009585382416844368f, 0.009585382416844368f), pair_of(0.05590662732720375f, 0.05590662732720375f));
-  y = pair_fma(f, y, pair_of(0.24024038016796112f, 0.24024038016796112f));
-  y = pair_fma(f, y, pair_of(0.6931241750717163f, 0.6931241750717163f));
-  y = pair_fma(f, y, one);
-  const float2 r = pair_split(y), n = pair_split(t);
-  return make_float2(__uint_as_float((__float_as_uint(n.x) << 23) + __float_as_uint(r.x)),
-                     __uint_as_float((__float_as_uint(n.y) << 23) + __float_as_uint(r.y)));
+  return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
 }
 
 __device__ __forceinline__ void tmem_store_16(uint32_t addr, const float* v) {
@@ -63,22 +44,21 @@ __device__ __forceinline__ void tmem_store_16(uint32_t addr, const float* v) {
       : "memory");
 }
 
-// Probabilities 2^(s * scale + shift) of N scores (32 or 64) into N / 2 columns of tensor memory, as pairs of the element type; `part` adds
-// them up. Of every eight pairs, FMA go by the FMA units.
-template <bool BF16, int N, int FMA>
-__device__ __forceinline__ void store_probabilities(const float* s, float scale, float shift, float (&part)[4], uint32_t to) {
+// Probabilities 2^(s * scale + shift) of 32 scores into 16 columns of tensor memory, as pairs of the element type; `part` adds them up.
+// All by the exponential unit, 16 results a cycle and SM: to compute some on the FMA units instead (a polynomial behind a split of the
+// exponent) made every case slower, 2 to 15 %, by the code that it takes.
+template <bool BF16>
+__device__ __forceinline__ void store_probabilities(const float (&s)[32], float scale, float shift, float (&part)[4], uint32_t to) {
   const Pair scale2 = pair_of(scale, scale), shift2 = pair_of(shift, shift);
-  float packed[N / 2];
+  float packed[16];
 #pragma unroll
-  for (int e = 0; e < N / 2; e++) {
+  for (int e = 0; e < 16; e++) {
     const float2 x = pair_split(pair_fma(pair_of(s[2 * e], s[2 * e + 1]), scale2, shift2));
-    const float2 y = e % 8 >= 8 - FMA ? exp2_by_fma(x) : make_float2(exp2_approx(x.x), exp2_approx(x.y));
-    const uint32_t pair = pack_pair<BF16>(y.x, y.y);
+    const uint32_t pair = pack_pair<BF16>(exp2_approx(x.x), exp2_approx(x.y));
     add_pair<BF16>(pair, part[(2 * e) & 3], part[(2 * e + 1) & 3]);
     packed[e] = __uint_as_float(pair);
   }
-  if constexpr (N == 64) tmem_store_32(to, packed);
-  else tmem_store_16(to, packed);
+  tmem_store_16(to, packed);
 }
 // Whether one of two packed 16-bit elements is infinite or NaN.
 template <bool BF16>

@@ -25,7 +25,6 @@ namespace pjrtx {
 namespace umma {
 
 constexpr int kTreeLoaders = 4;
-constexpr int kByFma = 0;
 constexpr int kOddRing = 16, kCleanRing = 16;  // longer than a checker can be ahead, which has the slots
 __host__ __device__ constexpr int tree_keys(int hd) { return hd == 256 ? 64 : 128; }
 __host__ __device__ constexpr int tree_slot_bytes(int hd) { return tree_keys(hd) * hd * 2; }
@@ -558,25 +557,24 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
           }
           m_block *= a.scale_log2;
           if (special) asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-          float corr = 1.f;
-          if (m_block > m_used + Probability<BF16>::kGrow) {
-            corr = exp2_approx(m_used - m_block);  // 0 the first time
-            m_used = m_block;
+          if (__any_sync(0xffffffffu, m_block > m_used + Probability<BF16>::kGrow)) {
+            const float top = fmaxf(m_used, m_block), corr = top == m_used ? 1.f : exp2_approx(m_used - top);  // 0 the first time
+            m_used = top;
             sum *= corr;
-          }
-          if (!first && __any_sync(0xffffffffu, corr != 1.f)) {
-            // With two buffers the product of the step before may still be adding to the results.
-            if (kBuffers == 2) ok = wait(&bar.s_full[t][buffer ^ 1], (unsigned)((step - 1) / 2 + 1) & 1u);
-            if (!ok) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (!first) {
+              // With two buffers the product of the step before may still be adding to the results.
+              if (kBuffers == 2) ok = wait(&bar.s_full[t][buffer ^ 1], (unsigned)((step - 1) / 2 + 1) & 1u);
+              if (!ok) break;
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-            for (int c = 0; c < HD; c += 32) {
-              float o[32];
-              tmem_load_32(o_addr + c, o);
-              asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+              for (int c = 0; c < HD; c += 32) {
+                float o[32];
+                tmem_load_32(o_addr + c, o);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-              for (int e = 0; e < 32; e++) o[e] *= corr;
-              tmem_store_32(o_addr + c, o);
+                for (int e = 0; e < 32; e++) o[e] *= corr;
+                tmem_store_32(o_addr + c, o);
+              }
             }
           }
           const float shift = m_used == -INFINITY ? 0.f : Probability<BF16>::kLift - m_used;
@@ -589,10 +587,9 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
             for (int h = 0; h < 2; h++) {
               asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
               if (c + h * 32 + 32 < kKeys) tmem_load_32(s_addr + c + h * 32 + 32, s[h ^ 1]);
-              store_probabilities<BF16, 32, kByFma>(s[h], a.scale_log2, shift, part, s_addr + (c + h * 32) / 2);
+              store_probabilities<BF16>(s[h], a.scale_log2, shift, part, s_addr + (c + h * 32) / 2);
             }
           sum += (part[0] + part[1]) + (part[2] + part[3]);
-          if (!(m_block < INFINITY)) sum = NAN;  // a score of NaN or infinity, which not every way to 2^x passes on
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         }
