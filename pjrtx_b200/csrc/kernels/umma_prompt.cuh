@@ -313,10 +313,11 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
         }
       }
       const float shift = m_used == -INFINITY ? 0.f : Probability<BF16>::kLift - m_used;
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
+      Pair part[2] = {0, 0};
 #pragma unroll
       for (int c = 0; c < kKeys / 32; c++) store_probabilities<BF16>(s[c], a.scale_log2, shift, part, s_addr + c * 16);
-      sum += (part[0] + part[1]) + (part[2] + part[3]);
+      const float2 block = pair_split(pair_add(part[0], part[1]));
+      sum += block.x + block.y;
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();

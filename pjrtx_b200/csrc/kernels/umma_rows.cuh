@@ -11,8 +11,10 @@
 namespace pjrtx {
 namespace umma {
 
-// Probabilities go to the tensor core in the element type, and the sum is taken of them as they are then, so that equal values under all
-// keys give that value. In f16 they are multiplied by 2^11 first: f16 then holds them down to 2^-35 of the largest, and not only to 2^-24.
+// Probabilities go to the tensor core in the element type: two 16-bit numbers for each would make the second product twice as long, and as
+// one they add about as much to a result's error as its own rounding does. Their sum is taken before they are rounded, since the log-sum-exp
+// is f32 (of the rounded ones it would be off by up to 2^-9). In f16 they are multiplied by 2^11 first: f16 then holds them down to
+// 2^-35 of the largest, and not only to 2^-24.
 // They are relative to a maximum that follows the row's when that has grown by 2^8 (f16: 2^4, so that they stay below 2^16): the factor
 // cancels in the division, and the results in tensor memory are rescaled that much more rarely. Where one row of a warp has to, all of them
 // follow theirs, so that the next time is later.
@@ -48,15 +50,15 @@ __device__ __forceinline__ void tmem_store_16(uint32_t addr, const float* v) {
 // All by the exponential unit, 16 results a cycle and SM: to compute some on the FMA units instead (a polynomial behind a split of the
 // exponent) made every case slower, 2 to 15 %, by the code that it takes.
 template <bool BF16>
-__device__ __forceinline__ void store_probabilities(const float (&s)[32], float scale, float shift, float (&part)[4], uint32_t to) {
+__device__ __forceinline__ void store_probabilities(const float (&s)[32], float scale, float shift, Pair (&part)[2], uint32_t to) {
   const Pair scale2 = pair_of(scale, scale), shift2 = pair_of(shift, shift);
   float packed[16];
 #pragma unroll
   for (int e = 0; e < 16; e++) {
     const float2 x = pair_split(pair_fma(pair_of(s[2 * e], s[2 * e + 1]), scale2, shift2));
-    const uint32_t pair = pack_pair<BF16>(exp2_approx(x.x), exp2_approx(x.y));
-    add_pair<BF16>(pair, part[(2 * e) & 3], part[(2 * e + 1) & 3]);
-    packed[e] = __uint_as_float(pair);
+    const float2 y = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+    part[e & 1] = pair_add(part[e & 1], pair_of(y.x, y.y));
+    packed[e] = __uint_as_float(pack_pair<BF16>(y.x, y.y));
   }
   tmem_store_16(to, packed);
 }

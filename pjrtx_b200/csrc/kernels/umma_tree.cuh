@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
             }
           }
           const float shift = m_used == -INFINITY ? 0.f : Probability<BF16>::kLift - m_used;
-          float part[4] = {0.f, 0.f, 0.f, 0.f};
+          Pair part[2] = {0, 0};
           float s[2][32];  // the next piece is on its way while this one is at work
           tmem_load_32(s_addr, s[0]);
 #pragma unroll 1
@@ -589,7 +589,8 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
               if (c + h * 32 + 32 < kKeys) tmem_load_32(s_addr + c + h * 32 + 32, s[h ^ 1]);
               store_probabilities<BF16>(s[h], a.scale_log2, shift, part, s_addr + (c + h * 32) / 2);
             }
-          sum += (part[0] + part[1]) + (part[2] + part[3]);
+          const float2 block = pair_split(pair_add(part[0], part[1]));
+          sum += block.x + block.y;
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         }

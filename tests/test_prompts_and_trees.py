@@ -2,8 +2,8 @@
 
 Tolerances follow from the arithmetic. A score is a sum of head_dim products in f32, off by at most
 (head_dim + 16) * 2^-24 * sum |q k| * |scale| =: e. A probability is off by the factor e twice (its own score's and those of the sum) and
-by 2^-17 for the exponential; in 16 bits it is rounded to the type (h = half a step), and the sum is taken of the rounded ones, so a
-weight is off by 2h at most. f16 holds probabilities below 2^-25 of the largest to multiples of 2^-35 only, half of which a key may lose. A
+by 2^-17 for the exponential; in 16 bits it is rounded to the type (h = half a step) before it meets the values, but not in the sum, so a
+weight is off by h more (2h are allowed), and the log-sum-exp by none of it. f16 holds probabilities below 2^-25 of the largest to multiples of 2^-35 only, half of which a key may lose. A
 result is rounded once. What a row does not see must not enter at all, whatever it holds.
 """
 import math
@@ -33,7 +33,7 @@ def _expected(dtype, q, k, v, scale):
     out = p @ v
     bound = (2 * e + 2.0 ** -17 + 2 * PROBABILITY[dtype]) * (p @ v.abs()) + LEAST[dtype] * v.abs().sum(0)
     bound = bound + HALF_STEP[dtype] * (out.abs() + bound) + SUBNORMAL[dtype]
-    return out, lse, bound, e + PROBABILITY[dtype] + 2.0 ** -20 * (1 + abs(float(lse)))
+    return out, lse, bound, e + 2.0 ** -17 + 2.0 ** -20 * (1 + abs(float(lse)))
 
 
 class _Compared:
