@@ -27,9 +27,20 @@ namespace {
 constexpr int kSegmentCost = 2;
 constexpr int kJoinWarps = 16;
 
+// What the query rows of a segment are.
+struct Segment {
+  int b, node0, nodes, g, h0, heads;  // nodes and heads of the tile
+  __device__ __forceinline__ bool place(int across, int row, int* node, int* head) const {  // `across`: heads of a full tile
+    *node = node0 + row / across;
+    *head = row % across;
+    return row / across < nodes && *head < heads;
+  }
+};
+
 // A segment that ends in another block than it begins in: written by the block it begins in, first >= last where there is none.
 struct Cut {
-  int b, group, first, last;
+  Segment seg;
+  int first, last;
 };
 
 struct TreeArgs {
@@ -158,16 +169,6 @@ __device__ __forceinline__ Share share_of_block(const TreeArgs& p, ShareSpace<TH
   return s;
 }
 
-// What the query rows of a segment are.
-struct Segment {
-  int b, node0, nodes, g, h0, heads;  // nodes and heads of the tile
-  __device__ __forceinline__ bool place(const TreeArgs& p, int row, int* node, int* head) const {
-    *node = node0 + row / p.heads;
-    *head = row % p.heads;
-    return row / p.heads < nodes && *head < heads;
-  }
-};
-
 __device__ __noinline__ Segment segment_of(const TreeArgs& p, int b, int group, int count) {
   Segment s;
   s.b = b;
@@ -208,10 +209,10 @@ __device__ __forceinline__ long long cached_row(const TreeArgs& p, int b, int t)
 
 // The slot of this block's part of a segment that other blocks share, and the cut that the join goes by; null where none does. Slot 1
 // of a block holds the segment that begins in it, slot 0 the one that began before.
-__device__ __forceinline__ float* part_of(const TreeArgs& p, const Share& share, const Cursor& u, long long segment) {
+__device__ __forceinline__ float* part_of(const TreeArgs& p, const Share& share, const Cursor& u, const Segment& seg, long long segment) {
   const long long first = segment / share.quota, last = (segment + u.s.tiles - 1) / share.quota;
   if (first == last) return nullptr;
-  if (threadIdx.x == 0 && blockIdx.x == first) p.cuts[blockIdx.x] = {u.b, u.group, (int)first, (int)last};
+  if (threadIdx.x == 0 && blockIdx.x == first) p.cuts[blockIdx.x] = {seg, (int)first, (int)last};
   return p.parts + ((long long)blockIdx.x * 2 + (blockIdx.x == first ? 1 : 0)) * p.slot_rows * (p.dims + 2);
 }
 
@@ -239,7 +240,7 @@ __global__ void __launch_bounds__(rows::kThreads) tree_rows_kernel(const __grid_
   __shared__ ShareSpace<kThreads> space;
   __shared__ unsigned long long ancestors[kTreeNodesMax];
   Space& s = *reinterpret_cast<Space*>(smem);
-  if (threadIdx.x == 0) p.cuts[blockIdx.x] = {0, 0, 0, 0};
+  if (threadIdx.x == 0) p.cuts[blockIdx.x] = {};
   const Share share = share_of_block(p, space);
   if (share.first >= share.size) return;
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -279,7 +280,7 @@ __global__ void __launch_bounds__(rows::kThreads) tree_rows_kernel(const __grid_
       constexpr int kOfWarp = Space::kRows / 8;
       int node, head;
       const float* q = nullptr;
-      if (lane < kOfWarp && seg.place(p, warp * kOfWarp + lane, &node, &head)) q = any + query_at(p, seg, node, head);
+      if (lane < kOfWarp && seg.place(p.heads, warp * kOfWarp + lane, &node, &head)) q = any + query_at(p, seg, node, head);
       request_rows<D, Space::kRows>(s.q, q, p.c.head_dim, any);
     }
     request(now.tile, stage);
@@ -291,7 +292,7 @@ __global__ void __launch_bounds__(rows::kThreads) tree_rows_kernel(const __grid_
     for (int i = 0; i < R; i++) {
       int node, head;
       sight[i] = {0, 0ull};
-      if (seg.place(p, ty * R + i, &node, &head)) sight[i] = {here.s.length, ancestors[node]};
+      if (seg.place(p.heads, ty * R + i, &node, &head)) sight[i] = {here.s.length, ancestors[node]};
     }
     const long long segment = share.begin + at - here.tile;  // number of its first unit
     for (bool same = true; same; stage++) {
@@ -302,7 +303,7 @@ __global__ void __launch_bounds__(rows::kThreads) tree_rows_kernel(const __grid_
         if (same) request(now.tile, stage + 1);
       });
     }
-    if (float* part = part_of(p, share, here, segment)) {
+    if (float* part = part_of(p, share, here, seg, segment)) {
 #pragma unroll
       for (int c = 0; c < D / 64; c++)
 #pragma unroll
@@ -320,7 +321,7 @@ __global__ void __launch_bounds__(rows::kThreads) tree_rows_kernel(const __grid_
 #pragma unroll
     for (int i = 0; i < R; i++) {
       int node, head;
-      if (!seg.place(p, ty * R + i, &node, &head)) continue;
+      if (!seg.place(p.heads, ty * R + i, &node, &head)) continue;
       const float inverse = inverse_of(sum.l[i]);
       float* out = static_cast<float*>(p.a.out) + out_at(p, seg, node, head);
 #pragma unroll
@@ -388,9 +389,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const __grid
   if (cut.first >= cut.last) return;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, row0 = blockIdx.y * 32, chunks = kJoinWarps / splits;
   const int first = blockIdx.z * chunks * kJoinDims, mine = warp / splits * kJoinDims, d0 = first + mine;  // dimensions: the block's, the warp's
-  const Segment seg = segment_of(p, cut.b, cut.group, sequence_of(p, cut.b).count);
+  const Segment& seg = cut.seg;
   int node, head;
-  const bool there = seg.place(p, row0 + lane, &node, &head);
+  const bool there = seg.place(p.heads, row0 + lane, &node, &head);
   if (!__any_sync(~0u, there)) return;  // the same rows in every warp
   float m = -INFINITY, total = 0.f, x[kJoinDims], y[kJoinDims];
 #pragma unroll
@@ -431,7 +432,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const __grid
 #pragma unroll 1
   for (int i = threadIdx.x; i < 32 * pieces; i += kJoinWarps * 32) {
     const int r = i / pieces, d = i % pieces * 4;
-    if (first + d < p.c.head_dim && seg.place(p, row0 + r, &node, &head))
+    if (first + d < p.c.head_dim && seg.place(p.heads, row0 + r, &node, &head))
       rows::store4(static_cast<T*>(p.a.out) + out_at(p, seg, node, head) + first + d, *reinterpret_cast<const float4*>(&results[r][d]));
   }
 }

@@ -106,8 +106,8 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kMmaWarp = 4, kCopyWarp = 5;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const PromptAttention& p = a.p.a;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   check_starts(p);
   const PromptTile item = prompt_tile(a.p, prompt_block());
   if (item.tile < 0) return;

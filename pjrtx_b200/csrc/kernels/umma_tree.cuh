@@ -118,9 +118,7 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kFirstLoader = 4 * TILES, kMmaWarp = kFirstLoader + kTreeLoaders;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const TreeArgs& p = a.p;
-  if (threadIdx.x == 0) p.cuts[blockIdx.x] = {0, 0, 0, 0};
   if (threadIdx.x == 0) {
     for (int i = 0; i < kQueries; i++) {
       mbar_init(&bar.q_full[i], kTreeLoaders * 32);
@@ -144,6 +142,9 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bar.tmem)), "r"(kTmemCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  // Tensor memory is asked for before the kernel in front has ended: no block of threads that holds some fits the SM beside this one.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (threadIdx.x == 0) p.cuts[blockIdx.x] = {};
   const Share share = share_of_block(p, bar.share);
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -267,7 +268,7 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
         const int r0 = lw * kEach + i, tile = r0 / kAttnRows;
         int node, head;
         unsigned long long row = 0;
-        if (seg.place(p, r0 + lane, &node, &head))
+        if (seg.place(p.heads, r0 + lane, &node, &head))
           row = (unsigned long long)(static_cast<const unsigned short*>(p.a.q) + query_at(p, seg, node, head));
 #pragma unroll 2
         for (int j = 0; j < 32 / kAcross; j++) {
@@ -516,7 +517,7 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
       const Segment seg = segment_of(p, here.b, here.group, here.s.count);
       const long long segment = share.begin + number - here.tile;  // number of its first unit
       int node, head;
-      const bool there = seg.place(p, row, &node, &head);
+      const bool there = seg.place(p.heads, row, &node, &head);
       const bool active = __any_sync(0xffffffffu, there);
       unsigned long long bits = 0;
       if (active) {
@@ -604,7 +605,7 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
            wait(&bar.odd_ready[segments % kOddRing], (unsigned)(segments / kOddRing) & 1u);
       step++;
       if (!ok) break;
-      float* part = part_of(p, share, here, segment);
+      float* part = part_of(p, share, here, seg, segment);
       if (!active) continue;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const unsigned long long odd = bar.odd[segments % kOddRing] & bits;
