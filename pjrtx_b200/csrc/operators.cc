@@ -183,6 +183,7 @@ int paged_cache_attend_tree(const PagedCache& cache, PagedView view, PagedTree a
       !stride_ok(a.new_node_stride, a.nodes, c.dtype) || !stride_ok(a.new_head_stride, c.kv_heads, c.dtype))
     return refuse("attend to a tree: its keys and values need 16-byte aligned pointers and strides (%lld, %lld, %lld elements)", a.new_batch_stride,
                   a.new_node_stride, a.new_head_stride);
+  if (a.out == a.q || a.out == a.k_new || a.out == a.v_new) return refuse("attend to a tree: the results can not take the place of an input");
   CurrentDevice scope(cache.device->ordinal);
   if (!entered(scope, cache.device)) return 0;
   return launched(paged_tree_launch(view, a, cache.device->sm_count, true, stream), "attend to a tree");
@@ -263,6 +264,7 @@ int prompt_attention(int ordinal, PromptAttention a, int64_t heads, int64_t kv_h
       !stride_ok(a.k_head_stride, kv_heads, a.dtype) || !stride_ok(a.v_stride, a.tokens, a.dtype) || !stride_ok(a.v_head_stride, kv_heads, a.dtype) ||
       !stride_ok(a.out_stride, a.tokens, a.dtype) || !stride_ok(a.out_head_stride, heads, a.dtype))
     return refuse("prompt attention: queries, keys, values and results need 16-byte aligned pointers and strides");
+  if (a.out == a.q || a.out == a.k || a.out == a.v) return refuse("prompt attention: the results can not take the place of an input");
   a.heads = (int)heads;
   a.kv_heads = (int)kv_heads;
   a.head_dim = (int)head_dim;

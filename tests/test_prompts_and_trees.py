@@ -303,6 +303,15 @@ def test_prompt_attention_refuses(backend, change, message):
         backend.prompt_attention(**_prompt_args(**change), stream=0)
 
 
+@pytest.mark.parametrize("taken", ["q", "k", "v"])
+def test_prompt_results_do_not_take_the_place_of_an_input(backend, taken):
+    place = dict(q=2 << 20, k=3 << 20, v=4 << 20, out=5 << 20)
+    place["out"] = place[taken]
+    change = {n: _Array("bfloat16", 9, 2 if n in "kv" else 8, 64, pointer=at) for n, at in place.items()}
+    with pytest.raises(be_mod.BackendError, match="can not take the place of an input"):
+        backend.prompt_attention(**_prompt_args(**change), stream=0)
+
+
 def test_prompt_structs_without_size_are_refused(backend):
     import ctypes
 
@@ -569,6 +578,9 @@ def test_tree_calls_refuse_bad_arguments(gpu_backend):
     refused(tree, "16-byte aligned", base(), k_new=_Array("bfloat16", 2, 5, 4, 64, pointer=(1 << 20) + 2))
     refused(tree, "null parents", base(), parents=_Array("int32", 2, 5, pointer=0))
     refused(tree, "not finite", base(), scale=math.nan)
+    for taken, shape in (("q", (2, 5, 8, 64)), ("k_new", (2, 5, 4, 64)), ("v_new", (2, 5, 4, 64))):
+        refused(tree, "can not take the place of an input", base(), **{taken: _Array("bfloat16", *shape, pointer=2 << 20)},
+                out=_Array("bfloat16", 2, 5, 8, 64, pointer=2 << 20))
     store = dict(k_pages=_Array("bfloat16", 9, 16, 4, 64), v_pages=_Array("bfloat16", 9, 16, 4, 64), k_new=_Array("bfloat16", 7, 4, 64),
                  v_new=_Array("bfloat16", 7, 4, 64), slots=_Array("int32", 7))
     refused(cache.store, "slots has shape", store, slots=_Array("int32", 6))
