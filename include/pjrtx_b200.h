@@ -455,7 +455,7 @@ int pjrtx_b200_dot_static_scratch_status(int device_ordinal, void *stream);
  * weights are f32, ids and lengths s32. Strides count elements; the innermost axis is dense.
  * 1 when enqueued, 0 with last_error set. What only the device sees (a page id or slot outside the pool, a length outside the page
  * table, a token id outside the vocabulary, a node's parent that does not come before it) is never followed out of bounds: the
- * kernel skips it and sets a word of its code (40, 41, 42, 43). pjrtx_b200_operators_status waits for the stream of a call and tells. The words are the device's, not the
+ * kernel skips it and sets a word of its code (40, 41, 42, 43); 44 is a bounded wait of a kernel that gave up, whose results do not hold. pjrtx_b200_operators_status waits for the stream of a call and tells. The words are the device's, not the
  * call's: pjrtx_b200_device_synchronize and copies to the host, which wait for the stream of pjrtx_b200_device_stream alone,
  * return 0 for what is set by then, whichever stream it came from, and what has been named once is not named again. */
 void *pjrtx_b200_device_stream(int device_ordinal);
@@ -575,7 +575,7 @@ int pjrtx_b200_paged_cache_attend_tree(PjrtxB200PagedCache *cache, const PjrtxB2
                                        const PjrtxB200PagedTreeArgs *args, void *stream);
 
 /* Rows of packed keys and values go to slots: a row's slot is its page times page_size plus the row in the page. Negative slots
- * are skipped. Of rows with the same slot, which one is stored is open (in pieces of 16 bytes). Takes no account of tracked weights. */
+ * are skipped, slots from pages * page_size on too, and reported (40). The rows may not lie in the pools. Of rows with the same slot, which one is stored is open (in pieces of 16 bytes). Takes no account of tracked weights. */
 typedef struct PjrtxB200PagedStoreArgs {
   uint64_t struct_size;
   const void *k_new; /* [rows, kv_heads, head_dim] through the strides */
@@ -625,7 +625,7 @@ int pjrtx_b200_paged_cache_assign(PjrtxB200PagedCache *cache, const PjrtxB200Pag
 typedef struct PjrtxB200PagedPathArgs {
   uint64_t struct_size;
   int64_t batch;
-  int64_t nodes;             /* 1..64 */
+  int64_t nodes;             /* up to 64 */
   const int32_t *page_table; /* [batch, max_pages], rows table_stride apart */
   int64_t table_stride;
   const int32_t *lengths;    /* [batch] */

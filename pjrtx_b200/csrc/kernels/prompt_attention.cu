@@ -5,7 +5,11 @@
 // starts[b] / positions + b on (a sequence of n tokens has at most that many before the next one's), and blocks without a tile leave. The
 // tiles of a sequence run from its end, where they have most to do, to its beginning, a tile for all KV heads before the next tile.
 //
-// 16-bit types go to the tensor cores (umma_prompt.cuh), f32 to the CUDA cores (row_attention.cuh).
+//
+//   out_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = e^(scale q_i . k_j - m_i), j <= i of the same sequence,  m_i following max_j scale q_i . k_j
+//
+// Of n tokens that is 2 n (n + 1) heads head_dim operations on 2 n (heads + kv_heads) head_dim elements: bound by arithmetic from some hundred
+// tokens on, by latency below. 16-bit types go to the tensor cores (umma_prompt.cuh), f32 to the CUDA cores (row_attention.cuh).
 #include <algorithm>
 #include <type_traits>
 

@@ -7,7 +7,10 @@
 //
 // 256 threads, 16, 32 or 64 rows and 64 keys (32 of 256 dimensions) at a time: a thread has up to four rows by four keys of the
 // scores, then its rows by a sixteenth of the dimensions of the values, two products an instruction; the running maximum and sum of a row are in
-// the sixteen threads that have it. The next keys and values come by cp.async while these are at work.
+// the sixteen threads that have it. The next keys and values come by cp.async while these are at work. One or two rows a
+// thread are for trees of few rows, which would compute rows that are not there. Bound by FMAs and the reads of shared memory beside them:
+// 16 sequences of up to 2000 rows, 32 heads of 128 over 8, take 173 us with 8 nodes, 154 with one and 634 with 40; prompts of 4 x 2048 tokens
+// of such heads 3.9 ms (35 TFLOP/s), 48 of up to 200, four heads of 64 over two, 37 us.
 // What a row does not see enters nothing: scores are replaced, and where values of a block are infinite or NaN the products with
 // hidden keys are left out one by one.
 #pragma once

@@ -5,7 +5,8 @@
 // query rows is some nodes of a sequence times the query heads of a KV head: row x is head x % heads of node x / heads. So each cached row
 // is read once for all nodes and heads that share it, which is what the operator is for: one node at a time would read it once for each.
 //
-// 16-bit types go to the tensor cores (umma_tree.cuh), f32 to the CUDA cores (row_attention.cuh).
+// Bound by the cached rows' bytes until a row is read for some 250 query rows (16 bits: 4 operations an element and query row). 16-bit types go
+// to the tensor cores (umma_tree.cuh), f32 to the CUDA cores (row_attention.cuh).
 #include <algorithm>
 
 #include "../common.h"
@@ -339,7 +340,7 @@ __global__ void __launch_bounds__(rows::kThreads) tree_rows_kernel(const __grid_
 
 // A block has 32 rows of a cut segment, a lane a row, a warp eight dimensions and every `splits`-th part, in an order that does not depend on
 // which is first. Many segments are cut once or twice and take the parts one after the other; where few blocks have a place, more warps share a row's
-// parts, and blocks go by the cuts that there are (looking for one takes a microsecond). Loops are not unrolled: every launch fetches
+// parts, and blocks go by the cuts that there are (looking for one takes 1 us). Loops are not unrolled: every launch fetches
 // its instructions anew, and 16 dimensions a warp with unrolled loops took 8 us for each part behind the first.
 constexpr int kJoinDims = 8;
 

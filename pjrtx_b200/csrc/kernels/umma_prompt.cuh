@@ -8,6 +8,15 @@
 //                  when the softmax warps are done with one
 //   softmax warps  four, a query row a thread (its lane of tensor memory), so a row's maximum and sum need no exchange
 //
+// What bounds it: a block of 128 rows and 64 keys of 128 elements takes 512 cycles of the tensor core's time and 512 of the exponential unit's
+// (8192 at 16 a cycle), and 128 rows' masks, maxima, sums and conversions take nearly as many issue slots; with two blocks of threads at
+// work these overlap in part. 8192 and 5461 tokens in f16, 32 heads of 128 over 8 KV heads, masked halves left out: 718 us, 1.11 PFLOP/s (of the
+// blocks on the diagonal, whose hidden half is computed too, 1.6 %); bf16 660 to 690. 4 x 2048 143 us, with 8 heads of 64 45 to 50; one prompt of 517 tokens
+// 10.5 us, where launch, first copies, nine blocks of keys one after the other and the way out follow each other.
+//
+// Exponentials all go to the exponential unit: a share of them by polynomials on the FMA units, as the tensor core's rate would want, made
+// every case 2 to 15 % slower, since issue slots are as scarce.
+//
 // Two tiles in a block of threads of twice the size, with blocks of 128 keys that they share and buffers for one block of scores each, were slower up to
 // 4096 tokens: 517 of 32 heads over 8 14.4 us (10.8), 64 x 20 28 (16), 4 x 2048 162 (149), 2 x 4096 258 (254); 2 x 8192 916 (947).
 //

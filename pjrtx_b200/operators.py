@@ -2,10 +2,9 @@
 
 Bindings of the `pjrtx_b200_paged_cache_*`, `pjrtx_b200_prompt_attention` and `pjrtx_b200_token_log_probs*` entry points of
 include/pjrtx_b200.h, reached through `Backend.paged_cache`, `Backend.prompt_attention`, `Backend.token_log_probs` and
-`Backend.token_log_probs_backward`. Arrays are `DeviceBuffer`s
-or any device tensors with `data_ptr()`, `shape`, `stride()` and `dtype` (torch's). Types, shapes and the device that an array
-says it is on (`get_device()` or `device`) are checked here, the rest behind the C ABI; nothing is copied, cast or kept. Calls
-enqueue on `stream`, a `cudaStream_t` as an integer (0: the default stream).
+`Backend.token_log_probs_backward`. Arrays are `DeviceBuffer`s or any device tensors with `data_ptr()`, `shape`, `stride()` and
+`dtype` (torch's). Types, shapes and the device that an array says it is on (`get_device()` or `device`) are checked here, the rest
+behind the C ABI; nothing is copied, cast or kept. Calls enqueue on `stream`, a `cudaStream_t` as an integer (0: the default stream).
 
 `stream=None` is the stream on which the backend's buffers and executables work. It does not wait for the default stream or for a
 tensor library's, nor they for it: tensors need the stream that they are worked on given, or events. Buffers are filled and freed
