@@ -125,9 +125,13 @@ __global__ void __launch_bounds__(rows::kThreads) prompt_rows_kernel(const __gri
     int position, head;
     sight[i] = {place(ty * R + i, &position, &head) ? position + 1 : 0, 0ull};
   }
+  int reach = 0;
+#pragma unroll
+  for (int i = 0; i < R; i++) reach = max(reach, sight[i].limit);
+  reach = __reduce_max_sync(~0u, reach);
   const int blocks = (keys + Space::kKeys - 1) / Space::kKeys;
   for (int j = 0; j < blocks; j++)
-    block_of_keys<D, R>(s, sum, sight, j, j * Space::kKeys, keys, keys, a.scale * kLog2e, [&] {
+    block_of_keys<true, D, R>(s, sum, sight, j, j * Space::kKeys, keys, reach, keys, a.scale * kLog2e, [&] {
       if (j + 1 < blocks) request(j + 1);
     });
 #pragma unroll

@@ -10,13 +10,16 @@
 // the sixteen threads that have it. The next keys and values come by cp.async while these are at work. One or two rows a
 // thread are for trees of few rows, which would compute rows that are not there. Bound by FMAs and the reads of shared memory beside them:
 // 16 sequences of up to 2000 rows, 32 heads of 128 over 8, take 173 us with 8 nodes, 154 with one and 634 with 40; prompts of 4 x 2048 tokens
-// of such heads 3.9 ms (35 TFLOP/s), 48 of up to 200, four heads of 64 over two, 37 us.
+// of such heads 3.9 ms (35 TFLOP/s), 517 tokens 76 us, 48 prompts of up to 200, four heads of 64 over two, 28. A warp leaves out keys that none of
+// its rows sees, half a block of scores or four values at a time (82 and 36 us without).
 // What a row does not see enters nothing: scores are replaced, and where values of a block are infinite or NaN the products with
 // hidden keys are left out one by one.
 #pragma once
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "arith.cuh"
 
@@ -118,11 +121,12 @@ __device__ __forceinline__ void request_rows(float (*to)[PITCH], const float* ro
 }
 
 // Block `stage & 1`: keys key0 .. (those before `keys`), which has been requested, into the sums; requests the next one by `next()`. The
-// queries are in shared memory once the first block is.
-template <int D, int R, typename Next>
-__device__ __forceinline__ void block_of_keys(Shared<D, R>& s, Sums<D, R>& sum, const Sight (&sight)[R], int stage, int key0, int keys, int base,
-                                              float scale2, Next next) {
+// queries are in shared memory once the first block is. No row of the warp sees keys from `reach` on.
+template <bool HALVES, int D, int R, typename Next>
+__device__ __forceinline__ void block_of_keys(Shared<D, R>& s, Sums<D, R>& sum, const Sight (&sight)[R], int stage, int key0, int keys, int reach,
+                                              int base, float scale2, Next next) {
   constexpr int kKeys = keys_of(D), kColumns = kKeys / 16;
+  const int end = min(kKeys, reach - key0);
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   float(*const sk)[D + 4] = s.k[stage & 1];
   float(*const sv)[D] = s.v[stage & 1];
@@ -134,23 +138,29 @@ __device__ __forceinline__ void block_of_keys(Shared<D, R>& s, Sums<D, R>& sum, 
   });
   const bool careful = __syncthreads_or(found);  // all rows have landed, and the other stage has been read
   next();
+  if (end <= 0) return;
   Pair a[R][kColumns];
 #pragma unroll
   for (int i = 0; i < R; i++)
 #pragma unroll
     for (int j = 0; j < kColumns; j++) a[i][j] = 0;
+  auto products = [&](auto columns) {
+    constexpr int kOf = decltype(columns)::value;
 #pragma unroll 4
-  for (int d = 0; d < D; d += 4) {
-    ulonglong2 q[R], k[kColumns];
+    for (int d = 0; d < D; d += 4) {
+      ulonglong2 q[R], k[kOf];
 #pragma unroll
-    for (int i = 0; i < R; i++) q[i] = *reinterpret_cast<const ulonglong2*>(&s.q[ty * R + i][d]);
+      for (int i = 0; i < R; i++) q[i] = *reinterpret_cast<const ulonglong2*>(&s.q[ty * R + i][d]);
 #pragma unroll
-    for (int j = 0; j < kColumns; j++) k[j] = *reinterpret_cast<const ulonglong2*>(&sk[tx + 16 * j][d]);
+      for (int j = 0; j < kOf; j++) k[j] = *reinterpret_cast<const ulonglong2*>(&sk[tx + 16 * j][d]);
 #pragma unroll
-    for (int i = 0; i < R; i++)
+      for (int i = 0; i < R; i++)
 #pragma unroll
-      for (int j = 0; j < kColumns; j++) a[i][j] = pair_fma(q[i].y, k[j].y, pair_fma(q[i].x, k[j].x, a[i][j]));
-  }
+        for (int j = 0; j < kOf; j++) a[i][j] = pair_fma(q[i].y, k[j].y, pair_fma(q[i].x, k[j].x, a[i][j]));
+    }
+  };
+  if (HALVES && end <= kKeys / 2) products(std::integral_constant<int, kColumns / 2>());
+  else products(std::integral_constant<int, kColumns>());
 #pragma unroll
   for (int i = 0; i < R; i++) {
     float x[kColumns], top = -INFINITY;
@@ -185,8 +195,7 @@ __device__ __forceinline__ void block_of_keys(Shared<D, R>& s, Sums<D, R>& sum, 
   }
   __syncwarp();  // a row's probabilities are written and read by the same warp
   if (careful) {
-    for (int t = 0; t < kKeys; t++) {
-      if (key0 + t >= keys) break;
+    for (int t = 0; t < end; t++) {
 #pragma unroll
       for (int i = 0; i < R; i++) {
         if (!sees(sight[i], key0 + t, base)) continue;
@@ -203,7 +212,7 @@ __device__ __forceinline__ void block_of_keys(Shared<D, R>& s, Sums<D, R>& sum, 
     return;
   }
 #pragma unroll 2
-  for (int t = 0; t < kKeys; t += 4) {
+  for (int t = 0; t < end; t += 4) {
     float4 p[R];
 #pragma unroll
     for (int i = 0; i < R; i++) p[i] = *reinterpret_cast<const float4*>(&s.p[ty * R + i][t]);

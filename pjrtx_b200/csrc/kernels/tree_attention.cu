@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(rows::kThreads) tree_rows_kernel(const __grid_
       const int tile = now.tile;
       more = next_unit(p, now, at, share.size);
       same = more && now.group == here.group && now.b == here.b;
-      block_of_keys<D, R>(s, sum, sight, stage, tile * Space::kKeys, keys, here.s.length, p.a.scale * kLog2e, [&] {
+      block_of_keys<false, D, R>(s, sum, sight, stage, tile * Space::kKeys, keys, keys, here.s.length, p.a.scale * kLog2e, [&] {
         if (same) request(now.tile, stage + 1);
       });
     }
