@@ -7,9 +7,11 @@
 // path: a drafted token is accepted when it lies on the way from the leaf to its root; its row is the number of those before it.
 //
 // All of it is a few hundred KB at most (a table of 512 x 256 pages and its copy: 1 MB), so what counts is the number of trips to memory
-// in a row: one launch of one cluster, whose blocks pass sums and pages to each other between cluster barriers. 32 sequences that grow by a
-// row take as long as the call (13 us), 512 that get new prompts of up to 4096 tokens, with the slots of all of these, 28; path slots of 256 trees of
-// 64 nodes as long as the call (10 us), with the ancestors in six rounds of doubling and not by up to 63 steps of a chain.
+// in a row: one launch of one cluster, whose blocks pass sums and pages to each other between cluster barriers, and loops that have several
+// loads under way. 32 sequences that grow by a row take 7.5 us, 512 that get new prompts of up to 4096 tokens, with the slots of all of these
+// (377 000, by a kernel of their own), 20.8 (27.3 with one load after the other, 20.4 with eight at a time, which takes 4096 sequences of 64 pages
+// from 49 to 59; blocks of 1024 threads 10.5, 21.1 and 38). Path slots of 256 trees of 64 nodes take less than a call from Python (10 us), with the
+// ancestors in six rounds of doubling and not by up to 63 steps of a chain.
 #include <cooperative_groups.h>
 
 #include "../common.h"
@@ -64,6 +66,25 @@ __device__ __forceinline__ long long block_prefix(long long x, long long* warp_s
 struct Sums {
   long long give, take, granted;
 };
+
+// For i = first, first + step, .. before last: from(i) for several of them, whose loads are then under way together, before to(i, what it gave).
+template <typename From, typename To>
+__device__ __forceinline__ void in_batches(long long first, long long last, int step, From from, To to) {
+  constexpr int kBatch = 4;
+  for (long long i0 = first; i0 < last; i0 += (long long)kBatch * step) {
+    int x[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; u++) {
+      const long long i = i0 + u * step;
+      x[u] = i < last ? from(i) : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; u++) {
+      const long long i = i0 + u * step;
+      if (i < last) to(i, x[u]);
+    }
+  }
+}
 
 // Slot of a packed token, once tables and page counts are written: the sequence by bisection, the row from its end.
 __device__ __forceinline__ int slot_of(const PagedAssign& a, long long t) {
@@ -139,12 +160,14 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads) page
   for (int b = first + warp; b < last; b += kWarps) {
     const Want w = want_of(a, b, stack_ok);
     const longlong2 at = offsets[b - first];
-    for (int j = lane; j < w.held - w.need; j += 32) {
-      const long long place = free_count + give_before + at.x + j;
-      const int page = a.table[b * a.table_stride + w.need + j];
-      if (page < 0 || page >= a.num_pages) report(a.error_words, kErrorPageId);
-      if (place < a.num_pages) a.free_pages_out[place] = page;
-    }
+    const int* surplus = a.table + b * a.table_stride + w.need;
+    const long long top = free_count + give_before + at.x;
+    in_batches(
+        lane, w.held - w.need, 32, [&](long long j) { return surplus[j]; },
+        [&](long long j, int page) {
+          if (page < 0 || page >= a.num_pages) report(a.error_words, kErrorPageId);
+          if (top + j < a.num_pages) a.free_pages_out[top + j] = page;
+        });
     const int wanted = w.need - w.held;
     if (wanted > 0 && take_before + at.y + wanted <= there) granted += wanted;
   }
@@ -172,24 +195,29 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads) page
     const int* from = a.table + b * a.table_stride;
     int* to = a.table_out + b * a.table_out_stride;
     const int c0 = copy_table ? 0 : min(w.held, held), c1 = copy_table ? a.max_pages : max(w.held, held);
-    for (int c = c0 + lane; c < c1; c += 32) {
-      int page;
-      if (c >= w.held && c < held) {
-        const int place = there - 1 - (int)(take_before + at.y + c - w.held);
-        page = place < free_count ? a.free_pages[place] : __ldcg(a.free_pages_out + place);
-        a.free_pages_out[place] = -1;
-        if (page < 0 || page >= a.num_pages) report(a.error_words, kErrorPageId);
-      } else {
-        page = c >= held && c < w.held ? -1 : from[c];
-      }
-      to[c] = page;
-    }
+    const long long top = there - 1 - (take_before + at.y) + w.held;  // where column 0 would come from
+    in_batches(
+        c0 + lane, c1, 32,
+        [&](long long c) {
+          if (c >= w.held && c < held) return __ldcg((top - c < free_count ? a.free_pages : a.free_pages_out) + (top - c));
+          return c >= held && c < w.held ? -1 : from[c];
+        },
+        [&](long long c, int page) {
+          if (c >= w.held && c < held) {
+            a.free_pages_out[top - c] = -1;
+            if (page < 0 || page >= a.num_pages) report(a.error_words, kErrorPageId);
+          }
+          to[c] = page;
+        });
     __syncwarp();  // in place: all lanes have read what the sequence had
     if (lane == 0) a.held_out[b] = w.ok ? held : a.held[b];
   }
   if (copy_stack)
-    for (int i = rank * kThreads + threadIdx.x; i < a.num_pages; i += kBlocks * kThreads)
-      if (i < min(count, free_count) || i >= there) a.free_pages_out[i] = a.free_pages[i];
+    in_batches(
+        rank * kThreads + threadIdx.x, a.num_pages, kBlocks * kThreads, [&](long long i) { return a.free_pages[i]; },
+        [&](long long i, int page) {
+          if (i < min(count, free_count) || i >= there) a.free_pages_out[i] = page;
+        });
   if (!slots) return;
   cluster.sync();
   for (long long t = rank * kThreads + threadIdx.x; t < a.tokens; t += kBlocks * kThreads) a.slots[t] = slot_of(a, t);
