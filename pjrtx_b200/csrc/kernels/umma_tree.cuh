@@ -19,7 +19,7 @@
 // with the tensor core.
 //
 // Hidden nodes have probability 0, and 0 times infinity or NaN is NaN on the tensor core. So a node with such a value is cleared in shared
-// memory (one more warp, the checker, looks at the nodes' values where they have landed), and rows that see it add their probability times its values when they take their results out. Rounding and the lazily
+// memory (one more warp, the cleaner, looks at the nodes' values where they have landed), and rows that see it add their probability times its values when they take their results out. Rounding and the lazily
 // followed maximum: umma_rows.cuh.
 #pragma once
 
@@ -29,7 +29,7 @@ namespace pjrtx {
 namespace umma {
 
 constexpr int kTreeLoaders = 4;
-constexpr int kOddRing = 16, kCleanRing = 16;  // longer than a checker can be ahead, which has the slots
+constexpr int kOddRing = 16, kCleanRing = 16;  // longer than a cleaner can be ahead, which has the slots
 __host__ __device__ constexpr int tree_keys(int hd) { return hd == 256 ? 64 : 128; }
 __host__ __device__ constexpr int tree_slot_bytes(int hd) { return tree_keys(hd) * hd * 2; }
 __host__ __device__ constexpr int tree_query_buffers(int hd, int tiles) { return tiles == 1 && hd <= 128 ? 2 : 1; }
@@ -45,7 +45,7 @@ __host__ __device__ constexpr size_t tree_smem(int hd, int tiles) {
   const size_t least = least_smem(512);
   return bytes < least ? least : bytes;
 }
-// Four softmax warps a tile, the loaders, the warp that issues, the checker.
+// Four softmax warps a tile, the loaders, the warp that issues, the cleaner.
 __host__ __device__ constexpr int tree_threads(int tiles) { return 128 * tiles + 32 * (kTreeLoaders + 2); }
 
 struct TreeKernelArgs {
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
     }
     for (int i = 0; i < kSlots; i++) {
       mbar_init(&bar.slot_full[i], kTreeLoaders * 32);
-      mbar_init(&bar.slot_empty[i], 2);  // the products, and the checker: it sees every use of a slot, or could take one for another
+      mbar_init(&bar.slot_empty[i], 2);  // the products, and the cleaner: it sees every use of a slot, or could take one for another
     }
     for (int t = 0; t < TILES; t++)
       for (int i = 0; i < kBuffers; i++) {
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
       __syncwarp();
     }
   } else if (warp == kMmaWarp + 1) {
-    // The checker: looks at the values of nodes where they have landed.
+    // The cleaner: looks at the values of nodes where they have landed.
     Cursor now = share.at;
     long long number = share.first, used = 0, checked = 0, segments = 0;
     unsigned long long odd = 0;
