@@ -908,3 +908,173 @@ def test_two_trees_on_two_streams(gpu_backend):
     torch.cuda.synchronize()
     for t, _ in pairs:
         t.check(some=150)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_more_prompts_than_an_axis_of_the_grid_has_blocks(gpu_backend, dtype):
+    """A sequence of one token has its own value as the result, whose weight is one."""
+    import torch
+
+    sequences = 140000
+    lengths = np.ones(sequences, np.int64)
+    lengths[::7] = 0
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    tokens = int(lengths.sum())
+    x = torch.randn((tokens + 4, 4, 8), generator=gen, device="cuda").to(_torch_type(dtype))
+    q, k, v = x[:, :2], x[:, 2:3], x[:, 3:]
+    starts = torch.tensor(np.concatenate([[0], np.cumsum(lengths)]), dtype=torch.int32, device="cuda")
+    out, lse = torch.full((tokens + 4, 2, 8), 7.0, dtype=x.dtype, device="cuda"), torch.full((tokens + 4, 2), 7.0, device="cuda")
+    gpu_backend.prompt_attention(q, k, v, starts, out, lse=lse, scale=0.3, stream=_stream())
+    gpu_backend.operators_status(stream=_stream())
+    want = v[:tokens].double().expand(tokens, 2, 8)
+    bound = (2.0 ** -17 + 2 * PROBABILITY[dtype]) * want.abs() + LEAST[dtype] * want.abs()
+    _within(out[:tokens], want, bound + HALF_STEP[dtype] * (want.abs() + bound) + SUBNORMAL[dtype], "values")
+    products = q[:tokens].double() * k[:tokens].double() * 0.3
+    score = products.sum(-1)
+    _within(lse[:tokens], score, products.abs().sum(-1) * 24 * 2.0 ** -24 + 2.0 ** -17 + 2.0 ** -20 * (1 + score.abs()), "lse")
+    assert (out[tokens:] == 7).all() and (lse[tokens:] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_trees_of_a_large_batch(gpu_backend, dtype):
+    lengths = np.random.default_rng(2).integers(0, 40, 3000).tolist()
+    t = _Trees(dtype, 4, 2, 64, 8, lengths, 2, seed=2)
+    t.run(gpu_backend)
+    t.check(some=2500)
+    gpu_backend.operators_status(stream=_stream())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("page", [16, 6])
+def test_trees_on_shared_pages(gpu_backend, dtype, page):
+    """Sequences may have pages in common: a prompt's, say."""
+    t = _Trees(dtype, 8, 2, 128, page, [400, 400, 333], 5, seed=6)
+    c = t.case
+    shared = 300 // page
+    c.table[1, :shared], c.table[2, :shared] = c.table[0, :shared].clone(), c.table[0, :shared].clone()
+    t.run(gpu_backend)
+    t.check(some=400)
+
+
+@pytest.mark.gpu
+def test_two_graphs_of_trees_on_one_handle(gpu_backend):
+    """Their calls share the handle's workspace and follow each other on a stream."""
+    import torch
+
+    t = _Trees("bf16", 16, 4, 128, 16, [3000, 17], 9, seed=3, counts=[9, 9])
+    t.run(gpu_backend)
+    torch.cuda.synchronize()
+    want = t.out.clone()
+    others, side = torch.empty_like(t.out), torch.cuda.Stream()
+    q = t.q * 0.5
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for graph, change in zip(graphs, ({}, {"q": q, "out": others})):
+        with torch.cuda.graph(graph, stream=side):
+            c = t.case
+            args = {"q": t.q, "out": t.out, **change}
+            t.cache.attend_tree(args["q"], c.k, c.v, c.table, c.lengths, args["out"], t.k, t.v, t.parents, counts=t.counts, stream=_stream())
+    t.out.fill_(7), others.fill_(7)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(5):
+            for graph in graphs:
+                graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(t.out, want)
+    eager, c = torch.empty_like(want), t.case
+    t.cache.attend_tree(q, c.k, c.v, c.table, c.lengths, eager, t.k, t.v, t.parents, counts=t.counts, stream=_stream())
+    assert torch.equal(eager, others)
+
+
+@pytest.mark.gpu
+def test_pages_slots_and_rows_in_a_graph(gpu_backend):
+    """One captured step that is replayed: the lengths grow, pages come as they are needed, and rows go where the slots say. The table is
+    changed in place, the stack is not: its copy is what the next step reads."""
+    import torch
+
+    batch, page, max_pages, pool, kv_heads, dim = 5, 4, 6, 40, 2, 16
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    cache = gpu_backend.paged_cache(P.F32, batch, 2, kv_heads, dim, page, max_pages)
+    k_pages, v_pages = (torch.zeros((pool, page, kv_heads, dim), device="cuda") for _ in "kv")
+    lengths, held, table = ints([0] * batch), ints([0] * batch), ints([[-1] * max_pages] * batch)
+    free, count, free_out, count_out = ints(list(range(pool))), ints([pool]), ints([7] * pool), ints([7])
+    parents, leaves, path, after = ints([[-1, 0, 1]] * batch), ints([2, 0, 1, -1, 2]), torch.zeros((batch, 3), dtype=torch.int32, device="cuda"), ints([0] * batch)
+    room = ints([0] * batch)
+    k_new, v_new = torch.zeros((batch, 3, kv_heads, dim), device="cuda"), torch.zeros((batch, 3, kv_heads, dim), device="cuda")
+
+    def step():
+        torch.add(lengths, 3, out=room)
+        cache.assign_pages(room, held, table, free, count, free_pages_out=free_out, free_count_out=count_out, stream=_stream())
+        free.copy_(free_out), count.copy_(count_out)
+        cache.path_slots(table, lengths, parents, leaves, path, lengths_out=after, stream=_stream())
+        cache.store(k_pages, v_pages, k_new.flatten(0, 1), v_new.flatten(0, 1), path.flatten(), stream=_stream())
+        lengths.copy_(after)
+
+    step()  # before the capture
+    for x, to in ((lengths, 0), (held, 0), (table, -1), (count, pool)):
+        x.fill_(to)
+    free.copy_(ints(list(range(pool))))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    steps, rows = 5, [[] for _ in range(batch)]
+    for i in range(steps):
+        k_new.copy_(torch.randn(k_new.shape, device="cuda")), v_new.copy_(k_new + 1)
+        graph.replay()
+        for b, n in enumerate([3, 1, 2, 0, 3]):
+            rows[b] += list(k_new[b, :n].clone())
+    gpu_backend.operators_status(stream=_stream())
+    assert lengths.tolist() == [15, 5, 10, 0, 15]
+    assert held.tolist() == [-(-(n * (steps - 1) + 3) // page) for n in [3, 1, 2, 0, 3]]
+    used = table[table >= 0].tolist()
+    assert len(set(used)) == len(used) == sum(held.tolist()) and int(count) == pool - len(used)
+    assert sorted(used + free[:int(count)].tolist()) == list(range(pool))
+    for b in range(batch):
+        for t, row in enumerate(rows[b]):
+            at = int(table[b, t // page]), t % page
+            assert torch.equal(k_pages[at], row) and torch.equal(v_pages[at], row + 1)
+
+
+@pytest.mark.gpu
+def test_prompts_trees_and_rows_of_the_backends_own_buffers(gpu_backend):
+    """DeviceBuffers on the backend's stream, with no waits between the calls."""
+    be, rng = gpu_backend, np.random.default_rng(4)
+    f32 = lambda *s: rng.standard_normal(s).astype(np.float32)
+    put = lambda x: be.buffer_from_host(np.ascontiguousarray(x))
+    cache = be.paged_cache(P.F32, 1, 2, 1, 16, 4, 3, tree=3)
+    q, k, v = f32(6, 2, 16), f32(6, 1, 16), f32(6, 1, 16)
+    table, held, lengths = put(np.full((1, 3), -1, np.int32)), put(np.zeros(1, np.int32)), put(np.array([6], np.int32))
+    starts, slots = put(np.array([0, 6], np.int32)), be.allocate_buffer(P.S32, [6])
+    free, count = put(np.arange(4, dtype=np.int32)), put(np.array([4], np.int32))
+    k_pages, v_pages = put(np.zeros((4, 4, 1, 16), np.float32)), put(np.zeros((4, 4, 1, 16), np.float32))
+    out, tree_out = be.allocate_buffer(P.F32, [6, 2, 16]), be.allocate_buffer(P.F32, [1, 3, 2, 16])
+    buffers = [put(x) for x in (q, k, v)]
+    cache.assign_pages(lengths, held, table, free, count, starts=starts, slots=slots)
+    be.prompt_attention(*buffers, starts, out)
+    cache.store(k_pages, v_pages, buffers[1], buffers[2], slots)
+    tree = [f32(1, 3, 2, 16), f32(1, 3, 1, 16), f32(1, 3, 1, 16)]
+    parents, leaves, path = put(np.array([[-1, 0, 0]], np.int32)), put(np.array([2], np.int32)), be.allocate_buffer(P.S32, [1, 3])
+    tree_buffers = [put(x) for x in tree]
+    cache.attend_tree(tree_buffers[0], k_pages, v_pages, table, lengths, tree_out, tree_buffers[1], tree_buffers[2], parents)
+    cache.path_slots(table, lengths, parents, leaves, path)
+    be.operators_status()
+
+    def expected(q, k, v):
+        s = k.astype(np.float64) @ q.astype(np.float64) / 4
+        p = np.exp(s - s.max())
+        return p @ v.astype(np.float64) / p.sum()
+
+    # scores off by 32 * 2^-24 * sum |q k| / 4 < 4e-5 twice, 2^-17 for the exponentials, values below 5
+    for i in range(6):
+        for h in range(2):
+            assert np.abs(out.to_numpy()[i, h] - expected(q[i, h], k[:i + 1, 0], v[:i + 1, 0])).max() < 5e-4
+    for i, way in enumerate(([0], [0, 1], [0, 2])):
+        for h in range(2):
+            want = expected(tree[0][0, i, h], np.concatenate([k[:, 0], tree[1][0, way, 0]]), np.concatenate([v[:, 0], tree[2][0, way, 0]]))
+            assert np.abs(tree_out.to_numpy()[0, i, h] - want).max() < 5e-4
+    assert table.to_numpy().tolist() == [[3, 2, -1]] and slots.to_numpy().tolist() == [12, 13, 14, 15, 8, 9]
+    assert path.to_numpy().tolist() == [[10, -1, 11]] and lengths.to_numpy().tolist() == [8]
