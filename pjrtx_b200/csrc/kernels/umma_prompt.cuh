@@ -122,7 +122,7 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
   check_starts(p);
   const PromptTile item = prompt_tile(a.p, prompt_block());
   if (item.tile < 0) return;
-  const WaitBudget budget{global_timer_ns() + a.timeout_ns, flags};
+  const auto budget = budget_from_now(a.timeout_ns, flags);
   const int g = blockIdx.x / a.p.groups, h0 = blockIdx.x % a.p.groups * a.p.heads, heads = min(a.p.heads, a.p.rep - h0);
   const int first = item.tile * a.p.positions, keys = min(first + a.p.positions, item.tokens);  // the first position, and behind the last
   const int blocks = (keys + kKeys - 1) / kKeys;

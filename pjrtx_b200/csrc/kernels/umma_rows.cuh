@@ -37,6 +37,11 @@ __device__ __forceinline__ float max_of(const float* s, float (&mx)[4]) {
   return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
 }
 
+// Waits end that long after now; launches say how long.
+__device__ __forceinline__ WaitBudget budget_from_now(unsigned long long timeout_ns, volatile int* abort) {
+  return WaitBudget{global_timer_ns() + timeout_ns, abort};
+}
+
 __device__ __forceinline__ void tmem_store_16(uint32_t addr, const float* v) {
   const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
   asm volatile(

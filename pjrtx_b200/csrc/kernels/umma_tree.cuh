@@ -158,8 +158,8 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
   const bool work = share.first < share.size;
   auto s_col = [&](int t, int buffer) { return tmem_base + (uint32_t)((t * kBuffers + buffer) * kKeys); };
   auto o_col = [&](int t) { return tmem_base + (uint32_t)(TILES * kBuffers * kKeys + t * HD); };
-  WaitBudget budget{global_timer_ns() + a.timeout_ns, &bar.abort};  // renewed with every segment
-  auto renew = [&]() { budget.deadline = global_timer_ns() + a.timeout_ns; };
+  auto budget = budget_from_now(a.timeout_ns, &bar.abort);  // renewed with every segment
+  auto renew = [&]() { budget = budget_from_now(a.timeout_ns, &bar.abort); };
   auto wait = [&](uint64_t* b, unsigned parity) { return warp_wait(b, parity, budget.deadline, budget.abort); };
   auto has_nodes = [&](const Cursor& u) { return (u.tile + 1) * kKeys > u.s.length; };
 
