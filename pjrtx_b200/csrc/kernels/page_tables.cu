@@ -10,7 +10,7 @@
 // in a row: one launch of one cluster, whose blocks pass sums and pages to each other between cluster barriers, and loops that have several
 // loads under way. 32 sequences that grow by a row take 7.5 us, 512 that get new prompts of up to 4096 tokens, with the slots of all of these
 // (377 000, by a kernel of their own), 20.8 (27.3 with one load after the other, 20.4 with eight at a time, which takes 4096 sequences of 64 pages
-// from 49 to 59; blocks of 1024 threads 10.5, 21.1 and 38). Path slots of 256 trees of 64 nodes take less than a call from Python (10 us), with the
+// from 49 to 59; blocks of 1024 threads 10.5, 21.1 and 38). Path slots of 256 trees of 64 nodes take 2.3 us, with the
 // ancestors in six rounds of doubling and not by up to 63 steps of a chain.
 #include <cooperative_groups.h>
 

@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(PagedView 
 // ---- store ---------------------------------------------------------------------------------------------------------
 
 // The same for packed rows with a slot each: a thread a 16-byte piece of a key and of its value. Bound by memory or the call: 4 prompts of up to
-// 2048 rows, 8 heads of 128 in bf16, 50 MB in and out, in 11.1 us.
+// 2048 rows, 8 heads of 128 in bf16, 50 MB in and out, in 6.6 us out of L2 and 11 as a call from Python.
 __global__ void __launch_bounds__(kAppendThreads) paged_store_kernel(PagedView c, PagedStore a, int pieces, int esize) {
   PJRTX_PDL_PROLOGUE();
   const int per_row = c.kv_heads * pieces;

@@ -12,8 +12,8 @@
 // (8192 at 16 a cycle), and moves 96 KB through shared memory, 768 cycles at 128 bytes a cycle: the scores' product reads the queries (32 KB) and
 // the block's keys, the other one the values, and the copies write both. Measured are 1050 cycles, tensor core and exponential unit 48 % busy. Eight softmax
 // warps a tile, four for every other block, which hand the rows' maxima to each other, hide more latency and gain nothing (4 x 2048 146 -> 155 us), so it
-// is not the softmax. 8192 and 5461 tokens in f16, 32 heads of 128 over 8 KV heads, masked halves left out: 718 us, 1.11 PFLOP/s (of the
-// blocks on the diagonal, whose hidden half is computed too, 1.6 %); bf16 660 to 690. 4 x 2048 143 us, with 8 heads of 64 45 to 50; one prompt of 517 tokens
+// is not the softmax. 8192 and 5461 tokens in f16, 32 heads of 128 over 8 KV heads, masked halves left out: 718 to 735 us, 1.1 PFLOP/s (of the
+// blocks on the diagonal, whose hidden half is computed too, 1.6 %); bf16 660 to 690. 4 x 2048 143 us, with 8 heads of 64 42; one prompt of 517 tokens
 // 10.5 us, where launch, first copies, nine blocks of keys one after the other and the way out follow each other.
 //
 // Exponentials all go to the exponential unit: a share of them by polynomials on the FMA units, as the tensor core's rate would want, made

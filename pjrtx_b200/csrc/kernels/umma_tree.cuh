@@ -13,9 +13,9 @@
 //
 // Bound by memory up to two tiles: 128 keys of 128 elements are 64 KB of keys and values, 2650 cycles as measured in the middle of a long share (7 TB/s
 // over all SMs), and take 1024 cycles of tensor core and of exponentials for each tile. Around that stand 6 to 7 us of launch, shares, page ids and first rows,
-// and 5 to 10 of the join: 16 sequences of up to 4096 rows, 16 nodes of 32 heads over 8, pages of 16 rows 54.4 us (182 MB, 3.3 TB/s; 46.9 without the
-// join), one sequence of 65536 rows and 32 nodes 64, 517 rows and 8 nodes 14.0. 65536 rows and 64 nodes of 64 heads over 8, four tiles a KV
-// head that read every row twice, 165 us: 137 GFLOP at 0.83 PFLOP/s, bound by two tiles' exponentials and their instructions taking turns
+// and 5 to 10 of the join: 16 sequences of up to 4096 rows, 16 nodes of 32 heads over 8, pages of 16 rows 54 to 56 us (182 MB, 3.3 TB/s; 46.9 without the
+// join), one sequence of 65536 rows and 32 nodes 64 to 67, 517 rows and 8 nodes 13.3. 65536 rows and 64 nodes of 64 heads over 8, four tiles a KV
+// head that read every row twice, 161 to 165 us: 137 GFLOP at 0.85 PFLOP/s, bound by two tiles' exponentials and their instructions taking turns
 // with the tensor core.
 //
 // Hidden nodes have probability 0, and 0 times infinity or NaN is NaN on the tensor core. So a node with such a value is cleared in shared
