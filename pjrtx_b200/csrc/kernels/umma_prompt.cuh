@@ -362,7 +362,8 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
       if (p.lse && pos >= 0)
         p.lse[(long long)(item.start + pos) * p.heads + h] =
             sum == 0.f ? -INFINITY : fmaf(m_used - Probability<BF16>::kLift, rows::kLn2, logf(sum));
-      // Rows that a hidden value may have spoilt.
+      // Rows that a hidden value may have spoilt. All lanes write them once more: behind what each has stored of its own.
+      __syncwarp();
       const unsigned short* k = static_cast<const unsigned short*>(p.k) + (long long)item.start * p.k_stride + (long long)g * p.k_head_stride;
       const unsigned short* v = static_cast<const unsigned short*>(p.v) + (long long)item.start * p.v_stride + (long long)g * p.v_head_stride;
       for (unsigned left = __ballot_sync(0xffffffffu, odd && pos >= 0); left; left &= left - 1) {
