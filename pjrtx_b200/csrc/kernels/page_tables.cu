@@ -14,6 +14,8 @@
 // ancestors in six rounds of doubling and not by up to 63 steps of a chain.
 #include <cooperative_groups.h>
 
+#include <utility>
+
 #include "../common.h"
 #include "kernels.h"
 #include "paged.cuh"
@@ -125,6 +127,7 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads) page
   const bool stack_ok = had >= 0 && had <= a.num_pages;
   const int free_count = stack_ok ? had : 0;
   if (!stack_ok && rank == 0 && threadIdx.x == 0) report(a.error_words, kErrorLength);
+  auto started = cluster.barrier_arrive();  // the other blocks' shared memory is written once they are known to run
 
   // How many pages the sequences before have to give and want.
   long long give = 0, take = 0;
@@ -140,6 +143,7 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads) page
     give += given;
     take += taken;
   }
+  cluster.barrier_wait(std::move(started));
   if (threadIdx.x < kBlocks) *cluster.map_shared_rank(&sums[rank], threadIdx.x) = Sums{give, take, 0};
   cluster.sync();
   long long give_before = 0, take_before = 0, returned = 0;
