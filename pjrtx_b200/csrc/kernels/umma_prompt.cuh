@@ -22,10 +22,13 @@
 // Two tiles in a block of threads of twice the size, with blocks of 128 keys that they share and buffers for one block of scores each, were slower up to
 // 4096 tokens: 517 of 32 heads over 8 14.4 us (10.8), 64 x 20 28 (16), 4 x 2048 162 (149), 2 x 4096 258 (254); 2 x 8192 916 (947).
 //
-// Hidden keys have probability 0, but the tensor core multiplies it by their values, and 0 times infinity or NaN is NaN. So values
-// behind the last position of the block of threads are cleared in shared memory, and a row with a result that is not finite looks at
-// the values between its position and there; only where one is infinite or NaN it is computed once more, by its warp and without them.
+// Hidden keys have probability 0, but the tensor core multiplies it by their values, and 0 times infinity or NaN is NaN; so it does where a
+// probability is lost in 16 bits. So values behind the last position of the block of threads are cleared in shared memory, and a warp with results that
+// are not finite looks at the values once: rows from which one that is not finite is hidden, and rows that see an infinite one, are computed
+// once more, by the warp, without the hidden ones and with probabilities in f32.
 #pragma once
+
+#include <climits>
 
 #include "umma_rows.cuh"
 
@@ -362,19 +365,28 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
       if (p.lse && pos >= 0)
         p.lse[(long long)(item.start + pos) * p.heads + h] =
             sum == 0.f ? -INFINITY : fmaf(m_used - Probability<BF16>::kLift, rows::kLn2, logf(sum));
-      // Rows that a hidden value may have spoilt. All lanes write them once more: behind what each has stored of its own.
+      // Rows that a value may have spoilt (not where the sum is NaN, as every result then is). All lanes write them once more: behind what each has
+      // stored of its own.
       __syncwarp();
+      unsigned left = __ballot_sync(0xffffffffu, odd && pos >= 0 && sum == sum);
       const unsigned short* k = static_cast<const unsigned short*>(p.k) + (long long)item.start * p.k_stride + (long long)g * p.k_head_stride;
       const unsigned short* v = static_cast<const unsigned short*>(p.v) + (long long)item.start * p.v_stride + (long long)g * p.v_head_stride;
-      for (unsigned left = __ballot_sync(0xffffffffu, odd && pos >= 0); left; left &= left - 1) {
-        const int r = __ffs(left) - 1, row_pos = __shfl_sync(0xffffffffu, pos, r), row_h = __shfl_sync(0xffffffffu, h, r);
-        bool spoilt = false;
-        const int pieces = p.head_dim / 8;
-        for (long long i = (long long)(row_pos + 1) * pieces + lane; i < (long long)keys * pieces; i += 32) {
-          const uint4 x = *reinterpret_cast<const uint4*>(v + i / pieces * p.v_stride + i % pieces * 8);
-          spoilt = spoilt || odd_pair<BF16>(x.x) || odd_pair<BF16>(x.y) || odd_pair<BF16>(x.z) || odd_pair<BF16>(x.w);
+      int last_odd = -1, first_infinite = INT_MAX;
+      if (left) {
+        constexpr int kPieces = HD / 8;
+        const int piece = lane % kPieces * 8;
+        for (int key = lane / kPieces; key < keys && piece < p.head_dim; key += 32 / kPieces) {
+          const uint4 x = *reinterpret_cast<const uint4*>(v + key * p.v_stride + piece);
+          if (!(odd_pair<BF16>(x.x) || odd_pair<BF16>(x.y) || odd_pair<BF16>(x.z) || odd_pair<BF16>(x.w))) continue;
+          last_odd = key;
+          if (infinite_pair<BF16>(x.x) || infinite_pair<BF16>(x.y) || infinite_pair<BF16>(x.z) || infinite_pair<BF16>(x.w)) first_infinite = min(first_infinite, key);
         }
-        if (!__any_sync(0xffffffffu, spoilt)) continue;
+        last_odd = __reduce_max_sync(0xffffffffu, last_odd);
+        first_infinite = __reduce_min_sync(0xffffffffu, first_infinite);
+      }
+      for (; left; left &= left - 1) {
+        const int r = __ffs(left) - 1, row_pos = __shfl_sync(0xffffffffu, pos, r), row_h = __shfl_sync(0xffffffffu, h, r);
+        if (last_odd <= row_pos && first_infinite > row_pos) continue;
         const long long token = item.start + row_pos;
         redo_row<BF16, HD>(a, static_cast<const unsigned short*>(p.q) + token * p.q_stride + row_h * p.q_head_stride, k, v,
                            static_cast<unsigned short*>(p.out) + token * p.out_stride + row_h * p.out_head_stride, row_pos,

@@ -74,6 +74,13 @@ __device__ __forceinline__ bool odd_pair(uint32_t w) {
   return (w & kExponent) == kExponent || (w >> 16 & kExponent) == kExponent;
 }
 
+// Whether one of them is infinite.
+template <bool BF16>
+__device__ __forceinline__ bool infinite_pair(uint32_t w) {
+  constexpr uint32_t kInfinity = BF16 ? 0x7f80u : 0x7c00u;
+  return (w & 0x7fffu) == kInfinity || (w >> 16 & 0x7fffu) == kInfinity;
+}
+
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 

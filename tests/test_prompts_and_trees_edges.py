@@ -8,7 +8,7 @@ import pytest
 
 from pjrtx_b200 import plan as P
 from tests import test_prompts_and_trees as base
-from tests.test_operators import _stream
+from tests.test_operators import _stream, _within
 
 
 @pytest.mark.gpu
@@ -31,6 +31,100 @@ def test_every_row_of_a_warp_is_computed_once_more(gpu_backend, dtype, heads, kv
                 c.add(dtype, p.out[a + i, h], p.lse[a + i, h], p.q[a + i, h], p.k[a:a + i + 1, h // rep], p.v[a:a + i + 1, h // rep], head_dim ** -0.5)
         assert (p.out[a + n - 1] == math.inf).all()
     c.check("rows before the last")
+
+
+ODD = [(17, 0.5), (3, -5.0), (100, -17.0), (200, -30.0), (299, -60.0), (150, -80.0)]  # key and score; values of dimensions 2 j and 2 j + 1 are infinite
+
+
+def _place_odd_values(k, v, gen):
+    """Keys [300, heads, d] whose first elements are the scores, and their values."""
+    k[:, :, 1:] = 0
+    k[:, :, 0] = -(gen.initial_seed() % 7 + 53) * (0.1 + 0.9 * k[:, :, 0].float().abs().clamp(max=1)).to(k.dtype)
+    k[40, :, 0] = -math.inf  # probability 0 with finite values: nothing
+    for j, (t, score) in enumerate(ODD):
+        k[t, :, 0] = score
+        v[t, :, 2 * j] = math.inf
+        v[t, :, 2 * j + 1] = -math.inf
+    v[20, :, 0] = -math.inf  # both: NaN
+    v[8, :, 1] = math.nan
+
+
+def _check_odd(dtype, out, k, v, seen):
+    """Rows of one head: out [rows, d] over scores k [keys] and values v [keys, d], row i over the keys of seen [rows, keys]; q is 1 and 0 elsewhere."""
+    import torch
+
+    k, v = k.double(), v.double()
+    s = torch.where(seen, k, -math.inf)
+    p = torch.softmax(s, 1)
+    e = float(k[k.isfinite()].abs().max()) * (v.shape[1] + 16) * 2.0 ** -24
+    plain = torch.where(v.isfinite(), v, 0)
+    sees = lambda what: (p > 0).double() @ what.double() > 0
+    plus, minus, nan = sees(v == math.inf), sees(v == -math.inf), sees(v.isnan())
+    odd, got = plus | minus | nan, out.double()
+    want = torch.where(nan | plus & minus, math.nan, torch.where(plus, math.inf, -math.inf))[odd]
+    assert ((got[odd] == want) | (got[odd].isnan() & want.isnan())).all(), (int((got[odd] != want).sum()), got[odd][:8], want[:8])
+    want = p @ plain
+    bound = (2 * e + 2.0 ** -17 + 2 * base.PROBABILITY[dtype]) * (p @ plain.abs()) + base.LEAST[dtype] * plain.abs().sum(0)
+    bound = bound + base.HALF_STEP[dtype] * (want.abs() + bound) + base.SUBNORMAL[dtype]
+    _within(got[~odd], want[~odd], bound[~odd], "beside the infinities")
+    return int(odd.sum())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("heads,kv_heads,head_dim", [(8, 2, 128), (4, 2, 64), (2, 1, 256), (9, 3, 40)])
+def test_prompts_keep_infinite_values_at_any_probability(gpu_backend, dtype, heads, kv_heads, head_dim):
+    """A value that a row sees makes its dimension infinite however small its (f32) probability is, and nothing else."""
+    import torch
+
+    p = base._Prompts(dtype, heads, kv_heads, head_dim, [65, 300, 9], seed=head_dim)
+    p.q[:, :, 0], p.q[:, :, 1:] = 1, 0
+    a = p.ends[1]
+    _place_odd_values(p.k[a:a + 300], p.v[a:a + 300], p.gen)
+    p.run(gpu_backend, scale=1.0)
+    seen = torch.ones((300, 300), dtype=torch.bool, device="cuda").tril()
+    for h in range(heads):
+        g = h // (heads // kv_heads)
+        assert _check_odd(dtype, p.out[a:a + 300, h], p.k[a:a + 300, g, 0], p.v[a:a + 300, g], seen) > 1000
+    p.check(1.0, some=300, skip=(1,))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("heads,kv_heads,head_dim", [(8, 2, 128), (4, 2, 64), (2, 1, 256), (9, 3, 40)])
+@pytest.mark.parametrize("nodes", [9, 64])
+@pytest.mark.parametrize("page", [16, 6])
+def test_trees_keep_infinite_values_at_any_probability(gpu_backend, dtype, heads, kv_heads, head_dim, nodes, page):
+    """The same for cached rows, in parts and whole, and for nodes."""
+    import torch
+
+    t = base._Trees(dtype, heads, kv_heads, head_dim, page, [300, 4000, 0, 70], nodes, seed=head_dim, counts=[nodes, nodes - 1, nodes, nodes])
+    c = t.case
+    t.q[:, :, :, 0], t.q[:, :, :, 1:] = 1, 0
+    for b in (0, 1):
+        pg, row = c.places(b, c.lengths_list[b])
+        c.k[pg, row, :, 1:] = 0
+        c.k[pg, row, :, 0] = -40
+        k, v = c.k[pg[-300:], row[-300:]], c.v[pg[-300:], row[-300:]]
+        _place_odd_values(k, v, c.gen)
+        c.k[pg[-300:], row[-300:]], c.v[pg[-300:], row[-300:]] = k, v
+    t.k[:, :, :, 1:] = 0
+    t.k[:, 5, :, 0] = -70
+    t.v[:, 5, :, 20], t.v[:, 5, :, 21], t.v[:, 6, :, 22] = math.inf, -math.inf, math.nan
+    t.run(gpu_backend, scale=1.0)
+    for b, n in enumerate(t.counts_list):
+        length = c.lengths_list[b]
+        seen = torch.zeros((n, length + nodes), dtype=torch.bool, device="cuda")
+        seen[:, :length] = True
+        for i in range(n):
+            seen[i, [length + j for j in base._way(t.parents_list[b], i)]] = True
+        pg, row = c.places(b, length)
+        for h in range(heads):
+            g = h // (heads // kv_heads)
+            k, v = (torch.cat([pool[pg, row, g], new[b, :, g]]) for pool, new in ((c.k, t.k), (c.v, t.v)))
+            assert _check_odd(dtype, t.out[b, :n, h], k[:, 0], v, seen) >= (11 * n if b < 2 else 1)
+        assert (t.out[b, n:] == 7).all()
+    gpu_backend.operators_status(stream=_stream())
 
 
 # ---- page tables ---------------------------------------------------------------------------------------------------
