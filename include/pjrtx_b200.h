@@ -548,8 +548,9 @@ int pjrtx_b200_paged_cache_attend(PjrtxB200PagedCache *cache, const PjrtxB200Pag
  * log-sum-exp. parents[b, i] is a node before i, or -1 for a root, of which there may be several; any other parent counts as
  * -1 and is reported (43). Nothing is stored, lengths count cached rows only, and weights are not tracked. Results of nodes from counts[b]
  * on are left as they were. Keys and values that a node does not see enter nothing, whatever they hold; infinities and NaN in those
- * that it sees go on as in the formula, with probabilities below 2^-126 of the largest as zero. In 16 bits, probabilities are
- * rounded to the element type (f16: to multiples of 2^-35 of the largest below 2^-25) before they meet finite values; sums and lse are f32. */
+ * that it sees go on as in the formula, with probabilities below 2^-126 of the largest as zero. In 16 bits, a probability
+ * meets finite values as two numbers of the element type, off by 2^-16 of it (bf16) or 2^-22 (f16, and to multiples of 2^-36 of the largest); sums and
+ * lse are f32. */
 typedef struct PjrtxB200PagedTreeArgs {
   uint64_t struct_size;
   const void *q; /* [batch, nodes, heads, head_dim] through the strides */

@@ -263,7 +263,7 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
           const uint64_t v = desc_advance(v_first, (uint32_t)v_slot * kSlotBytes);
 #pragma unroll
           for (int kk = 0; kk < kKeys / 16; kk++)
-            mma_f16_tmem_a(o_col, s_col(buffer) + (uint32_t)kk * 8u, desc_advance(v, (uint32_t)kk * 2048u), idesc_o, (j > 0 || kk) ? 1u : 0u);
+            mma_values(o_col, s_col(buffer) + (uint32_t)kk * 16u, desc_advance(v, (uint32_t)kk * 2048u), idesc_o, (j > 0 || kk) ? 1u : 0u);
           if (more) scores(buffer, k_slot);
           mma_commit(&s_full[buffer]);
           mma_commit(&slot_empty[v_slot]);
@@ -329,7 +329,7 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
       const float shift = m_used == -INFINITY ? 0.f : Probability<BF16>::kLift - m_used;
       Pair part[2] = {0, 0};
 #pragma unroll
-      for (int c = 0; c < kKeys / 32; c++) store_probabilities<BF16>(s[c], a.scale_log2, shift, part, s_addr + c * 16);
+      for (int c = 0; c < kKeys / 32; c++) store_probabilities<BF16>(s[c], a.scale_log2, shift, part, s_addr + c * 32);
       const float2 block = pair_split(pair_add(part[0], part[1]));
       sum += block.x + block.y;
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");

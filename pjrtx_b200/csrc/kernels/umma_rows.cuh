@@ -11,15 +11,16 @@
 namespace pjrtx {
 namespace umma {
 
-// Probabilities go to the tensor core in the element type: two 16-bit numbers for each would make the second product twice as long, and as
-// one they add about as much to a result's error as its own rounding does. Their sum is taken before they are rounded, since the log-sum-exp
-// is f32 (of the rounded ones it would be off by up to 2^-9). In f16 they are multiplied by 2^11 first: f16 then holds them down to
-// 2^-35 of the largest, and not only to 2^-24.
-// They are relative to a maximum that follows the row's when that has grown by 2^8 (f16: 2^4, so that they stay below 2^16): the factor
+// A probability goes to the tensor core as two numbers of the element type: as one, it would be as far off as the result's own rounding, and results
+// 1.1 to 1.4 times as far from the exact ones as that leaves them (1.0 so). The second product and the split take 20 to 30 % of
+// long prompts (4 x 2048 tokens, 32 heads of 128 over 8: 146 us with one number, 181 with two) and 5 to 10 % of trees over cached rows, which are
+// bound by these. The sum is taken in f32, before. In f16 they are multiplied by 2^12 first: f16 then holds them down to 2^-36 of
+// the largest, and not only to 2^-24.
+// They are relative to a maximum that follows the row's when that has grown by 2^8 (f16: 2^3, so that they stay below 2^16): the factor
 // cancels in the division, and the results in tensor memory are rescaled that much more rarely. Where one row of a warp has to, all of them
 // follow theirs, so that the next time is later.
 template <bool BF16> struct Probability { static constexpr float kLift = 0.f, kGrow = 8.f; };
-template <> struct Probability<false> { static constexpr float kLift = 11.f, kGrow = 4.f; };
+template <> struct Probability<false> { static constexpr float kLift = 12.f, kGrow = 3.f; };
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float y;
@@ -51,22 +52,46 @@ __device__ __forceinline__ void tmem_store_16(uint32_t addr, const float* v) {
       : "memory");
 }
 
-// Probabilities 2^(s * scale + shift) of 32 scores into 16 columns of tensor memory, as pairs of the element type; `part` adds them up.
+// (y.x, y.y) >= 0 as the sum of two pairs, what is left of it when cut off and the rest, rounded: off by 2^-16 of it in bf16 and 2^-22 in f16, or,
+// where f16 is subnormal, by 2^-24 (2^-36 of the largest).
+template <bool BF16>
+__device__ __forceinline__ uint2 split_probabilities(float2 y) {
+  constexpr uint32_t kKeep = BF16 ? 0xffff0000u : 0xffffe000u;
+  const float2 cut = make_float2(__uint_as_float(__float_as_uint(y.x) & kKeep), __uint_as_float(__float_as_uint(y.y) & kKeep));
+  const float2 rest = pair_split(pair_fma(pair_of(cut.x, cut.y), pair_of(-1.f, -1.f), pair_of(y.x, y.y)));
+  const uint32_t high = BF16 ? __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x7632) : pack_pair<BF16>(cut.x, cut.y);
+  return make_uint2(high, pack_pair<BF16>(rest.x, rest.y));
+}
+
+// Probabilities 2^(s * scale + shift) of 32 scores, in the place of these: of 16 keys, eight columns of their first numbers and eight of the second ones,
+// as pairs; `part` adds them up.
 // All by the exponential unit, 16 results a cycle and SM: to compute some on the FMA units instead (a polynomial behind a split of the
 // exponent) made every case slower, 2 to 15 %, by the code that it takes.
 template <bool BF16>
 __device__ __forceinline__ void store_probabilities(const float (&s)[32], float scale, float shift, Pair (&part)[2], uint32_t to) {
   const Pair scale2 = pair_of(scale, scale), shift2 = pair_of(shift, shift);
-  float packed[16];
 #pragma unroll
-  for (int e = 0; e < 16; e++) {
-    const float2 x = pair_split(pair_fma(pair_of(s[2 * e], s[2 * e + 1]), scale2, shift2));
-    const float2 y = make_float2(exp2_approx(x.x), exp2_approx(x.y));
-    part[e & 1] = pair_add(part[e & 1], pair_of(y.x, y.y));
-    packed[e] = __uint_as_float(pack_pair<BF16>(y.x, y.y));
+  for (int h = 0; h < 32; h += 16) {
+    float packed[16];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const float2 x = pair_split(pair_fma(pair_of(s[h + 2 * e], s[h + 2 * e + 1]), scale2, shift2));
+      const float2 y = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+      part[e & 1] = pair_add(part[e & 1], pair_of(y.x, y.y));
+      const uint2 numbers = split_probabilities<BF16>(y);
+      packed[e] = __uint_as_float(numbers.x);
+      packed[8 + e] = __uint_as_float(numbers.y);
+    }
+    tmem_store_16(to + h, packed);
   }
-  tmem_store_16(to, packed);
 }
+
+// results += P . V for 16 keys, P at `probabilities` as above.
+__device__ __forceinline__ void mma_values(uint32_t results, uint32_t probabilities, uint64_t v, uint32_t idesc, uint32_t accumulate) {
+  mma_f16_tmem_a(results, probabilities, v, idesc, accumulate);
+  mma_f16_tmem_a(results, probabilities + 8, v, idesc, 1u);
+}
+
 // Whether one of two packed 16-bit elements is infinite or NaN.
 template <bool BF16>
 __device__ __forceinline__ bool odd_pair(uint32_t w) {

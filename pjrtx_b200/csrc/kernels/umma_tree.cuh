@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
             const uint64_t v = desc_advance(v_first, (uint32_t)v_slot * kSlotBytes);
 #pragma unroll
             for (int kk = 0; kk < kKeys / 16; kk++)
-              mma_f16_tmem_a(o_col(t), s_col(t, buffer) + (uint32_t)kk * 8u, desc_advance(v, (uint32_t)kk * 2048u), idesc_o, (!first || kk) ? 1u : 0u);
+              mma_values(o_col(t), s_col(t, buffer) + (uint32_t)kk * 16u, desc_advance(v, (uint32_t)kk * 2048u), idesc_o, (!first || kk) ? 1u : 0u);
             if (more) scores(t);
             mma_commit(&bar.s_full[t][buffer]);
           }
@@ -645,16 +645,15 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
           }
           const float shift = m_used == -INFINITY ? 0.f : Probability<BF16>::kLift - m_used;
           Pair part[2] = {0, 0};
-          float s[2][32];  // the next piece is on its way while this one is at work
-          tmem_load_32(s_addr, s[0]);
+          // One piece after the other: a second one on its way while the first is at work takes registers and code, and was slower (16 sequences of up to
+          // 4096 rows and 16 nodes 62 us, not 59, 32 of up to 2048 and 40 nodes 107, not 101), as were pieces of 16 (60 and 105).
 #pragma unroll 1
-          for (int c = 0; c < kKeys; c += 64)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-              asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-              if (c + h * 32 + 32 < kKeys) tmem_load_32(s_addr + c + h * 32 + 32, s[h ^ 1]);
-              store_probabilities<BF16>(s[h], a.scale_log2, shift, part, s_addr + (c + h * 32) / 2);
-            }
+          for (int c = 0; c < kKeys; c += 32) {
+            float s[32];
+            tmem_load_32(s_addr + c, s);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            store_probabilities<BF16>(s, a.scale_log2, shift, part, s_addr + c);
+          }
           const float2 block = pair_split(pair_add(part[0], part[1]));
           sum += block.x + block.y;
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");

@@ -33,6 +33,49 @@ def test_every_row_of_a_warp_is_computed_once_more(gpu_backend, dtype, heads, kv
     c.check("rows before the last")
 
 
+# A probability meets the values in 16 bits as two numbers, itself cut off and the rest rounded. The rest is below the last place that is kept, so that
+# half of its own last place is 2^-16 of a bf16 or 2^-22 of an f16; of f16 numbers that are subnormal, in 2^12 times the largest, twice 2^-25 may go.
+TWO_NUMBERS = {"f32": 0.0, "f16": 2.0 ** -22, "bf16": 2.0 ** -16}
+
+
+@pytest.fixture
+def finer(monkeypatch):
+    """The module's bounds with what two numbers lose of a probability, once: the sum has it in f32."""
+    monkeypatch.setattr(base, "PROBABILITY", {t: x / 2 for t, x in TWO_NUMBERS.items()})  # the bounds take it twice
+
+
+def _level(q, v, axis):
+    """Scores close to each other, whose own errors are small then, over values that nearly cancel."""
+    q *= 0.05
+    v.abs_()
+    for i in range(1, v.shape[axis], 2):
+        v.select(axis, i).neg_()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("heads,kv_heads,head_dim", [(8, 2, 128), (4, 2, 64), (2, 1, 256), (9, 3, 40)])
+@pytest.mark.parametrize("level", [False, True])
+def test_prompts_are_as_exact_as_their_rounding(gpu_backend, finer, dtype, heads, kv_heads, head_dim, level):
+    p = base._Prompts(dtype, heads, kv_heads, head_dim, [300, 1, 70, 0, 129], seed=heads)
+    if level:
+        _level(p.q, p.v, 0)
+    p.run(gpu_backend)
+    p.check(some=1500)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("heads,kv_heads,head_dim", [(8, 2, 128), (4, 2, 64), (2, 1, 256), (9, 3, 40)])
+@pytest.mark.parametrize("lengths,nodes,level", [([900, 0, 33], 1, False), ([900, 0, 33], 9, False), ([900, 0, 33], 64, False), ([0, 0, 0], 64, True)])
+def test_trees_are_as_exact_as_their_rounding(gpu_backend, finer, dtype, heads, kv_heads, head_dim, lengths, nodes, level):
+    t = base._Trees(dtype, heads, kv_heads, head_dim, 16, lengths, nodes, seed=nodes, counts=[nodes] * 3)
+    if level:
+        _level(t.q, t.v, 1)
+    t.run(gpu_backend)
+    t.check(some=900)
+
+
 ODD = [(17, 0.5), (3, -5.0), (100, -17.0), (200, -30.0), (299, -60.0), (150, -80.0)]  # key and score; values of dimensions 2 j and 2 j + 1 are infinite
 
 
