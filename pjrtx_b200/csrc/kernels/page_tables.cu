@@ -245,7 +245,8 @@ __global__ void __launch_bounds__(kPathThreads) paged_path_kernel(const PagedPat
   const int b = (blockIdx.x * kPathThreads + threadIdx.x) / 32, lane = threadIdx.x % 32;
   if (b >= a.batch) return;
   const int length = a.lengths[b], leaf = a.leaves[b];
-  const Ancestors above = tree_ancestors(a.parents + (long long)b * a.nodes, a.nodes, a.error_words);
+  const int known = leaf < 0 || leaf >= a.nodes ? 0 : leaf + 1;  // a way goes to lower nodes
+  const Ancestors above = tree_ancestors(a.parents + (long long)b * a.nodes, known, a.error_words);
   unsigned long long path = tree_of_node(above, max(0, min(leaf, kTreeNodesMax - 1)));
   const int rows = __popcll(path);
   if (leaf < 0) path = 0;

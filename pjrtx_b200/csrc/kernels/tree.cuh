@@ -16,7 +16,8 @@ __device__ __forceinline__ unsigned long long tree_of_node(const Ancestors& a, i
 }
 
 // By doubling: after i rounds a node knows its 2^i nearest ancestors and where to go on. Called by a whole warp; a parent that is not a
-// node before its child is reported and counts as none, so every way ends.
+// node before its child is reported and counts as none, so every way ends. Only the parents of the first `nodes` are read: what lies behind
+// a sequence's nodes may hold anything.
 __device__ __forceinline__ Ancestors tree_ancestors(const int* parents, int nodes, int* error_words) {
   const int lane = threadIdx.x % 32;
   int up[2];

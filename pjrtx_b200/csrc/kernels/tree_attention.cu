@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(rows::kThreads) tree_rows_kernel(const __grid_
     };
     __syncthreads();  // the segment before has been read
     if (warp == 0) {
-      const Ancestors above = tree_ancestors(p.a.parents + (long long)seg.b * p.a.nodes, p.a.nodes, p.c.error_words);
+      const Ancestors above = tree_ancestors(p.a.parents + (long long)seg.b * p.a.nodes, here.s.count, p.c.error_words);
       ancestors[lane] = above.low;
       ancestors[lane + 32] = above.high;
     }

@@ -586,7 +586,7 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
       const bool active = __any_sync(0xffffffffu, there);
       unsigned long long bits = 0;
       if (active) {
-        const Ancestors above = tree_ancestors(p.a.parents + (long long)seg.b * p.a.nodes, p.a.nodes, p.c.error_words);
+        const Ancestors above = tree_ancestors(p.a.parents + (long long)seg.b * p.a.nodes, here.s.count, p.c.error_words);
         bits = tree_of_node(above, there ? node : 0);
         if (!there) bits = 0;
       }

@@ -6,6 +6,7 @@ import re
 import numpy as np
 import pytest
 
+from pjrtx_b200 import backend as be_mod
 from pjrtx_b200 import plan as P
 from tests import test_prompts_and_trees as base
 from tests.test_operators import _stream, _within
@@ -167,6 +168,43 @@ def test_trees_keep_infinite_values_at_any_probability(gpu_backend, dtype, heads
             k, v = (torch.cat([pool[pg, row, g], new[b, :, g]]) for pool, new in ((c.k, t.k), (c.v, t.v)))
             assert _check_odd(dtype, t.out[b, :n, h], k[:, 0], v, seen) >= (11 * n if b < 2 else 1)
         assert (t.out[b, n:] == 7).all()
+    gpu_backend.operators_status(stream=_stream())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rubbish", [0, -7, 63, 1 << 30])
+def test_parents_behind_a_sequences_nodes_may_be_anything(gpu_backend, dtype, rubbish):
+    t = base._Trees(dtype, 8, 2, 64, 16, [40, 100, 0, 33], 40, seed=12, counts=[7, 0, 39, 40])
+    for b, n in enumerate(t.counts_list):
+        t.parents[b, n:] = rubbish
+    t.run(gpu_backend)
+    t.check(some=300)
+    gpu_backend.operators_status(stream=_stream())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rubbish", [0, -7, 63, 1 << 30])
+def test_parents_that_no_path_takes_may_be_anything(gpu_backend, rubbish):
+    """Of idle sequences and behind a path's leaf; those up to the leaf are still looked at."""
+    import torch
+
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    cache = gpu_backend.paged_cache(P.BF16_CODE, 4, 2, 1, 8, 4, 20)
+    parents = torch.full((4, 64), rubbish, dtype=torch.int32, device="cuda")
+    parents[1, :3], parents[3, :40] = ints([-1, 0, 0]), torch.arange(40, device="cuda").int() - 1
+    table, lengths = torch.arange(80, device="cuda").int().reshape(4, 20), ints([3, 5, 9, 0])
+    slots, out = torch.zeros((4, 64), dtype=torch.int32, device="cuda"), ints([0] * 4)
+    cache.path_slots(table, lengths, parents, ints([-1, 2, -5, 39]), slots, lengths_out=out, stream=_stream())
+    gpu_backend.operators_status(stream=_stream())
+    want = [[-1] * 64 for _ in range(4)]
+    want[1][0], want[1][2] = 85, 86
+    want[3][:40] = range(240, 280)
+    assert slots.tolist() == want and out.tolist() == [3, 7, 9, 40]
+    cache.path_slots(table, lengths, parents, ints([-1, 3, -5, 39]), slots, lengths_out=out, stream=_stream())
+    if rubbish:  # node 3 may have node 0 for its parent
+        with pytest.raises(be_mod.BackendError, match="code 43"):
+            gpu_backend.operators_status(stream=_stream())
     gpu_backend.operators_status(stream=_stream())
 
 
