@@ -592,8 +592,9 @@ int pjrtx_b200_paged_cache_store(PjrtxB200PagedCache *cache, const PjrtxB200Page
 
 /* Gives every sequence the pages of lengths[b] rows. held[b] counts the pages a sequence has; free_pages is a stack of
  * *free_count page ids, its top at the end. First, pages beyond what the lengths need go onto the stack, by sequence and column, and
- * their table entries become -1. Then sequences take what they lack from the top, in order; the first that wants more than is
- * left, and all behind it that want any, keep what they have (held_out[b] * page_size < lengths[b] tells). Popped places of the
+ * their table entries become -1; entries that name no page of the pool are reported (40) and go nowhere. Then sequences take what they lack from the top, in order; the first that wants more than is
+ * left, and all behind it that want any, keep what they have (held_out[b] * page_size < lengths[b] tells). An id on the stack
+ * that is none of the pool's goes to the sequence whose turn it is, is reported (40), and its slots are -1. Popped places of the
  * stack become -1. A sequence whose length or page count the table cannot hold is reported (41) and left as it is. With `slots`: packed
  * token t of sequence b, starts[b] <= t < starts[b + 1], is one of its last starts[b + 1] - starts[b] rows, and slots[t] that row's
  * slot; -1 for tokens of no sequence and of one without enough pages. Page tables must not name a page twice. The results may

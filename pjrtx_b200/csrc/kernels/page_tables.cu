@@ -1,6 +1,7 @@
 // Page tables and slots of a paged key-value cache, built where the lengths are: on the device.
 //
-// assign: need = ceil(length / page_size). Surplus pages go onto the stack of free ones, ordered by (sequence, column); then the i-th page
+// assign: need = ceil(length / page_size). Surplus pages go onto the stack of free ones, ordered by (sequence, column), entries that name no
+// page of the pool left out; then the i-th page
 // wanted, in the same order, is the i-th from the top, for the sequences whose running sum of wants fits what is there. Both orders are
 // prefix sums over the batch, so the result does not depend on who is first.
 //
@@ -129,16 +130,36 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads) page
   if (!stack_ok && rank == 0 && threadIdx.x == 0) report(a.error_words, kErrorLength);
   auto started = cluster.barrier_arrive();  // the other blocks' shared memory is written once they are known to run
 
+  // What each sequence has to give and wants.
+  bool gives = false;
+  for (int b = first + threadIdx.x; b < last; b += kThreads) {
+    const Want w = want_of(a, b, stack_ok);
+    if (!w.ok) report(a.error_words, kErrorLength);
+    offsets[b - first] = make_longlong2(max(0, w.held - w.need), max(0, w.need - w.held));
+    gives = gives || w.held > w.need;
+  }
+  // Of surplus entries, those that name a page: the others go nowhere, or another sequence would get them.
+  if (__syncthreads_or(gives)) {
+    for (int b = first + warp; b < last; b += kWarps) {
+      const int surplus = (int)offsets[b - first].x;
+      if (surplus == 0) continue;
+      const int* from = a.table + b * a.table_stride + want_of(a, b, stack_ok).need;
+      int pages = 0;
+      in_batches(lane, surplus, 32, [&](long long j) { return from[j]; }, [&](long long, int page) { pages += page >= 0 && page < a.num_pages; });
+      pages = __reduce_add_sync(~0u, pages);
+      if (lane == 0) offsets[b - first].x = pages;
+      if (lane == 0 && pages < surplus) report(a.error_words, kErrorPageId);
+    }
+    __syncthreads();
+  }
   // How many pages the sequences before have to give and want.
   long long give = 0, take = 0;
   for (int b0 = first; b0 < last; b0 += kThreads) {
     const int b = b0 + threadIdx.x;
-    Want w = {0, 0, 1};
-    if (b < last) w = want_of(a, b, stack_ok);
-    if (!w.ok) report(a.error_words, kErrorLength);
+    const longlong2 mine = b < last ? offsets[b - first] : make_longlong2(0, 0);
     long long given, taken;
-    const long long give_at = give + block_prefix(max(0, w.held - w.need), warp_sums, &given);
-    const long long take_at = take + block_prefix(max(0, w.need - w.held), warp_sums, &taken);
+    const long long give_at = give + block_prefix(mine.x, warp_sums, &given);
+    const long long take_at = take + block_prefix(mine.y, warp_sums, &taken);
     if (b < last) offsets[b - first] = make_longlong2(give_at, take_at);
     give += given;
     take += taken;
@@ -165,13 +186,23 @@ __global__ void __cluster_dims__(kBlocks, 1, 1) __launch_bounds__(kThreads) page
     const Want w = want_of(a, b, stack_ok);
     const longlong2 at = offsets[b - first];
     const int* surplus = a.table + b * a.table_stride + w.need;
-    const long long top = free_count + give_before + at.x;
-    in_batches(
-        lane, w.held - w.need, 32, [&](long long j) { return surplus[j]; },
-        [&](long long j, int page) {
-          if (page < 0 || page >= a.num_pages) report(a.error_words, kErrorPageId);
-          if (top + j < a.num_pages) a.free_pages_out[top + j] = page;
-        });
+    long long top = free_count + give_before + at.x;
+    for (int j0 = 0; j0 < w.held - w.need; j0 += 128) {
+      int page[4];
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int j = j0 + u * 32 + lane;
+        page[u] = j < w.held - w.need ? surplus[j] : -1;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const bool valid = page[u] >= 0 && page[u] < a.num_pages;
+        const unsigned pages = __ballot_sync(~0u, valid);
+        const long long to = top + __popc(pages & ((1u << lane) - 1));
+        if (valid && to < a.num_pages) a.free_pages_out[to] = page[u];
+        top += __popc(pages);
+      }
+    }
     const int wanted = w.need - w.held;
     if (wanted > 0 && take_before + at.y + wanted <= there) granted += wanted;
   }

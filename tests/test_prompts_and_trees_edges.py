@@ -259,3 +259,52 @@ def test_assign_pages_while_other_kernels_hold_the_device(gpu_backend):
         assert outs[0].tolist() == want_held and np.array_equal(outs[1].cpu().numpy(), want_table)
         assert outs[2][:len(want_free)].tolist() == want_free and int(outs[3]) == len(want_free)
     gpu_backend.operators_status(stream=_stream())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("bad", [-1, -5, 400, 1 << 30])
+def test_surplus_entries_that_name_no_page_go_nowhere(gpu_backend, in_place, bad):
+    """What a sequence gives back counts as far as it is pages of the pool, and the others get nothing else."""
+    import torch
+
+    rng = np.random.default_rng(11)
+    batch, page, max_pages, pool = 40, 4, 300, 400
+    ints = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device="cuda")
+    held, need = np.zeros(batch, int), np.zeros(batch, int)
+    held[[1, 5, 20, 39]], need[[1, 5, 20, 39]] = [200, 3, 40, 20], [10, 0, 39, 20]
+    need[[0, 2, 6, 30]] = [3, 150, 9, 40]  # 202 in all, of 10 free ones and those that come back
+    pages, at = rng.permutation(pool), 0
+    table = np.full((batch, max_pages), -1)
+    for b, n in enumerate(held):
+        table[b, :n] = pages[at:at + n]
+        at += n
+    for b, columns in ((1, [10, 17, 42, 137, 138, 199]), (5, [0, 1, 2]), (20, [39])):
+        table[b, columns] = bad
+    free = pages[at:at + 10].tolist()
+    good = lambda x: 0 <= x < pool
+    want_free = free + [x for b in range(batch) for x in table[b, need[b]:held[b]].tolist() if good(x)]
+    want_table, want_held = table.copy(), held.copy()
+    for b in range(batch):
+        want_table[b, need[b]:held[b]] = -1
+        want_held[b] = min(held[b], need[b])
+    assert len(want_free) == 10 + 190 - 6 and need[[0, 2, 6]].sum() <= len(want_free) < need[[0, 2, 6, 30]].sum()
+    for b in (0, 2, 6):  # the last one's 40 are not there
+        want_table[b, :need[b]] = [want_free.pop() for _ in range(need[b])]
+        want_held[b] = need[b]
+    stack = np.full(pool, -1)
+    stack[:10] = free
+    args = [ints(need * page), ints(held), ints(table), ints(stack), ints([10])]
+    outs = {} if in_place else {n: torch.full_like(a, 77) for n, a in zip(("held_out", "page_table_out", "free_pages_out", "free_count_out"), args[1:])}
+    cache = gpu_backend.paged_cache(P.BF16_CODE, batch, 2, 1, 8, page, max_pages)
+    starts, slots = ints(range(batch + 1)), torch.zeros(batch, dtype=torch.int32, device="cuda")
+    cache.assign_pages(*args, starts=starts, slots=slots, stream=_stream(), **outs)
+    with pytest.raises(be_mod.BackendError, match="code 40"):
+        gpu_backend.operators_status(stream=_stream())
+    got = [x.cpu().numpy() for x in (args[1:] if in_place else outs.values())]
+    assert got[0].tolist() == want_held.tolist() and np.array_equal(got[1], want_table)
+    assert int(got[3][0]) == len(want_free) and got[2][:len(want_free)].tolist() == want_free
+    assert slots[2] == want_table[2, 149] * page + 3 and slots[30] == -1
+    # and the call after it, with what is left
+    cache.assign_pages(ints([page] * batch), *[ints(x) for x in got], stream=_stream())
+    gpu_backend.operators_status(stream=_stream())
