@@ -115,7 +115,8 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
   uint64_t* v_clean = slot_empty + kSlots;      // values behind the last position have been cleared
   uint64_t* s_full = v_clean + 1;  // [2] scores of a block are in tensor memory, and the product two blocks before it is done
   uint64_t* p_ready = s_full + 2;  // [2] its probabilities are
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_ready + 2);
+  uint64_t* drained = p_ready + 2;  // no product is under way
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   int* flags = reinterpret_cast<int*>(tmem_slot + 1);  // [0] abort
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -138,6 +139,7 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
       mbar_init(&slot_empty[s], 1);
     }
     mbar_init(v_clean, 1);
+    mbar_init(drained, 1);
     for (int i = 0; i < 2; i++) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_ready[i], 4);
@@ -169,18 +171,10 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
       int slot = 0;
       unsigned phase = 0;
       bool ok = true;
-      int keys_of = 0, values_of = 0;  // the next blocks
-      for (int i = 0; i < 2 * blocks; i++) {
-        if (i >= kSlots && !__all_sync(0xffffffffu, mbar_wait(&slot_empty[slot], phase ^ 1, budget))) {
-          // The copies in flight get a bounded time to land before the block of threads leaves.
-          for (int r = 1; r <= kSlots && leader; r++) {
-            const int j = i - r;
-            for (unsigned spin = 0; spin < (1u << 16) && !mbar_try_wait(&slot_full[j % kSlots], (unsigned)(j / kSlots) & 1u); spin++) {
-            }
-          }
-          ok = false;
-          break;
-        }
+      int keys_of = 0, values_of = 0, issued = 0;  // the next blocks, and copies into slots
+      for (; issued < 2 * blocks; issued++) {
+        ok = issued < kSlots || __all_sync(0xffffffffu, mbar_wait(&slot_empty[slot], phase ^ 1, budget));
+        if (!ok) break;
         const bool is_keys = keys_of < blocks && keys_of < values_of + 2;
         const int block = is_keys ? keys_of++ : values_of++;
         if (leader) {
@@ -206,6 +200,11 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
           __syncwarp();
           if (lane == 0) mbar_arrive(v_clean);
         }
+      }
+      if (leader) {
+        const unsigned long long until = global_timer_ns() + kLandNs;
+        wait_landed(q_full, 0, until);
+        for (int i = issued - 1; i >= 0 && i >= issued - kSlots; i--) wait_landed(&slot_full[i % kSlots], (unsigned)(i / kSlots) & 1u, until);
       }
       __syncwarp();
     } else if (warp == kMmaWarp) {
@@ -271,7 +270,11 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
         }
         __syncwarp();
       }
-      if (!ok && leader) report(p.error_words, kErrorWait);
+      if (leader) {
+        if (!ok) report(p.error_words, kErrorWait);
+        mma_commit(drained);
+        wait_landed(drained, 0, global_timer_ns() + kLandNs);
+      }
       __syncwarp();
     }
   } else {

@@ -43,6 +43,14 @@ __device__ __forceinline__ WaitBudget budget_from_now(unsigned long long timeout
   return WaitBudget{global_timer_ns() + timeout_ns, abort};
 }
 
+// A block of threads leaves behind the copies and products that it has under way, whichever of its warps has given up: these waits are for them
+// alone, which end by themselves, and take 17 ms at most, where a barrier's other arrivals do not come.
+constexpr unsigned long long kLandNs = 1ull << 24;
+__device__ __forceinline__ void wait_landed(uint64_t* bar, unsigned parity, unsigned long long until) {
+  while (!mbar_try_wait(bar, parity) && global_timer_ns() < until) {
+  }
+}
+
 __device__ __forceinline__ void tmem_store_16(uint32_t addr, const float* v) {
   const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
   asm volatile(

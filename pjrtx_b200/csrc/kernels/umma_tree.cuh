@@ -169,6 +169,7 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
     uint64_t p_ready[TILES][kBuffers];  // its probabilities are
     uint64_t clean[kCleanRing];         // nodes with values that are infinite or NaN have been cleared in the slot
     uint64_t odd_ready[kOddRing];       // of a segment
+    uint64_t drained;                   // no product is under way
     unsigned long long odd[kOddRing];   // which nodes these are
     uint32_t tmem;
     int abort;
@@ -200,6 +201,7 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
       }
     for (int i = 0; i < kCleanRing; i++) mbar_init(&bar.clean[i], 1);
     for (int i = 0; i < kOddRing; i++) mbar_init(&bar.odd_ready[i], 1);
+    mbar_init(&bar.drained, 1);
     bar.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -264,7 +266,8 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
     unsigned phase = 0;
     long long used = 0;
     auto take_slot = [&](uint32_t* at) {  // false: given up
-      if (used++ >= kSlots && !wait(&bar.slot_empty[slot], phase ^ 1)) return false;
+      if (used >= kSlots && !wait(&bar.slot_empty[slot], phase ^ 1)) return false;
+      used++;
       *at = ring + (uint32_t)slot * kSlotBytes;
       return true;
     };
@@ -392,10 +395,8 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
         }
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
-      // Given up: the boxes under way get a bounded time to land before the block of threads leaves.
-      for (long long u = used - 1; !ok && u >= 0 && u >= used - kSlots; u--)
-        for (unsigned spin = 0; spin < (1u << 14) && !mbar_try_wait(&bar.slot_full[u % kSlots], (unsigned)(u / kSlots) & 1u); spin++) {
-        }
+      const unsigned long long until = global_timer_ns() + kLandNs;
+      for (long long u = used - 1; u >= 0 && u >= used - kSlots; u--) wait_landed(&bar.slot_full[u % kSlots], (unsigned)(u / kSlots) & 1u, until);
     }
   } else if (warp == kMmaWarp) {
     const bool leader = elect_one();
@@ -497,7 +498,11 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
         if (!next_unit(p, now, number, share.size)) break;
         first = now.b != here.b || now.group != here.group;
       }
-      if (!ok && leader) report(p.c.error_words, kErrorWait);
+      if (leader) {
+        if (!ok) report(p.c.error_words, kErrorWait);
+        mma_commit(&bar.drained);
+        wait_landed(&bar.drained, 0, global_timer_ns() + kLandNs);
+      }
       __syncwarp();
     }
   } else if (warp == kMmaWarp + 1) {

@@ -2,6 +2,8 @@
 import math
 import os
 import re
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -10,6 +12,8 @@ from pjrtx_b200 import backend as be_mod
 from pjrtx_b200 import plan as P
 from tests import test_prompts_and_trees as base
 from tests.test_operators import _stream, _within
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 @pytest.mark.gpu
@@ -208,12 +212,58 @@ def test_parents_that_no_path_takes_may_be_anything(gpu_backend, rubbish):
     gpu_backend.operators_status(stream=_stream())
 
 
+_GIVE_UP = """
+import torch
+from pjrtx_b200 import backend as be_mod
+from pjrtx_b200 import plan as P
+be = be_mod.Backend()
+stream = torch.cuda.current_stream().cuda_stream
+gen = torch.Generator(device="cuda").manual_seed(1)
+rand = lambda *shape: torch.randn(shape, generator=gen, device="cuda").bfloat16()
+batch, heads, page, rows = 600, 32, 16, 2000
+cache = be.paged_cache(P.BF16_CODE, batch, heads, 1, 64, page, rows // page, tree=1)
+ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+k_pages, v_pages, table = rand(rows // page, page, 1, 64), rand(rows // page, page, 1, 64), torch.arange(rows // page, device="cuda").int().repeat(batch, 1)
+q, k, v = rand(batch, 1, heads, 64), rand(batch, 1, 1, 64), rand(batch, 1, 1, 64)
+def run():
+    out = torch.zeros_like(q)
+    cache.attend_tree(q, k_pages, v_pages, table, ints([rows] * batch), out, k, v, ints([[-1]] * batch), stream=stream)
+    keys, values = (torch.cat([x.reshape(1, rows, 64).expand(batch, -1, -1), y.reshape(batch, 1, 64)], 1).double() for x, y in ((k_pages, k), (v_pages, v)))
+    want = torch.softmax(q[:, 0].double() @ keys.transpose(1, 2) / 8, 2) @ values
+    try:
+        be.operators_status(stream=stream)
+        status = "fine"
+    except be_mod.BackendError as e:
+        status = str(e)
+    print(float((out[:, 0].double() - want)[:, :, 1:].abs().max()) < 0.01, status)
+run()
+v_pages[5, 3, 0, 0] = float("inf")
+run()
+v_pages[5, 3, 0, 0] = 0
+run()
+"""
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
+def test_waits_that_run_out_end_the_call_and_are_reported(gpu_backend):
+    """With a budget of a millisecond, and rows that are computed once more for some milliseconds while the other warps wait for theirs: the kernel gives
+    up, says so (44), and the next call is right."""
+    done = subprocess.run([sys.executable, "-c", _GIVE_UP], capture_output=True, text=True, timeout=250, cwd=ROOT,
+                          env={**os.environ, "PJRTX_B200_WAIT_TIMEOUT_MS": "1"})
+    assert done.returncode == 0, done.stderr[-2000:]
+    lines = done.stdout.splitlines()
+    assert lines[0] == lines[2] == "True fine" and "code 44" in lines[1], lines
+    done = subprocess.run([sys.executable, "-c", _GIVE_UP], capture_output=True, text=True, timeout=250, cwd=ROOT)
+    assert done.returncode == 0 and done.stdout.splitlines() == ["True fine"] * 3, (done.stdout, done.stderr[-2000:])
+
+
 # ---- page tables ---------------------------------------------------------------------------------------------------
 
 
 def test_blocks_of_a_cluster_are_known_to_run_before_one_writes_another(backend):
     """Shared memory of another block may be written once it has started, which the cluster's barrier tells."""
-    kernels = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "pjrtx_b200", "csrc", "kernels")
+    kernels = os.path.join(ROOT, "pjrtx_b200", "csrc", "kernels")
     seen = 0
     for name in sorted(os.listdir(kernels)):
         with open(os.path.join(kernels, name)) as f:
