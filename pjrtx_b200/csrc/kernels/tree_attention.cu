@@ -498,7 +498,7 @@ bool start(void (*kernel)(const umma::TreeKernelArgs, const CUtensorMap, const C
     const long long extents[4] = {c.head_dim, c.page_size, c.kv_heads, c.num_pages}, strides[3] = {c.row_stride, c.head_stride, c.page_stride};
     const int box[4] = {64, a.box, 1, 1};
     if (!umma::encode_map(&kmap, c.k, c.dtype == kF16, 4, extents, strides, box) || !umma::encode_map(&vmap, c.v, c.dtype == kF16, 4, extents, strides, box))
-      a.box = 0;  // rows one by one
+      return false;
   }
   return launch_kernel(kernel, dim3((unsigned)p.blocks), dim3((unsigned)plan.threads), plan.smem, stream, pdl, a, kmap, vmap) == cudaSuccess;
 }

@@ -212,6 +212,41 @@ def test_parents_that_no_path_takes_may_be_anything(gpu_backend, rubbish):
     gpu_backend.operators_status(stream=_stream())
 
 
+# Of head_dim 64 and 128 a loader has 32 rows of a block, of 256 16: pages of 8, 16 and 32 rows are a box each, of 64 to 128 several, of 24 and 48 not whole ones.
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("heads,kv_heads,head_dim", [(8, 2, 64), (8, 2, 128), (4, 2, 256)])
+@pytest.mark.parametrize("page,layout", [(8, "nhd"), (16, "hnd"), (24, "nhd"), (32, "nhd"), (32, "hnd"), (48, "hnd"), (64, "nhd"), (96, "hnd"), (128, "nhd")])
+@pytest.mark.parametrize("nodes", [5, 50])
+def test_trees_on_pages_of_boxes(gpu_backend, finer, dtype, heads, kv_heads, head_dim, page, layout, nodes):
+    """Blocks of whole boxes, and what is left of the last one; a table entry that names no page, in a box of its own or in one of several."""
+    t = base._Trees(dtype, heads, kv_heads, head_dim, page, [1200, 128, 515, 127], nodes, seed=page + nodes, layout=layout, counts=[nodes, 1, nodes - 2, nodes])
+    t.run(gpu_backend)
+    t.check(some=250)
+    gpu_backend.operators_status(stream=_stream())
+    for entry in (-1, t.case.k.shape[0], 1 << 30):
+        table = t.case.table.clone()
+        t.case.table[0, 1200 // page // 2] = entry
+        t.out.fill_(7), t.lse.fill_(7)
+        t.run(gpu_backend)
+        with pytest.raises(be_mod.BackendError, match="code 40"):
+            gpu_backend.operators_status(stream=_stream())
+        t.case.table = table
+        t.check(some=120, skip=(0,), what="the other sequences")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("order", [(0, 2, 1), (1, 0, 2), (1, 2, 0), (2, 0, 1), (2, 1, 0)])
+@pytest.mark.parametrize("page", [16, 6])
+def test_trees_on_pages_whose_axes_lie_in_any_order(gpu_backend, dtype, order, page):
+    t = base._Trees(dtype, 6, 3, 64, page, [300, 0, 77], 9, seed=5)
+    c, back = t.case, [order.index(i) for i in range(3)]
+    c.k, c.v = (x.permute(*order, 3).contiguous().permute(*back, 3) for x in (c.k, c.v))
+    t.run(gpu_backend)
+    t.check(some=200)
+
+
 _GIVE_UP = """
 import torch
 from pjrtx_b200 import backend as be_mod
