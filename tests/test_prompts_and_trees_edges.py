@@ -393,3 +393,21 @@ def test_surplus_entries_that_name_no_page_go_nowhere(gpu_backend, in_place, bad
     # and the call after it, with what is left
     cache.assign_pages(ints([page] * batch), *[ints(x) for x in got], stream=_stream())
     gpu_backend.operators_status(stream=_stream())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 4095, 4096, 4097, 9000])
+def test_slots_by_the_cluster_and_by_a_kernel_of_their_own(gpu_backend, tokens):
+    import torch
+
+    ints = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device="cuda")
+    page, max_pages, lengths = 16, 400, [0, tokens // 2, 300, tokens - tokens // 2]
+    new, rng = [0, tokens // 2, 0, tokens - tokens // 2], np.random.default_rng(tokens)
+    table, starts = rng.permutation(4 * max_pages).reshape(4, max_pages), np.cumsum([0] + new)
+    held = [-(-n // page) for n in lengths]
+    cache = gpu_backend.paged_cache(P.BF16_CODE, 4, 2, 1, 8, page, max_pages)
+    slots, free = torch.full((tokens,), 77, dtype=torch.int32, device="cuda"), ints([-1] * 4 * max_pages)
+    cache.assign_pages(ints(lengths), ints(held), ints(table), free, ints([0]), starts=ints(starts), slots=slots, stream=_stream())
+    gpu_backend.operators_status(stream=_stream())
+    want = np.concatenate([table[b, np.arange(n) // page] * page + np.arange(n) % page for b, n in enumerate(lengths) if new[b]])
+    assert np.array_equal(slots.cpu().numpy(), want)
