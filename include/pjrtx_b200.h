@@ -549,7 +549,7 @@ int pjrtx_b200_paged_cache_attend(PjrtxB200PagedCache *cache, const PjrtxB200Pag
  * -1 and is reported (43); from counts[b] on they are not read. Nothing is stored, lengths count cached rows only, and weights are not tracked. Results of nodes from counts[b]
  * on are left as they were. Keys and values that a node does not see enter nothing, whatever they hold; infinities and NaN in those
  * that it sees go on as in the formula, with probabilities below 2^-126 of the largest as zero. In 16 bits, a probability
- * meets finite values as two numbers of the element type, off by 2^-16 of it (bf16) or 2^-22 (f16, and to multiples of 2^-36 of the largest); sums and
+ * meets finite values as two numbers of the element type, off by 2^-16 of it (bf16) or 2^-22 (f16, and to multiples of 2^-35 of the largest); sums and
  * lse are f32. */
 typedef struct PjrtxB200PagedTreeArgs {
   uint64_t struct_size;

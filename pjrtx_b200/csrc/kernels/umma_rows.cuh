@@ -14,13 +14,13 @@ namespace umma {
 // A probability goes to the tensor core as two numbers of the element type: as one, it would be as far off as the result's own rounding, and results
 // 1.1 to 1.4 times as far from the exact ones as that leaves them (1.0 so). The second product and the split take 20 to 30 % of
 // long prompts (4 x 2048 tokens, 32 heads of 128 over 8: 146 us with one number, 181 with two) and 5 to 10 % of trees over cached rows, which are
-// bound by these. The sum is taken in f32, before. In f16 they are multiplied by 2^12 first: f16 then holds them down to 2^-36 of
+// bound by these. The sum is taken in f32, before. In f16 they are multiplied by 2^11 first: f16 then holds them down to 2^-35 of
 // the largest, and not only to 2^-24.
-// They are relative to a maximum that follows the row's when that has grown by 2^8 (f16: 2^3, so that they stay below 2^16): the factor
-// cancels in the division, and the results in tensor memory are rescaled that much more rarely. Where one row of a warp has to, all of them
-// follow theirs, so that the next time is later.
+// They are relative to a maximum that follows the row's when that has grown by 2^8 (f16: 2^4, so that they stay below 2^16; by 2^3 long prompts take
+// 3 % more): the factor cancels in the division, and the results in tensor memory are rescaled that much more rarely. Where one row of a warp has
+// to, all of them follow theirs, so that the next time is later.
 template <bool BF16> struct Probability { static constexpr float kLift = 0.f, kGrow = 8.f; };
-template <> struct Probability<false> { static constexpr float kLift = 12.f, kGrow = 3.f; };
+template <> struct Probability<false> { static constexpr float kLift = 11.f, kGrow = 4.f; };
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float y;
@@ -61,13 +61,19 @@ __device__ __forceinline__ void tmem_store_16(uint32_t addr, const float* v) {
 }
 
 // (y.x, y.y) >= 0 as the sum of two pairs, what is left of it when cut off and the rest, rounded: off by 2^-16 of it in bf16 and 2^-22 in f16, or,
-// where f16 is subnormal, by 2^-24 (2^-36 of the largest).
+// where the rest is subnormal, by 2^-25 (2^-36 of the largest).
 template <bool BF16>
 __device__ __forceinline__ uint2 split_probabilities(float2 y) {
-  constexpr uint32_t kKeep = BF16 ? 0xffff0000u : 0xffffe000u;
-  const float2 cut = make_float2(__uint_as_float(__float_as_uint(y.x) & kKeep), __uint_as_float(__float_as_uint(y.y) & kKeep));
+  uint32_t high;
+  float2 cut;
+  if (BF16) {
+    high = __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x7632);
+    cut = make_float2(__uint_as_float(__float_as_uint(y.x) & 0xffff0000u), __uint_as_float(__float_as_uint(y.y) & 0xffff0000u));
+  } else {
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(high) : "f"(y.y), "f"(y.x));
+    cut = __half22float2(*reinterpret_cast<const __half2*>(&high));
+  }
   const float2 rest = pair_split(pair_fma(pair_of(cut.x, cut.y), pair_of(-1.f, -1.f), pair_of(y.x, y.y)));
-  const uint32_t high = BF16 ? __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x7632) : pack_pair<BF16>(cut.x, cut.y);
   return make_uint2(high, pack_pair<BF16>(rest.x, rest.y));
 }
 

@@ -39,7 +39,7 @@ def test_every_row_of_a_warp_is_computed_once_more(gpu_backend, dtype, heads, kv
 
 
 # A probability meets the values in 16 bits as two numbers, itself cut off and the rest rounded. The rest is below the last place that is kept, so that
-# half of its own last place is 2^-16 of a bf16 or 2^-22 of an f16; of f16 numbers that are subnormal, in 2^12 times the largest, twice 2^-25 may go.
+# half of its own last place is 2^-16 of a bf16 or 2^-22 of an f16; an f16 that is subnormal, in 2^11 times the largest, may lose 2^-25.
 TWO_NUMBERS = {"f32": 0.0, "f16": 2.0 ** -22, "bf16": 2.0 ** -16}
 
 
