@@ -1,17 +1,16 @@
 // Page tables and slots of a paged key-value cache, built where the lengths are: on the device.
 //
 // assign: need = ceil(length / page_size). Surplus pages go onto the stack of free ones, ordered by (sequence, column), entries that name no
-// page of the pool left out; then the i-th page
-// wanted, in the same order, is the i-th from the top, for the sequences whose running sum of wants fits what is there. Both orders are
-// prefix sums over the batch, so the result does not depend on who is first.
+// page of the pool left out; then the i-th page wanted, in the same order, is the i-th from the top, for the sequences whose running sum of wants
+// fits what is there. Both orders are prefix sums over the batch, so the result does not depend on who is first.
 //
 // path: a drafted token is accepted when it lies on the way from the leaf to its root; its row is the number of those before it.
 //
 // All of it is a few hundred KB at most (a table of 512 x 256 pages and its copy: 1 MB), so what counts is the number of trips to memory
 // in a row: one launch of one cluster, whose blocks pass sums and pages to each other between cluster barriers, and loops that have several
-// loads under way. 32 sequences that grow by a row take 7.5 us, 512 that get new prompts of up to 4096 tokens, with the slots of all of these
-// (377 000, by a kernel of their own), 20.8 (27.3 with one load after the other, 20.4 with eight at a time, which takes 4096 sequences of 64 pages
-// from 49 to 59; blocks of 1024 threads 10.5, 21.1 and 38). Path slots of 256 trees of 64 nodes take 2.3 us, with the
+// loads under way. 32 sequences that grow by a row take 7.8 us, 512 that get new prompts of up to 4096 tokens, with the slots of all of these
+// (377 000, by a kernel of their own), 23.0, of which counting the surplus pages first is 1.7; 4096 sequences of 64 pages 55. Before that count, one load
+// after the other took 27.3, not 20.8, eight at a time 20.4 and 59, not 49, with 4096 sequences; blocks of 1024 threads 10.5, 21.1 and 38. Path slots of 256 trees of 64 nodes take 2.5 us, with the
 // ancestors in six rounds of doubling and not by up to 63 steps of a chain.
 #include <cooperative_groups.h>
 

@@ -10,8 +10,8 @@
 // the sixteen threads that have it. The next keys and values come by cp.async while these are at work. One or two rows a
 // thread are for trees of few rows, which would compute rows that are not there. Bound by FMAs and the reads of shared memory beside them:
 // 16 sequences of up to 2000 rows, 32 heads of 128 over 8, take 173 us with 8 nodes, 154 with one and 634 with 40; prompts of 4 x 2048 tokens
-// of such heads 3.9 ms (35 TFLOP/s), 517 tokens 76 us, 48 prompts of up to 200, four heads of 64 over two, 28. A warp leaves out keys that none of
-// its rows sees, half a block of scores or four values at a time (82 and 36 us without).
+// of such heads 3.9 ms (35 TFLOP/s), 517 tokens 76 us, 48 prompts of 67 to 200, four heads of 64 over two, 30 from long to short and 37
+// in no order. A warp leaves out keys that none of its rows sees, half a block of scores or four values at a time (517 tokens 82 us without).
 // What a row does not see enters nothing: scores are replaced, and where values of a block are infinite or NaN the products with
 // hidden keys are left out one by one.
 #pragma once

@@ -11,12 +11,15 @@
 //                  64 keys, for which two buffers fit: 211 us, not 171, where 64 nodes of 64 heads see 65536 rows)
 //   softmax warps  four a tile, a query row a thread; those whose rows are not there only count along
 //
-// Bound by memory up to two tiles: 128 keys of 128 elements are 64 KB of keys and values, 2650 cycles as measured in the middle of a long share (7 TB/s
-// over all SMs), and take 1024 cycles of tensor core and of exponentials for each tile. Around that stand 6 to 7 us of launch, shares, page ids and first rows,
-// and 5 to 10 of the join: 16 sequences of up to 4096 rows, 16 nodes of 32 heads over 8, pages of 16 rows 54 to 56 us (182 MB, 3.3 TB/s; 46.9 without the
-// join), one sequence of 65536 rows and 32 nodes 64 to 67, 517 rows and 8 nodes 13.3. 65536 rows and 64 nodes of 64 heads over 8, four tiles a KV
-// head that read every row twice, 161 to 165 us: 137 GFLOP at 0.85 PFLOP/s, bound by two tiles' exponentials and their instructions taking turns
-// with the tensor core.
+// Bound by memory up to two tiles, nearly: 128 keys of 128 elements are 64 KB of keys and values, 2650 cycles as measured in the middle of a long share
+// (7 TB/s over all SMs), and take 1024 cycles of exponentials and, with two numbers a probability, 1536 of the tensor core for each tile. Around that stand
+// 6 to 7 us of launch, shares, page ids and first rows, and 5 to 10 of the join: 16 sequences of up to 4096 rows, 16 nodes of 32 heads over 8, pages of 16
+// rows 56 to 59 us (184 MB, 3.2 TB/s), one sequence of 65536 rows and 32 nodes 70 to 78, 517 rows and 8 nodes 14.1. 65536 rows and 64 nodes of 64 heads over
+// 8, four tiles a KV head that read every row twice, 202 to 210 us: 137 GFLOP, of which half count twice, at 1.0 PFLOP/s, bound by two tiles' exponentials
+// and their instructions taking turns with the tensor core; there is one buffer of scores a tile.
+//
+// Registers: the 14 warps of a block with two tiles are four on two of the SM's sub-partitions, so 128 a thread, and 64 to 72 bytes are spilled with rows of
+// 128 elements (none with 64); ten warps with one tile have 168 and spill 36 bytes in bf16, for what a row that is computed once more needs.
 //
 // Hidden nodes have probability 0, and 0 times infinity or NaN is NaN on the tensor core. So a node with such a value is cleared in shared
 // memory (one more warp, the cleaner, looks at the nodes' values where they have landed), and rows that see it add their probability times its values
