@@ -546,12 +546,12 @@ int pjrtx_b200_paged_cache_attend(PjrtxB200PagedCache *cache, const PjrtxB200Pag
 /* Attention of a tree of drafted tokens per sequence, and of a further piece of a prompt (a tree that is a chain). Node i of
  * sequence b sees the lengths[b] cached rows, its ancestors and itself: out = softmax(scale * q . k) v over these, lse its
  * log-sum-exp. parents[b, i] is a node before i, or -1 for a root, of which there may be several; any other parent counts as
- * -1 and is reported (43); from counts[b] on they are not read. Nothing is stored, lengths count cached rows only, and weights are not tracked. Results of nodes from counts[b]
- * on are left as they were. Keys and values that a node does not see enter nothing, whatever they hold; infinities and NaN in those
- * that it sees go on as in the formula, with probabilities below 2^-126 of the largest as zero; a cached row whose page the pool does not have (40) counts
- * as zeros. In 16 bits, a probability
- * meets finite values as two numbers of the element type, off by 2^-16 of it (bf16) or 2^-22 (f16, and to multiples of 2^-35 of the largest); sums and
- * lse are f32. */
+ * -1 and is reported (43); from counts[b] on they are not read. Nothing is stored, lengths count cached rows only, and weights are
+ * not tracked. Results of nodes from counts[b] on are left as they were. Keys and values that a node does not see enter nothing,
+ * whatever they hold; infinities and NaN in those that it sees go on as in the formula. Probabilities below 2^-126 of the largest may
+ * count as zero, and an infinite value with such a one gives an infinity or NaN. A cached row whose page the pool does not have (40)
+ * counts as zeros. In 16 bits, a probability meets finite values as two numbers of the element type, off by 2^-16 of it (bf16) or
+ * 2^-22 (f16, and to multiples of 2^-35 of the largest); sums and lse are f32. */
 typedef struct PjrtxB200PagedTreeArgs {
   uint64_t struct_size;
   const void *q; /* [batch, nodes, heads, head_dim] through the strides */

@@ -25,13 +25,11 @@
 // Two tiles in a block of threads of twice the size, with blocks of 128 keys that they share and buffers for one block of scores each, were slower up to
 // 4096 tokens (with one number a probability, as are the present form's figures in brackets): 517 of 32 heads over 8 14.4 us (10.8), 64 x 20 28 (16), 4 x 2048 162 (149), 2 x 4096 258 (254); 2 x 8192 916 (947).
 //
-// Hidden keys have probability 0, but the tensor core multiplies it by their values, and 0 times infinity or NaN is NaN; so it does where a
-// probability is lost in 16 bits. So values behind the last position of the block of threads are cleared in shared memory, and a warp with results that
-// are not finite looks at the values once: rows from which one that is not finite is hidden, and rows that see an infinite one, are computed
-// once more, by the warp, without the hidden ones and with probabilities in f32.
+// Hidden keys have probability 0, but the tensor core multiplies it by their values, and 0 times infinity or NaN is NaN. So values
+// behind the last position of the block of threads are cleared in shared memory, and a warp with a result that is not finite looks at that result's columns:
+// which infinities and NaN a row sees says what its results are there, and a row with a result that only a hidden value has spoilt is computed once more, by
+// the warp, without these and with probabilities in f32.
 #pragma once
-
-#include <climits>
 
 #include "umma_rows.cuh"
 
@@ -97,6 +95,26 @@ __device__ __noinline__ void redo_row(const PromptKernelArgs& a, const unsigned 
 #pragma unroll
   for (int e = 0; e < HD / 32; e++)
     if (e * 32 + lane < p.head_dim) reinterpret_cast<T*>(out)[e * 32 + lane] = rows::from_float<T>(o[e] * inverse);
+}
+
+// Of the keys up to `pos`, for all lanes of a warp, whose positions are first_pos .. last_pos (some lanes may have none).
+template <bool BF16>
+__device__ __noinline__ OddColumns prompt_odd_columns(const PromptAttention& p, const unsigned short* k, const unsigned short* v, int c, int first_pos, int last_pos,
+                                                      int pos) {
+  const int lane = threadIdx.x % 32;
+  OddColumns all = {0, 0, 0};
+  for (int key = lane; key <= first_pos; key += 32) all.add(odd_columns<BF16>(k + key * p.k_stride, v + key * p.v_stride, c, p.head_dim));
+  all.join_lanes();
+  for (int key0 = first_pos + 1; key0 <= last_pos; key0 += 32) {
+    OddColumns mine = {0, 0, 0};
+    if (key0 + lane <= last_pos) mine = odd_columns<BF16>(k + (key0 + lane) * p.k_stride, v + (key0 + lane) * p.v_stride, c, p.head_dim);
+    __syncwarp();
+    for (int i = 0; i < 32; i++) {
+      const OddColumns of_key = {__shfl_sync(0xffffffffu, mine.nan, i), __shfl_sync(0xffffffffu, mine.plus, i), __shfl_sync(0xffffffffu, mine.minus, i)};
+      if (key0 + i <= pos) all.add(of_key);
+    }
+  }
+  return all;
 }
 
 template <bool BF16, int HD>
@@ -349,50 +367,45 @@ umma_prompt_kernel(const __grid_constant__ PromptKernelArgs a, const __grid_cons
       const float inverse = rows::inverse_of(sum);
       const int h = g * a.p.rep + h0 + head;
       unsigned short* out = static_cast<unsigned short*>(p.out) + (long long)(item.start + pos) * p.out_stride + h * p.out_head_stride;
-      bool odd = false;
-#pragma unroll
+      const unsigned short* k = static_cast<const unsigned short*>(p.k) + (long long)item.start * p.k_stride + (long long)g * p.k_head_stride;
+      const unsigned short* v = static_cast<const unsigned short*>(p.v) + (long long)item.start * p.v_stride + (long long)g * p.v_head_stride;
+      bool spoilt = false;  // by a hidden value
+#pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
         float o[32];
         tmem_load_32(o_addr + c, o);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        Pair nan = 0;
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) nan = pair_fma(pair_of(o[e], o[e + 1]), 0, nan);
+        const float2 sums = pair_split(nan);
+        // Not where the sum is NaN, as every result then is.
+        if (__any_sync(0xffffffffu, sums.x + sums.y != 0.f && pos >= 0 && sum == sum)) {
+          OddColumns seen = prompt_odd_columns<BF16>(p, k, v, c, first_pos, __reduce_max_sync(0xffffffffu, pos), pos);
+          if (sum == 0.f) seen = {seen.any(), 0, 0};
+#pragma unroll
+          for (int e = 0; e < 32; e++) {
+            if (seen.any() >> e & 1) o[e] = seen.of(e);
+            else spoilt = spoilt || rows::odd(o[e]);
+          }
+        }
         if (pos >= 0) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-              odd = odd || rows::odd(o[e + 2 * i]) || rows::odd(o[e + 2 * i + 1]);
-              w[i] = pack_pair<BF16>(o[e + 2 * i] * inverse, o[e + 2 * i + 1] * inverse);
-            }
-            if (c + e < p.head_dim) *reinterpret_cast<uint4*>(out + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
+          for (int e = 0; e < 32; e += 8)
+            if (c + e < p.head_dim)
+              *reinterpret_cast<uint4*>(out + c + e) =
+                  make_uint4(pack_pair<BF16>(o[e] * inverse, o[e + 1] * inverse), pack_pair<BF16>(o[e + 2] * inverse, o[e + 3] * inverse),
+                             pack_pair<BF16>(o[e + 4] * inverse, o[e + 5] * inverse), pack_pair<BF16>(o[e + 6] * inverse, o[e + 7] * inverse));
         }
       }
       if (p.lse && pos >= 0)
         p.lse[(long long)(item.start + pos) * p.heads + h] =
             sum == 0.f ? -INFINITY : fmaf(m_used - Probability<BF16>::kLift, rows::kLn2, logf(sum));
-      // Rows that a value may have spoilt (not where the sum is NaN, as every result then is). All lanes write them once more: behind what each has
-      // stored of its own.
+      // All lanes write a row once more: behind what each has stored of its own.
       __syncwarp();
-      unsigned left = __ballot_sync(0xffffffffu, odd && pos >= 0 && sum == sum);
-      const unsigned short* k = static_cast<const unsigned short*>(p.k) + (long long)item.start * p.k_stride + (long long)g * p.k_head_stride;
-      const unsigned short* v = static_cast<const unsigned short*>(p.v) + (long long)item.start * p.v_stride + (long long)g * p.v_head_stride;
-      int last_odd = -1, first_infinite = INT_MAX;
-      if (left) {
-        constexpr int kPieces = HD / 8;
-        const int piece = lane % kPieces * 8;
-        for (int key = lane / kPieces; key < keys && piece < p.head_dim; key += 32 / kPieces) {
-          const uint4 x = *reinterpret_cast<const uint4*>(v + key * p.v_stride + piece);
-          if (!(odd_pair<BF16>(x.x) || odd_pair<BF16>(x.y) || odd_pair<BF16>(x.z) || odd_pair<BF16>(x.w))) continue;
-          last_odd = key;
-          if (infinite_pair<BF16>(x.x) || infinite_pair<BF16>(x.y) || infinite_pair<BF16>(x.z) || infinite_pair<BF16>(x.w)) first_infinite = min(first_infinite, key);
-        }
-        last_odd = __reduce_max_sync(0xffffffffu, last_odd);
-        first_infinite = __reduce_min_sync(0xffffffffu, first_infinite);
-      }
+      unsigned left = __ballot_sync(0xffffffffu, spoilt && pos >= 0);
       for (; left; left &= left - 1) {
         const int r = __ffs(left) - 1, row_pos = __shfl_sync(0xffffffffu, pos, r), row_h = __shfl_sync(0xffffffffu, h, r);
-        if (last_odd <= row_pos && first_infinite > row_pos) continue;
         const long long token = item.start + row_pos;
         redo_row<BF16, HD>(a, static_cast<const unsigned short*>(p.q) + token * p.q_stride + row_h * p.q_head_stride, k, v,
                            static_cast<unsigned short*>(p.out) + token * p.out_stride + row_h * p.out_head_stride, row_pos,

@@ -113,11 +113,59 @@ __device__ __forceinline__ bool odd_pair(uint32_t w) {
   return (w & kExponent) == kExponent || (w >> 16 & kExponent) == kExponent;
 }
 
-// Whether one of them is infinite.
+// Of 32 columns of values that a row sees, those with a NaN, an infinity, a negative one. What the row's results there are follows from these alone, as long as
+// its scores are finite: a probability above 0 times infinity is infinite, however small it is, and the tensor core makes NaN of it where one of the
+// probability's two numbers is 0.
+struct OddColumns {
+  unsigned nan, plus, minus;
+  __device__ __forceinline__ void add(const OddColumns& o) {
+    nan |= o.nan;
+    plus |= o.plus;
+    minus |= o.minus;
+  }
+  __device__ __forceinline__ void join_lanes() {
+    nan = __reduce_or_sync(0xffffffffu, nan);
+    plus = __reduce_or_sync(0xffffffffu, plus);
+    minus = __reduce_or_sync(0xffffffffu, minus);
+  }
+  __device__ __forceinline__ unsigned any() const { return nan | plus | minus; }
+  // Result of column e, one of any().
+  __device__ __forceinline__ float of(int e) const {
+    return nan >> e & 1 || (plus & minus) >> e & 1 ? __int_as_float(0x7fffffff) : plus >> e & 1 ? INFINITY : -INFINITY;
+  }
+};
+
+// Whether one of a row's elements is infinite or NaN.
 template <bool BF16>
-__device__ __forceinline__ bool infinite_pair(uint32_t w) {
-  constexpr uint32_t kInfinity = BF16 ? 0x7f80u : 0x7c00u;
-  return (w & 0x7fffu) == kInfinity || (w >> 16 & 0x7fffu) == kInfinity;
+__device__ __forceinline__ bool odd_row(const unsigned short* x, int head_dim) {
+  bool found = false;
+#pragma unroll 1
+  for (int d = 0; d < head_dim; d += 8) {
+    const uint4 w = *reinterpret_cast<const uint4*>(x + d);
+    found = found || odd_pair<BF16>(w.x) || odd_pair<BF16>(w.y) || odd_pair<BF16>(w.z) || odd_pair<BF16>(w.w);
+  }
+  return found;
+}
+
+// Those of columns c .. c + 31 of a key's values. A row that sees a key with an infinite element and has a finite sum has a score of -inf there: a
+// probability of 0, which makes NaN of an infinity.
+template <bool BF16>
+__device__ __forceinline__ OddColumns odd_columns(const unsigned short* k, const unsigned short* v, int c, int head_dim) {
+  OddColumns o = {0, 0, 0};
+#pragma unroll 1
+  for (int d = 0; d < 32 && c + d < head_dim; d += 8) {
+    const uint4 x = *reinterpret_cast<const uint4*>(v + c + d);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const uint32_t y = w[e / 2] >> (e % 2 * 16) & 0xffffu, infinity = BF16 ? 0x7f80u : 0x7c00u, bit = 1u << (d + e);
+      if ((y & 0x7fffu) > infinity) o.nan |= bit;
+      if (y == infinity) o.plus |= bit;
+      if (y == (infinity | 0x8000u)) o.minus |= bit;
+    }
+  }
+  if ((o.plus | o.minus) && odd_row<BF16>(k, head_dim)) o = {o.any(), 0, 0};
+  return o;
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,

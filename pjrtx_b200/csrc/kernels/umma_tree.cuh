@@ -18,14 +18,14 @@
 // 8, four tiles a KV head that read every row twice, 202 to 210 us: 137 GFLOP, of which half count twice, at 1.0 PFLOP/s, bound by two tiles' exponentials
 // and their instructions taking turns with the tensor core; there is one buffer of scores a tile.
 //
-// Registers: the 14 warps of a block with two tiles are four on two of the SM's sub-partitions, so 128 a thread, and 64 to 72 bytes are spilled with rows of
-// 128 elements (none with 64); ten warps with one tile have 168 and spill 36 bytes in bf16, for what a row that is computed once more needs.
+// Registers: the 14 warps of a block with two tiles are four on two of the SM's sub-partitions, so 128 a thread, and 64 bytes are spilled with rows of
+// 128 elements (none with 64); ten warps with one tile take 162 to 168 and spill none.
 //
 // Hidden nodes have probability 0, and 0 times infinity or NaN is NaN on the tensor core. So a node with such a value is cleared in shared
 // memory (one more warp, the cleaner, looks at the nodes' values where they have landed), and rows that see it add their probability times its values
-// when they take their results out. The same product spoils an infinite value of a cached row whose probability is lost in 16 bits: a warp with results
-// that are not finite looks at the cached values, and where one is infinite it computes its rows once more with probabilities in f32, some 30
-// instructions a key and row while the other warps wait for theirs. Rounding and the lazily followed maximum: umma_rows.cuh.
+// when they take their results out. The same product makes NaN of an infinite cached value where one of its probability's numbers is 0: a warp with a result
+// that is not finite looks at that result's columns of the cached rows, and which infinities and NaN these have says what it is. Rounding and the lazily
+// followed maximum: umma_rows.cuh.
 #pragma once
 
 #include "umma_rows.cuh"
@@ -98,63 +98,19 @@ __device__ __noinline__ float node_probability(const TreeKernelArgs& a, const un
   return exp2_approx(fmaf(s * a.sign, a.scale_log2, shift));
 }
 
-// Whether rows [first, end) of sequence b have an infinite value; called by a whole warp.
-template <bool BF16, int HD>
-__device__ __noinline__ bool infinite_values(const TreeKernelArgs& a, int b, int g, int first, int end) {
-  constexpr int kPieces = HD / 8;
-  const int lane = threadIdx.x % 32, piece = lane % kPieces * 8;
-  bool found = false;
-  for (int t = first + lane / kPieces; t < end && piece < a.p.c.head_dim; t += 32 / kPieces) {
-    const long long row = cached_row(a.p, b, t);
+// Of cached rows [first, end) of a sequence, for a whole warp.
+template <bool BF16>
+__device__ __noinline__ OddColumns cached_odd_columns(const TreeArgs& p, int b, int g, int c, int first, int end) {
+  OddColumns all = {0, 0, 0};
+  for (int t = first + threadIdx.x % 32; t < end; t += 32) {
+    const long long row = cached_row(p, b, t);
     if (row < 0) continue;
-    const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(a.p.c.v) + row + g * a.p.c.head_stride + piece);
-    found = found || infinite_pair<BF16>(x.x) || infinite_pair<BF16>(x.y) || infinite_pair<BF16>(x.z) || infinite_pair<BF16>(x.w);
+    const long long at = row + g * p.c.head_stride;
+    all.add(odd_columns<BF16>(static_cast<const unsigned short*>(p.c.k) + at, static_cast<const unsigned short*>(p.c.v) + at, c, p.c.head_dim));
   }
-  return __any_sync(0xffffffffu, found);
-}
-
-// A query row once more over keys [first, end) as far as it sees them; called by a whole warp. To `part`, or `out` times `inverse`.
-template <bool BF16, int HD>
-__device__ __noinline__ void redo_tree_row(const TreeKernelArgs& a, const Segment& seg, int node, int head, unsigned long long bits, int length, int first, int end,
-                                           float shift, float inverse, float* part, unsigned short* out) {
-  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-  const TreeArgs& p = a.p;
-  const int lane = threadIdx.x % 32;
-  const unsigned short* q = static_cast<const unsigned short*>(p.a.q) + query_at(p, seg, node, head);
-  float o[HD / 32];
-#pragma unroll
-  for (int e = 0; e < HD / 32; e++) o[e] = 0.f;
-  for (int key0 = first; key0 < end; key0 += 32) {
-    const int key = key0 + lane, fresh = key - length;
-    const unsigned short *k = nullptr, *v = nullptr;
-    if (key < end && fresh < 0) {
-      const long long row = cached_row(p, seg.b, key);
-      if (row >= 0) {
-        k = static_cast<const unsigned short*>(p.c.k) + row + seg.g * p.c.head_stride;
-        v = static_cast<const unsigned short*>(p.c.v) + row + seg.g * p.c.head_stride;
-      }
-    } else if (key < end && bits >> fresh & 1) {
-      const long long row = seg.b * p.a.new_batch_stride + fresh * p.a.new_node_stride + seg.g * p.a.new_head_stride;
-      k = static_cast<const unsigned short*>(p.a.k_new) + row;
-      v = static_cast<const unsigned short*>(p.a.v_new) + row;
-    }
-    const float mine = k ? node_probability<BF16>(a, q, k, shift) : 0.f;
-    __syncwarp();
-    for (int i = 0; i < 32; i++) {
-      const unsigned long long at = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(v), i);
-      const float w = __shfl_sync(0xffffffffu, mine, i);
-      if (!at) continue;
-#pragma unroll
-      for (int e = 0; e < HD / 32; e++)
-        if (e * 32 + lane < p.c.head_dim) o[e] = fmaf(w, (float)reinterpret_cast<const T*>(at)[e * 32 + lane], o[e]);
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < HD / 32; e++) {
-    const int d = e * 32 + lane;
-    if (part) part[(long long)d * p.slot_rows] = o[e];
-    else if (d < p.c.head_dim) reinterpret_cast<T*>(out)[d] = rows::from_float<T>(o[e] * inverse);
-  }
+  __syncwarp();
+  all.join_lanes();
+  return all;
 }
 
 template <bool BF16, int HD, int TILES>
@@ -687,15 +643,24 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
       const float inverse = part ? 1.f : rows::inverse_of(sum);
       const long long fresh = seg.b * p.a.new_batch_stride + seg.g * p.a.new_head_stride;
       unsigned short* out = static_cast<unsigned short*>(p.a.out) + (there ? out_at(p, seg, node, head) : 0);
-      Pair spoilt = 0;  // NaN with a result that is not finite
 #pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
         float o[32];
         tmem_load_32(o_addr + c, o);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        if (!there) continue;
+        Pair nan = 0;
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) spoilt = pair_fma(pair_of(o[e], o[e + 1]), 0, spoilt);
+        for (int e = 0; e < 32; e += 2) nan = pair_fma(pair_of(o[e], o[e + 1]), 0, nan);
+        const float2 sums = pair_split(nan);
+        // Not where the sum is NaN, as every result then is.
+        if (__any_sync(0xffffffffu, there && sums.x + sums.y != 0.f && sum == sum)) {
+          OddColumns seen = cached_odd_columns<BF16>(p, seg.b, seg.g, c, here.tile * kKeys, min(tile_end * kKeys, here.s.length));
+          if (sum == 0.f) seen = {seen.any(), 0, 0};
+#pragma unroll
+          for (int e = 0; e < 32; e++)
+            if (seen.any() >> e & 1) o[e] = seen.of(e);
+        }
+        if (!there) continue;
         for (unsigned long long left = odd; left; left &= left - 1) {
           using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
           const long long at = fresh + (__ffsll(left) - 1) * p.a.new_node_stride;
@@ -717,21 +682,9 @@ __global__ void __launch_bounds__(tree_threads(TILES), 1) umma_tree_kernel(const
                              pack_pair<BF16>(o[e + 4] * inverse, o[e + 5] * inverse), pack_pair<BF16>(o[e + 6] * inverse, o[e + 7] * inverse));
         }
       }
-      if (there && part) store_statistics(p, part, row, m, sum);
-      else if (there && p.a.lse) p.a.lse[lse_at(p, seg, node, head)] = sum == 0.f ? -INFINITY : fmaf(m, rows::kLn2, logf(sum));
-      // Not where the sum is NaN, as every result then is. All lanes write the rows: behind what each has stored of its own.
-      const float2 nan = pair_split(spoilt);
-      __syncwarp();
-      unsigned again = __ballot_sync(0xffffffffu, there && nan.x + nan.y != 0.f && sum == sum);
-      const int first = here.tile * kKeys, last = tile_end * kKeys;
-      if (again && !infinite_values<BF16, HD>(a, seg.b, seg.g, first, min(last, here.s.length))) again = 0;
-      for (; again; again &= again - 1) {
-        const int r = __ffs(again) - 1;
-        redo_tree_row<BF16, HD>(a, seg, __shfl_sync(0xffffffffu, node, r), __shfl_sync(0xffffffffu, head, r), __shfl_sync(0xffffffffu, bits, r), here.s.length,
-                                first, min(last, here.s.length + here.s.count), __shfl_sync(0xffffffffu, shift, r), __shfl_sync(0xffffffffu, inverse, r),
-                                part ? part + row - lane + r : nullptr,
-                                reinterpret_cast<unsigned short*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(out), r)));
-      }
+      if (!there) continue;
+      if (part) store_statistics(p, part, row, m, sum);
+      else if (p.a.lse) p.a.lse[lse_at(p, seg, node, head)] = sum == 0.f ? -INFINITY : fmaf(m, rows::kLn2, logf(sum));
     }
     if (!ok && lane == 0) report(p.c.error_words, kErrorWait);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
