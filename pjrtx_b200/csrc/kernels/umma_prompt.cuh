@@ -14,16 +14,18 @@
 // the tensor core 61 % busy, the exponential unit 41 %, issue slots 43 %. What fills the rest is not one unit but the order of things: a block's scores,
 // maximum, exponentials and product follow each other, and two independent blocks of threads do not hide all of it from each other. Eight softmax
 // warps a tile, four for every other block, which hand the rows' maxima to each other, gained nothing (with one number a probability, 4 x 2048 146 -> 155
-// us). 8192 and 5461 tokens, 32 heads of 128 over 8 KV heads, masked halves left out: 943 to 1000 us in f16 and 856 to 876 in bf16, 0.8 to 0.9
+// us). 8192 and 5461 tokens, 32 heads of 128 over 8 KV heads, masked halves left out: 933 to 1000 us in f16 and 856 to 876 in bf16, 0.8 to 0.9
 // PFLOP/s that count, once more by half with the second product, in bursts; 1110 from call to call, where the clock settles lower. 4 x 2048 181 to 185 us,
 // with 8 heads of 64 47; one prompt of 517 tokens 11.6 us, where launch, first copies, nine blocks of keys one after the other and the way out follow
 // each other.
 //
 // Exponentials all go to the exponential unit: a share of them by polynomials on the FMA units, as the tensor core's rate would want, made
-// every case 2 to 15 % slower by the code and the issue slots that it takes. Scores that are read twice in loops, as in umma_tree.cuh, are 2 to 4 % slower here.
+// every case 2 to 15 % slower by the code and the issue slots that it takes. Scores that are read twice in loops, as in umma_tree.cuh, make it 2 to 4 %
+// slower here.
 //
 // Two tiles in a block of threads of twice the size, with blocks of 128 keys that they share and buffers for one block of scores each, were slower up to
-// 4096 tokens (with one number a probability, as are the present form's figures in brackets): 517 of 32 heads over 8 14.4 us (10.8), 64 x 20 28 (16), 4 x 2048 162 (149), 2 x 4096 258 (254); 2 x 8192 916 (947).
+// 4096 tokens (with one number a probability, as are the present form's figures in brackets): 517 of 32 heads over 8 14.4 us (10.8), 64 x 20 28 (16),
+// 4 x 2048 162 (149), 2 x 4096 258 (254); 2 x 8192 916 (947).
 //
 // Hidden keys have probability 0, but the tensor core multiplies it by their values, and 0 times infinity or NaN is NaN. So values
 // behind the last position of the block of threads are cleared in shared memory, and a warp with a result that is not finite looks at that result's columns:

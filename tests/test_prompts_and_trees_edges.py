@@ -11,7 +11,7 @@ import pytest
 from pjrtx_b200 import backend as be_mod
 from pjrtx_b200 import plan as P
 from tests import test_prompts_and_trees as base
-from tests.test_operators import _stream, _within
+from tests.test_operators import _stream, _torch_type, _within
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -249,6 +249,43 @@ def test_trees_on_pages_whose_axes_lie_in_any_order(gpu_backend, dtype, order, p
     t.check(some=200)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_the_most_tokens_and_sequences(gpu_backend, dtype):
+    """2^24 tokens of 2^20 sequences, one of which has most of them."""
+    import torch
+
+    tokens, count, long = 1 << 24, 1 << 20, 3000
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    q, k, v = (torch.randn((tokens, 1, 8), generator=gen, device="cuda").to(_torch_type(dtype)) for _ in "qkv")
+    lengths = torch.full((count,), 15, dtype=torch.int64)
+    lengths[count // 3] = long
+    starts = torch.cat([torch.zeros(1, dtype=torch.int64), lengths.cumsum(0)])
+    out, lse = torch.full_like(q, 7), torch.full((tokens, 1), 7.0, device="cuda")
+    gpu_backend.prompt_attention(q, k, v, starts.int().cuda(), out, lse=lse, stream=_stream())
+    gpu_backend.operators_status(stream=_stream())
+    c, ends = base._Compared(), starts.tolist()
+    for b in [0, 1, 77, count // 3 - 1, count // 3, count // 3 + 1, count - 2, count - 1] + np.random.default_rng(1).integers(0, count, 60).tolist():
+        for i in (0, 7, int(lengths[b]) - 1):
+            r, a = ends[b] + i, ends[b]
+            c.add(dtype, out[r, 0], lse[r, 0], q[r, 0], k[a:r + 1, 0], v[a:r + 1, 0], 8 ** -0.5)
+    c.check("most tokens")
+    assert (out[ends[-1]:] == 7).all() and not (out[:ends[-1]] == 7).all(2).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("heads,kv_heads", [(65535, 65535), (65535, 1), (32768, 16384)])
+def test_the_most_heads(gpu_backend, dtype, heads, kv_heads):
+    p = base._Prompts(dtype, heads, kv_heads, 8, [2, 0, 3], seed=8)
+    p.run(gpu_backend)
+    p.check(some=400)
+    t = base._Trees(dtype, heads, kv_heads, 8, 4, [5, 0], 3, seed=8, counts=[3, 2])
+    t.run(gpu_backend)
+    t.check(some=400)
+    gpu_backend.operators_status(stream=_stream())
+
+
 _GIVE_UP = """
 import torch
 from pjrtx_b200 import backend as be_mod
@@ -415,3 +452,34 @@ def test_slots_by_the_cluster_and_by_a_kernel_of_their_own(gpu_backend, tokens):
     gpu_backend.operators_status(stream=_stream())
     want = np.concatenate([table[b, np.arange(n) // page] * page + np.arange(n) % page for b, n in enumerate(lengths) if new[b]])
     assert np.array_equal(slots.cpu().numpy(), want)
+
+
+@pytest.mark.gpu
+def test_the_largest_batch_of_page_tables_and_paths(gpu_backend):
+    """65535 sequences that grow by a page or give theirs back, and the slots of their paths."""
+    import torch
+
+    batch, page, max_pages = 65535, 2, 3
+    b = torch.arange(batch, device="cuda").int()
+    held, lengths = b % 4, (b * 7) % 7
+    table = torch.full((batch, max_pages), -1, dtype=torch.int32, device="cuda")
+    has = torch.arange(max_pages, device="cuda")[None] < held[:, None]
+    table[has] = torch.arange(int(has.sum()), device="cuda").int()
+    need = (lengths + page - 1) // page
+    used, wanted = int(has.sum()), int((need - held).clamp(min=0).sum())
+    pool = used + wanted
+    stack = torch.full((pool,), -1, dtype=torch.int32, device="cuda")
+    stack[:wanted] = torch.arange(used, pool, device="cuda").int()
+    count = torch.tensor([wanted], dtype=torch.int32, device="cuda")
+    cache = gpu_backend.paged_cache(P.BF16_CODE, batch, 2, 1, 8, page, max_pages)
+    want = base._assigned(lengths.tolist(), held.tolist(), table.tolist(), stack[:wanted].tolist(), page, max_pages)
+    cache.assign_pages(lengths, held, table, stack, count, stream=_stream())
+    gpu_backend.operators_status(stream=_stream())
+    assert held.tolist() == want[0] and table.tolist() == want[1] and stack[:int(count)].tolist() == want[2]
+    n = (lengths - 1).clamp(min=0)
+    parents, leaves, slots = torch.full((batch, 1), -1, dtype=torch.int32, device="cuda"), torch.where(lengths > 0, 0, -1).int(), torch.zeros((batch, 1), dtype=torch.int32, device="cuda")
+    cache.path_slots(table, n, parents, leaves, slots, stream=_stream())
+    gpu_backend.operators_status(stream=_stream())
+    row = (lengths - 1).clamp(min=0).long()
+    at = table.gather(1, (row // page)[:, None])[:, 0] * page + row % page
+    assert torch.equal(slots[:, 0], torch.where(lengths > 0, at.int(), -1).int()) and torch.equal(n, lengths)
