@@ -15,7 +15,7 @@
 // maximum, exponentials and product follow each other, and two independent blocks of threads do not hide all of it from each other. Eight softmax
 // warps a tile, four for every other block, which hand the rows' maxima to each other, gained nothing (with one number a probability, 4 x 2048 146 -> 155
 // us). 8192 and 5461 tokens, 32 heads of 128 over 8 KV heads, masked halves left out: 933 to 1000 us in f16 and 856 to 876 in bf16, 0.8 to 0.9
-// PFLOP/s that count, once more by half with the second product, in bursts; 1110 from call to call, where the clock settles lower. 4 x 2048 181 to 185 us,
+// PFLOP/s that count, once more by half with the second product, in bursts; 1084 to 1130 from call to call, where the clock settles lower. 4 x 2048 181 to 185 us,
 // with 8 heads of 64 47; one prompt of 517 tokens 11.6 us, where launch, first copies, nine blocks of keys one after the other and the way out follow
 // each other.
 //

@@ -15,7 +15,7 @@
 // (7 TB/s over all SMs), and take 1024 cycles of exponentials and, with two numbers a probability, 1536 of the tensor core for each tile. Around that stand
 // 6 to 7 us of launch, shares, page ids and first rows, and 5 to 10 of the join: 16 sequences of up to 4096 rows, 16 nodes of 32 heads over 8, pages of 16
 // rows 56 to 59 us (184 MB, 3.2 TB/s), one sequence of 65536 rows and 32 nodes 70 to 78, 517 rows and 8 nodes 14.1. 65536 rows and 64 nodes of 64 heads over
-// 8, four tiles a KV head that read every row twice, 202 to 210 us: 137 GFLOP, of which half count twice, at 1.0 PFLOP/s, bound by two tiles' exponentials
+// 8, four tiles a KV head that read every row twice, 196 to 210 us: 137 GFLOP, of which half count twice, at 1.0 PFLOP/s, bound by two tiles' exponentials
 // and their instructions taking turns with the tensor core; there is one buffer of scores a tile.
 //
 // Registers: the 14 warps of a block with two tiles are four on two of the SM's sub-partitions, so 128 a thread, and 64 bytes are spilled with rows of
